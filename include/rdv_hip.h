@@ -58,7 +58,8 @@ enum {
   RDV_ACT_RELU = 1,
   RDV_ACT_SOFTPLUS = 2,   /* log(1 + exp(x))                                   */
   RDV_ACT_SIGMOID = 3,    /* 1 / (1 + exp(-x))                                 */
-  RDV_ACT_DENSITY_RGB = 4 /* channel 0 softplus, channels 1.. sigmoid          */
+  RDV_ACT_DENSITY_RGB = 4, /* channel 0 softplus, channels 1.. sigmoid         */
+  RDV_ACT_SILU = 5        /* x / (1 + exp(-x)); rdv_group_norm only            */
 };
 
 /* Arithmetic of a layer.
@@ -153,7 +154,8 @@ const char* rdv_mlp_kernel_name(const rdv_mlp_desc* desc);
 /* Image layouts (one image = batch element): HWC is the reference's
  * channels-last [H*W, C] (src/rdv/domain/nn.py:1018-1024); CHW is NCHW. */
 enum { RDV_LAYOUT_HWC = 0, RDV_LAYOUT_CHW = 1 };
-enum { RDV_DTYPE_F32 = 0, RDV_DTYPE_F16 = 1 };
+/* BF16: the image-network operators below only. */
+enum { RDV_DTYPE_F32 = 0, RDV_DTYPE_F16 = 1, RDV_DTYPE_BF16 = 2 };
 /* Filter layouts: RSCK is the reference's [3][3][CIN][COUT]; KCRS is PyTorch OIHW. */
 enum { RDV_WLAYOUT_RSCK = 0, RDV_WLAYOUT_KCRS = 1 };
 
@@ -541,6 +543,93 @@ int rdv_volume_profile_finish(const rdv_volume_profile_desc* vp, const float* al
 /* out[rows, width] = value[width] repeated on every row: a Constant map over
  * rows (src/rdv/maths/__init__.py:1659-1668, shaders/maps/constant.h). */
 int rdv_broadcast_rows(const float* value, int32_t width, int64_t rows, float* out, void* stream);
+
+/* ------------------------------------------- image-network operators
+ * Build-defined (no counterpart in the reference): what a network over images
+ * needs beside its convolutions.  Tensors are fp32, fp16 or bf16 (RDV_DTYPE_*);
+ * sums, statistics and softmax terms are fp32 and results are rounded once.
+ * Strides are in elements.  Results are the same from call to call (no
+ * atomics).  Workspaces are 16-byte aligned device memory that one call uses
+ * alone until it has run; their contents need not be kept or cleared. */
+
+/* Group normalisation of channels-last images x[images, rows, channels]
+ * (rows = H W): the channels fall into `groups` equal runs, and with mean and
+ * var (biased) over an image's rows and a run's channels
+ *   y = act(weight[c] (x - mean) / sqrt(var + eps) + bias[c]). */
+typedef struct rdv_group_norm_desc {
+  int64_t images, rows;                    /* >= 0                                          */
+  int64_t x_image_stride, x_row_stride;    /* of x; a row's channels are contiguous         */
+  int64_t g_image_stride, g_row_stride;    /* of grad (backward only)                       */
+  int32_t channels, groups;                /* groups divides channels                       */
+  int32_t act;                             /* RDV_ACT_NONE, RDV_ACT_RELU or RDV_ACT_SILU    */
+  int32_t dtype;                           /* RDV_DTYPE_* of x, grad, y and dx              */
+  float eps;                               /* >= 0                                          */
+  int32_t reserved;                        /* 0                                             */
+} rdv_group_norm_desc;
+
+/* Bytes of workspace of the forward (backward = 0) or the backward call; < 0 on error. */
+int64_t rdv_group_norm_workspace_bytes(const rdv_group_norm_desc* desc, int32_t backward);
+
+/* y[images, rows, channels] (contiguous, not overlapping x) and, where stats is
+ * not NULL, stats[images, groups, 2] = (mean, 1 / sqrt(var + eps)).  weight and
+ * bias are fp32 [channels] or NULL (ones, zeros). */
+int rdv_group_norm(const rdv_group_norm_desc* desc, const void* x, const float* weight, const float* bias, void* y,
+                   float* stats, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* The gradients of rdv_group_norm for grad = dL/dy: dx (contiguous, desc's
+ * dtype) and, where not NULL, fp32 dweight[channels] and dbias[channels].
+ * stats is what the forward call wrote for the same x. */
+int rdv_group_norm_backward(const rdv_group_norm_desc* desc, const void* grad, const void* x, const float* weight,
+                            const float* bias, const float* stats, void* dx, float* dweight, float* dbias,
+                            void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Attention from q[batch, queries, heads, dim] to the states of another
+ * sequence, k and v[batch, keys, kv_heads, dim]; head h reads state head
+ * h / (heads / kv_heads).  A state j of item b counts if j < key_lengths[b]
+ * (int32 [batch], clamped to [0, keys]) and key_mask[b, j] != 0 (bytes), where
+ * given.  Over the states that count
+ *   out[b, i, h] = sum_j softmax_j(scale q . k_j) v_j,
+ *   lse[b, h, i] = ln sum_j exp(scale q . k_j),
+ * and a query with no state gets out = 0, lse = -inf.  What k and v hold at
+ * states that do not count has no effect on any result. */
+#define RDV_ATTENTION_MAX_DIM 128
+typedef struct rdv_attention_desc {
+  int32_t batch, queries, keys;            /* >= 0                                          */
+  int32_t heads, kv_heads;                 /* kv_heads divides heads                        */
+  int32_t dim;                             /* 1..RDV_ATTENTION_MAX_DIM                      */
+  int32_t dtype;                           /* RDV_DTYPE_* of every tensor but lse           */
+  float scale;
+  int64_t q_stride[3], k_stride[3], v_stride[3];  /* batch, row, head; dim is contiguous    */
+  int64_t g_stride[3];                     /* of grad (backward only)                       */
+  int64_t mask_stride;                     /* of key_mask, batch to batch                   */
+} rdv_attention_desc;
+
+/* Bytes of workspace of the forward (backward = 0) or the backward call; < 0 on error. */
+int64_t rdv_cross_attention_workspace_bytes(const rdv_attention_desc* desc, int32_t backward);
+
+/* out[batch, queries, heads, dim] (contiguous) and, where lse is not NULL, lse[batch, heads, queries] fp32. */
+int rdv_cross_attention(const rdv_attention_desc* desc, const void* q, const void* k, const void* v,
+                        const int32_t* key_lengths, const uint8_t* key_mask, void* out, float* lse, void* workspace,
+                        int64_t workspace_bytes, void* stream);
+
+/* The gradients of rdv_cross_attention for grad = dL/dout, given the out and
+ * lse that it wrote: dq[batch, queries, heads, dim], dk and dv[batch, keys,
+ * kv_heads, dim], contiguous; the gradients of a state head are summed over the
+ * heads that read it, and are 0 at states that do not count. */
+int rdv_cross_attention_backward(const rdv_attention_desc* desc, const void* grad, const void* q, const void* k,
+                                 const void* v, const void* out, const float* lse, const int32_t* key_lengths,
+                                 const uint8_t* key_mask, void* dq, void* dk, void* dv, void* workspace,
+                                 int64_t workspace_bytes, void* stream);
+
+/* y[i] = residual[i] + (word_i >= floor(p 2^32) ? x[i] / (1 - p) : 0) for i < n,
+ * with residual NULL for zeros and 0 <= p <= 1.  word_i is word i % 4 of
+ * Philox4x32-10 (Salmon, Moraes, Dror, Shaw: "Parallel random numbers: as easy
+ * as 1, 2, 3", 2011) at counter (i / 4, subsequence), 64 bits each, low word
+ * first, and key `seed`.  The mask is a function of (seed, subsequence, i)
+ * alone and is never stored: the gradient of x is the same call on dL/dy with
+ * no residual.  y may be x or residual itself. */
+int rdv_dropout(const void* x, const void* residual, void* y, int64_t n, int32_t dtype, double p, uint64_t seed,
+                uint64_t subsequence, void* stream);
 
 #ifdef __cplusplus
 }

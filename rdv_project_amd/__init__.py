@@ -82,6 +82,14 @@ from .types import (
     vec4,
 )
 from ._conv import Winograd3x3Conv2d, winograd3x3_conv2d
+from ._image_ops import (
+    cross_attention,
+    cross_attention_backward,
+    dropout,
+    dropout_backward,
+    group_norm,
+    group_norm_backward,
+)
 from ._render import composite
 from .grids import (
     Conv2D,
@@ -120,7 +128,10 @@ from .nn import (
     Conv2DTensorOpSimple3x3,
     Conv2DTensorOpWindow3x3,
     Conv2DTensorOpWinograd3x3,
+    CrossAttentionTensorOp,
     Downsample2xTensorOp,
+    DropoutTensorOp,
+    GroupNormTensorOp,
     Upsample2xTensorOp,
     DensityRGB,
     LinearTensorOp,

@@ -24,10 +24,11 @@ MLP_MAX_WIDTH = 256
 TRAIN_STATIC_SCRATCH_BYTES = 64 << 20  # RDV_TRAIN_STATIC_SCRATCH_BYTES
 
 ACT_NONE, ACT_RELU, ACT_SOFTPLUS, ACT_SIGMOID, ACT_DENSITY_RGB = 0, 1, 2, 3, 4
+ACT_SILU = 5  # group normalisation only
 PREC_F32, PREC_F16 = 0, 1
 ENC_NONE, ENC_FREQ = 0, 1
 LAYOUT_HWC, LAYOUT_CHW = 0, 1
-DTYPE_F32, DTYPE_F16 = 0, 1
+DTYPE_F32, DTYPE_F16, DTYPE_BF16 = 0, 1, 2
 WLAYOUT_RSCK, WLAYOUT_KCRS = 0, 1
 WKIND_F32, WKIND_F16, WKIND_F16_TILED16 = 0, 1, 2
 
@@ -157,6 +158,46 @@ class MajorantGridDesc(C.Structure):
 GRID_MAX_RANK = 8
 
 
+class GroupNormDesc(C.Structure):
+    """Mirror of rdv_group_norm_desc."""
+    _fields_ = [
+        ("images", C.c_int64),
+        ("rows", C.c_int64),
+        ("x_image_stride", C.c_int64),
+        ("x_row_stride", C.c_int64),
+        ("g_image_stride", C.c_int64),
+        ("g_row_stride", C.c_int64),
+        ("channels", C.c_int32),
+        ("groups", C.c_int32),
+        ("act", C.c_int32),
+        ("dtype", C.c_int32),
+        ("eps", C.c_float),
+        ("reserved", C.c_int32),
+    ]
+
+
+ATTENTION_MAX_DIM = 128
+
+
+class AttentionDesc(C.Structure):
+    """Mirror of rdv_attention_desc."""
+    _fields_ = [
+        ("batch", C.c_int32),
+        ("queries", C.c_int32),
+        ("keys", C.c_int32),
+        ("heads", C.c_int32),
+        ("kv_heads", C.c_int32),
+        ("dim", C.c_int32),
+        ("dtype", C.c_int32),
+        ("scale", C.c_float),
+        ("q_stride", C.c_int64 * 3),
+        ("k_stride", C.c_int64 * 3),
+        ("v_stride", C.c_int64 * 3),
+        ("g_stride", C.c_int64 * 3),
+        ("mask_stride", C.c_int64),
+    ]
+
+
 class RDVError(RuntimeError):
     """A HIP runtime failure reported by the library."""
 
@@ -227,6 +268,14 @@ _SIGNATURES = {
                                                    C.c_void_p, C.c_void_p]),
     "rdv_winograd3x3_forward": (C.c_int, [C.POINTER(ConvDesc), C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
                                           C.c_void_p]),
+    "rdv_group_norm_workspace_bytes": (C.c_int64, [C.POINTER(GroupNormDesc), C.c_int32]),
+    "rdv_group_norm": (C.c_int, [C.POINTER(GroupNormDesc), *[C.c_void_p] * 6, C.c_int64, C.c_void_p]),
+    "rdv_group_norm_backward": (C.c_int, [C.POINTER(GroupNormDesc), *[C.c_void_p] * 9, C.c_int64, C.c_void_p]),
+    "rdv_cross_attention_workspace_bytes": (C.c_int64, [C.POINTER(AttentionDesc), C.c_int32]),
+    "rdv_cross_attention": (C.c_int, [C.POINTER(AttentionDesc), *[C.c_void_p] * 8, C.c_int64, C.c_void_p]),
+    "rdv_cross_attention_backward": (C.c_int, [C.POINTER(AttentionDesc), *[C.c_void_p] * 12, C.c_int64, C.c_void_p]),
+    "rdv_dropout": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_int32, C.c_double, C.c_uint64,
+                              C.c_uint64, C.c_void_p]),
 }
 
 _lib = None

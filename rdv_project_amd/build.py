@@ -35,6 +35,7 @@ SOURCES = [
     "mlp_generic.hip",
     "train_fused.hip",
     "train.hip",
+    "attention.hip",
     "winograd.hip",
     "conv_op.hip",
     "mlp_fused.hip",
@@ -42,7 +43,9 @@ SOURCES = [
     "capi.cpp",
     "mlp_pack.hip",
     "mlp_f32.hip",
+    "group_norm.hip",
     "tensor_data.hip",
+    "dropout.hip",
     "grid_batch.hip",
 ]
 

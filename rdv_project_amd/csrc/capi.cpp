@@ -42,6 +42,13 @@ int device_info(DeviceInfo* out) {
   return RDV_OK;
 }
 
+// CUs that a split of work is planned for: the current device's, or an MI355X's where there is none (sizes of
+// workspaces can be asked for on a host without a GPU).
+static int plan_cu_count() {
+  DeviceInfo info;
+  return device_info(&info) == RDV_OK && info.cu_count > 0 ? info.cu_count : 256;
+}
+
 // ---------------------------------------------------------- MLP launchers
 struct FusedEntry;
 const FusedEntry* find_fused(const rdv_mlp_desc& d, const MlpLayout& lay);
@@ -115,6 +122,22 @@ int launch_conv2d(const rdv_conv2d_desc& d, const float* x, const float* w, cons
 int launch_downsample2x(const float* x, int64_t H, int64_t W, int C, float* y, hipStream_t stream);
 int launch_upsample2x(const float* x, int64_t H, int64_t W, int C, float* y, hipStream_t stream);
 int launch_concat(const float* x1, int C1, const float* x2, int C2, int64_t rows, float* y, hipStream_t stream);
+
+int64_t group_norm_workspace_bytes(const rdv_group_norm_desc& d, bool backward, int cu);
+int launch_group_norm(const rdv_group_norm_desc& d, const void* x, const float* weight, const float* bias, void* y,
+                      float* stats, void* ws, hipStream_t stream);
+int launch_group_norm_backward(const rdv_group_norm_desc& d, const void* grad, const void* x, const float* weight,
+                               const float* bias, const float* stats, void* dx, float* dweight, float* dbias,
+                               void* ws, hipStream_t stream);
+int64_t attention_workspace_bytes(const rdv_attention_desc& d, bool backward, int cu);
+int launch_attention(const rdv_attention_desc& d, const void* q, const void* k, const void* v,
+                     const int32_t* key_lengths, const uint8_t* key_mask, void* out, float* lse, void* ws,
+                     hipStream_t stream);
+int launch_attention_backward(const rdv_attention_desc& d, const void* grad, const void* q, const void* k,
+                              const void* v, const void* out, const float* lse, const int32_t* key_lengths,
+                              const uint8_t* key_mask, void* dq, void* dk, void* dv, void* ws, hipStream_t stream);
+int launch_dropout(const void* x, const void* residual, void* y, int64_t n, int dtype, double p, uint64_t seed,
+                   uint64_t subsequence, hipStream_t stream);
 
 static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
@@ -725,6 +748,134 @@ int rdv_majorant_grid(const rdv_majorant_grid_desc* desc, const float* fine, flo
   }
   if (!fine || !out) return fail(RDV_ERR_INVALID, "rdv_majorant_grid: NULL pointer argument");
   return launch_majorant_grid(*desc, fine, out, static_cast<hipStream_t>(stream));
+}
+
+// ------------------------------------------------- image-network operators
+// Size limits of these: every extent below 2^31, every tensor below 2^40 elements.
+static bool stride_ok(int64_t s) { return s >= 0 && s < (int64_t(1) << 40); }
+
+static int check_group_norm(const rdv_group_norm_desc* d, bool backward) {
+  if (!d) return fail(RDV_ERR_INVALID, "group norm: NULL descriptor");
+  if (d->images < 0 || d->images >= (int64_t(1) << 31) || d->rows < 0 || d->rows >= (int64_t(1) << 31))
+    return fail(RDV_ERR_INVALID, "group norm: images and rows must be in [0, 2^31)");
+  if (d->channels < 1 || d->channels > (1 << 20)) return fail(RDV_ERR_INVALID, "group norm: channels must be in [1, 2^20]");
+  if (d->groups < 1 || d->channels % d->groups != 0)
+    return fail(RDV_ERR_INVALID, "group norm: groups must be >= 1 and divide channels");
+  if (d->images > 0 && d->rows > 0 && d->images * d->rows > (int64_t(1) << 40) / d->channels)
+    return fail(RDV_ERR_INVALID, "group norm: tensor too large");
+  if (d->act != RDV_ACT_NONE && d->act != RDV_ACT_RELU && d->act != RDV_ACT_SILU)
+    return fail(RDV_ERR_INVALID, "group norm: the activation must be none, relu or silu");
+  if (d->dtype < RDV_DTYPE_F32 || d->dtype > RDV_DTYPE_BF16) return fail(RDV_ERR_INVALID, "group norm: unknown dtype");
+  if (!(d->eps >= 0.0f)) return fail(RDV_ERR_INVALID, "group norm: eps must be >= 0");
+  if (d->reserved != 0) return fail(RDV_ERR_INVALID, "reserved must be 0");
+  if (!stride_ok(d->x_image_stride) || !stride_ok(d->x_row_stride) ||
+      (backward && (!stride_ok(d->g_image_stride) || !stride_ok(d->g_row_stride))))
+    return fail(RDV_ERR_INVALID, "group norm: strides must be in [0, 2^40)");
+  return RDV_OK;
+}
+
+int64_t rdv_group_norm_workspace_bytes(const rdv_group_norm_desc* desc, int32_t backward) {
+  const int rc = check_group_norm(desc, backward != 0);
+  if (rc != RDV_OK) return rc;
+  if (desc->images == 0 || desc->rows == 0) return 0;
+  return group_norm_workspace_bytes(*desc, backward != 0, plan_cu_count());
+}
+
+int rdv_group_norm(const rdv_group_norm_desc* desc, const void* x, const float* weight, const float* bias, void* y,
+                   float* stats, void* workspace, int64_t workspace_bytes, void* stream) {
+  const int rc = check_group_norm(desc, false);
+  if (rc != RDV_OK) return rc;
+  if (desc->images == 0 || desc->rows == 0) return RDV_OK;
+  if (!x || !y) return fail(RDV_ERR_INVALID, "rdv_group_norm: NULL pointer argument");
+  const int64_t need = group_norm_workspace_bytes(*desc, false, plan_cu_count());
+  if (need > 0 && (!workspace || workspace_bytes < need || !aligned16(workspace)))
+    return fail(RDV_ERR_WORKSPACE, "rdv_group_norm: workspace too small or not 16-byte aligned");
+  return launch_group_norm(*desc, x, weight, bias, y, stats, workspace, static_cast<hipStream_t>(stream));
+}
+
+int rdv_group_norm_backward(const rdv_group_norm_desc* desc, const void* grad, const void* x, const float* weight,
+                            const float* bias, const float* stats, void* dx, float* dweight, float* dbias,
+                            void* workspace, int64_t workspace_bytes, void* stream) {
+  const int rc = check_group_norm(desc, true);
+  if (rc != RDV_OK) return rc;
+  if (desc->images > 0 && desc->rows > 0) {
+    if (!grad || !x || !stats || !dx) return fail(RDV_ERR_INVALID, "rdv_group_norm_backward: NULL pointer argument");
+    const int64_t need = group_norm_workspace_bytes(*desc, true, plan_cu_count());
+    if (need > 0 && (!workspace || workspace_bytes < need || !aligned16(workspace)))
+      return fail(RDV_ERR_WORKSPACE, "rdv_group_norm_backward: workspace too small or not 16-byte aligned");
+  }
+  return launch_group_norm_backward(*desc, grad, x, weight, bias, stats, dx, dweight, dbias, workspace,
+                                    static_cast<hipStream_t>(stream));
+}
+
+static int check_attention(const rdv_attention_desc* d, bool backward) {
+  if (!d) return fail(RDV_ERR_INVALID, "attention: NULL descriptor");
+  if (d->batch < 0 || d->queries < 0 || d->keys < 0)
+    return fail(RDV_ERR_INVALID, "attention: batch, queries and keys must be >= 0");
+  if (d->heads < 1 || d->heads > (1 << 16) || d->kv_heads < 1 || d->heads % d->kv_heads != 0)
+    return fail(RDV_ERR_INVALID, "attention: heads must be in [1, 65536] and kv_heads must divide it");
+  if (d->dim < 1) return fail(RDV_ERR_INVALID, "attention: dim must be >= 1");
+  if (d->dim > RDV_ATTENTION_MAX_DIM)
+    return fail(RDV_ERR_UNSUPPORTED, "attention: dim must be at most " + std::to_string(RDV_ATTENTION_MAX_DIM));
+  if (d->dtype < RDV_DTYPE_F32 || d->dtype > RDV_DTYPE_BF16) return fail(RDV_ERR_INVALID, "attention: unknown dtype");
+  if (!(d->scale > -3.0e38f && d->scale < 3.0e38f)) return fail(RDV_ERR_INVALID, "attention: scale must be finite");
+  const int64_t longest = d->queries > d->keys ? d->queries : d->keys;
+  if (longest >= (int64_t(1) << 31) - 1024 ||
+      (d->batch > 0 && longest > 0 && int64_t(d->batch) * d->heads > (int64_t(1) << 40) / d->dim / longest))
+    return fail(RDV_ERR_INVALID, "attention: tensor too large");
+  for (int i = 0; i < 3; ++i)
+    if (!stride_ok(d->q_stride[i]) || !stride_ok(d->k_stride[i]) || !stride_ok(d->v_stride[i]) ||
+        (backward && !stride_ok(d->g_stride[i])))
+      return fail(RDV_ERR_INVALID, "attention: strides must be in [0, 2^40)");
+  if (!stride_ok(d->mask_stride)) return fail(RDV_ERR_INVALID, "attention: strides must be in [0, 2^40)");
+  return RDV_OK;
+}
+
+int64_t rdv_cross_attention_workspace_bytes(const rdv_attention_desc* desc, int32_t backward) {
+  const int rc = check_attention(desc, backward != 0);
+  if (rc != RDV_OK) return rc;
+  return attention_workspace_bytes(*desc, backward != 0, plan_cu_count());
+}
+
+int rdv_cross_attention(const rdv_attention_desc* desc, const void* q, const void* k, const void* v,
+                        const int32_t* key_lengths, const uint8_t* key_mask, void* out, float* lse, void* workspace,
+                        int64_t workspace_bytes, void* stream) {
+  const int rc = check_attention(desc, false);
+  if (rc != RDV_OK) return rc;
+  if (desc->batch == 0 || desc->queries == 0) return RDV_OK;
+  if (!q || !out || (desc->keys > 0 && (!k || !v)))
+    return fail(RDV_ERR_INVALID, "rdv_cross_attention: NULL pointer argument");
+  const int64_t need = attention_workspace_bytes(*desc, false, plan_cu_count());
+  if (need > 0 && (!workspace || workspace_bytes < need || !aligned16(workspace)))
+    return fail(RDV_ERR_WORKSPACE, "rdv_cross_attention: workspace too small or not 16-byte aligned");
+  return launch_attention(*desc, q, k, v, key_lengths, key_mask, out, lse, workspace,
+                          static_cast<hipStream_t>(stream));
+}
+
+int rdv_cross_attention_backward(const rdv_attention_desc* desc, const void* grad, const void* q, const void* k,
+                                 const void* v, const void* out, const float* lse, const int32_t* key_lengths,
+                                 const uint8_t* key_mask, void* dq, void* dk, void* dv, void* workspace,
+                                 int64_t workspace_bytes, void* stream) {
+  const int rc = check_attention(desc, true);
+  if (rc != RDV_OK) return rc;
+  if (desc->batch == 0) return RDV_OK;
+  if ((desc->queries > 0 && (!grad || !q || !out || !lse || !dq)) || (desc->keys > 0 && (!k || !v || !dk || !dv)))
+    return fail(RDV_ERR_INVALID, "rdv_cross_attention_backward: NULL pointer argument");
+  const int64_t need = attention_workspace_bytes(*desc, true, plan_cu_count());
+  if (need > 0 && (!workspace || workspace_bytes < need || !aligned16(workspace)))
+    return fail(RDV_ERR_WORKSPACE, "rdv_cross_attention_backward: workspace too small or not 16-byte aligned");
+  return launch_attention_backward(*desc, grad, q, k, v, out, lse, key_lengths, key_mask, dq, dk, dv, workspace,
+                                   static_cast<hipStream_t>(stream));
+}
+
+int rdv_dropout(const void* x, const void* residual, void* y, int64_t n, int32_t dtype, double p, uint64_t seed,
+                uint64_t subsequence, void* stream) {
+  if (n < 0 || n > (int64_t(1) << 40)) return fail(RDV_ERR_INVALID, "rdv_dropout: n must be in [0, 2^40]");
+  if (dtype < RDV_DTYPE_F32 || dtype > RDV_DTYPE_BF16) return fail(RDV_ERR_INVALID, "rdv_dropout: unknown dtype");
+  if (!(p >= 0.0 && p <= 1.0)) return fail(RDV_ERR_INVALID, "rdv_dropout: p must be in [0, 1]");
+  if (n == 0) return RDV_OK;
+  if (!x || !y) return fail(RDV_ERR_INVALID, "rdv_dropout: NULL pointer argument");
+  return launch_dropout(x, residual, y, n, dtype, p, seed, subsequence, static_cast<hipStream_t>(stream));
 }
 
 const char* rdv_mlp_kernel_name(const rdv_mlp_desc* desc) {

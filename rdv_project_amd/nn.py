@@ -19,14 +19,15 @@ TensorOperation nodes dispatch eagerly, one kernel per op:
   Downsample2xTensorOp           nn.py:1090-1107
   Upsample2xTensorOp             nn.py:1110-1125
   ConcatTensorOp                 nn.py:1128-1150
-Build-defined additions (no reference counterpart, needed by the benchmark
-configurations): FrequencyEncoding, Softplus, Sigmoid, DensityRGB.
+Build-defined additions (no reference counterpart): FrequencyEncoding, Softplus,
+Sigmoid, DensityRGB, and the image networks' GroupNormTensorOp,
+CrossAttentionTensorOp and DropoutTensorOp.
 """
 from __future__ import annotations
 
 import torch
 
-from . import _conv, _lib, _tensor_ops
+from . import _conv, _image_ops, _lib, _tensor_ops
 from .core import RDVObject, wrap
 from .maths import Map, TensorOperation, _as_op_input
 
@@ -579,3 +580,96 @@ class Conv2DTensorOpWindow3x3(_Conv2DTensorOpBase):
         shared_bytes = (fetch * fetch * in_channels + 16 * 9 * in_channels) * 2 + 64 * 16 * 2 + 64 * 16 * 4
         assert shared_bytes <= 49152, f"in_channels ({in_channels}) needs {shared_bytes} bytes of shared memory (48KB budget)"
         self._finish()
+
+
+# ------------------------------------------------- image networks (build-defined)
+class GroupNormTensorOp(TensorOperation):
+    """activation(weight * (x - mean) / sqrt(var + eps) + bias) over one
+    channels-last image x [H*W, C], statistics over the image and each of
+    `groups` runs of channels; activation "none", "relu" or "silu".  result
+    [H*W, C] fp32.  group_norm is the form for batches, other types and
+    training."""
+
+    _TILE_ROWS = 1
+    _TILE_COLS = 1
+
+    def __init__(self, x, weight, bias, groups: int, eps: float = 1e-5, activation: str = "none") -> None:
+        data, shape, upstream = _as_op_input(x)
+        assert len(shape) == 2, "GroupNormTensorOp requires a 2D (H*W, C) input"
+        self.x_buf = _op_float32(data, "x")
+        self.weight, self.bias = (None if p is None else wrap(_float32(p) if not isinstance(p, RDVObject) else p)
+                                  for p in (weight, bias))
+        self.groups, self.eps, self.activation = int(groups), float(eps), activation
+        self._inputs()  # checked before anything is allocated
+        self._upstream = upstream
+        super().__init__(shape)
+
+    def _inputs(self):
+        return _image_ops._norm_inputs(self.x_buf, self.weight, self.bias, self.groups, self.eps, self.activation)
+
+    def _forward(self) -> None:
+        x, weight, bias, d = self._inputs()
+        _image_ops._group_norm_into(d, x, weight, bias, self._result_t, None)
+
+
+class CrossAttentionTensorOp(TensorOperation):
+    """softmax(q k^T / sqrt(D)) v per head, from q [rows, heads * D] to the states
+    k and v [states, kv_heads * D] (kv_heads defaults to heads and divides it;
+    D at most 128); each input a buffer or an upstream TensorOperation.  result
+    [rows, heads * D] fp32.  cross_attention is the form for batches, masks,
+    other types and training."""
+
+    _TILE_ROWS = 1
+    _TILE_COLS = 1
+
+    def __init__(self, q, k, v, heads: int, kv_heads: int | None = None) -> None:
+        (qd, qs, qu), (kd, ks, ku), (vd, vs, vu) = _as_op_input(q), _as_op_input(k), _as_op_input(v)
+        kv_heads = heads if kv_heads is None else kv_heads
+        assert len(qs) == 2 and len(ks) == 2 and ks == vs, \
+            "CrossAttentionTensorOp requires 2D (rows, heads * D) inputs, k and v of one shape"
+        assert heads >= 1 and kv_heads >= 1 and heads % kv_heads == 0, \
+            f"kv_heads ({kv_heads}) must divide heads ({heads})"
+        assert qs[1] % heads == 0, f"q's channels ({qs[1]}) must be a multiple of heads ({heads})"
+        dim = qs[1] // heads
+        assert ks[1] == kv_heads * dim, f"k and v must have kv_heads * {dim} = {kv_heads * dim} channels, got {ks[1]}"
+        self.q_buf, self.k_buf, self.v_buf = _op_float32(qd, "q"), _op_float32(kd, "k"), _op_float32(vd, "v")
+        self.heads, self.kv_heads, self.D = int(heads), int(kv_heads), int(dim)
+        ups = [u for u in (qu, ku, vu) if u is not None]
+        self._upstream = ups[0] if ups else None
+        self._extra_upstreams = tuple(ups[1:])
+        super().__init__(qs)
+
+    def _forward(self) -> None:
+        q, k, v = (t.as_tensor("torch").unflatten(1, (h, self.D)).unsqueeze(0) for t, h in
+                   ((self.q_buf, self.heads), (self.k_buf, self.kv_heads), (self.v_buf, self.kv_heads)))
+        q, k, v, _, _, d = _image_ops._attention_inputs(q, k, v, None, None, None)
+        _image_ops._cross_attention_into(d, q, k, v, None, None, self._result_t, None)
+
+
+class DropoutTensorOp(TensorOperation):
+    """residual + x * keep / (1 - p) over x [rows, C] (a buffer or an upstream
+    TensorOperation, and so residual, which may be None); the mask follows from
+    (seed, subsequence) as dropout's does.  evaluate() draws the same mask
+    again; set `subsequence` for another.  result [rows, C] fp32."""
+
+    _TILE_ROWS = 1
+    _TILE_COLS = 1
+
+    def __init__(self, x, p: float, seed: int, subsequence: int = 0, residual=None) -> None:
+        data, shape, upstream = _as_op_input(x)
+        self.x_buf = _op_float32(data, "x")
+        self.residual_buf, extra = None, None
+        if residual is not None:
+            rdata, rshape, extra = _as_op_input(residual)
+            assert rshape == shape, f"residual must have x's shape {shape}, got {rshape}"
+            self.residual_buf = _op_float32(rdata, "residual")
+        self.p, self.seed, self.subsequence = p, seed, subsequence
+        _image_ops._dropout_inputs(self.x_buf, p, seed, subsequence)
+        self._upstream = upstream
+        self._extra_upstreams = (extra,) if extra is not None else ()
+        super().__init__(shape)
+
+    def _forward(self) -> None:
+        x, p, seed, subsequence = _image_ops._dropout_inputs(self.x_buf, self.p, self.seed, self.subsequence)
+        residual = None if self.residual_buf is None else self.residual_buf.as_tensor("torch")
+        _image_ops._dropout_into(x, p, seed, subsequence, residual, self._result_t)

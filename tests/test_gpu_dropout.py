@@ -1,0 +1,104 @@
+"""GPU parity of dropout and dropout_backward against oracle/image_ops.py: masks equal, values to one rounding of the
+factor, the product and the sum in fp32 and one to the type."""
+import numpy as np
+import pytest
+import torch
+
+import rdv_project_amd as rdv
+from oracle import image_ops as O
+
+pytestmark = pytest.mark.gpu
+
+TYPES = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+
+
+def _np(t):
+    return t.detach().double().cpu().numpy()
+
+
+def _bound(ref, parts, dtype):
+    return 3 * O.U32 * parts + O._stored(ref, dtype)
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("n", [1, 3, 4, 5, 8, 31, 1023, 4096, 5001])
+@pytest.mark.parametrize("p", [0.0, 0.25, 0.9])
+def test_matches_oracle(dtype, n, p):
+    g = torch.Generator().manual_seed(n)
+    x, r = (torch.randn(n, generator=g).to(TYPES[dtype]).cuda() for _ in range(2))
+    seed, sub = 0xDEADBEEF12345678, (1 << 40) + n
+    ref = O.dropout(_np(x), p, seed, sub)
+    got = rdv.dropout(x, p, seed, sub)
+    assert ((_np(got) != 0) == (ref != 0)).all()
+    assert (np.abs(_np(got) - ref) <= _bound(ref, np.abs(ref), dtype)).all()
+    ref2 = ref + _np(r)
+    got2 = rdv.dropout(x, p, seed, sub, residual=r)
+    assert (np.abs(_np(got2) - ref2) <= _bound(ref2, np.abs(ref) + np.abs(_np(r)), dtype)).all()
+    back = rdv.dropout_backward(r, p, seed, sub)
+    refb = O.dropout(_np(r), p, seed, sub)
+    assert (np.abs(_np(back) - refb) <= _bound(refb, np.abs(refb), dtype)).all()
+
+
+def test_gradient_against_differences():
+    """Linear in x: the difference quotient along any direction is the gradient's."""
+    g = torch.Generator().manual_seed(1)
+    x, d, w = (torch.randn(3001, generator=g).cuda() for _ in range(3))
+    f = lambda t: (rdv.dropout(t, 0.3, 5, 6).double() * w.double()).sum().item()
+    slope = (f(x + d) - f(x - d)) / 2
+    grad = (rdv.dropout_backward(w, 0.3, 5, 6).double() * d.double()).sum().item()
+    assert abs(slope - grad) <= 8 * O.U32 * 1.5 * ((x.abs() + d.abs()) * w.abs()).sum().item()
+
+
+def test_everything_dropped_or_kept():
+    x = torch.randn(1001).cuda()
+    r = torch.randn(1001).cuda()
+    x[3], x[4] = float("nan"), float("inf")
+    assert not rdv.dropout(x, 1.0, 1).any()
+    assert torch.equal(rdv.dropout(x, 1.0, 1, residual=r), r)
+    y = rdv.dropout(x, 0.0, 1)
+    assert torch.equal(torch.nan_to_num(y), torch.nan_to_num(x)) and torch.isnan(y[3])
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_views_and_buffers(dtype):
+    """The mask goes by the row-major index, whatever the strides and alignment; out may be an input."""
+    base = torch.randn(41, 37).to(TYPES[dtype]).cuda()
+    expect = rdv.dropout(base.clone(), 0.5, 9, 2, residual=base)
+    assert torch.equal(rdv.dropout(base.t().contiguous().t(), 0.5, 9, 2, residual=base), expect)
+    for shift in (1, 2, 3):
+        flat = torch.zeros(41 * 37 + 3, dtype=base.dtype, device="cuda")
+        x = flat[shift:shift + 41 * 37].reshape(41, 37)
+        x.copy_(base)
+        assert torch.equal(rdv.dropout(x, 0.5, 9, 2, residual=base), expect)
+        assert rdv.dropout(x, 0.5, 9, 2, residual=x, out=x) is x and torch.equal(x, expect)
+        assert not flat[:shift].any() and not flat[shift + 41 * 37:].any()
+
+
+def test_streams_of_numbers_are_apart():
+    x = torch.ones(1 << 16, device="cuda")
+    masks = [rdv.dropout(x, 0.5, s, q) != 0 for s, q in ((1, 0), (2, 0), (1, 1), (1, 1 << 32), (1 << 32, 0))]
+    for i, a in enumerate(masks):
+        assert abs(a.float().mean().item() - 0.5) < 5 * 0.5 / 256
+        for b in masks[:i]:
+            assert abs((a == b).float().mean().item() - 0.5) < 5 * 0.5 / 256
+
+
+def test_more_elements_than_32_bits_count():
+    n = (1 << 32) + 9
+    x = torch.ones(n, dtype=torch.bfloat16, device="cuda")
+    y = rdv.dropout(x, 0.5, 77, 3, out=x)
+    for i in [0, 5, (1 << 31) - 1, 1 << 31, (1 << 32) - 1, 1 << 32, n - 1]:
+        assert y[i].item() == (2.0 if O.dropout_keep(i, 0.5, 77, 3) else 0.0), i
+
+
+def test_empty():
+    assert rdv.dropout(torch.empty(0, 5, device="cuda"), 0.5, 1).shape == (0, 5)
+
+
+def test_tensor_op():
+    x, r = torch.randn(12, 16).cuda(), torch.randn(12, 16).cuda()
+    op = rdv.DropoutTensorOp(rdv.ReLUTensorOp(x), 0.4, 3, 8, residual=r)
+    assert torch.equal(op.as_type("torch"), rdv.dropout(x.relu(), 0.4, 3, 8, residual=r))
+    op.subsequence = 9
+    op.evaluate()
+    assert torch.equal(op.as_type("torch"), rdv.dropout(x.relu(), 0.4, 3, 9, residual=r))

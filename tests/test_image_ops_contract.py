@@ -1,0 +1,130 @@
+"""What the image-network operators refuse, and how; sizes the library reports (CPU only, no launches)."""
+import ctypes as C
+
+import pytest
+import torch
+
+import rdv_project_amd as rdv
+from rdv_project_amd import _lib
+
+X, W, B = torch.zeros(2, 5, 12), torch.ones(12), torch.zeros(12)
+Q, K = torch.zeros(2, 3, 4, 8), torch.zeros(2, 6, 2, 8)
+LSE = torch.zeros(2, 4, 3)
+
+
+@pytest.mark.parametrize("call,error,text", [
+    (lambda: rdv.group_norm(X, W, B, 5), AssertionError, "divide the channels"),
+    (lambda: rdv.group_norm(X, W, B, 0), AssertionError, "divide the channels"),
+    (lambda: rdv.group_norm(X[0, 0], W, B, 3), AssertionError, "rows, channels"),
+    (lambda: rdv.group_norm(X, W[:6], B, 3), AssertionError, "weight must be"),
+    (lambda: rdv.group_norm(X, W, B.half(), 3), TypeError, "bias must be float32"),
+    (lambda: rdv.group_norm(X.int(), W, B, 3), TypeError, "x must be float32"),
+    (lambda: rdv.group_norm([1.0], W, B, 3), TypeError, "torch tensor"),
+    (lambda: rdv.group_norm(X, W, B, 3, activation="gelu"), ValueError, "activation"),
+    (lambda: rdv.group_norm_backward(X.half(), X, W, B, 3, torch.zeros(2, 3, 2)), TypeError, "grad must be"),
+    (lambda: rdv.group_norm_backward(X[:1], X, W, B, 3, torch.zeros(2, 3, 2)), AssertionError, "grad must have"),
+    (lambda: rdv.group_norm_backward(X, X, W, B, 3, torch.zeros(2, 4, 2)), AssertionError, "stats must be"),
+    (lambda: rdv.cross_attention(Q[0], K, K), AssertionError, "q must be"),
+    (lambda: rdv.cross_attention(Q, K, K[:, :5]), AssertionError, "k and v"),
+    (lambda: rdv.cross_attention(Q[:1], K, K), AssertionError, "batch"),
+    (lambda: rdv.cross_attention(Q[..., :7], K, K), AssertionError, "dimensions"),
+    (lambda: rdv.cross_attention(Q[:, :, :3], K, K), AssertionError, "kv_heads"),
+    (lambda: rdv.cross_attention(Q.half(), K, K), TypeError, "one type"),
+    (lambda: rdv.cross_attention(Q, K, K, key_lengths=torch.zeros(2)), TypeError, "key_lengths must be int32"),
+    (lambda: rdv.cross_attention(Q, K, K, key_lengths=torch.zeros(3, dtype=torch.int32)), AssertionError, "batch"),
+    (lambda: rdv.cross_attention(Q, K, K, key_mask=torch.zeros(2, 6)), TypeError, "bool"),
+    (lambda: rdv.cross_attention(Q, K, K, key_mask=torch.zeros(6, dtype=torch.bool)), AssertionError, "key_mask"),
+    (lambda: rdv.cross_attention(Q, K, K, scale=float("inf")), ValueError, "finite"),
+    (lambda: rdv.dropout(X, -0.1, 1), ValueError, "p must be"),
+    (lambda: rdv.dropout(X, float("nan"), 1), ValueError, "p must be"),
+    (lambda: rdv.dropout(X, 0.5, -1), ValueError, "seed must be"),
+    (lambda: rdv.dropout(X, 0.5, 1, 1 << 64), ValueError, "subsequence must be"),
+    (lambda: rdv.dropout(X, 0.5, 1, residual=X[:1]), AssertionError, "residual must have"),
+    (lambda: rdv.dropout(X, 0.5, 1, residual=X.half()), TypeError, "residual must be"),
+    # no CPU path
+    (lambda: rdv.group_norm(X, W, B, 3), TypeError, "GPU tensor"),
+    (lambda: rdv.cross_attention(Q, K, K), TypeError, "GPU tensor"),
+    (lambda: rdv.dropout(X, 0.5, 1), TypeError, "GPU tensor"),
+])
+def test_refusals(call, error, text):
+    with pytest.raises(error, match=text):
+        call()
+
+
+@pytest.mark.gpu
+def test_refusals_of_buffers():
+    x, q, k, lse = X.cuda(), Q.cuda(), K.cuda(), LSE.cuda()
+    w, b, st = W.cuda(), B.cuda(), torch.zeros(2, 3, 2).cuda()
+    for call, error, text in (
+        (lambda: rdv.group_norm(x, w, b, 3, out=x), AssertionError, "share memory"),
+        (lambda: rdv.group_norm(x, w, b, 3, out=x.half()), TypeError, "out must be"),
+        (lambda: rdv.group_norm(x, w, b, 3, out=x[:1]), AssertionError, "out must have"),
+        (lambda: rdv.group_norm(x, w, b, 3, out=torch.empty(5, 2, 12).cuda().transpose(0, 1)), AssertionError,
+         "contiguous"),
+        (lambda: rdv.group_norm(x, W, b, 3), TypeError, "weight must be a GPU tensor"),
+        (lambda: rdv.group_norm_backward(x, x, w, b, 3, st, grads=(x,)), TypeError, "grads must be"),
+        (lambda: rdv.group_norm_backward(x, x, w, b, 3, st, grads=(x, w, b)), AssertionError, "share memory"),
+        (lambda: rdv.cross_attention(q, k, k, out=q), AssertionError, "share memory"),
+        (lambda: rdv.cross_attention(q, k, k, key_mask=torch.zeros(2, 6, dtype=torch.bool)), TypeError, "key_mask"),
+        (lambda: rdv.cross_attention_backward(q, q, k, k, q, lse[:1]), AssertionError, "lse must be"),
+        (lambda: rdv.cross_attention(torch.zeros(1, 1, 1, 129).cuda(), *[torch.zeros(1, 1, 1, 129).cuda()] * 2),
+         NotImplementedError, "at most 128"),
+        (lambda: rdv.dropout(x, 0.5, 1, out=x[:, :3]), AssertionError, "out must have"),
+        (lambda: rdv.dropout(x[:, 1:4], 0.5, 1, out=x.flatten()[:72].reshape(2, 3, 12)), AssertionError,
+         "share memory"),
+    ):
+        with pytest.raises(error, match=text):
+            call()
+
+
+def _norm_desc(**kw):
+    d = _lib.GroupNormDesc(images=1, rows=4, channels=8, groups=2, act=_lib.ACT_NONE, dtype=_lib.DTYPE_F32, eps=1e-5,
+                           x_row_stride=8, x_image_stride=32, g_row_stride=8, g_image_stride=32)
+    for name, value in kw.items():
+        setattr(d, name, value)
+    return d
+
+
+@pytest.mark.parametrize("kw,text", [
+    (dict(groups=3), "divide"), (dict(channels=0), "channels"), (dict(images=-1), "images"), (dict(act=2), "activation"),
+    (dict(dtype=3), "dtype"), (dict(eps=-1.0), "eps"), (dict(eps=float("nan")), "eps"), (dict(reserved=1), "reserved"),
+    (dict(rows=1 << 31), "rows"), (dict(images=1 << 30, rows=1 << 30), "too large"), (dict(x_row_stride=-1), "strides"),
+])
+def test_library_refuses_group_norm(kw, text):
+    lib = _lib.load()
+    d = _norm_desc(**kw)
+    assert lib.rdv_group_norm_workspace_bytes(C.byref(d), 0) == _lib.RDV_ERR_INVALID and text in _lib.last_error()
+    assert lib.rdv_group_norm(C.byref(d), 16, None, None, 16, None, None, 0, None) == _lib.RDV_ERR_INVALID
+
+
+def _attn_desc(**kw):
+    d = _lib.AttentionDesc(batch=1, queries=2, keys=3, heads=4, kv_heads=2, dim=8, dtype=_lib.DTYPE_F16, scale=1.0)
+    for name, value in kw.items():
+        setattr(d, name, value)
+    return d
+
+
+@pytest.mark.parametrize("kw,code,text", [
+    (dict(heads=3), -1, "divide"), (dict(kv_heads=0), -1, "divide"), (dict(dim=0), -1, "dim"),
+    (dict(dim=129), -2, "at most 128"), (dict(keys=-1), -1, "keys"), (dict(dtype=5), -1, "dtype"),
+    (dict(scale=float("inf")), -1, "scale"), (dict(mask_stride=-1), -1, "strides"),
+    (dict(batch=1 << 30, queries=1 << 30), -1, "too large"),
+])
+def test_library_refuses_attention(kw, code, text):
+    lib = _lib.load()
+    d = _attn_desc(**kw)
+    assert lib.rdv_cross_attention_workspace_bytes(C.byref(d), 1) == code and text in _lib.last_error()
+    assert lib.rdv_cross_attention(C.byref(d), 16, 16, 16, None, None, 16, None, None, 0, None) == code
+
+
+def test_library_refuses_null_pointers_and_dropout_arguments():
+    lib = _lib.load()
+    assert lib.rdv_group_norm(None, 16, None, None, 16, None, None, 0, None) == _lib.RDV_ERR_INVALID
+    assert lib.rdv_group_norm(C.byref(_norm_desc()), None, None, None, 16, None, None, 0, None) == _lib.RDV_ERR_INVALID
+    d = _attn_desc()
+    assert lib.rdv_cross_attention(C.byref(d), 16, None, 16, None, None, 16, None, None, 0, None) == _lib.RDV_ERR_INVALID
+    assert lib.rdv_cross_attention_backward(C.byref(d), *[16] * 6, *[None] * 6, 0, None) == _lib.RDV_ERR_INVALID
+    for args in ((16, None, 16, -1, 0, 0.5), (16, None, 16, 4, 3, 0.5), (16, None, 16, 4, 0, 1.5),
+                 (16, None, 16, 4, 0, float("nan")), (None, None, 16, 4, 0, 0.5)):
+        assert lib.rdv_dropout(*args, 0, 0, None) == _lib.RDV_ERR_INVALID
+    assert lib.rdv_dropout(None, None, None, 0, 0, 0.5, 0, 0, None) == _lib.RDV_OK
