@@ -550,7 +550,9 @@ int rdv_broadcast_rows(const float* value, int32_t width, int64_t rows, float* o
  * sums, statistics and softmax terms are fp32 and results are rounded once.
  * Strides are in elements.  Results are the same from call to call (no
  * atomics).  Workspaces are 16-byte aligned device memory that one call uses
- * alone until it has run; their contents need not be kept or cleared. */
+ * alone until it has run; their contents need not be kept or cleared.  Results
+ * (not rdv_dropout's) are 16-byte aligned, and so is every attention input
+ * whose dim and strides are multiples of 16 bytes; others need no alignment. */
 
 /* Group normalisation of channels-last images x[images, rows, channels]
  * (rows = H W): the channels fall into `groups` equal runs, and with mean and

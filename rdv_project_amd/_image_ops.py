@@ -57,7 +57,7 @@ def _on_gpu(*named) -> None:
             raise TypeError(f"{what} is on {t.device}, the current GPU is cuda:{torch.cuda.current_device()}")
 
 
-def _out_tensor(out, shape, dtype, device, what: str = "out") -> torch.Tensor:
+def _out_tensor(out, shape, dtype, device, what: str = "out", aligned: bool = True) -> torch.Tensor:
     """The caller's buffer, checked to be what the kernels write, or a fresh one."""
     if out is None:
         return torch.empty(shape, dtype=dtype, device=device)
@@ -66,6 +66,7 @@ def _out_tensor(out, shape, dtype, device, what: str = "out") -> torch.Tensor:
     if out.dtype != dtype or out.device != device:
         raise TypeError(f"{what} must be {dtype} on {device}, got {out.dtype} on {out.device}")
     assert out.is_contiguous(), f"{what} must be contiguous"
+    assert not aligned or out.data_ptr() % 16 == 0, f"{what} must be 16-byte aligned"
     return out
 
 
@@ -216,6 +217,13 @@ def _innermost(t: torch.Tensor) -> torch.Tensor:
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
+def _rows_in_place(t: torch.Tensor) -> torch.Tensor:
+    """t [batch, length, heads, dim] as the library reads it: the innermost dimension contiguous and, as rows whose
+    strides are multiples of 16 bytes are read in pieces of that size, such a tensor itself aligned to it."""
+    t = _innermost(t)
+    return t if t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
+
+
 def _attention_inputs(q, k, v, key_lengths, key_mask, scale):
     q, k, v = _data(q, "q"), _data(k, "k"), _data(v, "v")
     assert q.dim() == 4, "q must be [batch, queries, heads, dim]"
@@ -241,7 +249,7 @@ def _attention_inputs(q, k, v, key_lengths, key_mask, scale):
     if not math.isfinite(scale):
         raise ValueError(f"scale must be finite, got {scale}")
     _on_gpu((q, "q"), (k, "k"), (v, "v"), (key_lengths, "key_lengths"), (key_mask, "key_mask"))
-    q, k, v = _innermost(q), _innermost(k), _innermost(v)
+    q, k, v = _rows_in_place(q), _rows_in_place(k), _rows_in_place(v)
     d = _lib.AttentionDesc()
     d.batch, d.queries, d.keys, d.heads, d.kv_heads, d.dim = b, lq, lk, hq, hkv, dim
     d.dtype, d.scale = _DTYPES[q.dtype], scale
@@ -303,7 +311,7 @@ def cross_attention_backward(grad, q, k, v, out, lse, key_lengths=None, key_mask
     if lse.dtype != torch.float32:
         raise TypeError(f"lse must be float32, got {lse.dtype}")
     _on_gpu((grad, "grad"), (out, "out"), (lse, "lse"))
-    grad = _innermost(grad)
+    grad = _rows_in_place(grad)
     d.g_stride[:] = grad.stride()[:3]
     given = grads is not None
     grads = _grad_tensors(grads, (q.shape, k.shape, v.shape), (q.dtype,) * 3, q.device, ("dq", "dk", "dv"))
@@ -357,7 +365,7 @@ def dropout(x, p: float, seed: int, subsequence: int = 0, residual=None, out=Non
     if residual is not None:
         residual = _like(residual, x, "residual")
     _on_gpu((x, "x"), (residual, "residual"))
-    y = _out_tensor(out, x.shape, x.dtype, x.device)
+    y = _out_tensor(out, x.shape, x.dtype, x.device, aligned=False)
     if out is not None:
         for t, what in ((x, "x"), (residual, "residual")):
             if t is not None and not (t.data_ptr() == y.data_ptr() and t.is_contiguous()):

@@ -35,7 +35,9 @@ SOURCES = [
     "mlp_generic.hip",
     "train_fused.hip",
     "train.hip",
-    "attention.hip",
+    "attention_f32.hip",
+    "attention_f16.hip",
+    "attention_bf16.hip",
     "winograd.hip",
     "conv_op.hip",
     "mlp_fused.hip",
@@ -43,6 +45,7 @@ SOURCES = [
     "capi.cpp",
     "mlp_pack.hip",
     "mlp_f32.hip",
+    "attention.hip",
     "group_norm.hip",
     "tensor_data.hip",
     "dropout.hip",

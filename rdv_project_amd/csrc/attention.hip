@@ -1,161 +1,184 @@
-// Attention from an image's points to an encoder's states, forward and backward.
-// Build-defined (no counterpart in the reference).
-//
-// S = scale Q K^T over the states that count, P = exp(S - lse), O = P V; backward with dO:
-//   delta = rowsum(dO O);  dV = P^T dO;  dS = P (dO V^T - delta) scale;  dQ = dS K;  dK = dS^T Q.
-#include "operators.h"
+// Attention from an image's points to an encoder's states: planning, workspaces and the passes around the matrix-core
+// kernels of attention.h.  Build-defined (no counterpart in the reference).
+#include <algorithm>
+
+#include "attention.h"
 
 namespace rdv {
 
 namespace {
 
-struct AttnArgs {
-  const void *q, *k, *v, *g, *o;
-  const int32_t* lengths;
-  const uint8_t* mask;
-  void *out, *dq, *dk, *dv;
-  float* lse;
-  int64_t qs[3], ks[3], vs[3], gs[3], ms;
-  int batch, queries, keys, heads, kv_heads, dim, share;
-  float scale;
+int64_t align256(int64_t bytes) { return (bytes + 255) / 256 * 256; }
+int element_bytes(int dtype) { return dtype == RDV_DTYPE_F32 ? 4 : 2; }
+
+// Whether the kernels can read a tensor in place: rows are whole 16-byte pieces.
+bool in_place(const rdv_attention_desc& d, const int64_t (&s)[3], int length, int heads) {
+  const int e = 16 / element_bytes(d.dtype);
+  return d.dim % e == 0 && (d.batch == 1 || s[0] % e == 0) && (length == 1 || s[1] % e == 0) &&
+         (heads == 1 || s[2] % e == 0);
+}
+
+// How an axis of `length` is split among blocks so that `blocks` of them become about `want`: every split takes a
+// multiple of `step` and at least `least`.
+struct Split {
+  int count, chunk;
+};
+Split split_axis(int64_t blocks, int64_t want, int length, int step, int least) {
+  int64_t n = blocks > 0 ? want / blocks : 1;
+  n = std::min<int64_t>(n, length / least);
+  if (n < 2) return Split{1, length};
+  const int64_t chunk = (int64_t(length) + n * step - 1) / (n * step) * step;
+  return Split{int((length + chunk - 1) / chunk), int(chunk)};
+}
+
+struct Plan {
+  int rows, dim, pdim;            // folded rows; dimensions rounded up to 16 bytes, to 4
+  int64_t bh;
+  bool few;
+  Split forward, dq, dkv;
+  int row_tiles, key_tiles;
+  // byte offsets in the workspace, and its size
+  int64_t packs[4], stats, part, part2, ml, bytes;
 };
 
-__device__ __forceinline__ float wave_sum(float v) {
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
-  return v;
-}
-
-__device__ __forceinline__ int key_limit(const AttnArgs& a, int b) {
-  return a.lengths ? min(max(a.lengths[b], 0), a.keys) : a.keys;
-}
-
-// One wave per query row; lane l holds dimensions l and l + 64.
-template <class T>
-__global__ __launch_bounds__(64) void attn_forward_kernel(AttnArgs a) {
-  const int lane = int(threadIdx.x);
-  const int64_t row = blockIdx.x;  // (b, query, head)
-  const int h = int(row % a.heads), i = int(row / a.heads % a.queries), b = int(row / a.heads / a.queries);
-  const int hk = h / a.share, d0 = lane, d1 = lane + 64;
-  const T* const q = static_cast<const T*>(a.q) + b * a.qs[0] + i * a.qs[1] + h * a.qs[2];
-  const T* const k = static_cast<const T*>(a.k) + b * a.ks[0] + hk * a.ks[2];
-  const T* const v = static_cast<const T*>(a.v) + b * a.vs[0] + hk * a.vs[2];
-  const float q0 = d0 < a.dim ? to_f32(q[d0]) * a.scale : 0.0f, q1 = d1 < a.dim ? to_f32(q[d1]) * a.scale : 0.0f;
-  float top = -INFINITY, total = 0.0f, o0 = 0.0f, o1 = 0.0f;
-  const int n = key_limit(a, b);
-  for (int j = 0; j < n; ++j) {
-    if (a.mask && !a.mask[b * a.ms + j]) continue;
-    const T* const kj = k + j * a.ks[1];
-    const T* const vj = v + j * a.vs[1];
-    const float s = wave_sum((d0 < a.dim ? q0 * to_f32(kj[d0]) : 0.0f) + (d1 < a.dim ? q1 * to_f32(kj[d1]) : 0.0f));
-    const float t = fmaxf(top, s), keep = top == t ? 1.0f : expf(top - t), p = expf(s - t);
-    total = total * keep + p;
-    o0 = o0 * keep + (d0 < a.dim ? p * to_f32(vj[d0]) : 0.0f);
-    o1 = o1 * keep + (d1 < a.dim ? p * to_f32(vj[d1]) : 0.0f);
-    top = t;
+Plan make_plan(const rdv_attention_desc& d, bool backward, int cu) {
+  Plan p{};
+  const int e = 16 / element_bytes(d.dtype);
+  p.rows = int(int64_t(d.heads / d.kv_heads) * d.queries);
+  p.dim = (d.dim + e - 1) / e * e;
+  p.pdim = (d.dim + 3) / 4 * 4;
+  p.bh = int64_t(d.batch) * d.kv_heads;
+  p.few = p.rows <= 32;
+  p.row_tiles = p.few ? 1 : (p.rows + 127) / 128;
+  p.key_tiles = (d.keys + 127) / 128;
+  int64_t at = 0;
+  // copies of inputs that cannot be read in place
+  const int64_t q_rows = int64_t(d.batch) * d.queries * d.heads, k_rows = int64_t(d.batch) * d.keys * d.kv_heads;
+  const int64_t rows[4] = {in_place(d, d.q_stride, d.queries, d.heads) ? 0 : q_rows,
+                           in_place(d, d.k_stride, d.keys, d.kv_heads) ? 0 : k_rows,
+                           in_place(d, d.v_stride, d.keys, d.kv_heads) ? 0 : k_rows,
+                           !backward || in_place(d, d.g_stride, d.queries, d.heads) ? 0 : q_rows};
+  for (int i = 0; i < 4; ++i) {
+    p.packs[i] = at;
+    at += align256(rows[i] * p.dim * element_bytes(d.dtype));
   }
-  const float inv = total > 0.0f ? 1.0f / total : 0.0f;
-  T* const out = static_cast<T*>(a.out) + row * a.dim;
-  if (d0 < a.dim) out[d0] = T(o0 * inv);
-  if (d1 < a.dim) out[d1] = T(o1 * inv);
-  if (a.lse && lane == 0)
-    a.lse[(int64_t(b) * a.heads + h) * a.queries + i] = total > 0.0f ? top + logf(total) : -INFINITY;
-}
-
-// One wave per query row: dQ.
-template <class T>
-__global__ __launch_bounds__(64) void attn_dq_kernel(AttnArgs a) {
-  const int lane = int(threadIdx.x);
-  const int64_t row = blockIdx.x;
-  const int h = int(row % a.heads), i = int(row / a.heads % a.queries), b = int(row / a.heads / a.queries);
-  const int hk = h / a.share;
-  const T* const q = static_cast<const T*>(a.q) + b * a.qs[0] + i * a.qs[1] + h * a.qs[2];
-  const T* const g = static_cast<const T*>(a.g) + b * a.gs[0] + i * a.gs[1] + h * a.gs[2];
-  const T* const o = static_cast<const T*>(a.o) + row * a.dim;
-  const T* const k = static_cast<const T*>(a.k) + b * a.ks[0] + hk * a.ks[2];
-  const T* const v = static_cast<const T*>(a.v) + b * a.vs[0] + hk * a.vs[2];
-  float qd[2], gd[2], acc[2] = {0.0f, 0.0f}, dl = 0.0f;
-  for (int e = 0; e < 2; ++e) {
-    const int d = lane + 64 * e;
-    qd[e] = d < a.dim ? to_f32(q[d]) * a.scale : 0.0f;
-    gd[e] = d < a.dim ? to_f32(g[d]) : 0.0f;
-    dl += d < a.dim ? gd[e] * to_f32(o[d]) : 0.0f;
-  }
-  const float delta = wave_sum(dl);
-  const float lse = a.lse[(int64_t(b) * a.heads + h) * a.queries + i];
-  const int n = key_limit(a, b);
-  for (int j = 0; j < n; ++j) {
-    if (a.mask && !a.mask[b * a.ms + j]) continue;
-    float kd[2], s = 0.0f, dp = 0.0f;
-    for (int e = 0; e < 2; ++e) {
-      const int d = lane + 64 * e;
-      kd[e] = d < a.dim ? to_f32(k[j * a.ks[1] + d]) : 0.0f;
-      s += qd[e] * kd[e];
-      dp += d < a.dim ? gd[e] * to_f32(v[j * a.vs[1] + d]) : 0.0f;
+  if (!backward) {
+    // two blocks per CU (four where states are streamed); a split reads at least 128 states
+    p.forward = split_axis(p.bh * p.row_tiles, p.few ? 4 * int64_t(cu) : 2 * int64_t(cu), d.keys, 128, p.few ? 256 : 128);
+    if (p.forward.count > 1) {
+      const int64_t partial = p.forward.count * p.bh * p.rows;
+      p.part = at;
+      at += align256(partial * p.pdim * 4);
+      p.ml = at;
+      at += align256(partial * 8);
     }
-    const float ds = expf(wave_sum(s) - lse) * (wave_sum(dp) - delta) * a.scale;
-    for (int e = 0; e < 2; ++e) acc[e] += ds * kd[e];
+  } else {
+    p.stats = at;
+    at += align256(p.bh * p.rows * 8);
+    p.dq = split_axis(p.bh * ((p.rows + 127) / 128), 2 * int64_t(cu), d.keys, 32, 128);
+    p.dkv = split_axis(p.bh * p.key_tiles, 2 * int64_t(cu), p.rows, 32, 128);
+    const int64_t a = p.dq.count > 1 ? align256(p.dq.count * p.bh * p.rows * p.pdim * 4) : 0;
+    const int64_t b = p.dkv.count > 1 ? align256(p.dkv.count * p.bh * d.keys * p.pdim * 4) : 0;
+    p.part = at;  // dQ's partials are summed before dK's and dV's are written
+    p.part2 = at + b;
+    at += std::max(a, 2 * b);
   }
-  for (int e = 0; e < 2; ++e)
-    if (lane + 64 * e < a.dim) static_cast<T*>(a.dq)[row * a.dim + lane + 64 * e] = T(acc[e]);
+  p.bytes = at;
+  return p;
 }
 
-// One wave per state: dK and dV, over the heads that read it and their queries.
+// A strided tensor [batch, length, heads, dim] as contiguous rows of pdim elements, zeros past dim.
 template <class T>
-__global__ __launch_bounds__(64) void attn_dkv_kernel(AttnArgs a) {
-  const int lane = int(threadIdx.x);
-  const int64_t row = blockIdx.x;  // (b, key, kv head)
-  const int hk = int(row % a.kv_heads), j = int(row / a.kv_heads % a.keys), b = int(row / a.kv_heads / a.keys);
-  const T* const k = static_cast<const T*>(a.k) + b * a.ks[0] + j * a.ks[1] + hk * a.ks[2];
-  const T* const v = static_cast<const T*>(a.v) + b * a.vs[0] + j * a.vs[1] + hk * a.vs[2];
-  const bool counts = j < key_limit(a, b) && (!a.mask || a.mask[b * a.ms + j]);
-  float dk[2] = {0.0f, 0.0f}, dv[2] = {0.0f, 0.0f};
-  if (counts) {
-    for (int h = hk * a.share; h < (hk + 1) * a.share; ++h) {
-      for (int i = 0; i < a.queries; ++i) {
-        const T* const q = static_cast<const T*>(a.q) + b * a.qs[0] + i * a.qs[1] + h * a.qs[2];
-        const T* const g = static_cast<const T*>(a.g) + b * a.gs[0] + i * a.gs[1] + h * a.gs[2];
-        const T* const o = static_cast<const T*>(a.o) + ((int64_t(b) * a.queries + i) * a.heads + h) * a.dim;
-        float s = 0.0f, dp = 0.0f, qd[2], gd[2];
-        for (int e = 0; e < 2; ++e) {
-          const int d = lane + 64 * e;
-          const bool in = d < a.dim;
-          qd[e] = in ? to_f32(q[d]) * a.scale : 0.0f;
-          gd[e] = in ? to_f32(g[d]) : 0.0f;
-          s += in ? qd[e] * to_f32(k[d]) : 0.0f;
-          dp += in ? gd[e] * (to_f32(v[d]) - to_f32(o[d])) : 0.0f;
-        }
-        const float p = expf(wave_sum(s) - a.lse[(int64_t(b) * a.heads + h) * a.queries + i]);
-        const float ds = p * wave_sum(dp);
-        for (int e = 0; e < 2; ++e) {
-          dk[e] += ds * qd[e];
-          dv[e] += p * gd[e];
-        }
-      }
-    }
-  }
-  for (int e = 0; e < 2; ++e) {
-    const int d = lane + 64 * e;
-    if (d < a.dim) {
-      static_cast<T*>(a.dk)[row * a.dim + d] = T(dk[e]);
-      static_cast<T*>(a.dv)[row * a.dim + d] = T(dv[e]);
-    }
+__global__ __launch_bounds__(256) void attn_pack_kernel(const T* x, T* y, int64_t total, int length, int heads, int dim,
+                                                        int pdim, int64_t s0, int64_t s1, int64_t s2) {
+  for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < total; i += int64_t(gridDim.x) * 256) {
+    const int64_t row = i / pdim, d = i - row * pdim;
+    const int64_t rest = row / heads, h = row - rest * heads, b = rest / length, l = rest - b * length;
+    y[i] = d < dim ? x[b * s0 + l * s1 + h * s2 + d] : T(0.0f);
   }
 }
 
-AttnArgs attn_args(const rdv_attention_desc& d, const void* q, const void* k, const void* v, const int32_t* lengths,
-                   const uint8_t* mask) {
+// Joins the forward splits of one row per wave: weights 2^(top_i - top).
+template <class T>
+__global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
+  const int lane = int(threadIdx.x) & 63;
+  const int64_t n = int64_t(a.batch) * a.kv_heads * a.rows, row = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
+  if (row >= n) return;
+  float top = -INFINITY;
+  for (int s = 0; s < a.splits; ++s) top = fmaxf(top, a.part_ml[s * n + row].x);
+  const float ref = top == -INFINITY ? 0.0f : top;
+  float total = 0.0f, o0 = 0.0f, o1 = 0.0f;
+  for (int s = 0; s < a.splits; ++s) {
+    const float2 m = a.part_ml[s * n + row];
+    if (m.y == 0.0f) continue;  // no state of this split counts: its partial row is not written
+    const float w = __builtin_amdgcn_exp2f(m.x - ref);
+    total += m.y * w;
+    const float* const p = a.part + (s * n + row) * a.pdim;
+    if (lane < a.pdim) o0 += w * p[lane];
+    if (lane + 64 < a.pdim) o1 += w * p[lane + 64];
+  }
+  const float inv = total > 0.0f ? 1.0f / total : (total == 0.0f ? 0.0f : total);
+  const int bh = int(row / a.rows), r = int(row - int64_t(bh) * a.rows), item = bh / a.kv_heads;
+  const RowAt at = row_at(a, bh - item * a.kv_heads, r);
+  T* const out = static_cast<T*>(a.out) + ((int64_t(item) * a.queries + at.query) * a.heads + at.head) * a.odim;
+  if (lane < a.odim) out[lane] = T(o0 * inv);
+  if (lane + 64 < a.odim) out[lane + 64] = T(o1 * inv);
+  if (a.lse && lane == 0) a.lse[row] = total == 0.0f ? -INFINITY : (top + __builtin_amdgcn_logf(total)) * kLn2;
+}
+
+// stats[row] = (lse log2 e, or +inf where no state counts; delta = rowsum(dO O)), 8 lanes per row.
+template <class T>
+__global__ __launch_bounds__(256) void attn_delta_kernel(AttnArgs a) {
+  const int64_t n = int64_t(a.batch) * a.kv_heads * a.rows, row = int64_t(blockIdx.x) * 32 + (threadIdx.x >> 3);
+  if (row >= n) return;
+  const int l = int(threadIdx.x) & 7;
+  const int bh = int(row / a.rows), r = int(row - int64_t(bh) * a.rows), item = bh / a.kv_heads;
+  const RowAt at = row_at(a, bh - item * a.kv_heads, r);
+  const T* const g = static_cast<const T*>(a.g) + item * a.gs[0] + at.query * a.gs[1] + at.head * a.gs[2];
+  const T* const o = static_cast<const T*>(a.o) + ((int64_t(item) * a.queries + at.query) * a.heads + at.head) * a.odim;
+  float sum = 0.0f;
+  for (int d = l; d < a.odim; d += 8) sum += to_f32(g[d]) * to_f32(o[d]);
+  for (int x = 4; x > 0; x >>= 1) sum += __shfl_xor(sum, x);
+  const float lse = a.lse[row];
+  if (l == 0) a.stats[row] = float2{lse == -INFINITY ? INFINITY : lse * kLog2e, sum};
+}
+
+// The sum of the splits of dQ (KEYS false: rows of the queries) or of dK and dV (KEYS true: z picks the tensor).
+template <class T, bool KEYS>
+__global__ __launch_bounds__(256) void attn_sum_kernel(AttnArgs a) {
+  const int64_t len = KEYS ? a.keys : a.rows, n = int64_t(a.batch) * a.kv_heads * len * a.pdim;
+  const int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x;
+  if (i >= n) return;
+  const float* const part = KEYS && blockIdx.y ? a.part2 : a.part;
+  float sum = 0.0f;
+  for (int s = 0; s < a.splits; ++s) sum += part[s * n + i];
+  const int64_t row = i / a.pdim, d = i - row * a.pdim;
+  if (d >= a.odim) return;
+  const int bh = int(row / len), x = int(row - int64_t(bh) * len), item = bh / a.kv_heads, hk = bh - item * a.kv_heads;
+  if constexpr (KEYS) {
+    static_cast<T*>(blockIdx.y ? a.dv : a.dk)[((int64_t(item) * a.keys + x) * a.kv_heads + hk) * a.odim + d] = T(sum);
+  } else {
+    const RowAt at = row_at(a, hk, x);
+    static_cast<T*>(a.dq)[((int64_t(item) * a.queries + at.query) * a.heads + at.head) * a.odim + d] = T(sum);
+  }
+}
+
+__global__ __launch_bounds__(256) void attn_zero_kernel(uint16_t* p, int64_t n) {
+  for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < n; i += int64_t(gridDim.x) * 256) p[i] = 0;
+}
+
+int zero(void* p, int64_t bytes, hipStream_t stream) {
+  if (bytes == 0) return RDV_OK;
+  attn_zero_kernel<<<dim3(unsigned(std::min<int64_t>((bytes / 2 + 255) / 256, 4096))), 256, 0, stream>>>(
+      static_cast<uint16_t*>(p), bytes / 2);
+  RDV_HIP_TRY(hipGetLastError());
+  return RDV_OK;
+}
+
+AttnArgs make_args(const rdv_attention_desc& d, const Plan& p, const int32_t* lengths, const uint8_t* mask) {
   AttnArgs a{};
-  a.q = q;
-  a.k = k;
-  a.v = v;
   a.lengths = lengths;
   a.mask = mask;
-  for (int i = 0; i < 3; ++i) {
-    a.qs[i] = d.q_stride[i];
-    a.ks[i] = d.k_stride[i];
-    a.vs[i] = d.v_stride[i];
-    a.gs[i] = d.g_stride[i];
-  }
   a.ms = d.mask_stride;
   a.batch = d.batch;
   a.queries = d.queries;
@@ -163,24 +186,85 @@ AttnArgs attn_args(const rdv_attention_desc& d, const void* q, const void* k, co
   a.heads = d.heads;
   a.kv_heads = d.kv_heads;
   a.share = d.heads / d.kv_heads;
-  a.dim = d.dim;
+  a.rows = p.rows;
+  a.dim = p.dim;
+  a.odim = d.dim;
+  a.pdim = p.pdim;
   a.scale = d.scale;
   return a;
 }
 
+// The tensor itself, or its aligned copy in the workspace.
+int input(const rdv_attention_desc& d, const Plan& p, int which, const void* x, const int64_t (&s)[3], int length,
+          int heads, uint8_t* ws, const void** out, int64_t (&os)[3], hipStream_t stream) {
+  if (length == 0 || in_place(d, s, length, heads)) {
+    if (length > 0 && reinterpret_cast<uintptr_t>(x) % 16 != 0)
+      return fail(RDV_ERR_INVALID, "attention: a tensor of aligned strides must be 16-byte aligned itself");
+    *out = x;
+    for (int i = 0; i < 3; ++i) os[i] = s[i];
+    return RDV_OK;
+  }
+  void* const y = ws + p.packs[which];
+  const int64_t total = int64_t(d.batch) * length * heads * p.dim;
+  const unsigned blocks = unsigned(std::min<int64_t>((total + 255) / 256, 65536));
+  *out = y;
+  os[0] = int64_t(length) * heads * p.dim;
+  os[1] = int64_t(heads) * p.dim;
+  os[2] = p.dim;
+  return with_dtype(d.dtype, [&](auto t) {
+    using T = decltype(t);
+    attn_pack_kernel<T><<<dim3(blocks), 256, 0, stream>>>(static_cast<const T*>(x), static_cast<T*>(y), total, length,
+                                                          heads, d.dim, p.dim, s[0], s[1], s[2]);
+    RDV_HIP_TRY(hipGetLastError());
+    return int(RDV_OK);
+  });
+}
+
+int launch_matrix(int dtype, AttnKernel which, const AttnArgs& a, hipStream_t stream) {
+  const int64_t blocks = int64_t(a.batch) * a.kv_heads * a.splits * a.tiles;
+  if (blocks >= (int64_t(1) << 31)) return fail(RDV_ERR_UNSUPPORTED, "attention: too many blocks");
+  if (dtype == RDV_DTYPE_F16) return launch_attn_f16(which, a, unsigned(blocks), stream);
+  if (dtype == RDV_DTYPE_BF16) return launch_attn_bf16(which, a, unsigned(blocks), stream);
+  return launch_attn_f32(which, a, unsigned(blocks), stream);
+}
+
+int check_plan(const rdv_attention_desc& d) {
+  const int64_t rows = int64_t(d.heads / d.kv_heads) * d.queries;
+  if (rows >= (int64_t(1) << 31) - 256 || int64_t(d.batch) * d.kv_heads * std::max<int64_t>(rows, d.keys) >= (int64_t(1) << 33))
+    return fail(RDV_ERR_UNSUPPORTED, "attention: too many rows");
+  return RDV_OK;
+}
+
 }  // namespace
 
-int64_t attention_workspace_bytes(const rdv_attention_desc&, bool, int) { return 0; }
+int64_t attention_workspace_bytes(const rdv_attention_desc& d, bool backward, int cu) {
+  const int rc = check_plan(d);
+  return rc != RDV_OK ? rc : make_plan(d, backward, cu).bytes;
+}
 
 int launch_attention(const rdv_attention_desc& d, const void* q, const void* k, const void* v,
-                     const int32_t* lengths, const uint8_t* mask, void* out, float* lse, void*, hipStream_t stream) {
-  AttnArgs a = attn_args(d, q, k, v, lengths, mask);
+                     const int32_t* lengths, const uint8_t* mask, void* out, float* lse, void* workspace, int cu,
+                     hipStream_t stream) {
+  const Plan p = make_plan(d, false, cu);
+  uint8_t* const ws = static_cast<uint8_t*>(workspace);
+  AttnArgs a = make_args(d, p, lengths, mask);
+  int rc = input(d, p, 0, q, d.q_stride, d.queries, d.heads, ws, &a.q, a.qs, stream);
+  if (rc == RDV_OK) rc = input(d, p, 1, k, d.k_stride, d.keys, d.kv_heads, ws, &a.k, a.ks, stream);
+  if (rc == RDV_OK) rc = input(d, p, 2, v, d.v_stride, d.keys, d.kv_heads, ws, &a.v, a.vs, stream);
+  if (rc != RDV_OK) return rc;
   a.out = out;
   a.lse = lse;
-  const int64_t rows = int64_t(d.batch) * d.queries * d.heads;
-  if (rows >= (int64_t(1) << 31)) return fail(RDV_ERR_UNSUPPORTED, "attention: too many rows");
+  a.tiles = p.row_tiles;
+  a.splits = p.forward.count;
+  a.chunk = p.forward.chunk;
+  a.part = reinterpret_cast<float*>(ws + p.part);
+  a.part_ml = reinterpret_cast<float2*>(ws + p.ml);
+  rc = launch_matrix(d.dtype, p.few ? kAttnFew : kAttnTile, a, stream);
+  if (rc != RDV_OK || a.splits == 1) return rc;
+  const int64_t blocks = (p.bh * p.rows + 3) / 4;
+  if (blocks >= (int64_t(1) << 31)) return fail(RDV_ERR_UNSUPPORTED, "attention: too many rows");
   return with_dtype(d.dtype, [&](auto t) {
-    attn_forward_kernel<decltype(t)><<<dim3(unsigned(rows)), 64, 0, stream>>>(a);
+    attn_join_kernel<decltype(t)><<<dim3(unsigned(blocks)), 256, 0, stream>>>(a);
     RDV_HIP_TRY(hipGetLastError());
     return int(RDV_OK);
   });
@@ -188,21 +272,61 @@ int launch_attention(const rdv_attention_desc& d, const void* q, const void* k, 
 
 int launch_attention_backward(const rdv_attention_desc& d, const void* grad, const void* q, const void* k,
                               const void* v, const void* out, const float* lse, const int32_t* lengths,
-                              const uint8_t* mask, void* dq, void* dk, void* dv, void*, hipStream_t stream) {
-  AttnArgs a = attn_args(d, q, k, v, lengths, mask);
-  a.g = grad;
+                              const uint8_t* mask, void* dq, void* dk, void* dv, void* workspace, int cu,
+                              hipStream_t stream) {
+  const int64_t q_bytes = int64_t(d.batch) * d.queries * d.heads * d.dim * element_bytes(d.dtype);
+  const int64_t k_bytes = int64_t(d.batch) * d.keys * d.kv_heads * d.dim * element_bytes(d.dtype);
+  if (d.queries == 0 || d.keys == 0) {
+    int rc = zero(dq, q_bytes, stream);
+    if (rc == RDV_OK) rc = zero(dk, k_bytes, stream);
+    return rc == RDV_OK ? zero(dv, k_bytes, stream) : rc;
+  }
+  const Plan p = make_plan(d, true, cu);
+  uint8_t* const ws = static_cast<uint8_t*>(workspace);
+  AttnArgs a = make_args(d, p, lengths, mask);
+  int rc = input(d, p, 0, q, d.q_stride, d.queries, d.heads, ws, &a.q, a.qs, stream);
+  if (rc == RDV_OK) rc = input(d, p, 1, k, d.k_stride, d.keys, d.kv_heads, ws, &a.k, a.ks, stream);
+  if (rc == RDV_OK) rc = input(d, p, 2, v, d.v_stride, d.keys, d.kv_heads, ws, &a.v, a.vs, stream);
+  if (rc == RDV_OK) rc = input(d, p, 3, grad, d.g_stride, d.queries, d.heads, ws, &a.g, a.gs, stream);
+  if (rc != RDV_OK) return rc;
   a.o = out;
   a.lse = const_cast<float*>(lse);
+  a.stats = reinterpret_cast<float2*>(ws + p.stats);
   a.dq = dq;
   a.dk = dk;
   a.dv = dv;
-  const int64_t rows = int64_t(d.batch) * d.queries * d.heads, states = int64_t(d.batch) * d.keys * d.kv_heads;
-  if (rows >= (int64_t(1) << 31) || states >= (int64_t(1) << 31))
+  const int64_t n = p.bh * p.rows;
+  const int64_t sums = (std::max(n, p.bh * int64_t(d.keys)) * p.pdim + 255) / 256;
+  if ((n + 31) / 32 >= (int64_t(1) << 31) || sums >= (int64_t(1) << 31))
     return fail(RDV_ERR_UNSUPPORTED, "attention: too many rows");
+  rc = with_dtype(d.dtype, [&](auto t) {
+    attn_delta_kernel<decltype(t)><<<dim3(unsigned((n + 31) / 32)), 256, 0, stream>>>(a);
+    RDV_HIP_TRY(hipGetLastError());
+    return int(RDV_OK);
+  });
+  if (rc != RDV_OK) return rc;
+  a.tiles = (p.rows + 127) / 128;
+  a.splits = p.dq.count;
+  a.chunk = p.dq.chunk;
+  a.part = reinterpret_cast<float*>(ws + p.part);
+  rc = launch_matrix(d.dtype, kAttnDq, a, stream);
+  if (rc != RDV_OK) return rc;
+  if (a.splits > 1) {
+    rc = with_dtype(d.dtype, [&](auto t) {
+      attn_sum_kernel<decltype(t), false><<<dim3(unsigned((n * p.pdim + 255) / 256)), 256, 0, stream>>>(a);
+      RDV_HIP_TRY(hipGetLastError());
+      return int(RDV_OK);
+    });
+    if (rc != RDV_OK) return rc;
+  }
+  a.tiles = p.key_tiles;
+  a.splits = p.dkv.count;
+  a.chunk = p.dkv.chunk;
+  a.part2 = reinterpret_cast<float*>(ws + p.part2);
+  rc = launch_matrix(d.dtype, kAttnDkv, a, stream);
+  if (rc != RDV_OK || a.splits == 1) return rc;
   return with_dtype(d.dtype, [&](auto t) {
-    using T = decltype(t);
-    if (rows > 0) attn_dq_kernel<T><<<dim3(unsigned(rows)), 64, 0, stream>>>(a);
-    if (states > 0) attn_dkv_kernel<T><<<dim3(unsigned(states)), 64, 0, stream>>>(a);
+    attn_sum_kernel<decltype(t), true><<<dim3(unsigned((p.bh * d.keys * p.pdim + 255) / 256), 2), 256, 0, stream>>>(a);
     RDV_HIP_TRY(hipGetLastError());
     return int(RDV_OK);
   });

@@ -131,11 +131,12 @@ int launch_group_norm_backward(const rdv_group_norm_desc& d, const void* grad, c
                                void* ws, hipStream_t stream);
 int64_t attention_workspace_bytes(const rdv_attention_desc& d, bool backward, int cu);
 int launch_attention(const rdv_attention_desc& d, const void* q, const void* k, const void* v,
-                     const int32_t* key_lengths, const uint8_t* key_mask, void* out, float* lse, void* ws,
+                     const int32_t* key_lengths, const uint8_t* key_mask, void* out, float* lse, void* ws, int cu,
                      hipStream_t stream);
 int launch_attention_backward(const rdv_attention_desc& d, const void* grad, const void* q, const void* k,
                               const void* v, const void* out, const float* lse, const int32_t* key_lengths,
-                              const uint8_t* key_mask, void* dq, void* dk, void* dv, void* ws, hipStream_t stream);
+                              const uint8_t* key_mask, void* dq, void* dk, void* dv, void* ws, int cu,
+                              hipStream_t stream);
 int launch_dropout(const void* x, const void* residual, void* y, int64_t n, int dtype, double p, uint64_t seed,
                    uint64_t subsequence, hipStream_t stream);
 
@@ -787,6 +788,7 @@ int rdv_group_norm(const rdv_group_norm_desc* desc, const void* x, const float* 
   if (rc != RDV_OK) return rc;
   if (desc->images == 0 || desc->rows == 0) return RDV_OK;
   if (!x || !y) return fail(RDV_ERR_INVALID, "rdv_group_norm: NULL pointer argument");
+  if (!aligned16(y)) return fail(RDV_ERR_INVALID, "rdv_group_norm: y must be 16-byte aligned");
   const int64_t need = group_norm_workspace_bytes(*desc, false, plan_cu_count());
   if (need > 0 && (!workspace || workspace_bytes < need || !aligned16(workspace)))
     return fail(RDV_ERR_WORKSPACE, "rdv_group_norm: workspace too small or not 16-byte aligned");
@@ -800,6 +802,7 @@ int rdv_group_norm_backward(const rdv_group_norm_desc* desc, const void* grad, c
   if (rc != RDV_OK) return rc;
   if (desc->images > 0 && desc->rows > 0) {
     if (!grad || !x || !stats || !dx) return fail(RDV_ERR_INVALID, "rdv_group_norm_backward: NULL pointer argument");
+    if (!aligned16(dx)) return fail(RDV_ERR_INVALID, "rdv_group_norm_backward: dx must be 16-byte aligned");
     const int64_t need = group_norm_workspace_bytes(*desc, true, plan_cu_count());
     if (need > 0 && (!workspace || workspace_bytes < need || !aligned16(workspace)))
       return fail(RDV_ERR_WORKSPACE, "rdv_group_norm_backward: workspace too small or not 16-byte aligned");
@@ -845,10 +848,13 @@ int rdv_cross_attention(const rdv_attention_desc* desc, const void* q, const voi
   if (desc->batch == 0 || desc->queries == 0) return RDV_OK;
   if (!q || !out || (desc->keys > 0 && (!k || !v)))
     return fail(RDV_ERR_INVALID, "rdv_cross_attention: NULL pointer argument");
-  const int64_t need = attention_workspace_bytes(*desc, false, plan_cu_count());
+  if (!aligned16(out)) return fail(RDV_ERR_INVALID, "rdv_cross_attention: out must be 16-byte aligned");
+  const int cu = plan_cu_count();
+  const int64_t need = attention_workspace_bytes(*desc, false, cu);
+  if (need < 0) return int(need);
   if (need > 0 && (!workspace || workspace_bytes < need || !aligned16(workspace)))
     return fail(RDV_ERR_WORKSPACE, "rdv_cross_attention: workspace too small or not 16-byte aligned");
-  return launch_attention(*desc, q, k, v, key_lengths, key_mask, out, lse, workspace,
+  return launch_attention(*desc, q, k, v, key_lengths, key_mask, out, lse, workspace, cu,
                           static_cast<hipStream_t>(stream));
 }
 
@@ -861,11 +867,15 @@ int rdv_cross_attention_backward(const rdv_attention_desc* desc, const void* gra
   if (desc->batch == 0) return RDV_OK;
   if ((desc->queries > 0 && (!grad || !q || !out || !lse || !dq)) || (desc->keys > 0 && (!k || !v || !dk || !dv)))
     return fail(RDV_ERR_INVALID, "rdv_cross_attention_backward: NULL pointer argument");
-  const int64_t need = attention_workspace_bytes(*desc, true, plan_cu_count());
+  if (!aligned16(dq) || !aligned16(dk) || !aligned16(dv))
+    return fail(RDV_ERR_INVALID, "rdv_cross_attention_backward: dq, dk and dv must be 16-byte aligned");
+  const int cu = plan_cu_count();
+  const int64_t need = attention_workspace_bytes(*desc, true, cu);
+  if (need < 0) return int(need);
   if (need > 0 && (!workspace || workspace_bytes < need || !aligned16(workspace)))
     return fail(RDV_ERR_WORKSPACE, "rdv_cross_attention_backward: workspace too small or not 16-byte aligned");
   return launch_attention_backward(*desc, grad, q, k, v, out, lse, key_lengths, key_mask, dq, dk, dv, workspace,
-                                   static_cast<hipStream_t>(stream));
+                                   cu, static_cast<hipStream_t>(stream));
 }
 
 int rdv_dropout(const void* x, const void* residual, void* y, int64_t n, int32_t dtype, double p, uint64_t seed,
