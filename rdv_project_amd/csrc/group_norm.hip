@@ -5,6 +5,22 @@
 //   y = act(z);  dz = dy act'(z);  per (image, channel) A = sum dz, B = sum dz xhat;
 //   dbias = sum over images of A, dweight = sum over images of B;
 //   dx = rstd (w dz - (sum_c w A) / m - xhat (sum_c w B) / m).
+//
+// Geometry.  A block takes a slab of whole groups (channels) and a run of an image's rows.  Thread (tr, col) reads the
+// 16-byte (or narrower, by the alignment) piece `col` of the slab in rows tr, tr + TR, ...: its channels stay the same,
+// so per-channel constants and sums are registers, whatever the group width; sums join over tr in an LDS tree and
+// over a group's channels in 16 lanes.  Bound: HBM; each kernel reads what it needs once, in whole lines.
+//   * An image's slab that fits the registers of a block is normalised by one launch that reads x once
+//     (norm_whole_kernel, norm_whole_back_kernel).
+//   * Larger images take two launches over the same grid: the first leaves each block's statistics, the second joins
+//     them (every block the same way, in one order) and reads its rows again, from the L2 that the first filled where
+//     the tensor fits.
+//   * A group wider than a slab can be takes one block per (image, group or channel) (norm_wide_*).
+// Variance.  Squares are taken of deviations from a mean of the thread's own values, and blocks' (mean, sum of squared
+// deviations) are joined with their means' distances: no difference of large sums.
+#include <algorithm>
+#include <numeric>
+
 #include "operators.h"
 
 namespace rdv {
@@ -16,13 +32,43 @@ struct NormArgs {
   const void* grad;
   const float* weight;
   const float* bias;
-  void* y;
-  float* stats;  // [images, groups, 2]
-  float* sums;   // [images, channels, 2]
+  void* y;               // or dx
+  float* stats;          // [images, groups, 2]: mean, rstd (forward: may be NULL)
+  float2* parts;         // forward: [images, groups, chunks] (mean, squared deviations); backward: [images, chunks, channels] (A, B)
+  float *dweight, *dbias;
   int64_t images, rows, x_image, x_row, g_image, g_row;
   int channels, groups, width, act;
   float eps;
+  int slab, slabs, pieces, tr;   // channels of a slab, slabs, pieces of a slab's row, rows side by side in a block
+  int chunks, chunk_rows;        // blocks of an image's slab, rows of one
 };
+
+template <class T, int VE>
+struct Piece {
+  typedef T vec __attribute__((ext_vector_type(VE)));
+  vec v;
+  __device__ __forceinline__ float operator[](int i) const { return to_f32(T(v[i])); }
+};
+template <class T>
+struct Piece<T, 1> {
+  T v;
+  __device__ __forceinline__ float operator[](int) const { return to_f32(v); }
+};
+template <class T, int VE>
+__device__ __forceinline__ Piece<T, VE> load_piece(const T* p) {
+  return *reinterpret_cast<const Piece<T, VE>*>(p);
+}
+template <class T, int VE>
+__device__ __forceinline__ void store_piece(T* p, const float (&y)[VE]) {
+  Piece<T, VE> out;
+  if constexpr (VE == 1) {
+    out.v = T(y[0]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < VE; ++i) out.v[i] = T(y[i]);
+  }
+  *reinterpret_cast<Piece<T, VE>*>(p) = out;
+}
 
 __device__ __forceinline__ float silu_slope(float z) {
   const float s = fast_sigmoid(z);
@@ -37,7 +83,527 @@ __device__ __forceinline__ float norm_act_slope(int act, float z) {
   return act == RDV_ACT_SILU ? silu_slope(z) : 1.0f;
 }
 
-// Sum over the block's 256 threads, the same in every thread.
+// Where a block and a thread are.
+struct NormAt {
+  int64_t image;
+  int tr, col, c0, channels, groups;  // the slab's first channel, its channels and groups (the last slab may be shorter)
+  int channel;                        // the thread's first channel, within the slab
+  bool on;                            // the thread has a piece
+};
+template <int VE>
+__device__ __forceinline__ NormAt norm_at(const NormArgs& a, int64_t image, int slab) {
+  NormAt p;
+  p.image = image;
+  p.tr = int(threadIdx.x) / a.pieces;
+  p.col = int(threadIdx.x) - p.tr * a.pieces;
+  p.c0 = slab * a.slab;
+  p.channels = min(a.slab, a.channels - p.c0);
+  p.groups = p.channels / a.width;
+  p.channel = p.col * VE;
+  p.on = p.tr < a.tr && p.channel < p.channels;
+  return p;
+}
+
+// Sums v over the block's tr, per channel of the slab, into red[channel]; every thread takes part, threads without a
+// piece with any value.  red: blockDim.x * VE floats.
+template <int VE>
+__device__ __forceinline__ void sum_rows(const NormArgs& a, const NormAt& p, const float (&v)[VE], float* red) {
+  float* const mine = red + threadIdx.x * VE;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < VE; ++i) mine[i] = v[i];
+  for (int n = a.tr; n > 1;) {
+    const int half = (n + 1) >> 1;
+    __syncthreads();
+    if (p.tr < n - half) {
+#pragma unroll
+      for (int i = 0; i < VE; ++i) mine[i] += mine[half * a.pieces * VE + i];
+    }
+    n = half;
+  }
+  __syncthreads();
+}
+
+// out[g] = f(sum of per[channel] over the channels of the slab's group g), 16 lanes per group.
+template <class P, class F>
+__device__ __forceinline__ void sum_groups(const NormArgs& a, const NormAt& p, float* out, P per, F f) {
+  const int l = int(threadIdx.x) & 15, lanes = int(blockDim.x) >> 4;
+  for (int g = int(threadIdx.x) >> 4; g < p.groups; g += lanes) {
+    float s = 0.0f;
+    for (int c = l; c < a.width; c += 16) s += per(g * a.width + c);
+    for (int o = 8; o > 0; o >>= 1) s += __shfl_xor(s, o);
+    if (l == 0) out[g] = f(s);
+  }
+  __syncthreads();
+}
+
+template <int VE>
+__device__ __forceinline__ void load_affine(const NormArgs& a, const NormAt& p, float (&w)[VE], float (&b)[VE]) {
+#pragma unroll
+  for (int i = 0; i < VE; ++i) {
+    w[i] = p.on && a.weight ? a.weight[p.c0 + p.channel + i] : 1.0f;
+    b[i] = p.on && a.bias ? a.bias[p.c0 + p.channel + i] : 0.0f;
+  }
+}
+
+template <class T, int VE>
+__device__ __forceinline__ void normalise(const NormArgs& a, const Piece<T, VE>& x, const float (&mean)[VE],
+                                          const float (&scale)[VE], const float (&b)[VE], T* y) {
+  float z[VE];
+#pragma unroll
+  for (int i = 0; i < VE; ++i) z[i] = fmaf(x[i] - mean[i], scale[i], b[i]);
+  if (a.act == RDV_ACT_SILU) {
+#pragma unroll
+    for (int i = 0; i < VE; ++i) z[i] *= fast_sigmoid(z[i]);
+  } else if (a.act == RDV_ACT_RELU) {
+#pragma unroll
+    for (int i = 0; i < VE; ++i) z[i] = fmaxf(z[i], 0.0f);
+  }
+  store_piece<T, VE>(y, z);
+}
+
+// dz and xhat of a piece.
+template <class T, int VE>
+__device__ __forceinline__ void slopes(const NormArgs& a, const Piece<T, VE>& x, const Piece<T, VE>& g,
+                                       const float (&mean)[VE], const float (&rstd)[VE], const float (&w)[VE],
+                                       const float (&b)[VE], float (&xhat)[VE], float (&dz)[VE]) {
+#pragma unroll
+  for (int i = 0; i < VE; ++i) {
+    xhat[i] = (x[i] - mean[i]) * rstd[i];
+    dz[i] = g[i];
+  }
+  if (a.act == RDV_ACT_SILU) {
+#pragma unroll
+    for (int i = 0; i < VE; ++i) dz[i] *= silu_slope(fmaf(xhat[i], w[i], b[i]));
+  } else if (a.act == RDV_ACT_RELU) {
+#pragma unroll
+    for (int i = 0; i < VE; ++i) dz[i] = fmaf(xhat[i], w[i], b[i]) > 0.0f ? dz[i] : 0.0f;
+  }
+}
+
+// Runs f(row, piece...) over rows first .. end - 1 of the thread, U at a time with their loads first.
+constexpr int kNormUnroll = 4;
+
+// ------------------------------------------------------------------ one launch
+
+// An image's slab in the registers of a block, at most R pieces per thread.
+template <class T, int VE, int R>
+__global__ __launch_bounds__(1024) void norm_whole_kernel(NormArgs a) {
+  extern __shared__ float norm_lds[];
+  const NormAt p = norm_at<VE>(a, blockIdx.x / a.slabs, int(blockIdx.x % a.slabs));
+  float* const red = norm_lds;
+  float* const mean_g = red + blockDim.x * VE;
+  float* const rstd_g = mean_g + a.slab / a.width;
+  const T* const x = static_cast<const T*>(a.x) + p.image * a.x_image + p.c0 + p.channel;
+  Piece<T, VE> v[R];
+  float s[VE] = {};
+#pragma unroll
+  for (int k = 0; k < R; ++k) {
+    const int64_t r = p.tr + int64_t(k) * a.tr;
+    if (p.on && r < a.rows) v[k] = load_piece<T, VE>(x + r * a.x_row);
+  }
+#pragma unroll
+  for (int k = 0; k < R; ++k)
+    if (p.on && p.tr + int64_t(k) * a.tr < a.rows) {
+#pragma unroll
+      for (int i = 0; i < VE; ++i) s[i] += v[k][i];
+    }
+  const float inv = 1.0f / (float(a.rows) * float(a.width));
+  sum_rows<VE>(a, p, s, red);
+  sum_groups(a, p, mean_g, [&](int c) { return red[c]; }, [&](float t) { return t * inv; });
+  float mean[VE], scale[VE], w[VE], b[VE];
+  load_affine<VE>(a, p, w, b);
+#pragma unroll
+  for (int i = 0; i < VE; ++i) {
+    mean[i] = p.on ? mean_g[(p.channel + i) / a.width] : 0.0f;
+    s[i] = 0.0f;
+  }
+#pragma unroll
+  for (int k = 0; k < R; ++k)
+    if (p.on && p.tr + int64_t(k) * a.tr < a.rows) {
+#pragma unroll
+      for (int i = 0; i < VE; ++i) s[i] = fmaf(v[k][i] - mean[i], v[k][i] - mean[i], s[i]);
+    }
+  sum_rows<VE>(a, p, s, red);
+  sum_groups(a, p, rstd_g, [&](int c) { return red[c]; }, [&](float t) { return 1.0f / sqrtf(t * inv + a.eps); });
+#pragma unroll
+  for (int i = 0; i < VE; ++i) scale[i] = p.on ? w[i] * rstd_g[(p.channel + i) / a.width] : 0.0f;
+  T* const y = static_cast<T*>(a.y) + p.image * a.rows * a.channels + p.c0 + p.channel;
+#pragma unroll
+  for (int k = 0; k < R; ++k) {
+    const int64_t r = p.tr + int64_t(k) * a.tr;
+    if (p.on && r < a.rows) normalise<T, VE>(a, v[k], mean, scale, b, y + r * a.channels);
+  }
+  if (a.stats) {
+    float* const st = a.stats + 2 * (p.image * a.groups + p.c0 / a.width);
+    for (int g = int(threadIdx.x); g < p.groups; g += int(blockDim.x)) {
+      st[2 * g] = mean_g[g];
+      st[2 * g + 1] = rstd_g[g];
+    }
+  }
+}
+
+// The thread's channels' constants from stats.
+template <int VE>
+__device__ __forceinline__ void load_stats(const NormArgs& a, const NormAt& p, float (&mean)[VE], float (&rstd)[VE]) {
+#pragma unroll
+  for (int i = 0; i < VE; ++i) {
+    const int64_t g = p.image * a.groups + (p.on ? (p.c0 + p.channel + i) / a.width : 0);
+    mean[i] = a.stats[2 * g];
+    rstd[i] = a.stats[2 * g + 1];
+  }
+}
+
+// From the slab's per-channel sums A (in `red`, then B): dx's two means per group, m1 and m2.
+template <int VE>
+__device__ __forceinline__ void join_sums(const NormArgs& a, const NormAt& p, const float (&sa)[VE], const float (&sb)[VE],
+                                          float* red, float* m1, float* m2, float2* channel_sums) {
+  const float inv = 1.0f / (float(a.rows) * float(a.width));
+  for (int which = 0; which < 2; ++which) {
+    sum_rows<VE>(a, p, which ? sb : sa, red);
+    if (channel_sums)
+      for (int c = int(threadIdx.x); c < p.channels; c += int(blockDim.x))
+        (which ? channel_sums[p.c0 + c].y : channel_sums[p.c0 + c].x) = red[c];
+    sum_groups(a, p, which ? m2 : m1,
+               [&](int c) { return red[c] * (a.weight ? a.weight[p.c0 + c] : 1.0f); },
+               [&](float t) { return t * inv; });
+  }
+}
+
+// The same for the gradients; per-channel sums go to `parts` as one chunk's.
+template <class T, int VE, int R>
+__global__ __launch_bounds__(1024) void norm_whole_back_kernel(NormArgs a) {
+  extern __shared__ float norm_lds[];
+  const NormAt p = norm_at<VE>(a, blockIdx.x / a.slabs, int(blockIdx.x % a.slabs));
+  float* const red = norm_lds;
+  float* const m1 = red + blockDim.x * VE;
+  float* const m2 = m1 + a.slab / a.width;
+  const T* const x = static_cast<const T*>(a.x) + p.image * a.x_image + p.c0 + p.channel;
+  const T* const g = static_cast<const T*>(a.grad) + p.image * a.g_image + p.c0 + p.channel;
+  Piece<T, VE> vx[R], vg[R];
+#pragma unroll
+  for (int k = 0; k < R; ++k) {
+    const int64_t r = p.tr + int64_t(k) * a.tr;
+    if (p.on && r < a.rows) {
+      vx[k] = load_piece<T, VE>(x + r * a.x_row);
+      vg[k] = load_piece<T, VE>(g + r * a.g_row);
+    }
+  }
+  float mean[VE], rstd[VE], w[VE], b[VE], sa[VE] = {}, sb[VE] = {}, xhat[VE], dz[VE];
+  load_affine<VE>(a, p, w, b);
+  load_stats<VE>(a, p, mean, rstd);
+#pragma unroll
+  for (int k = 0; k < R; ++k)
+    if (p.on && p.tr + int64_t(k) * a.tr < a.rows) {
+      slopes<T, VE>(a, vx[k], vg[k], mean, rstd, w, b, xhat, dz);
+#pragma unroll
+      for (int i = 0; i < VE; ++i) {
+        sa[i] += dz[i];
+        sb[i] = fmaf(dz[i], xhat[i], sb[i]);
+      }
+    }
+  join_sums<VE>(a, p, sa, sb, red, m1, m2, a.parts + p.image * a.channels);
+  if (!p.on) return;
+  T* const dx = static_cast<T*>(a.y) + p.image * a.rows * a.channels + p.c0 + p.channel;
+#pragma unroll
+  for (int k = 0; k < R; ++k) {
+    const int64_t r = p.tr + int64_t(k) * a.tr;
+    if (r < a.rows) {
+      slopes<T, VE>(a, vx[k], vg[k], mean, rstd, w, b, xhat, dz);
+#pragma unroll
+      for (int i = 0; i < VE; ++i) {
+        const int gi = (p.channel + i) / a.width;
+        dz[i] = rstd[i] * (w[i] * dz[i] - m1[gi] - xhat[i] * m2[gi]);
+      }
+      store_piece<T, VE>(dx + r * a.channels, dz);
+    }
+  }
+}
+
+// ------------------------------------------------------------------ two launches
+
+// Block (image, slab, chunk) of the two-launch kernels.
+struct NormChunk {
+  int64_t image, first, end;
+  int slab, chunk;
+};
+__device__ __forceinline__ NormChunk norm_chunk(const NormArgs& a, int64_t block) {
+  NormChunk c;
+  c.chunk = int(block % a.chunks);
+  const int64_t rest = block / a.chunks;
+  c.slab = int(rest % a.slabs);
+  c.image = rest / a.slabs;
+  c.first = int64_t(c.chunk) * a.chunk_rows;
+  c.end = min(c.first + a.chunk_rows, a.rows);
+  return c;
+}
+
+// First launch, forward: a chunk's mean and squared deviations per group.
+template <class T, int VE>
+__global__ __launch_bounds__(256) void norm_stats_kernel(NormArgs a) {
+  extern __shared__ float norm_lds[];
+  constexpr int U = kNormUnroll;
+  const NormChunk ch = norm_chunk(a, blockIdx.x);
+  const NormAt p = norm_at<VE>(a, ch.image, ch.slab);
+  float* const red = norm_lds;
+  float* const mean_g = red + blockDim.x * VE;
+  float* const dev_g = mean_g + a.slab / a.width;
+  const T* const x = static_cast<const T*>(a.x) + p.image * a.x_image + p.c0 + p.channel;
+  // deviations from the mean of the thread's first U values
+  float shift[VE] = {}, s1[VE] = {}, s2[VE] = {};
+  int n = 0;
+  if (p.on) {
+    for (int64_t r0 = ch.first + p.tr; r0 < ch.end; r0 += int64_t(U) * a.tr) {
+      Piece<T, VE> v[U];
+#pragma unroll
+      for (int k = 0; k < U; ++k) v[k] = load_piece<T, VE>(x + min(r0 + int64_t(k) * a.tr, a.rows - 1) * a.x_row);
+      int have = 0;
+#pragma unroll
+      for (int k = 0; k < U; ++k) have += r0 + int64_t(k) * a.tr < ch.end;
+      if (n == 0) {
+#pragma unroll
+        for (int i = 0; i < VE; ++i) {
+          for (int k = 0; k < U; ++k)
+            if (k < have) shift[i] += v[k][i];
+          shift[i] /= float(have);
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < U; ++k)
+        if (k < have) {
+#pragma unroll
+          for (int i = 0; i < VE; ++i) {
+            const float d = v[k][i] - shift[i];
+            s1[i] += d;
+            s2[i] = fmaf(d, d, s2[i]);
+          }
+        }
+      n += have;
+    }
+  }
+  const float fn = float(n), inv = n ? 1.0f / fn : 0.0f;
+  float q[VE], mean[VE];
+#pragma unroll
+  for (int i = 0; i < VE; ++i) {
+    mean[i] = fmaf(s1[i], inv, shift[i]);
+    q[i] = fn * mean[i];
+  }
+  const float count = float(ch.end - ch.first) * float(a.width);
+  sum_rows<VE>(a, p, q, red);
+  sum_groups(a, p, mean_g, [&](int c) { return red[c]; }, [&](float t) { return t / count; });
+#pragma unroll
+  for (int i = 0; i < VE; ++i) {
+    const float d = p.on ? mean[i] - mean_g[(p.channel + i) / a.width] : 0.0f;
+    q[i] = fmaxf(s2[i] - s1[i] * s1[i] * inv, 0.0f) + fn * d * d;
+  }
+  sum_rows<VE>(a, p, q, red);
+  sum_groups(a, p, dev_g, [&](int c) { return red[c]; }, [&](float t) { return t; });
+  float2* const part = a.parts + (p.image * a.groups + p.c0 / a.width) * a.chunks + ch.chunk;
+  for (int g = int(threadIdx.x); g < p.groups; g += int(blockDim.x))
+    part[int64_t(g) * a.chunks] = float2{mean_g[g], dev_g[g]};
+}
+
+// Second launch, forward: the chunks' statistics joined, 16 lanes per group, and the rows normalised.
+template <class T, int VE>
+__global__ __launch_bounds__(256) void norm_apply_kernel(NormArgs a) {
+  extern __shared__ float norm_lds[];
+  constexpr int U = kNormUnroll;
+  const NormChunk ch = norm_chunk(a, blockIdx.x);
+  const NormAt p = norm_at<VE>(a, ch.image, ch.slab);
+  float* const mean_g = norm_lds;
+  float* const rstd_g = mean_g + a.slab / a.width;
+  const T* const x = static_cast<const T*>(a.x) + p.image * a.x_image + p.c0 + p.channel;
+  float w[VE], b[VE], mean[VE], scale[VE];
+  load_affine<VE>(a, p, w, b);
+  {
+    const int l = int(threadIdx.x) & 15;
+    const float total = float(a.rows) * float(a.width);
+    for (int g = int(threadIdx.x) >> 4; g < p.groups; g += int(blockDim.x) >> 4) {
+      const float2* const part = a.parts + (p.image * a.groups + p.c0 / a.width + g) * a.chunks;
+      float s = 0.0f;
+      for (int i = l; i < a.chunks; i += 16) s += part[i].x * float(min(int64_t(a.chunk_rows), a.rows - int64_t(i) * a.chunk_rows));
+      for (int o = 8; o > 0; o >>= 1) s += __shfl_xor(s, o);
+      const float m = s / float(a.rows);
+      s = 0.0f;
+      for (int i = l; i < a.chunks; i += 16) {
+        const float2 t = part[i];
+        s += t.y + (t.x - m) * (t.x - m) * float(min(int64_t(a.chunk_rows), a.rows - int64_t(i) * a.chunk_rows)) * float(a.width);
+      }
+      for (int o = 8; o > 0; o >>= 1) s += __shfl_xor(s, o);
+      if (l == 0) {
+        mean_g[g] = m;
+        rstd_g[g] = 1.0f / sqrtf(s / total + a.eps);
+        if (a.stats && ch.chunk == 0) {
+          float* const st = a.stats + 2 * (p.image * a.groups + p.c0 / a.width + g);
+          st[0] = m;
+          st[1] = rstd_g[g];
+        }
+      }
+    }
+  }
+  __syncthreads();
+  if (!p.on) return;
+#pragma unroll
+  for (int i = 0; i < VE; ++i) {
+    const int g = (p.channel + i) / a.width;
+    mean[i] = mean_g[g];
+    scale[i] = w[i] * rstd_g[g];
+  }
+  T* const y = static_cast<T*>(a.y) + p.image * a.rows * a.channels + p.c0 + p.channel;
+  for (int64_t r0 = ch.first + p.tr; r0 < ch.end; r0 += int64_t(U) * a.tr) {
+    Piece<T, VE> v[U];
+#pragma unroll
+    for (int k = 0; k < U; ++k) v[k] = load_piece<T, VE>(x + min(r0 + int64_t(k) * a.tr, a.rows - 1) * a.x_row);
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      const int64_t r = r0 + int64_t(k) * a.tr;
+      if (r < ch.end) normalise<T, VE>(a, v[k], mean, scale, b, y + r * a.channels);
+    }
+  }
+}
+
+// First launch, backward: a chunk's A and B per channel.
+template <class T, int VE>
+__global__ __launch_bounds__(256) void norm_sums_kernel(NormArgs a) {
+  extern __shared__ float norm_lds[];
+  constexpr int U = kNormUnroll;
+  const NormChunk ch = norm_chunk(a, blockIdx.x);
+  const NormAt p = norm_at<VE>(a, ch.image, ch.slab);
+  const T* const x = static_cast<const T*>(a.x) + p.image * a.x_image + p.c0 + p.channel;
+  const T* const g = static_cast<const T*>(a.grad) + p.image * a.g_image + p.c0 + p.channel;
+  float mean[VE], rstd[VE], w[VE], b[VE], sa[VE] = {}, sb[VE] = {}, xhat[VE], dz[VE];
+  load_affine<VE>(a, p, w, b);
+  load_stats<VE>(a, p, mean, rstd);
+  if (p.on) {
+    for (int64_t r0 = ch.first + p.tr; r0 < ch.end; r0 += int64_t(U) * a.tr) {
+      Piece<T, VE> vx[U], vg[U];
+#pragma unroll
+      for (int k = 0; k < U; ++k) {
+        const int64_t r = min(r0 + int64_t(k) * a.tr, a.rows - 1);
+        vx[k] = load_piece<T, VE>(x + r * a.x_row);
+        vg[k] = load_piece<T, VE>(g + r * a.g_row);
+      }
+#pragma unroll
+      for (int k = 0; k < U; ++k)
+        if (r0 + int64_t(k) * a.tr < ch.end) {
+          slopes<T, VE>(a, vx[k], vg[k], mean, rstd, w, b, xhat, dz);
+#pragma unroll
+          for (int i = 0; i < VE; ++i) {
+            sa[i] += dz[i];
+            sb[i] = fmaf(dz[i], xhat[i], sb[i]);
+          }
+        }
+    }
+  }
+  float2* const part = a.parts + (p.image * a.chunks + ch.chunk) * a.channels + p.c0;
+  for (int which = 0; which < 2; ++which) {
+    sum_rows<VE>(a, p, which ? sb : sa, norm_lds);
+    for (int c = int(threadIdx.x); c < p.channels; c += int(blockDim.x)) (which ? part[c].y : part[c].x) = norm_lds[c];
+  }
+}
+
+// Sums `count` rows of per-channel (A, B) of `parts` from row `first` on over the block.
+template <int VE>
+__device__ __forceinline__ void gather_sums(const NormArgs& a, const NormAt& p, int64_t first, int64_t count,
+                                            float (&sa)[VE], float (&sb)[VE]) {
+#pragma unroll
+  for (int i = 0; i < VE; ++i) sa[i] = sb[i] = 0.0f;
+  if (!p.on) return;
+  for (int64_t k = p.tr; k < count; k += a.tr) {
+    const float2* const part = a.parts + (first + k) * a.channels + p.c0 + p.channel;
+#pragma unroll
+    for (int i = 0; i < VE; ++i) {
+      sa[i] += part[i].x;
+      sb[i] += part[i].y;
+    }
+  }
+}
+
+// The last launch, backward.  Its first `slabs` blocks sum dweight and dbias over images and chunks; the others join
+// their image's chunks and write dx.
+template <class T, int VE>
+__global__ __launch_bounds__(256) void norm_dx_kernel(NormArgs a) {
+  extern __shared__ float norm_lds[];
+  constexpr int U = kNormUnroll;
+  float* const red = norm_lds;
+  float sa[VE], sb[VE];
+  if (int(blockIdx.x) < a.slabs) {
+    const NormAt p = norm_at<VE>(a, 0, int(blockIdx.x));
+    gather_sums<VE>(a, p, 0, a.images * a.chunks, sa, sb);
+    for (int which = 0; which < 2; ++which) {
+      sum_rows<VE>(a, p, which ? sb : sa, red);
+      float* const out = which ? a.dweight : a.dbias;
+      if (out)
+        for (int c = int(threadIdx.x); c < p.channels; c += int(blockDim.x)) out[p.c0 + c] = red[c];
+    }
+    return;
+  }
+  const NormChunk ch = norm_chunk(a, int64_t(blockIdx.x) - a.slabs);
+  const NormAt p = norm_at<VE>(a, ch.image, ch.slab);
+  float* const m1 = red + blockDim.x * VE;
+  float* const m2 = m1 + a.slab / a.width;
+  gather_sums<VE>(a, p, p.image * a.chunks, a.chunks, sa, sb);
+  join_sums<VE>(a, p, sa, sb, red, m1, m2, nullptr);
+  if (!p.on) return;
+  const T* const x = static_cast<const T*>(a.x) + p.image * a.x_image + p.c0 + p.channel;
+  const T* const g = static_cast<const T*>(a.grad) + p.image * a.g_image + p.c0 + p.channel;
+  T* const dx = static_cast<T*>(a.y) + p.image * a.rows * a.channels + p.c0 + p.channel;
+  float mean[VE], rstd[VE], w[VE], b[VE], xhat[VE], dz[VE], g1[VE], g2[VE];
+  load_affine<VE>(a, p, w, b);
+  load_stats<VE>(a, p, mean, rstd);
+#pragma unroll
+  for (int i = 0; i < VE; ++i) {
+    g1[i] = m1[(p.channel + i) / a.width];
+    g2[i] = m2[(p.channel + i) / a.width];
+  }
+  for (int64_t r0 = ch.first + p.tr; r0 < ch.end; r0 += int64_t(U) * a.tr) {
+    Piece<T, VE> vx[U], vg[U];
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      const int64_t r = min(r0 + int64_t(k) * a.tr, a.rows - 1);
+      vx[k] = load_piece<T, VE>(x + r * a.x_row);
+      vg[k] = load_piece<T, VE>(g + r * a.g_row);
+    }
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      const int64_t r = r0 + int64_t(k) * a.tr;
+      if (r < ch.end) {
+        slopes<T, VE>(a, vx[k], vg[k], mean, rstd, w, b, xhat, dz);
+#pragma unroll
+        for (int i = 0; i < VE; ++i) dz[i] = rstd[i] * (w[i] * dz[i] - g1[i] - xhat[i] * g2[i]);
+        store_piece<T, VE>(dx + r * a.channels, dz);
+      }
+    }
+  }
+}
+
+// dweight and dbias alone, from `chunks` rows of sums per image.
+__global__ __launch_bounds__(256) void norm_params_kernel(NormArgs a) {
+  __shared__ float2 red[256];
+  const int c = int(blockIdx.x * 16 + (threadIdx.x & 15)), tr = int(threadIdx.x >> 4);
+  float2 s{0.0f, 0.0f};
+  if (c < a.channels)
+    for (int64_t k = tr; k < a.images * a.chunks; k += 16) {
+      const float2 t = a.parts[k * a.channels + c];
+      s.x += t.x;
+      s.y += t.y;
+    }
+  red[threadIdx.x] = s;
+  for (int n = 8; n > 0; n >>= 1) {
+    __syncthreads();
+    if (tr < n) {
+      red[threadIdx.x].x += red[threadIdx.x + 16 * n].x;
+      red[threadIdx.x].y += red[threadIdx.x + 16 * n].y;
+    }
+  }
+  if (tr == 0 && c < a.channels) {
+    if (a.dbias) a.dbias[c] = red[threadIdx.x].x;
+    if (a.dweight) a.dweight[c] = red[threadIdx.x].y;
+  }
+}
+
+// ------------------------------------------------------------------ groups wider than a slab
+
 __device__ __forceinline__ float block_sum(float v, float* scratch) {
   for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
   __syncthreads();
@@ -48,104 +614,172 @@ __device__ __forceinline__ float block_sum(float v, float* scratch) {
 
 // One block per (image, group): mean, then the squared deviations from it, then y.
 template <class T>
-__global__ __launch_bounds__(256) void norm_forward_kernel(NormArgs a) {
+__global__ __launch_bounds__(256) void norm_wide_kernel(NormArgs a) {
   __shared__ float scratch[4];
   const int64_t image = blockIdx.x / a.groups;
   const int group = int(blockIdx.x % a.groups), c0 = group * a.width;
   const T* const x = static_cast<const T*>(a.x) + image * a.x_image + c0;
   T* const y = static_cast<T*>(a.y) + image * a.rows * a.channels + c0;
-  const int64_t m = a.rows * a.width;
-  float s = 0.0f;
-  for (int64_t i = threadIdx.x; i < m; i += 256) s += to_f32(x[i / a.width * a.x_row + i % a.width]);
-  const float mean = block_sum(s, scratch) / float(m);
-  s = 0.0f;
-  for (int64_t i = threadIdx.x; i < m; i += 256) {
-    const float d = to_f32(x[i / a.width * a.x_row + i % a.width]) - mean;
-    s += d * d;
+  const float m = float(a.rows) * float(a.width);
+  float mean = 0.0f, rstd = 0.0f;
+  for (int pass = 0; pass < 2; ++pass) {
+    float s = 0.0f;
+    for (int64_t r = 0; r < a.rows; ++r) {
+      float t = 0.0f;  // a row's sum first: shorter chains of additions
+      for (int c = int(threadIdx.x); c < a.width; c += 256) {
+        const float v = to_f32(x[r * a.x_row + c]) - mean;
+        t += pass ? v * v : v;
+      }
+      s += t;
+    }
+    s = block_sum(s, scratch) / m;
+    if (pass) rstd = 1.0f / sqrtf(s + a.eps);
+    else mean = s;
   }
-  const float rstd = 1.0f / sqrtf(block_sum(s, scratch) / float(m) + a.eps);
   if (a.stats && threadIdx.x == 0) {
-    a.stats[2 * blockIdx.x] = mean;
-    a.stats[2 * blockIdx.x + 1] = rstd;
+    a.stats[2 * int64_t(blockIdx.x)] = mean;
+    a.stats[2 * int64_t(blockIdx.x) + 1] = rstd;
   }
-  for (int64_t i = threadIdx.x; i < m; i += 256) {
-    const int c = int(i % a.width);
-    const float w = a.weight ? a.weight[c0 + c] : 1.0f, b = a.bias ? a.bias[c0 + c] : 0.0f;
-    const float xhat = (to_f32(x[i / a.width * a.x_row + c]) - mean) * rstd;
-    y[i / a.width * a.channels + c] = T(norm_act(a.act, xhat * w + b));
-  }
+  for (int64_t r = 0; r < a.rows; ++r)
+    for (int c = int(threadIdx.x); c < a.width; c += 256) {
+      const float w = a.weight ? a.weight[c0 + c] : 1.0f, b = a.bias ? a.bias[c0 + c] : 0.0f;
+      y[r * a.channels + c] = T(norm_act(a.act, fmaf(to_f32(x[r * a.x_row + c]) - mean, rstd * w, b)));
+    }
 }
 
-// One block per (image, channel): A and B.
+// One thread per (image, channel): A and B.
 template <class T>
-__global__ __launch_bounds__(256) void norm_sums_kernel(NormArgs a) {
-  __shared__ float scratch[4];
-  const int64_t image = blockIdx.x / a.channels;
-  const int c = int(blockIdx.x % a.channels);
+__global__ __launch_bounds__(256) void norm_wide_sums_kernel(NormArgs a) {
+  const int64_t per = (a.channels + 255) / 256, image = blockIdx.x / per;
+  const int c = int(blockIdx.x % per) * 256 + int(threadIdx.x);
+  if (c >= a.channels) return;
   const T* const x = static_cast<const T*>(a.x) + image * a.x_image + c;
   const T* const g = static_cast<const T*>(a.grad) + image * a.g_image + c;
   const float* const st = a.stats + 2 * (image * a.groups + c / a.width);
   const float w = a.weight ? a.weight[c] : 1.0f, b = a.bias ? a.bias[c] : 0.0f;
-  float sa = 0.0f, sb = 0.0f;
-  for (int64_t i = threadIdx.x; i < a.rows; i += 256) {
-    const float xhat = (to_f32(x[i * a.x_row]) - st[0]) * st[1];
-    const float dz = to_f32(g[i * a.g_row]) * norm_act_slope(a.act, xhat * w + b);
-    sa += dz;
-    sb += dz * xhat;
+  float2 s{0.0f, 0.0f};
+  for (int64_t r = 0; r < a.rows; ++r) {
+    const float xhat = (to_f32(x[r * a.x_row]) - st[0]) * st[1];
+    const float dz = to_f32(g[r * a.g_row]) * norm_act_slope(a.act, fmaf(xhat, w, b));
+    s.x += dz;
+    s.y = fmaf(dz, xhat, s.y);
   }
-  sa = block_sum(sa, scratch);
-  sb = block_sum(sb, scratch);
-  if (threadIdx.x == 0) {
-    a.sums[2 * blockIdx.x] = sa;
-    a.sums[2 * blockIdx.x + 1] = sb;
-  }
+  a.parts[image * a.channels + c] = s;
 }
 
 // One block per (image, group): dx.
 template <class T>
-__global__ __launch_bounds__(256) void norm_dx_kernel(NormArgs a) {
+__global__ __launch_bounds__(256) void norm_wide_dx_kernel(NormArgs a) {
+  __shared__ float scratch[4];
   const int64_t image = blockIdx.x / a.groups;
   const int group = int(blockIdx.x % a.groups), c0 = group * a.width;
   const T* const x = static_cast<const T*>(a.x) + image * a.x_image + c0;
   const T* const g = static_cast<const T*>(a.grad) + image * a.g_image + c0;
   T* const dx = static_cast<T*>(a.y) + image * a.rows * a.channels + c0;
-  const int64_t m = a.rows * a.width;
+  const float m = float(a.rows) * float(a.width);
   float m1 = 0.0f, m2 = 0.0f;
-  for (int c = c0; c < c0 + a.width; ++c) {
-    const float w = a.weight ? a.weight[c] : 1.0f;
-    m1 += w * a.sums[2 * (image * a.channels + c)];
-    m2 += w * a.sums[2 * (image * a.channels + c) + 1];
+  for (int c = int(threadIdx.x); c < a.width; c += 256) {
+    const float w = a.weight ? a.weight[c0 + c] : 1.0f;
+    const float2 s = a.parts[image * a.channels + c0 + c];
+    m1 += w * s.x;
+    m2 += w * s.y;
   }
-  m1 /= float(m);
-  m2 /= float(m);
-  const float mean = a.stats[2 * blockIdx.x], rstd = a.stats[2 * blockIdx.x + 1];
-  for (int64_t i = threadIdx.x; i < m; i += 256) {
-    const int c = int(i % a.width);
-    const int64_t r = i / a.width;
-    const float w = a.weight ? a.weight[c0 + c] : 1.0f, b = a.bias ? a.bias[c0 + c] : 0.0f;
-    const float xhat = (to_f32(x[r * a.x_row + c]) - mean) * rstd;
-    const float dz = to_f32(g[r * a.g_row + c]) * norm_act_slope(a.act, xhat * w + b);
-    dx[r * a.channels + c] = T(rstd * (w * dz - m1 - xhat * m2));
-  }
+  m1 = block_sum(m1, scratch) / m;
+  m2 = block_sum(m2, scratch) / m;
+  const float mean = a.stats[2 * int64_t(blockIdx.x)], rstd = a.stats[2 * int64_t(blockIdx.x) + 1];
+  for (int64_t r = 0; r < a.rows; ++r)
+    for (int c = int(threadIdx.x); c < a.width; c += 256) {
+      const float w = a.weight ? a.weight[c0 + c] : 1.0f, b = a.bias ? a.bias[c0 + c] : 0.0f;
+      const float xhat = (to_f32(x[r * a.x_row + c]) - mean) * rstd;
+      const float dz = to_f32(g[r * a.g_row + c]) * norm_act_slope(a.act, fmaf(xhat, w, b));
+      dx[r * a.channels + c] = T(rstd * (w * dz - m1 - xhat * m2));
+    }
 }
 
-__global__ __launch_bounds__(256) void norm_params_kernel(NormArgs a, float* dweight, float* dbias) {
-  const int c = int(blockIdx.x * 256 + threadIdx.x);
-  if (c >= a.channels) return;
-  float sa = 0.0f, sb = 0.0f;
-  for (int64_t i = 0; i < a.images; ++i) {
-    sa += a.sums[2 * (i * a.channels + c)];
-    sb += a.sums[2 * (i * a.channels + c) + 1];
-  }
-  if (dweight) dweight[c] = sb;
-  if (dbias) dbias[c] = sa;
+// ------------------------------------------------------------------ planning
+
+struct NormPlan {
+  enum Kind { kWhole, kChunked, kWide } kind;
+  int ve, slab, slabs, pieces, tr, threads, chunks, chunk_rows;
+  int64_t bytes;
+};
+
+// Elements per piece: 16 bytes, or the largest power of two that the channel count and the strides allow.  Base
+// pointers are checked at the launch and can only make it smaller, which leaves the plan's other figures valid upper
+// bounds (see launch); `align` is the pointers' alignment in bytes.
+int piece_elements(const rdv_group_norm_desc& d, bool backward, int align) {
+  const int size = d.dtype == RDV_DTYPE_F32 ? 4 : 2;
+  int ve = 16 / size;
+  auto fits = [&](int e) {
+    return d.channels % e == 0 && (d.rows == 1 || d.x_row_stride % e == 0) && (d.images == 1 || d.x_image_stride % e == 0) &&
+           (!backward || ((d.rows == 1 || d.g_row_stride % e == 0) && (d.images == 1 || d.g_image_stride % e == 0))) &&
+           align % (e * size) == 0;
+  };
+  while (ve > 1 && !fits(ve)) ve /= 2;
+  return ve;
 }
 
-NormArgs norm_args(const rdv_group_norm_desc& d, const void* x, const float* weight, const float* bias) {
+constexpr int kWholePieces = 8, kWholeBackPieces = 4;
+
+NormPlan norm_plan(const rdv_group_norm_desc& d, bool backward, int cu, int align) {
+  NormPlan p{};
+  const int size = d.dtype == RDV_DTYPE_F32 ? 4 : 2, width = d.channels / d.groups;
+  p.ve = piece_elements(d, backward, align);
+  const int64_t unit = std::lcm(int64_t(width), int64_t(p.ve));  // channels of the narrowest slab
+  if (unit > int64_t(256) * p.ve) {
+    p.kind = NormPlan::kWide;
+    p.slab = d.channels;
+    p.chunks = 1;
+    p.bytes = backward ? d.images * d.channels * 8 : 0;
+    return p;
+  }
+  auto set_slab = [&](int64_t slab) {
+    p.slab = int(std::min<int64_t>(slab, d.channels));
+    p.pieces = p.slab / p.ve;
+    p.slabs = (d.channels + p.slab - 1) / p.slab;
+  };
+  // one launch: slabs of at least 64 bytes a row, wider while blocks abound
+  const int64_t per_thread = backward ? kWholeBackPieces : kWholePieces;
+  int64_t slab = unit;
+  while (slab < d.channels && slab * size < 64) slab += unit;
+  set_slab(slab);
+  if (d.rows * p.pieces <= 1024 * per_thread && p.pieces <= 256) {
+    while (p.slab < d.channels && d.images * p.slabs > 2 * int64_t(cu) && 2 * p.pieces <= 256 &&
+           2 * d.rows * p.pieces <= 256 * per_thread)
+      set_slab(2 * int64_t(p.slab));
+    for (int threads : {256, 512, 1024}) {
+      p.threads = threads;
+      p.tr = threads / p.pieces;
+      if (d.rows <= p.tr * per_thread) {
+        p.kind = NormPlan::kWhole;
+        p.chunks = 1;
+        p.bytes = backward ? d.images * d.channels * 8 : 0;
+        return p;
+      }
+    }
+  }
+  // two launches: the widest slab, two blocks per CU
+  p.kind = NormPlan::kChunked;
+  p.threads = 256;
+  set_slab(int64_t(256) * p.ve / unit * unit);
+  p.tr = 256 / p.pieces;
+  const int64_t least = int64_t(p.tr) * kNormUnroll;  // rows that give every thread its first loads
+  int64_t chunks = std::max<int64_t>(1, 2 * int64_t(cu) / std::max<int64_t>(1, d.images * p.slabs));
+  chunks = std::min(chunks, (d.rows + least - 1) / least);
+  const int64_t rows = (d.rows + chunks - 1) / chunks;
+  p.chunk_rows = int((rows + p.tr - 1) / p.tr * p.tr);
+  p.chunks = int((d.rows + p.chunk_rows - 1) / p.chunk_rows);
+  p.bytes = d.images * p.chunks * 8 * (backward ? d.channels : d.groups);
+  return p;
+}
+
+NormArgs norm_args(const rdv_group_norm_desc& d, const NormPlan& p, const void* x, const float* weight,
+                   const float* bias, void* ws) {
   NormArgs a{};
   a.x = x;
   a.weight = weight;
   a.bias = bias;
+  a.parts = static_cast<float2*>(ws);
   a.images = d.images;
   a.rows = d.rows;
   a.x_image = d.x_image_stride;
@@ -157,23 +791,75 @@ NormArgs norm_args(const rdv_group_norm_desc& d, const void* x, const float* wei
   a.width = d.channels / d.groups;
   a.act = d.act;
   a.eps = d.eps;
+  a.slab = p.slab;
+  a.slabs = p.slabs;
+  a.pieces = p.pieces;
+  a.tr = p.tr;
+  a.chunks = p.chunks;
+  a.chunk_rows = p.chunk_rows;
   return a;
+}
+
+// Calls f(T{}, integral_constant<int, VE>{}) for the type and the elements of a piece.
+template <class F>
+int with_piece(int dtype, int ve, F&& f) {
+  return with_dtype(dtype, [&](auto t) {
+    switch (ve) {
+      case 8:
+        if constexpr (sizeof(t) == 2) return f(t, std::integral_constant<int, 8>{});
+        [[fallthrough]];
+      case 4: return f(t, std::integral_constant<int, 4>{});
+      case 2: return f(t, std::integral_constant<int, 2>{});
+      default: return f(t, std::integral_constant<int, 1>{});
+    }
+  });
+}
+
+int alignment(std::initializer_list<const void*> ps) {
+  uintptr_t bits = 16;
+  for (const void* p : ps) bits |= reinterpret_cast<uintptr_t>(p);
+  return int(bits & (~bits + 1));
+}
+
+int check_blocks(int64_t n) {
+  return n < (int64_t(1) << 31) ? int(RDV_OK) : fail(RDV_ERR_UNSUPPORTED, "group norm: too many blocks");
 }
 
 }  // namespace
 
-int64_t group_norm_workspace_bytes(const rdv_group_norm_desc& d, bool backward, int) {
-  return backward ? d.images * d.channels * 8 : 0;
+// The base pointers' alignment is not known here: the most any of the piece sizes asks for.
+int64_t group_norm_workspace_bytes(const rdv_group_norm_desc& d, bool backward, int cu) {
+  int64_t bytes = 0;
+  for (int align = 16; align >= 2; align /= 2) bytes = std::max(bytes, norm_plan(d, backward, cu, align).bytes);
+  return bytes;
 }
 
 int launch_group_norm(const rdv_group_norm_desc& d, const void* x, const float* weight, const float* bias, void* y,
-                      float* stats, void*, hipStream_t stream) {
-  NormArgs a = norm_args(d, x, weight, bias);
+                      float* stats, void* ws, int cu, hipStream_t stream) {
+  const NormPlan p = norm_plan(d, false, cu, alignment({x, y}));
+  NormArgs a = norm_args(d, p, x, weight, bias, ws);
   a.y = y;
   a.stats = stats;
-  if (d.images * d.groups >= (int64_t(1) << 31)) return fail(RDV_ERR_UNSUPPORTED, "group norm: too many groups");
-  return with_dtype(d.dtype, [&](auto t) {
-    norm_forward_kernel<decltype(t)><<<dim3(unsigned(d.images * d.groups)), 256, 0, stream>>>(a);
+  if (p.kind == NormPlan::kWide) {
+    if (int rc = check_blocks(d.images * d.groups)) return rc;
+    return with_dtype(d.dtype, [&](auto t) {
+      norm_wide_kernel<decltype(t)><<<dim3(unsigned(d.images * d.groups)), 256, 0, stream>>>(a);
+      RDV_HIP_TRY(hipGetLastError());
+      return int(RDV_OK);
+    });
+  }
+  const int64_t blocks = d.images * p.slabs * p.chunks;
+  if (int rc = check_blocks(blocks)) return rc;
+  const unsigned lds = unsigned(p.threads * p.ve + 2 * (p.slab / a.width)) * 4;
+  return with_piece(d.dtype, p.ve, [&](auto t, auto ve) {
+    using T = decltype(t);
+    constexpr int VE = decltype(ve)::value;
+    if (p.kind == NormPlan::kWhole) {
+      norm_whole_kernel<T, VE, kWholePieces><<<dim3(unsigned(blocks)), p.threads, lds, stream>>>(a);
+    } else {
+      norm_stats_kernel<T, VE><<<dim3(unsigned(blocks)), p.threads, lds, stream>>>(a);
+      norm_apply_kernel<T, VE><<<dim3(unsigned(blocks)), p.threads, unsigned(2 * (p.slab / a.width) * 4), stream>>>(a);
+    }
     RDV_HIP_TRY(hipGetLastError());
     return int(RDV_OK);
   });
@@ -181,22 +867,44 @@ int launch_group_norm(const rdv_group_norm_desc& d, const void* x, const float* 
 
 int launch_group_norm_backward(const rdv_group_norm_desc& d, const void* grad, const void* x, const float* weight,
                                const float* bias, const float* stats, void* dx, float* dweight, float* dbias,
-                               void* ws, hipStream_t stream) {
-  NormArgs a = norm_args(d, x, weight, bias);
+                               void* ws, int cu, hipStream_t stream) {
+  const bool empty = d.images == 0 || d.rows == 0;
+  const NormPlan p = empty ? NormPlan{} : norm_plan(d, true, cu, alignment({x, grad, dx}));
+  NormArgs a = norm_args(d, p, x, weight, bias, ws);
   a.grad = grad;
   a.stats = const_cast<float*>(stats);
-  a.sums = static_cast<float*>(ws);
   a.y = dx;
-  if (d.images * d.channels >= (int64_t(1) << 31)) return fail(RDV_ERR_UNSUPPORTED, "group norm: too many channels");
-  return with_dtype(d.dtype, [&](auto t) {
+  a.dweight = dweight;
+  a.dbias = dbias;
+  if (empty) a.images = 0;
+  const unsigned param_blocks = unsigned((d.channels + 15) / 16);
+  if (empty || p.kind == NormPlan::kWide) {
+    const int64_t per = (d.channels + 255) / 256;
+    if (int rc = check_blocks(d.images * std::max<int64_t>(d.groups, per))) return rc;
+    return with_dtype(d.dtype, [&](auto t) {
+      using T = decltype(t);
+      if (!empty) {
+        norm_wide_sums_kernel<T><<<dim3(unsigned(d.images * per)), 256, 0, stream>>>(a);
+        norm_wide_dx_kernel<T><<<dim3(unsigned(d.images * d.groups)), 256, 0, stream>>>(a);
+      }
+      norm_params_kernel<<<dim3(param_blocks), 256, 0, stream>>>(a);
+      RDV_HIP_TRY(hipGetLastError());
+      return int(RDV_OK);
+    });
+  }
+  const int64_t blocks = d.images * p.slabs * p.chunks + (p.kind == NormPlan::kChunked ? p.slabs : 0);
+  if (int rc = check_blocks(blocks)) return rc;
+  const unsigned lds = unsigned(p.threads * p.ve + 2 * (p.slab / a.width)) * 4;
+  return with_piece(d.dtype, p.ve, [&](auto t, auto ve) {
     using T = decltype(t);
-    if (d.images > 0 && d.rows > 0) {
-      norm_sums_kernel<T><<<dim3(unsigned(d.images * d.channels)), 256, 0, stream>>>(a);
-      norm_dx_kernel<T><<<dim3(unsigned(d.images * d.groups)), 256, 0, stream>>>(a);
+    constexpr int VE = decltype(ve)::value;
+    if (p.kind == NormPlan::kWhole) {
+      norm_whole_back_kernel<T, VE, kWholeBackPieces><<<dim3(unsigned(blocks)), p.threads, lds, stream>>>(a);
+      norm_params_kernel<<<dim3(param_blocks), 256, 0, stream>>>(a);
     } else {
-      a.images = 0;
+      norm_sums_kernel<T, VE><<<dim3(unsigned(blocks - p.slabs)), p.threads, lds, stream>>>(a);
+      norm_dx_kernel<T, VE><<<dim3(unsigned(blocks)), p.threads, lds, stream>>>(a);
     }
-    norm_params_kernel<<<dim3(unsigned((d.channels + 255) / 256)), 256, 0, stream>>>(a, dweight, dbias);
     RDV_HIP_TRY(hipGetLastError());
     return int(RDV_OK);
   });
