@@ -11,6 +11,7 @@ are in nn.py.  There is no CPU path."""
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import math
 
 import torch
@@ -46,15 +47,21 @@ def _like(t, x: torch.Tensor, what: str) -> torch.Tensor:
     return t
 
 
+def _gpu_index() -> int:
+    """The current GPU, or -1 where there is none (arguments are still checked there)."""
+    return torch.cuda.current_device() if torch.cuda.is_initialized() else -1
+
+
 def _on_gpu(*named) -> None:
-    """Every tensor on the current GPU: launches go there, on its current stream."""
-    for t, what in named:
-        if t is None:
-            continue
-        if not t.is_cuda:
+    """Every tensor (followed by its name) on the current GPU: launches go there, on its current stream."""
+    current = _gpu_index()
+    for t, what in zip(named[::2], named[1::2]):
+        if t is not None and t.get_device() != current:
+            if not t.is_cuda:
+                raise TypeError(f"{what} must be a GPU tensor, got device {t.device}")
+            raise TypeError(f"{what} is on {t.device}, the current GPU is cuda:{current}")
+        if t is not None and current < 0:
             raise TypeError(f"{what} must be a GPU tensor, got device {t.device}")
-        if t.device.index != torch.cuda.current_device():
-            raise TypeError(f"{what} is on {t.device}, the current GPU is cuda:{torch.cuda.current_device()}")
 
 
 def _out_tensor(out, shape, dtype, device, what: str = "out", aligned: bool = True) -> torch.Tensor:
@@ -88,14 +95,9 @@ def _apart(out: torch.Tensor, *inputs) -> None:
                 f"out must not share memory with {what}"
 
 
-def _workspace(nbytes: int, what: str, device) -> tuple:
-    """(tensor, pointer, bytes): scratch of one call, from the allocator so that calls on other streams get their own."""
-    if nbytes < 0:
-        _lib.check(int(nbytes), what)
-    if nbytes == 0:
-        return None, 0, 0
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
-    return ws, ws.data_ptr(), nbytes
+def _check(rc: int, what: str) -> None:
+    if rc:
+        _lib.check(rc, what)
 
 
 def _ptr(t) -> int:
@@ -105,59 +107,72 @@ def _ptr(t) -> int:
 # ------------------------------------------------------------ group normalisation
 
 
-def _image_rows(t: torch.Tensor) -> tuple:
-    """(t or its contiguous copy, image stride, row stride) of t [images, ..., channels] or [rows, channels]."""
-    if not t.is_contiguous():
-        shape, stride = t.shape, t.stride()
-        first = 1 if t.dim() > 2 else 0
-        merged = stride[-1] == 1 or shape[-1] == 1
-        step, count = None, 1
-        for i in range(t.dim() - 2, first - 1, -1):  # the dimensions of the rows, innermost first
-            if shape[i] == 1:
-                continue
-            if step is None:
-                step = stride[i]
-            merged = merged and stride[i] == step * count
-            count *= shape[i]
-        if merged:
-            return t, (stride[0] if first else 0), (step or 0)
-        t = t.contiguous()
-    channels = t.shape[-1]
-    return t, (t.numel() // max(1, t.shape[0]) if t.dim() > 2 else 0), channels
+def _image_rows(shape, stride):
+    """(image stride, row stride) of a tensor [images, ..., channels] or [rows, channels] of these strides, or None
+    where its rows do not lie at one distance with contiguous channels."""
+    if stride[-1] != 1 and shape[-1] != 1:
+        return None
+    first = 1 if len(shape) > 2 else 0
+    step, count = None, 1
+    for i in range(len(shape) - 2, first - 1, -1):  # the dimensions of the rows, innermost first
+        if shape[i] == 1:
+            continue
+        if step is None:
+            step = stride[i]
+        elif stride[i] != step * count:
+            return None
+        count *= shape[i]
+    return (stride[0] if first else 0), (step or 0)
 
 
-def _norm_inputs(x, weight, bias, groups, eps, activation):
-    x = _data(x, "x")
-    assert x.dim() >= 2, "x must be [rows, channels] (one image) or [images, ..., channels]"
-    channels = int(x.shape[-1])
-    assert channels >= 1 and int(groups) >= 1 and channels % int(groups) == 0, \
+@functools.lru_cache(maxsize=4096)
+def _norm_plan(shape, x_stride, g_stride, dtype, groups, eps, activation, device):
+    """What a call on tensors of this layout needs, by layout alone: (descriptor, whether x and grad have to be copied
+    first, workspace bytes).  g_stride is None for the forward call; `device` is the GPU it is planned for."""
+    channels = shape[-1]
+    assert channels >= 1 and groups >= 1 and channels % groups == 0, \
         f"groups ({groups}) must divide the channels ({channels})"
     if activation not in _ACTIVATIONS:
         raise ValueError(f"activation must be one of {sorted(_ACTIVATIONS)}, got {activation!r}")
+    images = shape[0] if len(shape) > 2 else 1
+    rows = math.prod(shape[1:-1]) if len(shape) > 2 else shape[0]
+    dense = (rows * channels if len(shape) > 2 else 0, channels)
+    d = _lib.GroupNormDesc()
+    d.images, d.rows, d.channels, d.groups, d.eps = images, rows, channels, groups, eps
+    d.act, d.dtype = _ACTIVATIONS[activation], _DTYPES[dtype]
+    at = _image_rows(shape, x_stride)
+    d.x_image_stride, d.x_row_stride = at or dense
+    g_at = dense if g_stride is None else _image_rows(shape, g_stride)
+    d.g_image_stride, d.g_row_stride = g_at or dense
+    nbytes = _lib.load().rdv_group_norm_workspace_bytes(C.byref(d), 0 if g_stride is None else 1)
+    if nbytes < 0:
+        _lib.check(int(nbytes), "group_norm")
+    return d, at is None, g_at is None, nbytes
+
+
+def _norm_inputs(x, weight, bias):
+    x = _data(x, "x")
+    assert x.dim() >= 2, "x must be [rows, channels] (one image) or [images, ..., channels]"
     params = []
     for p, what in ((weight, "weight"), (bias, "bias")):
         if p is not None:
             p = _tensor(p, what)
-            assert tuple(p.shape) == (channels,), f"{what} must be [channels]"
+            assert p.dim() == 1 and p.shape[0] == x.shape[-1], f"{what} must be [channels]"
             if p.dtype != torch.float32:
                 raise TypeError(f"{what} must be float32, got {p.dtype}")
             p = p.contiguous()
         params.append(p)
-    d = _lib.GroupNormDesc()
-    d.images = int(x.shape[0]) if x.dim() > 2 else 1
-    d.rows = math.prod(x.shape[1:-1]) if x.dim() > 2 else int(x.shape[0])
-    d.channels, d.groups, d.eps = channels, int(groups), float(eps)
-    d.act, d.dtype = _ACTIVATIONS[activation], _DTYPES[x.dtype]
-    return x, params[0], params[1], d
+    return x, params[0], params[1]
 
 
-def _group_norm_into(d, x, weight, bias, y, stats) -> None:
+def _group_norm_into(plan, x, weight, bias, y, stats) -> None:
     """Launches rdv_group_norm into y and stats (or None)."""
-    x, d.x_image_stride, d.x_row_stride = _image_rows(x)
-    lib = _lib.load()
-    ws, wp, wn = _workspace(lib.rdv_group_norm_workspace_bytes(C.byref(d), 0), "group_norm", x.device)
-    _lib.check(lib.rdv_group_norm(C.byref(d), x.data_ptr(), _ptr(weight), _ptr(bias), y.data_ptr(), _ptr(stats), wp,
-                                  wn, current_stream_handle()), "group_norm")
+    d, copy, _, nbytes = plan
+    if copy:
+        x = x.contiguous()
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
+    _check(_lib.load().rdv_group_norm(C.byref(d), x.data_ptr(), _ptr(weight), _ptr(bias), y.data_ptr(), _ptr(stats),
+                                      _ptr(ws), nbytes, current_stream_handle()), "group_norm")
 
 
 def group_norm(x, weight, bias, groups: int, eps: float = 1e-5, activation: str = "none", out=None,
@@ -170,14 +185,17 @@ def group_norm(x, weight, bias, groups: int, eps: float = 1e-5, activation: str 
     ReLUTensorOp does) or "silu".  Returns y like x, contiguous, and with
     return_stats also stats [images, groups, 2] = (mean, 1 / std) in float32,
     which group_norm_backward takes."""
-    x, weight, bias, d = _norm_inputs(x, weight, bias, groups, eps, activation)
-    _on_gpu((x, "x"), (weight, "weight"), (bias, "bias"))
+    x, weight, bias = _norm_inputs(x, weight, bias)
+    plan = _norm_plan(x.shape, x.stride(), None, x.dtype, int(groups), float(eps), activation, _gpu_index())
+    _on_gpu(x, "x", weight, "weight", bias, "bias")
     y = _out_tensor(out, x.shape, x.dtype, x.device)
     if out is not None:
         _apart(y, (x, "x"), (weight, "weight"), (bias, "bias"))
-    stats = torch.empty((d.images, d.groups, 2), dtype=torch.float32, device=x.device) if return_stats else None
+    stats = None
+    if return_stats:
+        stats = torch.empty((plan[0].images, plan[0].groups, 2), dtype=torch.float32, device=x.device)
     with launch_scope():
-        _group_norm_into(d, x, weight, bias, y, stats)
+        _group_norm_into(plan, x, weight, bias, y, stats)
     return (y, stats) if return_stats else y
 
 
@@ -186,90 +204,111 @@ def group_norm_backward(grad, x, weight, bias, groups: int, stats, activation: s
     returned for the same x, weight, bias, groups and activation.  dx is like
     x, dweight and dbias are float32 [channels]; `grads` supplies the three
     buffers."""
-    x, weight, bias, d = _norm_inputs(x, weight, bias, groups, 0.0, activation)
+    x, weight, bias = _norm_inputs(x, weight, bias)
     grad = _like(grad, x, "grad")
+    d, copy_x, copy_g, nbytes = _norm_plan(x.shape, x.stride(), grad.stride(), x.dtype, int(groups), 0.0, activation,
+                                           _gpu_index())
     stats = _tensor(stats, "stats")
     assert tuple(stats.shape) == (d.images, d.groups, 2) and stats.is_contiguous(), \
         f"stats must be a contiguous [{d.images}, {d.groups}, 2] tensor, as group_norm returns it"
     if stats.dtype != torch.float32:
         raise TypeError(f"stats must be float32, got {stats.dtype}")
-    _on_gpu((x, "x"), (grad, "grad"), (weight, "weight"), (bias, "bias"), (stats, "stats"))
+    _on_gpu(x, "x", grad, "grad", weight, "weight", bias, "bias", stats, "stats")
     dx, dw, db = _grad_tensors(grads, (x.shape, (d.channels,), (d.channels,)), (x.dtype, torch.float32, torch.float32),
                                x.device, ("dx", "dweight", "dbias"))
     if grads is not None:
         for t in (dx, dw, db):
             _apart(t, (x, "x"), (grad, "grad"), (weight, "weight"), (bias, "bias"), (stats, "stats"))
-    lib = _lib.load()
     with launch_scope():
-        x, d.x_image_stride, d.x_row_stride = _image_rows(x)
-        grad, d.g_image_stride, d.g_row_stride = _image_rows(grad)
-        ws, wp, wn = _workspace(lib.rdv_group_norm_workspace_bytes(C.byref(d), 1), "group_norm_backward", x.device)
-        _lib.check(lib.rdv_group_norm_backward(C.byref(d), grad.data_ptr(), x.data_ptr(), _ptr(weight), _ptr(bias),
-                                               stats.data_ptr(), dx.data_ptr(), dw.data_ptr(), db.data_ptr(), wp, wn,
-                                               current_stream_handle()), "group_norm_backward")
+        if copy_x:
+            x = x.contiguous()
+        if copy_g:
+            grad = grad.contiguous()
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
+        _check(_lib.load().rdv_group_norm_backward(C.byref(d), grad.data_ptr(), x.data_ptr(), _ptr(weight), _ptr(bias),
+                                                   stats.data_ptr(), dx.data_ptr(), dw.data_ptr(), db.data_ptr(),
+                                                   _ptr(ws), nbytes, current_stream_handle()), "group_norm_backward")
     return dx, dw, db
 
 
 # ------------------------------------------------------------ cross attention
 
 
-def _innermost(t: torch.Tensor) -> torch.Tensor:
-    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
-
-
 def _rows_in_place(t: torch.Tensor) -> torch.Tensor:
     """t [batch, length, heads, dim] as the library reads it: the innermost dimension contiguous and, as rows whose
     strides are multiples of 16 bytes are read in pieces of that size, such a tensor itself aligned to it."""
-    t = _innermost(t)
+    if t.stride(-1) != 1 and t.shape[-1] != 1:
+        t = t.contiguous()
     return t if t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
 
 
-def _attention_inputs(q, k, v, key_lengths, key_mask, scale):
-    q, k, v = _data(q, "q"), _data(k, "k"), _data(v, "v")
-    assert q.dim() == 4, "q must be [batch, queries, heads, dim]"
-    assert k.dim() == 4 and k.shape == v.shape, "k and v must both be [batch, keys, kv_heads, dim]"
-    b, lq, hq, dim = (int(n) for n in q.shape)
-    lk, hkv = int(k.shape[1]), int(k.shape[2])
-    assert int(k.shape[0]) == b, f"q has a batch of {b}, k and v of {k.shape[0]}"
-    assert int(k.shape[3]) == dim, f"q has heads of {dim} dimensions, k and v of {k.shape[3]}"
+@functools.lru_cache(maxsize=4096)
+def _attention_plan(q_shape, k_shape, v_shape, q_stride, k_stride, v_stride, g_stride, mask_stride, dtype, scale, device):
+    """What a call on tensors of this layout needs, by layout alone: (descriptor, workspace bytes).  g_stride is None
+    for the forward call; `device` is the GPU it is planned for."""
+    assert len(q_shape) == 4, "q must be [batch, queries, heads, dim]"
+    assert len(k_shape) == 4 and k_shape == v_shape, "k and v must both be [batch, keys, kv_heads, dim]"
+    b, lq, hq, dim = q_shape
+    _, lk, hkv, k_dim = k_shape
+    assert k_shape[0] == b, f"q has a batch of {b}, k and v of {k_shape[0]}"
+    assert k_dim == dim, f"q has heads of {dim} dimensions, k and v of {k_dim}"
     assert hkv >= 1 and hq >= 1 and hq % hkv == 0, f"kv_heads ({hkv}) must divide heads ({hq})"
-    if k.dtype != q.dtype or v.dtype != q.dtype:
-        raise TypeError(f"q, k and v must have one type, got {q.dtype}, {k.dtype} and {v.dtype}")
-    if key_lengths is not None:
-        key_lengths = _tensor(key_lengths, "key_lengths")
-        assert tuple(key_lengths.shape) == (b,), f"key_lengths must be [batch] = [{b}]"
-        if key_lengths.dtype not in (torch.int32, torch.int64):
-            raise TypeError(f"key_lengths must be int32 or int64, got {key_lengths.dtype}")
-    if key_mask is not None:
-        key_mask = _tensor(key_mask, "key_mask")
-        assert tuple(key_mask.shape) == (b, lk), f"key_mask must be [batch, keys] = [{b}, {lk}]"
-        if key_mask.dtype != torch.bool:
-            raise TypeError(f"key_mask must be bool, got {key_mask.dtype}")
-    scale = 1.0 / math.sqrt(dim) if scale is None else float(scale)
+    scale = 1.0 / math.sqrt(dim) if scale is None else scale
     if not math.isfinite(scale):
         raise ValueError(f"scale must be finite, got {scale}")
-    _on_gpu((q, "q"), (k, "k"), (v, "v"), (key_lengths, "key_lengths"), (key_mask, "key_mask"))
-    q, k, v = _rows_in_place(q), _rows_in_place(k), _rows_in_place(v)
     d = _lib.AttentionDesc()
     d.batch, d.queries, d.keys, d.heads, d.kv_heads, d.dim = b, lq, lk, hq, hkv, dim
-    d.dtype, d.scale = _DTYPES[q.dtype], scale
-    d.q_stride[:], d.k_stride[:], d.v_stride[:] = q.stride()[:3], k.stride()[:3], v.stride()[:3]
-    if key_lengths is not None:
-        key_lengths = key_lengths.clamp(0, lk).to(torch.int32) if key_lengths.dtype == torch.int64 else key_lengths
-        key_lengths = key_lengths.contiguous()
+    d.dtype, d.scale, d.mask_stride = _DTYPES[dtype], scale, mask_stride
+    d.q_stride[:], d.k_stride[:], d.v_stride[:] = q_stride[:3], k_stride[:3], v_stride[:3]
+    if g_stride is not None:
+        d.g_stride[:] = g_stride[:3]
+    nbytes = _lib.load().rdv_cross_attention_workspace_bytes(C.byref(d), 0 if g_stride is None else 1)
+    if nbytes < 0:
+        _lib.check(int(nbytes), "cross_attention")
+    return d, nbytes
+
+
+def _attention_inputs(q, k, v, key_lengths, key_mask, scale, grad=None):
+    """The checked inputs as the library reads them, and the plan."""
+    q, k, v = _data(q, "q"), _data(k, "k"), _data(v, "v")
+    if k.dtype != q.dtype or v.dtype != q.dtype:
+        raise TypeError(f"q, k and v must have one type, got {q.dtype}, {k.dtype} and {v.dtype}")
+    if q.dim() == k.dim() == v.dim() == 4:  # else the plan refuses
+        q, k, v = _rows_in_place(q), _rows_in_place(k), _rows_in_place(v)
+    if grad is not None:
+        grad = _rows_in_place(_like(grad, q, "grad"))
+    mask_stride = 0
     if key_mask is not None:
-        key_mask = _innermost(key_mask) if lk else None
-        d.mask_stride = key_mask.stride(0) if lk else 0
-    return q, k, v, key_lengths, key_mask, d
+        key_mask = _tensor(key_mask, "key_mask")
+        assert key_mask.dim() == 2 and k.dim() == 4 and key_mask.shape == k.shape[:2], "key_mask must be [batch, keys]"
+        if key_mask.dtype != torch.bool:
+            raise TypeError(f"key_mask must be bool, got {key_mask.dtype}")
+        if key_mask.stride(1) != 1:
+            key_mask = key_mask.contiguous()
+        mask_stride = key_mask.stride(0)
+    plan = _attention_plan(q.shape, k.shape, v.shape, q.stride(), k.stride(), v.stride(),
+                           None if grad is None else grad.stride(), mask_stride, q.dtype,
+                           None if scale is None else float(scale), _gpu_index())
+    if key_lengths is not None:
+        key_lengths = _tensor(key_lengths, "key_lengths")
+        assert tuple(key_lengths.shape) == (q.shape[0],), f"key_lengths must be [batch] = [{q.shape[0]}]"
+        if key_lengths.dtype not in (torch.int32, torch.int64):
+            raise TypeError(f"key_lengths must be int32 or int64, got {key_lengths.dtype}")
+    _on_gpu(q, "q", k, "k", v, "v", key_lengths, "key_lengths", key_mask, "key_mask", grad, "grad")
+    if key_lengths is not None:
+        if key_lengths.dtype == torch.int64:
+            key_lengths = key_lengths.clamp(0, k.shape[1]).to(torch.int32)
+        key_lengths = key_lengths.contiguous()
+    return q, k, v, key_lengths, key_mask, grad, plan
 
 
-def _cross_attention_into(d, q, k, v, key_lengths, key_mask, out, lse) -> None:
+def _cross_attention_into(plan, q, k, v, key_lengths, key_mask, out, lse) -> None:
     """Launches rdv_cross_attention into out and lse (or None)."""
-    lib = _lib.load()
-    ws, wp, wn = _workspace(lib.rdv_cross_attention_workspace_bytes(C.byref(d), 0), "cross_attention", q.device)
-    _lib.check(lib.rdv_cross_attention(C.byref(d), q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(key_lengths),
-                                       _ptr(key_mask), out.data_ptr(), _ptr(lse), wp, wn, current_stream_handle()),
-               "cross_attention")
+    d, nbytes = plan
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
+    _check(_lib.load().rdv_cross_attention(C.byref(d), q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(key_lengths),
+                                           _ptr(key_mask), out.data_ptr(), _ptr(lse), _ptr(ws), nbytes,
+                                           current_stream_handle()), "cross_attention")
 
 
 def cross_attention(q, k, v, key_lengths=None, key_mask=None, scale: float | None = None, out=None,
@@ -286,15 +325,19 @@ def cross_attention(q, k, v, key_lengths=None, key_mask=None, scale: float | Non
     cross_attention_backward takes.  float16 and bfloat16 inputs: the matrix
     cores take softmax terms rounded to that type; float32: float32
     throughout."""
-    q, k, v, key_lengths, key_mask, d = _attention_inputs(q, k, v, key_lengths, key_mask, scale)
-    given = out is not None
-    out = _out_tensor(out, q.shape, q.dtype, q.device)
-    if given:
-        _apart(out, (q, "q"), (k, "k"), (v, "v"), (key_lengths, "key_lengths"), (key_mask, "key_mask"))
-    lse = torch.empty((d.batch, d.heads, d.queries), dtype=torch.float32, device=q.device) if return_lse else None
+    given = q, k, v
+    q, k, v, key_lengths, key_mask, _, plan = _attention_inputs(q, k, v, key_lengths, key_mask, scale)
+    y = _out_tensor(out, q.shape, q.dtype, q.device)
+    if out is not None:
+        _apart(y, (_tensor(given[0], "q"), "q"), (_tensor(given[1], "k"), "k"), (_tensor(given[2], "v"), "v"),
+               (key_lengths, "key_lengths"), (key_mask, "key_mask"))
+    lse = None
+    if return_lse:
+        d = plan[0]
+        lse = torch.empty((d.batch, d.heads, d.queries), dtype=torch.float32, device=q.device)
     with launch_scope():
-        _cross_attention_into(d, q, k, v, key_lengths, key_mask, out, lse)
-    return (out, lse) if return_lse else out
+        _cross_attention_into(plan, q, k, v, key_lengths, key_mask, y, lse)
+    return (y, lse) if return_lse else y
 
 
 def cross_attention_backward(grad, q, k, v, out, lse, key_lengths=None, key_mask=None, scale: float | None = None,
@@ -303,31 +346,27 @@ def cross_attention_backward(grad, q, k, v, out, lse, key_lengths=None, key_mask
     it returned for the same arguments.  dk and dv are summed over the heads
     that share a state head and are 0 at states that do not count; `grads`
     supplies the three buffers."""
-    q, k, v, key_lengths, key_mask, d = _attention_inputs(q, k, v, key_lengths, key_mask, scale)
-    grad, out = _like(grad, q, "grad"), _like(out, q, "out").contiguous()
+    q, k, v, key_lengths, key_mask, grad, (d, nbytes) = _attention_inputs(q, k, v, key_lengths, key_mask, scale, grad)
+    out = _like(out, q, "out").contiguous()
     lse = _tensor(lse, "lse")
     assert tuple(lse.shape) == (d.batch, d.heads, d.queries) and lse.is_contiguous(), \
         f"lse must be a contiguous [{d.batch}, {d.heads}, {d.queries}] tensor, as cross_attention returns it"
     if lse.dtype != torch.float32:
         raise TypeError(f"lse must be float32, got {lse.dtype}")
-    _on_gpu((grad, "grad"), (out, "out"), (lse, "lse"))
-    grad = _rows_in_place(grad)
-    d.g_stride[:] = grad.stride()[:3]
+    _on_gpu(out, "out", lse, "lse")
     given = grads is not None
-    grads = _grad_tensors(grads, (q.shape, k.shape, v.shape), (q.dtype,) * 3, q.device, ("dq", "dk", "dv"))
+    dq, dk, dv = _grad_tensors(grads, (q.shape, k.shape, v.shape), (q.dtype,) * 3, q.device, ("dq", "dk", "dv"))
     if given:
-        for t in grads:
+        for t in (dq, dk, dv):
             _apart(t, (grad, "grad"), (q, "q"), (k, "k"), (v, "v"), (out, "out"), (lse, "lse"),
                    (key_lengths, "key_lengths"), (key_mask, "key_mask"))
-    dq, dk, dv = grads
-    lib = _lib.load()
     with launch_scope():
-        ws, wp, wn = _workspace(lib.rdv_cross_attention_workspace_bytes(C.byref(d), 1), "cross_attention_backward",
-                                q.device)
-        _lib.check(lib.rdv_cross_attention_backward(C.byref(d), grad.data_ptr(), q.data_ptr(), k.data_ptr(),
-                                                    v.data_ptr(), out.data_ptr(), lse.data_ptr(), _ptr(key_lengths),
-                                                    _ptr(key_mask), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), wp,
-                                                    wn, current_stream_handle()), "cross_attention_backward")
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
+        _check(_lib.load().rdv_cross_attention_backward(C.byref(d), grad.data_ptr(), q.data_ptr(), k.data_ptr(),
+                                                        v.data_ptr(), out.data_ptr(), lse.data_ptr(),
+                                                        _ptr(key_lengths), _ptr(key_mask), dq.data_ptr(),
+                                                        dk.data_ptr(), dv.data_ptr(), _ptr(ws), nbytes,
+                                                        current_stream_handle()), "cross_attention_backward")
     return dq, dk, dv
 
 
@@ -349,8 +388,8 @@ def _dropout_into(x, p, seed, subsequence, residual, y) -> None:
     """Launches rdv_dropout into y."""
     x = x.contiguous()
     residual = None if residual is None else residual.contiguous()
-    _lib.check(_lib.load().rdv_dropout(x.data_ptr(), _ptr(residual), y.data_ptr(), x.numel(), _DTYPES[x.dtype], p,
-                                       seed, subsequence, current_stream_handle()), "dropout")
+    _check(_lib.load().rdv_dropout(x.data_ptr(), _ptr(residual), y.data_ptr(), x.numel(), _DTYPES[x.dtype], p, seed,
+                                   subsequence, current_stream_handle()), "dropout")
 
 
 def dropout(x, p: float, seed: int, subsequence: int = 0, residual=None, out=None):
@@ -364,7 +403,7 @@ def dropout(x, p: float, seed: int, subsequence: int = 0, residual=None, out=Non
     x, p, seed, subsequence = _dropout_inputs(x, p, seed, subsequence)
     if residual is not None:
         residual = _like(residual, x, "residual")
-    _on_gpu((x, "x"), (residual, "residual"))
+    _on_gpu(x, "x", residual, "residual")
     y = _out_tensor(out, x.shape, x.dtype, x.device, aligned=False)
     if out is not None:
         for t, what in ((x, "x"), (residual, "residual")):

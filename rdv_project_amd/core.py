@@ -16,7 +16,6 @@ Device memory is PyTorch-ROCm's (one GPU, torch's current device and stream).
 """
 from __future__ import annotations
 
-import contextlib
 import enum
 import time as _time
 import weakref
@@ -61,19 +60,26 @@ def device() -> torch.device:
 
 
 def current_stream_handle() -> int:
-    return torch.cuda.current_stream().cuda_stream
+    """The current stream's handle, without making a torch.cuda.Stream of it (3.5 us of a call's host time)."""
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
 
 
-@contextlib.contextmanager
-def launch_scope():
+class launch_scope:
     """Wraps one logical dispatch: optional wait + profiling, as `dispatch` does."""
-    global __submit_times__
-    t0 = _time.perf_counter() if __PROFILING__ else 0.0
-    yield
-    if __SYNCHRONOUS__:
-        torch.cuda.current_stream().synchronize()
-    if __PROFILING__:
-        __submit_times__ += _time.perf_counter() - t0
+
+    __slots__ = ("_t0",)
+
+    def __enter__(self) -> None:
+        self._t0 = _time.perf_counter() if __PROFILING__ else 0.0
+
+    def __exit__(self, error, *_) -> None:
+        global __submit_times__
+        if error is not None:
+            return
+        if __SYNCHRONOUS__:
+            torch.cuda.current_stream().synchronize()
+        if __PROFILING__:
+            __submit_times__ += _time.perf_counter() - self._t0
 
 
 def _as_device_tensor(data) -> torch.Tensor:

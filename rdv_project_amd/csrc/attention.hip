@@ -98,32 +98,46 @@ __global__ __launch_bounds__(256) void attn_pack_kernel(const T* x, T* y, int64_
   }
 }
 
-// Joins the forward splits of one row per wave: weights 2^(top_i - top).
+// Joins the forward splits of a row with weights 2^(top_i - top): one block of 4 waves per row, the splits spread over
+// groups of lanes that hold 4 dimensions each, so that a row's loads are all in flight together.
 template <class T>
 __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
-  const int lane = int(threadIdx.x) & 63;
-  const int64_t n = int64_t(a.batch) * a.kv_heads * a.rows, row = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
-  if (row >= n) return;
+  __shared__ __attribute__((aligned(16))) float sums[8][RDV_ATTENTION_MAX_DIM];
+  __shared__ float totals[8];
+  const int64_t n = int64_t(a.batch) * a.kv_heads * a.rows, row = blockIdx.x;
+  const int l = int(threadIdx.x) & 31, g = int(threadIdx.x) >> 5;
   float top = -INFINITY;
-  for (int s = 0; s < a.splits; ++s) top = fmaxf(top, a.part_ml[s * n + row].x);
+  for (int s = l; s < a.splits; s += 32) top = fmaxf(top, a.part_ml[s * n + row].x);
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
   const float ref = top == -INFINITY ? 0.0f : top;
-  float total = 0.0f, o0 = 0.0f, o1 = 0.0f;
-  for (int s = 0; s < a.splits; ++s) {
+  float total = 0.0f;
+  f32x4 o4{};
+  for (int s = g; s < a.splits; s += 8) {
     const float2 m = a.part_ml[s * n + row];
-    if (m.y == 0.0f) continue;  // no state of this split counts: its partial row is not written
+    f32x4 v{};
+    if (m.y != 0.0f && 4 * l < a.pdim)  // else no state of this split counts: its partial row is not written
+      v = *reinterpret_cast<const f32x4*>(a.part + (s * n + row) * a.pdim + 4 * l);
     const float w = __builtin_amdgcn_exp2f(m.x - ref);
     total += m.y * w;
-    const float* const p = a.part + (s * n + row) * a.pdim;
-    if (lane < a.pdim) o0 += w * p[lane];
-    if (lane + 64 < a.pdim) o1 += w * p[lane + 64];
+    o4 += v * w;
+  }
+  if (l == 0) totals[g] = total;
+  *reinterpret_cast<f32x4*>(&sums[g][4 * l]) = o4;
+  __syncthreads();
+  if (g != 0) return;
+  total = 0.0f;
+  o4 = f32x4{};
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    total += totals[i];
+    o4 += *reinterpret_cast<const f32x4*>(&sums[i][4 * l]);
   }
   const float inv = total > 0.0f ? 1.0f / total : (total == 0.0f ? 0.0f : total);
   const int bh = int(row / a.rows), r = int(row - int64_t(bh) * a.rows), item = bh / a.kv_heads;
   const RowAt at = row_at(a, bh - item * a.kv_heads, r);
   T* const out = static_cast<T*>(a.out) + ((int64_t(item) * a.queries + at.query) * a.heads + at.head) * a.odim;
-  if (lane < a.odim) out[lane] = T(o0 * inv);
-  if (lane + 64 < a.odim) out[lane + 64] = T(o1 * inv);
-  if (a.lse && lane == 0) a.lse[row] = total == 0.0f ? -INFINITY : (top + __builtin_amdgcn_logf(total)) * kLn2;
+  store_quad(out, 4 * l, a.odim, o4[0] * inv, o4[1] * inv, o4[2] * inv, o4[3] * inv);
+  if (a.lse && l == 0) a.lse[row] = total == 0.0f ? -INFINITY : (top + __builtin_amdgcn_logf(total)) * kLn2;
 }
 
 // stats[row] = (lse log2 e, or +inf where no state counts; delta = rowsum(dO O)), 8 lanes per row.
@@ -261,7 +275,7 @@ int launch_attention(const rdv_attention_desc& d, const void* q, const void* k, 
   a.part_ml = reinterpret_cast<float2*>(ws + p.ml);
   rc = launch_matrix(d.dtype, p.few ? kAttnFew : kAttnTile, a, stream);
   if (rc != RDV_OK || a.splits == 1) return rc;
-  const int64_t blocks = (p.bh * p.rows + 3) / 4;
+  const int64_t blocks = p.bh * p.rows;
   if (blocks >= (int64_t(1) << 31)) return fail(RDV_ERR_UNSUPPORTED, "attention: too many rows");
   return with_dtype(d.dtype, [&](auto t) {
     attn_join_kernel<decltype(t)><<<dim3(unsigned(blocks)), 256, 0, stream>>>(a);

@@ -31,19 +31,55 @@ __device__ __forceinline__ void philox4x32(uint64_t block, uint64_t subsequence,
   w[3] = c3;
 }
 
-template <class T>
-__global__ void dropout_kernel(const T* x, const T* residual, T* y, int64_t n, uint64_t threshold, float factor,
-                               uint64_t seed, uint64_t subsequence) {
-  const int64_t block = int64_t(blockIdx.x) * blockDim.x + threadIdx.x;
-  if (4 * block >= n) return;
-  uint32_t w[4];
-  philox4x32(uint64_t(block), subsequence, seed, w);
+// y[i] for i < n, one word each.  VEC: 16-byte pieces of aligned tensors, kPieces per thread, a block apart so that a
+// wave's loads are whole lines; the last, partial piece and unaligned tensors go element by element.
+constexpr int kPieces = 2;
+
+template <class T, bool VEC>
+__global__ __launch_bounds__(256) void dropout_kernel(const T* x, const T* residual, T* y, int64_t n,
+                                                      uint64_t threshold, float factor, uint64_t seed,
+                                                      uint64_t subsequence) {
+  constexpr int E = VEC ? 16 / int(sizeof(T)) : 4;  // elements of a piece
+  typedef T vec __attribute__((ext_vector_type(E)));
+  const int64_t first = (int64_t(blockIdx.x) * kPieces * 256 + threadIdx.x) * E;
+  vec vx[kPieces], vr[kPieces];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int64_t i = 4 * block + j;
-    if (i < n) {
-      const float v = uint64_t(w[j]) >= threshold ? to_f32(x[i]) * factor : 0.0f;
-      y[i] = T(residual ? to_f32(residual[i]) + v : v);
+  for (int k = 0; k < kPieces; ++k) {
+    const int64_t i = first + int64_t(k) * 256 * E;
+    if (VEC && i + E <= n) {
+      vx[k] = *reinterpret_cast<const vec*>(x + i);
+      if (residual) vr[k] = *reinterpret_cast<const vec*>(residual + i);
+    } else {
+#pragma unroll
+      for (int j = 0; j < E; ++j)
+        if (i + j < n) {
+          vx[k][j] = x[i + j];
+          if (residual) vr[k][j] = residual[i + j];
+        }
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < kPieces; ++k) {
+    const int64_t i = first + int64_t(k) * 256 * E;
+    if (i >= n) break;
+    vec out;
+#pragma unroll
+    for (int q = 0; q < E / 4; ++q) {
+      uint32_t w[4];
+      philox4x32(uint64_t(i) / 4 + q, subsequence, seed, w);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int e = 4 * q + j;
+        const float v = uint64_t(w[j]) >= threshold ? to_f32(T(vx[k][e])) * factor : 0.0f;
+        out[e] = T(residual ? to_f32(T(vr[k][e])) + v : v);
+      }
+    }
+    if (VEC && i + E <= n) {
+      *reinterpret_cast<vec*>(y + i) = out;
+    } else {
+#pragma unroll
+      for (int j = 0; j < E; ++j)
+        if (i + j < n) y[i + j] = out[j];
     }
   }
 }
@@ -54,14 +90,16 @@ int launch_dropout(const void* x, const void* residual, void* y, int64_t n, int 
                    uint64_t subsequence, hipStream_t stream) {
   const uint64_t threshold = uint64_t(p * 4294967296.0);
   const float factor = p < 1.0 ? float(1.0 / (1.0 - p)) : 0.0f;
-  const int64_t blocks = ((n + 3) / 4 + 255) / 256;
+  const bool aligned = ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(residual) |
+                         reinterpret_cast<uintptr_t>(y)) & 15) == 0;
+  const int64_t per = int64_t(256) * kPieces * (aligned ? (dtype == RDV_DTYPE_F32 ? 4 : 8) : 4);
+  const int64_t blocks = (n + per - 1) / per;
   if (blocks >= (int64_t(1) << 31)) return fail(RDV_ERR_UNSUPPORTED, "rdv_dropout: n is too large");
   return with_dtype(dtype, [&](auto t) {
     using T = decltype(t);
-    dropout_kernel<T><<<dim3(unsigned(blocks)), 256, 0, stream>>>(static_cast<const T*>(x),
-                                                                  static_cast<const T*>(residual),
-                                                                  static_cast<T*>(y), n, threshold, factor, seed,
-                                                                  subsequence);
+    const auto kernel = aligned ? dropout_kernel<T, true> : dropout_kernel<T, false>;
+    kernel<<<dim3(unsigned(blocks)), 256, 0, stream>>>(static_cast<const T*>(x), static_cast<const T*>(residual),
+                                                       static_cast<T*>(y), n, threshold, factor, seed, subsequence);
     RDV_HIP_TRY(hipGetLastError());
     return int(RDV_OK);
   });

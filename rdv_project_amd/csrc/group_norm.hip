@@ -40,6 +40,7 @@ struct NormArgs {
   int channels, groups, width, act;
   float eps;
   int slab, slabs, pieces, tr;   // channels of a slab, slabs, pieces of a slab's row, rows side by side in a block
+  int wave_rows;                 // rows side by side in a wave, 0 where a row's pieces spread over waves
   int chunks, chunk_rows;        // blocks of an image's slab, rows of one
 };
 
@@ -94,8 +95,9 @@ template <int VE>
 __device__ __forceinline__ NormAt norm_at(const NormArgs& a, int64_t image, int slab) {
   NormAt p;
   p.image = image;
-  p.tr = int(threadIdx.x) / a.pieces;
-  p.col = int(threadIdx.x) - p.tr * a.pieces;
+  const int t = a.wave_rows ? int(threadIdx.x) & 63 : int(threadIdx.x), row = t / a.pieces;
+  p.col = t - row * a.pieces;
+  p.tr = a.wave_rows ? (row < a.wave_rows ? int(threadIdx.x >> 6) * a.wave_rows + row : a.tr) : row;
   p.c0 = slab * a.slab;
   p.channels = min(a.slab, a.channels - p.c0);
   p.groups = p.channels / a.width;
@@ -104,27 +106,44 @@ __device__ __forceinline__ NormAt norm_at(const NormArgs& a, int64_t image, int 
   return p;
 }
 
-// Sums v over the block's tr, per channel of the slab, into red[channel]; every thread takes part, threads without a
-// piece with any value.  red: blockDim.x * VE floats.
+// Sums v over the block's tr, per channel of the slab; channel_sum() then gives a channel's sum.  Every thread takes
+// part, threads without a piece with zeros.  Rows side by side in a wave join by lane moves, waves (or rows, where a
+// row spans waves) through LDS.  red: blockDim.x * VE floats.
 template <int VE>
-__device__ __forceinline__ void sum_rows(const NormArgs& a, const NormAt& p, const float (&v)[VE], float* red) {
-  float* const mine = red + threadIdx.x * VE;
-  __syncthreads();
+__device__ __forceinline__ void sum_rows(const NormArgs& a, const NormAt& p, float (&v)[VE], float* red) {
+  if (a.wave_rows) {
+    const int row = p.tr == a.tr ? 64 : p.tr % a.wave_rows;
+    for (int n = a.wave_rows; n > 1;) {
+      const int half = (n + 1) >> 1;
 #pragma unroll
-  for (int i = 0; i < VE; ++i) mine[i] = v[i];
-  for (int n = a.tr; n > 1;) {
-    const int half = (n + 1) >> 1;
-    __syncthreads();
-    if (p.tr < n - half) {
-#pragma unroll
-      for (int i = 0; i < VE; ++i) mine[i] += mine[half * a.pieces * VE + i];
+      for (int i = 0; i < VE; ++i) {
+        const float t = __shfl_down(v[i], unsigned(half * a.pieces));
+        if (row < n - half) v[i] += t;
+      }
+      n = half;
     }
-    n = half;
+    __syncthreads();
+    if (row == 0) {
+#pragma unroll
+      for (int i = 0; i < VE; ++i) red[(int(threadIdx.x >> 6) * a.pieces + p.col) * VE + i] = v[i];
+    }
+  } else {
+    float* const mine = red + threadIdx.x * VE;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < VE; ++i) mine[i] = v[i];
   }
   __syncthreads();
 }
+template <int VE>
+__device__ __forceinline__ float channel_sum(const NormArgs& a, const float* red, int c) {
+  const int rows = a.wave_rows ? int(blockDim.x >> 6) : a.tr;
+  float s = 0.0f;
+  for (int r = 0; r < rows; ++r) s += red[r * a.pieces * VE + c];
+  return s;
+}
 
-// out[g] = f(sum of per[channel] over the channels of the slab's group g), 16 lanes per group.
+// out[g] = f(sum of per(channel) over the channels of the slab's group g), 16 lanes per group.
 template <class P, class F>
 __device__ __forceinline__ void sum_groups(const NormArgs& a, const NormAt& p, float* out, P per, F f) {
   const int l = int(threadIdx.x) & 15, lanes = int(blockDim.x) >> 4;
@@ -181,8 +200,9 @@ __device__ __forceinline__ void slopes(const NormArgs& a, const Piece<T, VE>& x,
   }
 }
 
-// Runs f(row, piece...) over rows first .. end - 1 of the thread, U at a time with their loads first.
-constexpr int kNormUnroll = 4;
+// Two-launch kernels: rows that a thread loads at a time, and threads of a block.  One block per CU with 1,024 threads
+// keeps 64 KiB of loads in flight on it, and few blocks leave few partial statistics to join.
+constexpr int kNormUnroll = 4, kNormThreads = 1024;
 
 // ------------------------------------------------------------------ one launch
 
@@ -196,7 +216,7 @@ __global__ __launch_bounds__(1024) void norm_whole_kernel(NormArgs a) {
   float* const rstd_g = mean_g + a.slab / a.width;
   const T* const x = static_cast<const T*>(a.x) + p.image * a.x_image + p.c0 + p.channel;
   Piece<T, VE> v[R];
-  float s[VE] = {};
+  float s[VE] = {}, mean[VE], scale[VE], w[VE], b[VE];
 #pragma unroll
   for (int k = 0; k < R; ++k) {
     const int64_t r = p.tr + int64_t(k) * a.tr;
@@ -208,11 +228,10 @@ __global__ __launch_bounds__(1024) void norm_whole_kernel(NormArgs a) {
 #pragma unroll
       for (int i = 0; i < VE; ++i) s[i] += v[k][i];
     }
+  load_affine<VE>(a, p, w, b);
   const float inv = 1.0f / (float(a.rows) * float(a.width));
   sum_rows<VE>(a, p, s, red);
-  sum_groups(a, p, mean_g, [&](int c) { return red[c]; }, [&](float t) { return t * inv; });
-  float mean[VE], scale[VE], w[VE], b[VE];
-  load_affine<VE>(a, p, w, b);
+  sum_groups(a, p, mean_g, [&](int c) { return channel_sum<VE>(a, red, c); }, [&](float t) { return t * inv; });
 #pragma unroll
   for (int i = 0; i < VE; ++i) {
     mean[i] = p.on ? mean_g[(p.channel + i) / a.width] : 0.0f;
@@ -225,7 +244,7 @@ __global__ __launch_bounds__(1024) void norm_whole_kernel(NormArgs a) {
       for (int i = 0; i < VE; ++i) s[i] = fmaf(v[k][i] - mean[i], v[k][i] - mean[i], s[i]);
     }
   sum_rows<VE>(a, p, s, red);
-  sum_groups(a, p, rstd_g, [&](int c) { return red[c]; }, [&](float t) { return 1.0f / sqrtf(t * inv + a.eps); });
+  sum_groups(a, p, rstd_g, [&](int c) { return channel_sum<VE>(a, red, c); }, [&](float t) { return 1.0f / sqrtf(t * inv + a.eps); });
 #pragma unroll
   for (int i = 0; i < VE; ++i) scale[i] = p.on ? w[i] * rstd_g[(p.channel + i) / a.width] : 0.0f;
   T* const y = static_cast<T*>(a.y) + p.image * a.rows * a.channels + p.c0 + p.channel;
@@ -256,16 +275,16 @@ __device__ __forceinline__ void load_stats(const NormArgs& a, const NormAt& p, f
 
 // From the slab's per-channel sums A (in `red`, then B): dx's two means per group, m1 and m2.
 template <int VE>
-__device__ __forceinline__ void join_sums(const NormArgs& a, const NormAt& p, const float (&sa)[VE], const float (&sb)[VE],
+__device__ __forceinline__ void join_sums(const NormArgs& a, const NormAt& p, float (&sa)[VE], float (&sb)[VE],
                                           float* red, float* m1, float* m2, float2* channel_sums) {
   const float inv = 1.0f / (float(a.rows) * float(a.width));
   for (int which = 0; which < 2; ++which) {
     sum_rows<VE>(a, p, which ? sb : sa, red);
     if (channel_sums)
       for (int c = int(threadIdx.x); c < p.channels; c += int(blockDim.x))
-        (which ? channel_sums[p.c0 + c].y : channel_sums[p.c0 + c].x) = red[c];
+        (which ? channel_sums[p.c0 + c].y : channel_sums[p.c0 + c].x) = channel_sum<VE>(a, red, c);
     sum_groups(a, p, which ? m2 : m1,
-               [&](int c) { return red[c] * (a.weight ? a.weight[p.c0 + c] : 1.0f); },
+               [&](int c) { return channel_sum<VE>(a, red, c) * (a.weight ? a.weight[p.c0 + c] : 1.0f); },
                [&](float t) { return t * inv; });
   }
 }
@@ -340,7 +359,7 @@ __device__ __forceinline__ NormChunk norm_chunk(const NormArgs& a, int64_t block
 
 // First launch, forward: a chunk's mean and squared deviations per group.
 template <class T, int VE>
-__global__ __launch_bounds__(256) void norm_stats_kernel(NormArgs a) {
+__global__ __launch_bounds__(kNormThreads) void norm_stats_kernel(NormArgs a) {
   extern __shared__ float norm_lds[];
   constexpr int U = kNormUnroll;
   const NormChunk ch = norm_chunk(a, blockIdx.x);
@@ -390,14 +409,14 @@ __global__ __launch_bounds__(256) void norm_stats_kernel(NormArgs a) {
   }
   const float count = float(ch.end - ch.first) * float(a.width);
   sum_rows<VE>(a, p, q, red);
-  sum_groups(a, p, mean_g, [&](int c) { return red[c]; }, [&](float t) { return t / count; });
+  sum_groups(a, p, mean_g, [&](int c) { return channel_sum<VE>(a, red, c); }, [&](float t) { return t / count; });
 #pragma unroll
   for (int i = 0; i < VE; ++i) {
     const float d = p.on ? mean[i] - mean_g[(p.channel + i) / a.width] : 0.0f;
     q[i] = fmaxf(s2[i] - s1[i] * s1[i] * inv, 0.0f) + fn * d * d;
   }
   sum_rows<VE>(a, p, q, red);
-  sum_groups(a, p, dev_g, [&](int c) { return red[c]; }, [&](float t) { return t; });
+  sum_groups(a, p, dev_g, [&](int c) { return channel_sum<VE>(a, red, c); }, [&](float t) { return t; });
   float2* const part = a.parts + (p.image * a.groups + p.c0 / a.width) * a.chunks + ch.chunk;
   for (int g = int(threadIdx.x); g < p.groups; g += int(blockDim.x))
     part[int64_t(g) * a.chunks] = float2{mean_g[g], dev_g[g]};
@@ -405,7 +424,7 @@ __global__ __launch_bounds__(256) void norm_stats_kernel(NormArgs a) {
 
 // Second launch, forward: the chunks' statistics joined, 16 lanes per group, and the rows normalised.
 template <class T, int VE>
-__global__ __launch_bounds__(256) void norm_apply_kernel(NormArgs a) {
+__global__ __launch_bounds__(kNormThreads) void norm_apply_kernel(NormArgs a) {
   extern __shared__ float norm_lds[];
   constexpr int U = kNormUnroll;
   const NormChunk ch = norm_chunk(a, blockIdx.x);
@@ -416,20 +435,22 @@ __global__ __launch_bounds__(256) void norm_apply_kernel(NormArgs a) {
   float w[VE], b[VE], mean[VE], scale[VE];
   load_affine<VE>(a, p, w, b);
   {
-    const int l = int(threadIdx.x) & 15;
+    int lanes = 16;  // per group
+    while (lanes < 64 && 2 * lanes * p.groups <= int(blockDim.x)) lanes *= 2;
+    const int l = int(threadIdx.x) & (lanes - 1);
     const float total = float(a.rows) * float(a.width);
-    for (int g = int(threadIdx.x) >> 4; g < p.groups; g += int(blockDim.x) >> 4) {
+    for (int g = int(threadIdx.x) / lanes; g < p.groups; g += int(blockDim.x) / lanes) {
       const float2* const part = a.parts + (p.image * a.groups + p.c0 / a.width + g) * a.chunks;
       float s = 0.0f;
-      for (int i = l; i < a.chunks; i += 16) s += part[i].x * float(min(int64_t(a.chunk_rows), a.rows - int64_t(i) * a.chunk_rows));
-      for (int o = 8; o > 0; o >>= 1) s += __shfl_xor(s, o);
+      for (int i = l; i < a.chunks; i += lanes) s += part[i].x * float(min(int64_t(a.chunk_rows), a.rows - int64_t(i) * a.chunk_rows));
+      for (int o = lanes >> 1; o > 0; o >>= 1) s += __shfl_xor(s, o);
       const float m = s / float(a.rows);
       s = 0.0f;
-      for (int i = l; i < a.chunks; i += 16) {
+      for (int i = l; i < a.chunks; i += lanes) {
         const float2 t = part[i];
         s += t.y + (t.x - m) * (t.x - m) * float(min(int64_t(a.chunk_rows), a.rows - int64_t(i) * a.chunk_rows)) * float(a.width);
       }
-      for (int o = 8; o > 0; o >>= 1) s += __shfl_xor(s, o);
+      for (int o = lanes >> 1; o > 0; o >>= 1) s += __shfl_xor(s, o);
       if (l == 0) {
         mean_g[g] = m;
         rstd_g[g] = 1.0f / sqrtf(s / total + a.eps);
@@ -464,7 +485,7 @@ __global__ __launch_bounds__(256) void norm_apply_kernel(NormArgs a) {
 
 // First launch, backward: a chunk's A and B per channel.
 template <class T, int VE>
-__global__ __launch_bounds__(256) void norm_sums_kernel(NormArgs a) {
+__global__ __launch_bounds__(kNormThreads) void norm_sums_kernel(NormArgs a) {
   extern __shared__ float norm_lds[];
   constexpr int U = kNormUnroll;
   const NormChunk ch = norm_chunk(a, blockIdx.x);
@@ -498,7 +519,7 @@ __global__ __launch_bounds__(256) void norm_sums_kernel(NormArgs a) {
   float2* const part = a.parts + (p.image * a.chunks + ch.chunk) * a.channels + p.c0;
   for (int which = 0; which < 2; ++which) {
     sum_rows<VE>(a, p, which ? sb : sa, norm_lds);
-    for (int c = int(threadIdx.x); c < p.channels; c += int(blockDim.x)) (which ? part[c].y : part[c].x) = norm_lds[c];
+    for (int c = int(threadIdx.x); c < p.channels; c += int(blockDim.x)) (which ? part[c].y : part[c].x) = channel_sum<VE>(a, norm_lds, c);
   }
 }
 
@@ -522,7 +543,7 @@ __device__ __forceinline__ void gather_sums(const NormArgs& a, const NormAt& p, 
 // The last launch, backward.  Its first `slabs` blocks sum dweight and dbias over images and chunks; the others join
 // their image's chunks and write dx.
 template <class T, int VE>
-__global__ __launch_bounds__(256) void norm_dx_kernel(NormArgs a) {
+__global__ __launch_bounds__(kNormThreads) void norm_dx_kernel(NormArgs a) {
   extern __shared__ float norm_lds[];
   constexpr int U = kNormUnroll;
   float* const red = norm_lds;
@@ -534,7 +555,7 @@ __global__ __launch_bounds__(256) void norm_dx_kernel(NormArgs a) {
       sum_rows<VE>(a, p, which ? sb : sa, red);
       float* const out = which ? a.dweight : a.dbias;
       if (out)
-        for (int c = int(threadIdx.x); c < p.channels; c += int(blockDim.x)) out[p.c0 + c] = red[c];
+        for (int c = int(threadIdx.x); c < p.channels; c += int(blockDim.x)) out[p.c0 + c] = channel_sum<VE>(a, red, c);
     }
     return;
   }
@@ -700,7 +721,7 @@ __global__ __launch_bounds__(256) void norm_wide_dx_kernel(NormArgs a) {
 
 struct NormPlan {
   enum Kind { kWhole, kChunked, kWide } kind;
-  int ve, slab, slabs, pieces, tr, threads, chunks, chunk_rows;
+  int ve, slab, slabs, pieces, tr, wave_rows, threads, chunks, chunk_rows;
   int64_t bytes;
 };
 
@@ -738,6 +759,12 @@ NormPlan norm_plan(const rdv_group_norm_desc& d, bool backward, int cu, int alig
     p.pieces = p.slab / p.ve;
     p.slabs = (d.channels + p.slab - 1) / p.slab;
   };
+  // rows of up to 32 pieces lie side by side in a wave
+  auto set_threads = [&](int threads) {
+    p.threads = threads;
+    p.wave_rows = p.pieces <= 32 ? 64 / p.pieces : 0;
+    p.tr = p.wave_rows ? threads / 64 * p.wave_rows : threads / p.pieces;
+  };
   // one launch: slabs of at least 64 bytes a row, wider while blocks abound
   const int64_t per_thread = backward ? kWholeBackPieces : kWholePieces;
   int64_t slab = unit;
@@ -748,8 +775,7 @@ NormPlan norm_plan(const rdv_group_norm_desc& d, bool backward, int cu, int alig
            2 * d.rows * p.pieces <= 256 * per_thread)
       set_slab(2 * int64_t(p.slab));
     for (int threads : {256, 512, 1024}) {
-      p.threads = threads;
-      p.tr = threads / p.pieces;
+      set_threads(threads);
       if (d.rows <= p.tr * per_thread) {
         p.kind = NormPlan::kWhole;
         p.chunks = 1;
@@ -758,13 +784,12 @@ NormPlan norm_plan(const rdv_group_norm_desc& d, bool backward, int cu, int alig
       }
     }
   }
-  // two launches: the widest slab, two blocks per CU
+  // two launches: the widest slab, one block per CU
   p.kind = NormPlan::kChunked;
-  p.threads = 256;
   set_slab(int64_t(256) * p.ve / unit * unit);
-  p.tr = 256 / p.pieces;
+  set_threads(kNormThreads);
   const int64_t least = int64_t(p.tr) * kNormUnroll;  // rows that give every thread its first loads
-  int64_t chunks = std::max<int64_t>(1, 2 * int64_t(cu) / std::max<int64_t>(1, d.images * p.slabs));
+  int64_t chunks = std::max<int64_t>(1, int64_t(cu) / std::max<int64_t>(1, d.images * p.slabs));
   chunks = std::min(chunks, (d.rows + least - 1) / least);
   const int64_t rows = (d.rows + chunks - 1) / chunks;
   p.chunk_rows = int((rows + p.tr - 1) / p.tr * p.tr);
@@ -795,6 +820,7 @@ NormArgs norm_args(const rdv_group_norm_desc& d, const NormPlan& p, const void* 
   a.slabs = p.slabs;
   a.pieces = p.pieces;
   a.tr = p.tr;
+  a.wave_rows = p.wave_rows;
   a.chunks = p.chunks;
   a.chunk_rows = p.chunk_rows;
   return a;

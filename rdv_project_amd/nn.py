@@ -605,11 +605,12 @@ class GroupNormTensorOp(TensorOperation):
         super().__init__(shape)
 
     def _inputs(self):
-        return _image_ops._norm_inputs(self.x_buf, self.weight, self.bias, self.groups, self.eps, self.activation)
+        x, weight, bias = _image_ops._norm_inputs(self.x_buf, self.weight, self.bias)
+        return _image_ops._norm_plan(x.shape, x.stride(), None, x.dtype, self.groups, self.eps, self.activation,
+                                     _image_ops._gpu_index()), x, weight, bias
 
     def _forward(self) -> None:
-        x, weight, bias, d = self._inputs()
-        _image_ops._group_norm_into(d, x, weight, bias, self._result_t, None)
+        _image_ops._group_norm_into(*self._inputs(), self._result_t, None)
 
 
 class CrossAttentionTensorOp(TensorOperation):
@@ -642,8 +643,8 @@ class CrossAttentionTensorOp(TensorOperation):
     def _forward(self) -> None:
         q, k, v = (t.as_tensor("torch").unflatten(1, (h, self.D)).unsqueeze(0) for t, h in
                    ((self.q_buf, self.heads), (self.k_buf, self.kv_heads), (self.v_buf, self.kv_heads)))
-        q, k, v, _, _, d = _image_ops._attention_inputs(q, k, v, None, None, None)
-        _image_ops._cross_attention_into(d, q, k, v, None, None, self._result_t, None)
+        q, k, v, _, _, _, plan = _image_ops._attention_inputs(q, k, v, None, None, None)
+        _image_ops._cross_attention_into(plan, q, k, v, None, None, self._result_t, None)
 
 
 class DropoutTensorOp(TensorOperation):
