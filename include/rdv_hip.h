@@ -559,7 +559,7 @@ int rdv_broadcast_rows(const float* value, int32_t width, int64_t rows, float* o
  * var (biased) over an image's rows and a run's channels
  *   y = act(weight[c] (x - mean) / sqrt(var + eps) + bias[c]). */
 typedef struct rdv_group_norm_desc {
-  int64_t images, rows;                    /* >= 0                                          */
+  int64_t images, rows;                    /* 0 .. 2^31 - 2^16 - 1                          */
   int64_t x_image_stride, x_row_stride;    /* of x; a row's channels are contiguous         */
   int64_t g_image_stride, g_row_stride;    /* of grad (backward only)                       */
   int32_t channels, groups;                /* groups divides channels                       */

@@ -204,8 +204,8 @@ struct Staged {
 
 // Blocks run round robin over the 8 XCDs, each with its own L2: every XCD takes a contiguous run of the work, so the
 // blocks that read one (item, state head) share an L2.
-__device__ __forceinline__ int64_t xcd_contiguous(int64_t block, int64_t total) {
-  const int64_t each = total / 8, rest = total % 8, x = block % 8;
+__device__ __forceinline__ uint32_t xcd_contiguous(uint32_t block, uint32_t total) {
+  const uint32_t each = total / 8, rest = total % 8, x = block % 8;
   return x * each + min(x, rest) + block / 8;
 }
 
@@ -213,13 +213,11 @@ struct BlockAt {
   int item, hk, bh, split, tile;
 };
 __device__ __forceinline__ BlockAt block_at(const AttnArgs& a) {
-  const int64_t per = int64_t(a.splits) * a.tiles;
-  const int64_t w = xcd_contiguous(blockIdx.x, int64_t(a.batch) * a.kv_heads * per);
+  const uint32_t w = xcd_contiguous(blockIdx.x, gridDim.x), rest = w / uint32_t(a.tiles);
   BlockAt p;
-  p.bh = int(w / per);
-  const int rest = int(w - p.bh * per);
-  p.split = rest / a.tiles;
-  p.tile = rest - p.split * a.tiles;
+  p.tile = int(w - rest * a.tiles);
+  p.bh = int(rest / uint32_t(a.splits));
+  p.split = int(rest) - p.bh * a.splits;
   p.item = p.bh / a.kv_heads;
   p.hk = p.bh - p.item * a.kv_heads;
   return p;

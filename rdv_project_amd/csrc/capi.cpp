@@ -757,8 +757,9 @@ static bool stride_ok(int64_t s) { return s >= 0 && s < (int64_t(1) << 40); }
 
 static int check_group_norm(const rdv_group_norm_desc* d, bool backward) {
   if (!d) return fail(RDV_ERR_INVALID, "group norm: NULL descriptor");
-  if (d->images < 0 || d->images >= (int64_t(1) << 31) || d->rows < 0 || d->rows >= (int64_t(1) << 31))
-    return fail(RDV_ERR_INVALID, "group norm: images and rows must be in [0, 2^31)");
+  if (d->images < 0 || d->images >= (int64_t(1) << 31) - (1 << 16) || d->rows < 0 ||
+      d->rows >= (int64_t(1) << 31) - (1 << 16))  // row indexes run a block's rows past the last one
+    return fail(RDV_ERR_INVALID, "group norm: images and rows must be in [0, 2^31 - 2^16)");
   if (d->channels < 1 || d->channels > (1 << 20)) return fail(RDV_ERR_INVALID, "group norm: channels must be in [1, 2^20]");
   if (d->groups < 1 || d->channels % d->groups != 0)
     return fail(RDV_ERR_INVALID, "group norm: groups must be >= 1 and divide channels");

@@ -36,11 +36,13 @@ struct NormArgs {
   float* stats;          // [images, groups, 2]: mean, rstd (forward: may be NULL)
   float2* parts;         // forward: [images, groups, chunks] (mean, squared deviations); backward: [images, chunks, channels] (A, B)
   float *dweight, *dbias;
-  int64_t images, rows, x_image, x_row, g_image, g_row;
-  int channels, groups, width, act;
+  int64_t x_image, x_row, g_image, g_row;
+  int images, rows, channels, groups, width, act;
+  uint32_t by_width;             // ceil(2^32 / width): a channel of a slab divides by a product (see group_of)
   float eps;
   int slab, slabs, pieces, tr;   // channels of a slab, slabs, pieces of a slab's row, rows side by side in a block
   int wave_rows;                 // rows side by side in a wave, 0 where a row's pieces spread over waves
+  int red;                       // floats of one statistic of a block's LDS rows (a wave's, or a row's)
   int chunks, chunk_rows;        // blocks of an image's slab, rows of one
 };
 
@@ -86,13 +88,18 @@ __device__ __forceinline__ float norm_act_slope(int act, float z) {
 
 // Where a block and a thread are.
 struct NormAt {
-  int64_t image;
+  int64_t image;  // widened for offsets
   int tr, col, c0, channels, groups;  // the slab's first channel, its channels and groups (the last slab may be shorter)
   int channel;                        // the thread's first channel, within the slab
   bool on;                            // the thread has a piece
 };
+// channel / width: exact while channel width < 2^32, and a slab's width is at most 2,048, channels at most 2^20.
+__device__ __forceinline__ int group_of(const NormArgs& a, int channel) {
+  return a.width == 1 ? channel : int(__umulhi(uint32_t(channel), a.by_width));
+}
+
 template <int VE>
-__device__ __forceinline__ NormAt norm_at(const NormArgs& a, int64_t image, int slab) {
+__device__ __forceinline__ NormAt norm_at(const NormArgs& a, int image, int slab) {
   NormAt p;
   p.image = image;
   const int t = a.wave_rows ? int(threadIdx.x) & 63 : int(threadIdx.x), row = t / a.pieces;
@@ -156,6 +163,69 @@ __device__ __forceinline__ void sum_groups(const NormArgs& a, const NormAt& p, f
   __syncthreads();
 }
 
+// Statistics of the slab's groups over the block from each thread's per-channel mean and squared deviations of n rows:
+// joined in a wave by lane moves, m = (n m + n' m') / (n + n') and d = d + d' + (m - m')^2 n n' / (n + n'), then over
+// LDS rows and channels by 16 lanes per group.  red: 2 a.red + 64 floats; mean_g and dev_g are per group.
+template <int VE, class F>
+__device__ __forceinline__ void group_stats(const NormArgs& a, const NormAt& p, float n, float (&m)[VE], float (&d)[VE],
+                                            float count, float* red, float* mean_g, float* dev_g, F f) {
+  int row = p.tr < a.tr ? p.tr : 64, rows = a.tr;
+  if (a.wave_rows) {
+    const int r = p.tr < a.tr ? p.tr % a.wave_rows : 64;
+    for (int k = a.wave_rows; k > 1;) {
+      const int half = (k + 1) >> 1;
+      const unsigned by = unsigned(half * a.pieces);
+      const float n2 = __shfl_down(n, by);
+      const bool take = r < k - half && n2 > 0.0f;
+      const float sum = n + n2, part = take ? n2 / sum : 0.0f;
+#pragma unroll
+      for (int i = 0; i < VE; ++i) {
+        const float m2 = __shfl_down(m[i], by), d2 = __shfl_down(d[i], by), diff = m2 - m[i];
+        if (take) {
+          m[i] = fmaf(diff, part, m[i]);
+          d[i] += d2 + diff * diff * part * n;
+        }
+      }
+      if (take) n = sum;
+      k = half;
+    }
+    row = r == 0 ? int(threadIdx.x >> 6) : 64;
+    rows = int(blockDim.x >> 6);
+  }
+  float* const dev = red + a.red;
+  float* const counts = dev + a.red;
+  __syncthreads();
+  if (row < rows) {
+    if (p.col == 0) counts[row] = n;
+#pragma unroll
+    for (int i = 0; i < VE; ++i) {
+      red[(row * a.pieces + p.col) * VE + i] = m[i];
+      dev[(row * a.pieces + p.col) * VE + i] = d[i];
+    }
+  }
+  __syncthreads();
+  const int l = int(threadIdx.x) & 15, lanes = int(blockDim.x) >> 4, step = a.pieces * VE;
+  for (int g = int(threadIdx.x) >> 4; g < p.groups; g += lanes) {
+    float s = 0.0f;
+    for (int c = l; c < a.width; c += 16)
+      for (int r = 0; r < rows; ++r) s = fmaf(counts[r], red[r * step + g * a.width + c], s);
+    for (int o = 8; o > 0; o >>= 1) s += __shfl_xor(s, o);
+    const float mean = s / count;
+    s = 0.0f;
+    for (int c = l; c < a.width; c += 16)
+      for (int r = 0; r < rows; ++r) {
+        const float t = red[r * step + g * a.width + c] - mean;
+        s += fmaf(counts[r] * t, t, dev[r * step + g * a.width + c]);
+      }
+    for (int o = 8; o > 0; o >>= 1) s += __shfl_xor(s, o);
+    if (l == 0) {
+      mean_g[g] = mean;
+      dev_g[g] = f(s);
+    }
+  }
+  __syncthreads();
+}
+
 template <int VE>
 __device__ __forceinline__ void load_affine(const NormArgs& a, const NormAt& p, float (&w)[VE], float (&b)[VE]) {
 #pragma unroll
@@ -200,9 +270,10 @@ __device__ __forceinline__ void slopes(const NormArgs& a, const Piece<T, VE>& x,
   }
 }
 
-// Two-launch kernels: rows that a thread loads at a time, and threads of a block.  One block per CU with 1,024 threads
-// keeps 64 KiB of loads in flight on it, and few blocks leave few partial statistics to join.
-constexpr int kNormUnroll = 4, kNormThreads = 1024;
+// Two-launch kernels: rows that a thread loads at a time (the next ones' loads are in flight meanwhile), and threads of
+// a block.  One block per CU keeps 128 KiB of loads in flight on it, and few blocks leave few partial sums to join.  The
+// backward kernels hold two tensors' pieces and six constants per channel: at 1,024 threads they would spill.
+constexpr int kNormUnroll = 4, kNormThreads = 1024, kNormBackThreads = 512;
 
 // ------------------------------------------------------------------ one launch
 
@@ -210,49 +281,51 @@ constexpr int kNormUnroll = 4, kNormThreads = 1024;
 template <class T, int VE, int R>
 __global__ __launch_bounds__(1024) void norm_whole_kernel(NormArgs a) {
   extern __shared__ float norm_lds[];
-  const NormAt p = norm_at<VE>(a, blockIdx.x / a.slabs, int(blockIdx.x % a.slabs));
+  const NormAt p = norm_at<VE>(a, int(blockIdx.x) / a.slabs, int(blockIdx.x) % a.slabs);
   float* const red = norm_lds;
-  float* const mean_g = red + blockDim.x * VE;
+  float* const mean_g = red + 2 * a.red + 64;
   float* const rstd_g = mean_g + a.slab / a.width;
   const T* const x = static_cast<const T*>(a.x) + p.image * a.x_image + p.c0 + p.channel;
   Piece<T, VE> v[R];
-  float s[VE] = {}, mean[VE], scale[VE], w[VE], b[VE];
+  float mean[VE] = {}, dev[VE] = {}, scale[VE], w[VE], b[VE];
+  int n = 0;
 #pragma unroll
   for (int k = 0; k < R; ++k) {
-    const int64_t r = p.tr + int64_t(k) * a.tr;
-    if (p.on && r < a.rows) v[k] = load_piece<T, VE>(x + r * a.x_row);
+    const int r = p.tr + k * a.tr;
+    if (p.on && r < a.rows) {
+      v[k] = load_piece<T, VE>(x + r * a.x_row);
+      ++n;
+    }
   }
+  load_affine<VE>(a, p, w, b);
 #pragma unroll
   for (int k = 0; k < R; ++k)
-    if (p.on && p.tr + int64_t(k) * a.tr < a.rows) {
+    if (k < n) {
 #pragma unroll
-      for (int i = 0; i < VE; ++i) s[i] += v[k][i];
+      for (int i = 0; i < VE; ++i) mean[i] += v[k][i];
     }
-  load_affine<VE>(a, p, w, b);
-  const float inv = 1.0f / (float(a.rows) * float(a.width));
-  sum_rows<VE>(a, p, s, red);
-  sum_groups(a, p, mean_g, [&](int c) { return channel_sum<VE>(a, red, c); }, [&](float t) { return t * inv; });
+  const float fn = float(n), inv = n ? 1.0f / fn : 0.0f;
+#pragma unroll
+  for (int i = 0; i < VE; ++i) mean[i] *= inv;
+#pragma unroll
+  for (int k = 0; k < R; ++k)
+    if (k < n) {
+#pragma unroll
+      for (int i = 0; i < VE; ++i) dev[i] = fmaf(v[k][i] - mean[i], v[k][i] - mean[i], dev[i]);
+    }
+  const float count = float(a.rows) * float(a.width);
+  group_stats<VE>(a, p, fn, mean, dev, count, red, mean_g, rstd_g,
+                  [&](float d) { return 1.0f / sqrtf(d / count + a.eps); });
 #pragma unroll
   for (int i = 0; i < VE; ++i) {
-    mean[i] = p.on ? mean_g[(p.channel + i) / a.width] : 0.0f;
-    s[i] = 0.0f;
+    const int g = p.on ? group_of(a, p.channel + i) : 0;
+    mean[i] = mean_g[g];
+    scale[i] = w[i] * rstd_g[g];
   }
-#pragma unroll
-  for (int k = 0; k < R; ++k)
-    if (p.on && p.tr + int64_t(k) * a.tr < a.rows) {
-#pragma unroll
-      for (int i = 0; i < VE; ++i) s[i] = fmaf(v[k][i] - mean[i], v[k][i] - mean[i], s[i]);
-    }
-  sum_rows<VE>(a, p, s, red);
-  sum_groups(a, p, rstd_g, [&](int c) { return channel_sum<VE>(a, red, c); }, [&](float t) { return 1.0f / sqrtf(t * inv + a.eps); });
-#pragma unroll
-  for (int i = 0; i < VE; ++i) scale[i] = p.on ? w[i] * rstd_g[(p.channel + i) / a.width] : 0.0f;
   T* const y = static_cast<T*>(a.y) + p.image * a.rows * a.channels + p.c0 + p.channel;
 #pragma unroll
-  for (int k = 0; k < R; ++k) {
-    const int64_t r = p.tr + int64_t(k) * a.tr;
-    if (p.on && r < a.rows) normalise<T, VE>(a, v[k], mean, scale, b, y + r * a.channels);
-  }
+  for (int k = 0; k < R; ++k)
+    if (k < n) normalise<T, VE>(a, v[k], mean, scale, b, y + int64_t(p.tr + k * a.tr) * a.channels);
   if (a.stats) {
     float* const st = a.stats + 2 * (p.image * a.groups + p.c0 / a.width);
     for (int g = int(threadIdx.x); g < p.groups; g += int(blockDim.x)) {
@@ -267,7 +340,7 @@ template <int VE>
 __device__ __forceinline__ void load_stats(const NormArgs& a, const NormAt& p, float (&mean)[VE], float (&rstd)[VE]) {
 #pragma unroll
   for (int i = 0; i < VE; ++i) {
-    const int64_t g = p.image * a.groups + (p.on ? (p.c0 + p.channel + i) / a.width : 0);
+    const int64_t g = p.image * a.groups + (p.on ? group_of(a, p.c0) + group_of(a, p.channel + i) : 0);
     mean[i] = a.stats[2 * g];
     rstd[i] = a.stats[2 * g + 1];
   }
@@ -293,7 +366,7 @@ __device__ __forceinline__ void join_sums(const NormArgs& a, const NormAt& p, fl
 template <class T, int VE, int R>
 __global__ __launch_bounds__(1024) void norm_whole_back_kernel(NormArgs a) {
   extern __shared__ float norm_lds[];
-  const NormAt p = norm_at<VE>(a, blockIdx.x / a.slabs, int(blockIdx.x % a.slabs));
+  const NormAt p = norm_at<VE>(a, int(blockIdx.x) / a.slabs, int(blockIdx.x) % a.slabs);
   float* const red = norm_lds;
   float* const m1 = red + blockDim.x * VE;
   float* const m2 = m1 + a.slab / a.width;
@@ -302,7 +375,7 @@ __global__ __launch_bounds__(1024) void norm_whole_back_kernel(NormArgs a) {
   Piece<T, VE> vx[R], vg[R];
 #pragma unroll
   for (int k = 0; k < R; ++k) {
-    const int64_t r = p.tr + int64_t(k) * a.tr;
+    const int r = p.tr + k * a.tr;
     if (p.on && r < a.rows) {
       vx[k] = load_piece<T, VE>(x + r * a.x_row);
       vg[k] = load_piece<T, VE>(g + r * a.g_row);
@@ -313,7 +386,7 @@ __global__ __launch_bounds__(1024) void norm_whole_back_kernel(NormArgs a) {
   load_stats<VE>(a, p, mean, rstd);
 #pragma unroll
   for (int k = 0; k < R; ++k)
-    if (p.on && p.tr + int64_t(k) * a.tr < a.rows) {
+    if (p.on && p.tr + k * a.tr < a.rows) {
       slopes<T, VE>(a, vx[k], vg[k], mean, rstd, w, b, xhat, dz);
 #pragma unroll
       for (int i = 0; i < VE; ++i) {
@@ -326,15 +399,15 @@ __global__ __launch_bounds__(1024) void norm_whole_back_kernel(NormArgs a) {
   T* const dx = static_cast<T*>(a.y) + p.image * a.rows * a.channels + p.c0 + p.channel;
 #pragma unroll
   for (int k = 0; k < R; ++k) {
-    const int64_t r = p.tr + int64_t(k) * a.tr;
+    const int r = p.tr + k * a.tr;
     if (r < a.rows) {
       slopes<T, VE>(a, vx[k], vg[k], mean, rstd, w, b, xhat, dz);
 #pragma unroll
       for (int i = 0; i < VE; ++i) {
-        const int gi = (p.channel + i) / a.width;
+        const int gi = group_of(a, p.channel + i);
         dz[i] = rstd[i] * (w[i] * dz[i] - m1[gi] - xhat[i] * m2[gi]);
       }
-      store_piece<T, VE>(dx + r * a.channels, dz);
+      store_piece<T, VE>(dx + int64_t(r) * a.channels, dz);
     }
   }
 }
@@ -343,18 +416,24 @@ __global__ __launch_bounds__(1024) void norm_whole_back_kernel(NormArgs a) {
 
 // Block (image, slab, chunk) of the two-launch kernels.
 struct NormChunk {
-  int64_t image, first, end;
-  int slab, chunk;
+  int image, first, end, slab, chunk;
 };
-__device__ __forceinline__ NormChunk norm_chunk(const NormArgs& a, int64_t block) {
+__device__ __forceinline__ NormChunk norm_chunk(const NormArgs& a, int block) {
   NormChunk c;
-  c.chunk = int(block % a.chunks);
-  const int64_t rest = block / a.chunks;
-  c.slab = int(rest % a.slabs);
+  const int rest = block / a.chunks;
+  c.chunk = block - rest * a.chunks;
   c.image = rest / a.slabs;
-  c.first = int64_t(c.chunk) * a.chunk_rows;
-  c.end = min(c.first + a.chunk_rows, a.rows);
+  c.slab = rest - c.image * a.slabs;
+  c.first = c.chunk * a.chunk_rows;
+  c.end = c.first + min(a.chunk_rows, a.rows - c.first);
   return c;
+}
+
+// Rows of a thread, U at a time (row r + k tr; rows past the image read its last one, and count for nothing).
+template <class T, int VE, int U>
+__device__ __forceinline__ void load_rows(const NormArgs& a, const T* x, int64_t stride, int r, Piece<T, VE> (&v)[U]) {
+#pragma unroll
+  for (int k = 0; k < U; ++k) v[k] = load_piece<T, VE>(x + min(r + k * a.tr, a.rows - 1) * stride);
 }
 
 // First launch, forward: a chunk's mean and squared deviations per group.
@@ -362,26 +441,29 @@ template <class T, int VE>
 __global__ __launch_bounds__(kNormThreads) void norm_stats_kernel(NormArgs a) {
   extern __shared__ float norm_lds[];
   constexpr int U = kNormUnroll;
-  const NormChunk ch = norm_chunk(a, blockIdx.x);
+  const NormChunk ch = norm_chunk(a, int(blockIdx.x));
   const NormAt p = norm_at<VE>(a, ch.image, ch.slab);
   float* const red = norm_lds;
-  float* const mean_g = red + blockDim.x * VE;
+  float* const mean_g = red + 2 * a.red + 64;
   float* const dev_g = mean_g + a.slab / a.width;
   const T* const x = static_cast<const T*>(a.x) + p.image * a.x_image + p.c0 + p.channel;
   // deviations from the mean of the thread's first U values
   float shift[VE] = {}, s1[VE] = {}, s2[VE] = {};
   int n = 0;
   if (p.on) {
-    for (int64_t r0 = ch.first + p.tr; r0 < ch.end; r0 += int64_t(U) * a.tr) {
-      Piece<T, VE> v[U];
-#pragma unroll
-      for (int k = 0; k < U; ++k) v[k] = load_piece<T, VE>(x + min(r0 + int64_t(k) * a.tr, a.rows - 1) * a.x_row);
+    const int step = U * a.tr;
+    Piece<T, VE> v[U], next[U];
+    int r = ch.first + p.tr;
+    if (r < ch.end) load_rows<T, VE, U>(a, x, a.x_row, r, v);
+    for (; r < ch.end; r += step) {
+      if (r + step < ch.end) load_rows<T, VE, U>(a, x, a.x_row, r + step, next);
       int have = 0;
 #pragma unroll
-      for (int k = 0; k < U; ++k) have += r0 + int64_t(k) * a.tr < ch.end;
+      for (int k = 0; k < U; ++k) have += r + k * a.tr < ch.end;
       if (n == 0) {
 #pragma unroll
         for (int i = 0; i < VE; ++i) {
+#pragma unroll
           for (int k = 0; k < U; ++k)
             if (k < have) shift[i] += v[k][i];
           shift[i] /= float(have);
@@ -398,25 +480,18 @@ __global__ __launch_bounds__(kNormThreads) void norm_stats_kernel(NormArgs a) {
           }
         }
       n += have;
+#pragma unroll
+      for (int k = 0; k < U; ++k) v[k] = next[k];
     }
   }
   const float fn = float(n), inv = n ? 1.0f / fn : 0.0f;
-  float q[VE], mean[VE];
 #pragma unroll
   for (int i = 0; i < VE; ++i) {
-    mean[i] = fmaf(s1[i], inv, shift[i]);
-    q[i] = fn * mean[i];
+    s2[i] = fmaxf(s2[i] - s1[i] * s1[i] * inv, 0.0f);
+    shift[i] = fmaf(s1[i], inv, shift[i]);
   }
-  const float count = float(ch.end - ch.first) * float(a.width);
-  sum_rows<VE>(a, p, q, red);
-  sum_groups(a, p, mean_g, [&](int c) { return channel_sum<VE>(a, red, c); }, [&](float t) { return t / count; });
-#pragma unroll
-  for (int i = 0; i < VE; ++i) {
-    const float d = p.on ? mean[i] - mean_g[(p.channel + i) / a.width] : 0.0f;
-    q[i] = fmaxf(s2[i] - s1[i] * s1[i] * inv, 0.0f) + fn * d * d;
-  }
-  sum_rows<VE>(a, p, q, red);
-  sum_groups(a, p, dev_g, [&](int c) { return channel_sum<VE>(a, red, c); }, [&](float t) { return t; });
+  group_stats<VE>(a, p, fn, shift, s2, float(ch.end - ch.first) * float(a.width), red, mean_g, dev_g,
+                  [](float d) { return d; });
   float2* const part = a.parts + (p.image * a.groups + p.c0 / a.width) * a.chunks + ch.chunk;
   for (int g = int(threadIdx.x); g < p.groups; g += int(blockDim.x))
     part[int64_t(g) * a.chunks] = float2{mean_g[g], dev_g[g]};
@@ -427,12 +502,16 @@ template <class T, int VE>
 __global__ __launch_bounds__(kNormThreads) void norm_apply_kernel(NormArgs a) {
   extern __shared__ float norm_lds[];
   constexpr int U = kNormUnroll;
-  const NormChunk ch = norm_chunk(a, blockIdx.x);
+  const NormChunk ch = norm_chunk(a, int(blockIdx.x));
   const NormAt p = norm_at<VE>(a, ch.image, ch.slab);
   float* const mean_g = norm_lds;
   float* const rstd_g = mean_g + a.slab / a.width;
   const T* const x = static_cast<const T*>(a.x) + p.image * a.x_image + p.c0 + p.channel;
   float w[VE], b[VE], mean[VE], scale[VE];
+  const int step = U * a.tr;
+  int r = ch.first + p.tr;
+  Piece<T, VE> v[U], next[U];
+  if (p.on && r < ch.end) load_rows<T, VE, U>(a, x, a.x_row, r, v);  // in flight while the statistics are joined
   load_affine<VE>(a, p, w, b);
   {
     int lanes = 16;  // per group
@@ -442,13 +521,13 @@ __global__ __launch_bounds__(kNormThreads) void norm_apply_kernel(NormArgs a) {
     for (int g = int(threadIdx.x) / lanes; g < p.groups; g += int(blockDim.x) / lanes) {
       const float2* const part = a.parts + (p.image * a.groups + p.c0 / a.width + g) * a.chunks;
       float s = 0.0f;
-      for (int i = l; i < a.chunks; i += lanes) s += part[i].x * float(min(int64_t(a.chunk_rows), a.rows - int64_t(i) * a.chunk_rows));
+      for (int i = l; i < a.chunks; i += lanes) s += part[i].x * float(min(a.chunk_rows, a.rows - i * a.chunk_rows));
       for (int o = lanes >> 1; o > 0; o >>= 1) s += __shfl_xor(s, o);
       const float m = s / float(a.rows);
       s = 0.0f;
       for (int i = l; i < a.chunks; i += lanes) {
         const float2 t = part[i];
-        s += t.y + (t.x - m) * (t.x - m) * float(min(int64_t(a.chunk_rows), a.rows - int64_t(i) * a.chunk_rows)) * float(a.width);
+        s += t.y + (t.x - m) * (t.x - m) * float(min(a.chunk_rows, a.rows - i * a.chunk_rows)) * float(a.width);
       }
       for (int o = lanes >> 1; o > 0; o >>= 1) s += __shfl_xor(s, o);
       if (l == 0) {
@@ -466,29 +545,28 @@ __global__ __launch_bounds__(kNormThreads) void norm_apply_kernel(NormArgs a) {
   if (!p.on) return;
 #pragma unroll
   for (int i = 0; i < VE; ++i) {
-    const int g = (p.channel + i) / a.width;
+    const int g = group_of(a, p.channel + i);
     mean[i] = mean_g[g];
     scale[i] = w[i] * rstd_g[g];
   }
   T* const y = static_cast<T*>(a.y) + p.image * a.rows * a.channels + p.c0 + p.channel;
-  for (int64_t r0 = ch.first + p.tr; r0 < ch.end; r0 += int64_t(U) * a.tr) {
-    Piece<T, VE> v[U];
-#pragma unroll
-    for (int k = 0; k < U; ++k) v[k] = load_piece<T, VE>(x + min(r0 + int64_t(k) * a.tr, a.rows - 1) * a.x_row);
+  for (; r < ch.end; r += step) {
+    if (r + step < ch.end) load_rows<T, VE, U>(a, x, a.x_row, r + step, next);
 #pragma unroll
     for (int k = 0; k < U; ++k) {
-      const int64_t r = r0 + int64_t(k) * a.tr;
-      if (r < ch.end) normalise<T, VE>(a, v[k], mean, scale, b, y + r * a.channels);
+      const int at = r + k * a.tr;
+      if (at < ch.end) normalise<T, VE>(a, v[k], mean, scale, b, y + int64_t(at) * a.channels);
+      v[k] = next[k];
     }
   }
 }
 
 // First launch, backward: a chunk's A and B per channel.
 template <class T, int VE>
-__global__ __launch_bounds__(kNormThreads) void norm_sums_kernel(NormArgs a) {
+__global__ __launch_bounds__(kNormBackThreads) void norm_sums_kernel(NormArgs a) {
   extern __shared__ float norm_lds[];
   constexpr int U = kNormUnroll;
-  const NormChunk ch = norm_chunk(a, blockIdx.x);
+  const NormChunk ch = norm_chunk(a, int(blockIdx.x));
   const NormAt p = norm_at<VE>(a, ch.image, ch.slab);
   const T* const x = static_cast<const T*>(a.x) + p.image * a.x_image + p.c0 + p.channel;
   const T* const g = static_cast<const T*>(a.grad) + p.image * a.g_image + p.c0 + p.channel;
@@ -496,17 +574,21 @@ __global__ __launch_bounds__(kNormThreads) void norm_sums_kernel(NormArgs a) {
   load_affine<VE>(a, p, w, b);
   load_stats<VE>(a, p, mean, rstd);
   if (p.on) {
-    for (int64_t r0 = ch.first + p.tr; r0 < ch.end; r0 += int64_t(U) * a.tr) {
-      Piece<T, VE> vx[U], vg[U];
-#pragma unroll
-      for (int k = 0; k < U; ++k) {
-        const int64_t r = min(r0 + int64_t(k) * a.tr, a.rows - 1);
-        vx[k] = load_piece<T, VE>(x + r * a.x_row);
-        vg[k] = load_piece<T, VE>(g + r * a.g_row);
+    const int step = U * a.tr;
+    Piece<T, VE> vx[U], vg[U], nx[U], ng[U];
+    int r = ch.first + p.tr;
+    if (r < ch.end) {
+      load_rows<T, VE, U>(a, x, a.x_row, r, vx);
+      load_rows<T, VE, U>(a, g, a.g_row, r, vg);
+    }
+    for (; r < ch.end; r += step) {
+      if (r + step < ch.end) {
+        load_rows<T, VE, U>(a, x, a.x_row, r + step, nx);
+        load_rows<T, VE, U>(a, g, a.g_row, r + step, ng);
       }
 #pragma unroll
-      for (int k = 0; k < U; ++k)
-        if (r0 + int64_t(k) * a.tr < ch.end) {
+      for (int k = 0; k < U; ++k) {
+        if (r + k * a.tr < ch.end) {
           slopes<T, VE>(a, vx[k], vg[k], mean, rstd, w, b, xhat, dz);
 #pragma unroll
           for (int i = 0; i < VE; ++i) {
@@ -514,6 +596,9 @@ __global__ __launch_bounds__(kNormThreads) void norm_sums_kernel(NormArgs a) {
             sb[i] = fmaf(dz[i], xhat[i], sb[i]);
           }
         }
+        vx[k] = nx[k];
+        vg[k] = ng[k];
+      }
     }
   }
   float2* const part = a.parts + (p.image * a.chunks + ch.chunk) * a.channels + p.c0;
@@ -543,14 +628,14 @@ __device__ __forceinline__ void gather_sums(const NormArgs& a, const NormAt& p, 
 // The last launch, backward.  Its first `slabs` blocks sum dweight and dbias over images and chunks; the others join
 // their image's chunks and write dx.
 template <class T, int VE>
-__global__ __launch_bounds__(kNormThreads) void norm_dx_kernel(NormArgs a) {
+__global__ __launch_bounds__(kNormBackThreads) void norm_dx_kernel(NormArgs a) {
   extern __shared__ float norm_lds[];
   constexpr int U = kNormUnroll;
   float* const red = norm_lds;
   float sa[VE], sb[VE];
   if (int(blockIdx.x) < a.slabs) {
     const NormAt p = norm_at<VE>(a, 0, int(blockIdx.x));
-    gather_sums<VE>(a, p, 0, a.images * a.chunks, sa, sb);
+    gather_sums<VE>(a, p, 0, int64_t(a.images) * a.chunks, sa, sb);
     for (int which = 0; which < 2; ++which) {
       sum_rows<VE>(a, p, which ? sb : sa, red);
       float* const out = which ? a.dweight : a.dbias;
@@ -559,41 +644,47 @@ __global__ __launch_bounds__(kNormThreads) void norm_dx_kernel(NormArgs a) {
     }
     return;
   }
-  const NormChunk ch = norm_chunk(a, int64_t(blockIdx.x) - a.slabs);
+  const NormChunk ch = norm_chunk(a, int(blockIdx.x) - a.slabs);
   const NormAt p = norm_at<VE>(a, ch.image, ch.slab);
   float* const m1 = red + blockDim.x * VE;
   float* const m2 = m1 + a.slab / a.width;
-  gather_sums<VE>(a, p, p.image * a.chunks, a.chunks, sa, sb);
-  join_sums<VE>(a, p, sa, sb, red, m1, m2, nullptr);
-  if (!p.on) return;
   const T* const x = static_cast<const T*>(a.x) + p.image * a.x_image + p.c0 + p.channel;
   const T* const g = static_cast<const T*>(a.grad) + p.image * a.g_image + p.c0 + p.channel;
   T* const dx = static_cast<T*>(a.y) + p.image * a.rows * a.channels + p.c0 + p.channel;
+  const int step = U * a.tr;
+  Piece<T, VE> vx[U], vg[U], nx[U], ng[U];
+  int r = ch.first + p.tr;
+  if (p.on && r < ch.end) {  // in flight while the sums are joined
+    load_rows<T, VE, U>(a, x, a.x_row, r, vx);
+    load_rows<T, VE, U>(a, g, a.g_row, r, vg);
+  }
+  gather_sums<VE>(a, p, p.image * a.chunks, a.chunks, sa, sb);
+  join_sums<VE>(a, p, sa, sb, red, m1, m2, nullptr);
+  if (!p.on) return;
   float mean[VE], rstd[VE], w[VE], b[VE], xhat[VE], dz[VE], g1[VE], g2[VE];
   load_affine<VE>(a, p, w, b);
   load_stats<VE>(a, p, mean, rstd);
 #pragma unroll
   for (int i = 0; i < VE; ++i) {
-    g1[i] = m1[(p.channel + i) / a.width];
-    g2[i] = m2[(p.channel + i) / a.width];
+    g1[i] = m1[group_of(a, p.channel + i)];
+    g2[i] = m2[group_of(a, p.channel + i)];
   }
-  for (int64_t r0 = ch.first + p.tr; r0 < ch.end; r0 += int64_t(U) * a.tr) {
-    Piece<T, VE> vx[U], vg[U];
-#pragma unroll
-    for (int k = 0; k < U; ++k) {
-      const int64_t r = min(r0 + int64_t(k) * a.tr, a.rows - 1);
-      vx[k] = load_piece<T, VE>(x + r * a.x_row);
-      vg[k] = load_piece<T, VE>(g + r * a.g_row);
+  for (; r < ch.end; r += step) {
+    if (r + step < ch.end) {
+      load_rows<T, VE, U>(a, x, a.x_row, r + step, nx);
+      load_rows<T, VE, U>(a, g, a.g_row, r + step, ng);
     }
 #pragma unroll
     for (int k = 0; k < U; ++k) {
-      const int64_t r = r0 + int64_t(k) * a.tr;
-      if (r < ch.end) {
+      const int at = r + k * a.tr;
+      if (at < ch.end) {
         slopes<T, VE>(a, vx[k], vg[k], mean, rstd, w, b, xhat, dz);
 #pragma unroll
         for (int i = 0; i < VE; ++i) dz[i] = rstd[i] * (w[i] * dz[i] - g1[i] - xhat[i] * g2[i]);
-        store_piece<T, VE>(dx + r * a.channels, dz);
+        store_piece<T, VE>(dx + int64_t(at) * a.channels, dz);
       }
+      vx[k] = nx[k];
+      vg[k] = ng[k];
     }
   }
 }
@@ -604,7 +695,7 @@ __global__ __launch_bounds__(256) void norm_params_kernel(NormArgs a) {
   const int c = int(blockIdx.x * 16 + (threadIdx.x & 15)), tr = int(threadIdx.x >> 4);
   float2 s{0.0f, 0.0f};
   if (c < a.channels)
-    for (int64_t k = tr; k < a.images * a.chunks; k += 16) {
+    for (int64_t k = tr; k < int64_t(a.images) * a.chunks; k += 16) {
       const float2 t = a.parts[k * a.channels + c];
       s.x += t.x;
       s.y += t.y;
@@ -637,8 +728,8 @@ __device__ __forceinline__ float block_sum(float v, float* scratch) {
 template <class T>
 __global__ __launch_bounds__(256) void norm_wide_kernel(NormArgs a) {
   __shared__ float scratch[4];
-  const int64_t image = blockIdx.x / a.groups;
-  const int group = int(blockIdx.x % a.groups), c0 = group * a.width;
+  const int64_t image = int(blockIdx.x) / a.groups;
+  const int group = int(blockIdx.x) % a.groups, c0 = group * a.width;
   const T* const x = static_cast<const T*>(a.x) + image * a.x_image + c0;
   T* const y = static_cast<T*>(a.y) + image * a.rows * a.channels + c0;
   const float m = float(a.rows) * float(a.width);
@@ -671,8 +762,9 @@ __global__ __launch_bounds__(256) void norm_wide_kernel(NormArgs a) {
 // One thread per (image, channel): A and B.
 template <class T>
 __global__ __launch_bounds__(256) void norm_wide_sums_kernel(NormArgs a) {
-  const int64_t per = (a.channels + 255) / 256, image = blockIdx.x / per;
-  const int c = int(blockIdx.x % per) * 256 + int(threadIdx.x);
+  const int per = (a.channels + 255) / 256;
+  const int64_t image = int(blockIdx.x) / per;
+  const int c = int(blockIdx.x) % per * 256 + int(threadIdx.x);
   if (c >= a.channels) return;
   const T* const x = static_cast<const T*>(a.x) + image * a.x_image + c;
   const T* const g = static_cast<const T*>(a.grad) + image * a.g_image + c;
@@ -692,8 +784,8 @@ __global__ __launch_bounds__(256) void norm_wide_sums_kernel(NormArgs a) {
 template <class T>
 __global__ __launch_bounds__(256) void norm_wide_dx_kernel(NormArgs a) {
   __shared__ float scratch[4];
-  const int64_t image = blockIdx.x / a.groups;
-  const int group = int(blockIdx.x % a.groups), c0 = group * a.width;
+  const int64_t image = int(blockIdx.x) / a.groups;
+  const int group = int(blockIdx.x) % a.groups, c0 = group * a.width;
   const T* const x = static_cast<const T*>(a.x) + image * a.x_image + c0;
   const T* const g = static_cast<const T*>(a.grad) + image * a.g_image + c0;
   T* const dx = static_cast<T*>(a.y) + image * a.rows * a.channels + c0;
@@ -761,8 +853,9 @@ NormPlan norm_plan(const rdv_group_norm_desc& d, bool backward, int cu, int alig
   };
   // rows of up to 32 pieces lie side by side in a wave
   auto set_threads = [&](int threads) {
-    p.threads = threads;
     p.wave_rows = p.pieces <= 32 ? 64 / p.pieces : 0;
+    threads = p.wave_rows ? threads : std::min(threads, 512);  // their sums' LDS rows are one per row, not per wave
+    p.threads = threads;
     p.tr = p.wave_rows ? threads / 64 * p.wave_rows : threads / p.pieces;
   };
   // one launch: slabs of at least 64 bytes a row, wider while blocks abound
@@ -787,7 +880,7 @@ NormPlan norm_plan(const rdv_group_norm_desc& d, bool backward, int cu, int alig
   // two launches: the widest slab, one block per CU
   p.kind = NormPlan::kChunked;
   set_slab(int64_t(256) * p.ve / unit * unit);
-  set_threads(kNormThreads);
+  set_threads(backward ? kNormBackThreads : kNormThreads);
   const int64_t least = int64_t(p.tr) * kNormUnroll;  // rows that give every thread its first loads
   int64_t chunks = std::max<int64_t>(1, int64_t(cu) / std::max<int64_t>(1, d.images * p.slabs));
   chunks = std::min(chunks, (d.rows + least - 1) / least);
@@ -805,8 +898,8 @@ NormArgs norm_args(const rdv_group_norm_desc& d, const NormPlan& p, const void* 
   a.weight = weight;
   a.bias = bias;
   a.parts = static_cast<float2*>(ws);
-  a.images = d.images;
-  a.rows = d.rows;
+  a.images = int(d.images);
+  a.rows = int(d.rows);
   a.x_image = d.x_image_stride;
   a.x_row = d.x_row_stride;
   a.g_image = d.g_image_stride;
@@ -814,6 +907,7 @@ NormArgs norm_args(const rdv_group_norm_desc& d, const NormPlan& p, const void* 
   a.channels = d.channels;
   a.groups = d.groups;
   a.width = d.channels / d.groups;
+  a.by_width = a.width > 1 ? uint32_t(((uint64_t(1) << 32) + a.width - 1) / a.width) : 0;
   a.act = d.act;
   a.eps = d.eps;
   a.slab = p.slab;
@@ -821,6 +915,7 @@ NormArgs norm_args(const rdv_group_norm_desc& d, const NormPlan& p, const void* 
   a.pieces = p.pieces;
   a.tr = p.tr;
   a.wave_rows = p.wave_rows;
+  a.red = (p.wave_rows ? p.threads / 64 : p.tr) * p.slab;
   a.chunks = p.chunks;
   a.chunk_rows = p.chunk_rows;
   return a;
@@ -876,7 +971,7 @@ int launch_group_norm(const rdv_group_norm_desc& d, const void* x, const float* 
   }
   const int64_t blocks = d.images * p.slabs * p.chunks;
   if (int rc = check_blocks(blocks)) return rc;
-  const unsigned lds = unsigned(p.threads * p.ve + 2 * (p.slab / a.width)) * 4;
+  const unsigned lds = unsigned(2 * a.red + 64 + 2 * (p.slab / a.width)) * 4;
   return with_piece(d.dtype, p.ve, [&](auto t, auto ve) {
     using T = decltype(t);
     constexpr int VE = decltype(ve)::value;
