@@ -429,11 +429,11 @@ struct AttnFew {
   using G = AttnTile<T, NC>;
   static constexpr int kTile = 32 * G::kRow;
   static constexpr int kJoin = 32 * (G::ND * 32 + 4) * 4;  // bytes of a wave's columns
-  static constexpr int kLds = 4 * (kTile > kJoin ? kTile : kJoin);
+  static constexpr int kLds = 4 * kTile > 2 * kJoin ? 4 * kTile : 2 * kJoin;
 };
 
 template <class T, int NC>
-__global__ __launch_bounds__(256) void attn_few_kernel(AttnArgs a) {
+__global__ __launch_bounds__(256, NC * sizeof(T) > 16 ? 1 : 2) void attn_few_kernel(AttnArgs a) {
   using G = AttnTile<T, NC>;
   using F = AttnFew<T, NC>;
   constexpr int ND = G::ND;
@@ -460,19 +460,29 @@ __global__ __launch_bounds__(256) void attn_few_kernel(AttnArgs a) {
   sm.clear();
   const int begin = p.split * a.chunk, limit = key_limit(a, p.item);
   const int end = min(begin + a.chunk, limit);
-  for (int first = begin + 32 * wave; first < end; first += 128) {
-    Staged<T, NC, 32, 64> sv;
-    typename Elem<T>::frag kf[NC];
+  // A tile's K and V registers take the next tile's loads as soon as they are read: K after its products, V once it is
+  // in LDS.  Past the end the last state's row is read again, for nothing.
+  int first = begin + 32 * wave;
+  Staged<T, NC, 32, 64> sv;
+  typename Elem<T>::frag kf[NC];
+  uint32_t bits = 0;
+  if (first < end) {
     load_frags<T, NC>(k + int64_t(min(first + n32, end - 1)) * a.ks[1], a.dim, h, kf);
     sv.load(v, a.vs[1], first, end - 1, a.dim, lane);
-    const uint32_t bits = uint32_t(key_bits<32>(a, p.item, first, end, lane));
-    if (!bits) continue;
+    bits = uint32_t(key_bits<32>(a, p.item, first, end, lane));
+  }
+  for (; first < end; first += 128) {
+    const uint32_t now = bits;
     f32x16 s[1] = {f32x16{}};
 #pragma unroll
     for (int e = 0; e < NC; ++e) s[0] = mma(kf[e], qf[e], s[0]);
-    if (bits != ~uint32_t(0)) mask_result(s[0], bits, h, -INFINITY);
+    load_frags<T, NC>(k + int64_t(min(first + 128 + n32, end - 1)) * a.ks[1], a.dim, h, kf);
+    sv.store(mine, now, lane);
+    sv.load(v, a.vs[1], first + 128, end - 1, a.dim, lane);
+    bits = uint32_t(key_bits<32>(a, p.item, first + 128, end, lane));
+    if (!now) continue;
+    if (now != ~uint32_t(0)) mask_result(s[0], now, h, -INFINITY);
     sm.take(s, c);
-    sv.store(mine, bits, lane);
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
@@ -494,30 +504,33 @@ __global__ __launch_bounds__(256) void attn_few_kernel(AttnArgs a) {
 #pragma unroll
   for (int w = 0; w < 4; ++w) sum += ml[w][n32].y * __builtin_amdgcn_exp2f(ml[w][n32].x - ref);
   const float weight = __builtin_amdgcn_exp2f(sm.top - ref);
-  float* const col = reinterpret_cast<float*>(few_lds + wave * F::kJoin) + n32 * (ND * 32 + 4);
 #pragma unroll
-  for (int d = 0; d < ND; ++d)
+  for (int d = 0; d < ND; ++d) sm.o[d] *= weight;
+  for (int n = 2; n > 0; n >>= 1) {  // waves n .. 2 n - 1 hand theirs to waves 0 .. n - 1
+    float* const col = reinterpret_cast<float*>(few_lds + (wave & (n - 1)) * F::kJoin) + n32 * (ND * 32 + 4) + 4 * h;
+    if (wave >= n && wave < 2 * n) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      *reinterpret_cast<f32x4*>(col + 32 * d + 8 * j + 4 * h) =
-          f32x4{sm.o[d][4 * j] * weight, sm.o[d][4 * j + 1] * weight, sm.o[d][4 * j + 2] * weight,
-                sm.o[d][4 * j + 3] * weight};
-  __syncthreads();
+      for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          *reinterpret_cast<f32x4*>(col + 32 * d + 8 * j) =
+              f32x4{sm.o[d][4 * j], sm.o[d][4 * j + 1], sm.o[d][4 * j + 2], sm.o[d][4 * j + 3]};
+    }
+    __syncthreads();
+    if (wave < n) {
+#pragma unroll
+      for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const f32x4 x = *reinterpret_cast<const f32x4*>(col + 32 * d + 8 * j);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) sm.o[d][4 * j + i] += x[i];
+        }
+    }
+    __syncthreads();
+  }
   if (wave != 0) return;
   sm.top = top;
-#pragma unroll
-  for (int d = 0; d < ND; ++d)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      f32x4 x{};
-#pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        const f32x4 y = *reinterpret_cast<const f32x4*>(few_lds + w * F::kJoin + (n32 * (ND * 32 + 4) + 32 * d + 8 * j + 4 * h) * 4);
-        x += y;
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) sm.o[d][4 * j + i] = x[i];
-    }
   finish_row<T, ND>(a, p, n32, sm, sum, h);
 }
 

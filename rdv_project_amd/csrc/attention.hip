@@ -98,40 +98,46 @@ __global__ __launch_bounds__(256) void attn_pack_kernel(const T* x, T* y, int64_
   }
 }
 
-// Joins the forward splits of a row with weights 2^(top_i - top): one block of 4 waves per row, the splits spread over
-// groups of lanes that hold 4 dimensions each, so that a row's loads are all in flight together.
+// Joins the forward splits of each row with weights 2^(top_i - top).  32 lanes hold a row's dimensions, 4 each; `per`
+// such groups of a block (1, 2, 4 or 8) share a row's splits, so that few rows of many splits have their loads in
+// flight together and many rows of few splits fill a block.
 template <class T>
-__global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
+__global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a, int per) {
   __shared__ __attribute__((aligned(16))) float sums[8][RDV_ATTENTION_MAX_DIM];
   __shared__ float totals[8];
-  const int64_t n = int64_t(a.batch) * a.kv_heads * a.rows, row = blockIdx.x;
-  const int l = int(threadIdx.x) & 31, g = int(threadIdx.x) >> 5;
+  const int64_t n = int64_t(a.batch) * a.kv_heads * a.rows;
+  const int l = int(threadIdx.x) & 31, g = int(threadIdx.x) >> 5, part = g % per;
+  const int64_t row = int64_t(blockIdx.x) * (8 / per) + g / per;
+  const bool on = row < n;
   float top = -INFINITY;
-  for (int s = l; s < a.splits; s += 32) top = fmaxf(top, a.part_ml[s * n + row].x);
+  if (on)
+    for (int s = l; s < a.splits; s += 32) top = fmaxf(top, a.part_ml[s * n + row].x);
   for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
   const float ref = top == -INFINITY ? 0.0f : top;
   float total = 0.0f;
   f32x4 o4{};
-  for (int s = g; s < a.splits; s += 8) {
-    const float2 m = a.part_ml[s * n + row];
-    f32x4 v{};
-    if (m.y != 0.0f && 4 * l < a.pdim)  // else no state of this split counts: its partial row is not written
-      v = *reinterpret_cast<const f32x4*>(a.part + (s * n + row) * a.pdim + 4 * l);
-    const float w = __builtin_amdgcn_exp2f(m.x - ref);
-    total += m.y * w;
-    o4 += v * w;
+  if (on) {
+    for (int s = part; s < a.splits; s += per) {
+      const float2 m = a.part_ml[s * n + row];
+      f32x4 v{};
+      if (m.y != 0.0f && 4 * l < a.pdim)  // else no state of this split counts: its partial row is not written
+        v = *reinterpret_cast<const f32x4*>(a.part + (s * n + row) * a.pdim + 4 * l);
+      const float w = __builtin_amdgcn_exp2f(m.x - ref);
+      total += m.y * w;
+      o4 += v * w;
+    }
   }
-  if (l == 0) totals[g] = total;
-  *reinterpret_cast<f32x4*>(&sums[g][4 * l]) = o4;
-  __syncthreads();
-  if (g != 0) return;
-  total = 0.0f;
-  o4 = f32x4{};
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    total += totals[i];
-    o4 += *reinterpret_cast<const f32x4*>(&sums[i][4 * l]);
+  if (per > 1) {
+    if (l == 0) totals[g] = total;
+    *reinterpret_cast<f32x4*>(&sums[g][4 * l]) = o4;
+    __syncthreads();
+    if (part != 0) return;
+    for (int i = 1; i < per; ++i) {
+      total += totals[g + i];
+      o4 += *reinterpret_cast<const f32x4*>(&sums[g + i][4 * l]);
+    }
   }
+  if (!on) return;
   const float inv = total > 0.0f ? 1.0f / total : (total == 0.0f ? 0.0f : total);
   const int bh = int(row / a.rows), r = int(row - int64_t(bh) * a.rows), item = bh / a.kv_heads;
   const RowAt at = row_at(a, bh - item * a.kv_heads, r);
@@ -275,10 +281,12 @@ int launch_attention(const rdv_attention_desc& d, const void* q, const void* k, 
   a.part_ml = reinterpret_cast<float2*>(ws + p.ml);
   rc = launch_matrix(d.dtype, p.few ? kAttnFew : kAttnTile, a, stream);
   if (rc != RDV_OK || a.splits == 1) return rc;
-  const int64_t blocks = p.bh * p.rows;
+  int per = 1;
+  while (per < 8 && 4 * per < a.splits) per *= 2;
+  const int64_t blocks = (p.bh * p.rows + 8 / per - 1) / (8 / per);
   if (blocks >= (int64_t(1) << 31)) return fail(RDV_ERR_UNSUPPORTED, "attention: too many rows");
   return with_dtype(d.dtype, [&](auto t) {
-    attn_join_kernel<decltype(t)><<<dim3(unsigned(blocks)), 256, 0, stream>>>(a);
+    attn_join_kernel<decltype(t)><<<dim3(unsigned(blocks)), 256, 0, stream>>>(a, per);
     RDV_HIP_TRY(hipGetLastError());
     return int(RDV_OK);
   });

@@ -346,23 +346,29 @@ __device__ __forceinline__ void load_stats(const NormArgs& a, const NormAt& p, f
   }
 }
 
-// From the slab's per-channel sums A (in `red`, then B): dx's two means per group, m1 and m2.
+// dx's two means per group, m1 and m2, from the threads' sums A and B; with `keep` the channels' sums are stored too.
 template <int VE>
 __device__ __forceinline__ void join_sums(const NormArgs& a, const NormAt& p, float (&sa)[VE], float (&sb)[VE],
-                                          float* red, float* m1, float* m2, float2* channel_sums) {
+                                          float* red, float* m1, float* m2, bool keep) {
   const float inv = 1.0f / (float(a.rows) * float(a.width));
   for (int which = 0; which < 2; ++which) {
     sum_rows<VE>(a, p, which ? sb : sa, red);
-    if (channel_sums)
-      for (int c = int(threadIdx.x); c < p.channels; c += int(blockDim.x))
-        (which ? channel_sums[p.c0 + c].y : channel_sums[p.c0 + c].x) = channel_sum<VE>(a, red, c);
+    if (keep) {  // an only image's sums are the parameters' gradients
+      float* const param = which ? a.dweight : a.dbias;
+      float2* const part = a.parts + p.image * a.channels + p.c0;
+      for (int c = int(threadIdx.x); c < p.channels; c += int(blockDim.x)) {
+        const float s = channel_sum<VE>(a, red, c);
+        if (a.images > 1) (which ? part[c].y : part[c].x) = s;
+        else if (param) param[p.c0 + c] = s;
+      }
+    }
     sum_groups(a, p, which ? m2 : m1,
                [&](int c) { return channel_sum<VE>(a, red, c) * (a.weight ? a.weight[p.c0 + c] : 1.0f); },
                [&](float t) { return t * inv; });
   }
 }
 
-// The same for the gradients; per-channel sums go to `parts` as one chunk's.
+// The same for the gradients.
 template <class T, int VE, int R>
 __global__ __launch_bounds__(1024) void norm_whole_back_kernel(NormArgs a) {
   extern __shared__ float norm_lds[];
@@ -394,7 +400,7 @@ __global__ __launch_bounds__(1024) void norm_whole_back_kernel(NormArgs a) {
         sb[i] = fmaf(dz[i], xhat[i], sb[i]);
       }
     }
-  join_sums<VE>(a, p, sa, sb, red, m1, m2, a.parts + p.image * a.channels);
+  join_sums<VE>(a, p, sa, sb, red, m1, m2, true);
   if (!p.on) return;
   T* const dx = static_cast<T*>(a.y) + p.image * a.rows * a.channels + p.c0 + p.channel;
 #pragma unroll
@@ -659,7 +665,7 @@ __global__ __launch_bounds__(kNormBackThreads) void norm_dx_kernel(NormArgs a) {
     load_rows<T, VE, U>(a, g, a.g_row, r, vg);
   }
   gather_sums<VE>(a, p, p.image * a.chunks, a.chunks, sa, sb);
-  join_sums<VE>(a, p, sa, sb, red, m1, m2, nullptr);
+  join_sums<VE>(a, p, sa, sb, red, m1, m2, false);
   if (!p.on) return;
   float mean[VE], rstd[VE], w[VE], b[VE], xhat[VE], dz[VE], g1[VE], g2[VE];
   load_affine<VE>(a, p, w, b);
@@ -832,7 +838,9 @@ int piece_elements(const rdv_group_norm_desc& d, bool backward, int align) {
   return ve;
 }
 
-constexpr int kWholePieces = 8, kWholeBackPieces = 4;
+// Pieces per thread of the one-launch kernels, at most: what 128 registers hold without spills (constants and sums are
+// per channel, and the backward kernel holds two tensors).  Where 4 do, the kernel with 4 runs.
+constexpr int whole_pieces(bool backward, int ve) { return backward ? (ve == 8 ? 4 : 8) : (ve == 8 ? 8 : 16); }
 
 NormPlan norm_plan(const rdv_group_norm_desc& d, bool backward, int cu, int align) {
   NormPlan p{};
@@ -858,18 +866,22 @@ NormPlan norm_plan(const rdv_group_norm_desc& d, bool backward, int cu, int alig
     p.threads = threads;
     p.tr = p.wave_rows ? threads / 64 * p.wave_rows : threads / p.pieces;
   };
-  // one launch: slabs of at least 64 bytes a row, wider while blocks abound
-  const int64_t per_thread = backward ? kWholeBackPieces : kWholePieces;
+  // one launch: slabs of at least 32 bytes a row (a small image's slabs are few, and a CU reads each), wider while
+  // blocks abound
+  const int64_t per_thread = whole_pieces(backward, p.ve);
   int64_t slab = unit;
-  while (slab < d.channels && slab * size < 64) slab += unit;
+  while (slab < d.channels && slab * size < 32) slab += unit;
   set_slab(slab);
   if (d.rows * p.pieces <= 1024 * per_thread && p.pieces <= 256) {
-    while (p.slab < d.channels && d.images * p.slabs > 2 * int64_t(cu) && 2 * p.pieces <= 256 &&
-           2 * d.rows * p.pieces <= 256 * per_thread)
+    while (p.slab < d.channels && d.images * p.slabs > int64_t(cu) && 2 * p.pieces <= 256 &&
+           2 * d.rows * p.pieces <= 1024)
       set_slab(2 * int64_t(p.slab));
+    // threads enough for 4 pieces each, or as many as there are
     for (int threads : {256, 512, 1024}) {
       set_threads(threads);
-      if (d.rows <= p.tr * per_thread) {
+      // more than 4 pieces only where the blocks fill the chip: a 3 x 4,081 x 48 fp32 batch in 18 blocks of 8 pieces
+      // took 13.6 us, in two launches 12.5 (backward 22 and 15)
+      if (d.rows <= p.tr * (threads == 1024 && d.images * p.slabs >= cu ? per_thread : 4)) {
         p.kind = NormPlan::kWhole;
         p.chunks = 1;
         p.bytes = backward ? d.images * d.channels * 8 : 0;
@@ -976,7 +988,8 @@ int launch_group_norm(const rdv_group_norm_desc& d, const void* x, const float* 
     using T = decltype(t);
     constexpr int VE = decltype(ve)::value;
     if (p.kind == NormPlan::kWhole) {
-      norm_whole_kernel<T, VE, kWholePieces><<<dim3(unsigned(blocks)), p.threads, lds, stream>>>(a);
+      const auto kernel = d.rows <= 4 * p.tr ? norm_whole_kernel<T, VE, 4> : norm_whole_kernel<T, VE, whole_pieces(false, VE)>;
+      kernel<<<dim3(unsigned(blocks)), p.threads, lds, stream>>>(a);
     } else {
       norm_stats_kernel<T, VE><<<dim3(unsigned(blocks)), p.threads, lds, stream>>>(a);
       norm_apply_kernel<T, VE><<<dim3(unsigned(blocks)), p.threads, unsigned(2 * (p.slab / a.width) * 4), stream>>>(a);
@@ -1020,8 +1033,9 @@ int launch_group_norm_backward(const rdv_group_norm_desc& d, const void* grad, c
     using T = decltype(t);
     constexpr int VE = decltype(ve)::value;
     if (p.kind == NormPlan::kWhole) {
-      norm_whole_back_kernel<T, VE, kWholeBackPieces><<<dim3(unsigned(blocks)), p.threads, lds, stream>>>(a);
-      norm_params_kernel<<<dim3(param_blocks), 256, 0, stream>>>(a);
+      const auto kernel = d.rows <= 4 * p.tr ? norm_whole_back_kernel<T, VE, 4> : norm_whole_back_kernel<T, VE, whole_pieces(true, VE)>;
+      kernel<<<dim3(unsigned(blocks)), p.threads, lds, stream>>>(a);
+      if (d.images > 1) norm_params_kernel<<<dim3(param_blocks), 256, 0, stream>>>(a);
     } else {
       norm_sums_kernel<T, VE><<<dim3(unsigned(blocks - p.slabs)), p.threads, lds, stream>>>(a);
       norm_dx_kernel<T, VE><<<dim3(unsigned(blocks)), p.threads, lds, stream>>>(a);
