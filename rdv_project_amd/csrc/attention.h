@@ -78,38 +78,56 @@ __device__ __forceinline__ f32x16 mma(f32x8 a, f32x8 b, f32x16 c) {
   return c;
 }
 
-// Geometry of a kernel for heads of up to 16 NC dimensions.
+// Geometry of a kernel for heads of up to 16 NC dimensions, and the layout of its LDS tiles: rows of a power of two of
+// bytes whose 16-byte pieces are permuted, piece c of row r at c ^ swizzle(r), so that both kinds of read find different
+// banks (64 of 4 bytes): 16 rows of one piece (row_frag), and 4 rows of 4 neighbouring pieces (col_frag).  With padded
+// rows one of the two conflicted: 29% of the CU cycles at 128 dimensions.
 template <class T, int NC>
 struct AttnTile {
   static constexpr int kPiece = Elem<T>::kPiece;
-  static constexpr int ND = (NC + 1) / 2;                    // 32-wide blocks of the output's dimensions
-  static constexpr int kPieces = NC * 16 / kPiece;           // 16-byte pieces of a row
-  static constexpr int kRow = ND * 32 * int(sizeof(T)) + 16; // bytes of a row in LDS
+  static constexpr int ND = (NC + 1) / 2;                     // 32-wide blocks of the output's dimensions
+  static constexpr int kPieces = NC * 16 / kPiece;            // 16-byte pieces of a row that can hold dimensions
+  static constexpr int kRow = (ND == 3 ? 4 : ND) * 32 * int(sizeof(T));
+  __device__ __forceinline__ static int swizzle(int row) {
+    const int high = kRow >= 256 ? row & 3 : kRow == 128 ? (row >> 1) & 1 : 0;
+    return high << 2 | ((row >> 2) & 3);
+  }
+  __device__ __forceinline__ static int at(int row, int piece) { return row * kRow + ((piece ^ swizzle(row)) << 4); }
 };
 
-// Fragment c of row `row` of a row-major LDS tile.
-template <class T>
-__device__ __forceinline__ typename Elem<T>::frag row_frag(const uint8_t* row, int c, int h) {
-  return *reinterpret_cast<const typename Elem<T>::frag*>(row + (16 * c + 8 * h) * int(sizeof(T)));
+// Fragment c of a row (`row` in the tile; rows 32 apart are permuted alike).
+template <class T, int NC>
+__device__ __forceinline__ typename Elem<T>::frag row_frag(const uint8_t* tile, int row, int c, int h) {
+  using G = AttnTile<T, NC>;
+  if constexpr (sizeof(T) == 2) {
+    return *reinterpret_cast<const typename Elem<T>::frag*>(tile + G::at(row, 2 * c + h));
+  } else {
+    const f32x4 lo = *reinterpret_cast<const f32x4*>(tile + G::at(row, 4 * c + 2 * h));
+    const f32x4 hi = *reinterpret_cast<const f32x4*>(tile + G::at(row, 4 * c + 2 * h + 1));
+    return f32x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+  }
 }
 
-// The fragment whose slot 4 jj + r is the tile's row 16 s + 8 jj + 4 h + r, column 32 db + lane % 32.  `tile` is the
-// tile's first row; for 16-bit types a transposing read hands lane i of 16 column i of a 4 x 16 block, lane i pointing
-// at its 8-byte piece i % 4 of row i / 4.
-template <class T, int ROW>
+// The fragment whose slot 4 jj + r is the tile's row 16 s + 8 jj + 4 h + r, column 32 db + lane % 32.  For 16-bit types
+// a transposing read hands lane i of 16 column i of a 4 x 16 block, lane i pointing at its 8-byte piece i % 4 of row
+// i / 4.
+template <class T, int NC>
 __device__ __forceinline__ typename Elem<T>::frag col_frag(const uint8_t* tile, int s, int db, int lane) {
+  using G = AttnTile<T, NC>;
   const int h = lane >> 5;
   if constexpr (sizeof(T) == 4) {
-    const uint8_t* p = tile + (16 * s + 4 * h) * ROW + (32 * db + (lane & 31)) * 4;
     f32x8 f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = *reinterpret_cast<const float*>(p + (8 * (i >> 2) + (i & 3)) * ROW);
+    for (int i = 0; i < 8; ++i)
+      f[i] = *reinterpret_cast<const float*>(tile + G::at(16 * s + 8 * (i >> 2) + 4 * h + (i & 3), 8 * db + ((lane & 31) >> 2)) +
+                                             (lane & 3) * 4);
     return f;
   } else {
     typedef __attribute__((address_space(3))) s16x4 lds_s4;
-    const uint8_t* p = tile + (16 * s + 4 * h + ((lane & 15) >> 2)) * ROW + (32 * db + (lane & 16) + 4 * (lane & 3)) * 2;
-    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(p));
-    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(p + 8 * ROW));
+    const int row = 16 * s + 4 * h + ((lane & 15) >> 2), piece = 4 * db + ((lane & 16) >> 3) + ((lane & 3) >> 1);
+    const uint8_t* p = tile + (lane & 1) * 8;
+    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(p + G::at(row, piece)));
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(p + G::at(row + 8, piece)));
     return __builtin_bit_cast(typename Elem<T>::frag, s16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]});
   }
 }
@@ -174,19 +192,6 @@ struct Staged {
         piece[i] = *reinterpret_cast<const f32x4*>(base + int64_t(min(first + row, last)) * stride + d);
     }
   }
-  // folded rows (see row_at) instead of evenly spaced ones; rows past `last` are zero
-  __device__ __forceinline__ void load_rows(const AttnArgs& a, const T* base, int64_t row_stride, int64_t head_stride,
-                                            int hk, int first, int tid) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int id = tid + i * THREADS, row = first + id / G::kPieces, d = id % G::kPieces * G::kPiece;
-      piece[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-      if ((kTotal % THREADS == 0 || id < kTotal) && d < a.dim && row < a.rows) {
-        const RowAt at = row_at(a, hk, row);
-        piece[i] = *reinterpret_cast<const f32x4*>(base + at.query * row_stride + at.head * head_stride + d);
-      }
-    }
-  }
   // rows whose bit in `valid` is 0 become zero: what they hold must not reach a product
   __device__ __forceinline__ void store(uint8_t* tile, uint64_t valid, int tid) const {
 #pragma unroll
@@ -196,11 +201,108 @@ struct Staged {
         const bool ok = (valid >> row) & 1;
         f32x4 v = piece[i];
         if (!ok) v = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        *reinterpret_cast<f32x4*>(tile + row * G::kRow + id % G::kPieces * 16) = v;
+        *reinterpret_cast<f32x4*>(tile + G::at(row, id % G::kPieces)) = v;
       }
     }
   }
 };
+
+// Tiles of R rows straight from global memory to LDS (global_load_lds_dwordx4: an instruction of a wave writes the 1 KiB
+// of LDS at M0, lane l its bytes 16 l ..), issued by the 4 waves of a block; no registers hold the data, and the
+// permutation of the layout is in the addresses.  Pieces past dim are not written: clear() makes them zero, once.
+// The compiler does not see these loads: dma_wait() before the barrier that hands a tile over.
+__device__ __attribute__((aligned(16))) const uint32_t g_attn_zero[4] = {0, 0, 0, 0};
+
+__device__ __forceinline__ void dma_wait() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
+template <class T, int NC, int R>
+struct Dma {
+  using G = AttnTile<T, NC>;
+  static constexpr int kBytes = R * G::kRow, kTotal = kBytes / 1024, N = (kTotal + 3) / 4;
+  static_assert(4 * kBytes <= 64 * 1024, "M0 holds 16 bits of an LDS address");
+  uint32_t off[N];  // of the lane's piece from the tile's first row, in bytes
+  bool near;        // offsets fit 32 bits
+  int wave, lane, dim;
+  int64_t stride;   // bytes
+
+  __device__ __forceinline__ int slot(int i) const { return (i * 4 + wave) * 1024 + lane * 16; }
+  __device__ __forceinline__ int row(int i) const { return slot(i) / G::kRow; }
+  __device__ __forceinline__ int piece(int i) const { return ((slot(i) % G::kRow) >> 4) ^ G::swizzle(row(i)); }
+  __device__ __forceinline__ bool on(int i) const {
+    return (kTotal % 4 == 0 || i * 4 + wave < kTotal) && piece(i) * G::kPiece < dim;
+  }
+  __device__ __forceinline__ void init(int64_t row_stride, int dimensions, int w, int l) {
+    wave = w;
+    lane = l;
+    dim = dimensions;
+    stride = row_stride * int(sizeof(T));
+    near = stride * R < (int64_t(1) << 31);
+#pragma unroll
+    for (int i = 0; i < N; ++i) off[i] = uint32_t(row(i)) * uint32_t(stride) + piece(i) * 16;
+  }
+  __device__ __forceinline__ static uint32_t lds_address(const uint8_t* p) {
+    return uint32_t(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const uint8_t*)p));
+  }
+  // R rows from `first` on, evenly spaced; `first` is the same in every lane
+  __device__ __forceinline__ void load(const T* first, const uint8_t* tile) const {
+    const uint32_t lds = lds_address(tile);
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (on(i)) {
+        uint32_t saved;
+        asm volatile(
+            "s_mov_b32 %0, m0\n\t"
+            "s_mov_b32 m0, %3\n\t"
+            "s_nop 0\n\t"
+            "global_load_lds_dwordx4 %1, %2\n\t"
+            "s_mov_b32 m0, %0"
+            : "=&s"(saved)
+            : "v"(off[i]), "s"(first), "s"(__builtin_amdgcn_readfirstlane(lds + (i * 4 + wave) * 1024))
+            : "memory");
+      }
+  }
+  // row r of the tile from row_of(r), zeros where that is NULL
+  template <class F>
+  __device__ __forceinline__ void load_each(F row_of, const uint8_t* tile) const {
+    const uint32_t lds = lds_address(tile);
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (on(i)) {
+        const T* const p = row_of(row(i));
+        const uint8_t* const src = p ? reinterpret_cast<const uint8_t*>(p) + piece(i) * 16
+                                     : reinterpret_cast<const uint8_t*>(g_attn_zero);
+        uint32_t saved;
+        asm volatile(
+            "s_mov_b32 %0, m0\n\t"
+            "s_mov_b32 m0, %2\n\t"
+            "s_nop 0\n\t"
+            "global_load_lds_dwordx4 %1, off\n\t"
+            "s_mov_b32 m0, %0"
+            : "=&s"(saved)
+            : "v"(src), "s"(__builtin_amdgcn_readfirstlane(lds + (i * 4 + wave) * 1024))
+            : "memory");
+      }
+  }
+  // rows first .. first + R - 1 of a tensor at base, those whose bit in `valid` is set
+  __device__ __forceinline__ void load_keys(const T* base, int64_t row_stride, int first, uint64_t valid,
+                                            const uint8_t* tile) const {
+    if (near && valid == all_rows()) {
+      load(base + first * row_stride, tile);
+    } else {
+      load_each([&](int r) { return (valid >> r) & 1 ? base + int64_t(first + r) * row_stride : nullptr; }, tile);
+    }
+  }
+  __device__ __forceinline__ static uint64_t all_rows() { return R == 64 ? ~uint64_t(0) : (uint64_t(1) << (R & 63)) - 1; }
+};
+
+// Zeroes a block's tiles where dim leaves pieces unwritten; followed by a barrier before the first load.
+template <class T, int NC>
+__device__ __forceinline__ void clear_tiles(uint8_t* tiles, int bytes, int dim) {
+  if (dim * int(sizeof(T)) == AttnTile<T, NC>::kRow) return;
+  for (int i = int(threadIdx.x) * 16; i < bytes; i += int(blockDim.x) * 16)
+    *reinterpret_cast<f32x4*>(tiles + i) = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  __syncthreads();
+}
 
 // Blocks run round robin over the 8 XCDs, each with its own L2: every XCD takes a contiguous run of the work, so the
 // blocks that read one (item, state head) share an L2.
@@ -227,17 +329,18 @@ __device__ __forceinline__ int key_limit(const AttnArgs& a, int item) {
   return a.lengths ? min(max(a.lengths[item], 0), a.keys) : a.keys;
 }
 
-// Which of the states first .. first + R - 1 count, as bits; R <= 64.
+// Which of the states first .. first + R - 1 count, as bits (R <= 64): the lane's mask byte, loaded ahead, and the vote.
+__device__ __forceinline__ int key_byte(const AttnArgs& a, int item, int first, int lane) {
+  return a.mask ? a.mask[item * a.ms + min(first + lane, a.keys - 1)] : 1;
+}
 template <int R>
-__device__ __forceinline__ uint64_t key_bits(const AttnArgs& a, int item, int first, int end, int lane) {
-  const int key = first + lane;
-  bool ok = lane < R && key < end;
-  if (a.mask) ok = ok && a.mask[item * a.ms + min(key, a.keys - 1)] != 0;
-  return __ballot(ok);
+__device__ __forceinline__ uint64_t key_bits(int byte, int first, int end, int lane) {
+  return __ballot(lane < R && first + lane < end && byte != 0);
 }
 
 // Results that do not count become -inf: register 4 j + r of half h is the state at bit 8 j + 4 h + r.
 __device__ __forceinline__ void mask_result(f32x16& s, uint32_t bits, int h, float fill) {
+  asm volatile("" ::: "memory");  // or the tests below are hoisted out of the callers' rare branch: 100 instructions
   const uint32_t mine = bits >> (4 * h);
 #pragma unroll
   for (int i = 0; i < 16; ++i) s[i] = (mine >> (8 * (i >> 2) + (i & 3))) & 1 ? s[i] : fill;
@@ -335,13 +438,45 @@ __device__ __forceinline__ void finish_row(const AttnArgs& a, const BlockAt& p, 
   if (a.lse && h == 0) a.lse[row] = total == 0.0f ? -INFINITY : (sm.top + __builtin_amdgcn_logf(total)) * kLn2;
 }
 
-// Many rows: a block of 4 waves, 32 rows each, walks its share of the states in tiles of KT, staged in LDS (two
-// buffers, one barrier per tile: the next tile's loads are in flight under this tile's products).
+// Many rows: a block of 4 waves, 32 rows each, walks its share of the states in tiles of KT in LDS (two buffers, one
+// barrier per tile: the next tile's loads are in flight under this tile's products).
 template <class T>
 constexpr int attn_tile_keys() { return sizeof(T) == 4 ? 32 : 64; }
 
+// The pipeline of the kernels that walk states: body(tile of K, tile of V, bits) per tile, in order.
+template <class T, int NC, int KT, class F>
+__device__ __forceinline__ void walk_keys(const AttnArgs& a, const BlockAt& p, const T* k, const T* v, int begin, int end,
+                                          uint8_t (*tiles)[2][KT * AttnTile<T, NC>::kRow], int wave, int lane, F body) {
+  const int steps = end > begin ? (end - begin + KT - 1) / KT : 0;
+  if (steps == 0) return;
+  clear_tiles<T, NC>(&tiles[0][0][0], 4 * KT * AttnTile<T, NC>::kRow, a.dim);
+  Dma<T, NC, KT> dk, dv;
+  dk.init(a.ks[1], a.dim, wave, lane);
+  dv.init(a.vs[1], a.dim, wave, lane);
+  int byte = key_byte(a, p.item, begin, lane);
+  uint64_t now = key_bits<KT>(byte, begin, end, lane);
+  byte = key_byte(a, p.item, begin + KT, lane);
+  dk.load_keys(k, a.ks[1], begin, now, tiles[0][0]);
+  dv.load_keys(v, a.vs[1], begin, now, tiles[0][1]);
+  dma_wait();
+  __syncthreads();
+  for (int t = 0; t < steps; ++t) {
+    const int next = begin + (t + 1) * KT;
+    const uint64_t then = key_bits<KT>(byte, next, end, lane);
+    if (t + 1 < steps) {
+      dk.load_keys(k, a.ks[1], next, then, tiles[(t + 1) & 1][0]);
+      dv.load_keys(v, a.vs[1], next, then, tiles[(t + 1) & 1][1]);
+      byte = key_byte(a, p.item, next + KT, lane);
+    }
+    if (now) body(tiles[t & 1][0], tiles[t & 1][1], now);
+    now = then;
+    dma_wait();
+    __syncthreads();
+  }
+}
+
 template <class T, int NC>
-__global__ __launch_bounds__(256, 2) void attn_tile_kernel(AttnArgs a) {
+__global__ __launch_bounds__(256, NC * sizeof(T) > 24 ? 1 : 2) void attn_tile_kernel(AttnArgs a) {
   using G = AttnTile<T, NC>;
   constexpr int KT = attn_tile_keys<T>(), SUB = KT / 32, ND = G::ND;
   __shared__ __attribute__((aligned(16))) uint8_t tiles[2][2][KT * G::kRow];
@@ -350,8 +485,6 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(AttnArgs a) {
   const BlockAt p = block_at(a);
   const int row0 = p.tile * 128 + wave * 32, r = row0 + n32;
   const bool active = row0 < a.rows;
-  const T* const k = static_cast<const T*>(a.k) + p.item * a.ks[0] + p.hk * a.ks[2];
-  const T* const v = static_cast<const T*>(a.v) + p.item * a.vs[0] + p.hk * a.vs[2];
   typename Elem<T>::frag qf[NC];
   {
     const RowAt at = row_at(a, p.hk, min(r, a.rows - 1));
@@ -366,58 +499,34 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(AttnArgs a) {
   const float c = fmaxf(fabsf(a.scale) * kLog2e, 1.2e-38f);  // above 0, or a masked result's -inf would become NaN
   Softmax<ND> sm;
   sm.clear();
-
-  const int begin = p.split * a.chunk, limit = key_limit(a, p.item);
-  const int end = min(begin + a.chunk, limit);
-  const int steps = end > begin ? (end - begin + KT - 1) / KT : 0;
-  Staged<T, NC, KT, 256> sk, sv;
-  uint64_t bits = 0;
-  if (steps > 0) {
-    bits = key_bits<KT>(a, p.item, begin, end, lane);
-    sk.load(k, a.ks[1], begin, end - 1, a.dim, tid);
-    sv.load(v, a.vs[1], begin, end - 1, a.dim, tid);
-    sk.store(tiles[0][0], bits, tid);
-    sv.store(tiles[0][1], bits, tid);
-  }
-  for (int t = 0; t < steps; ++t) {
-    __syncthreads();
-    const uint64_t now = bits;
-    if (t + 1 < steps) {
-      const int first = begin + (t + 1) * KT;
-      bits = key_bits<KT>(a, p.item, first, end, lane);
-      sk.load(k, a.ks[1], first, end - 1, a.dim, tid);
-      sv.load(v, a.vs[1], first, end - 1, a.dim, tid);
-    }
-    if (active && now) {
-      const uint8_t* const tk = tiles[t & 1][0];
-      const uint8_t* const tv = tiles[t & 1][1];
-      f32x16 s[SUB];
+  const int begin = p.split * a.chunk, end = min(begin + a.chunk, key_limit(a, p.item));
+  walk_keys<T, NC, KT>(
+      a, p, static_cast<const T*>(a.k) + p.item * a.ks[0] + p.hk * a.ks[2],
+      static_cast<const T*>(a.v) + p.item * a.vs[0] + p.hk * a.vs[2], begin, end, tiles, wave, lane,
+      [&](const uint8_t* tk, const uint8_t* tv, uint64_t now) {
+        if (!active) return;
+        f32x16 s[SUB];
 #pragma unroll
-      for (int u = 0; u < SUB; ++u) {
-        s[u] = f32x16{};
+        for (int u = 0; u < SUB; ++u) s[u] = f32x16{};
 #pragma unroll
-        for (int e = 0; e < NC; ++e) s[u] = mma(row_frag<T>(tk + (32 * u + n32) * G::kRow, e, h), qf[e], s[u]);
-      }
-      if (now != (KT == 64 ? ~uint64_t(0) : (uint64_t(1) << (KT & 63)) - 1)) {
+        for (int e = 0; e < NC; ++e)
 #pragma unroll
-        for (int u = 0; u < SUB; ++u) mask_result(s[u], uint32_t(now >> (32 * u)), h, -INFINITY);
-      }
-      sm.take(s, c);
+          for (int u = 0; u < SUB; ++u) s[u] = mma(row_frag<T, NC>(tk + 32 * u * G::kRow, n32, e, h), qf[e], s[u]);
+        if (now != Dma<T, NC, KT>::all_rows()) {
 #pragma unroll
-      for (int u = 0; u < SUB; ++u)
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const auto pf = result_frag<T>(s[u], half);
-#pragma unroll
-          for (int d = 0; d < ND; ++d)
-            sm.o[d] = mma(col_frag<T, G::kRow>(tv, 2 * u + half, d, lane), pf, sm.o[d]);
+          for (int u = 0; u < SUB; ++u) mask_result(s[u], uint32_t(now >> (32 * u)), h, -INFINITY);
         }
-    }
-    if (t + 1 < steps) {
-      sk.store(tiles[(t + 1) & 1][0], bits, tid);
-      sv.store(tiles[(t + 1) & 1][1], bits, tid);
-    }
-  }
+        sm.take(s, c);
+#pragma unroll
+        for (int u = 0; u < SUB; ++u)
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const auto pf = result_frag<T>(s[u], half);
+#pragma unroll
+            for (int d = 0; d < ND; ++d)
+              sm.o[d] = mma(col_frag<T, NC>(tv + 32 * u * G::kRow, half, d, lane), pf, sm.o[d]);
+          }
+      });
   if (active) finish_row<T, ND>(a, p, r, sm, sm.total + other_half(sm.total), h);
 }
 
@@ -469,7 +578,7 @@ __global__ __launch_bounds__(256, NC * sizeof(T) > 16 ? 1 : 2) void attn_few_ker
   if (first < end) {
     load_frags<T, NC>(k + int64_t(min(first + n32, end - 1)) * a.ks[1], a.dim, h, kf);
     sv.load(v, a.vs[1], first, end - 1, a.dim, lane);
-    bits = uint32_t(key_bits<32>(a, p.item, first, end, lane));
+    bits = uint32_t(key_bits<32>(key_byte(a, p.item, first, lane), first, end, lane));
   }
   for (; first < end; first += 128) {
     const uint32_t now = bits;
@@ -479,7 +588,7 @@ __global__ __launch_bounds__(256, NC * sizeof(T) > 16 ? 1 : 2) void attn_few_ker
     load_frags<T, NC>(k + int64_t(min(first + 128 + n32, end - 1)) * a.ks[1], a.dim, h, kf);
     sv.store(mine, now, lane);
     sv.load(v, a.vs[1], first + 128, end - 1, a.dim, lane);
-    bits = uint32_t(key_bits<32>(a, p.item, first + 128, end, lane));
+    bits = uint32_t(key_bits<32>(key_byte(a, p.item, first + 128, lane), first + 128, end, lane));
     if (!now) continue;
     if (now != ~uint32_t(0)) mask_result(s[0], now, h, -INFINITY);
     sm.take(s, c);
@@ -488,7 +597,7 @@ __global__ __launch_bounds__(256, NC * sizeof(T) > 16 ? 1 : 2) void attn_few_ker
     for (int half = 0; half < 2; ++half) {
       const auto pf = result_frag<T>(s[0], half);
 #pragma unroll
-      for (int d = 0; d < ND; ++d) sm.o[d] = mma(col_frag<T, G::kRow>(mine, half, d, lane), pf, sm.o[d]);
+      for (int d = 0; d < ND; ++d) sm.o[d] = mma(col_frag<T, NC>(mine, half, d, lane), pf, sm.o[d]);
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   }
@@ -572,20 +681,18 @@ __device__ __forceinline__ float fit_terms(f32x16& ds, float& shrink) {
   return 1.0f;
 }
 
-// dQ: a block of 4 waves, 32 rows each (Q and dO fragments in registers), walks its share of the states in tiles of
-// 32: S^T = K Q^T and dP^T = V dO^T from K's and V's rows, dQ^T += K^T dS^T from K's columns.
+// dQ: a block of 4 waves, 32 rows each (Q and dO fragments in registers), walks its share of the states: S^T = K Q^T and
+// dP^T = V dO^T from K's and V's rows, dQ^T += K^T dS^T from K's columns.
 template <class T, int NC>
 __global__ __launch_bounds__(256, NC * sizeof(T) > 16 ? 1 : 2) void attn_dq_kernel(AttnArgs a) {
   using G = AttnTile<T, NC>;
-  constexpr int KT = 32, ND = G::ND;
+  constexpr int KT = attn_tile_keys<T>(), SUB = KT / 32, ND = G::ND;
   __shared__ __attribute__((aligned(16))) uint8_t tiles[2][2][KT * G::kRow];
   const int tid = int(threadIdx.x), lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int h = lane >> 5, n32 = lane & 31;
   const BlockAt p = block_at(a);
   const int row0 = p.tile * 128 + wave * 32, r = row0 + n32;
   const bool active = row0 < a.rows;
-  const T* const k = static_cast<const T*>(a.k) + p.item * a.ks[0] + p.hk * a.ks[2];
-  const T* const v = static_cast<const T*>(a.v) + p.item * a.vs[0] + p.hk * a.vs[2];
   const int rc = min(r, a.rows - 1);
   const RowAt at = row_at(a, p.hk, rc);
   typename Elem<T>::frag qf[NC], gf[NC];
@@ -597,56 +704,38 @@ __global__ __launch_bounds__(256, NC * sizeof(T) > 16 ? 1 : 2) void attn_dq_kern
 #pragma unroll
   for (int d = 0; d < ND; ++d) acc[d] = f32x16{};
   float shrink = 1.0f;
-
   const int begin = p.split * a.chunk, end = min(begin + a.chunk, key_limit(a, p.item));
-  const int steps = end > begin ? (end - begin + KT - 1) / KT : 0;
-  Staged<T, NC, KT, 256> sk, sv;
-  uint64_t bits = 0;
-  if (steps > 0) {
-    bits = key_bits<KT>(a, p.item, begin, end, lane);
-    sk.load(k, a.ks[1], begin, end - 1, a.dim, tid);
-    sv.load(v, a.vs[1], begin, end - 1, a.dim, tid);
-    sk.store(tiles[0][0], bits, tid);
-    sv.store(tiles[0][1], bits, tid);
-  }
-  for (int t = 0; t < steps; ++t) {
-    __syncthreads();
-    const uint32_t now = uint32_t(bits);
-    if (t + 1 < steps) {
-      const int first = begin + (t + 1) * KT;
-      bits = key_bits<KT>(a, p.item, first, end, lane);
-      sk.load(k, a.ks[1], first, end - 1, a.dim, tid);
-      sv.load(v, a.vs[1], first, end - 1, a.dim, tid);
-    }
-    if (active && now) {
-      const uint8_t* const tk = tiles[t & 1][0];
-      const uint8_t* const tv = tiles[t & 1][1];
-      f32x16 s{}, dp{};
+  walk_keys<T, NC, KT>(
+      a, p, static_cast<const T*>(a.k) + p.item * a.ks[0] + p.hk * a.ks[2],
+      static_cast<const T*>(a.v) + p.item * a.vs[0] + p.hk * a.vs[2], begin, end, tiles, wave, lane,
+      [&](const uint8_t* tk, const uint8_t* tv, uint64_t bits) {
+        if (!active) return;
 #pragma unroll
-      for (int e = 0; e < NC; ++e) {
-        s = mma(row_frag<T>(tk + n32 * G::kRow, e, h), qf[e], s);
-        dp = mma(row_frag<T>(tv + n32 * G::kRow, e, h), gf[e], dp);
-      }
+        for (int u = 0; u < SUB; ++u) {
+          const uint32_t now = uint32_t(bits >> (32 * u));
+          f32x16 s{}, dp{};
 #pragma unroll
-      for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], c, -base)) * (dp[i] - delta);
-      if (now != ~uint32_t(0)) mask_result(s, now, h, 0.0f);
-      const float rescale = fit_terms<T>(s, shrink);
-      if (rescale != 1.0f) {
+          for (int e = 0; e < NC; ++e) {
+            s = mma(row_frag<T, NC>(tk + 32 * u * G::kRow, n32, e, h), qf[e], s);
+            dp = mma(row_frag<T, NC>(tv + 32 * u * G::kRow, n32, e, h), gf[e], dp);
+          }
 #pragma unroll
-        for (int d = 0; d < ND; ++d) acc[d] *= rescale;
-      }
+          for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], c, -base)) * (dp[i] - delta);
+          if (now != ~uint32_t(0)) mask_result(s, now, h, 0.0f);
+          const float rescale = fit_terms<T>(s, shrink);
+          if (rescale != 1.0f) {
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const auto sf = result_frag<T>(s, half);
+            for (int d = 0; d < ND; ++d) acc[d] *= rescale;
+          }
 #pragma unroll
-        for (int d = 0; d < ND; ++d) acc[d] = mma(col_frag<T, G::kRow>(tk, half, d, lane), sf, acc[d]);
-      }
-    }
-    if (t + 1 < steps) {
-      sk.store(tiles[(t + 1) & 1][0], bits, tid);
-      sv.store(tiles[(t + 1) & 1][1], bits, tid);
-    }
-  }
+          for (int half = 0; half < 2; ++half) {
+            const auto sf = result_frag<T>(s, half);
+#pragma unroll
+            for (int d = 0; d < ND; ++d)
+              acc[d] = mma(col_frag<T, NC>(tk + 32 * u * G::kRow, half, d, lane), sf, acc[d]);
+          }
+        }
+      });
   if (r >= a.rows) return;
   const float f = a.scale * __builtin_amdgcn_exp2f(-Terms<T>::kLog2) / shrink;
   T* const out = static_cast<T*>(a.dq) + ((int64_t(p.item) * a.queries + at.query) * a.heads + at.head) * a.odim;
@@ -668,9 +757,15 @@ __global__ __launch_bounds__(256, NC * sizeof(T) > 16 ? 1 : 2) void attn_dq_kern
 template <class T, int NC>
 __global__ __launch_bounds__(256, NC * sizeof(T) > 8 ? 1 : 2) void attn_dkv_kernel(AttnArgs a) {
   using G = AttnTile<T, NC>;
-  constexpr int RT = 32, ND = G::ND;
-  __shared__ __attribute__((aligned(16))) uint8_t tiles[2][2][RT * G::kRow];
-  __shared__ __attribute__((aligned(16))) float row_lse[2][RT], row_delta[2][RT];
+  constexpr int RT = attn_tile_keys<T>(), SUB = RT / 32, ND = G::ND;
+  // one variable: the tiles come first, within the 64 KiB that the direct loads reach
+  __shared__ __attribute__((aligned(16))) struct {
+    uint8_t tiles[2][2][RT * G::kRow];
+    float row_lse[2][RT], row_delta[2][RT];
+  } lds;
+  auto& tiles = lds.tiles;
+  auto& row_lse = lds.row_lse;
+  auto& row_delta = lds.row_delta;
   const int tid = int(threadIdx.x), lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int h = lane >> 5, n32 = lane & 31;
   const BlockAt p = block_at(a);
@@ -698,69 +793,86 @@ __global__ __launch_bounds__(256, NC * sizeof(T) > 8 ? 1 : 2) void attn_dkv_kern
 
   const int begin = p.split * a.chunk, end = key0 < limit ? min(begin + a.chunk, a.rows) : begin;
   const int steps = end > begin ? (end - begin + RT - 1) / RT : 0;
-  Staged<T, NC, RT, 256> sq, sg;
+  Dma<T, NC, RT> dq, dg;
+  dq.init(a.qs[1], a.dim, wave, lane);
+  dg.init(a.gs[1], a.dim, wave, lane);
   float2 st{INFINITY, 0.0f};
-  auto load = [&](int first) {
-    sq.load_rows(a, q, a.qs[1], a.qs[2], p.hk, first, tid);
-    sg.load_rows(a, g, a.gs[1], a.gs[2], p.hk, first, tid);
+  auto load = [&](int first, int buf) {
+    const int x = first / a.queries, query = first - x * a.queries, head = p.hk * a.share + x;
+    if (dq.near && dg.near && query + RT <= a.queries) {  // rows of one head
+      dq.load(q + query * a.qs[1] + head * a.qs[2], tiles[buf][0]);
+      dg.load(g + query * a.gs[1] + head * a.gs[2], tiles[buf][1]);
+    } else {
+      auto row_of = [&](const T* t, const int64_t (&s)[3]) {
+        return [&a, &p, first, t, &s](int row) -> const T* {
+          if (first + row >= a.rows) return nullptr;
+          const RowAt at = row_at(a, p.hk, first + row);
+          return t + at.query * s[1] + at.head * s[2];
+        };
+      };
+      dq.load_each(row_of(q, a.qs), tiles[buf][0]);
+      dg.load_each(row_of(g, a.gs), tiles[buf][1]);
+    }
     if (tid < RT) {
       st = float2{INFINITY, 0.0f};
       if (first + tid < a.rows) st = a.stats[int64_t(p.bh) * a.rows + first + tid];
-      st.x -= Terms<T>::kLog2;
     }
   };
-  auto store = [&](int buf) {
-    sq.store(tiles[buf][0], ~uint64_t(0), tid);
-    sg.store(tiles[buf][1], ~uint64_t(0), tid);
+  auto hand_over = [&](int buf) {
     if (tid < RT) {
-      row_lse[buf][tid] = st.x;
+      row_lse[buf][tid] = st.x - Terms<T>::kLog2;
       row_delta[buf][tid] = st.y;
     }
+    dma_wait();
+    __syncthreads();
   };
   if (steps > 0) {
-    load(begin);
-    store(0);
+    clear_tiles<T, NC>(&tiles[0][0][0], 4 * RT * G::kRow, a.dim);
+    load(begin, 0);
+    hand_over(0);
   }
   for (int t = 0; t < steps; ++t) {
-    __syncthreads();
-    if (t + 1 < steps) load(begin + (t + 1) * RT);
+    if (t + 1 < steps) load(begin + (t + 1) * RT, (t + 1) & 1);
     if (active) {
-      const uint8_t* const tq = tiles[t & 1][0];
-      const uint8_t* const tg = tiles[t & 1][1];
-      f32x16 s{}, dp{};
 #pragma unroll
-      for (int e = 0; e < NC; ++e) {
-        s = mma(row_frag<T>(tq + n32 * G::kRow, e, h), kf[e], s);
-        dp = mma(row_frag<T>(tg + n32 * G::kRow, e, h), vf[e], dp);
-      }
+      for (int u = 0; u < SUB; ++u) {
+        const uint8_t* const tq = tiles[t & 1][0] + 32 * u * G::kRow;
+        const uint8_t* const tg = tiles[t & 1][1] + 32 * u * G::kRow;
+        f32x16 s{}, dp{};
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const f32x4 l = *reinterpret_cast<const f32x4*>(&row_lse[t & 1][8 * j + 4 * h]);
-        const f32x4 w = *reinterpret_cast<const f32x4*>(&row_delta[t & 1][8 * j + 4 * h]);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          s[4 * j + i] = __builtin_amdgcn_exp2f(fmaf(s[4 * j + i], c, -l[i]));
-          dp[4 * j + i] = s[4 * j + i] * (dp[4 * j + i] - w[i]);
+        for (int e = 0; e < NC; ++e) {
+          s = mma(row_frag<T, NC>(tq, n32, e, h), kf[e], s);
+          dp = mma(row_frag<T, NC>(tg, n32, e, h), vf[e], dp);
         }
-      }
-      if (!counts) dp = f32x16{};
-      const float rescale = fit_terms<T>(dp, shrink);
-      if (rescale != 1.0f) {
 #pragma unroll
-        for (int d = 0; d < ND; ++d) dk[d] *= rescale;
-      }
+        for (int j = 0; j < 4; ++j) {
+          const f32x4 l = *reinterpret_cast<const f32x4*>(&row_lse[t & 1][32 * u + 8 * j + 4 * h]);
+          const f32x4 w = *reinterpret_cast<const f32x4*>(&row_delta[t & 1][32 * u + 8 * j + 4 * h]);
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const auto pf = result_frag<T>(s, half);
-        const auto sf = result_frag<T>(dp, half);
+          for (int i = 0; i < 4; ++i) {
+            s[4 * j + i] = __builtin_amdgcn_exp2f(fmaf(s[4 * j + i], c, -l[i]));
+            dp[4 * j + i] = s[4 * j + i] * (dp[4 * j + i] - w[i]);
+          }
+        }
+        if (Terms<T>::kLog2 != 0.0f && !counts) dp = f32x16{};
+        const float rescale = fit_terms<T>(dp, shrink);
+        if (rescale != 1.0f) {
 #pragma unroll
-        for (int d = 0; d < ND; ++d) {
-          dv[d] = mma(col_frag<T, G::kRow>(tg, half, d, lane), pf, dv[d]);
-          dk[d] = mma(col_frag<T, G::kRow>(tq, half, d, lane), sf, dk[d]);
+          for (int d = 0; d < ND; ++d) dk[d] *= rescale;
+        }
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const auto pf = result_frag<T>(s, half);
+          const auto sf = result_frag<T>(dp, half);
+#pragma unroll
+          for (int d = 0; d < ND; ++d) {
+            dv[d] = mma(col_frag<T, NC>(tg, half, d, lane), pf, dv[d]);
+            dk[d] = mma(col_frag<T, NC>(tq, half, d, lane), sf, dk[d]);
+          }
         }
       }
     }
-    if (t + 1 < steps) store((t + 1) & 1);
+    hand_over((t + 1) & 1);
   }
   if (key >= a.keys) return;
   const float fv = __builtin_amdgcn_exp2f(-Terms<T>::kLog2), fk = a.scale * fv / shrink;

@@ -75,8 +75,9 @@ Plan make_plan(const rdv_attention_desc& d, bool backward, int cu) {
   } else {
     p.stats = at;
     at += align256(p.bh * p.rows * 8);
-    p.dq = split_axis(p.bh * ((p.rows + 127) / 128), 2 * int64_t(cu), d.keys, 32, 128);
-    p.dkv = split_axis(p.bh * p.key_tiles, 2 * int64_t(cu), p.rows, 32, 128);
+    // a split is a whole number of the kernels' tiles (at most 64): dK and dV's rows end with a tile, not with a split
+    p.dq = split_axis(p.bh * ((p.rows + 127) / 128), 2 * int64_t(cu), d.keys, 64, 128);
+    p.dkv = split_axis(p.bh * p.key_tiles, 2 * int64_t(cu), p.rows, 64, 128);
     const int64_t a = p.dq.count > 1 ? align256(p.dq.count * p.bh * p.rows * p.pdim * 4) : 0;
     const int64_t b = p.dkv.count > 1 ? align256(p.dkv.count * p.bh * d.keys * p.pdim * 4) : 0;
     p.part = at;  // dQ's partials are summed before dK's and dV's are written
