@@ -22,16 +22,16 @@
 namespace rdv {
 
 struct AttnArgs {
-  const void *q, *k, *v, *g, *o;     // rows of `dim` elements, 16-byte aligned (dim a multiple of 16 bytes)
+  const void *q, *k, *v, *g, *o;     // rows of `dim` elements, 16-byte aligned (dim a multiple of 16 bytes); o: out
   const int32_t* lengths;
   const uint8_t* mask;
   void *out, *dq, *dk, *dv;          // contiguous rows of `odim` elements
   float* lse;                        // [batch, heads, queries] = [item, state head][row]
-  float2* stats;                     // backward: (lse log2 e, delta) per [item, state head][row]
+  float2* stats;                     // backward: (lse log2 e, delta) per [item, state head][row], by attn_dq_kernel
   float* part;                       // splits > 1: fp32 results [split][item, state head][row or key][pdim]
   float2* part_ml;                   // forward: (running maximum, log2; sum) per partial row
   float* part2;                      // dV's partials
-  int64_t qs[3], ks[3], vs[3], gs[3], ms;
+  int64_t qs[3], ks[3], vs[3], gs[3], os[3], ms;
   int batch, queries, keys, heads, kv_heads, share, rows, dim, odim, pdim;
   int tiles, splits, chunk;          // blocks: (item, state head) x split x tile; a split's share of the other axis
   float scale;
@@ -438,10 +438,10 @@ __device__ __forceinline__ void finish_row(const AttnArgs& a, const BlockAt& p, 
   if (a.lse && h == 0) a.lse[row] = total == 0.0f ? -INFINITY : (sm.top + __builtin_amdgcn_logf(total)) * kLn2;
 }
 
-// Many rows: a block of 4 waves, 32 rows each, walks its share of the states in tiles of KT in LDS (two buffers, one
-// barrier per tile: the next tile's loads are in flight under this tile's products).
-template <class T>
-constexpr int attn_tile_keys() { return sizeof(T) == 4 ? 32 : 64; }
+// Many rows: a block of 4 waves, 32 rows each (or 64 rows shared by pairs of waves), walks its share of the states in
+// tiles of KT in LDS (two buffers, one barrier per tile: the next tile's loads are in flight under this tile's products).
+template <class T, int NC>
+constexpr int attn_tile_keys() { return sizeof(T) == 4 && NC > 4 ? 32 : 64; }
 
 // The pipeline of the kernels that walk states: body(tile of K, tile of V, bits) per tile, in order.
 template <class T, int NC, int KT, class F>
@@ -475,16 +475,61 @@ __device__ __forceinline__ void walk_keys(const AttnArgs& a, const BlockAt& p, c
   }
 }
 
-template <class T, int NC>
+// Where the 4 waves of a block stand: 4 / WK groups of 32 rows, each shared by WK waves that take every WK-th 32 states
+// of a tile.  WK = 2 makes blocks of 64 rows: twice as many where 128-row blocks would leave CUs idle.
+template <int WK>
+struct WaveAt {
+  int wave, lane, h, n32, wk, row0;
+  __device__ __forceinline__ explicit WaveAt(int tile) {
+    lane = int(threadIdx.x) & 63;
+    wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) >> 6);
+    h = lane >> 5;
+    n32 = lane & 31;
+    wk = wave / (4 / WK);
+    row0 = tile * (128 / WK) + wave % (4 / WK) * 32;
+  }
+};
+
+// Columns of 32 rows' results in LDS: a wave's place in the exchange between the WK = 2 waves of a row group.
+template <int ND>
+struct JoinTile {
+  static constexpr int kCol = ND * 32 + 4, kFloats = 32 * kCol;
+  __device__ __forceinline__ static void put(float* at, const f32x16 (&o)[ND], int n32, int h) {
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        *reinterpret_cast<f32x4*>(at + n32 * kCol + 32 * d + 8 * j + 4 * h) =
+            f32x4{o[d][4 * j], o[d][4 * j + 1], o[d][4 * j + 2], o[d][4 * j + 3]};
+  }
+  // o = o * mine + theirs * other
+  __device__ __forceinline__ static void add(const float* at, f32x16 (&o)[ND], float mine, float other, int n32, int h) {
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const f32x4 x = *reinterpret_cast<const f32x4*>(at + n32 * kCol + 32 * d + 8 * j + 4 * h);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[d][4 * j + i] = fmaf(x[i], other, o[d][4 * j + i] * mine);
+      }
+  }
+};
+
+template <class T, int NC, int WK>
 __global__ __launch_bounds__(256, NC * sizeof(T) > 24 ? 1 : 2) void attn_tile_kernel(AttnArgs a) {
   using G = AttnTile<T, NC>;
-  constexpr int KT = attn_tile_keys<T>(), SUB = KT / 32, ND = G::ND;
-  __shared__ __attribute__((aligned(16))) uint8_t tiles[2][2][KT * G::kRow];
-  const int tid = int(threadIdx.x), lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int h = lane >> 5, n32 = lane & 31;
+  constexpr int KT = attn_tile_keys<T, NC>(), SUB = KT / 32 / WK, ND = G::ND;
+  static_assert(SUB >= 1, "a tile has 32 states for every wave of a row group");
+  // one variable: the tiles come first, within the 64 KiB that the direct loads reach
+  __shared__ __attribute__((aligned(16))) struct {
+    uint8_t tiles[2][2][KT * G::kRow];
+    float2 ml[WK - 1][2][32];
+  } lds;
+  auto& tiles = lds.tiles;
   const BlockAt p = block_at(a);
-  const int row0 = p.tile * 128 + wave * 32, r = row0 + n32;
-  const bool active = row0 < a.rows;
+  const WaveAt<WK> w(p.tile);
+  const int h = w.h, n32 = w.n32, lane = w.lane, r = w.row0 + n32;
+  const bool active = w.row0 < a.rows;
   typename Elem<T>::frag qf[NC];
   {
     const RowAt at = row_at(a, p.hk, min(r, a.rows - 1));
@@ -502,8 +547,14 @@ __global__ __launch_bounds__(256, NC * sizeof(T) > 24 ? 1 : 2) void attn_tile_ke
   const int begin = p.split * a.chunk, end = min(begin + a.chunk, key_limit(a, p.item));
   walk_keys<T, NC, KT>(
       a, p, static_cast<const T*>(a.k) + p.item * a.ks[0] + p.hk * a.ks[2],
-      static_cast<const T*>(a.v) + p.item * a.vs[0] + p.hk * a.vs[2], begin, end, tiles, wave, lane,
+      static_cast<const T*>(a.v) + p.item * a.vs[0] + p.hk * a.vs[2], begin, end, tiles, w.wave, lane,
       [&](const uint8_t* tk, const uint8_t* tv, uint64_t now) {
+        if (WK > 1) {  // this wave's 32 states
+          tk += 32 * w.wk * G::kRow;
+          tv += 32 * w.wk * G::kRow;
+          now = uint32_t(now >> (32 * w.wk));
+          if (!now) return;
+        }
         if (!active) return;
         f32x16 s[SUB];
 #pragma unroll
@@ -512,7 +563,7 @@ __global__ __launch_bounds__(256, NC * sizeof(T) > 24 ? 1 : 2) void attn_tile_ke
         for (int e = 0; e < NC; ++e)
 #pragma unroll
           for (int u = 0; u < SUB; ++u) s[u] = mma(row_frag<T, NC>(tk + 32 * u * G::kRow, n32, e, h), qf[e], s[u]);
-        if (now != Dma<T, NC, KT>::all_rows()) {
+        if (now != (SUB == 2 ? ~uint64_t(0) : uint64_t(~uint32_t(0)))) {
 #pragma unroll
           for (int u = 0; u < SUB; ++u) mask_result(s[u], uint32_t(now >> (32 * u)), h, -INFINITY);
         }
@@ -527,7 +578,26 @@ __global__ __launch_bounds__(256, NC * sizeof(T) > 24 ? 1 : 2) void attn_tile_ke
               sm.o[d] = mma(col_frag<T, NC>(tv + 32 * u * G::kRow, half, d, lane), pf, sm.o[d]);
           }
       });
-  if (active) finish_row<T, ND>(a, p, r, sm, sm.total + other_half(sm.total), h);
+  float total = sm.total + other_half(sm.total);
+  if constexpr (WK > 1) {  // the second wave of a row group hands over its columns, maximum and sum
+    auto& ml = lds.ml[0];
+    float* const at = reinterpret_cast<float*>(&tiles[0][0][0]) + (w.wave & 1) * JoinTile<ND>::kFloats;
+    static_assert(2 * JoinTile<ND>::kFloats * 4 <= int(sizeof(tiles)), "the exchange fits the tiles");
+    __syncthreads();
+    if (w.wk == 1) {
+      JoinTile<ND>::put(at, sm.o, n32, h);
+      if (h == 0) ml[w.wave & 1][n32] = float2{sm.top, total};
+    }
+    __syncthreads();
+    if (w.wk == 1) return;
+    const float2 other = ml[w.wave & 1][n32];
+    const float top = fmaxf(sm.top, other.x), ref = top == -INFINITY ? 0.0f : top;
+    const float mine = __builtin_amdgcn_exp2f(sm.top - ref), theirs = __builtin_amdgcn_exp2f(other.x - ref);
+    JoinTile<ND>::add(at, sm.o, mine, theirs, n32, h);
+    sm.top = top;
+    total = total * mine + other.y * theirs;
+  }
+  if (active) finish_row<T, ND>(a, p, r, sm, total, h);
 }
 
 // At most 32 rows per (item, state head): a single token's heads, or few.  The states are what is read, so the waves
@@ -659,11 +729,12 @@ struct Terms<half_t> {
 
 // dS's factor for a wave's tile: 1 but for fp16.  Returns by how much the accumulators have to be scaled.
 template <class T>
-__device__ __forceinline__ float fit_terms(f32x16& ds, float& shrink) {
+__device__ __forceinline__ float fit_terms(f32x16& ds, float& shrink, bool counts) {
   if constexpr (Terms<T>::kLog2 != 0.0f) {
     float most = 0.0f;
 #pragma unroll
     for (int i = 0; i < 16; ++i) most = fmaxf(most, fabsf(ds[i]));
+    if (!counts) most = 0.0f;  // a column that is not used
     float rescale = 1.0f;
     if (__any(most * shrink > 32768.0f)) {
       for (int o = 32; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor(most, o));
@@ -681,25 +752,40 @@ __device__ __forceinline__ float fit_terms(f32x16& ds, float& shrink) {
   return 1.0f;
 }
 
-// dQ: a block of 4 waves, 32 rows each (Q and dO fragments in registers), walks its share of the states: S^T = K Q^T and
-// dP^T = V dO^T from K's and V's rows, dQ^T += K^T dS^T from K's columns.
-template <class T, int NC>
+// dQ: blocks and waves as attn_tile_kernel's, Q and dO fragments in registers: S^T = K Q^T and dP^T = V dO^T from K's and
+// V's rows, dQ^T += K^T dS^T from K's columns.  A row's delta is summed here and kept, with its lse, for attn_dkv_kernel.
+template <class T, int NC, int WK>
 __global__ __launch_bounds__(256, NC * sizeof(T) > 16 ? 1 : 2) void attn_dq_kernel(AttnArgs a) {
   using G = AttnTile<T, NC>;
-  constexpr int KT = attn_tile_keys<T>(), SUB = KT / 32, ND = G::ND;
-  __shared__ __attribute__((aligned(16))) uint8_t tiles[2][2][KT * G::kRow];
-  const int tid = int(threadIdx.x), lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int h = lane >> 5, n32 = lane & 31;
+  constexpr int KT = attn_tile_keys<T, NC>(), SUB = KT / 32 / WK, ND = G::ND;
+  static_assert(SUB >= 1, "a tile has 32 states for every wave of a row group");
+  __shared__ __attribute__((aligned(16))) struct {
+    uint8_t tiles[2][2][KT * G::kRow];
+    float factor[WK - 1][2];
+  } lds;
+  auto& tiles = lds.tiles;
   const BlockAt p = block_at(a);
-  const int row0 = p.tile * 128 + wave * 32, r = row0 + n32;
-  const bool active = row0 < a.rows;
+  const WaveAt<WK> w(p.tile);
+  const int h = w.h, n32 = w.n32, lane = w.lane, r = w.row0 + n32;
+  const bool active = w.row0 < a.rows;
   const int rc = min(r, a.rows - 1);
   const RowAt at = row_at(a, p.hk, rc);
   typename Elem<T>::frag qf[NC], gf[NC];
   load_frags<T, NC>(static_cast<const T*>(a.q) + p.item * a.qs[0] + at.query * a.qs[1] + at.head * a.qs[2], a.dim, h, qf);
   load_frags<T, NC>(static_cast<const T*>(a.g) + p.item * a.gs[0] + at.query * a.gs[1] + at.head * a.gs[2], a.dim, h, gf);
-  const float2 st = a.stats[int64_t(p.bh) * a.rows + rc];
-  const float c = a.scale * kLog2e, base = st.x - Terms<T>::kLog2, delta = st.y;
+  float lse = a.lse[int64_t(p.bh) * a.rows + rc], delta = 0.0f;
+  {
+    typename Elem<T>::frag of[NC];
+    load_frags<T, NC>(static_cast<const T*>(a.o) + p.item * a.os[0] + at.query * a.os[1] + at.head * a.os[2], a.dim, h, of);
+#pragma unroll
+    for (int e = 0; e < NC; ++e)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) delta = fmaf(to_f32(T(gf[e][i])), to_f32(T(of[e][i])), delta);
+    delta += other_half(delta);
+  }
+  lse = lse == -INFINITY ? INFINITY : lse * kLog2e;  // a row without states: terms of 0
+  if (p.split == 0 && w.wk == 0 && h == 0 && r < a.rows) a.stats[int64_t(p.bh) * a.rows + r] = float2{lse, delta};
+  const float c = a.scale * kLog2e, base = lse - Terms<T>::kLog2;
   f32x16 acc[ND];
 #pragma unroll
   for (int d = 0; d < ND; ++d) acc[d] = f32x16{};
@@ -707,22 +793,25 @@ __global__ __launch_bounds__(256, NC * sizeof(T) > 16 ? 1 : 2) void attn_dq_kern
   const int begin = p.split * a.chunk, end = min(begin + a.chunk, key_limit(a, p.item));
   walk_keys<T, NC, KT>(
       a, p, static_cast<const T*>(a.k) + p.item * a.ks[0] + p.hk * a.ks[2],
-      static_cast<const T*>(a.v) + p.item * a.vs[0] + p.hk * a.vs[2], begin, end, tiles, wave, lane,
+      static_cast<const T*>(a.v) + p.item * a.vs[0] + p.hk * a.vs[2], begin, end, tiles, w.wave, lane,
       [&](const uint8_t* tk, const uint8_t* tv, uint64_t bits) {
         if (!active) return;
 #pragma unroll
         for (int u = 0; u < SUB; ++u) {
-          const uint32_t now = uint32_t(bits >> (32 * u));
+          const int sub = WK > 1 ? w.wk : u;
+          const uint8_t* const uk = tk + 32 * sub * G::kRow;
+          const uint8_t* const uv = tv + 32 * sub * G::kRow;
+          const uint32_t now = uint32_t(bits >> (32 * sub));
           f32x16 s{}, dp{};
 #pragma unroll
           for (int e = 0; e < NC; ++e) {
-            s = mma(row_frag<T, NC>(tk + 32 * u * G::kRow, n32, e, h), qf[e], s);
-            dp = mma(row_frag<T, NC>(tv + 32 * u * G::kRow, n32, e, h), gf[e], dp);
+            s = mma(row_frag<T, NC>(uk, n32, e, h), qf[e], s);
+            dp = mma(row_frag<T, NC>(uv, n32, e, h), gf[e], dp);
           }
 #pragma unroll
           for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], c, -base)) * (dp[i] - delta);
           if (now != ~uint32_t(0)) mask_result(s, now, h, 0.0f);
-          const float rescale = fit_terms<T>(s, shrink);
+          const float rescale = fit_terms<T>(s, shrink, true);
           if (rescale != 1.0f) {
 #pragma unroll
             for (int d = 0; d < ND; ++d) acc[d] *= rescale;
@@ -731,13 +820,26 @@ __global__ __launch_bounds__(256, NC * sizeof(T) > 16 ? 1 : 2) void attn_dq_kern
           for (int half = 0; half < 2; ++half) {
             const auto sf = result_frag<T>(s, half);
 #pragma unroll
-            for (int d = 0; d < ND; ++d)
-              acc[d] = mma(col_frag<T, NC>(tk + 32 * u * G::kRow, half, d, lane), sf, acc[d]);
+            for (int d = 0; d < ND; ++d) acc[d] = mma(col_frag<T, NC>(uk, half, d, lane), sf, acc[d]);
           }
         }
       });
+  float f = a.scale * __builtin_amdgcn_exp2f(-Terms<T>::kLog2) / shrink;
+  if constexpr (WK > 1) {
+    auto& factor = lds.factor[0];
+    float* const place = reinterpret_cast<float*>(&tiles[0][0][0]) + (w.wave & 1) * JoinTile<ND>::kFloats;
+    static_assert(2 * JoinTile<ND>::kFloats * 4 <= int(sizeof(tiles)), "the exchange fits the tiles");
+    __syncthreads();
+    if (w.wk == 1) {
+      JoinTile<ND>::put(place, acc, n32, h);
+      if (lane == 0) factor[w.wave & 1] = f;
+    }
+    __syncthreads();
+    if (w.wk == 1) return;
+    JoinTile<ND>::add(place, acc, f, factor[w.wave & 1], n32, h);
+    f = 1.0f;
+  }
   if (r >= a.rows) return;
-  const float f = a.scale * __builtin_amdgcn_exp2f(-Terms<T>::kLog2) / shrink;
   T* const out = static_cast<T*>(a.dq) + ((int64_t(p.item) * a.queries + at.query) * a.heads + at.head) * a.odim;
   float* const part = a.splits > 1 ? a.part + ((int64_t(p.split) * a.batch * a.kv_heads + p.bh) * a.rows + r) * a.pdim : nullptr;
 #pragma unroll
@@ -757,7 +859,7 @@ __global__ __launch_bounds__(256, NC * sizeof(T) > 16 ? 1 : 2) void attn_dq_kern
 template <class T, int NC>
 __global__ __launch_bounds__(256, NC * sizeof(T) > 8 ? 1 : 2) void attn_dkv_kernel(AttnArgs a) {
   using G = AttnTile<T, NC>;
-  constexpr int RT = attn_tile_keys<T>(), SUB = RT / 32, ND = G::ND;
+  constexpr int RT = attn_tile_keys<T, NC>(), SUB = RT / 32, ND = G::ND;
   // one variable: the tiles come first, within the 64 KiB that the direct loads reach
   __shared__ __attribute__((aligned(16))) struct {
     uint8_t tiles[2][2][RT * G::kRow];
@@ -820,8 +922,8 @@ __global__ __launch_bounds__(256, NC * sizeof(T) > 8 ? 1 : 2) void attn_dkv_kern
   };
   auto hand_over = [&](int buf) {
     if (tid < RT) {
-      row_lse[buf][tid] = st.x - Terms<T>::kLog2;
-      row_delta[buf][tid] = st.y;
+      row_lse[buf][tid] = Terms<T>::kLog2 - st.x;  // both negated, as the sums take them
+      row_delta[buf][tid] = -st.y;
     }
     dma_wait();
     __syncthreads();
@@ -838,7 +940,13 @@ __global__ __launch_bounds__(256, NC * sizeof(T) > 8 ? 1 : 2) void attn_dkv_kern
       for (int u = 0; u < SUB; ++u) {
         const uint8_t* const tq = tiles[t & 1][0] + 32 * u * G::kRow;
         const uint8_t* const tg = tiles[t & 1][1] + 32 * u * G::kRow;
-        f32x16 s{}, dp{};
+        f32x16 s{}, dp;  // dP's sums begin at -delta
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const f32x4 w = *reinterpret_cast<const f32x4*>(&row_delta[t & 1][32 * u + 8 * j + 4 * h]);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) dp[4 * j + i] = w[i];
+        }
 #pragma unroll
         for (int e = 0; e < NC; ++e) {
           s = mma(row_frag<T, NC>(tq, n32, e, h), kf[e], s);
@@ -847,15 +955,13 @@ __global__ __launch_bounds__(256, NC * sizeof(T) > 8 ? 1 : 2) void attn_dkv_kern
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const f32x4 l = *reinterpret_cast<const f32x4*>(&row_lse[t & 1][32 * u + 8 * j + 4 * h]);
-          const f32x4 w = *reinterpret_cast<const f32x4*>(&row_delta[t & 1][32 * u + 8 * j + 4 * h]);
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            s[4 * j + i] = __builtin_amdgcn_exp2f(fmaf(s[4 * j + i], c, -l[i]));
-            dp[4 * j + i] = s[4 * j + i] * (dp[4 * j + i] - w[i]);
+            s[4 * j + i] = __builtin_amdgcn_exp2f(fmaf(s[4 * j + i], c, l[i]));
+            dp[4 * j + i] *= s[4 * j + i];
           }
         }
-        if (Terms<T>::kLog2 != 0.0f && !counts) dp = f32x16{};
-        const float rescale = fit_terms<T>(dp, shrink);
+        const float rescale = fit_terms<T>(dp, shrink, counts);
         if (rescale != 1.0f) {
 #pragma unroll
           for (int d = 0; d < ND; ++d) dk[d] *= rescale;
@@ -899,31 +1005,38 @@ __global__ __launch_bounds__(256, NC * sizeof(T) > 8 ? 1 : 2) void attn_dkv_kern
 
 // ------------------------------------------------------------------ launches by type
 
-enum AttnKernel { kAttnTile, kAttnFew, kAttnDq, kAttnDkv };
+enum AttnKernel { kAttnTile, kAttnTilePairs, kAttnFew, kAttnDq, kAttnDqPairs, kAttnDkv };
 
 template <class T, int NC>
 int launch_attn_nc(AttnKernel which, const AttnArgs& a, unsigned blocks, hipStream_t stream) {
+  constexpr int kPairs = attn_tile_keys<T, NC>() / 32;  // waves that can share a row group
   switch (which) {
-    case kAttnTile: attn_tile_kernel<T, NC><<<blocks, 256, 0, stream>>>(a); break;
+    case kAttnTile: attn_tile_kernel<T, NC, 1><<<blocks, 256, 0, stream>>>(a); break;
+    case kAttnTilePairs: attn_tile_kernel<T, NC, kPairs><<<blocks, 256, 0, stream>>>(a); break;
     case kAttnFew: {
       constexpr int lds = AttnFew<T, NC>::kLds;
-      if constexpr (lds > 64 * 1024)
-        RDV_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(&attn_few_kernel<T, NC>),
-                                        hipFuncAttributeMaxDynamicSharedMemorySize, lds));
+      static_assert(lds <= 64 * 1024, "no attribute needed");
       attn_few_kernel<T, NC><<<blocks, 256, lds, stream>>>(a);
       break;
     }
-    case kAttnDq: attn_dq_kernel<T, NC><<<blocks, 256, 0, stream>>>(a); break;
+    case kAttnDq: attn_dq_kernel<T, NC, 1><<<blocks, 256, 0, stream>>>(a); break;
+    case kAttnDqPairs: attn_dq_kernel<T, NC, kPairs><<<blocks, 256, 0, stream>>>(a); break;
     case kAttnDkv: attn_dkv_kernel<T, NC><<<blocks, 256, 0, stream>>>(a); break;
   }
   RDV_HIP_TRY(hipGetLastError());
   return RDV_OK;
 }
 
+// Whether attn_tile_kernel and attn_dq_kernel come with pairs of waves: not for fp32 heads of more than 64 dimensions,
+// whose tiles hold 32 states.
+inline bool attn_has_pairs(int dtype, int dim) { return dtype != RDV_DTYPE_F32 || dim <= 64; }
+
 template <class T>
 int launch_attn_typed(AttnKernel which, const AttnArgs& a, unsigned blocks, hipStream_t stream) {
   if (a.dim <= 32) return launch_attn_nc<T, 2>(which, a, blocks, stream);
+  if (a.dim <= 48) return launch_attn_nc<T, 3>(which, a, blocks, stream);
   if (a.dim <= 64) return launch_attn_nc<T, 4>(which, a, blocks, stream);
+  if (a.dim <= 80) return launch_attn_nc<T, 5>(which, a, blocks, stream);
   if (a.dim <= 96) return launch_attn_nc<T, 6>(which, a, blocks, stream);
   return launch_attn_nc<T, 8>(which, a, blocks, stream);
 }

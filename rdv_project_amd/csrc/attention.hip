@@ -34,11 +34,11 @@ Split split_axis(int64_t blocks, int64_t want, int length, int step, int least) 
 struct Plan {
   int rows, dim, pdim;            // folded rows; dimensions rounded up to 16 bytes, to 4
   int64_t bh;
-  bool few;
+  bool few, pairs;                // forward: at most 32 rows; forward and dQ: pairs of waves share 32 rows
   Split forward, dq, dkv;
   int row_tiles, key_tiles;
   // byte offsets in the workspace, and its size
-  int64_t packs[4], stats, part, part2, ml, bytes;
+  int64_t packs[5], stats, part, part2, ml, bytes;
 };
 
 Plan make_plan(const rdv_attention_desc& d, bool backward, int cu) {
@@ -49,22 +49,29 @@ Plan make_plan(const rdv_attention_desc& d, bool backward, int cu) {
   p.pdim = (d.dim + 3) / 4 * 4;
   p.bh = int64_t(d.batch) * d.kv_heads;
   p.few = p.rows <= 32;
-  p.row_tiles = p.few ? 1 : (p.rows + 127) / 128;
+  // blocks of 128 rows, or of 64 whose waves share the states in pairs where those would not fill the chip
+  p.pairs = p.bh * ((p.rows + 127) / 128) < cu && d.keys > 32 && attn_has_pairs(d.dtype, d.dim);
+  const int block_rows = p.pairs ? 64 : 128;
+  p.row_tiles = (p.rows + block_rows - 1) / block_rows;
   p.key_tiles = (d.keys + 127) / 128;
   int64_t at = 0;
   // copies of inputs that cannot be read in place
   const int64_t q_rows = int64_t(d.batch) * d.queries * d.heads, k_rows = int64_t(d.batch) * d.keys * d.kv_heads;
-  const int64_t rows[4] = {in_place(d, d.q_stride, d.queries, d.heads) ? 0 : q_rows,
+  const int64_t rows[5] = {in_place(d, d.q_stride, d.queries, d.heads) ? 0 : q_rows,
                            in_place(d, d.k_stride, d.keys, d.kv_heads) ? 0 : k_rows,
                            in_place(d, d.v_stride, d.keys, d.kv_heads) ? 0 : k_rows,
-                           !backward || in_place(d, d.g_stride, d.queries, d.heads) ? 0 : q_rows};
-  for (int i = 0; i < 4; ++i) {
+                           !backward || in_place(d, d.g_stride, d.queries, d.heads) ? 0 : q_rows,
+                           !backward || d.dim % e == 0 ? 0 : q_rows};
+  for (int i = 0; i < 5; ++i) {
     p.packs[i] = at;
     at += align256(rows[i] * p.dim * element_bytes(d.dtype));
   }
   if (!backward) {
-    // two blocks per CU (four where states are streamed); a split reads at least 128 states
-    p.forward = split_axis(p.bh * p.row_tiles, p.few ? 4 * int64_t(cu) : 2 * int64_t(cu), d.keys, 128, p.few ? 256 : 128);
+    // The states are split among blocks where the rows' blocks alone leave CUs idle, and each still has 256 states or
+    // more: the partial results cost a write, a read and a launch.  4,096 rows x 8 heads (256 blocks) x 256 states of
+    // 64 dimensions in fp16 took 25 us in two splits.  Few rows stream the states: four blocks per CU.
+    p.forward = p.few ? split_axis(p.bh, 4 * int64_t(cu), d.keys, 128, 256)
+                      : split_axis(p.bh * p.row_tiles, cu, d.keys, 64, 256);
     if (p.forward.count > 1) {
       const int64_t partial = p.forward.count * p.bh * p.rows;
       p.part = at;
@@ -76,7 +83,7 @@ Plan make_plan(const rdv_attention_desc& d, bool backward, int cu) {
     p.stats = at;
     at += align256(p.bh * p.rows * 8);
     // a split is a whole number of the kernels' tiles (at most 64): dK and dV's rows end with a tile, not with a split
-    p.dq = split_axis(p.bh * ((p.rows + 127) / 128), 2 * int64_t(cu), d.keys, 64, 128);
+    p.dq = split_axis(p.bh * p.row_tiles, cu, d.keys, 64, 256);
     p.dkv = split_axis(p.bh * p.key_tiles, 2 * int64_t(cu), p.rows, 64, 128);
     const int64_t a = p.dq.count > 1 ? align256(p.dq.count * p.bh * p.rows * p.pdim * 4) : 0;
     const int64_t b = p.dkv.count > 1 ? align256(p.dkv.count * p.bh * d.keys * p.pdim * 4) : 0;
@@ -145,23 +152,6 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a, int per) {
   T* const out = static_cast<T*>(a.out) + ((int64_t(item) * a.queries + at.query) * a.heads + at.head) * a.odim;
   store_quad(out, 4 * l, a.odim, o4[0] * inv, o4[1] * inv, o4[2] * inv, o4[3] * inv);
   if (a.lse && l == 0) a.lse[row] = total == 0.0f ? -INFINITY : (top + __builtin_amdgcn_logf(total)) * kLn2;
-}
-
-// stats[row] = (lse log2 e, or +inf where no state counts; delta = rowsum(dO O)), 8 lanes per row.
-template <class T>
-__global__ __launch_bounds__(256) void attn_delta_kernel(AttnArgs a) {
-  const int64_t n = int64_t(a.batch) * a.kv_heads * a.rows, row = int64_t(blockIdx.x) * 32 + (threadIdx.x >> 3);
-  if (row >= n) return;
-  const int l = int(threadIdx.x) & 7;
-  const int bh = int(row / a.rows), r = int(row - int64_t(bh) * a.rows), item = bh / a.kv_heads;
-  const RowAt at = row_at(a, bh - item * a.kv_heads, r);
-  const T* const g = static_cast<const T*>(a.g) + item * a.gs[0] + at.query * a.gs[1] + at.head * a.gs[2];
-  const T* const o = static_cast<const T*>(a.o) + ((int64_t(item) * a.queries + at.query) * a.heads + at.head) * a.odim;
-  float sum = 0.0f;
-  for (int d = l; d < a.odim; d += 8) sum += to_f32(g[d]) * to_f32(o[d]);
-  for (int x = 4; x > 0; x >>= 1) sum += __shfl_xor(sum, x);
-  const float lse = a.lse[row];
-  if (l == 0) a.stats[row] = float2{lse == -INFINITY ? INFINITY : lse * kLog2e, sum};
 }
 
 // The sum of the splits of dQ (KEYS false: rows of the queries) or of dK and dV (KEYS true: z picks the tensor).
@@ -275,12 +265,12 @@ int launch_attention(const rdv_attention_desc& d, const void* q, const void* k, 
   if (rc != RDV_OK) return rc;
   a.out = out;
   a.lse = lse;
-  a.tiles = p.row_tiles;
+  a.tiles = p.few ? 1 : p.row_tiles;
   a.splits = p.forward.count;
   a.chunk = p.forward.chunk;
   a.part = reinterpret_cast<float*>(ws + p.part);
   a.part_ml = reinterpret_cast<float2*>(ws + p.ml);
-  rc = launch_matrix(d.dtype, p.few ? kAttnFew : kAttnTile, a, stream);
+  rc = launch_matrix(d.dtype, p.few ? kAttnFew : p.pairs ? kAttnTilePairs : kAttnTile, a, stream);
   if (rc != RDV_OK || a.splits == 1) return rc;
   int per = 1;
   while (per < 8 && 4 * per < a.splits) per *= 2;
@@ -312,7 +302,9 @@ int launch_attention_backward(const rdv_attention_desc& d, const void* grad, con
   if (rc == RDV_OK) rc = input(d, p, 2, v, d.v_stride, d.keys, d.kv_heads, ws, &a.v, a.vs, stream);
   if (rc == RDV_OK) rc = input(d, p, 3, grad, d.g_stride, d.queries, d.heads, ws, &a.g, a.gs, stream);
   if (rc != RDV_OK) return rc;
-  a.o = out;
+  const int64_t o_stride[3] = {int64_t(d.queries) * d.heads * d.dim, int64_t(d.heads) * d.dim, d.dim};
+  rc = input(d, p, 4, out, o_stride, d.queries, d.heads, ws, &a.o, a.os, stream);
+  if (rc != RDV_OK) return rc;
   a.lse = const_cast<float*>(lse);
   a.stats = reinterpret_cast<float2*>(ws + p.stats);
   a.dq = dq;
@@ -320,19 +312,12 @@ int launch_attention_backward(const rdv_attention_desc& d, const void* grad, con
   a.dv = dv;
   const int64_t n = p.bh * p.rows;
   const int64_t sums = (std::max(n, p.bh * int64_t(d.keys)) * p.pdim + 255) / 256;
-  if ((n + 31) / 32 >= (int64_t(1) << 31) || sums >= (int64_t(1) << 31))
-    return fail(RDV_ERR_UNSUPPORTED, "attention: too many rows");
-  rc = with_dtype(d.dtype, [&](auto t) {
-    attn_delta_kernel<decltype(t)><<<dim3(unsigned((n + 31) / 32)), 256, 0, stream>>>(a);
-    RDV_HIP_TRY(hipGetLastError());
-    return int(RDV_OK);
-  });
-  if (rc != RDV_OK) return rc;
-  a.tiles = (p.rows + 127) / 128;
+  if (sums >= (int64_t(1) << 31)) return fail(RDV_ERR_UNSUPPORTED, "attention: too many rows");
+  a.tiles = p.row_tiles;
   a.splits = p.dq.count;
   a.chunk = p.dq.chunk;
   a.part = reinterpret_cast<float*>(ws + p.part);
-  rc = launch_matrix(d.dtype, kAttnDq, a, stream);
+  rc = launch_matrix(d.dtype, p.pairs ? kAttnDqPairs : kAttnDq, a, stream);
   if (rc != RDV_OK) return rc;
   if (a.splits > 1) {
     rc = with_dtype(d.dtype, [&](auto t) {
