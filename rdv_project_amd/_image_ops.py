@@ -64,6 +64,13 @@ def _on_gpu(*named) -> None:
             raise TypeError(f"{what} must be a GPU tensor, got device {t.device}")
 
 
+def _like_out(out, x: torch.Tensor, aligned: bool = True) -> torch.Tensor:
+    """The caller's buffer for a result like x, or a fresh contiguous one."""
+    if out is None:
+        return torch.empty_like(x) if x.is_contiguous() else x.new_empty(x.shape)
+    return _out_tensor(out, x.shape, x.dtype, x.device, "out", aligned)
+
+
 def _out_tensor(out, shape, dtype, device, what: str = "out", aligned: bool = True) -> torch.Tensor:
     """The caller's buffer, checked to be what the kernels write, or a fresh one."""
     if out is None:
@@ -77,12 +84,13 @@ def _out_tensor(out, shape, dtype, device, what: str = "out", aligned: bool = Tr
     return out
 
 
-def _grad_tensors(grads, shapes, dtypes, device, names):
+def _grad_tensors(grads, likes, names):
+    """The caller's buffers for gradients of `likes`, or fresh contiguous ones."""
     if grads is None:
-        grads = (None,) * len(shapes)
-    if not isinstance(grads, (list, tuple)) or len(grads) != len(shapes):
+        return tuple(_like_out(None, t) for t in likes)
+    if not isinstance(grads, (list, tuple)) or len(grads) != len(likes):
         raise TypeError(f"grads must be ({', '.join(names)})")
-    return tuple(_out_tensor(g, s, t, device, n) for g, s, t, n in zip(grads, shapes, dtypes, names))
+    return tuple(_out_tensor(g, t.shape, t.dtype, t.device, n) for g, t, n in zip(grads, likes, names))
 
 
 def _apart(out: torch.Tensor, *inputs) -> None:
@@ -150,19 +158,20 @@ def _norm_plan(shape, x_stride, g_stride, dtype, groups, eps, activation, device
     return d, at is None, g_at is None, nbytes
 
 
+def _norm_param(p, x, what: str):
+    if p is None:
+        return None
+    p = _tensor(p, what)
+    assert p.dim() == 1 and p.shape[0] == x.shape[-1], f"{what} must be [channels]"
+    if p.dtype != torch.float32:
+        raise TypeError(f"{what} must be float32, got {p.dtype}")
+    return p.contiguous()
+
+
 def _norm_inputs(x, weight, bias):
     x = _data(x, "x")
     assert x.dim() >= 2, "x must be [rows, channels] (one image) or [images, ..., channels]"
-    params = []
-    for p, what in ((weight, "weight"), (bias, "bias")):
-        if p is not None:
-            p = _tensor(p, what)
-            assert p.dim() == 1 and p.shape[0] == x.shape[-1], f"{what} must be [channels]"
-            if p.dtype != torch.float32:
-                raise TypeError(f"{what} must be float32, got {p.dtype}")
-            p = p.contiguous()
-        params.append(p)
-    return x, params[0], params[1]
+    return x, _norm_param(weight, x, "weight"), _norm_param(bias, x, "bias")
 
 
 def _group_norm_into(plan, x, weight, bias, y, stats) -> None:
@@ -188,7 +197,7 @@ def group_norm(x, weight, bias, groups: int, eps: float = 1e-5, activation: str 
     x, weight, bias = _norm_inputs(x, weight, bias)
     plan = _norm_plan(x.shape, x.stride(), None, x.dtype, int(groups), float(eps), activation, _gpu_index())
     _on_gpu(x, "x", weight, "weight", bias, "bias")
-    y = _out_tensor(out, x.shape, x.dtype, x.device)
+    y = _like_out(out, x)
     if out is not None:
         _apart(y, (x, "x"), (weight, "weight"), (bias, "bias"))
     stats = None
@@ -214,8 +223,10 @@ def group_norm_backward(grad, x, weight, bias, groups: int, stats, activation: s
     if stats.dtype != torch.float32:
         raise TypeError(f"stats must be float32, got {stats.dtype}")
     _on_gpu(x, "x", grad, "grad", weight, "weight", bias, "bias", stats, "stats")
-    dx, dw, db = _grad_tensors(grads, (x.shape, (d.channels,), (d.channels,)), (x.dtype, torch.float32, torch.float32),
-                               x.device, ("dx", "dweight", "dbias"))
+    param = weight if weight is not None else bias
+    if param is None:
+        param = torch.empty(d.channels, dtype=torch.float32, device=x.device)
+    dx, dw, db = _grad_tensors(grads, (x, param, param), ("dx", "dweight", "dbias"))
     if grads is not None:
         for t in (dx, dw, db):
             _apart(t, (x, "x"), (grad, "grad"), (weight, "weight"), (bias, "bias"), (stats, "stats"))
@@ -327,7 +338,7 @@ def cross_attention(q, k, v, key_lengths=None, key_mask=None, scale: float | Non
     throughout."""
     given = q, k, v
     q, k, v, key_lengths, key_mask, _, plan = _attention_inputs(q, k, v, key_lengths, key_mask, scale)
-    y = _out_tensor(out, q.shape, q.dtype, q.device)
+    y = _like_out(out, q)
     if out is not None:
         _apart(y, (_tensor(given[0], "q"), "q"), (_tensor(given[1], "k"), "k"), (_tensor(given[2], "v"), "v"),
                (key_lengths, "key_lengths"), (key_mask, "key_mask"))
@@ -355,7 +366,7 @@ def cross_attention_backward(grad, q, k, v, out, lse, key_lengths=None, key_mask
         raise TypeError(f"lse must be float32, got {lse.dtype}")
     _on_gpu(out, "out", lse, "lse")
     given = grads is not None
-    dq, dk, dv = _grad_tensors(grads, (q.shape, k.shape, v.shape), (q.dtype,) * 3, q.device, ("dq", "dk", "dv"))
+    dq, dk, dv = _grad_tensors(grads, (q, k, v), ("dq", "dk", "dv"))
     if given:
         for t in (dq, dk, dv):
             _apart(t, (grad, "grad"), (q, "q"), (k, "k"), (v, "v"), (out, "out"), (lse, "lse"),
@@ -404,7 +415,7 @@ def dropout(x, p: float, seed: int, subsequence: int = 0, residual=None, out=Non
     if residual is not None:
         residual = _like(residual, x, "residual")
     _on_gpu(x, "x", residual, "residual")
-    y = _out_tensor(out, x.shape, x.dtype, x.device, aligned=False)
+    y = _like_out(out, x, aligned=False)
     if out is not None:
         for t, what in ((x, "x"), (residual, "residual")):
             if t is not None and not (t.data_ptr() == y.data_ptr() and t.is_contiguous()):

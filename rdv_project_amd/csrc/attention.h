@@ -34,6 +34,7 @@ struct AttnArgs {
   int64_t qs[3], ks[3], vs[3], gs[3], os[3], ms;
   int batch, queries, keys, heads, kv_heads, share, rows, dim, odim, pdim;
   int tiles, splits, chunk;          // blocks: (item, state head) x split x tile; a split's share of the other axis
+  int by_xcd;                        // whether an XCD takes a contiguous run of the blocks
   float scale;
 };
 
@@ -304,7 +305,7 @@ __device__ __forceinline__ void clear_tiles(uint8_t* tiles, int bytes, int dim) 
   __syncthreads();
 }
 
-// Blocks run round robin over the 8 XCDs, each with its own L2: every XCD takes a contiguous run of the work, so the
+// Blocks run round robin over the 8 XCDs, each with its own L2: here every XCD takes a contiguous run of the work, so the
 // blocks that read one (item, state head) share an L2.
 __device__ __forceinline__ uint32_t xcd_contiguous(uint32_t block, uint32_t total) {
   const uint32_t each = total / 8, rest = total % 8, x = block % 8;
@@ -315,9 +316,17 @@ struct BlockAt {
   int item, hk, bh, split, tile;
 };
 __device__ __forceinline__ BlockAt block_at(const AttnArgs& a) {
-  const uint32_t w = xcd_contiguous(blockIdx.x, gridDim.x), rest = w / uint32_t(a.tiles);
+  const uint32_t w = a.by_xcd ? xcd_contiguous(blockIdx.x, gridDim.x) : blockIdx.x, rest = w / uint32_t(a.tiles);
   BlockAt p;
   p.tile = int(w - rest * a.tiles);
+  if (a.tiles == 1) {  // neighbouring blocks read the state heads of the same states, which lie side by side
+    const uint32_t most = rest / uint32_t(a.kv_heads);
+    p.hk = int(rest - most * a.kv_heads);
+    p.item = int(most / uint32_t(a.splits));
+    p.split = int(most) - p.item * a.splits;
+    p.bh = p.item * a.kv_heads + p.hk;
+    return p;
+  }
   p.bh = int(rest / uint32_t(a.splits));
   p.split = int(rest) - p.bh * a.splits;
   p.item = p.bh / a.kv_heads;

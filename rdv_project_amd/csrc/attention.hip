@@ -231,9 +231,13 @@ int input(const rdv_attention_desc& d, const Plan& p, int which, const void* x, 
   });
 }
 
-int launch_matrix(int dtype, AttnKernel which, const AttnArgs& a, hipStream_t stream) {
+int launch_matrix(int dtype, AttnKernel which, AttnArgs& a, int cu, hipStream_t stream) {
   const int64_t blocks = int64_t(a.batch) * a.kv_heads * a.splits * a.tiles;
   if (blocks >= (int64_t(1) << 31)) return fail(RDV_ERR_UNSUPPORTED, "attention: too many blocks");
+  // Contiguous runs per XCD share tiles in its L2, but also give an XCD whole items: with lengths, or in about one round
+  // of blocks, the longest item's XCD would finish last (dK and dV of four items of 0 to 333 states x 2,000 rows in fp32:
+  // 51 us, in plain order 34).  Blocks of few rows share nothing.
+  a.by_xcd = which != kAttnFew && !a.lengths && blocks >= 2 * int64_t(cu);
   if (dtype == RDV_DTYPE_F16) return launch_attn_f16(which, a, unsigned(blocks), stream);
   if (dtype == RDV_DTYPE_BF16) return launch_attn_bf16(which, a, unsigned(blocks), stream);
   return launch_attn_f32(which, a, unsigned(blocks), stream);
@@ -270,7 +274,7 @@ int launch_attention(const rdv_attention_desc& d, const void* q, const void* k, 
   a.chunk = p.forward.chunk;
   a.part = reinterpret_cast<float*>(ws + p.part);
   a.part_ml = reinterpret_cast<float2*>(ws + p.ml);
-  rc = launch_matrix(d.dtype, p.few ? kAttnFew : p.pairs ? kAttnTilePairs : kAttnTile, a, stream);
+  rc = launch_matrix(d.dtype, p.few ? kAttnFew : p.pairs ? kAttnTilePairs : kAttnTile, a, cu, stream);
   if (rc != RDV_OK || a.splits == 1) return rc;
   int per = 1;
   while (per < 8 && 4 * per < a.splits) per *= 2;
@@ -317,7 +321,7 @@ int launch_attention_backward(const rdv_attention_desc& d, const void* grad, con
   a.splits = p.dq.count;
   a.chunk = p.dq.chunk;
   a.part = reinterpret_cast<float*>(ws + p.part);
-  rc = launch_matrix(d.dtype, p.pairs ? kAttnDqPairs : kAttnDq, a, stream);
+  rc = launch_matrix(d.dtype, p.pairs ? kAttnDqPairs : kAttnDq, a, cu, stream);
   if (rc != RDV_OK) return rc;
   if (a.splits > 1) {
     rc = with_dtype(d.dtype, [&](auto t) {
@@ -331,7 +335,7 @@ int launch_attention_backward(const rdv_attention_desc& d, const void* grad, con
   a.splits = p.dkv.count;
   a.chunk = p.dkv.chunk;
   a.part2 = reinterpret_cast<float*>(ws + p.part2);
-  rc = launch_matrix(d.dtype, kAttnDkv, a, stream);
+  rc = launch_matrix(d.dtype, kAttnDkv, a, cu, stream);
   if (rc != RDV_OK || a.splits == 1) return rc;
   return with_dtype(d.dtype, [&](auto t) {
     attn_sum_kernel<decltype(t), true><<<dim3(unsigned((p.bh * d.keys * p.pdim + 255) / 256), 2), 256, 0, stream>>>(a);

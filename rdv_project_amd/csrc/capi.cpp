@@ -125,10 +125,10 @@ int launch_concat(const float* x1, int C1, const float* x2, int C2, int64_t rows
 
 int64_t group_norm_workspace_bytes(const rdv_group_norm_desc& d, bool backward, int cu);
 int launch_group_norm(const rdv_group_norm_desc& d, const void* x, const float* weight, const float* bias, void* y,
-                      float* stats, void* ws, int cu, hipStream_t stream);
+                      float* stats, void* ws, int64_t ws_bytes, int cu, hipStream_t stream);
 int launch_group_norm_backward(const rdv_group_norm_desc& d, const void* grad, const void* x, const float* weight,
                                const float* bias, const float* stats, void* dx, float* dweight, float* dbias,
-                               void* ws, int cu, hipStream_t stream);
+                               void* ws, int64_t ws_bytes, int cu, hipStream_t stream);
 int64_t attention_workspace_bytes(const rdv_attention_desc& d, bool backward, int cu);
 int launch_attention(const rdv_attention_desc& d, const void* q, const void* k, const void* v,
                      const int32_t* key_lengths, const uint8_t* key_mask, void* out, float* lse, void* ws, int cu,
@@ -791,10 +791,9 @@ int rdv_group_norm(const rdv_group_norm_desc* desc, const void* x, const float* 
   if (!x || !y) return fail(RDV_ERR_INVALID, "rdv_group_norm: NULL pointer argument");
   if (!aligned16(y)) return fail(RDV_ERR_INVALID, "rdv_group_norm: y must be 16-byte aligned");
   const int cu = plan_cu_count();
-  const int64_t need = group_norm_workspace_bytes(*desc, false, cu);
-  if (need > 0 && (!workspace || workspace_bytes < need || !aligned16(workspace)))
-    return fail(RDV_ERR_WORKSPACE, "rdv_group_norm: workspace too small or not 16-byte aligned");
-  return launch_group_norm(*desc, x, weight, bias, y, stats, workspace, cu, static_cast<hipStream_t>(stream));
+  if (!aligned16(workspace)) return fail(RDV_ERR_WORKSPACE, "rdv_group_norm: the workspace must be 16-byte aligned");
+  return launch_group_norm(*desc, x, weight, bias, y, stats, workspace, workspace ? workspace_bytes : 0, cu,
+                           static_cast<hipStream_t>(stream));
 }
 
 int rdv_group_norm_backward(const rdv_group_norm_desc* desc, const void* grad, const void* x, const float* weight,
@@ -806,12 +805,11 @@ int rdv_group_norm_backward(const rdv_group_norm_desc* desc, const void* grad, c
   if (desc->images > 0 && desc->rows > 0) {
     if (!grad || !x || !stats || !dx) return fail(RDV_ERR_INVALID, "rdv_group_norm_backward: NULL pointer argument");
     if (!aligned16(dx)) return fail(RDV_ERR_INVALID, "rdv_group_norm_backward: dx must be 16-byte aligned");
-    const int64_t need = group_norm_workspace_bytes(*desc, true, cu);
-    if (need > 0 && (!workspace || workspace_bytes < need || !aligned16(workspace)))
-      return fail(RDV_ERR_WORKSPACE, "rdv_group_norm_backward: workspace too small or not 16-byte aligned");
+    if (!aligned16(workspace))
+      return fail(RDV_ERR_WORKSPACE, "rdv_group_norm_backward: the workspace must be 16-byte aligned");
   }
-  return launch_group_norm_backward(*desc, grad, x, weight, bias, stats, dx, dweight, dbias, workspace, cu,
-                                    static_cast<hipStream_t>(stream));
+  return launch_group_norm_backward(*desc, grad, x, weight, bias, stats, dx, dweight, dbias, workspace,
+                                    workspace ? workspace_bytes : 0, cu, static_cast<hipStream_t>(stream));
 }
 
 static int check_attention(const rdv_attention_desc* d, bool backward) {

@@ -968,8 +968,9 @@ int64_t group_norm_workspace_bytes(const rdv_group_norm_desc& d, bool backward, 
 }
 
 int launch_group_norm(const rdv_group_norm_desc& d, const void* x, const float* weight, const float* bias, void* y,
-                      float* stats, void* ws, int cu, hipStream_t stream) {
+                      float* stats, void* ws, int64_t ws_bytes, int cu, hipStream_t stream) {
   const NormPlan p = norm_plan(d, false, cu, alignment({x, y}));
+  if (ws_bytes < p.bytes) return fail(RDV_ERR_WORKSPACE, "rdv_group_norm: workspace too small");
   NormArgs a = norm_args(d, p, x, weight, bias, ws);
   a.y = y;
   a.stats = stats;
@@ -1001,9 +1002,10 @@ int launch_group_norm(const rdv_group_norm_desc& d, const void* x, const float* 
 
 int launch_group_norm_backward(const rdv_group_norm_desc& d, const void* grad, const void* x, const float* weight,
                                const float* bias, const float* stats, void* dx, float* dweight, float* dbias,
-                               void* ws, int cu, hipStream_t stream) {
+                               void* ws, int64_t ws_bytes, int cu, hipStream_t stream) {
   const bool empty = d.images == 0 || d.rows == 0;
   const NormPlan p = empty ? NormPlan{} : norm_plan(d, true, cu, alignment({x, grad, dx}));
+  if (ws_bytes < p.bytes) return fail(RDV_ERR_WORKSPACE, "rdv_group_norm_backward: workspace too small");
   NormArgs a = norm_args(d, p, x, weight, bias, ws);
   a.grad = grad;
   a.stats = const_cast<float*>(stats);
