@@ -143,23 +143,44 @@ __device__ __forceinline__ void sum_rows(const NormArgs& a, const NormAt& p, flo
   __syncthreads();
 }
 template <int VE>
+__device__ __forceinline__ int lds_rows(const NormArgs& a) { return a.wave_rows ? int(blockDim.x >> 6) : a.tr; }
+
+template <int VE>
 __device__ __forceinline__ float channel_sum(const NormArgs& a, const float* red, int c) {
-  const int rows = a.wave_rows ? int(blockDim.x >> 6) : a.tr;
+  const int rows = lds_rows<VE>(a);
   float s = 0.0f;
+#pragma unroll 8
   for (int r = 0; r < rows; ++r) s += red[r * a.pieces * VE + c];
   return s;
 }
 
-// out[g] = f(sum of per(channel) over the channels of the slab's group g), 16 lanes per group.
-template <class P, class F>
-__device__ __forceinline__ void sum_groups(const NormArgs& a, const NormAt& p, float* out, P per, F f) {
-  const int l = int(threadIdx.x) & 15, lanes = int(blockDim.x) >> 4;
-  for (int g = int(threadIdx.x) >> 4; g < p.groups; g += lanes) {
+// Runs f(group, lane, lanes, sum over the group's lanes) for the slab's groups, each by as many lanes (16 to 64) as the
+// block has for it: a group's channels times the LDS rows are spread over them, few additions in a row.
+template <class F>
+__device__ __forceinline__ void for_groups(const NormAt& p, F f) {
+  int lanes = 16;
+  while (lanes < 64 && 2 * lanes * p.groups <= int(blockDim.x)) lanes *= 2;
+  const int l = int(threadIdx.x) & (lanes - 1);
+  for (int g = int(threadIdx.x) / lanes; g < p.groups; g += int(blockDim.x) / lanes)
+    f(g, l, lanes, [&](float s) {
+      for (int o = lanes >> 1; o > 0; o >>= 1) s += __shfl_xor(s, o);
+      return s;
+    });
+}
+
+// out[g] = f(sum of the LDS rows' per-channel sums, times weight(channel), over the channels of the slab's group g).
+template <int VE, class W, class F>
+__device__ __forceinline__ void sum_groups(const NormArgs& a, const NormAt& p, const float* red, float* out, W weight, F f) {
+  const int items = lds_rows<VE>(a) * a.width, step = a.pieces * VE;
+  for_groups(p, [&](int g, int l, int lanes, auto join) {
     float s = 0.0f;
-    for (int c = l; c < a.width; c += 16) s += per(g * a.width + c);
-    for (int o = 8; o > 0; o >>= 1) s += __shfl_xor(s, o);
+    for (int k = l; k < items; k += lanes) {
+      const int row = group_of(a, k), c = g * a.width + k - row * a.width;
+      s = fmaf(red[row * step + c], weight(c), s);
+    }
+    s = join(s);
     if (l == 0) out[g] = f(s);
-  }
+  });
   __syncthreads();
 }
 
@@ -204,25 +225,26 @@ __device__ __forceinline__ void group_stats(const NormArgs& a, const NormAt& p, 
     }
   }
   __syncthreads();
-  const int l = int(threadIdx.x) & 15, lanes = int(blockDim.x) >> 4, step = a.pieces * VE;
-  for (int g = int(threadIdx.x) >> 4; g < p.groups; g += lanes) {
+  const int items = rows * a.width, step = a.pieces * VE;
+  for_groups(p, [&](int g, int l, int lanes, auto join) {
     float s = 0.0f;
-    for (int c = l; c < a.width; c += 16)
-      for (int r = 0; r < rows; ++r) s = fmaf(counts[r], red[r * step + g * a.width + c], s);
-    for (int o = 8; o > 0; o >>= 1) s += __shfl_xor(s, o);
-    const float mean = s / count;
+    for (int k = l; k < items; k += lanes) {
+      const int r = group_of(a, k), c = g * a.width + k - r * a.width;
+      s = fmaf(counts[r], red[r * step + c], s);
+    }
+    const float mean = join(s) / count;
     s = 0.0f;
-    for (int c = l; c < a.width; c += 16)
-      for (int r = 0; r < rows; ++r) {
-        const float t = red[r * step + g * a.width + c] - mean;
-        s += fmaf(counts[r] * t, t, dev[r * step + g * a.width + c]);
-      }
-    for (int o = 8; o > 0; o >>= 1) s += __shfl_xor(s, o);
+    for (int k = l; k < items; k += lanes) {
+      const int r = group_of(a, k), c = g * a.width + k - r * a.width;
+      const float t = red[r * step + c] - mean;
+      s += fmaf(counts[r] * t, t, dev[r * step + c]);
+    }
+    s = join(s);
     if (l == 0) {
       mean_g[g] = mean;
       dev_g[g] = f(s);
     }
-  }
+  });
   __syncthreads();
 }
 
@@ -362,9 +384,8 @@ __device__ __forceinline__ void join_sums(const NormArgs& a, const NormAt& p, fl
         else if (param) param[p.c0 + c] = s;
       }
     }
-    sum_groups(a, p, which ? m2 : m1,
-               [&](int c) { return channel_sum<VE>(a, red, c) * (a.weight ? a.weight[p.c0 + c] : 1.0f); },
-               [&](float t) { return t * inv; });
+    sum_groups<VE>(a, p, red, which ? m2 : m1, [&](int c) { return a.weight ? a.weight[p.c0 + c] : 1.0f; },
+                   [&](float t) { return t * inv; });
   }
 }
 
@@ -520,22 +541,20 @@ __global__ __launch_bounds__(kNormThreads) void norm_apply_kernel(NormArgs a) {
   if (p.on && r < ch.end) load_rows<T, VE, U>(a, x, a.x_row, r, v);  // in flight while the statistics are joined
   load_affine<VE>(a, p, w, b);
   {
-    int lanes = 16;  // per group
-    while (lanes < 64 && 2 * lanes * p.groups <= int(blockDim.x)) lanes *= 2;
-    const int l = int(threadIdx.x) & (lanes - 1);
     const float total = float(a.rows) * float(a.width);
-    for (int g = int(threadIdx.x) / lanes; g < p.groups; g += int(blockDim.x) / lanes) {
+    for_groups(p, [&](int g, int l, int lanes, auto join) {
       const float2* const part = a.parts + (p.image * a.groups + p.c0 / a.width + g) * a.chunks;
       float s = 0.0f;
+#pragma unroll 4
       for (int i = l; i < a.chunks; i += lanes) s += part[i].x * float(min(a.chunk_rows, a.rows - i * a.chunk_rows));
-      for (int o = lanes >> 1; o > 0; o >>= 1) s += __shfl_xor(s, o);
-      const float m = s / float(a.rows);
+      const float m = join(s) / float(a.rows);
       s = 0.0f;
+#pragma unroll 4
       for (int i = l; i < a.chunks; i += lanes) {
         const float2 t = part[i];
         s += t.y + (t.x - m) * (t.x - m) * float(min(a.chunk_rows, a.rows - i * a.chunk_rows)) * float(a.width);
       }
-      for (int o = lanes >> 1; o > 0; o >>= 1) s += __shfl_xor(s, o);
+      s = join(s);
       if (l == 0) {
         mean_g[g] = m;
         rstd_g[g] = 1.0f / sqrtf(s / total + a.eps);
@@ -545,7 +564,7 @@ __global__ __launch_bounds__(kNormThreads) void norm_apply_kernel(NormArgs a) {
           st[1] = rstd_g[g];
         }
       }
-    }
+    });
   }
   __syncthreads();
   if (!p.on) return;
