@@ -463,6 +463,13 @@ __device__ __forceinline__ void load_rows(const NormArgs& a, const T* x, int64_t
   for (int k = 0; k < U; ++k) v[k] = load_piece<T, VE>(x + min(r + k * a.tr, a.rows - 1) * stride);
 }
 
+// The first of the thread's last U rows of the chunk (below ch.first where it has none).  The second launches walk their
+// rows from the end: what the first launch read last is what the caches still hold.
+__device__ __forceinline__ int last_rows(const NormChunk& ch, const NormAt& p, int step) {
+  const int rows = ch.end - ch.first - p.tr;
+  return rows > 0 ? ch.first + p.tr + (rows - 1) / step * step : ch.first - 1;
+}
+
 // First launch, forward: a chunk's mean and squared deviations per group.
 template <class T, int VE>
 __global__ __launch_bounds__(kNormThreads) void norm_stats_kernel(NormArgs a) {
@@ -536,9 +543,9 @@ __global__ __launch_bounds__(kNormThreads) void norm_apply_kernel(NormArgs a) {
   const T* const x = static_cast<const T*>(a.x) + p.image * a.x_image + p.c0 + p.channel;
   float w[VE], b[VE], mean[VE], scale[VE];
   const int step = U * a.tr;
-  int r = ch.first + p.tr;
+  int r = last_rows(ch, p, step);
   Piece<T, VE> v[U], next[U];
-  if (p.on && r < ch.end) load_rows<T, VE, U>(a, x, a.x_row, r, v);  // in flight while the statistics are joined
+  if (p.on && r >= ch.first) load_rows<T, VE, U>(a, x, a.x_row, r, v);  // in flight while the statistics are joined
   load_affine<VE>(a, p, w, b);
   {
     const float total = float(a.rows) * float(a.width);
@@ -575,8 +582,8 @@ __global__ __launch_bounds__(kNormThreads) void norm_apply_kernel(NormArgs a) {
     scale[i] = w[i] * rstd_g[g];
   }
   T* const y = static_cast<T*>(a.y) + p.image * a.rows * a.channels + p.c0 + p.channel;
-  for (; r < ch.end; r += step) {
-    if (r + step < ch.end) load_rows<T, VE, U>(a, x, a.x_row, r + step, next);
+  for (; r >= ch.first; r -= step) {
+    if (r - step >= ch.first) load_rows<T, VE, U>(a, x, a.x_row, r - step, next);
 #pragma unroll
     for (int k = 0; k < U; ++k) {
       const int at = r + k * a.tr;
@@ -678,8 +685,8 @@ __global__ __launch_bounds__(kNormBackThreads) void norm_dx_kernel(NormArgs a) {
   T* const dx = static_cast<T*>(a.y) + p.image * a.rows * a.channels + p.c0 + p.channel;
   const int step = U * a.tr;
   Piece<T, VE> vx[U], vg[U], nx[U], ng[U];
-  int r = ch.first + p.tr;
-  if (p.on && r < ch.end) {  // in flight while the sums are joined
+  int r = last_rows(ch, p, step);
+  if (p.on && r >= ch.first) {  // in flight while the sums are joined
     load_rows<T, VE, U>(a, x, a.x_row, r, vx);
     load_rows<T, VE, U>(a, g, a.g_row, r, vg);
   }
@@ -694,10 +701,10 @@ __global__ __launch_bounds__(kNormBackThreads) void norm_dx_kernel(NormArgs a) {
     g1[i] = m1[group_of(a, p.channel + i)];
     g2[i] = m2[group_of(a, p.channel + i)];
   }
-  for (; r < ch.end; r += step) {
-    if (r + step < ch.end) {
-      load_rows<T, VE, U>(a, x, a.x_row, r + step, nx);
-      load_rows<T, VE, U>(a, g, a.g_row, r + step, ng);
+  for (; r >= ch.first; r -= step) {
+    if (r - step >= ch.first) {
+      load_rows<T, VE, U>(a, x, a.x_row, r - step, nx);
+      load_rows<T, VE, U>(a, g, a.g_row, r - step, ng);
     }
 #pragma unroll
     for (int k = 0; k < U; ++k) {
