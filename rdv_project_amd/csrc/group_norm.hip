@@ -273,22 +273,43 @@ __device__ __forceinline__ void normalise(const NormArgs& a, const Piece<T, VE>&
   store_piece<T, VE>(y, z);
 }
 
-// dz and xhat of a piece.
-template <class T, int VE>
-__device__ __forceinline__ void slopes(const NormArgs& a, const Piece<T, VE>& x, const Piece<T, VE>& g,
-                                       const float (&mean)[VE], const float (&rstd)[VE], const float (&w)[VE],
-                                       const float (&b)[VE], float (&xhat)[VE], float (&dz)[VE]) {
+// A thread's channels in the backward kernels, as lines in x so that an element costs one multiply-add each:
+// xhat = hat x + hat0, z = lin x + lin0.
+template <int VE>
+struct BackLines {
+  float hat[VE], hat0[VE], lin[VE], lin0[VE];
+};
+template <int VE>
+__device__ __forceinline__ BackLines<VE> back_lines(const NormArgs& a, const NormAt& p, float (&w)[VE]) {
+  BackLines<VE> k;
 #pragma unroll
   for (int i = 0; i < VE; ++i) {
-    xhat[i] = (x[i] - mean[i]) * rstd[i];
-    dz[i] = g[i];
+    const int64_t g = p.image * a.groups + (p.on ? group_of(a, p.c0) + group_of(a, p.channel + i) : 0);
+    const float mean = a.stats[2 * g], rstd = a.stats[2 * g + 1];
+    w[i] = p.on && a.weight ? a.weight[p.c0 + p.channel + i] : 1.0f;
+    k.hat[i] = rstd;
+    k.hat0[i] = -mean * rstd;
+    k.lin[i] = rstd * w[i];
+    k.lin0[i] = fmaf(k.hat0[i], w[i], p.on && a.bias ? a.bias[p.c0 + p.channel + i] : 0.0f);
   }
-  if (a.act == RDV_ACT_SILU) {
+  return k;
+}
+
+// dz of a piece.
+template <class T, int VE>
+__device__ __forceinline__ void slopes(const NormArgs& a, const BackLines<VE>& k, const Piece<T, VE>& x,
+                                       const Piece<T, VE>& g, float (&dz)[VE]) {
 #pragma unroll
-    for (int i = 0; i < VE; ++i) dz[i] *= silu_slope(fmaf(xhat[i], w[i], b[i]));
+  for (int i = 0; i < VE; ++i) dz[i] = g[i];
+  if (a.act == RDV_ACT_SILU) {  // s + z s (1 - s), s = 1 / (1 + e^-z)
+#pragma unroll
+    for (int i = 0; i < VE; ++i) {
+      const float z = fmaf(x[i], k.lin[i], k.lin0[i]), s = fast_sigmoid(z);
+      dz[i] *= fmaf(z * s, 1.0f - s, s);
+    }
   } else if (a.act == RDV_ACT_RELU) {
 #pragma unroll
-    for (int i = 0; i < VE; ++i) dz[i] = fmaf(xhat[i], w[i], b[i]) > 0.0f ? dz[i] : 0.0f;
+    for (int i = 0; i < VE; ++i) dz[i] = fmaf(x[i], k.lin[i], k.lin0[i]) > 0.0f ? dz[i] : 0.0f;
   }
 }
 
@@ -357,17 +378,6 @@ __global__ __launch_bounds__(1024) void norm_whole_kernel(NormArgs a) {
   }
 }
 
-// The thread's channels' constants from stats.
-template <int VE>
-__device__ __forceinline__ void load_stats(const NormArgs& a, const NormAt& p, float (&mean)[VE], float (&rstd)[VE]) {
-#pragma unroll
-  for (int i = 0; i < VE; ++i) {
-    const int64_t g = p.image * a.groups + (p.on ? group_of(a, p.c0) + group_of(a, p.channel + i) : 0);
-    mean[i] = a.stats[2 * g];
-    rstd[i] = a.stats[2 * g + 1];
-  }
-}
-
 // dx's two means per group, m1 and m2, from the threads' sums A and B; with `keep` the channels' sums are stored too.
 template <int VE>
 __device__ __forceinline__ void join_sums(const NormArgs& a, const NormAt& p, float (&sa)[VE], float (&sb)[VE],
@@ -386,6 +396,19 @@ __device__ __forceinline__ void join_sums(const NormArgs& a, const NormAt& p, fl
     }
     sum_groups<VE>(a, p, red, which ? m2 : m1, [&](int c) { return a.weight ? a.weight[p.c0 + c] : 1.0f; },
                    [&](float t) { return t * inv; });
+  }
+}
+
+// dx = lin dz + slope x + offset: the part of dx that is a line in x, -rstd (m1 + xhat m2).
+template <int VE>
+__device__ __forceinline__ void dx_lines(const NormArgs& a, const NormAt& p, const BackLines<VE>& k, const float* m1,
+                                         const float* m2, float (&slope)[VE], float (&offset)[VE]) {
+#pragma unroll
+  for (int i = 0; i < VE; ++i) {
+    const int g = group_of(a, p.channel + i);
+    const float t = -k.hat[i] * m2[g];
+    slope[i] = t * k.hat[i];
+    offset[i] = fmaf(t, k.hat0[i], -k.hat[i] * m1[g]);
   }
 }
 
@@ -408,32 +431,29 @@ __global__ __launch_bounds__(1024) void norm_whole_back_kernel(NormArgs a) {
       vg[k] = load_piece<T, VE>(g + r * a.g_row);
     }
   }
-  float mean[VE], rstd[VE], w[VE], b[VE], sa[VE] = {}, sb[VE] = {}, xhat[VE], dz[VE];
-  load_affine<VE>(a, p, w, b);
-  load_stats<VE>(a, p, mean, rstd);
+  float w[VE], sa[VE] = {}, sb[VE] = {}, dz[VE];
+  const BackLines<VE> lines = back_lines<VE>(a, p, w);
 #pragma unroll
   for (int k = 0; k < R; ++k)
     if (p.on && p.tr + k * a.tr < a.rows) {
-      slopes<T, VE>(a, vx[k], vg[k], mean, rstd, w, b, xhat, dz);
+      slopes<T, VE>(a, lines, vx[k], vg[k], dz);
 #pragma unroll
       for (int i = 0; i < VE; ++i) {
         sa[i] += dz[i];
-        sb[i] = fmaf(dz[i], xhat[i], sb[i]);
+        sb[i] = fmaf(dz[i], fmaf(vx[k][i], lines.hat[i], lines.hat0[i]), sb[i]);
       }
     }
   join_sums<VE>(a, p, sa, sb, red, m1, m2, true);
   if (!p.on) return;
+  dx_lines<VE>(a, p, lines, m1, m2, sb, sa);
   T* const dx = static_cast<T*>(a.y) + p.image * a.rows * a.channels + p.c0 + p.channel;
 #pragma unroll
   for (int k = 0; k < R; ++k) {
     const int r = p.tr + k * a.tr;
     if (r < a.rows) {
-      slopes<T, VE>(a, vx[k], vg[k], mean, rstd, w, b, xhat, dz);
+      slopes<T, VE>(a, lines, vx[k], vg[k], dz);
 #pragma unroll
-      for (int i = 0; i < VE; ++i) {
-        const int gi = group_of(a, p.channel + i);
-        dz[i] = rstd[i] * (w[i] * dz[i] - m1[gi] - xhat[i] * m2[gi]);
-      }
+      for (int i = 0; i < VE; ++i) dz[i] = fmaf(dz[i], lines.lin[i], fmaf(vx[k][i], sb[i], sa[i]));
       store_piece<T, VE>(dx + int64_t(r) * a.channels, dz);
     }
   }
@@ -602,9 +622,8 @@ __global__ __launch_bounds__(kNormBackThreads) void norm_sums_kernel(NormArgs a)
   const NormAt p = norm_at<VE>(a, ch.image, ch.slab);
   const T* const x = static_cast<const T*>(a.x) + p.image * a.x_image + p.c0 + p.channel;
   const T* const g = static_cast<const T*>(a.grad) + p.image * a.g_image + p.c0 + p.channel;
-  float mean[VE], rstd[VE], w[VE], b[VE], sa[VE] = {}, sb[VE] = {}, xhat[VE], dz[VE];
-  load_affine<VE>(a, p, w, b);
-  load_stats<VE>(a, p, mean, rstd);
+  float w[VE], sa[VE] = {}, sb[VE] = {}, dz[VE];
+  const BackLines<VE> lines = back_lines<VE>(a, p, w);
   if (p.on) {
     const int step = U * a.tr;
     Piece<T, VE> vx[U], vg[U], nx[U], ng[U];
@@ -621,11 +640,11 @@ __global__ __launch_bounds__(kNormBackThreads) void norm_sums_kernel(NormArgs a)
 #pragma unroll
       for (int k = 0; k < U; ++k) {
         if (r + k * a.tr < ch.end) {
-          slopes<T, VE>(a, vx[k], vg[k], mean, rstd, w, b, xhat, dz);
+          slopes<T, VE>(a, lines, vx[k], vg[k], dz);
 #pragma unroll
           for (int i = 0; i < VE; ++i) {
             sa[i] += dz[i];
-            sb[i] = fmaf(dz[i], xhat[i], sb[i]);
+            sb[i] = fmaf(dz[i], fmaf(vx[k][i], lines.hat[i], lines.hat0[i]), sb[i]);
           }
         }
         vx[k] = nx[k];
@@ -693,14 +712,9 @@ __global__ __launch_bounds__(kNormBackThreads) void norm_dx_kernel(NormArgs a) {
   gather_sums<VE>(a, p, p.image * a.chunks, a.chunks, sa, sb);
   join_sums<VE>(a, p, sa, sb, red, m1, m2, false);
   if (!p.on) return;
-  float mean[VE], rstd[VE], w[VE], b[VE], xhat[VE], dz[VE], g1[VE], g2[VE];
-  load_affine<VE>(a, p, w, b);
-  load_stats<VE>(a, p, mean, rstd);
-#pragma unroll
-  for (int i = 0; i < VE; ++i) {
-    g1[i] = m1[group_of(a, p.channel + i)];
-    g2[i] = m2[group_of(a, p.channel + i)];
-  }
+  float w[VE], dz[VE];
+  const BackLines<VE> lines = back_lines<VE>(a, p, w);
+  dx_lines<VE>(a, p, lines, m1, m2, sb, sa);
   for (; r >= ch.first; r -= step) {
     if (r - step >= ch.first) {
       load_rows<T, VE, U>(a, x, a.x_row, r - step, nx);
@@ -710,9 +724,9 @@ __global__ __launch_bounds__(kNormBackThreads) void norm_dx_kernel(NormArgs a) {
     for (int k = 0; k < U; ++k) {
       const int at = r + k * a.tr;
       if (at < ch.end) {
-        slopes<T, VE>(a, vx[k], vg[k], mean, rstd, w, b, xhat, dz);
+        slopes<T, VE>(a, lines, vx[k], vg[k], dz);
 #pragma unroll
-        for (int i = 0; i < VE; ++i) dz[i] = rstd[i] * (w[i] * dz[i] - g1[i] - xhat[i] * g2[i]);
+        for (int i = 0; i < VE; ++i) dz[i] = fmaf(dz[i], lines.lin[i], fmaf(vx[k][i], sb[i], sa[i]));
         store_piece<T, VE>(dx + int64_t(at) * a.channels, dz);
       }
       vx[k] = nx[k];
