@@ -257,12 +257,13 @@ __device__ __forceinline__ void load_affine(const NormArgs& a, const NormAt& p, 
   }
 }
 
+// act(scale x + offset) of a piece.
 template <class T, int VE>
-__device__ __forceinline__ void normalise(const NormArgs& a, const Piece<T, VE>& x, const float (&mean)[VE],
-                                          const float (&scale)[VE], const float (&b)[VE], T* y) {
+__device__ __forceinline__ void normalise(const NormArgs& a, const Piece<T, VE>& x, const float (&scale)[VE],
+                                          const float (&offset)[VE], T* y) {
   float z[VE];
 #pragma unroll
-  for (int i = 0; i < VE; ++i) z[i] = fmaf(x[i] - mean[i], scale[i], b[i]);
+  for (int i = 0; i < VE; ++i) z[i] = fmaf(x[i], scale[i], offset[i]);
   if (a.act == RDV_ACT_SILU) {
 #pragma unroll
     for (int i = 0; i < VE; ++i) z[i] *= fast_sigmoid(z[i]);
@@ -362,13 +363,13 @@ __global__ __launch_bounds__(1024) void norm_whole_kernel(NormArgs a) {
 #pragma unroll
   for (int i = 0; i < VE; ++i) {
     const int g = p.on ? group_of(a, p.channel + i) : 0;
-    mean[i] = mean_g[g];
     scale[i] = w[i] * rstd_g[g];
+    b[i] = fmaf(-mean_g[g], scale[i], b[i]);
   }
   T* const y = static_cast<T*>(a.y) + p.image * a.rows * a.channels + p.c0 + p.channel;
 #pragma unroll
   for (int k = 0; k < R; ++k)
-    if (k < n) normalise<T, VE>(a, v[k], mean, scale, b, y + int64_t(p.tr + k * a.tr) * a.channels);
+    if (k < n) normalise<T, VE>(a, v[k], scale, b, y + int64_t(p.tr + k * a.tr) * a.channels);
   if (a.stats) {
     float* const st = a.stats + 2 * (p.image * a.groups + p.c0 / a.width);
     for (int g = int(threadIdx.x); g < p.groups; g += int(blockDim.x)) {
@@ -561,7 +562,7 @@ __global__ __launch_bounds__(kNormThreads) void norm_apply_kernel(NormArgs a) {
   float* const mean_g = norm_lds;
   float* const rstd_g = mean_g + a.slab / a.width;
   const T* const x = static_cast<const T*>(a.x) + p.image * a.x_image + p.c0 + p.channel;
-  float w[VE], b[VE], mean[VE], scale[VE];
+  float w[VE], b[VE], scale[VE];
   const int step = U * a.tr;
   int r = last_rows(ch, p, step);
   Piece<T, VE> v[U], next[U];
@@ -598,8 +599,8 @@ __global__ __launch_bounds__(kNormThreads) void norm_apply_kernel(NormArgs a) {
 #pragma unroll
   for (int i = 0; i < VE; ++i) {
     const int g = group_of(a, p.channel + i);
-    mean[i] = mean_g[g];
     scale[i] = w[i] * rstd_g[g];
+    b[i] = fmaf(-mean_g[g], scale[i], b[i]);
   }
   T* const y = static_cast<T*>(a.y) + p.image * a.rows * a.channels + p.c0 + p.channel;
   for (; r >= ch.first; r -= step) {
@@ -607,7 +608,7 @@ __global__ __launch_bounds__(kNormThreads) void norm_apply_kernel(NormArgs a) {
 #pragma unroll
     for (int k = 0; k < U; ++k) {
       const int at = r + k * a.tr;
-      if (at < ch.end) normalise<T, VE>(a, v[k], mean, scale, b, y + int64_t(at) * a.channels);
+      if (at < ch.end) normalise<T, VE>(a, v[k], scale, b, y + int64_t(at) * a.channels);
       v[k] = next[k];
     }
   }
