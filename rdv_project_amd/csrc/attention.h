@@ -355,7 +355,18 @@ __device__ __forceinline__ void mask_result(f32x16& s, uint32_t bits, int h, flo
   for (int i = 0; i < 16; ++i) s[i] = (mine >> (8 * (i >> 2) + (i & 3))) & 1 ? s[i] : fill;
 }
 
-__device__ __forceinline__ float other_half(float v) { return __shfl_xor(v, 32); }
+// The value of lane l + 32 (mod 64).  v_permlane32_swap exchanges its second operand's first half with its first one's
+// second half: of two copies of v, one ends as the first half twice and the other as the second.  (In assembly with its
+// wait states: this compiler's builtin does not model the write to the second register.)
+__device__ __forceinline__ float2 both_halves(float v) {
+  float a = v, b = v;
+  asm("s_nop 1\n\tv_permlane32_swap_b32 %0, %1\n\ts_nop 1" : "+v"(a), "+v"(b));
+  return float2{a, b};
+}
+__device__ __forceinline__ float sum_halves(float v) {
+  const float2 x = both_halves(v);
+  return x.x + x.y;
+}
 
 // Stores 4 consecutive values (d .. d + 3) of an output row of odim elements.
 template <class T>
@@ -392,7 +403,8 @@ struct Softmax {
     for (int n = 0; n < N; ++n)
 #pragma unroll
       for (int i = 0; i < 16; ++i) m = fmaxf(m, s[n][i]);
-    m = fmaxf(m, other_half(m)) * c;
+    const float2 halves = both_halves(m);
+    m = fmaxf(halves.x, halves.y) * c;
     if (__any(m > top)) {
       const float t = fmaxf(m, top);
       const float keep = t == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(top - t);
@@ -587,7 +599,7 @@ __global__ __launch_bounds__(256, NC * sizeof(T) > 24 ? 1 : 2) void attn_tile_ke
               sm.o[d] = mma(col_frag<T, NC>(tv + 32 * u * G::kRow, half, d, lane), pf, sm.o[d]);
           }
       });
-  float total = sm.total + other_half(sm.total);
+  float total = sum_halves(sm.total);
   if constexpr (WK > 1) {  // the second wave of a row group hands over its columns, maximum and sum
     auto& ml = lds.ml[0];
     float* const at = reinterpret_cast<float*>(&tiles[0][0][0]) + (w.wave & 1) * JoinTile<ND>::kFloats;
@@ -681,7 +693,7 @@ __global__ __launch_bounds__(256, NC * sizeof(T) > 16 ? 1 : 2) void attn_few_ker
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   }
   // join the waves: columns in LDS at the block's largest maximum, added by wave 0
-  const float total = sm.total + other_half(sm.total);
+  const float total = sum_halves(sm.total);
   if (h == 0) ml[wave][n32] = float2{sm.top, total};
   __syncthreads();
   float top = -INFINITY;
@@ -790,7 +802,7 @@ __global__ __launch_bounds__(256, NC * sizeof(T) > 16 ? 1 : 2) void attn_dq_kern
     for (int e = 0; e < NC; ++e)
 #pragma unroll
       for (int i = 0; i < 8; ++i) delta = fmaf(to_f32(T(gf[e][i])), to_f32(T(of[e][i])), delta);
-    delta += other_half(delta);
+    delta = sum_halves(delta);
   }
   lse = lse == -INFINITY ? INFINITY : lse * kLog2e;  // a row without states: terms of 0
   if (p.split == 0 && w.wk == 0 && h == 0 && r < a.rows) a.stats[int64_t(p.bh) * a.rows + r] = float2{lse, delta};
