@@ -88,6 +88,7 @@ struct AttnTile {
   static constexpr int kPiece = Elem<T>::kPiece;
   static constexpr int ND = (NC + 1) / 2;                     // 32-wide blocks of the output's dimensions
   static constexpr int kPieces = NC * 16 / kPiece;            // 16-byte pieces of a row that can hold dimensions
+  static constexpr int kLeast = NC == 2 ? 1 : NC == 8 ? 97 : 16 * NC - 15;  // dimensions this geometry is used for, at least
   static constexpr int kRow = (ND == 3 ? 4 : ND) * 32 * int(sizeof(T));
   __device__ __forceinline__ static int swizzle(int row) {
     const int high = kRow >= 256 ? row & 3 : kRow == 128 ? (row >> 1) & 1 : 0;
@@ -142,6 +143,18 @@ __device__ __forceinline__ typename Elem<T>::frag result_frag(const f32x16& v, i
   return f;
 }
 
+// The 16 bytes at row + d, zeros from dim on.  Without a branch, so that the loads around it stay countable: a piece past
+// dim reads the row's first one.  sure: d is below dim for every dim of the geometry.
+template <class T>
+__device__ __forceinline__ f32x4 load_16(const T* row, int d, int dim, bool sure) {
+  if (sure) return *reinterpret_cast<const f32x4*>(row + d);
+  const bool in = d < dim;
+  f32x4 v = *reinterpret_cast<const f32x4*>(row + (in ? d : 0));
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = in ? v[i] : 0.0f;
+  return v;
+}
+
 // Fragments of one row in global memory: pieces past dim are zero.
 template <class T, int NC>
 __device__ __forceinline__ void load_frags(const T* row, int dim, int h, typename Elem<T>::frag (&f)[NC]) {
@@ -150,11 +163,8 @@ __device__ __forceinline__ void load_frags(const T* row, int dim, int h, typenam
   for (int c = 0; c < NC; ++c) {
     f32x4 piece[8 / E];
 #pragma unroll
-    for (int p = 0; p < 8 / E; ++p) {
-      const int d = 16 * c + 8 * h + E * p;
-      piece[p] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-      if (d < dim) piece[p] = *reinterpret_cast<const f32x4*>(row + d);
-    }
+    for (int p = 0; p < 8 / E; ++p)
+      piece[p] = load_16(row, 16 * c + 8 * h + E * p, dim, 16 * c + 15 < AttnTile<T, NC>::kLeast);
     if constexpr (E == 8) {
       f[c] = __builtin_bit_cast(typename Elem<T>::frag, piece[0]);
     } else {
@@ -165,6 +175,16 @@ __device__ __forceinline__ void load_frags(const T* row, int dim, int h, typenam
       }
     }
   }
+}
+
+// A negative scale's sign goes into Q, so that the largest s c is c times the largest s.  (On the bits: this compiler made
+// the negation of a vector of halves that a select had produced unconditional.)
+template <class T, class F, int NC>
+__device__ __forceinline__ void take_sign(F (&f)[NC], float scale) {
+  typedef uint32_t words __attribute__((ext_vector_type(sizeof(F) / 4)));
+  const uint32_t flip = scale < 0.0f ? (sizeof(T) == 2 ? 0x80008000u : 0x80000000u) : 0u;
+#pragma unroll
+  for (int c = 0; c < NC; ++c) f[c] = __builtin_bit_cast(F, __builtin_bit_cast(words, f[c]) ^ flip);
 }
 
 // Where row r's query is: item-and-head base plus row offset, in elements.
@@ -187,10 +207,8 @@ struct Staged {
   __device__ __forceinline__ void load(const T* base, int64_t stride, int first, int last, int dim, int tid) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int id = tid + i * THREADS, row = id / G::kPieces, d = id % G::kPieces * G::kPiece;
-      piece[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-      if ((kTotal % THREADS == 0 || id < kTotal) && d < dim)
-        piece[i] = *reinterpret_cast<const f32x4*>(base + int64_t(min(first + row, last)) * stride + d);
+      const int id = tid + i * THREADS, row = min(id / G::kPieces, R - 1), d = id % G::kPieces * G::kPiece;
+      piece[i] = load_16(base + int64_t(min(first + row, last)) * stride, d, dim, G::kPieces * G::kPiece <= G::kLeast);
     }
   }
   // rows whose bit in `valid` is 0 become zero: what they hold must not reach a product
@@ -211,10 +229,23 @@ struct Staged {
 // Tiles of R rows straight from global memory to LDS (global_load_lds_dwordx4: an instruction of a wave writes the 1 KiB
 // of LDS at M0, lane l its bytes 16 l ..), issued by the 4 waves of a block; no registers hold the data, and the
 // permutation of the layout is in the addresses.  Pieces past dim are not written: clear() makes them zero, once.
-// The compiler does not see these loads: dma_wait() before the barrier that hands a tile over.
+// The compiler does not see these loads: dma_wait() before the barrier that hands a tile over.  (The builtin, which the
+// compiler counts: after an assembly wait it would wait for earlier loads of its own, and so for these, inside the loop.)
 __device__ __attribute__((aligned(16))) const uint32_t g_attn_zero[4] = {0, 0, 0, 0};
 
-__device__ __forceinline__ void dma_wait() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+__device__ __forceinline__ void dma_wait() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
+  asm volatile("" ::: "memory");
+}
+
+// Fragments loaded before a loop, as used here: or the compiler waits for them at their first use inside it, every time,
+// and with them for the loop's own loads.
+template <class F, int N>
+__device__ __forceinline__ void settle(F (&f)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) asm volatile("" : "+v"(f[i]));
+}
 
 template <class T, int NC, int R>
 struct Dma {
@@ -557,11 +588,7 @@ __global__ __launch_bounds__(256, NC * sizeof(T) > 24 ? 1 : 2) void attn_tile_ke
     load_frags<T, NC>(static_cast<const T*>(a.q) + p.item * a.qs[0] + at.query * a.qs[1] + at.head * a.qs[2], a.dim, h,
                       qf);
   }
-  // a negative scale's sign goes into Q, so that the largest s c is c times the largest s
-  if (a.scale < 0.0f) {
-#pragma unroll
-    for (int c = 0; c < NC; ++c) qf[c] = -qf[c];
-  }
+  take_sign<T>(qf, a.scale);
   const float c = fmaxf(fabsf(a.scale) * kLog2e, 1.2e-38f);  // above 0, or a masked result's -inf would become NaN
   Softmax<ND> sm;
   sm.clear();
@@ -651,10 +678,7 @@ __global__ __launch_bounds__(256, NC * sizeof(T) > 16 ? 1 : 2) void attn_few_ker
     load_frags<T, NC>(static_cast<const T*>(a.q) + p.item * a.qs[0] + at.query * a.qs[1] + at.head * a.qs[2], a.dim, h,
                       qf);
   }
-  if (a.scale < 0.0f) {
-#pragma unroll
-    for (int c = 0; c < NC; ++c) qf[c] = -qf[c];
-  }
+  take_sign<T>(qf, a.scale);
   const float c = fmaxf(fabsf(a.scale) * kLog2e, 1.2e-38f);  // above 0, or a masked result's -inf would become NaN
   Softmax<ND> sm;
   sm.clear();
@@ -665,21 +689,21 @@ __global__ __launch_bounds__(256, NC * sizeof(T) > 16 ? 1 : 2) void attn_few_ker
   int first = begin + 32 * wave;
   Staged<T, NC, 32, 64> sv;
   typename Elem<T>::frag kf[NC];
-  uint32_t bits = 0;
+  int byte = 1;
   if (first < end) {
     load_frags<T, NC>(k + int64_t(min(first + n32, end - 1)) * a.ks[1], a.dim, h, kf);
     sv.load(v, a.vs[1], first, end - 1, a.dim, lane);
-    bits = uint32_t(key_bits<32>(key_byte(a, p.item, first, lane), first, end, lane));
+    byte = key_byte(a, p.item, first, lane);
   }
   for (; first < end; first += 128) {
-    const uint32_t now = bits;
+    const uint32_t now = uint32_t(key_bits<32>(byte, first, end, lane));
     f32x16 s[1] = {f32x16{}};
 #pragma unroll
     for (int e = 0; e < NC; ++e) s[0] = mma(kf[e], qf[e], s[0]);
     load_frags<T, NC>(k + int64_t(min(first + 128 + n32, end - 1)) * a.ks[1], a.dim, h, kf);
     sv.store(mine, now, lane);
     sv.load(v, a.vs[1], first + 128, end - 1, a.dim, lane);
-    bits = uint32_t(key_bits<32>(key_byte(a, p.item, first + 128, lane), first + 128, end, lane));
+    byte = key_byte(a, p.item, first + 128, lane);
     if (!now) continue;
     if (now != ~uint32_t(0)) mask_result(s[0], now, h, -INFINITY);
     sm.take(s, c);
@@ -942,64 +966,66 @@ __global__ __launch_bounds__(256, NC * sizeof(T) > 8 ? 1 : 2) void attn_dkv_kern
     }
   };
   auto hand_over = [&](int buf) {
+    dma_wait();
     if (tid < RT) {
       row_lse[buf][tid] = Terms<T>::kLog2 - st.x;  // both negated, as the sums take them
       row_delta[buf][tid] = -st.y;
     }
-    dma_wait();
     __syncthreads();
   };
   if (steps > 0) {
     clear_tiles<T, NC>(&tiles[0][0][0], 4 * RT * G::kRow, a.dim);
     load(begin, 0);
     hand_over(0);
-  }
-  for (int t = 0; t < steps; ++t) {
-    if (t + 1 < steps) load(begin + (t + 1) * RT, (t + 1) & 1);
-    if (active) {
-#pragma unroll
-      for (int u = 0; u < SUB; ++u) {
-        const uint8_t* const tq = tiles[t & 1][0] + 32 * u * G::kRow;
-        const uint8_t* const tg = tiles[t & 1][1] + 32 * u * G::kRow;
-        f32x16 s{}, dp;  // dP's sums begin at -delta
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const f32x4 w = *reinterpret_cast<const f32x4*>(&row_delta[t & 1][32 * u + 8 * j + 4 * h]);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) dp[4 * j + i] = w[i];
-        }
-#pragma unroll
-        for (int e = 0; e < NC; ++e) {
-          s = mma(row_frag<T, NC>(tq, n32, e, h), kf[e], s);
-          dp = mma(row_frag<T, NC>(tg, n32, e, h), vf[e], dp);
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const f32x4 l = *reinterpret_cast<const f32x4*>(&row_lse[t & 1][32 * u + 8 * j + 4 * h]);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            s[4 * j + i] = __builtin_amdgcn_exp2f(fmaf(s[4 * j + i], c, l[i]));
-            dp[4 * j + i] *= s[4 * j + i];
+    settle(kf);
+    settle(vf);
+    for (int t = 0; t < steps; ++t) {
+      if (t + 1 < steps) load(begin + (t + 1) * RT, (t + 1) & 1);
+      if (active) {
+  #pragma unroll
+        for (int u = 0; u < SUB; ++u) {
+          const uint8_t* const tq = tiles[t & 1][0] + 32 * u * G::kRow;
+          const uint8_t* const tg = tiles[t & 1][1] + 32 * u * G::kRow;
+          f32x16 s{}, dp;  // dP's sums begin at -delta
+  #pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const f32x4 w = *reinterpret_cast<const f32x4*>(&row_delta[t & 1][32 * u + 8 * j + 4 * h]);
+  #pragma unroll
+            for (int i = 0; i < 4; ++i) dp[4 * j + i] = w[i];
           }
-        }
-        const float rescale = fit_terms<T>(dp, shrink, counts);
-        if (rescale != 1.0f) {
-#pragma unroll
-          for (int d = 0; d < ND; ++d) dk[d] *= rescale;
-        }
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const auto pf = result_frag<T>(s, half);
-          const auto sf = result_frag<T>(dp, half);
-#pragma unroll
-          for (int d = 0; d < ND; ++d) {
-            dv[d] = mma(col_frag<T, NC>(tg, half, d, lane), pf, dv[d]);
-            dk[d] = mma(col_frag<T, NC>(tq, half, d, lane), sf, dk[d]);
+  #pragma unroll
+          for (int e = 0; e < NC; ++e) {
+            s = mma(row_frag<T, NC>(tq, n32, e, h), kf[e], s);
+            dp = mma(row_frag<T, NC>(tg, n32, e, h), vf[e], dp);
+          }
+  #pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const f32x4 l = *reinterpret_cast<const f32x4*>(&row_lse[t & 1][32 * u + 8 * j + 4 * h]);
+  #pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              s[4 * j + i] = __builtin_amdgcn_exp2f(fmaf(s[4 * j + i], c, l[i]));
+              dp[4 * j + i] *= s[4 * j + i];
+            }
+          }
+          const float rescale = fit_terms<T>(dp, shrink, counts);
+          if (rescale != 1.0f) {
+  #pragma unroll
+            for (int d = 0; d < ND; ++d) dk[d] *= rescale;
+          }
+  #pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const auto pf = result_frag<T>(s, half);
+            const auto sf = result_frag<T>(dp, half);
+  #pragma unroll
+            for (int d = 0; d < ND; ++d) {
+              dv[d] = mma(col_frag<T, NC>(tg, half, d, lane), pf, dv[d]);
+              dk[d] = mma(col_frag<T, NC>(tq, half, d, lane), sf, dk[d]);
+            }
           }
         }
       }
+      hand_over((t + 1) & 1);
     }
-    hand_over((t + 1) & 1);
   }
   if (key >= a.keys) return;
   const float fv = __builtin_amdgcn_exp2f(-Terms<T>::kLog2), fk = a.scale * fv / shrink;
