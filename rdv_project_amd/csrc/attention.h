@@ -414,7 +414,12 @@ __device__ __forceinline__ void store_quad(T* row, int d, int odim, float x0, fl
 
 // ------------------------------------------------------------------ forward
 
-// The online softmax of a lane's column: maximum (of s c, log2), sum of this half's terms, output accumulators.
+// The online softmax of a lane's column: reference (of s c, log2), sum of this half's terms, output accumulators.  The
+// reference follows the running maximum from up to kSlack below, so terms reach 2^kSlack: of 32 columns of a wave one
+// has a new maximum in most tiles, and only some of those need the accumulators rescaled.  (Rescaled at each new
+// maximum, 64 dimensions in fp16 over 1,024 states spent a third of their vector instructions on it.)
+constexpr float kSlack = 8.0f;
+
 template <int ND>
 struct Softmax {
   float top, total;
@@ -436,7 +441,7 @@ struct Softmax {
       for (int i = 0; i < 16; ++i) m = fmaxf(m, s[n][i]);
     const float2 halves = both_halves(m);
     m = fmaxf(halves.x, halves.y) * c;
-    if (__any(m > top)) {
+    if (__any(m > top + kSlack)) {
       const float t = fmaxf(m, top);
       const float keep = t == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(top - t);
       top = t;
