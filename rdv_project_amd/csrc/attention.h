@@ -495,6 +495,9 @@ __device__ __forceinline__ void finish_row(const AttnArgs& a, const BlockAt& p, 
   if (a.lse && h == 0) a.lse[row] = total == 0.0f ? -INFINITY : (sm.top + __builtin_amdgcn_logf(total)) * kLn2;
 }
 
+// s_setprio around the products: a wave with matrix instructions to issue goes first, so that the waves of a SIMD come to
+// alternate between products and softmax (547 -> 535 us for 2 x 16,384 x 4,096 x 8 heads of 128 in bf16).
+//
 // Many rows: a block of 4 waves, 32 rows each (or 64 rows shared by pairs of waves), walks its share of the states in
 // tiles of KT in LDS (two buffers, one barrier per tile: the next tile's loads are in flight under this tile's products).
 template <class T, int NC>
@@ -610,17 +613,20 @@ __global__ __launch_bounds__(256, NC * sizeof(T) > 24 ? 1 : 2) void attn_tile_ke
         }
         if (!active) return;
         f32x16 s[SUB];
+        __builtin_amdgcn_s_setprio(1);
 #pragma unroll
         for (int u = 0; u < SUB; ++u) s[u] = f32x16{};
 #pragma unroll
         for (int e = 0; e < NC; ++e)
 #pragma unroll
           for (int u = 0; u < SUB; ++u) s[u] = mma(row_frag<T, NC>(tk + 32 * u * G::kRow, n32, e, h), qf[e], s[u]);
+        __builtin_amdgcn_s_setprio(0);
         if (now != (SUB == 2 ? ~uint64_t(0) : uint64_t(~uint32_t(0)))) {
 #pragma unroll
           for (int u = 0; u < SUB; ++u) mask_result(s[u], uint32_t(now >> (32 * u)), h, -INFINITY);
         }
         sm.take(s, c);
+        __builtin_amdgcn_s_setprio(1);
 #pragma unroll
         for (int u = 0; u < SUB; ++u)
 #pragma unroll
@@ -630,6 +636,7 @@ __global__ __launch_bounds__(256, NC * sizeof(T) > 24 ? 1 : 2) void attn_tile_ke
             for (int d = 0; d < ND; ++d)
               sm.o[d] = mma(col_frag<T, NC>(tv + 32 * u * G::kRow, half, d, lane), pf, sm.o[d]);
           }
+        __builtin_amdgcn_s_setprio(0);
       });
   float total = sum_halves(sm.total);
   if constexpr (WK > 1) {  // the second wave of a row group hands over its columns, maximum and sum
@@ -766,8 +773,8 @@ __global__ __launch_bounds__(256, NC * sizeof(T) > 16 ? 1 : 2) void attn_few_ker
 // ------------------------------------------------------------------ backward
 
 // Softmax terms and dS in fp16.  A term is at most 1 and typically 1 / states, so it is kept times 2^14: below fp16's
-// normal range (2^-14) only from 2^-28 on.  dS (with that factor) can exceed fp16's range; `shrink` is a power of two
-// that a column's accumulator is held at, lowered when a value would not fit, so no gradient overflows inside.
+// normal range (2^-14) only from 2^-28 on.  dS (with that factor) can exceed fp16's range; then the factor and what is
+// summed with it so far are lowered by a power of two, so no gradient overflows inside.
 template <class T>
 struct Terms {
   static constexpr float kLog2 = 0.0f;
@@ -777,27 +784,21 @@ struct Terms<half_t> {
   static constexpr float kLog2 = 14.0f;
 };
 
-// dS's factor for a wave's tile: 1 but for fp16.  Returns by how much the accumulators have to be scaled.
+// Whether a wave's dS fits fp16 with room for its rounding; else the power of two that makes it fit (other types always
+// fit).  `counts`: the column is used.
 template <class T>
-__device__ __forceinline__ float fit_terms(f32x16& ds, float& shrink, bool counts) {
+__device__ __forceinline__ float fit_terms(const f32x16& ds, bool counts) {
   if constexpr (Terms<T>::kLog2 != 0.0f) {
     float most = 0.0f;
 #pragma unroll
     for (int i = 0; i < 16; ++i) most = fmaxf(most, fabsf(ds[i]));
-    if (!counts) most = 0.0f;  // a column that is not used
-    float rescale = 1.0f;
-    if (__any(most * shrink > 32768.0f)) {
+    // an infinity is its column's own: no factor helps it, and the others keep theirs
+    most = counts && most < INFINITY ? most : 0.0f;
+    if (__builtin_expect(__any(most > 32768.0f), 0)) {
       for (int o = 32; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor(most, o));
-      while (most * shrink > 32768.0f && shrink > 1e-30f) {
-        shrink *= 0.0625f;
-        rescale *= 0.0625f;
-      }
+      const int bits = __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, most));
+      return __builtin_bit_cast(float, (127 + 14 + 127 - ((bits >> 23) & 255)) << 23);  // 2^(14 - e) for 2^e <= most < 2^(e + 1)
     }
-    if (shrink != 1.0f) {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) ds[i] *= shrink;
-    }
-    return rescale;
   }
   return 1.0f;
 }
@@ -835,11 +836,11 @@ __global__ __launch_bounds__(256, NC * sizeof(T) > 16 ? 1 : 2) void attn_dq_kern
   }
   lse = lse == -INFINITY ? INFINITY : lse * kLog2e;  // a row without states: terms of 0
   if (p.split == 0 && w.wk == 0 && h == 0 && r < a.rows) a.stats[int64_t(p.bh) * a.rows + r] = float2{lse, delta};
-  const float c = a.scale * kLog2e, base = lse - Terms<T>::kLog2;
+  const float c = a.scale * kLog2e;
+  float base = lse - Terms<T>::kLog2, factor_log2 = Terms<T>::kLog2;
   f32x16 acc[ND];
 #pragma unroll
   for (int d = 0; d < ND; ++d) acc[d] = f32x16{};
-  float shrink = 1.0f;
   const int begin = p.split * a.chunk, end = min(begin + a.chunk, key_limit(a, p.item));
   walk_keys<T, NC, KT>(
       a, p, static_cast<const T*>(a.k) + p.item * a.ks[0] + p.hk * a.ks[2],
@@ -853,28 +854,35 @@ __global__ __launch_bounds__(256, NC * sizeof(T) > 16 ? 1 : 2) void attn_dq_kern
           const uint8_t* const uv = tv + 32 * sub * G::kRow;
           const uint32_t now = uint32_t(bits >> (32 * sub));
           f32x16 s{}, dp{};
+          __builtin_amdgcn_s_setprio(1);
 #pragma unroll
           for (int e = 0; e < NC; ++e) {
             s = mma(row_frag<T, NC>(uk, n32, e, h), qf[e], s);
             dp = mma(row_frag<T, NC>(uv, n32, e, h), gf[e], dp);
           }
+          __builtin_amdgcn_s_setprio(0);
 #pragma unroll
           for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], c, -base)) * (dp[i] - delta);
           if (now != ~uint32_t(0)) mask_result(s, now, h, 0.0f);
-          const float rescale = fit_terms<T>(s, shrink, true);
-          if (rescale != 1.0f) {
+          const float fit = fit_terms<T>(s, true);
+          if (fit != 1.0f) {
+            s *= fit;
+            base -= __builtin_amdgcn_logf(fit);
+            factor_log2 += __builtin_amdgcn_logf(fit);
 #pragma unroll
-            for (int d = 0; d < ND; ++d) acc[d] *= rescale;
+            for (int d = 0; d < ND; ++d) acc[d] *= fit;
           }
+          __builtin_amdgcn_s_setprio(1);
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
             const auto sf = result_frag<T>(s, half);
 #pragma unroll
             for (int d = 0; d < ND; ++d) acc[d] = mma(col_frag<T, NC>(uk, half, d, lane), sf, acc[d]);
           }
+          __builtin_amdgcn_s_setprio(0);
         }
       });
-  float f = a.scale * __builtin_amdgcn_exp2f(-Terms<T>::kLog2) / shrink;
+  float f = a.scale * __builtin_amdgcn_exp2f(-factor_log2);
   if constexpr (WK > 1) {
     auto& factor = lds.factor[0];
     float* const place = reinterpret_cast<float*>(&tiles[0][0][0]) + (w.wave & 1) * JoinTile<ND>::kFloats;
@@ -941,7 +949,7 @@ __global__ __launch_bounds__(256, NC * sizeof(T) > 8 ? 1 : 2) void attn_dkv_kern
   f32x16 dk[ND], dv[ND];
 #pragma unroll
   for (int d = 0; d < ND; ++d) dk[d] = dv[d] = f32x16{};
-  float shrink = 1.0f;
+  float shrink = 1.0f;  // of dK's terms, as they have come to need it
 
   const int begin = p.split * a.chunk, end = key0 < limit ? min(begin + a.chunk, a.rows) : begin;
   const int steps = end > begin ? (end - begin + RT - 1) / RT : 0;
@@ -998,11 +1006,13 @@ __global__ __launch_bounds__(256, NC * sizeof(T) > 8 ? 1 : 2) void attn_dkv_kern
   #pragma unroll
             for (int i = 0; i < 4; ++i) dp[4 * j + i] = w[i];
           }
-  #pragma unroll
+            __builtin_amdgcn_s_setprio(1);
+#pragma unroll
           for (int e = 0; e < NC; ++e) {
             s = mma(row_frag<T, NC>(tq, n32, e, h), kf[e], s);
             dp = mma(row_frag<T, NC>(tg, n32, e, h), vf[e], dp);
           }
+          __builtin_amdgcn_s_setprio(0);
   #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const f32x4 l = *reinterpret_cast<const f32x4*>(&row_lse[t & 1][32 * u + 8 * j + 4 * h]);
@@ -1012,21 +1022,26 @@ __global__ __launch_bounds__(256, NC * sizeof(T) > 8 ? 1 : 2) void attn_dkv_kern
               dp[4 * j + i] *= s[4 * j + i];
             }
           }
-          const float rescale = fit_terms<T>(dp, shrink, counts);
-          if (rescale != 1.0f) {
-  #pragma unroll
-            for (int d = 0; d < ND; ++d) dk[d] *= rescale;
+          if (shrink != 1.0f) dp *= shrink;
+          const float fit = fit_terms<T>(dp, counts);
+          if (fit != 1.0f) {
+            dp *= fit;
+            shrink *= fit;
+#pragma unroll
+            for (int d = 0; d < ND; ++d) dk[d] *= fit;
           }
-  #pragma unroll
+          __builtin_amdgcn_s_setprio(1);
+#pragma unroll
           for (int half = 0; half < 2; ++half) {
             const auto pf = result_frag<T>(s, half);
             const auto sf = result_frag<T>(dp, half);
-  #pragma unroll
+#pragma unroll
             for (int d = 0; d < ND; ++d) {
               dv[d] = mma(col_frag<T, NC>(tg, half, d, lane), pf, dv[d]);
               dk[d] = mma(col_frag<T, NC>(tq, half, d, lane), sf, dk[d]);
             }
           }
+          __builtin_amdgcn_s_setprio(0);
         }
       }
       hand_over((t + 1) & 1);

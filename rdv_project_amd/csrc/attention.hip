@@ -154,24 +154,27 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a, int per) {
   if (a.lse && l == 0) a.lse[row] = total == 0.0f ? -INFINITY : (top + __builtin_amdgcn_logf(total)) * kLn2;
 }
 
-// The sum of the splits of dQ (KEYS false: rows of the queries) or of dK and dV (KEYS true: z picks the tensor).
+// The sum of the splits of dQ (KEYS false: rows of the queries) or of dK and dV (KEYS true: blockIdx.y picks the tensor),
+// four dimensions per thread.
 template <class T, bool KEYS>
 __global__ __launch_bounds__(256) void attn_sum_kernel(AttnArgs a) {
-  const int64_t len = KEYS ? a.keys : a.rows, n = int64_t(a.batch) * a.kv_heads * len * a.pdim;
-  const int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x;
-  if (i >= n) return;
-  const float* const part = KEYS && blockIdx.y ? a.part2 : a.part;
-  float sum = 0.0f;
-  for (int s = 0; s < a.splits; ++s) sum += part[s * n + i];
-  const int64_t row = i / a.pdim, d = i - row * a.pdim;
-  if (d >= a.odim) return;
-  const int bh = int(row / len), x = int(row - int64_t(bh) * len), item = bh / a.kv_heads, hk = bh - item * a.kv_heads;
+  const uint32_t len = KEYS ? a.keys : a.rows, quads = uint32_t(a.pdim) / 4;
+  const uint32_t i = blockIdx.x * 256 + threadIdx.x, row = i / quads, d = 4 * (i - row * quads);
+  const int64_t n = int64_t(a.batch) * a.kv_heads * len;
+  if (row >= n) return;
+  const f32x4* part = reinterpret_cast<const f32x4*>(KEYS && blockIdx.y ? a.part2 : a.part) + int64_t(row) * quads + d / 4;
+  f32x4 sum{};
+#pragma unroll 4
+  for (int s = 0; s < a.splits; ++s) sum += part[s * n * quads];
+  const int bh = int(row / len), x = int(row - bh * len), item = bh / a.kv_heads, hk = bh - item * a.kv_heads;
+  T* out;
   if constexpr (KEYS) {
-    static_cast<T*>(blockIdx.y ? a.dv : a.dk)[((int64_t(item) * a.keys + x) * a.kv_heads + hk) * a.odim + d] = T(sum);
+    out = static_cast<T*>(blockIdx.y ? a.dv : a.dk) + ((int64_t(item) * a.keys + x) * a.kv_heads + hk) * a.odim;
   } else {
     const RowAt at = row_at(a, hk, x);
-    static_cast<T*>(a.dq)[((int64_t(item) * a.queries + at.query) * a.heads + at.head) * a.odim + d] = T(sum);
+    out = static_cast<T*>(a.dq) + ((int64_t(item) * a.queries + at.query) * a.heads + at.head) * a.odim;
   }
+  store_quad(out, int(d), a.odim, sum[0], sum[1], sum[2], sum[3]);
 }
 
 __global__ __launch_bounds__(256) void attn_zero_kernel(uint16_t* p, int64_t n) {
@@ -315,8 +318,7 @@ int launch_attention_backward(const rdv_attention_desc& d, const void* grad, con
   a.dk = dk;
   a.dv = dv;
   const int64_t n = p.bh * p.rows;
-  const int64_t sums = (std::max(n, p.bh * int64_t(d.keys)) * p.pdim + 255) / 256;
-  if (sums >= (int64_t(1) << 31)) return fail(RDV_ERR_UNSUPPORTED, "attention: too many rows");
+  if (std::max(n, p.bh * int64_t(d.keys)) * (p.pdim / 4) >= (int64_t(1) << 32) - 256) return fail(RDV_ERR_UNSUPPORTED, "attention: too many rows");
   a.tiles = p.row_tiles;
   a.splits = p.dq.count;
   a.chunk = p.dq.chunk;
@@ -325,7 +327,7 @@ int launch_attention_backward(const rdv_attention_desc& d, const void* grad, con
   if (rc != RDV_OK) return rc;
   if (a.splits > 1) {
     rc = with_dtype(d.dtype, [&](auto t) {
-      attn_sum_kernel<decltype(t), false><<<dim3(unsigned((n * p.pdim + 255) / 256)), 256, 0, stream>>>(a);
+      attn_sum_kernel<decltype(t), false><<<dim3(unsigned((n * (p.pdim / 4) + 255) / 256)), 256, 0, stream>>>(a);
       RDV_HIP_TRY(hipGetLastError());
       return int(RDV_OK);
     });
@@ -338,7 +340,7 @@ int launch_attention_backward(const rdv_attention_desc& d, const void* grad, con
   rc = launch_matrix(d.dtype, kAttnDkv, a, cu, stream);
   if (rc != RDV_OK || a.splits == 1) return rc;
   return with_dtype(d.dtype, [&](auto t) {
-    attn_sum_kernel<decltype(t), true><<<dim3(unsigned((p.bh * d.keys * p.pdim + 255) / 256), 2), 256, 0, stream>>>(a);
+    attn_sum_kernel<decltype(t), true><<<dim3(unsigned((p.bh * d.keys * (p.pdim / 4) + 255) / 256), 2), 256, 0, stream>>>(a);
     RDV_HIP_TRY(hipGetLastError());
     return int(RDV_OK);
   });

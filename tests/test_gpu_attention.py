@@ -179,6 +179,24 @@ def test_small_half_precision_gradients():
 
 
 @pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("value", [float("inf"), float("nan")])
+def test_bad_rows_stay_alone(dtype, value):
+    """An infinity or NaN of one query, or of its gradient, reaches that query's results only (and every state's gradient)."""
+    q, k, v, g = _inputs(1, 200, 300, 2, 1, 64, dtype)
+    out, lse = rdv.cross_attention(q, k, v, return_lse=True)
+    dq, _, _ = rdv.cross_attention_backward(g, q, k, v, out, lse)
+    others = torch.arange(200) != 37
+    bad = q.clone()
+    bad[0, 37] = value
+    assert torch.equal(rdv.cross_attention(bad, k, v)[0, others], out[0, others])
+    bad = g.clone()
+    bad[0, 37, :, 3] = value
+    got, _, dv = rdv.cross_attention_backward(bad, q, k, v, out, lse)
+    assert torch.equal(got[0, others], dq[0, others])
+    assert not torch.isfinite(got[0, 37].float()).all() and not torch.isfinite(dv[..., 3].float()).any()
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
 @pytest.mark.parametrize("shape", [(1, 2048, 77, 2, 2, 64), (1, 300, 2500, 2, 1, 64), (2, 1000, 1030, 2, 1, 128),
                                    (1, 40, 9000, 1, 1, 32)])
 def test_longer(dtype, shape):
