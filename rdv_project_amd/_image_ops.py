@@ -17,7 +17,7 @@ import math
 import torch
 
 from . import _lib
-from .core import RDVObject, current_stream_handle, launch_scope
+from .core import RDVObject, launch_scope
 
 _DTYPES = {torch.float32: _lib.DTYPE_F32, torch.float16: _lib.DTYPE_F16, torch.bfloat16: _lib.DTYPE_BF16}
 _ACTIVATIONS = {"none": _lib.ACT_NONE, "relu": _lib.ACT_RELU, "silu": _lib.ACT_SILU}
@@ -49,19 +49,22 @@ def _like(t, x: torch.Tensor, what: str) -> torch.Tensor:
 
 def _gpu_index() -> int:
     """The current GPU, or -1 where there is none (arguments are still checked there)."""
-    return torch.cuda.current_device() if torch.cuda.is_initialized() else -1
+    return torch._C._cuda_getDevice() if torch.cuda.is_initialized() else -1
 
 
-def _on_gpu(*named) -> None:
+def _stream(device: int) -> int:
+    """The handle of the device's current stream."""
+    return torch._C._cuda_getCurrentRawStream(device)
+
+
+def _on_gpu(device: int, *named) -> None:
     """Every tensor (followed by its name) on the current GPU: launches go there, on its current stream."""
-    current = _gpu_index()
-    for t, what in zip(named[::2], named[1::2]):
-        if t is not None and t.get_device() != current:
+    for i in range(0, len(named), 2):
+        t = named[i]
+        if t is not None and (t.get_device() != device or device < 0):
             if not t.is_cuda:
-                raise TypeError(f"{what} must be a GPU tensor, got device {t.device}")
-            raise TypeError(f"{what} is on {t.device}, the current GPU is cuda:{current}")
-        if t is not None and current < 0:
-            raise TypeError(f"{what} must be a GPU tensor, got device {t.device}")
+                raise TypeError(f"{named[i + 1]} must be a GPU tensor, got device {t.device}")
+            raise TypeError(f"{named[i + 1]} is on {t.device}, the current GPU is cuda:{device}")
 
 
 def _like_out(out, x: torch.Tensor, aligned: bool = True) -> torch.Tensor:
@@ -174,14 +177,14 @@ def _norm_inputs(x, weight, bias):
     return x, _norm_param(weight, x, "weight"), _norm_param(bias, x, "bias")
 
 
-def _group_norm_into(plan, x, weight, bias, y, stats) -> None:
+def _group_norm_into(plan, x, weight, bias, y, stats, device: int) -> None:
     """Launches rdv_group_norm into y and stats (or None)."""
     d, copy, _, nbytes = plan
     if copy:
         x = x.contiguous()
     ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
     _check(_lib.load().rdv_group_norm(C.byref(d), x.data_ptr(), _ptr(weight), _ptr(bias), y.data_ptr(), _ptr(stats),
-                                      _ptr(ws), nbytes, current_stream_handle()), "group_norm")
+                                      _ptr(ws), nbytes, _stream(device)), "group_norm")
 
 
 def group_norm(x, weight, bias, groups: int, eps: float = 1e-5, activation: str = "none", out=None,
@@ -195,8 +198,9 @@ def group_norm(x, weight, bias, groups: int, eps: float = 1e-5, activation: str 
     return_stats also stats [images, groups, 2] = (mean, 1 / std) in float32,
     which group_norm_backward takes."""
     x, weight, bias = _norm_inputs(x, weight, bias)
-    plan = _norm_plan(x.shape, x.stride(), None, x.dtype, int(groups), float(eps), activation, _gpu_index())
-    _on_gpu(x, "x", weight, "weight", bias, "bias")
+    device = _gpu_index()
+    plan = _norm_plan(x.shape, x.stride(), None, x.dtype, int(groups), float(eps), activation, device)
+    _on_gpu(device, x, "x", weight, "weight", bias, "bias")
     y = _like_out(out, x)
     if out is not None:
         _apart(y, (x, "x"), (weight, "weight"), (bias, "bias"))
@@ -204,7 +208,7 @@ def group_norm(x, weight, bias, groups: int, eps: float = 1e-5, activation: str 
     if return_stats:
         stats = torch.empty((plan[0].images, plan[0].groups, 2), dtype=torch.float32, device=x.device)
     with launch_scope():
-        _group_norm_into(plan, x, weight, bias, y, stats)
+        _group_norm_into(plan, x, weight, bias, y, stats, device)
     return (y, stats) if return_stats else y
 
 
@@ -215,14 +219,15 @@ def group_norm_backward(grad, x, weight, bias, groups: int, stats, activation: s
     buffers."""
     x, weight, bias = _norm_inputs(x, weight, bias)
     grad = _like(grad, x, "grad")
+    device = _gpu_index()
     d, copy_x, copy_g, nbytes = _norm_plan(x.shape, x.stride(), grad.stride(), x.dtype, int(groups), 0.0, activation,
-                                           _gpu_index())
+                                           device)
     stats = _tensor(stats, "stats")
     assert tuple(stats.shape) == (d.images, d.groups, 2) and stats.is_contiguous(), \
         f"stats must be a contiguous [{d.images}, {d.groups}, 2] tensor, as group_norm returns it"
     if stats.dtype != torch.float32:
         raise TypeError(f"stats must be float32, got {stats.dtype}")
-    _on_gpu(x, "x", grad, "grad", weight, "weight", bias, "bias", stats, "stats")
+    _on_gpu(device, x, "x", grad, "grad", weight, "weight", bias, "bias", stats, "stats")
     param = weight if weight is not None else bias
     if param is None:
         param = torch.empty(d.channels, dtype=torch.float32, device=x.device)
@@ -238,7 +243,7 @@ def group_norm_backward(grad, x, weight, bias, groups: int, stats, activation: s
         ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
         _check(_lib.load().rdv_group_norm_backward(C.byref(d), grad.data_ptr(), x.data_ptr(), _ptr(weight), _ptr(bias),
                                                    stats.data_ptr(), dx.data_ptr(), dw.data_ptr(), db.data_ptr(),
-                                                   _ptr(ws), nbytes, current_stream_handle()), "group_norm_backward")
+                                                   _ptr(ws), nbytes, _stream(device)), "group_norm_backward")
     return dx, dw, db
 
 
@@ -297,29 +302,30 @@ def _attention_inputs(q, k, v, key_lengths, key_mask, scale, grad=None):
         if key_mask.stride(1) != 1:
             key_mask = key_mask.contiguous()
         mask_stride = key_mask.stride(0)
+    device = _gpu_index()
     plan = _attention_plan(q.shape, k.shape, v.shape, q.stride(), k.stride(), v.stride(),
                            None if grad is None else grad.stride(), mask_stride, q.dtype,
-                           None if scale is None else float(scale), _gpu_index())
+                           None if scale is None else float(scale), device)
     if key_lengths is not None:
         key_lengths = _tensor(key_lengths, "key_lengths")
         assert tuple(key_lengths.shape) == (q.shape[0],), f"key_lengths must be [batch] = [{q.shape[0]}]"
         if key_lengths.dtype not in (torch.int32, torch.int64):
             raise TypeError(f"key_lengths must be int32 or int64, got {key_lengths.dtype}")
-    _on_gpu(q, "q", k, "k", v, "v", key_lengths, "key_lengths", key_mask, "key_mask", grad, "grad")
+    _on_gpu(device, q, "q", k, "k", v, "v", key_lengths, "key_lengths", key_mask, "key_mask", grad, "grad")
     if key_lengths is not None:
         if key_lengths.dtype == torch.int64:
             key_lengths = key_lengths.clamp(0, k.shape[1]).to(torch.int32)
         key_lengths = key_lengths.contiguous()
-    return q, k, v, key_lengths, key_mask, grad, plan
+    return q, k, v, key_lengths, key_mask, grad, plan, device
 
 
-def _cross_attention_into(plan, q, k, v, key_lengths, key_mask, out, lse) -> None:
+def _cross_attention_into(plan, q, k, v, key_lengths, key_mask, out, lse, device: int) -> None:
     """Launches rdv_cross_attention into out and lse (or None)."""
     d, nbytes = plan
     ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
     _check(_lib.load().rdv_cross_attention(C.byref(d), q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(key_lengths),
                                            _ptr(key_mask), out.data_ptr(), _ptr(lse), _ptr(ws), nbytes,
-                                           current_stream_handle()), "cross_attention")
+                                           _stream(device)), "cross_attention")
 
 
 def cross_attention(q, k, v, key_lengths=None, key_mask=None, scale: float | None = None, out=None,
@@ -337,7 +343,7 @@ def cross_attention(q, k, v, key_lengths=None, key_mask=None, scale: float | Non
     cores take softmax terms rounded to that type; float32: float32
     throughout."""
     given = q, k, v
-    q, k, v, key_lengths, key_mask, _, plan = _attention_inputs(q, k, v, key_lengths, key_mask, scale)
+    q, k, v, key_lengths, key_mask, _, plan, device = _attention_inputs(q, k, v, key_lengths, key_mask, scale)
     y = _like_out(out, q)
     if out is not None:
         _apart(y, (_tensor(given[0], "q"), "q"), (_tensor(given[1], "k"), "k"), (_tensor(given[2], "v"), "v"),
@@ -347,7 +353,7 @@ def cross_attention(q, k, v, key_lengths=None, key_mask=None, scale: float | Non
         d = plan[0]
         lse = torch.empty((d.batch, d.heads, d.queries), dtype=torch.float32, device=q.device)
     with launch_scope():
-        _cross_attention_into(plan, q, k, v, key_lengths, key_mask, y, lse)
+        _cross_attention_into(plan, q, k, v, key_lengths, key_mask, y, lse, device)
     return (y, lse) if return_lse else y
 
 
@@ -357,14 +363,15 @@ def cross_attention_backward(grad, q, k, v, out, lse, key_lengths=None, key_mask
     it returned for the same arguments.  dk and dv are summed over the heads
     that share a state head and are 0 at states that do not count; `grads`
     supplies the three buffers."""
-    q, k, v, key_lengths, key_mask, grad, (d, nbytes) = _attention_inputs(q, k, v, key_lengths, key_mask, scale, grad)
+    q, k, v, key_lengths, key_mask, grad, (d, nbytes), device = _attention_inputs(q, k, v, key_lengths, key_mask, scale,
+                                                                                  grad)
     out = _like(out, q, "out").contiguous()
     lse = _tensor(lse, "lse")
     assert tuple(lse.shape) == (d.batch, d.heads, d.queries) and lse.is_contiguous(), \
         f"lse must be a contiguous [{d.batch}, {d.heads}, {d.queries}] tensor, as cross_attention returns it"
     if lse.dtype != torch.float32:
         raise TypeError(f"lse must be float32, got {lse.dtype}")
-    _on_gpu(out, "out", lse, "lse")
+    _on_gpu(device, out, "out", lse, "lse")
     given = grads is not None
     dq, dk, dv = _grad_tensors(grads, (q, k, v), ("dq", "dk", "dv"))
     if given:
@@ -377,7 +384,7 @@ def cross_attention_backward(grad, q, k, v, out, lse, key_lengths=None, key_mask
                                                         v.data_ptr(), out.data_ptr(), lse.data_ptr(),
                                                         _ptr(key_lengths), _ptr(key_mask), dq.data_ptr(),
                                                         dk.data_ptr(), dv.data_ptr(), _ptr(ws), nbytes,
-                                                        current_stream_handle()), "cross_attention_backward")
+                                                        _stream(device)), "cross_attention_backward")
     return dq, dk, dv
 
 
@@ -395,12 +402,12 @@ def _dropout_inputs(x, p, seed, subsequence):
     return x, p, seed, subsequence
 
 
-def _dropout_into(x, p, seed, subsequence, residual, y) -> None:
+def _dropout_into(x, p, seed, subsequence, residual, y, device: int) -> None:
     """Launches rdv_dropout into y."""
     x = x.contiguous()
     residual = None if residual is None else residual.contiguous()
     _check(_lib.load().rdv_dropout(x.data_ptr(), _ptr(residual), y.data_ptr(), x.numel(), _DTYPES[x.dtype], p, seed,
-                                   subsequence, current_stream_handle()), "dropout")
+                                   subsequence, _stream(device)), "dropout")
 
 
 def dropout(x, p: float, seed: int, subsequence: int = 0, residual=None, out=None):
@@ -414,14 +421,15 @@ def dropout(x, p: float, seed: int, subsequence: int = 0, residual=None, out=Non
     x, p, seed, subsequence = _dropout_inputs(x, p, seed, subsequence)
     if residual is not None:
         residual = _like(residual, x, "residual")
-    _on_gpu(x, "x", residual, "residual")
+    device = _gpu_index()
+    _on_gpu(device, x, "x", residual, "residual")
     y = _like_out(out, x, aligned=False)
     if out is not None:
         for t, what in ((x, "x"), (residual, "residual")):
             if t is not None and not (t.data_ptr() == y.data_ptr() and t.is_contiguous()):
                 _apart(y, (t, what))
     with launch_scope():
-        _dropout_into(x, p, seed, subsequence, residual, y)
+        _dropout_into(x, p, seed, subsequence, residual, y, device)
     return y
 
 

@@ -610,7 +610,7 @@ class GroupNormTensorOp(TensorOperation):
                                      _image_ops._gpu_index()), x, weight, bias
 
     def _forward(self) -> None:
-        _image_ops._group_norm_into(*self._inputs(), self._result_t, None)
+        _image_ops._group_norm_into(*self._inputs(), self._result_t, None, _image_ops._gpu_index())
 
 
 class CrossAttentionTensorOp(TensorOperation):
@@ -643,8 +643,8 @@ class CrossAttentionTensorOp(TensorOperation):
     def _forward(self) -> None:
         q, k, v = (t.as_tensor("torch").unflatten(1, (h, self.D)).unsqueeze(0) for t, h in
                    ((self.q_buf, self.heads), (self.k_buf, self.kv_heads), (self.v_buf, self.kv_heads)))
-        q, k, v, _, _, _, plan = _image_ops._attention_inputs(q, k, v, None, None, None)
-        _image_ops._cross_attention_into(plan, q, k, v, None, None, self._result_t, None)
+        q, k, v, _, _, _, plan, device = _image_ops._attention_inputs(q, k, v, None, None, None)
+        _image_ops._cross_attention_into(plan, q, k, v, None, None, self._result_t, None, device)
 
 
 class DropoutTensorOp(TensorOperation):
@@ -673,4 +673,4 @@ class DropoutTensorOp(TensorOperation):
     def _forward(self) -> None:
         x, p, seed, subsequence = _image_ops._dropout_inputs(self.x_buf, self.p, self.seed, self.subsequence)
         residual = None if self.residual_buf is None else self.residual_buf.as_tensor("torch")
-        _image_ops._dropout_into(x, p, seed, subsequence, residual, self._result_t)
+        _image_ops._dropout_into(x, p, seed, subsequence, residual, self._result_t, _image_ops._gpu_index())
