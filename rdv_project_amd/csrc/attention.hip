@@ -84,7 +84,9 @@ Plan make_plan(const rdv_attention_desc& d, bool backward, int cu) {
     at += align256(p.bh * p.rows * 8);
     // a split is a whole number of the kernels' tiles (at most 64): dK and dV's rows end with a tile, not with a split
     p.dq = split_axis(p.bh * p.row_tiles, cu, d.keys, 64, 256);
-    p.dkv = split_axis(p.bh * p.key_tiles, 2 * int64_t(cu), p.rows, 64, 128);
+    // (fp32's products outweigh the partials: from 64 rows on.  4 x 1,000 x 333, 4 heads on 2 of 40: backward 75.7 us, from
+    // 128 rows on 82.8; fp16's do not: 4,096 x 77, 8 heads of 64: 32 and 27.5)
+    p.dkv = split_axis(p.bh * p.key_tiles, 2 * int64_t(cu), p.rows, 64, d.dtype == RDV_DTYPE_F32 ? 64 : 128);
     const int64_t a = p.dq.count > 1 ? align256(p.dq.count * p.bh * p.rows * p.pdim * 4) : 0;
     const int64_t b = p.dkv.count > 1 ? align256(p.dkv.count * p.bh * d.keys * p.pdim * 4) : 0;
     p.part = at;  // dQ's partials are summed before dK's and dV's are written
