@@ -257,13 +257,14 @@ __device__ __forceinline__ void load_affine(const NormArgs& a, const NormAt& p, 
   }
 }
 
-// act(scale x + offset) of a piece.
+// act(scale (x - mean) + b) of a piece.  (As one line in x it would be an operation less, but a group of nearly constant
+// values far from zero would become the rounding error of mean scale.)
 template <class T, int VE>
-__device__ __forceinline__ void normalise(const NormArgs& a, const Piece<T, VE>& x, const float (&scale)[VE],
-                                          const float (&offset)[VE], T* y) {
+__device__ __forceinline__ void normalise(const NormArgs& a, const Piece<T, VE>& x, const float (&mean)[VE],
+                                          const float (&scale)[VE], const float (&b)[VE], T* y) {
   float z[VE];
 #pragma unroll
-  for (int i = 0; i < VE; ++i) z[i] = fmaf(x[i], scale[i], offset[i]);
+  for (int i = 0; i < VE; ++i) z[i] = fmaf(x[i] - mean[i], scale[i], b[i]);
   if (a.act == RDV_ACT_SILU) {
 #pragma unroll
     for (int i = 0; i < VE; ++i) z[i] *= fast_sigmoid(z[i]);
@@ -274,43 +275,44 @@ __device__ __forceinline__ void normalise(const NormArgs& a, const Piece<T, VE>&
   store_piece<T, VE>(y, z);
 }
 
-// A thread's channels in the backward kernels, as lines in x so that an element costs one multiply-add each:
-// xhat = hat x + hat0, z = lin x + lin0.
+// A thread's channels in the backward kernels.  With t = x - mean an element costs one multiply-add for z = lin t + b, one
+// for the sum of dz t (rstd times which is B) and two for dx = lin dz + slope t + offset.
 template <int VE>
 struct BackLines {
-  float hat[VE], hat0[VE], lin[VE], lin0[VE];
+  float mean[VE], rstd[VE], lin[VE], b[VE];
 };
 template <int VE>
-__device__ __forceinline__ BackLines<VE> back_lines(const NormArgs& a, const NormAt& p, float (&w)[VE]) {
+__device__ __forceinline__ BackLines<VE> back_lines(const NormArgs& a, const NormAt& p) {
   BackLines<VE> k;
 #pragma unroll
   for (int i = 0; i < VE; ++i) {
     const int64_t g = p.image * a.groups + (p.on ? group_of(a, p.c0) + group_of(a, p.channel + i) : 0);
-    const float mean = a.stats[2 * g], rstd = a.stats[2 * g + 1];
-    w[i] = p.on && a.weight ? a.weight[p.c0 + p.channel + i] : 1.0f;
-    k.hat[i] = rstd;
-    k.hat0[i] = -mean * rstd;
-    k.lin[i] = rstd * w[i];
-    k.lin0[i] = fmaf(k.hat0[i], w[i], p.on && a.bias ? a.bias[p.c0 + p.channel + i] : 0.0f);
+    k.mean[i] = a.stats[2 * g];
+    k.rstd[i] = a.stats[2 * g + 1];
+    k.lin[i] = k.rstd[i] * (p.on && a.weight ? a.weight[p.c0 + p.channel + i] : 1.0f);
+    k.b[i] = p.on && a.bias ? a.bias[p.c0 + p.channel + i] : 0.0f;
   }
   return k;
 }
 
-// dz of a piece.
+// t and dz of a piece.
 template <class T, int VE>
 __device__ __forceinline__ void slopes(const NormArgs& a, const BackLines<VE>& k, const Piece<T, VE>& x,
-                                       const Piece<T, VE>& g, float (&dz)[VE]) {
+                                       const Piece<T, VE>& g, float (&t)[VE], float (&dz)[VE]) {
 #pragma unroll
-  for (int i = 0; i < VE; ++i) dz[i] = g[i];
+  for (int i = 0; i < VE; ++i) {
+    t[i] = x[i] - k.mean[i];
+    dz[i] = g[i];
+  }
   if (a.act == RDV_ACT_SILU) {  // s + z s (1 - s), s = 1 / (1 + e^-z)
 #pragma unroll
     for (int i = 0; i < VE; ++i) {
-      const float z = fmaf(x[i], k.lin[i], k.lin0[i]), s = fast_sigmoid(z);
+      const float z = fmaf(t[i], k.lin[i], k.b[i]), s = fast_sigmoid(z);
       dz[i] *= fmaf(z * s, 1.0f - s, s);
     }
   } else if (a.act == RDV_ACT_RELU) {
 #pragma unroll
-    for (int i = 0; i < VE; ++i) dz[i] = fmaf(x[i], k.lin[i], k.lin0[i]) > 0.0f ? dz[i] : 0.0f;
+    for (int i = 0; i < VE; ++i) dz[i] = fmaf(t[i], k.lin[i], k.b[i]) > 0.0f ? dz[i] : 0.0f;
   }
 }
 
@@ -364,12 +366,12 @@ __global__ __launch_bounds__(1024) void norm_whole_kernel(NormArgs a) {
   for (int i = 0; i < VE; ++i) {
     const int g = p.on ? group_of(a, p.channel + i) : 0;
     scale[i] = w[i] * rstd_g[g];
-    b[i] = fmaf(-mean_g[g], scale[i], b[i]);
+    mean[i] = mean_g[g];
   }
   T* const y = static_cast<T*>(a.y) + p.image * a.rows * a.channels + p.c0 + p.channel;
 #pragma unroll
   for (int k = 0; k < R; ++k)
-    if (k < n) normalise<T, VE>(a, v[k], scale, b, y + int64_t(p.tr + k * a.tr) * a.channels);
+    if (k < n) normalise<T, VE>(a, v[k], mean, scale, b, y + int64_t(p.tr + k * a.tr) * a.channels);
   if (a.stats) {
     float* const st = a.stats + 2 * (p.image * a.groups + p.c0 / a.width);
     for (int g = int(threadIdx.x); g < p.groups; g += int(blockDim.x)) {
@@ -400,16 +402,15 @@ __device__ __forceinline__ void join_sums(const NormArgs& a, const NormAt& p, fl
   }
 }
 
-// dx = lin dz + slope x + offset: the part of dx that is a line in x, -rstd (m1 + xhat m2).
+// dx = lin dz + slope t + offset: the part of dx that is a line in t, -rstd (m1 + rstd t m2).
 template <int VE>
 __device__ __forceinline__ void dx_lines(const NormArgs& a, const NormAt& p, const BackLines<VE>& k, const float* m1,
                                          const float* m2, float (&slope)[VE], float (&offset)[VE]) {
 #pragma unroll
   for (int i = 0; i < VE; ++i) {
     const int g = group_of(a, p.channel + i);
-    const float t = -k.hat[i] * m2[g];
-    slope[i] = t * k.hat[i];
-    offset[i] = fmaf(t, k.hat0[i], -k.hat[i] * m1[g]);
+    slope[i] = -k.rstd[i] * k.rstd[i] * m2[g];
+    offset[i] = -k.rstd[i] * m1[g];
   }
 }
 
@@ -432,18 +433,20 @@ __global__ __launch_bounds__(1024) void norm_whole_back_kernel(NormArgs a) {
       vg[k] = load_piece<T, VE>(g + r * a.g_row);
     }
   }
-  float w[VE], sa[VE] = {}, sb[VE] = {}, dz[VE];
-  const BackLines<VE> lines = back_lines<VE>(a, p, w);
+  float sa[VE] = {}, sb[VE] = {}, t[VE], dz[VE];
+  const BackLines<VE> lines = back_lines<VE>(a, p);
 #pragma unroll
   for (int k = 0; k < R; ++k)
     if (p.on && p.tr + k * a.tr < a.rows) {
-      slopes<T, VE>(a, lines, vx[k], vg[k], dz);
+      slopes<T, VE>(a, lines, vx[k], vg[k], t, dz);
 #pragma unroll
       for (int i = 0; i < VE; ++i) {
         sa[i] += dz[i];
-        sb[i] = fmaf(dz[i], fmaf(vx[k][i], lines.hat[i], lines.hat0[i]), sb[i]);
+        sb[i] = fmaf(dz[i], t[i], sb[i]);
       }
     }
+#pragma unroll
+  for (int i = 0; i < VE; ++i) sb[i] *= lines.rstd[i];
   join_sums<VE>(a, p, sa, sb, red, m1, m2, true);
   if (!p.on) return;
   dx_lines<VE>(a, p, lines, m1, m2, sb, sa);
@@ -452,9 +455,9 @@ __global__ __launch_bounds__(1024) void norm_whole_back_kernel(NormArgs a) {
   for (int k = 0; k < R; ++k) {
     const int r = p.tr + k * a.tr;
     if (r < a.rows) {
-      slopes<T, VE>(a, lines, vx[k], vg[k], dz);
+      slopes<T, VE>(a, lines, vx[k], vg[k], t, dz);
 #pragma unroll
-      for (int i = 0; i < VE; ++i) dz[i] = fmaf(dz[i], lines.lin[i], fmaf(vx[k][i], sb[i], sa[i]));
+      for (int i = 0; i < VE; ++i) dz[i] = fmaf(dz[i], lines.lin[i], fmaf(t[i], sb[i], sa[i]));
       store_piece<T, VE>(dx + int64_t(r) * a.channels, dz);
     }
   }
@@ -562,7 +565,7 @@ __global__ __launch_bounds__(kNormThreads) void norm_apply_kernel(NormArgs a) {
   float* const mean_g = norm_lds;
   float* const rstd_g = mean_g + a.slab / a.width;
   const T* const x = static_cast<const T*>(a.x) + p.image * a.x_image + p.c0 + p.channel;
-  float w[VE], b[VE], scale[VE];
+  float w[VE], b[VE], mean[VE], scale[VE];
   const int step = U * a.tr;
   int r = last_rows(ch, p, step);
   Piece<T, VE> v[U], next[U];
@@ -600,7 +603,7 @@ __global__ __launch_bounds__(kNormThreads) void norm_apply_kernel(NormArgs a) {
   for (int i = 0; i < VE; ++i) {
     const int g = group_of(a, p.channel + i);
     scale[i] = w[i] * rstd_g[g];
-    b[i] = fmaf(-mean_g[g], scale[i], b[i]);
+    mean[i] = mean_g[g];
   }
   T* const y = static_cast<T*>(a.y) + p.image * a.rows * a.channels + p.c0 + p.channel;
   for (; r >= ch.first; r -= step) {
@@ -608,7 +611,7 @@ __global__ __launch_bounds__(kNormThreads) void norm_apply_kernel(NormArgs a) {
 #pragma unroll
     for (int k = 0; k < U; ++k) {
       const int at = r + k * a.tr;
-      if (at < ch.end) normalise<T, VE>(a, v[k], scale, b, y + int64_t(at) * a.channels);
+      if (at < ch.end) normalise<T, VE>(a, v[k], mean, scale, b, y + int64_t(at) * a.channels);
       v[k] = next[k];
     }
   }
@@ -623,8 +626,8 @@ __global__ __launch_bounds__(kNormBackThreads) void norm_sums_kernel(NormArgs a)
   const NormAt p = norm_at<VE>(a, ch.image, ch.slab);
   const T* const x = static_cast<const T*>(a.x) + p.image * a.x_image + p.c0 + p.channel;
   const T* const g = static_cast<const T*>(a.grad) + p.image * a.g_image + p.c0 + p.channel;
-  float w[VE], sa[VE] = {}, sb[VE] = {}, dz[VE];
-  const BackLines<VE> lines = back_lines<VE>(a, p, w);
+  float sa[VE] = {}, sb[VE] = {}, t[VE], dz[VE];
+  const BackLines<VE> lines = back_lines<VE>(a, p);
   if (p.on) {
     const int step = U * a.tr;
     Piece<T, VE> vx[U], vg[U], nx[U], ng[U];
@@ -641,11 +644,11 @@ __global__ __launch_bounds__(kNormBackThreads) void norm_sums_kernel(NormArgs a)
 #pragma unroll
       for (int k = 0; k < U; ++k) {
         if (r + k * a.tr < ch.end) {
-          slopes<T, VE>(a, lines, vx[k], vg[k], dz);
+          slopes<T, VE>(a, lines, vx[k], vg[k], t, dz);
 #pragma unroll
           for (int i = 0; i < VE; ++i) {
             sa[i] += dz[i];
-            sb[i] = fmaf(dz[i], fmaf(vx[k][i], lines.hat[i], lines.hat0[i]), sb[i]);
+            sb[i] = fmaf(dz[i], t[i], sb[i]);
           }
         }
         vx[k] = nx[k];
@@ -653,6 +656,8 @@ __global__ __launch_bounds__(kNormBackThreads) void norm_sums_kernel(NormArgs a)
       }
     }
   }
+#pragma unroll
+  for (int i = 0; i < VE; ++i) sb[i] *= lines.rstd[i];
   float2* const part = a.parts + (p.image * a.chunks + ch.chunk) * a.channels + p.c0;
   for (int which = 0; which < 2; ++which) {
     sum_rows<VE>(a, p, which ? sb : sa, norm_lds);
@@ -713,8 +718,8 @@ __global__ __launch_bounds__(kNormBackThreads) void norm_dx_kernel(NormArgs a) {
   gather_sums<VE>(a, p, p.image * a.chunks, a.chunks, sa, sb);
   join_sums<VE>(a, p, sa, sb, red, m1, m2, false);
   if (!p.on) return;
-  float w[VE], dz[VE];
-  const BackLines<VE> lines = back_lines<VE>(a, p, w);
+  float t[VE], dz[VE];
+  const BackLines<VE> lines = back_lines<VE>(a, p);
   dx_lines<VE>(a, p, lines, m1, m2, sb, sa);
   for (; r >= ch.first; r -= step) {
     if (r - step >= ch.first) {
@@ -725,9 +730,9 @@ __global__ __launch_bounds__(kNormBackThreads) void norm_dx_kernel(NormArgs a) {
     for (int k = 0; k < U; ++k) {
       const int at = r + k * a.tr;
       if (at < ch.end) {
-        slopes<T, VE>(a, lines, vx[k], vg[k], dz);
+        slopes<T, VE>(a, lines, vx[k], vg[k], t, dz);
 #pragma unroll
-        for (int i = 0; i < VE; ++i) dz[i] = fmaf(dz[i], lines.lin[i], fmaf(vx[k][i], sb[i], sa[i]));
+        for (int i = 0; i < VE; ++i) dz[i] = fmaf(dz[i], lines.lin[i], fmaf(t[i], sb[i], sa[i]));
         store_piece<T, VE>(dx + int64_t(at) * a.channels, dz);
       }
       vx[k] = nx[k];

@@ -114,6 +114,20 @@ def test_constant_image_and_large_values():
     assert torch.equal(y.float(), torch.sign(big.float()))
 
 
+@pytest.mark.parametrize("rows", [100, 40000])
+def test_constant_groups_far_from_zero(rows):
+    """A constant group is its bias alone, whatever the constant: the mean of equal values is that value (to half a unit
+    in its last place, which 1 / sqrt(eps) = 316 turns into at most this)."""
+    value = torch.tensor([1000.1, -77.7, 0.3, 12345.678]).repeat_interleave(8)
+    x = value.expand(1, rows, 32).contiguous().cuda()
+    bias = torch.randn(32).cuda()
+    y, stats = rdv.group_norm(x, None, bias, 4, return_stats=True)
+    assert ((y - bias).abs() <= 317 * value.abs().cuda() * 2.0 ** -24).all()
+    dx, dw, db = rdv.group_norm_backward(torch.ones_like(x), x, None, bias, 4, stats)
+    assert torch.allclose(db, torch.full_like(db, rows))
+    assert (dw.abs() <= rows * 317 * value.abs().cuda() * 2.0 ** -24).all()
+
+
 def test_not_a_number_stays_in_its_group():
     x, grad, w, b = _inputs((2, 700, 32), "f32", 9)
     clean = rdv.group_norm(x, w, b, 4, activation="silu")
