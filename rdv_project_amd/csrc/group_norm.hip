@@ -341,7 +341,7 @@ __device__ __forceinline__ void slopes(const NormArgs& a, const BackLines<VE>& k
 // Two-launch kernels: rows that a thread loads at a time (the next ones' loads are in flight meanwhile), and threads of
 // a block.  One block per CU keeps 128 KiB of loads in flight on it, and few blocks leave few partial sums to join.  The
 // backward kernels hold two tensors' pieces and six constants per channel: at 1,024 threads they would spill.
-constexpr int kNormUnroll = 4, kNormThreads = 1024, kNormBackThreads = 512;
+constexpr int kNormUnroll = 4, kNormThreads = 1024, kNormBackThreads = 512, kNormBackUnroll = 2;
 
 // ------------------------------------------------------------------ one launch
 
@@ -642,9 +642,9 @@ __global__ __launch_bounds__(kNormThreads) void norm_apply_kernel(NormArgs a) {
 
 // First launch, backward: a chunk's A and B per channel.
 template <class T, int VE>
-__global__ __launch_bounds__(kNormBackThreads) void norm_sums_kernel(NormArgs a) {
+__global__ __launch_bounds__(kNormBackThreads, 4) void norm_sums_kernel(NormArgs a) {
   extern __shared__ float norm_lds[];
-  constexpr int U = kNormUnroll;
+  constexpr int U = kNormBackUnroll;
   const NormChunk ch = norm_chunk(a, int(blockIdx.x));
   const NormAt p = norm_at<VE>(a, ch.image, ch.slab);
   const T* const x = static_cast<const T*>(a.x) + p.image * a.x_image + p.c0 + p.channel;
@@ -708,9 +708,9 @@ __device__ __forceinline__ void gather_sums(const NormArgs& a, const NormAt& p, 
 // The last launch, backward.  Its first `slabs` blocks sum dweight and dbias over images and chunks; the others join
 // their image's chunks and write dx.
 template <class T, int VE>
-__global__ __launch_bounds__(kNormBackThreads) void norm_dx_kernel(NormArgs a) {
+__global__ __launch_bounds__(kNormBackThreads, 4) void norm_dx_kernel(NormArgs a) {
   extern __shared__ float norm_lds[];
-  constexpr int U = kNormUnroll;
+  constexpr int U = kNormBackUnroll;
   float* const red = norm_lds;
   float sa[VE], sb[VE];
   if (int(blockIdx.x) < a.slabs) {
@@ -962,8 +962,8 @@ NormPlan norm_plan(const rdv_group_norm_desc& d, bool backward, int cu, int alig
   p.kind = NormPlan::kChunked;
   set_slab(int64_t(256) * p.ve / unit * unit);
   set_threads(backward ? kNormBackThreads : kNormThreads);
-  const int64_t least = int64_t(p.tr) * kNormUnroll;  // rows that give every thread its first loads
-  int64_t chunks = std::max<int64_t>(1, int64_t(cu) / std::max<int64_t>(1, d.images * p.slabs));
+  const int64_t least = int64_t(p.tr) * (backward ? kNormBackUnroll : kNormUnroll);  // rows that give every thread its first loads
+  int64_t chunks = std::max<int64_t>(1, int64_t(backward ? 2 * cu : cu) / std::max<int64_t>(1, d.images * p.slabs));
   chunks = std::min(chunks, (d.rows + least - 1) / least);
   const int64_t rows = (d.rows + chunks - 1) / chunks;
   p.chunk_rows = int((rows + p.tr - 1) / p.tr * p.tr);
