@@ -69,8 +69,10 @@ Plan make_plan(const rdv_attention_desc& d, bool backward, int cu) {
   if (!backward) {
     // The states are split among blocks where the rows' blocks alone leave CUs idle, and each still has 256 states or
     // more: the partial results cost a write, a read and a launch.  4,096 rows x 8 heads (256 blocks) x 256 states of
-    // 64 dimensions in fp16 took 25 us in two splits.  Few rows stream the states: four blocks per CU.
-    p.forward = p.few ? split_axis(p.bh, 4 * int64_t(cu), d.keys, 128, 256)
+    // 64 dimensions in fp16 took 25 us in two splits.  Few rows stream the states: up to eight blocks per
+    // CU, of which two run, so that items of unequal lengths fill the chip to the end (8 tokens against 0 to 32,001 states,
+    // 4 heads of 128 in bf16: 82 us with four, 78.7 with eight, 81.5 with sixteen, whose join takes 8 us instead of 6.8).
+    p.forward = p.few ? split_axis(p.bh, 8 * int64_t(cu), d.keys, 128, 256)
                       : split_axis(p.bh * p.row_tiles, cu, d.keys, 64, 256);
     if (p.forward.count > 1) {
       const int64_t partial = p.forward.count * p.bh * p.rows;
