@@ -420,6 +420,18 @@ __device__ __forceinline__ void store_quad(T* row, int d, int odim, float x0, fl
 // maximum, 64 dimensions in fp16 over 1,024 states spent a third of their vector instructions on it.)
 constexpr float kSlack = 8.0f;
 
+// s c - ref.  In fp32 the product is rounded as the reference's was: the term at the reference is 1, and a row of one
+// state gives that state's v, bit for bit (16-bit results round a term that is off by 2^-22 away).
+template <class T>
+__device__ __forceinline__ float below(float s, float c, float ref) {
+  if constexpr (sizeof(T) == 4) {
+#pragma clang fp contract(off)
+    const float x = s * c;
+    return x - ref;
+  }
+  return fmaf(s, c, -ref);
+}
+
 template <int ND>
 struct Softmax {
   float top, total;
@@ -432,7 +444,7 @@ struct Softmax {
     for (int i = 0; i < ND; ++i) o[i] = f32x16{};
   }
   // takes N more result tiles of the column; on return they hold the terms exp2(s c - top)
-  template <int N>
+  template <class T, int N>
   __device__ __forceinline__ void take(f32x16 (&s)[N], float c) {
     float m = s[0][0];
 #pragma unroll
@@ -456,7 +468,7 @@ struct Softmax {
     for (int n = 0; n < N; ++n)
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        s[n][i] = __builtin_amdgcn_exp2f(fmaf(s[n][i], c, -ref));
+        s[n][i] = __builtin_amdgcn_exp2f(below<T>(s[n][i], c, ref));
         total += s[n][i];
       }
   }
@@ -625,7 +637,7 @@ __global__ __launch_bounds__(256, NC * sizeof(T) > 24 ? 1 : 2) void attn_tile_ke
 #pragma unroll
           for (int u = 0; u < SUB; ++u) mask_result(s[u], uint32_t(now >> (32 * u)), h, -INFINITY);
         }
-        sm.take(s, c);
+        sm.template take<T>(s, c);
         __builtin_amdgcn_s_setprio(1);
 #pragma unroll
         for (int u = 0; u < SUB; ++u)
@@ -718,7 +730,7 @@ __global__ __launch_bounds__(256, NC * sizeof(T) > 16 ? 1 : 2) void attn_few_ker
     byte = key_byte(a, p.item, first + 128, lane);
     if (!now) continue;
     if (now != ~uint32_t(0)) mask_result(s[0], now, h, -INFINITY);
-    sm.take(s, c);
+    sm.template take<T>(s, c);
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
@@ -825,13 +837,14 @@ __global__ __launch_bounds__(256, NC * sizeof(T) > 16 ? 1 : 2) void attn_dq_kern
   load_frags<T, NC>(static_cast<const T*>(a.q) + p.item * a.qs[0] + at.query * a.qs[1] + at.head * a.qs[2], a.dim, h, qf);
   load_frags<T, NC>(static_cast<const T*>(a.g) + p.item * a.gs[0] + at.query * a.gs[1] + at.head * a.gs[2], a.dim, h, gf);
   float lse = a.lse[int64_t(p.bh) * a.rows + rc], delta = 0.0f;
-  {
+  {  // the diagonal of O dO^T: dP's own sums, so that they cancel exactly where a row's result is one state's v
     typename Elem<T>::frag of[NC];
     load_frags<T, NC>(static_cast<const T*>(a.o) + p.item * a.os[0] + at.query * a.os[1] + at.head * a.os[2], a.dim, h, of);
+    f32x16 product{};
 #pragma unroll
-    for (int e = 0; e < NC; ++e)
+    for (int e = 0; e < NC; ++e) product = mma(of[e], gf[e], product);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) delta = fmaf(to_f32(T(gf[e][i])), to_f32(T(of[e][i])), delta);
+    for (int i = 0; i < 16; ++i) delta = n32 == 8 * (i >> 2) + 4 * h + (i & 3) ? product[i] : delta;
     delta = sum_halves(delta);
   }
   lse = lse == -INFINITY ? INFINITY : lse * kLog2e;  // a row without states: terms of 0
@@ -995,31 +1008,26 @@ __global__ __launch_bounds__(256, NC * sizeof(T) > 8 ? 1 : 2) void attn_dkv_kern
     for (int t = 0; t < steps; ++t) {
       if (t + 1 < steps) load(begin + (t + 1) * RT, (t + 1) & 1);
       if (active) {
-  #pragma unroll
+#pragma unroll
         for (int u = 0; u < SUB; ++u) {
           const uint8_t* const tq = tiles[t & 1][0] + 32 * u * G::kRow;
           const uint8_t* const tg = tiles[t & 1][1] + 32 * u * G::kRow;
-          f32x16 s{}, dp;  // dP's sums begin at -delta
-  #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const f32x4 w = *reinterpret_cast<const f32x4*>(&row_delta[t & 1][32 * u + 8 * j + 4 * h]);
-  #pragma unroll
-            for (int i = 0; i < 4; ++i) dp[4 * j + i] = w[i];
-          }
-            __builtin_amdgcn_s_setprio(1);
+          f32x16 s{}, dp{};
+          __builtin_amdgcn_s_setprio(1);
 #pragma unroll
           for (int e = 0; e < NC; ++e) {
             s = mma(row_frag<T, NC>(tq, n32, e, h), kf[e], s);
             dp = mma(row_frag<T, NC>(tg, n32, e, h), vf[e], dp);
           }
           __builtin_amdgcn_s_setprio(0);
-  #pragma unroll
+#pragma unroll
           for (int j = 0; j < 4; ++j) {
             const f32x4 l = *reinterpret_cast<const f32x4*>(&row_lse[t & 1][32 * u + 8 * j + 4 * h]);
-  #pragma unroll
+            const f32x4 w = *reinterpret_cast<const f32x4*>(&row_delta[t & 1][32 * u + 8 * j + 4 * h]);
+#pragma unroll
             for (int i = 0; i < 4; ++i) {
               s[4 * j + i] = __builtin_amdgcn_exp2f(fmaf(s[4 * j + i], c, l[i]));
-              dp[4 * j + i] *= s[4 * j + i];
+              dp[4 * j + i] = (dp[4 * j + i] + w[i]) * s[4 * j + i];  // delta is not where dP's sums begin: they would round otherwise
             }
           }
           if (shrink != 1.0f) dp *= shrink;

@@ -197,6 +197,33 @@ def test_bad_rows_stay_alone(dtype, value):
 
 
 @pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("lq,share", [(1, 1), (4, 2), (70, 2), (700, 1)])
+@pytest.mark.parametrize("lk", [1, 2, 100, 1000])
+@pytest.mark.parametrize("dim", [40, 64, 128])
+def test_one_state(dtype, lq, share, lk, dim):
+    """Where one state alone counts, the result is its v, whatever the score: v's gradient is the sum of the rows', q's
+    and k's are nothing at all."""
+    q, k, v, grad = _inputs(2, lq, lk, 2 * share, 2, dim, dtype, std=3.0)
+    for which in ("length", "mask"):
+        lengths = mask = None
+        at = 0
+        if which == "length":
+            lengths = torch.ones(2, dtype=torch.int32, device="cuda")
+        else:
+            at = lk - 1
+            mask = torch.zeros(2, lk, dtype=torch.bool, device="cuda")
+            mask[:, at] = True
+        args = dict(key_lengths=lengths, key_mask=mask)
+        out, lse = rdv.cross_attention(q, k, v, return_lse=True, **args)
+        assert torch.equal(out, v[:, at:at + 1].repeat_interleave(share, 2).expand_as(out)), which
+        dq, dk, dv = rdv.cross_attention_backward(grad, q, k, v, out, lse, **args)
+        assert not dq.any() and not dk.any(), which
+        only = torch.zeros_like(dv)
+        only[:, at] = dv[:, at]
+        assert torch.equal(only, dv), which
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
 @pytest.mark.parametrize("shape", [(1, 2048, 77, 2, 2, 64), (1, 300, 2500, 2, 1, 64), (2, 1000, 1030, 2, 1, 128),
                                    (1, 40, 9000, 1, 1, 32)])
 def test_longer(dtype, shape):
