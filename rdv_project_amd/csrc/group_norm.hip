@@ -8,14 +8,19 @@
 //
 // Geometry.  A block takes a slab of whole groups (channels) and a run of an image's rows.  Thread (tr, col) reads the
 // 16-byte (or narrower, by the alignment) piece `col` of the slab in rows tr, tr + TR, ...: its channels stay the same,
-// so per-channel constants and sums are registers, whatever the group width; sums join over tr in an LDS tree and
-// over a group's channels in 16 lanes.  Bound: HBM; each kernel reads what it needs once, in whole lines.
+// so per-channel constants and sums are registers, whatever the group width; sums join over tr by lane
+// moves and in LDS, over a group's channels in 16 or 64 lanes.  Bound: HBM; each kernel reads what it needs once, in whole lines.
 //   * An image's slab that fits the registers of a block is normalised by one launch that reads x once
 //     (norm_whole_kernel, norm_whole_back_kernel).
 //   * Larger images take two launches over the same grid: the first leaves each block's statistics, the second joins
 //     them (every block the same way, in one order) and reads its rows again, from the L2 that the first filled where
 //     the tensor fits.
 //   * A group wider than a slab can be takes one block per (image, group or channel) (norm_wide_*).
+// Measured, per launch.  8 x 256 x 256 x 64 in 16 groups, SiLU, fp16 (67 MB a tensor): 19 us for the statistics (3.5
+// TB/s), 25 for y (5.3), 32 for the gradients' sums (4.2; a sigmoid and its slope per element) and 36 for dx (5.6; a 2
+// GiB copy runs at 4.8): bound by HBM and by reading x and dy twice.  256 x 256 x 64, fp32: 5.9 and 8.3 us.  Images of
+// few rows are bound by latency: 16 x 16 x 128, fp32, in one launch 5.4 us, 3 x 77 x 53 x 48 in two launches 5.9 and 6.6
+// us, backward 6.6 and 5.2 us.
 // Variance.  Squares are taken of deviations from a mean of the thread's own values, and blocks' (mean, sum of squared
 // deviations) are joined with their means' distances: no difference of large sums.
 #include <algorithm>
@@ -35,6 +40,7 @@ struct NormArgs {
   void* y;               // or dx
   float* stats;          // [images, groups, 2]: mean, rstd (forward: may be NULL)
   float2* parts;         // forward: [images, groups, chunks] (mean, squared deviations); backward: [images, chunks, channels] (A, B)
+  float2* group_parts;   // backward, two launches: [images, groups, chunks] (sums of weight A, of weight B)
   float *dweight, *dbias;
   int64_t x_image, x_row, g_image, g_row;
   int images, rows, channels, groups, width, act;
@@ -114,32 +120,38 @@ __device__ __forceinline__ NormAt norm_at(const NormArgs& a, int image, int slab
   return p;
 }
 
-// Sums v over the block's tr, per channel of the slab; channel_sum() then gives a channel's sum.  Every thread takes
-// part, threads without a piece with zeros.  Rows side by side in a wave join by lane moves, waves (or rows, where a
-// row spans waves) through LDS.  red: blockDim.x * VE floats.
+// Sums va and vb over the block's tr, per channel of the slab; channel_sum() of red and of red + a.red then gives a
+// channel's.  Every thread takes part, threads without a piece with zeros.  Rows side by side in a wave join by lane
+// moves, waves (or rows, where a row spans waves) through LDS.  red: 2 a.red floats.
 template <int VE>
-__device__ __forceinline__ void sum_rows(const NormArgs& a, const NormAt& p, float (&v)[VE], float* red) {
+__device__ __forceinline__ void sum_rows(const NormArgs& a, const NormAt& p, float (&va)[VE], float (&vb)[VE], float* red) {
+  int row = p.tr, rows = a.tr;
   if (a.wave_rows) {
-    const int row = p.tr < a.tr ? p.tr - int(threadIdx.x >> 6) * a.wave_rows : 64;
+    const int r = p.tr < a.tr ? p.tr - int(threadIdx.x >> 6) * a.wave_rows : 64;
     for (int n = a.wave_rows; n > 1;) {
       const int half = (n + 1) >> 1;
+      const unsigned by = unsigned(half * a.pieces);
 #pragma unroll
       for (int i = 0; i < VE; ++i) {
-        const float t = __shfl_down(v[i], unsigned(half * a.pieces));
-        if (row < n - half) v[i] += t;
+        const float ta = __shfl_down(va[i], by), tb = __shfl_down(vb[i], by);
+        if (r < n - half) {
+          va[i] += ta;
+          vb[i] += tb;
+        }
       }
       n = half;
     }
-    __syncthreads();
-    if (row == 0) {
+    row = r == 0 ? int(threadIdx.x >> 6) : 64;
+    rows = int(blockDim.x >> 6);
+  }
+  __syncthreads();
+  if (row < rows) {
+    float* const mine = red + (row * a.pieces + p.col) * VE;
 #pragma unroll
-      for (int i = 0; i < VE; ++i) red[(int(threadIdx.x >> 6) * a.pieces + p.col) * VE + i] = v[i];
+    for (int i = 0; i < VE; ++i) {
+      mine[i] = va[i];
+      mine[a.red + i] = vb[i];
     }
-  } else {
-    float* const mine = red + threadIdx.x * VE;
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < VE; ++i) mine[i] = v[i];
   }
   __syncthreads();
 }
@@ -186,21 +198,23 @@ __device__ __forceinline__ void for_groups(const NormAt& p, F f) {
   }
 }
 
-// out[g] = f(sum of the LDS rows' per-channel sums, times weight(channel), over the channels of the slab's group g).
-template <int VE, class W, class F>
-__device__ __forceinline__ void sum_groups(const NormArgs& a, const NormAt& p, const float* red, float* out, W weight, F f) {
+// f(group, sums of the LDS rows' A and B times the channel's weight) for the slab's groups, by one lane each.
+template <int VE, class F>
+__device__ __forceinline__ void sum_groups(const NormArgs& a, const NormAt& p, const float* red, F f) {
   const int items = lds_rows<VE>(a) * a.width, step = a.pieces * VE;
   for_groups(p, [&](int g, int l, int lanes, auto join) {
-    float s = 0.0f;
+    float sa = 0.0f, sb = 0.0f;
 #pragma unroll 1
     for (int k = l; k < items; k += lanes) {
       const int row = group_of(a, k), c = g * a.width + k - row * a.width;
-      s = fmaf(red[row * step + c], weight(c), s);
+      const float w = a.weight ? a.weight[p.c0 + c] : 1.0f;
+      sa = fmaf(red[row * step + c], w, sa);
+      sb = fmaf(red[a.red + row * step + c], w, sb);
     }
-    s = join(s);
-    if (l == 0) out[g] = f(s);
+    sa = join(sa);
+    sb = join(sb);
+    if (l == 0) f(g, sa, sb);
   });
-  __syncthreads();
 }
 
 // Statistics of the slab's groups over the block from each thread's per-channel mean and squared deviations of n rows:
@@ -403,27 +417,6 @@ __global__ __launch_bounds__(1024) void norm_whole_kernel(NormArgs a) {
   }
 }
 
-// dx's two means per group, m1 and m2, from the threads' sums A and B; with `keep` the channels' sums are stored too.
-template <int VE>
-__device__ __forceinline__ void join_sums(const NormArgs& a, const NormAt& p, float (&sa)[VE], float (&sb)[VE],
-                                          float* red, float* m1, float* m2, bool keep) {
-  const float inv = 1.0f / (float(a.rows) * float(a.width));
-  for (int which = 0; which < 2; ++which) {
-    sum_rows<VE>(a, p, which ? sb : sa, red);
-    if (keep) {  // an only image's sums are the parameters' gradients
-      float* const param = which ? a.dweight : a.dbias;
-      float2* const part = a.parts + p.image * a.channels + p.c0;
-      for (int c = int(threadIdx.x); c < p.channels; c += int(blockDim.x)) {
-        const float s = channel_sum<VE>(a, red, c);
-        if (a.images > 1) (which ? part[c].y : part[c].x) = s;
-        else if (param) param[p.c0 + c] = s;
-      }
-    }
-    sum_groups<VE>(a, p, red, which ? m2 : m1, [&](int c) { return a.weight ? a.weight[p.c0 + c] : 1.0f; },
-                   [&](float t) { return t * inv; });
-  }
-}
-
 // dx = lin dz + slope t + offset: the part of dx that is a line in t, -rstd (m1 + rstd t m2).
 template <int VE>
 __device__ __forceinline__ void dx_lines(const NormArgs& a, const NormAt& p, const BackLines<VE>& k, const float* m1,
@@ -442,7 +435,7 @@ __global__ __launch_bounds__(1024) void norm_whole_back_kernel(NormArgs a) {
   extern __shared__ float norm_lds[];
   const NormAt p = norm_at<VE>(a, int(blockIdx.x) / a.slabs, int(blockIdx.x) % a.slabs);
   float* const red = norm_lds;
-  float* const m1 = red + blockDim.x * VE;
+  float* const m1 = red + 2 * a.red;
   float* const m2 = m1 + a.slab_groups;
   const T* const x = static_cast<const T*>(a.x) + p.image * a.x_image + p.c0 + p.channel;
   const T* const g = static_cast<const T*>(a.grad) + p.image * a.g_image + p.c0 + p.channel;
@@ -469,7 +462,23 @@ __global__ __launch_bounds__(1024) void norm_whole_back_kernel(NormArgs a) {
     }
 #pragma unroll
   for (int i = 0; i < VE; ++i) sb[i] *= lines.rstd[i];
-  join_sums<VE>(a, p, sa, sb, red, m1, m2, true);
+  sum_rows<VE>(a, p, sa, sb, red);
+  float2* const part = a.parts + p.image * a.channels + p.c0;
+  for (int c = int(threadIdx.x); c < p.channels; c += int(blockDim.x)) {
+    const float2 sum{channel_sum<VE>(a, red, c), channel_sum<VE>(a, red + a.red, c)};
+    if (a.images > 1) {
+      part[c] = sum;
+    } else {  // an only image's sums are the parameters' gradients
+      if (a.dbias) a.dbias[p.c0 + c] = sum.x;
+      if (a.dweight) a.dweight[p.c0 + c] = sum.y;
+    }
+  }
+  const float inv = 1.0f / (float(a.rows) * float(a.width));
+  sum_groups<VE>(a, p, red, [&](int g, float wa, float wb) {
+    m1[g] = wa * inv;
+    m2[g] = wb * inv;
+  });
+  __syncthreads();
   if (!p.on) return;
   dx_lines<VE>(a, p, lines, m1, m2, sb, sa);
   T* const dx = static_cast<T*>(a.y) + p.image * a.rows * a.channels + p.c0 + p.channel;
@@ -640,7 +649,7 @@ __global__ __launch_bounds__(kNormThreads) void norm_apply_kernel(NormArgs a) {
   }
 }
 
-// First launch, backward: a chunk's A and B per channel.
+// First launch, backward: a chunk's A and B per channel, and their weighted sums per group.
 template <class T, int VE>
 __global__ __launch_bounds__(kNormBackThreads, 4) void norm_sums_kernel(NormArgs a) {
   extern __shared__ float norm_lds[];
@@ -682,10 +691,11 @@ __global__ __launch_bounds__(kNormBackThreads, 4) void norm_sums_kernel(NormArgs
 #pragma unroll
   for (int i = 0; i < VE; ++i) sb[i] *= lines.rstd[i];
   float2* const part = a.parts + (p.image * a.chunks + ch.chunk) * a.channels + p.c0;
-  for (int which = 0; which < 2; ++which) {
-    sum_rows<VE>(a, p, which ? sb : sa, norm_lds);
-    for (int c = int(threadIdx.x); c < p.channels; c += int(blockDim.x)) (which ? part[c].y : part[c].x) = channel_sum<VE>(a, norm_lds, c);
-  }
+  sum_rows<VE>(a, p, sa, sb, norm_lds);
+  for (int c = int(threadIdx.x); c < p.channels; c += int(blockDim.x))
+    part[c] = float2{channel_sum<VE>(a, norm_lds, c), channel_sum<VE>(a, norm_lds + a.red, c)};
+  float2* const group_part = a.group_parts + (p.image * a.groups + p.g0) * a.chunks + ch.chunk;
+  sum_groups<VE>(a, p, norm_lds, [&](int g, float wa, float wb) { group_part[int64_t(g) * a.chunks] = float2{wa, wb}; });
 }
 
 // Sums `count` rows of per-channel (A, B) of `parts` from row `first` on over the block.
@@ -706,7 +716,8 @@ __device__ __forceinline__ void gather_sums(const NormArgs& a, const NormAt& p, 
 }
 
 // The last launch, backward.  Its first `slabs` blocks sum dweight and dbias over images and chunks; the others join
-// their image's chunks and write dx.
+// their image's chunks' sums per group and write dx.  (With every block joining the sums per channel, eight times the
+// bytes of groups of eight, 3 x 77 x 53 x 48 in fp32 took 7.7 us instead of 5.2.)
 template <class T, int VE>
 __global__ __launch_bounds__(kNormBackThreads, 4) void norm_dx_kernel(NormArgs a) {
   extern __shared__ float norm_lds[];
@@ -716,17 +727,16 @@ __global__ __launch_bounds__(kNormBackThreads, 4) void norm_dx_kernel(NormArgs a
   if (int(blockIdx.x) < a.slabs) {
     const NormAt p = norm_at<VE>(a, 0, int(blockIdx.x));
     gather_sums<VE>(a, p, 0, int64_t(a.images) * a.chunks, sa, sb);
-    for (int which = 0; which < 2; ++which) {
-      sum_rows<VE>(a, p, which ? sb : sa, red);
-      float* const out = which ? a.dweight : a.dbias;
-      if (out)
-        for (int c = int(threadIdx.x); c < p.channels; c += int(blockDim.x)) out[p.c0 + c] = channel_sum<VE>(a, red, c);
+    sum_rows<VE>(a, p, sa, sb, red);
+    for (int c = int(threadIdx.x); c < p.channels; c += int(blockDim.x)) {
+      if (a.dbias) a.dbias[p.c0 + c] = channel_sum<VE>(a, red, c);
+      if (a.dweight) a.dweight[p.c0 + c] = channel_sum<VE>(a, red + a.red, c);
     }
     return;
   }
   const NormChunk ch = norm_chunk(a, int(blockIdx.x) - a.slabs);
   const NormAt p = norm_at<VE>(a, ch.image, ch.slab);
-  float* const m1 = red + blockDim.x * VE;
+  float* const m1 = red + 2 * a.red;
   float* const m2 = m1 + a.slab_groups;
   const T* const x = static_cast<const T*>(a.x) + p.image * a.x_image + p.c0 + p.channel;
   const T* const g = static_cast<const T*>(a.grad) + p.image * a.g_image + p.c0 + p.channel;
@@ -738,8 +748,24 @@ __global__ __launch_bounds__(kNormBackThreads, 4) void norm_dx_kernel(NormArgs a
     load_rows<T, VE, U>(a, x, a.x_row, r, vx);
     load_rows<T, VE, U>(a, g, a.g_row, r, vg);
   }
-  gather_sums<VE>(a, p, p.image * a.chunks, a.chunks, sa, sb);
-  join_sums<VE>(a, p, sa, sb, red, m1, m2, false);
+  const float inv = 1.0f / (float(a.rows) * float(a.width));
+  for_groups(p, [&](int g, int l, int lanes, auto join) {
+    const float2* const part = a.group_parts + (p.image * a.groups + p.g0 + g) * a.chunks;
+    float wa = 0.0f, wb = 0.0f;
+#pragma unroll 4
+    for (int i = l; i < a.chunks; i += lanes) {
+      const float2 t = part[i];
+      wa += t.x;
+      wb += t.y;
+    }
+    wa = join(wa);
+    wb = join(wb);
+    if (l == 0) {
+      m1[g] = wa * inv;
+      m2[g] = wb * inv;
+    }
+  });
+  __syncthreads();
   if (!p.on) return;
   float t[VE], dz[VE];
   const BackLines<VE> lines = back_lines<VE>(a, p);
@@ -968,7 +994,7 @@ NormPlan norm_plan(const rdv_group_norm_desc& d, bool backward, int cu, int alig
   const int64_t rows = (d.rows + chunks - 1) / chunks;
   p.chunk_rows = int((rows + p.tr - 1) / p.tr * p.tr);
   p.chunks = int((d.rows + p.chunk_rows - 1) / p.chunk_rows);
-  p.bytes = d.images * p.chunks * 8 * (backward ? d.channels : d.groups);
+  p.bytes = d.images * p.chunks * 8 * (d.groups + (backward ? d.channels : 0));
   return p;
 }
 
@@ -1002,6 +1028,7 @@ NormArgs norm_args(const rdv_group_norm_desc& d, const NormPlan& p, const void* 
   a.red = (p.wave_rows ? p.threads / 64 : p.tr) * p.slab;
   a.chunks = p.chunks;
   a.chunk_rows = p.chunk_rows;
+  a.group_parts = a.parts ? a.parts + d.images * p.chunks * d.channels : nullptr;
   return a;
 }
 
@@ -1102,7 +1129,7 @@ int launch_group_norm_backward(const rdv_group_norm_desc& d, const void* grad, c
   }
   const int64_t blocks = d.images * p.slabs * p.chunks + (p.kind == NormPlan::kChunked ? p.slabs : 0);
   if (int rc = check_blocks(blocks)) return rc;
-  const unsigned lds = unsigned(p.threads * p.ve + 2 * (p.slab / a.width)) * 4;
+  const unsigned lds = unsigned(2 * a.red + 2 * a.slab_groups) * 4;
   return with_piece(d.dtype, p.ve, [&](auto t, auto ve) {
     using T = decltype(t);
     constexpr int VE = decltype(ve)::value;
