@@ -512,6 +512,11 @@ __device__ __forceinline__ void finish_row(const AttnArgs& a, const BlockAt& p, 
 //
 // Many rows: a block of 4 waves, 32 rows each (or 64 rows shared by pairs of waves), walks its share of the states in
 // tiles of KT in LDS (two buffers, one barrier per tile: the next tile's loads are in flight under this tile's products).
+// Bound: a SIMD's vector instructions (the softmax: an fma, an exp2, an addition, half a conversion per score) and matrix
+// instructions add up.  128 dimensions have twice the products of 64 per score:
+//   2 x 16,384 x 4,096, 8 heads of 128, bf16:              530 us, 1.03 PFLOP/s (an 8,192^3 product: 1.18)
+//   4 x 4,096 x 1,024, 8 heads on 4 of 64, fp16:            52 us, 0.66 PFLOP/s
+//   1 x 4,096 x 256, 4 heads of 64, fp32 (a wave per SIMD): 20 us, 54 TFLOP/s (an 8,192^3 product: 153)
 template <class T, int NC>
 constexpr int attn_tile_keys() { return sizeof(T) == 4 && NC > 4 ? 32 : 64; }
 
@@ -675,6 +680,7 @@ __global__ __launch_bounds__(256, NC * sizeof(T) > 24 ? 1 : 2) void attn_tile_ke
 // At most 32 rows per (item, state head): a single token's heads, or few.  The states are what is read, so the waves
 // split them: each of 4 walks its own tiles of 32, K's fragments straight from global memory (a lane holds a state)
 // and V through LDS of its own for the transposing reads, without barriers; at the end the waves' columns are joined.
+// Bound: HBM.  8 tokens against 0 to 32,001 states, 16 heads on 4 of 128, bf16: 65 us for 287 MB, 4.4 TB/s (a copy: 4.8).
 template <class T, int NC>
 struct AttnFew {
   using G = AttnTile<T, NC>;
@@ -817,6 +823,9 @@ __device__ __forceinline__ float fit_terms(const f32x16& ds, bool counts) {
 
 // dQ: blocks and waves as attn_tile_kernel's, Q and dO fragments in registers: S^T = K Q^T and dP^T = V dO^T from K's and
 // V's rows, dQ^T += K^T dS^T from K's columns.  A row's delta is summed here and kept, with its lse, for attn_dkv_kernel.
+// (S and dP are computed in both backward kernels, 7 products for the 5 of the formula: one kernel for all three results
+// would add dQ's or dK's tiles of other blocks' rows through memory, in an order of its own each time.)
+// 4 x 4,096 x 1,024, 8 heads on 4 of 64, fp16: 74 us, 0.70 PFLOP/s of its three products; bound as the forward kernel.
 template <class T, int NC, int WK>
 __global__ __launch_bounds__(256, NC * sizeof(T) > 16 ? 1 : 2) void attn_dq_kernel(AttnArgs a) {
   using G = AttnTile<T, NC>;
@@ -925,10 +934,14 @@ __global__ __launch_bounds__(256, NC * sizeof(T) > 16 ? 1 : 2) void attn_dq_kern
 }
 
 // dK and dV: a block of 4 waves, 32 states each (K and V fragments in registers), walks its share of the rows in tiles
-// of 32: S = Q K^T and dP = dO V^T from Q's and dO's rows, dV^T += dO^T P and dK^T += Q^T dS from their columns.  A
+// of RT: S = Q K^T and dP = dO V^T from Q's and dO's rows, dV^T += dO^T P and dK^T += Q^T dS from their columns.  A
 // state that does not count is a column of its own, and is written as 0; a row that does not has P = 0.
+// 4 x 4,096 x 1,024, 8 heads on 4 of 64, fp16: 88 us, 0.78 PFLOP/s of its four products, and 7.5 us for the sums of its
+// splits; bound as the forward kernel.  Two waves per SIMD up to 96 dimensions in 16 bits and 32 in fp32: with one, whose
+// registers hold more reads ahead, both backward kernels took 278 us instead of 222 at 96 dimensions; at 128, two spill
+// (362 us against 334), as in fp32 from 48 on (4 x 1,000 x 333, 4 heads on 2 of 40, both directions: 92 us against 78).
 template <class T, int NC>
-__global__ __launch_bounds__(256, NC * sizeof(T) > 8 ? 1 : 2) void attn_dkv_kernel(AttnArgs a) {
+__global__ __launch_bounds__(256, NC > (sizeof(T) == 4 ? 2 : 6) ? 1 : 2) void attn_dkv_kernel(AttnArgs a) {
   using G = AttnTile<T, NC>;
   constexpr int RT = attn_tile_keys<T, NC>(), SUB = RT / 32, ND = G::ND;
   // one variable: the tiles come first, within the 64 KiB that the direct loads reach
@@ -1027,7 +1040,8 @@ __global__ __launch_bounds__(256, NC * sizeof(T) > 8 ? 1 : 2) void attn_dkv_kern
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               s[4 * j + i] = __builtin_amdgcn_exp2f(fmaf(s[4 * j + i], c, l[i]));
-              dp[4 * j + i] = (dp[4 * j + i] + w[i]) * s[4 * j + i];  // delta is not where dP's sums begin: they would round otherwise
+              // delta is not where dP's sums begin: they would round otherwise
+              dp[4 * j + i] = (dp[4 * j + i] + w[i]) * s[4 * j + i];
             }
           }
           if (shrink != 1.0f) dp *= shrink;

@@ -33,6 +33,8 @@ __device__ __forceinline__ void philox4x32(uint64_t block, uint64_t subsequence,
 
 // y[i] for i < n, one word each.  VEC: 16-byte pieces of aligned tensors, kPieces per thread, a block apart so that a
 // wave's loads are whole lines; the last, partial piece and unaligned tensors go element by element.
+// Bound: HBM; the generator's 20 wide products per four elements hide under the loads.  2^20 x 64 in bf16: 70 us with a
+// residual (403 MB, 5.8 TB/s), 47 us without (268 MB, 5.7 TB/s; a 2 GiB copy runs at 4.8).
 constexpr int kPieces = 2;
 
 template <class T, bool VEC>
