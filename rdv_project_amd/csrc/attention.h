@@ -38,6 +38,9 @@ struct AttnArgs {
   float scale;
 };
 
+// Rows further apart than this are packed before: a tile's 64 rows lie within 2^31 bytes.
+constexpr int64_t kAttnFarStride = int64_t(1) << 25;
+
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 typedef bf16_t bf16x8 __attribute__((ext_vector_type(8)));
@@ -252,8 +255,7 @@ struct Dma {
   using G = AttnTile<T, NC>;
   static constexpr int kBytes = R * G::kRow, kTotal = kBytes / 1024, N = (kTotal + 3) / 4;
   static_assert(4 * kBytes <= 64 * 1024, "M0 holds 16 bits of an LDS address");
-  uint32_t off[N];  // of the lane's piece from the tile's first row, in bytes
-  bool near;        // offsets fit 32 bits
+  uint32_t off[N];  // of the lane's piece from the tile's first row, in bytes (see kAttnFarStride)
   int wave, lane, dim;
   int64_t stride;   // bytes
 
@@ -268,7 +270,6 @@ struct Dma {
     lane = l;
     dim = dimensions;
     stride = row_stride * int(sizeof(T));
-    near = stride * R < (int64_t(1) << 31);
 #pragma unroll
     for (int i = 0; i < N; ++i) off[i] = uint32_t(row(i)) * uint32_t(stride) + piece(i) * 16;
   }
@@ -293,6 +294,19 @@ struct Dma {
             : "memory");
       }
   }
+  // 16 bytes per lane from src to consecutive places at `lds`
+  __device__ __forceinline__ static void load_piece(const uint8_t* src, uint32_t lds) {
+    uint32_t saved;
+    asm volatile(
+        "s_mov_b32 %0, m0\n\t"
+        "s_mov_b32 m0, %2\n\t"
+        "s_nop 0\n\t"
+        "global_load_lds_dwordx4 %1, off\n\t"
+        "s_mov_b32 m0, %0"
+        : "=&s"(saved)
+        : "v"(src), "s"(__builtin_amdgcn_readfirstlane(lds))
+        : "memory");
+  }
   // row r of the tile from row_of(r), zeros where that is NULL
   template <class F>
   __device__ __forceinline__ void load_each(F row_of, const uint8_t* tile) const {
@@ -303,26 +317,30 @@ struct Dma {
         const T* const p = row_of(row(i));
         const uint8_t* const src = p ? reinterpret_cast<const uint8_t*>(p) + piece(i) * 16
                                      : reinterpret_cast<const uint8_t*>(g_attn_zero);
-        uint32_t saved;
-        asm volatile(
-            "s_mov_b32 %0, m0\n\t"
-            "s_mov_b32 m0, %2\n\t"
-            "s_nop 0\n\t"
-            "global_load_lds_dwordx4 %1, off\n\t"
-            "s_mov_b32 m0, %0"
-            : "=&s"(saved)
-            : "v"(src), "s"(__builtin_amdgcn_readfirstlane(lds + (i * 4 + wave) * 1024))
-            : "memory");
+        load_piece(src, lds + (i * 4 + wave) * 1024);
       }
   }
-  // rows first .. first + R - 1 of a tensor at base, those whose bit in `valid` is set
-  __device__ __forceinline__ void load_keys(const T* base, int64_t row_stride, int first, uint64_t valid,
+  // R rows from `first` on, evenly spaced, zeros where their bit in `valid` is not set (no address is formed from those)
+  __device__ __forceinline__ void load_some(const T* first, uint64_t valid, const uint8_t* tile) const {
+    constexpr int kRows = 1024 / G::kRow;  // of an instruction
+    const uint32_t lds = lds_address(tile);
+    const int r = lane * 16 / G::kRow;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (on(i)) {
+        const uint32_t part = uint32_t(valid >> ((i * 4 + wave) * kRows & 63));
+        const uint8_t* const src = (part >> r) & 1 ? reinterpret_cast<const uint8_t*>(first) + off[i]
+                                                   : reinterpret_cast<const uint8_t*>(g_attn_zero);
+        load_piece(src, lds + (i * 4 + wave) * 1024);
+      }
+  }
+  // Rows first .. first + R - 1 of a tensor [keys] at base, those whose bit in `valid` is set.  LOOSE: the others may be
+  // anything, so where the tensor has all of them they are read like these.
+  template <bool LOOSE>
+  __device__ __forceinline__ void load_keys(const T* base, int64_t row_stride, int first, int keys, uint64_t valid,
                                             const uint8_t* tile) const {
-    if (near && valid == all_rows()) {
-      load(base + first * row_stride, tile);
-    } else {
-      load_each([&](int r) { return (valid >> r) & 1 ? base + int64_t(first + r) * row_stride : nullptr; }, tile);
-    }
+    if (valid == all_rows() || (LOOSE && first + R <= keys)) load(base + first * row_stride, tile);
+    else load_some(base + first * row_stride, valid, tile);
   }
   __device__ __forceinline__ static uint64_t all_rows() { return R == 64 ? ~uint64_t(0) : (uint64_t(1) << (R & 63)) - 1; }
 };
@@ -381,9 +399,14 @@ __device__ __forceinline__ uint64_t key_bits(int byte, int first, int end, int l
 // Results that do not count become -inf: register 4 j + r of half h is the state at bit 8 j + 4 h + r.
 __device__ __forceinline__ void mask_result(f32x16& s, uint32_t bits, int h, float fill) {
   asm volatile("" ::: "memory");  // or the tests below are hoisted out of the callers' rare branch: 100 instructions
-  const uint32_t mine = bits >> (4 * h);
+  const uint32_t mine = bits >> (4 * h), other = __builtin_bit_cast(uint32_t, fill);
 #pragma unroll
-  for (int i = 0; i < 16; ++i) s[i] = (mine >> (8 * (i >> 2) + (i & 3))) & 1 ? s[i] : fill;
+  for (int i = 0; i < 16; ++i) {  // by the bit's mask: two instructions, a comparison and a choice are three and a wait
+    const float x = s[i];
+    int keep = __builtin_amdgcn_sbfe(int(mine), 8 * (i >> 2) + (i & 3), 1);
+    asm("" : "+v"(keep));  // or they become the three
+    s[i] = __builtin_bit_cast(float, (__builtin_bit_cast(uint32_t, x) & uint32_t(keep)) | (other & ~uint32_t(keep)));
+  }
 }
 
 // The value of lane l + 32 (mod 64).  v_permlane32_swap exchanges its second operand's first half with its first one's
@@ -516,12 +539,14 @@ __device__ __forceinline__ void finish_row(const AttnArgs& a, const BlockAt& p, 
 // instructions add up.  128 dimensions have twice the products of 64 per score:
 //   2 x 16,384 x 4,096, 8 heads of 128, bf16:              530 us, 1.03 PFLOP/s (an 8,192^3 product: 1.18)
 //   4 x 4,096 x 1,024, 8 heads on 4 of 64, fp16:            52 us, 0.66 PFLOP/s
-//   1 x 4,096 x 256, 4 heads of 64, fp32 (a wave per SIMD): 20 us, 54 TFLOP/s (an 8,192^3 product: 153)
+//   1 x 4,096 x 256, 4 heads of 64, fp32 (a wave per SIMD): 17 us, 63 TFLOP/s (an 8,192^3 product: 153)
+// 16-bit heads of up to 64 dimensions fit 128 registers, four blocks per CU (132: 57 us instead of 52 in the second line).
 template <class T, int NC>
 constexpr int attn_tile_keys() { return sizeof(T) == 4 && NC > 4 ? 32 : 64; }
 
 // The pipeline of the kernels that walk states: body(tile of K, tile of V, bits) per tile, in order.
-template <class T, int NC, int KT, class F>
+// Of a state that does not count K's row (LOOSE_K) or V's may be anything: its scores are replaced.
+template <class T, int NC, int KT, bool LOOSE_K, class F>
 __device__ __forceinline__ void walk_keys(const AttnArgs& a, const BlockAt& p, const T* k, const T* v, int begin, int end,
                                           uint8_t (*tiles)[2][KT * AttnTile<T, NC>::kRow], int wave, int lane, F body) {
   const int steps = end > begin ? (end - begin + KT - 1) / KT : 0;
@@ -533,16 +558,16 @@ __device__ __forceinline__ void walk_keys(const AttnArgs& a, const BlockAt& p, c
   int byte = key_byte(a, p.item, begin, lane);
   uint64_t now = key_bits<KT>(byte, begin, end, lane);
   byte = key_byte(a, p.item, begin + KT, lane);
-  dk.load_keys(k, a.ks[1], begin, now, tiles[0][0]);
-  dv.load_keys(v, a.vs[1], begin, now, tiles[0][1]);
+  dk.template load_keys<LOOSE_K>(k, a.ks[1], begin, a.keys, now, tiles[0][0]);
+  dv.template load_keys<!LOOSE_K>(v, a.vs[1], begin, a.keys, now, tiles[0][1]);
   dma_wait();
   __syncthreads();
   for (int t = 0; t < steps; ++t) {
     const int next = begin + (t + 1) * KT;
     const uint64_t then = key_bits<KT>(byte, next, end, lane);
     if (t + 1 < steps) {
-      dk.load_keys(k, a.ks[1], next, then, tiles[(t + 1) & 1][0]);
-      dv.load_keys(v, a.vs[1], next, then, tiles[(t + 1) & 1][1]);
+      dk.template load_keys<LOOSE_K>(k, a.ks[1], next, a.keys, then, tiles[(t + 1) & 1][0]);
+      dv.template load_keys<!LOOSE_K>(v, a.vs[1], next, a.keys, then, tiles[(t + 1) & 1][1]);
       byte = key_byte(a, p.item, next + KT, lane);
     }
     if (now) body(tiles[t & 1][0], tiles[t & 1][1], now);
@@ -593,7 +618,7 @@ struct JoinTile {
 };
 
 template <class T, int NC, int WK>
-__global__ __launch_bounds__(256, NC * sizeof(T) > 24 ? 1 : 2) void attn_tile_kernel(AttnArgs a) {
+__global__ __launch_bounds__(256, NC * sizeof(T) > 24 ? 1 : NC * sizeof(T) > 8 ? 2 : 4) void attn_tile_kernel(AttnArgs a) {
   using G = AttnTile<T, NC>;
   constexpr int KT = attn_tile_keys<T, NC>(), SUB = KT / 32 / WK, ND = G::ND;
   static_assert(SUB >= 1, "a tile has 32 states for every wave of a row group");
@@ -618,7 +643,7 @@ __global__ __launch_bounds__(256, NC * sizeof(T) > 24 ? 1 : 2) void attn_tile_ke
   Softmax<ND> sm;
   sm.clear();
   const int begin = p.split * a.chunk, end = min(begin + a.chunk, key_limit(a, p.item));
-  walk_keys<T, NC, KT>(
+  walk_keys<T, NC, KT, true>(
       a, p, static_cast<const T*>(a.k) + p.item * a.ks[0] + p.hk * a.ks[2],
       static_cast<const T*>(a.v) + p.item * a.vs[0] + p.hk * a.vs[2], begin, end, tiles, w.wave, lane,
       [&](const uint8_t* tk, const uint8_t* tv, uint64_t now) {
@@ -827,7 +852,7 @@ __device__ __forceinline__ float fit_terms(const f32x16& ds, bool counts) {
 // would add dQ's or dK's tiles of other blocks' rows through memory, in an order of its own each time.)
 // 4 x 4,096 x 1,024, 8 heads on 4 of 64, fp16: 74 us, 0.70 PFLOP/s of its three products; bound as the forward kernel.
 template <class T, int NC, int WK>
-__global__ __launch_bounds__(256, NC * sizeof(T) > 16 ? 1 : 2) void attn_dq_kernel(AttnArgs a) {
+__global__ __launch_bounds__(256, NC * sizeof(T) > 16 ? 1 : NC * sizeof(T) > 8 ? 2 : 3) void attn_dq_kernel(AttnArgs a) {
   using G = AttnTile<T, NC>;
   constexpr int KT = attn_tile_keys<T, NC>(), SUB = KT / 32 / WK, ND = G::ND;
   static_assert(SUB >= 1, "a tile has 32 states for every wave of a row group");
@@ -864,7 +889,7 @@ __global__ __launch_bounds__(256, NC * sizeof(T) > 16 ? 1 : 2) void attn_dq_kern
 #pragma unroll
   for (int d = 0; d < ND; ++d) acc[d] = f32x16{};
   const int begin = p.split * a.chunk, end = min(begin + a.chunk, key_limit(a, p.item));
-  walk_keys<T, NC, KT>(
+  walk_keys<T, NC, KT, false>(
       a, p, static_cast<const T*>(a.k) + p.item * a.ks[0] + p.hk * a.ks[2],
       static_cast<const T*>(a.v) + p.item * a.vs[0] + p.hk * a.vs[2], begin, end, tiles, w.wave, lane,
       [&](const uint8_t* tk, const uint8_t* tv, uint64_t bits) {
@@ -985,7 +1010,7 @@ __global__ __launch_bounds__(256, NC > (sizeof(T) == 4 ? 2 : 6) ? 1 : 2) void at
   float2 st{INFINITY, 0.0f};
   auto load = [&](int first, int buf) {
     const int x = first / a.queries, query = first - x * a.queries, head = p.hk * a.share + x;
-    if (dq.near && dg.near && query + RT <= a.queries) {  // rows of one head
+    if (query + RT <= a.queries) {  // rows of one head
       dq.load(q + query * a.qs[1] + head * a.qs[2], tiles[buf][0]);
       dg.load(g + query * a.gs[1] + head * a.gs[2], tiles[buf][1]);
     } else {

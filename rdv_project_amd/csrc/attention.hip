@@ -14,7 +14,8 @@ int element_bytes(int dtype) { return dtype == RDV_DTYPE_F32 ? 4 : 2; }
 // Whether the kernels can read a tensor in place: rows are whole 16-byte pieces.
 bool in_place(const rdv_attention_desc& d, const int64_t (&s)[3], int length, int heads) {
   const int e = 16 / element_bytes(d.dtype);
-  return d.dim % e == 0 && (d.batch == 1 || s[0] % e == 0) && (length == 1 || s[1] % e == 0) &&
+  return d.dim % e == 0 && (d.batch == 1 || s[0] % e == 0) &&
+         (length == 1 || (s[1] % e == 0 && s[1] * element_bytes(d.dtype) < kAttnFarStride)) &&
          (heads == 1 || s[2] % e == 0);
 }
 

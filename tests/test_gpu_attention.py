@@ -224,6 +224,25 @@ def test_one_state(dtype, lq, share, lk, dim):
 
 
 @pytest.mark.parametrize("dtype", list(TYPES))
+def test_rows_far_apart(dtype):
+    """Rows so far apart that a tile of them spans 2^31 bytes and more."""
+    q, k, v, grad = _inputs(1, 70, 5, 2, 1, 64, dtype)
+    apart = (1 << 25) // q.element_size()
+    for stride in (apart, apart + 64):
+        far = torch.zeros(4 * stride + 128, dtype=q.dtype, device="cuda")
+        for which in ("k", "v"):
+            at = far.as_strided((1, 5, 1, 64), (1, stride, 64, 1))
+            at.copy_(k if which == "k" else v)
+            args = (q, at, v) if which == "k" else (q, k, at)
+            out, lse = rdv.cross_attention(*args, return_lse=True)
+            ref, ref_lse = rdv.cross_attention(q, k, v, return_lse=True)
+            assert torch.equal(out, ref) and torch.equal(lse, ref_lse)
+            for a, b in zip(rdv.cross_attention_backward(grad, *args, out, lse),
+                            rdv.cross_attention_backward(grad, q, k, v, out, lse)):
+                assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
 @pytest.mark.parametrize("shape", [(1, 2048, 77, 2, 2, 64), (1, 300, 2500, 2, 1, 64), (2, 1000, 1030, 2, 1, 128),
                                    (1, 40, 9000, 1, 1, 32)])
 def test_longer(dtype, shape):
