@@ -67,14 +67,21 @@ Plan make_plan(const rdv_attention_desc& d, bool backward, int cu) {
     p.packs[i] = at;
     at += align256(rows[i] * p.dim * element_bytes(d.dtype));
   }
+  const bool wide = d.dtype == RDV_DTYPE_F32;  // products take 16 times as long
+  const int tile = attn_has_pairs(d.dtype, d.dim) ? 64 : 32;
   if (!backward) {
     // The states are split among blocks where the rows' blocks alone leave CUs idle, and each still has 256 states or
     // more: the partial results cost a write, a read and a launch.  4,096 rows x 8 heads (256 blocks) x 256 states of
-    // 64 dimensions in fp16 took 25 us in two splits.  Few rows stream the states: up to eight blocks per
+    // 64 dimensions in fp16 took 25 us in two splits.  In fp32 64 states are enough (1,000 x 300, 2 heads of 80: 39.5 us
+    // with 256, 23.4 with 64; backward 91 and 67), but forward not of 32 dimensions (12 and 16).  Few rows stream the states: up to eight blocks per
     // CU, of which two run, so that items of unequal lengths fill the chip to the end (8 tokens against 0 to 32,001 states,
     // 4 heads of 128 in bf16: 82 us with four, 78.7 with eight, 81.5 with sixteen, whose join takes 8 us instead of 6.8).
+    // Where that leaves CUs idle, down to 128 states (1 token, 1,000 states, 8 heads of 128 in fp32: 30.4 us, then 24.6),
+    // if there is a join anyway or in fp32 (4 tokens, 500 states, 8 heads of 64: fp32 16.4 and 14.4, bf16 10.3 and 14.2).
     p.forward = p.few ? split_axis(p.bh, 8 * int64_t(cu), d.keys, 128, 256)
-                      : split_axis(p.bh * p.row_tiles, cu, d.keys, 64, 256);
+                      : split_axis(p.bh * p.row_tiles, cu, d.keys, 64, wide && d.dim > 32 ? 64 : 256);
+    if (p.few && p.bh * p.forward.count < cu && (wide || p.forward.count > 1))
+      p.forward = split_axis(p.bh, cu, d.keys, 128, 128);
     if (p.forward.count > 1) {
       const int64_t partial = p.forward.count * p.bh * p.rows;
       p.part = at;
@@ -86,10 +93,11 @@ Plan make_plan(const rdv_attention_desc& d, bool backward, int cu) {
     p.stats = at;
     at += align256(p.bh * p.rows * 8);
     // a split is a whole number of the kernels' tiles (at most 64): dK and dV's rows end with a tile, not with a split
-    p.dq = split_axis(p.bh * p.row_tiles, cu, d.keys, 64, 256);
-    // (fp32's products outweigh the partials: from 64 rows on.  4 x 1,000 x 333, 4 heads on 2 of 40: backward 75.7 us, from
-    // 128 rows on 82.8; fp16's do not: 4,096 x 77, 8 heads of 64: 32 and 27.5)
-    p.dkv = split_axis(p.bh * p.key_tiles, 2 * int64_t(cu), p.rows, 64, d.dtype == RDV_DTYPE_F32 ? 64 : 128);
+    p.dq = split_axis(p.bh * p.row_tiles, cu, d.keys, 64, wide ? 64 : 256);
+    // (fp32's products outweigh the partials: from a tile's rows on.  4 x 1,000 x 333, 4 heads on 2 of 40: backward 75.7
+    // us, from 128 rows on 82.8; 1,000 x 300, 2 heads of 80: 57, from 64 rows on 67.  fp16's do not: 4,096 x 77, 8 heads of
+    // 64: 32 and 27.5)
+    p.dkv = split_axis(p.bh * p.key_tiles, 2 * int64_t(cu), p.rows, tile, wide ? tile : 128);
     const int64_t a = p.dq.count > 1 ? align256(p.dq.count * p.bh * p.rows * p.pdim * 4) : 0;
     const int64_t b = p.dkv.count > 1 ? align256(p.dkv.count * p.bh * d.keys * p.pdim * 4) : 0;
     p.part = at;  // dQ's partials are summed before dK's and dV's are written
