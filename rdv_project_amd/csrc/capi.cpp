@@ -827,6 +827,8 @@ static int check_attention(const rdv_attention_desc* d, bool backward) {
   if (longest >= (int64_t(1) << 31) - 1024 ||
       (d->batch > 0 && longest > 0 && int64_t(d->batch) * d->heads > (int64_t(1) << 40) / d->dim / longest))
     return fail(RDV_ERR_INVALID, "attention: tensor too large");
+  if (int64_t(d->heads / d->kv_heads) * d->queries >= (int64_t(1) << 31) - 1024)
+    return fail(RDV_ERR_UNSUPPORTED, "attention: too many rows per state head");
   for (int i = 0; i < 3; ++i)
     if (!stride_ok(d->q_stride[i]) || !stride_ok(d->k_stride[i]) || !stride_ok(d->v_stride[i]) ||
         (backward && !stride_ok(d->g_stride[i])))

@@ -117,6 +117,18 @@ def test_library_refuses_attention(kw, code, text):
     assert lib.rdv_cross_attention(C.byref(d), 16, 16, 16, None, None, 16, None, None, 0, None) == code
 
 
+def test_library_refuses_rows_past_32_bits():
+    """The queries of the heads on one state head are one axis, which counts in 31 bits."""
+    lib = _lib.load()
+    d = _attn_desc(queries=1 << 16, heads=1 << 15, kv_heads=1)
+    for backward in (0, 1):
+        assert lib.rdv_cross_attention_workspace_bytes(C.byref(d), backward) == _lib.RDV_ERR_UNSUPPORTED
+        assert "rows" in _lib.last_error()
+    d.queries = 1 << 14
+    for backward in (0, 1):
+        assert lib.rdv_cross_attention_workspace_bytes(C.byref(d), backward) >= 0
+
+
 def test_library_refuses_null_pointers_and_dropout_arguments():
     lib = _lib.load()
     assert lib.rdv_group_norm(None, 16, None, None, 16, None, None, 0, None) == _lib.RDV_ERR_INVALID
