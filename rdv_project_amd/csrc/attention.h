@@ -658,10 +658,18 @@ __global__ __launch_bounds__(256, NC * sizeof(T) > 24 ? 1 : NC * sizeof(T) > 8 ?
         __builtin_amdgcn_s_setprio(1);
 #pragma unroll
         for (int u = 0; u < SUB; ++u) s[u] = f32x16{};
+        if constexpr (sizeof(T) == 4) {
 #pragma unroll
-        for (int e = 0; e < NC; ++e)
+          for (int u = 0; u < SUB; ++u)
+            if (uint32_t(now >> (32 * u)))  // products that take long: not of 32 states that do not count
 #pragma unroll
-          for (int u = 0; u < SUB; ++u) s[u] = mma(row_frag<T, NC>(tk + 32 * u * G::kRow, n32, e, h), qf[e], s[u]);
+              for (int e = 0; e < NC; ++e) s[u] = mma(row_frag<T, NC>(tk + 32 * u * G::kRow, n32, e, h), qf[e], s[u]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < NC; ++e)
+#pragma unroll
+            for (int u = 0; u < SUB; ++u) s[u] = mma(row_frag<T, NC>(tk + 32 * u * G::kRow, n32, e, h), qf[e], s[u]);
+        }
         __builtin_amdgcn_s_setprio(0);
         if (now != (SUB == 2 ? ~uint64_t(0) : uint64_t(~uint32_t(0)))) {
 #pragma unroll
@@ -670,7 +678,8 @@ __global__ __launch_bounds__(256, NC * sizeof(T) > 24 ? 1 : NC * sizeof(T) > 8 ?
         sm.template take<T>(s, c);
         __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-        for (int u = 0; u < SUB; ++u)
+        for (int u = 0; u < SUB; ++u) {
+          if (sizeof(T) == 4 && !uint32_t(now >> (32 * u))) continue;
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
             const auto pf = result_frag<T>(s[u], half);
@@ -678,6 +687,7 @@ __global__ __launch_bounds__(256, NC * sizeof(T) > 24 ? 1 : NC * sizeof(T) > 8 ?
             for (int d = 0; d < ND; ++d)
               sm.o[d] = mma(col_frag<T, NC>(tv + 32 * u * G::kRow, half, d, lane), pf, sm.o[d]);
           }
+        }
         __builtin_amdgcn_s_setprio(0);
       });
   float total = sum_halves(sm.total);
@@ -900,6 +910,7 @@ __global__ __launch_bounds__(256, NC * sizeof(T) > 16 ? 1 : NC * sizeof(T) > 8 ?
           const uint8_t* const uk = tk + 32 * sub * G::kRow;
           const uint8_t* const uv = tv + 32 * sub * G::kRow;
           const uint32_t now = uint32_t(bits >> (32 * sub));
+          if (!now) continue;
           f32x16 s{}, dp{};
           __builtin_amdgcn_s_setprio(1);
 #pragma unroll
@@ -960,12 +971,13 @@ __global__ __launch_bounds__(256, NC * sizeof(T) > 16 ? 1 : NC * sizeof(T) > 8 ?
 
 // dK and dV: a block of 4 waves, 32 states each (K and V fragments in registers), walks its share of the rows in tiles
 // of RT: S = Q K^T and dP = dO V^T from Q's and dO's rows, dV^T += dO^T P and dK^T += Q^T dS from their columns.  A
-// state that does not count is a column of its own, and is written as 0; a row that does not has P = 0.
+// state that does not count is a column of its own, and is written as 0; a row that does not has P = 0.  WR = 4: at most
+// 32 states, the same in every wave, which takes every fourth 32 rows.
 // 4 x 4,096 x 1,024, 8 heads on 4 of 64, fp16: 88 us, 0.78 PFLOP/s of its four products, and 7.5 us for the sums of its
 // splits; bound as the forward kernel.  Two waves per SIMD up to 96 dimensions in 16 bits and 32 in fp32: with one, whose
 // registers hold more reads ahead, both backward kernels took 278 us instead of 222 at 96 dimensions; at 128, two spill
 // (362 us against 334), as in fp32 from 48 on (4 x 1,000 x 333, 4 heads on 2 of 40, both directions: 92 us against 78).
-template <class T, int NC>
+template <class T, int NC, int WR>
 __global__ __launch_bounds__(256, NC > (sizeof(T) == 4 ? 2 : 6) ? 1 : 2) void attn_dkv_kernel(AttnArgs a) {
   using G = AttnTile<T, NC>;
   constexpr int RT = attn_tile_keys<T, NC>(), SUB = RT / 32, ND = G::ND;
@@ -980,7 +992,8 @@ __global__ __launch_bounds__(256, NC > (sizeof(T) == 4 ? 2 : 6) ? 1 : 2) void at
   const int tid = int(threadIdx.x), lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int h = lane >> 5, n32 = lane & 31;
   const BlockAt p = block_at(a);
-  const int key0 = p.tile * 128, key = key0 + wave * 32 + n32;
+  const int group = wave % (4 / WR), share = wave / (4 / WR);
+  const int key0 = p.tile * (128 / WR), key = key0 + group * 32 + n32;
   const int limit = key_limit(a, p.item);
   const bool counts = key < limit && (!a.mask || a.mask[p.item * a.ms + key] != 0);
   const bool active = __any(counts);
@@ -1048,6 +1061,7 @@ __global__ __launch_bounds__(256, NC > (sizeof(T) == 4 ? 2 : 6) ? 1 : 2) void at
       if (active) {
 #pragma unroll
         for (int u = 0; u < SUB; ++u) {
+          if (WR > 1 && (t * SUB + u) % WR != share) continue;
           const uint8_t* const tq = tiles[t & 1][0] + 32 * u * G::kRow;
           const uint8_t* const tg = tiles[t & 1][1] + 32 * u * G::kRow;
           f32x16 s{}, dp{};
@@ -1094,8 +1108,30 @@ __global__ __launch_bounds__(256, NC > (sizeof(T) == 4 ? 2 : 6) ? 1 : 2) void at
       hand_over((t + 1) & 1);
     }
   }
+  float fv = __builtin_amdgcn_exp2f(-Terms<T>::kLog2), fk = a.scale * fv / shrink;
+  if constexpr (WR > 1) {
+    float* const place = reinterpret_cast<float*>(&tiles[0][0][0]);
+    static_assert(2 * JoinTile<ND>::kFloats * 4 <= int(sizeof(tiles)), "the exchange fits the tiles");
+#pragma unroll
+    for (int d = 0; d < ND; ++d) {
+      dk[d] *= fk;
+      dv[d] *= fv;
+    }
+    fk = fv = 1.0f;
+    for (int n = WR / 2; n > 0; n >>= 1) {  // shares n .. 2 n - 1 hand theirs to shares 0 .. n - 1
+      float* const mine = place + (share % n * (4 / WR) + group) * JoinTile<ND>::kFloats;
+      auto join = [&](f32x16(&x)[ND]) {
+        __syncthreads();
+        if (share >= n && share < 2 * n) JoinTile<ND>::put(mine, x, n32, h);
+        __syncthreads();
+        if (share < n) JoinTile<ND>::add(mine, x, 1.0f, 1.0f, n32, h);
+      };
+      join(dk);
+      join(dv);
+    }
+    if (share != 0) return;
+  }
   if (key >= a.keys) return;
-  const float fv = __builtin_amdgcn_exp2f(-Terms<T>::kLog2), fk = a.scale * fv / shrink;
   const int64_t at = (int64_t(p.split) * a.batch * a.kv_heads + p.bh) * a.keys + key;
   T* const ok = static_cast<T*>(a.dk) + ((int64_t(p.item) * a.keys + key) * a.kv_heads + p.hk) * a.odim;
   T* const ov = static_cast<T*>(a.dv) + ((int64_t(p.item) * a.keys + key) * a.kv_heads + p.hk) * a.odim;
@@ -1119,7 +1155,7 @@ __global__ __launch_bounds__(256, NC > (sizeof(T) == 4 ? 2 : 6) ? 1 : 2) void at
 
 // ------------------------------------------------------------------ launches by type
 
-enum AttnKernel { kAttnTile, kAttnTilePairs, kAttnFew, kAttnDq, kAttnDqPairs, kAttnDkv };
+enum AttnKernel { kAttnTile, kAttnTilePairs, kAttnFew, kAttnDq, kAttnDqPairs, kAttnDkv, kAttnDkvShared };
 
 template <class T, int NC>
 int launch_attn_nc(AttnKernel which, const AttnArgs& a, unsigned blocks, hipStream_t stream) {
@@ -1135,7 +1171,8 @@ int launch_attn_nc(AttnKernel which, const AttnArgs& a, unsigned blocks, hipStre
     }
     case kAttnDq: attn_dq_kernel<T, NC, 1><<<blocks, 256, 0, stream>>>(a); break;
     case kAttnDqPairs: attn_dq_kernel<T, NC, kPairs><<<blocks, 256, 0, stream>>>(a); break;
-    case kAttnDkv: attn_dkv_kernel<T, NC><<<blocks, 256, 0, stream>>>(a); break;
+    case kAttnDkv: attn_dkv_kernel<T, NC, 1><<<blocks, 256, 0, stream>>>(a); break;
+    case kAttnDkvShared: attn_dkv_kernel<T, NC, 4><<<blocks, 256, 0, stream>>>(a); break;
   }
   RDV_HIP_TRY(hipGetLastError());
   return RDV_OK;

@@ -36,6 +36,7 @@ struct Plan {
   int rows, dim, pdim;            // folded rows; dimensions rounded up to 16 bytes, to 4
   int64_t bh;
   bool few, pairs;                // forward: at most 32 rows; forward and dQ: pairs of waves share 32 rows
+  bool shared;                    // dK and dV: at most 32 states, which a block's waves share
   Split forward, dq, dkv;
   int row_tiles, key_tiles;
   // byte offsets in the workspace, and its size
@@ -97,7 +98,10 @@ Plan make_plan(const rdv_attention_desc& d, bool backward, int cu) {
     // (fp32's products outweigh the partials: from a tile's rows on.  4 x 1,000 x 333, 4 heads on 2 of 40: backward 75.7
     // us, from 128 rows on 82.8; 1,000 x 300, 2 heads of 80: 57, from 64 rows on 67.  fp16's do not: 4,096 x 77, 8 heads of
     // 64: 32 and 27.5)
-    p.dkv = split_axis(p.bh * p.key_tiles, 2 * int64_t(cu), p.rows, tile, wide ? tile : 128);
+    // With at most 32 states the four waves share the rows (15,702 x 7, 32 heads on 8 of 40 in
+    // fp32: both backward kernels 419 us, then 288; 2,452 x 9, 4 heads on 1 of 64: 44.7 and 36.2).
+    p.shared = d.keys <= 32;
+    p.dkv = split_axis(p.bh * p.key_tiles, 2 * int64_t(cu), p.rows, tile, p.shared ? (wide ? 128 : 256) : wide ? tile : 128);
     const int64_t a = p.dq.count > 1 ? align256(p.dq.count * p.bh * p.rows * p.pdim * 4) : 0;
     const int64_t b = p.dkv.count > 1 ? align256(p.dkv.count * p.bh * d.keys * p.pdim * 4) : 0;
     p.part = at;  // dQ's partials are summed before dK's and dV's are written
@@ -168,17 +172,28 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a, int per) {
 }
 
 // The sum of the splits of dQ (KEYS false: rows of the queries) or of dK and dV (KEYS true: blockIdx.y picks the tensor),
-// four dimensions per thread, always in the splits' order.  4 x 1,024 x 4 heads of 64 in 4 splits: 7.5 us for 38 MB.
+// four dimensions per thread, or per `per` threads (1 to 16) that share the splits where those are many, always in the
+// same order.  4 x 1,024 x 4 heads of 64 in 4 splits: 7.5 us for 38 MB; 9 states of 64 in 154 splits: 8.4 us, then 5.
 template <class T, bool KEYS>
-__global__ __launch_bounds__(256) void attn_sum_kernel(AttnArgs a) {
-  const uint32_t len = KEYS ? a.keys : a.rows, quads = uint32_t(a.pdim) / 4;
-  const uint32_t i = blockIdx.x * 256 + threadIdx.x, row = i / quads, d = 4 * (i - row * quads);
+__global__ __launch_bounds__(256) void attn_sum_kernel(AttnArgs a, int per) {
+  __shared__ f32x4 sums[256];
+  const uint32_t len = KEYS ? a.keys : a.rows, quads = uint32_t(a.pdim) / 4, width = 256 / per;
+  const uint32_t at = threadIdx.x & (width - 1), share = threadIdx.x / width;
+  const uint32_t i = blockIdx.x * width + at, row = i / quads, d = 4 * (i - row * quads);
   const int64_t n = int64_t(a.batch) * a.kv_heads * len;
-  if (row >= n) return;
   const f32x4* part = reinterpret_cast<const f32x4*>(KEYS && blockIdx.y ? a.part2 : a.part) + int64_t(row) * quads + d / 4;
   f32x4 sum{};
+  if (row < n) {
 #pragma unroll 4
-  for (int s = 0; s < a.splits; ++s) sum += part[s * n * quads];
+    for (int s = share; s < a.splits; s += per) sum += part[s * n * quads];
+  }
+  if (per > 1) {
+    sums[threadIdx.x] = sum;
+    __syncthreads();
+    if (share != 0) return;
+    for (int s = 1; s < per; ++s) sum += sums[s * width + at];
+  }
+  if (row >= n) return;
   const int bh = int(row / len), x = int(row - bh * len), item = bh / a.kv_heads, hk = bh - item * a.kv_heads;
   T* out;
   if constexpr (KEYS) {
@@ -189,6 +204,14 @@ __global__ __launch_bounds__(256) void attn_sum_kernel(AttnArgs a) {
   }
   store_quad(out, int(d), a.odim, sum[0], sum[1], sum[2], sum[3]);
 }
+
+// Threads that share the sum of `splits` partial results, 4 or more of them each.
+int sharers(int splits) {
+  int per = 1;
+  while (per < 16 && 8 * per <= splits) per *= 2;
+  return per;
+}
+unsigned sum_blocks(int64_t sums, int per) { return unsigned((sums * per + 255) / 256); }
 
 __global__ __launch_bounds__(256) void attn_zero_kernel(uint16_t* p, int64_t n) {
   for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < n; i += int64_t(gridDim.x) * 256) p[i] = 0;
@@ -339,8 +362,9 @@ int launch_attention_backward(const rdv_attention_desc& d, const void* grad, con
   rc = launch_matrix(d.dtype, p.pairs ? kAttnDqPairs : kAttnDq, a, cu, stream);
   if (rc != RDV_OK) return rc;
   if (a.splits > 1) {
+    const int per = sharers(a.splits);
     rc = with_dtype(d.dtype, [&](auto t) {
-      attn_sum_kernel<decltype(t), false><<<dim3(unsigned((n * (p.pdim / 4) + 255) / 256)), 256, 0, stream>>>(a);
+      attn_sum_kernel<decltype(t), false><<<dim3(sum_blocks(n * (p.pdim / 4), per)), 256, 0, stream>>>(a, per);
       RDV_HIP_TRY(hipGetLastError());
       return int(RDV_OK);
     });
@@ -350,10 +374,11 @@ int launch_attention_backward(const rdv_attention_desc& d, const void* grad, con
   a.splits = p.dkv.count;
   a.chunk = p.dkv.chunk;
   a.part2 = reinterpret_cast<float*>(ws + p.part2);
-  rc = launch_matrix(d.dtype, kAttnDkv, a, cu, stream);
+  rc = launch_matrix(d.dtype, p.shared ? kAttnDkvShared : kAttnDkv, a, cu, stream);
   if (rc != RDV_OK || a.splits == 1) return rc;
+  const int per = sharers(a.splits);
   return with_dtype(d.dtype, [&](auto t) {
-    attn_sum_kernel<decltype(t), true><<<dim3(unsigned((p.bh * d.keys * (p.pdim / 4) + 255) / 256), 2), 256, 0, stream>>>(a);
+    attn_sum_kernel<decltype(t), true><<<dim3(sum_blocks(p.bh * d.keys * (p.pdim / 4), per), 2), 256, 0, stream>>>(a, per);
     RDV_HIP_TRY(hipGetLastError());
     return int(RDV_OK);
   });

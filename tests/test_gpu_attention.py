@@ -243,6 +243,18 @@ def test_rows_far_apart(dtype):
 
 
 @pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("lk", [2, 7, 32, 33])
+def test_few_states_many_rows(dtype, lk):
+    """Few states, whose rows the waves of a block share; gradients of bands of rows differ by powers of two, up to those
+    whose dS is beyond fp16's range with the factor that the small ones get."""
+    q, k, v, grad = _inputs(2, 700, lk, 4, 2, 64, dtype)
+    grad = grad * (2.0 ** (torch.arange(700, device="cuda") // 32 % 7)).to(grad.dtype)[None, :, None, None]
+    mask = torch.rand(2, lk, generator=torch.Generator().manual_seed(lk)) < 0.8
+    mask[:, 0] = True
+    _check(q, k, v, grad, dtype, mask=mask.cuda(), what=f"{lk} states")
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
 @pytest.mark.parametrize("shape", [(1, 2048, 77, 2, 2, 64), (1, 300, 2500, 2, 1, 64), (2, 1000, 1030, 2, 1, 128),
                                    (1, 40, 9000, 1, 1, 32)])
 def test_longer(dtype, shape):
