@@ -74,9 +74,10 @@ Plan make_plan(const rdv_attention_desc& d, bool backward, int cu) {
     // The states are split among blocks where the rows' blocks alone leave CUs idle, and each still has 256 states or
     // more: the partial results cost a write, a read and a launch.  4,096 rows x 8 heads (256 blocks) x 256 states of
     // 64 dimensions in fp16 took 25 us in two splits.  In fp32 64 states are enough (1,000 x 300, 2 heads of 80: 39.5 us
-    // with 256, 23.4 with 64; backward 91 and 67), but forward not of 32 dimensions (12 and 16).  Few rows stream the states: up to eight blocks per
-    // CU, of which two run, so that items of unequal lengths fill the chip to the end (8 tokens against 0 to 32,001 states,
-    // 4 heads of 128 in bf16: 82 us with four, 78.7 with eight, 81.5 with sixteen, whose join takes 8 us instead of 6.8).
+    // with 256, 23.4 with 64; backward 91 and 67), but forward not of 32 dimensions (12 and 16).  Few rows stream the
+    // states: up to eight blocks per CU, of which two run, so that items of unequal lengths fill the chip to the end (8
+    // tokens against 0 to 32,001 states, 4 heads of 128 in bf16: 82 us with four, 78.7 with eight, 81.5 with sixteen, whose
+    // join takes 8 us instead of 6.8).
     // Where that leaves CUs idle, down to 128 states (1 token, 1,000 states, 8 heads of 128 in fp32: 30.4 us, then 24.6),
     // if there is a join anyway or in fp32 (4 tokens, 500 states, 8 heads of 64: fp32 16.4 and 14.4, bf16 10.3 and 14.2).
     p.forward = p.few ? split_axis(p.bh, 8 * int64_t(cu), d.keys, 128, 256)
