@@ -971,8 +971,8 @@ __global__ __launch_bounds__(256, NC * sizeof(T) > 16 ? 1 : NC * sizeof(T) > 8 ?
 
 // dK and dV: a block of 4 waves, 32 states each (K and V fragments in registers), walks its share of the rows in tiles
 // of RT: S = Q K^T and dP = dO V^T from Q's and dO's rows, dV^T += dO^T P and dK^T += Q^T dS from their columns.  A
-// state that does not count is a column of its own, and is written as 0; a row that does not has P = 0.  WR = 4: at most
-// 32 states, the same in every wave, which takes every fourth 32 rows.
+// state that does not count is a column of its own, and is written as 0; a row that does not has P = 0.  WR = 2: pairs of
+// waves share 32 states and take a half of each tile.
 // 4 x 4,096 x 1,024, 8 heads on 4 of 64, fp16: 88 us, 0.78 PFLOP/s of its four products, and 7.5 us for the sums of its
 // splits; bound as the forward kernel.  Two waves per SIMD up to 96 dimensions in 16 bits and 32 in fp32: with one, whose
 // registers hold more reads ahead, both backward kernels took 278 us instead of 222 at 96 dimensions; at 128, two spill
@@ -981,6 +981,7 @@ template <class T, int NC, int WR>
 __global__ __launch_bounds__(256, NC > (sizeof(T) == 4 ? 2 : 6) ? 1 : 2) void attn_dkv_kernel(AttnArgs a) {
   using G = AttnTile<T, NC>;
   constexpr int RT = attn_tile_keys<T, NC>(), SUB = RT / 32, ND = G::ND;
+  static_assert(SUB >= WR, "a tile has 32 rows for every wave of a state group");
   // one variable: the tiles come first, within the 64 KiB that the direct loads reach
   __shared__ __attribute__((aligned(16))) struct {
     uint8_t tiles[2][2][RT * G::kRow];
@@ -1061,7 +1062,7 @@ __global__ __launch_bounds__(256, NC > (sizeof(T) == 4 ? 2 : 6) ? 1 : 2) void at
       if (active) {
 #pragma unroll
         for (int u = 0; u < SUB; ++u) {
-          if (WR > 1 && (t * SUB + u) % WR != share) continue;
+          if (WR > 1 && u % WR != share) continue;
           const uint8_t* const tq = tiles[t & 1][0] + 32 * u * G::kRow;
           const uint8_t* const tg = tiles[t & 1][1] + 32 * u * G::kRow;
           f32x16 s{}, dp{};
@@ -1118,17 +1119,15 @@ __global__ __launch_bounds__(256, NC > (sizeof(T) == 4 ? 2 : 6) ? 1 : 2) void at
       dv[d] *= fv;
     }
     fk = fv = 1.0f;
-    for (int n = WR / 2; n > 0; n >>= 1) {  // shares n .. 2 n - 1 hand theirs to shares 0 .. n - 1
-      float* const mine = place + (share % n * (4 / WR) + group) * JoinTile<ND>::kFloats;
-      auto join = [&](f32x16(&x)[ND]) {
-        __syncthreads();
-        if (share >= n && share < 2 * n) JoinTile<ND>::put(mine, x, n32, h);
-        __syncthreads();
-        if (share < n) JoinTile<ND>::add(mine, x, 1.0f, 1.0f, n32, h);
-      };
-      join(dk);
-      join(dv);
-    }
+    float* const mine = place + group * JoinTile<ND>::kFloats;
+    auto join = [&](f32x16(&x)[ND]) {  // the second wave of a pair hands over its columns
+      __syncthreads();
+      if (share == 1) JoinTile<ND>::put(mine, x, n32, h);
+      __syncthreads();
+      if (share == 0) JoinTile<ND>::add(mine, x, 1.0f, 1.0f, n32, h);
+    };
+    join(dk);
+    join(dv);
     if (share != 0) return;
   }
   if (key >= a.keys) return;
@@ -1155,7 +1154,7 @@ __global__ __launch_bounds__(256, NC > (sizeof(T) == 4 ? 2 : 6) ? 1 : 2) void at
 
 // ------------------------------------------------------------------ launches by type
 
-enum AttnKernel { kAttnTile, kAttnTilePairs, kAttnFew, kAttnDq, kAttnDqPairs, kAttnDkv, kAttnDkvShared };
+enum AttnKernel { kAttnTile, kAttnTilePairs, kAttnFew, kAttnDq, kAttnDqPairs, kAttnDkv, kAttnDkvPairs };
 
 template <class T, int NC>
 int launch_attn_nc(AttnKernel which, const AttnArgs& a, unsigned blocks, hipStream_t stream) {
@@ -1172,7 +1171,7 @@ int launch_attn_nc(AttnKernel which, const AttnArgs& a, unsigned blocks, hipStre
     case kAttnDq: attn_dq_kernel<T, NC, 1><<<blocks, 256, 0, stream>>>(a); break;
     case kAttnDqPairs: attn_dq_kernel<T, NC, kPairs><<<blocks, 256, 0, stream>>>(a); break;
     case kAttnDkv: attn_dkv_kernel<T, NC, 1><<<blocks, 256, 0, stream>>>(a); break;
-    case kAttnDkvShared: attn_dkv_kernel<T, NC, 4><<<blocks, 256, 0, stream>>>(a); break;
+    case kAttnDkvPairs: attn_dkv_kernel<T, NC, kPairs><<<blocks, 256, 0, stream>>>(a); break;
   }
   RDV_HIP_TRY(hipGetLastError());
   return RDV_OK;

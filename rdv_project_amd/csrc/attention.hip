@@ -36,7 +36,7 @@ struct Plan {
   int rows, dim, pdim;            // folded rows; dimensions rounded up to 16 bytes, to 4
   int64_t bh;
   bool few, pairs;                // forward: at most 32 rows; forward and dQ: pairs of waves share 32 rows
-  bool shared;                    // dK and dV: at most 32 states, which a block's waves share
+  bool key_pairs;                 // dK and dV: pairs of waves share 32 states
   Split forward, dq, dkv;
   int row_tiles, key_tiles;
   // byte offsets in the workspace, and its size
@@ -99,10 +99,13 @@ Plan make_plan(const rdv_attention_desc& d, bool backward, int cu) {
     // (fp32's products outweigh the partials: from a tile's rows on.  4 x 1,000 x 333, 4 heads on 2 of 40: backward 75.7
     // us, from 128 rows on 82.8; 1,000 x 300, 2 heads of 80: 57, from 64 rows on 67.  fp16's do not: 4,096 x 77, 8 heads of
     // 64: 32 and 27.5)
-    // With at most 32 states the four waves share the rows (15,702 x 7, 32 heads on 8 of 40 in
-    // fp32: both backward kernels 419 us, then 288; 2,452 x 9, 4 heads on 1 of 64: 44.7 and 36.2).
-    p.shared = d.keys <= 32;
-    p.dkv = split_axis(p.bh * p.key_tiles, 2 * int64_t(cu), p.rows, tile, p.shared ? (wide ? 128 : 256) : wide ? tile : 128);
+    // Pairs of waves share 32 states where half of the waves would have none (2,452 x 9, 4 heads on 1 of 64 in fp32: both
+    // backward kernels 42, then 30 us) or the splits leave CUs idle (1,000 x 300, 2 heads of 64: 43.7 and 36.7).  Else the
+    // rows' tiles feed more states without (4 x 4,096 x 1,024 in fp16: 85 us and 92).
+    const int least = wide ? tile : 128;
+    p.key_pairs = tile == 64 && (d.keys <= 64 || p.bh * p.key_tiles * std::max(1, p.rows / least) < cu);
+    if (p.key_pairs) p.key_tiles = (d.keys + 63) / 64;
+    p.dkv = split_axis(p.bh * p.key_tiles, 2 * int64_t(cu), p.rows, tile, least);
     const int64_t a = p.dq.count > 1 ? align256(p.dq.count * p.bh * p.rows * p.pdim * 4) : 0;
     const int64_t b = p.dkv.count > 1 ? align256(p.dkv.count * p.bh * d.keys * p.pdim * 4) : 0;
     p.part = at;  // dQ's partials are summed before dK's and dV's are written
@@ -375,7 +378,7 @@ int launch_attention_backward(const rdv_attention_desc& d, const void* grad, con
   a.splits = p.dkv.count;
   a.chunk = p.dkv.chunk;
   a.part2 = reinterpret_cast<float*>(ws + p.part2);
-  rc = launch_matrix(d.dtype, p.shared ? kAttnDkvShared : kAttnDkv, a, cu, stream);
+  rc = launch_matrix(d.dtype, p.key_pairs ? kAttnDkvPairs : kAttnDkv, a, cu, stream);
   if (rc != RDV_OK || a.splits == 1) return rc;
   const int per = sharers(a.splits);
   return with_dtype(d.dtype, [&](auto t) {
