@@ -698,24 +698,46 @@ __global__ __launch_bounds__(kNormBackThreads, 4) void norm_sums_kernel(NormArgs
   sum_groups<VE>(a, p, norm_lds, [&](int g, float wa, float wb) { group_part[int64_t(g) * a.chunks] = float2{wa, wb}; });
 }
 
-// Sums `count` rows of per-channel (A, B) of `parts` from row `first` on over the block.
-template <int VE>
-__device__ __forceinline__ void gather_sums(const NormArgs& a, const NormAt& p, int64_t first, int64_t count,
-                                            float (&sa)[VE], float (&sb)[VE]) {
+// dweight and dbias of the block's 16 channels: the chunks' sums of all images, 4 W rows of 16 channels at a time over W
+// waves and eight of those in flight, joined in a fixed order.  Bound: latency.  One block for a whole slab, each thread
+// with one row's piece in flight, was the last of the launch to end: it took 17.9 us for a 13,083 x 192 bf16 image (409
+// chunks), so 13.8; for 256 x 256 x 64 in fp32 12.7 and 11.1.
+template <int W>
+__device__ __forceinline__ void sum_params(const NormArgs& a, int block) {
+  __shared__ float2 waves[W][16];
+  constexpr int U = 8;
+  const int c = block * 16 + (int(threadIdx.x) & 15), wave = int(threadIdx.x) >> 6;
+  const int64_t count = int64_t(a.images) * a.chunks;
+  float sa = 0.0f, sb = 0.0f;
+  for (int64_t k = int(threadIdx.x) >> 4; k < count; k += U * 4 * W) {
+    float2 t[U];
 #pragma unroll
-  for (int i = 0; i < VE; ++i) sa[i] = sb[i] = 0.0f;
-  if (!p.on) return;
-  for (int64_t k = p.tr; k < count; k += a.tr) {
-    const float2* const part = a.parts + (first + k) * a.channels + p.c0 + p.channel;
+    for (int j = 0; j < U; ++j)
+      t[j] = a.parts[min(k + j * 4 * W, count - 1) * a.channels + min(c, a.channels - 1)];
 #pragma unroll
-    for (int i = 0; i < VE; ++i) {
-      sa[i] += part[i].x;
-      sb[i] += part[i].y;
+    for (int j = 0; j < U; ++j) {
+      const bool on = k + j * 4 * W < count;
+      sa += on ? t[j].x : 0.0f;
+      sb += on ? t[j].y : 0.0f;
     }
   }
+  for (int o = 16; o < 64; o *= 2) {
+    sa += __shfl_xor(sa, o);
+    sb += __shfl_xor(sb, o);
+  }
+  if ((threadIdx.x & 63) < 16) waves[wave][threadIdx.x & 15] = float2{sa, sb};
+  __syncthreads();
+  if (threadIdx.x >= 16 || c >= a.channels) return;
+#pragma unroll
+  for (int w = 1; w < W; ++w) {
+    sa += waves[w][threadIdx.x].x;
+    sb += waves[w][threadIdx.x].y;
+  }
+  if (a.dbias) a.dbias[c] = sa;
+  if (a.dweight) a.dweight[c] = sb;
 }
 
-// The last launch, backward.  Its first `slabs` blocks sum dweight and dbias over images and chunks; the others join
+// The last launch, backward.  Its first blocks sum dweight and dbias over images and chunks; the others join
 // their image's chunks' sums per group and write dx.  (With every block joining the sums per channel, eight times the
 // bytes of groups of eight, 3 x 77 x 53 x 48 in fp32 took 7.7 us instead of 5.2.)
 template <class T, int VE>
@@ -724,17 +746,12 @@ __global__ __launch_bounds__(kNormBackThreads, 4) void norm_dx_kernel(NormArgs a
   constexpr int U = kNormBackUnroll;
   float* const red = norm_lds;
   float sa[VE], sb[VE];
-  if (int(blockIdx.x) < a.slabs) {
-    const NormAt p = norm_at<VE>(a, 0, int(blockIdx.x));
-    gather_sums<VE>(a, p, 0, int64_t(a.images) * a.chunks, sa, sb);
-    sum_rows<VE>(a, p, sa, sb, red);
-    for (int c = int(threadIdx.x); c < p.channels; c += int(blockDim.x)) {
-      if (a.dbias) a.dbias[p.c0 + c] = channel_sum<VE>(a, red, c);
-      if (a.dweight) a.dweight[p.c0 + c] = channel_sum<VE>(a, red + a.red, c);
-    }
+  const int param_blocks = (a.channels + 15) / 16;
+  if (int(blockIdx.x) < param_blocks) {
+    sum_params<kNormBackThreads / 64>(a, int(blockIdx.x));
     return;
   }
-  const NormChunk ch = norm_chunk(a, int(blockIdx.x) - a.slabs);
+  const NormChunk ch = norm_chunk(a, int(blockIdx.x) - param_blocks);
   const NormAt p = norm_at<VE>(a, ch.image, ch.slab);
   float* const m1 = red + 2 * a.red;
   float* const m2 = m1 + a.slab_groups;
@@ -791,29 +808,7 @@ __global__ __launch_bounds__(kNormBackThreads, 4) void norm_dx_kernel(NormArgs a
 }
 
 // dweight and dbias alone, from `chunks` rows of sums per image.
-__global__ __launch_bounds__(256) void norm_params_kernel(NormArgs a) {
-  __shared__ float2 red[256];
-  const int c = int(blockIdx.x * 16 + (threadIdx.x & 15)), tr = int(threadIdx.x >> 4);
-  float2 s{0.0f, 0.0f};
-  if (c < a.channels)
-    for (int64_t k = tr; k < int64_t(a.images) * a.chunks; k += 16) {
-      const float2 t = a.parts[k * a.channels + c];
-      s.x += t.x;
-      s.y += t.y;
-    }
-  red[threadIdx.x] = s;
-  for (int n = 8; n > 0; n >>= 1) {
-    __syncthreads();
-    if (tr < n) {
-      red[threadIdx.x].x += red[threadIdx.x + 16 * n].x;
-      red[threadIdx.x].y += red[threadIdx.x + 16 * n].y;
-    }
-  }
-  if (tr == 0 && c < a.channels) {
-    if (a.dbias) a.dbias[c] = red[threadIdx.x].x;
-    if (a.dweight) a.dweight[c] = red[threadIdx.x].y;
-  }
-}
+__global__ __launch_bounds__(256) void norm_params_kernel(NormArgs a) { sum_params<4>(a, int(blockIdx.x)); }
 
 // ------------------------------------------------------------------ groups wider than a slab
 
@@ -1127,7 +1122,7 @@ int launch_group_norm_backward(const rdv_group_norm_desc& d, const void* grad, c
       return int(RDV_OK);
     });
   }
-  const int64_t blocks = d.images * p.slabs * p.chunks + (p.kind == NormPlan::kChunked ? p.slabs : 0);
+  const int64_t blocks = d.images * p.slabs * p.chunks + (p.kind == NormPlan::kChunked ? param_blocks : 0);
   if (int rc = check_blocks(blocks)) return rc;
   const unsigned lds = unsigned(2 * a.red + 2 * a.slab_groups) * 4;
   return with_piece(d.dtype, p.ve, [&](auto t, auto ve) {
@@ -1138,7 +1133,7 @@ int launch_group_norm_backward(const rdv_group_norm_desc& d, const void* grad, c
       kernel<<<dim3(unsigned(blocks)), p.threads, lds, stream>>>(a);
       if (d.images > 1) norm_params_kernel<<<dim3(param_blocks), 256, 0, stream>>>(a);
     } else {
-      norm_sums_kernel<T, VE><<<dim3(unsigned(blocks - p.slabs)), p.threads, lds, stream>>>(a);
+      norm_sums_kernel<T, VE><<<dim3(unsigned(blocks - param_blocks)), p.threads, lds, stream>>>(a);
       norm_dx_kernel<T, VE><<<dim3(unsigned(blocks)), p.threads, lds, stream>>>(a);
     }
     RDV_HIP_TRY(hipGetLastError());
