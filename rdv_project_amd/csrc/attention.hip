@@ -39,9 +39,18 @@ struct Plan {
   bool key_pairs;                 // dK and dV: pairs of waves share 32 states
   Split forward, dq, dkv;
   int row_tiles, key_tiles;
+  bool packed[5];                 // q, k, v, grad, out: whether the kernels read a copy (see in_place)
   // byte offsets in the workspace, and its size
   int64_t packs[5], stats, part, part2, ml, bytes;
 };
+
+// The strides of `out`, which is contiguous.
+struct RowStrides {
+  int64_t s[3];
+};
+RowStrides out_strides(const rdv_attention_desc& d) {
+  return RowStrides{{int64_t(d.queries) * d.heads * d.dim, int64_t(d.heads) * d.dim, d.dim}};
+}
 
 Plan make_plan(const rdv_attention_desc& d, bool backward, int cu) {
   Plan p{};
@@ -59,14 +68,15 @@ Plan make_plan(const rdv_attention_desc& d, bool backward, int cu) {
   int64_t at = 0;
   // copies of inputs that cannot be read in place
   const int64_t q_rows = int64_t(d.batch) * d.queries * d.heads, k_rows = int64_t(d.batch) * d.keys * d.kv_heads;
-  const int64_t rows[5] = {in_place(d, d.q_stride, d.queries, d.heads) ? 0 : q_rows,
-                           in_place(d, d.k_stride, d.keys, d.kv_heads) ? 0 : k_rows,
-                           in_place(d, d.v_stride, d.keys, d.kv_heads) ? 0 : k_rows,
-                           !backward || in_place(d, d.g_stride, d.queries, d.heads) ? 0 : q_rows,
-                           !backward || d.dim % e == 0 ? 0 : q_rows};
+  const int64_t rows[5] = {q_rows, k_rows, k_rows, q_rows, q_rows};
+  p.packed[0] = !in_place(d, d.q_stride, d.queries, d.heads);
+  p.packed[1] = !in_place(d, d.k_stride, d.keys, d.kv_heads);
+  p.packed[2] = !in_place(d, d.v_stride, d.keys, d.kv_heads);
+  p.packed[3] = backward && !in_place(d, d.g_stride, d.queries, d.heads);
+  p.packed[4] = backward && !in_place(d, out_strides(d).s, d.queries, d.heads);
   for (int i = 0; i < 5; ++i) {
     p.packs[i] = at;
-    at += align256(rows[i] * p.dim * element_bytes(d.dtype));
+    if (p.packed[i]) at += align256(rows[i] * p.dim * element_bytes(d.dtype));
   }
   const bool wide = d.dtype == RDV_DTYPE_F32;  // products take 16 times as long
   const int tile = attn_has_pairs(d.dtype, d.dim) ? 64 : 32;
@@ -251,7 +261,7 @@ AttnArgs make_args(const rdv_attention_desc& d, const Plan& p, const int32_t* le
 // The tensor itself, or its aligned copy in the workspace.
 int input(const rdv_attention_desc& d, const Plan& p, int which, const void* x, const int64_t (&s)[3], int length,
           int heads, uint8_t* ws, const void** out, int64_t (&os)[3], hipStream_t stream) {
-  if (length == 0 || in_place(d, s, length, heads)) {
+  if (length == 0 || !p.packed[which]) {
     if (length > 0 && reinterpret_cast<uintptr_t>(x) % 16 != 0)
       return fail(RDV_ERR_INVALID, "attention: a tensor of aligned strides must be 16-byte aligned itself");
     *out = x;
@@ -349,8 +359,7 @@ int launch_attention_backward(const rdv_attention_desc& d, const void* grad, con
   if (rc == RDV_OK) rc = input(d, p, 2, v, d.v_stride, d.keys, d.kv_heads, ws, &a.v, a.vs, stream);
   if (rc == RDV_OK) rc = input(d, p, 3, grad, d.g_stride, d.queries, d.heads, ws, &a.g, a.gs, stream);
   if (rc != RDV_OK) return rc;
-  const int64_t o_stride[3] = {int64_t(d.queries) * d.heads * d.dim, int64_t(d.heads) * d.dim, d.dim};
-  rc = input(d, p, 4, out, o_stride, d.queries, d.heads, ws, &a.o, a.os, stream);
+  rc = input(d, p, 4, out, out_strides(d).s, d.queries, d.heads, ws, &a.o, a.os, stream);
   if (rc != RDV_OK) return rc;
   a.lse = const_cast<float*>(lse);
   a.stats = reinterpret_cast<float2*>(ws + p.stats);

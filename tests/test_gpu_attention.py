@@ -345,3 +345,18 @@ def test_tensor_op_chain():
     cond.mul_(-1.5)
     op.evaluate_chain()
     assert torch.equal(op.as_type("torch"), expect())
+
+
+def test_backward_of_rows_that_are_all_copied():
+    """65,536 heads of 128 in fp32: rows 2^25 bytes apart, so that q, grad and out are copied before they are read.  The
+    same heads as items of a batch, whose rows are near, give the same bits."""
+    heads = 1 << 16
+    q, k, v, grad = _inputs(1, 2, 1, heads, heads, 128, "f32")
+    out, lse = rdv.cross_attention(q, k, v, return_lse=True)
+    got = rdv.cross_attention_backward(grad, q, k, v, out, lse)
+    items = lambda t: t.reshape(t.shape[1], heads // 16, 16, 128).transpose(0, 1).contiguous()
+    near = [items(t) for t in (q, k, v)]
+    ref, ref_lse = rdv.cross_attention(*near, return_lse=True)
+    assert torch.equal(items(out), ref) and torch.equal(lse.reshape(ref_lse.shape), ref_lse)
+    for a, b in zip(got, rdv.cross_attention_backward(items(grad), *near, ref, ref_lse)):
+        assert torch.equal(items(a), b)

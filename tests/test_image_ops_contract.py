@@ -140,3 +140,16 @@ def test_library_refuses_null_pointers_and_dropout_arguments():
                  (16, None, 16, 4, 0, float("nan")), (None, None, 16, 4, 0, 0.5)):
         assert lib.rdv_dropout(*args, 0, 0, None) == _lib.RDV_ERR_INVALID
     assert lib.rdv_dropout(None, None, None, 0, 0, 0.5, 0, 0, None) == _lib.RDV_OK
+
+
+@pytest.mark.parametrize("heads", [65536, 32768])
+def test_library_holds_every_copy_that_the_backward_call_makes(heads):
+    """q, grad and out whose rows lie 2^25 bytes apart or more are copied before they are read: 65,536 heads of 128 in
+    fp32 are, half as many are read in place.  The workspace has the copies and the rows' statistics."""
+    lib = _lib.load()
+    d = _attn_desc(queries=2, keys=1, heads=heads, kv_heads=heads, dim=128, dtype=_lib.DTYPE_F32)
+    for stride, rows in ((d.q_stride, 2), (d.k_stride, 1), (d.v_stride, 1), (d.g_stride, 2)):
+        stride[:] = rows * heads * 128, heads * 128, 128
+    copy, stats = 2 * heads * 128 * 4, 2 * heads * 8
+    copies = 3 if heads * 128 * 4 >= 1 << 25 else 0
+    assert lib.rdv_cross_attention_workspace_bytes(C.byref(d), 1) >= copies * copy + stats
