@@ -23,7 +23,6 @@
 // us, backward 6.6 and 5.2 us.
 // Variance.  Squares are taken of deviations from a mean of the thread's own values, and blocks' (mean, sum of squared
 // deviations) are joined with their means' distances: no difference of large sums.
-#include <algorithm>
 #include <numeric>
 
 #include "operators.h"
@@ -51,7 +50,9 @@ struct NormArgs {
   int wave_rows;                 // rows side by side in a wave, 0 where a row's pieces spread over waves
   int red;                       // floats of one statistic of a block's LDS rows (a wave's, or a row's)
   int chunks, chunk_rows;        // blocks of an image's slab, rows of one
+  int block0;                    // this launch's first block
 };
+__device__ __forceinline__ int norm_block(const NormArgs& a) { return a.block0 + int(blockIdx.x); }
 
 template <class T, int VE>
 struct Piece {
@@ -363,7 +364,8 @@ constexpr int kNormUnroll = 4, kNormThreads = 1024, kNormBackThreads = 512, kNor
 template <class T, int VE, int R>
 __global__ __launch_bounds__(1024) void norm_whole_kernel(NormArgs a) {
   extern __shared__ float norm_lds[];
-  const NormAt p = norm_at<VE>(a, int(blockIdx.x) / a.slabs, int(blockIdx.x) % a.slabs);
+  const int block = norm_block(a);
+  const NormAt p = norm_at<VE>(a, block / a.slabs, block % a.slabs);
   float* const red = norm_lds;
   float* const mean_g = red + 2 * a.red + 64;
   float* const rstd_g = mean_g + a.slab_groups;
@@ -433,7 +435,8 @@ __device__ __forceinline__ void dx_lines(const NormArgs& a, const NormAt& p, con
 template <class T, int VE, int R>
 __global__ __launch_bounds__(1024) void norm_whole_back_kernel(NormArgs a) {
   extern __shared__ float norm_lds[];
-  const NormAt p = norm_at<VE>(a, int(blockIdx.x) / a.slabs, int(blockIdx.x) % a.slabs);
+  const int block = norm_block(a);
+  const NormAt p = norm_at<VE>(a, block / a.slabs, block % a.slabs);
   float* const red = norm_lds;
   float* const m1 = red + 2 * a.red;
   float* const m2 = m1 + a.slab_groups;
@@ -531,7 +534,7 @@ template <class T, int VE>
 __global__ __launch_bounds__(kNormThreads) void norm_stats_kernel(NormArgs a) {
   extern __shared__ float norm_lds[];
   constexpr int U = kNormUnroll;
-  const NormChunk ch = norm_chunk(a, int(blockIdx.x));
+  const NormChunk ch = norm_chunk(a, norm_block(a));
   const NormAt p = norm_at<VE>(a, ch.image, ch.slab);
   float* const red = norm_lds;
   float* const mean_g = red + 2 * a.red + 64;
@@ -591,7 +594,7 @@ template <class T, int VE>
 __global__ __launch_bounds__(kNormThreads) void norm_apply_kernel(NormArgs a) {
   extern __shared__ float norm_lds[];
   constexpr int U = kNormUnroll;
-  const NormChunk ch = norm_chunk(a, int(blockIdx.x));
+  const NormChunk ch = norm_chunk(a, norm_block(a));
   const NormAt p = norm_at<VE>(a, ch.image, ch.slab);
   float* const mean_g = norm_lds;
   float* const rstd_g = mean_g + a.slab_groups;
@@ -654,7 +657,7 @@ template <class T, int VE>
 __global__ __launch_bounds__(kNormBackThreads, 4) void norm_sums_kernel(NormArgs a) {
   extern __shared__ float norm_lds[];
   constexpr int U = kNormBackUnroll;
-  const NormChunk ch = norm_chunk(a, int(blockIdx.x));
+  const NormChunk ch = norm_chunk(a, norm_block(a));
   const NormAt p = norm_at<VE>(a, ch.image, ch.slab);
   const T* const x = static_cast<const T*>(a.x) + p.image * a.x_image + p.c0 + p.channel;
   const T* const g = static_cast<const T*>(a.grad) + p.image * a.g_image + p.c0 + p.channel;
@@ -747,11 +750,12 @@ __global__ __launch_bounds__(kNormBackThreads, 4) void norm_dx_kernel(NormArgs a
   float* const red = norm_lds;
   float sa[VE], sb[VE];
   const int param_blocks = (a.channels + 15) / 16;
-  if (int(blockIdx.x) < param_blocks) {
-    sum_params<kNormBackThreads / 64>(a, int(blockIdx.x));
+  const int block = norm_block(a);
+  if (block < param_blocks) {
+    sum_params<kNormBackThreads / 64>(a, block);
     return;
   }
-  const NormChunk ch = norm_chunk(a, int(blockIdx.x) - param_blocks);
+  const NormChunk ch = norm_chunk(a, block - param_blocks);
   const NormAt p = norm_at<VE>(a, ch.image, ch.slab);
   float* const m1 = red + 2 * a.red;
   float* const m2 = m1 + a.slab_groups;
@@ -824,8 +828,9 @@ __device__ __forceinline__ float block_sum(float v, float* scratch) {
 template <class T>
 __global__ __launch_bounds__(256) void norm_wide_kernel(NormArgs a) {
   __shared__ float scratch[4];
-  const int64_t image = int(blockIdx.x) / a.groups;
-  const int group = int(blockIdx.x) % a.groups, c0 = group * a.width;
+  const int block = norm_block(a);
+  const int64_t image = block / a.groups;
+  const int group = block % a.groups, c0 = group * a.width;
   const T* const x = static_cast<const T*>(a.x) + image * a.x_image + c0;
   T* const y = static_cast<T*>(a.y) + image * a.rows * a.channels + c0;
   const float m = float(a.rows) * float(a.width);
@@ -845,8 +850,8 @@ __global__ __launch_bounds__(256) void norm_wide_kernel(NormArgs a) {
     else mean = s;
   }
   if (a.stats && threadIdx.x == 0) {
-    a.stats[2 * int64_t(blockIdx.x)] = mean;
-    a.stats[2 * int64_t(blockIdx.x) + 1] = rstd;
+    a.stats[2 * int64_t(block)] = mean;
+    a.stats[2 * int64_t(block) + 1] = rstd;
   }
   for (int64_t r = 0; r < a.rows; ++r)
     for (int c = int(threadIdx.x); c < a.width; c += 256) {
@@ -858,9 +863,9 @@ __global__ __launch_bounds__(256) void norm_wide_kernel(NormArgs a) {
 // One thread per (image, channel): A and B.
 template <class T>
 __global__ __launch_bounds__(256) void norm_wide_sums_kernel(NormArgs a) {
-  const int per = (a.channels + 255) / 256;
-  const int64_t image = int(blockIdx.x) / per;
-  const int c = int(blockIdx.x) % per * 256 + int(threadIdx.x);
+  const int per = (a.channels + 255) / 256, block = norm_block(a);
+  const int64_t image = block / per;
+  const int c = block % per * 256 + int(threadIdx.x);
   if (c >= a.channels) return;
   const T* const x = static_cast<const T*>(a.x) + image * a.x_image + c;
   const T* const g = static_cast<const T*>(a.grad) + image * a.g_image + c;
@@ -880,8 +885,9 @@ __global__ __launch_bounds__(256) void norm_wide_sums_kernel(NormArgs a) {
 template <class T>
 __global__ __launch_bounds__(256) void norm_wide_dx_kernel(NormArgs a) {
   __shared__ float scratch[4];
-  const int64_t image = int(blockIdx.x) / a.groups;
-  const int group = int(blockIdx.x) % a.groups, c0 = group * a.width;
+  const int block = norm_block(a);
+  const int64_t image = block / a.groups;
+  const int group = block % a.groups, c0 = group * a.width;
   const T* const x = static_cast<const T*>(a.x) + image * a.x_image + c0;
   const T* const g = static_cast<const T*>(a.grad) + image * a.g_image + c0;
   T* const dx = static_cast<T*>(a.y) + image * a.rows * a.channels + c0;
@@ -895,7 +901,7 @@ __global__ __launch_bounds__(256) void norm_wide_dx_kernel(NormArgs a) {
   }
   m1 = block_sum(m1, scratch) / m;
   m2 = block_sum(m2, scratch) / m;
-  const float mean = a.stats[2 * int64_t(blockIdx.x)], rstd = a.stats[2 * int64_t(blockIdx.x) + 1];
+  const float mean = a.stats[2 * int64_t(block)], rstd = a.stats[2 * int64_t(block) + 1];
   for (int64_t r = 0; r < a.rows; ++r)
     for (int c = int(threadIdx.x); c < a.width; c += 256) {
       const float w = a.weight ? a.weight[c0 + c] : 1.0f, b = a.bias ? a.bias[c0 + c] : 0.0f;
@@ -1052,6 +1058,15 @@ int check_blocks(int64_t n) {
   return n < (int64_t(1) << 31) ? int(RDV_OK) : fail(RDV_ERR_UNSUPPORTED, "group norm: too many blocks");
 }
 
+// kernel(a) by `blocks` blocks, in as many launches as that takes.
+template <class K>
+int launch_norm(K kernel, NormArgs a, int64_t blocks, int threads, unsigned lds, hipStream_t stream) {
+  return launch_blocks(blocks, threads, [&](int64_t first, unsigned count) {
+    a.block0 = int(first);
+    kernel<<<dim3(count), threads, lds, stream>>>(a);
+  });
+}
+
 }  // namespace
 
 // The base pointers' alignment is not known here: the most any of the piece sizes asks for.
@@ -1071,9 +1086,7 @@ int launch_group_norm(const rdv_group_norm_desc& d, const void* x, const float* 
   if (p.kind == NormPlan::kWide) {
     if (int rc = check_blocks(d.images * d.groups)) return rc;
     return with_dtype(d.dtype, [&](auto t) {
-      norm_wide_kernel<decltype(t)><<<dim3(unsigned(d.images * d.groups)), 256, 0, stream>>>(a);
-      RDV_HIP_TRY(hipGetLastError());
-      return int(RDV_OK);
+      return launch_norm(norm_wide_kernel<decltype(t)>, a, d.images * d.groups, 256, 0, stream);
     });
   }
   const int64_t blocks = d.images * p.slabs * p.chunks;
@@ -1084,13 +1097,10 @@ int launch_group_norm(const rdv_group_norm_desc& d, const void* x, const float* 
     constexpr int VE = decltype(ve)::value;
     if (p.kind == NormPlan::kWhole) {
       const auto kernel = d.rows <= 4 * p.tr ? norm_whole_kernel<T, VE, 4> : norm_whole_kernel<T, VE, whole_pieces(false, VE)>;
-      kernel<<<dim3(unsigned(blocks)), p.threads, lds, stream>>>(a);
-    } else {
-      norm_stats_kernel<T, VE><<<dim3(unsigned(blocks)), p.threads, lds, stream>>>(a);
-      norm_apply_kernel<T, VE><<<dim3(unsigned(blocks)), p.threads, unsigned(2 * (p.slab / a.width) * 4), stream>>>(a);
+      return launch_norm(kernel, a, blocks, p.threads, lds, stream);
     }
-    RDV_HIP_TRY(hipGetLastError());
-    return int(RDV_OK);
+    if (int rc = launch_norm(norm_stats_kernel<T, VE>, a, blocks, p.threads, lds, stream)) return rc;
+    return launch_norm(norm_apply_kernel<T, VE>, a, blocks, p.threads, unsigned(2 * (p.slab / a.width) * 4), stream);
   });
 }
 
@@ -1107,19 +1117,17 @@ int launch_group_norm_backward(const rdv_group_norm_desc& d, const void* grad, c
   a.dweight = dweight;
   a.dbias = dbias;
   if (empty) a.images = 0;
-  const unsigned param_blocks = unsigned((d.channels + 15) / 16);
+  const int64_t param_blocks = (d.channels + 15) / 16;
   if (empty || p.kind == NormPlan::kWide) {
     const int64_t per = (d.channels + 255) / 256;
     if (int rc = check_blocks(d.images * std::max<int64_t>(d.groups, per))) return rc;
     return with_dtype(d.dtype, [&](auto t) {
       using T = decltype(t);
       if (!empty) {
-        norm_wide_sums_kernel<T><<<dim3(unsigned(d.images * per)), 256, 0, stream>>>(a);
-        norm_wide_dx_kernel<T><<<dim3(unsigned(d.images * d.groups)), 256, 0, stream>>>(a);
+        if (int rc = launch_norm(norm_wide_sums_kernel<T>, a, d.images * per, 256, 0, stream)) return rc;
+        if (int rc = launch_norm(norm_wide_dx_kernel<T>, a, d.images * d.groups, 256, 0, stream)) return rc;
       }
-      norm_params_kernel<<<dim3(param_blocks), 256, 0, stream>>>(a);
-      RDV_HIP_TRY(hipGetLastError());
-      return int(RDV_OK);
+      return launch_norm(norm_params_kernel, a, param_blocks, 256, 0, stream);
     });
   }
   const int64_t blocks = d.images * p.slabs * p.chunks + (p.kind == NormPlan::kChunked ? param_blocks : 0);
@@ -1130,14 +1138,11 @@ int launch_group_norm_backward(const rdv_group_norm_desc& d, const void* grad, c
     constexpr int VE = decltype(ve)::value;
     if (p.kind == NormPlan::kWhole) {
       const auto kernel = d.rows <= 4 * p.tr ? norm_whole_back_kernel<T, VE, 4> : norm_whole_back_kernel<T, VE, whole_pieces(true, VE)>;
-      kernel<<<dim3(unsigned(blocks)), p.threads, lds, stream>>>(a);
-      if (d.images > 1) norm_params_kernel<<<dim3(param_blocks), 256, 0, stream>>>(a);
-    } else {
-      norm_sums_kernel<T, VE><<<dim3(unsigned(blocks - param_blocks)), p.threads, lds, stream>>>(a);
-      norm_dx_kernel<T, VE><<<dim3(unsigned(blocks)), p.threads, lds, stream>>>(a);
+      const int rc = launch_norm(kernel, a, blocks, p.threads, lds, stream);
+      return rc || d.images == 1 ? rc : launch_norm(norm_params_kernel, a, param_blocks, 256, 0, stream);
     }
-    RDV_HIP_TRY(hipGetLastError());
-    return int(RDV_OK);
+    if (int rc = launch_norm(norm_sums_kernel<T, VE>, a, blocks - param_blocks, p.threads, lds, stream)) return rc;
+    return launch_norm(norm_dx_kernel<T, VE>, a, blocks, p.threads, lds, stream);
   });
 }
 

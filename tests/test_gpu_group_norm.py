@@ -202,3 +202,21 @@ def test_tensor_op_between_convolutions():
     x.mul_(2.0)
     norm.evaluate_chain()
     assert torch.equal(norm.as_type("torch"), rdv.group_norm(conv.as_type("torch"), w, b, 8, activation="silu"))
+
+
+def test_more_images_than_a_launch_takes():
+    """2^24 + 2 images, a block each: more than 2^32 threads.  Every image against the same one in a smaller call."""
+    n, step = (1 << 24) + 2, 1 << 21
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x, grad = (torch.randn(n, 1, 8, generator=g, device="cuda").half() for _ in range(2))
+    w, b = torch.rand(8, generator=g, device="cuda") + 0.5, torch.randn(8, generator=g, device="cuda")
+
+    def call(part):
+        y, stats = rdv.group_norm(x[part], w, b, 2, activation="silu", return_stats=True)
+        return y, stats, rdv.group_norm_backward(grad[part], x[part], w, b, 2, stats, activation="silu")[0]
+
+    whole = call(slice(None))
+    for first in range(0, n, step):
+        part = slice(first, min(first + step, n))
+        for got, ref, what in zip(whole, call(part), ("y", "stats", "dx")):
+            assert torch.equal(got[part], ref), f"{what} of images from {first}"
