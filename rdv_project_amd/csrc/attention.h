@@ -35,6 +35,7 @@ struct AttnArgs {
   int batch, queries, keys, heads, kv_heads, share, rows, dim, odim, pdim;
   int tiles, splits, chunk;          // blocks: (item, state head) x split x tile; a split's share of the other axis
   int by_xcd;                        // whether an XCD takes a contiguous run of the blocks
+  uint32_t blocks, block0;           // of all launches, and this one's first
   float scale;
 };
 
@@ -365,7 +366,8 @@ struct BlockAt {
   int item, hk, bh, split, tile;
 };
 __device__ __forceinline__ BlockAt block_at(const AttnArgs& a) {
-  const uint32_t w = a.by_xcd ? xcd_contiguous(blockIdx.x, gridDim.x) : blockIdx.x, rest = w / uint32_t(a.tiles);
+  const uint32_t b = a.block0 + blockIdx.x;
+  const uint32_t w = a.by_xcd ? xcd_contiguous(b, a.blocks) : b, rest = w / uint32_t(a.tiles);
   BlockAt p;
   p.tile = int(w - rest * a.tiles);
   if (a.tiles == 1) {  // neighbouring blocks read the state heads of the same states, which lie side by side
@@ -1152,12 +1154,12 @@ __global__ __launch_bounds__(256, NC > (sizeof(T) == 4 ? 2 : 6) ? 1 : 2) void at
     }
 }
 
-// ------------------------------------------------------------------ launches by type
+// ------------------------------------------------------------------ launches by type (errors: the caller)
 
 enum AttnKernel { kAttnTile, kAttnTilePairs, kAttnFew, kAttnDq, kAttnDqPairs, kAttnDkv, kAttnDkvPairs };
 
 template <class T, int NC>
-int launch_attn_nc(AttnKernel which, const AttnArgs& a, unsigned blocks, hipStream_t stream) {
+void launch_attn_nc(AttnKernel which, const AttnArgs& a, unsigned blocks, hipStream_t stream) {
   constexpr int kPairs = attn_tile_keys<T, NC>() / 32;  // waves that can share a row group
   switch (which) {
     case kAttnTile: attn_tile_kernel<T, NC, 1><<<blocks, 256, 0, stream>>>(a); break;
@@ -1173,8 +1175,6 @@ int launch_attn_nc(AttnKernel which, const AttnArgs& a, unsigned blocks, hipStre
     case kAttnDkv: attn_dkv_kernel<T, NC, 1><<<blocks, 256, 0, stream>>>(a); break;
     case kAttnDkvPairs: attn_dkv_kernel<T, NC, kPairs><<<blocks, 256, 0, stream>>>(a); break;
   }
-  RDV_HIP_TRY(hipGetLastError());
-  return RDV_OK;
 }
 
 // Whether attn_tile_kernel and attn_dq_kernel come with pairs of waves: not for fp32 heads of more than 64 dimensions,
@@ -1182,7 +1182,7 @@ int launch_attn_nc(AttnKernel which, const AttnArgs& a, unsigned blocks, hipStre
 inline bool attn_has_pairs(int dtype, int dim) { return dtype != RDV_DTYPE_F32 || dim <= 64; }
 
 template <class T>
-int launch_attn_typed(AttnKernel which, const AttnArgs& a, unsigned blocks, hipStream_t stream) {
+void launch_attn_typed(AttnKernel which, const AttnArgs& a, unsigned blocks, hipStream_t stream) {
   if (a.dim <= 32) return launch_attn_nc<T, 2>(which, a, blocks, stream);
   if (a.dim <= 48) return launch_attn_nc<T, 3>(which, a, blocks, stream);
   if (a.dim <= 64) return launch_attn_nc<T, 4>(which, a, blocks, stream);
@@ -1191,8 +1191,8 @@ int launch_attn_typed(AttnKernel which, const AttnArgs& a, unsigned blocks, hipS
   return launch_attn_nc<T, 8>(which, a, blocks, stream);
 }
 
-int launch_attn_f32(AttnKernel which, const AttnArgs& a, unsigned blocks, hipStream_t stream);
-int launch_attn_f16(AttnKernel which, const AttnArgs& a, unsigned blocks, hipStream_t stream);
-int launch_attn_bf16(AttnKernel which, const AttnArgs& a, unsigned blocks, hipStream_t stream);
+void launch_attn_f32(AttnKernel which, const AttnArgs& a, unsigned blocks, hipStream_t stream);
+void launch_attn_f16(AttnKernel which, const AttnArgs& a, unsigned blocks, hipStream_t stream);
+void launch_attn_bf16(AttnKernel which, const AttnArgs& a, unsigned blocks, hipStream_t stream);
 
 }  // namespace rdv

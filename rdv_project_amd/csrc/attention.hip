@@ -1,7 +1,5 @@
 // Attention from an image's points to an encoder's states: planning, workspaces and the passes around the matrix-core
 // kernels of attention.h.  Build-defined (no counterpart in the reference).
-#include <algorithm>
-
 #include "attention.h"
 
 namespace rdv {
@@ -291,9 +289,12 @@ int launch_matrix(int dtype, AttnKernel which, AttnArgs& a, int cu, hipStream_t 
   // of blocks, the longest item's XCD would finish last (dK and dV of four items of 0 to 333 states x 2,000 rows in fp32:
   // 51 us, in plain order 34).  Blocks of few rows share nothing.
   a.by_xcd = which != kAttnFew && !a.lengths && blocks >= 2 * int64_t(cu);
-  if (dtype == RDV_DTYPE_F16) return launch_attn_f16(which, a, unsigned(blocks), stream);
-  if (dtype == RDV_DTYPE_BF16) return launch_attn_bf16(which, a, unsigned(blocks), stream);
-  return launch_attn_f32(which, a, unsigned(blocks), stream);
+  a.blocks = uint32_t(blocks);
+  const auto launch = dtype == RDV_DTYPE_F16 ? launch_attn_f16 : dtype == RDV_DTYPE_BF16 ? launch_attn_bf16 : launch_attn_f32;
+  return launch_blocks(blocks, 256, [&](int64_t first, unsigned count) {
+    a.block0 = uint32_t(first);
+    return launch(which, a, count, stream);
+  });
 }
 
 int check_plan(const rdv_attention_desc& d) {

@@ -3,8 +3,8 @@
 
 namespace rdv {
 
-int launch_attn_f16(AttnKernel which, const AttnArgs& a, unsigned blocks, hipStream_t stream) {
-  return launch_attn_typed<half_t>(which, a, blocks, stream);
+void launch_attn_f16(AttnKernel which, const AttnArgs& a, unsigned blocks, hipStream_t stream) {
+  launch_attn_typed<half_t>(which, a, blocks, stream);
 }
 
 }  // namespace rdv

@@ -360,3 +360,36 @@ def test_backward_of_rows_that_are_all_copied():
     assert torch.equal(items(out), ref) and torch.equal(lse.reshape(ref_lse.shape), ref_lse)
     for a, b in zip(got, rdv.cross_attention_backward(items(grad), *near, ref, ref_lse)):
         assert torch.equal(items(a), b)
+
+
+def _items_equal(call, batch, step):
+    """call(slice(None))'s results against those of `step` items at a time."""
+    whole = call(slice(None))
+    for first in range(0, batch, step):
+        part = slice(first, min(first + step, batch))
+        for i, (got, ref) in enumerate(zip(whole, call(part))):
+            assert torch.equal(got[part], ref), f"result {i} of items from {first}"
+
+
+@pytest.mark.parametrize("batch", [1 << 20, (1 << 20) + 1])
+def test_more_state_heads_than_a_launch_takes(batch):
+    """2^24 blocks and more, 2^32 threads: every item against the same one in a smaller call."""
+    g = torch.Generator(device="cuda").manual_seed(batch)
+    make = lambda n: torch.randn(batch, n, 16, 8, generator=g, device="cuda", dtype=torch.float16)
+    q, k, v, grad = (make(n) for n in (1, 2, 2, 1))
+    lengths = torch.randint(0, 3, (batch,), generator=g, device="cuda", dtype=torch.int32)
+
+    def call(part):
+        args = dict(key_lengths=lengths[part])
+        out, lse = rdv.cross_attention(q[part], k[part], v[part], return_lse=True, **args)
+        return out, lse, *rdv.cross_attention_backward(grad[part], q[part], k[part], v[part], out, lse, **args)
+
+    _items_equal(call, batch, 1 << 17)
+
+
+def test_more_tiles_than_a_launch_takes():
+    """The same for 33 queries, whose forward kernel is the one of many rows."""
+    batch = (1 << 20) + 1
+    g = torch.Generator(device="cuda").manual_seed(3)
+    q, k, v = (torch.randn(batch, n, 16, 8, generator=g, device="cuda", dtype=torch.float16) for n in (33, 2, 2))
+    _items_equal(lambda part: (rdv.cross_attention(q[part], k[part], v[part]),), batch, 1 << 17)
