@@ -39,11 +39,11 @@ constexpr int kPieces = 2;
 
 template <class T, bool VEC>
 __global__ __launch_bounds__(256) void dropout_kernel(const T* x, const T* residual, T* y, int64_t n,
-                                                      uint64_t threshold, float factor, uint64_t seed,
-                                                      uint64_t subsequence) {
+                                                      uint32_t block0, uint64_t threshold, float factor,
+                                                      uint64_t seed, uint64_t subsequence) {
   constexpr int E = VEC ? 16 / int(sizeof(T)) : 4;  // elements of a piece
   typedef T vec __attribute__((ext_vector_type(E)));
-  const int64_t first = (int64_t(blockIdx.x) * kPieces * 256 + threadIdx.x) * E;
+  const int64_t first = (int64_t(block0 + blockIdx.x) * kPieces * 256 + threadIdx.x) * E;
   vec vx[kPieces], vr[kPieces];
 #pragma unroll
   for (int k = 0; k < kPieces; ++k) {
@@ -95,15 +95,15 @@ int launch_dropout(const void* x, const void* residual, void* y, int64_t n, int 
   const bool aligned = ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(residual) |
                          reinterpret_cast<uintptr_t>(y)) & 15) == 0;
   const int64_t per = int64_t(256) * kPieces * (aligned ? (dtype == RDV_DTYPE_F32 ? 4 : 8) : 4);
-  const int64_t blocks = (n + per - 1) / per;
-  if (blocks >= (int64_t(1) << 31)) return fail(RDV_ERR_UNSUPPORTED, "rdv_dropout: n is too large");
+  const int64_t blocks = (n + per - 1) / per;  // below 2^30: n is at most 2^40
   return with_dtype(dtype, [&](auto t) {
     using T = decltype(t);
     const auto kernel = aligned ? dropout_kernel<T, true> : dropout_kernel<T, false>;
-    kernel<<<dim3(unsigned(blocks)), 256, 0, stream>>>(static_cast<const T*>(x), static_cast<const T*>(residual),
-                                                       static_cast<T*>(y), n, threshold, factor, seed, subsequence);
-    RDV_HIP_TRY(hipGetLastError());
-    return int(RDV_OK);
+    return launch_blocks(blocks, 256, [&](int64_t block0, unsigned count) {
+      kernel<<<dim3(count), 256, 0, stream>>>(static_cast<const T*>(x), static_cast<const T*>(residual),
+                                              static_cast<T*>(y), n, uint32_t(block0), threshold, factor, seed,
+                                              subsequence);
+    });
   });
 }
 

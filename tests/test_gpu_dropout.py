@@ -102,3 +102,15 @@ def test_tensor_op():
     op.subsequence = 9
     op.evaluate()
     assert torch.equal(op.as_type("torch"), rdv.dropout(x.relu(), 0.4, 3, 9, residual=r))
+
+
+def test_more_elements_than_a_launch_takes():
+    """2^35 unaligned 16-bit elements (64 GiB, in place) and some: more than 2^32 threads."""
+    n = (1 << 35) + 5000
+    x = torch.empty(n + 1, dtype=torch.bfloat16, device="cuda")[1:].fill_(1.0)
+    assert rdv.dropout(x, 0.5, 77, 3, out=x) is x
+    for first in (0, (1 << 33) - 2500, (1 << 35) - 2500, n - 2500):
+        part = x[first:first + 2500].float().cpu()
+        for i in (0, 1, 2, 3, 1001, 2048, 2498, 2499):
+            assert part[i].item() == (2.0 if O.dropout_keep(first + i, 0.5, 77, 3) else 0.0), first + i
+        assert ((part == 0) | (part == 2)).all()
