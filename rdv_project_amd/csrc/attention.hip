@@ -19,6 +19,8 @@ bool in_place(const rdv_attention_desc& d, const int64_t (&s)[3], int length, in
 
 // How an axis of `length` is split among blocks so that `blocks` of them become about `want`: every split takes a
 // multiple of `step` and at least `least`.
+// (Where there is more than one, at most want / 2 blocks of at most 128 rows or states have partial results: the kernels
+// that join and sum those count in 32 bits.)
 struct Split {
   int count, chunk;
 };
@@ -333,7 +335,6 @@ int launch_attention(const rdv_attention_desc& d, const void* q, const void* k, 
   int per = 1;
   while (per < 8 && 4 * per < a.splits) per *= 2;
   const int64_t blocks = (p.bh * p.rows + 8 / per - 1) / (8 / per);
-  if (blocks >= (int64_t(1) << 31)) return fail(RDV_ERR_UNSUPPORTED, "attention: too many rows");
   return with_dtype(d.dtype, [&](auto t) {
     attn_join_kernel<decltype(t)><<<dim3(unsigned(blocks)), 256, 0, stream>>>(a, per);
     RDV_HIP_TRY(hipGetLastError());
@@ -368,7 +369,6 @@ int launch_attention_backward(const rdv_attention_desc& d, const void* grad, con
   a.dk = dk;
   a.dv = dv;
   const int64_t n = p.bh * p.rows;
-  if (std::max(n, p.bh * int64_t(d.keys)) * (p.pdim / 4) >= (int64_t(1) << 32) - 256) return fail(RDV_ERR_UNSUPPORTED, "attention: too many rows");
   a.tiles = p.row_tiles;
   a.splits = p.dq.count;
   a.chunk = p.dq.chunk;

@@ -393,3 +393,18 @@ def test_more_tiles_than_a_launch_takes():
     g = torch.Generator(device="cuda").manual_seed(3)
     q, k, v = (torch.randn(batch, n, 16, 8, generator=g, device="cuda", dtype=torch.float16) for n in (33, 2, 2))
     _items_equal(lambda part: (rdv.cross_attention(q[part], k[part], v[part]),), batch, 1 << 17)
+
+
+def test_backward_of_many_wide_rows():
+    """2^27 rows of 128 dimensions (32 GiB of out, and of dq) and one state: q's and k's gradients are nothing, v's is the
+    rows' sum, here of powers of two, without rounding."""
+    rows = 1 << 27
+    g = torch.Generator(device="cuda").manual_seed(1)
+    q, k, v = (torch.randn(1, 1, 1, 128, generator=g, device="cuda", dtype=torch.bfloat16) for _ in range(3))
+    q, grad = q.expand(1, rows, 1, 128), torch.full_like(q, 2.0 ** -20).expand(1, rows, 1, 128)
+    out, lse = rdv.cross_attention(q, k, v, return_lse=True)
+    dq, dk, dv = rdv.cross_attention_backward(grad, q, k, v, out, lse)
+    del out
+    for part in dq.split(1 << 23, 1):
+        assert not part.any()
+    assert not dk.any() and (dv == 2.0 ** 7).all()
