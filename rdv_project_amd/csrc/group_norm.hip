@@ -711,19 +711,26 @@ __device__ __forceinline__ void sum_params(const NormArgs& a, int block) {
   constexpr int U = 8;
   const int c = block * 16 + (int(threadIdx.x) & 15), wave = int(threadIdx.x) >> 6;
   const int64_t count = int64_t(a.images) * a.chunks;
-  float sa = 0.0f, sb = 0.0f;
+  double da = 0.0, db = 0.0;  // a chain as long as the images are many: its roundings would add up in 32 bits
   for (int64_t k = int(threadIdx.x) >> 4; k < count; k += U * 4 * W) {
     float2 t[U];
 #pragma unroll
     for (int j = 0; j < U; ++j)
       t[j] = a.parts[min(k + j * 4 * W, count - 1) * a.channels + min(c, a.channels - 1)];
 #pragma unroll
-    for (int j = 0; j < U; ++j) {
-      const bool on = k + j * 4 * W < count;
-      sa += on ? t[j].x : 0.0f;
-      sb += on ? t[j].y : 0.0f;
-    }
+    for (int j = 0; j < U; ++j)
+      if (k + j * 4 * W >= count) t[j] = float2{0.0f, 0.0f};
+#pragma unroll
+    for (int n = U / 2; n > 0; n /= 2)
+#pragma unroll
+      for (int j = 0; j < n; ++j) {
+        t[j].x += t[j + n].x;
+        t[j].y += t[j + n].y;
+      }
+    da += t[0].x;
+    db += t[0].y;
   }
+  float sa = float(da), sb = float(db);
   for (int o = 16; o < 64; o *= 2) {
     sa += __shfl_xor(sa, o);
     sb += __shfl_xor(sb, o);

@@ -220,3 +220,13 @@ def test_more_images_than_a_launch_takes():
         part = slice(first, min(first + step, n))
         for got, ref, what in zip(whole, call(part), ("y", "stats", "dx")):
             assert torch.equal(got[part], ref), f"{what} of images from {first}"
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("images", [1 << 14, 1 << 18])
+def test_parameter_gradients_of_many_images(images, dtype):
+    """Equal terms, whose roundings do not cancel: dweight and dbias of many small images are held to the same bound as
+    those of one."""
+    x = torch.tensor([1.0, -1.0]).repeat(8).expand(images, 1, 16).to(TYPES[dtype]).cuda()
+    grad = torch.full((images, 1, 16), 0.1, dtype=TYPES[dtype], device="cuda")
+    _check(x, grad, torch.ones(16).cuda(), torch.zeros(16).cuda(), 8, "none", dtype, f"{images} images {dtype}")
