@@ -230,3 +230,25 @@ def test_parameter_gradients_of_many_images(images, dtype):
     x = torch.tensor([1.0, -1.0]).repeat(8).expand(images, 1, 16).to(TYPES[dtype]).cuda()
     grad = torch.full((images, 1, 16), 0.1, dtype=TYPES[dtype], device="cuda")
     _check(x, grad, torch.ones(16).cuda(), torch.zeros(16).cuda(), 8, "none", dtype, f"{images} images {dtype}")
+
+
+def test_long_images_of_many_blocks():
+    """8,192 rows of 1,024 channels, two rows of which a block takes side by side, in images that alone give every CU its
+    blocks.  Equal terms, whose roundings do not cancel: the sums over an image's rows are held to the same bounds as
+    short ones'.  (One image 513 times.)"""
+    images, rows, c = 513, 8192, 1024
+    x = torch.full((1, rows, c), 0.1, device="cuda")
+    x[:, ::1024] = -0.1
+    grad = torch.full((1, rows, c), 0.1, device="cuda")
+    w, b = torch.ones(c, device="cuda"), torch.zeros(c, device="cuda")
+    ref = O.group_norm(_np(x), _np(w), _np(b), 8, grad=_np(grad))
+    many = lambda t: t.expand(images, -1, -1)
+    y, stats = rdv.group_norm(many(x), w, b, 8, return_stats=True)
+    assert torch.equal(y, y[:1].expand_as(y))
+    _close(y[:1], ref["y"], O.group_norm_bound(ref, _np(w), _np(b), "f32"), "y")
+    del y
+    dx, dw, db = rdv.group_norm_backward(many(grad), many(x), w, b, 8, stats)
+    assert torch.equal(dx, dx[:1].expand_as(dx))
+    _close(dx[:1], ref["dx"], ref["dx_err"] + O._stored(ref["dx"], "f32"), "dx")
+    _close(dw, images * ref["dweight"], images * ref["dweight_err"], "dweight")
+    _close(db, images * ref["dbias"], images * ref["dbias_err"], "dbias")
