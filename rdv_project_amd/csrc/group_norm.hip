@@ -823,8 +823,12 @@ __global__ __launch_bounds__(kNormBackThreads, 4) void norm_dx_kernel(NormArgs a
 __global__ __launch_bounds__(256) void norm_params_kernel(NormArgs a) { sum_params<4>(a, int(blockIdx.x)); }
 
 // ------------------------------------------------------------------ groups wider than a slab
+//
+// A thread's sums run over all rows, one after the other: in 64 bits, or their roundings would add up (4,096 rows of
+// 1,536 values of 1000.1 had a mean off by 0.013, and so a normalised value of 0.97 for 0).  Bound: latency of one block's
+// loads per group, or one thread's per channel: 4,096 x 1,280 in fp32 takes 18.4 ms, and 8.7 ms backward.
 
-__device__ __forceinline__ float block_sum(float v, float* scratch) {
+__device__ __forceinline__ double block_sum(double v, double* scratch) {
   for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
   __syncthreads();
   if ((threadIdx.x & 63) == 0) scratch[threadIdx.x >> 6] = v;
@@ -835,27 +839,24 @@ __device__ __forceinline__ float block_sum(float v, float* scratch) {
 // One block per (image, group): mean, then the squared deviations from it, then y.
 template <class T>
 __global__ __launch_bounds__(256) void norm_wide_kernel(NormArgs a) {
-  __shared__ float scratch[4];
+  __shared__ double scratch[4];
   const int block = norm_block(a);
   const int64_t image = block / a.groups;
   const int group = block % a.groups, c0 = group * a.width;
   const T* const x = static_cast<const T*>(a.x) + image * a.x_image + c0;
   T* const y = static_cast<T*>(a.y) + image * a.rows * a.channels + c0;
-  const float m = float(a.rows) * float(a.width);
+  const double m = double(a.rows) * a.width;
   float mean = 0.0f, rstd = 0.0f;
   for (int pass = 0; pass < 2; ++pass) {
-    float s = 0.0f;
-    for (int64_t r = 0; r < a.rows; ++r) {
-      float t = 0.0f;  // a row's sum first: shorter chains of additions
+    double s = 0.0;
+    for (int64_t r = 0; r < a.rows; ++r)
       for (int c = int(threadIdx.x); c < a.width; c += 256) {
         const float v = to_f32(x[r * a.x_row + c]) - mean;
-        t += pass ? v * v : v;
+        s += pass ? v * v : v;
       }
-      s += t;
-    }
-    s = block_sum(s, scratch) / m;
-    if (pass) rstd = 1.0f / sqrtf(s + a.eps);
-    else mean = s;
+    const float of = float(block_sum(s, scratch) / m);
+    if (pass) rstd = 1.0f / sqrtf(of + a.eps);
+    else mean = of;
   }
   if (a.stats && threadIdx.x == 0) {
     a.stats[2 * int64_t(block)] = mean;
@@ -879,36 +880,35 @@ __global__ __launch_bounds__(256) void norm_wide_sums_kernel(NormArgs a) {
   const T* const g = static_cast<const T*>(a.grad) + image * a.g_image + c;
   const float* const st = a.stats + 2 * (image * a.groups + c / a.width);
   const float w = a.weight ? a.weight[c] : 1.0f, b = a.bias ? a.bias[c] : 0.0f;
-  float2 s{0.0f, 0.0f};
+  double sa = 0.0, sb = 0.0;
   for (int64_t r = 0; r < a.rows; ++r) {
     const float xhat = (to_f32(x[r * a.x_row]) - st[0]) * st[1];
     const float dz = to_f32(g[r * a.g_row]) * norm_act_slope(a.act, fmaf(xhat, w, b));
-    s.x += dz;
-    s.y = fmaf(dz, xhat, s.y);
+    sa += dz;
+    sb += dz * xhat;
   }
-  a.parts[image * a.channels + c] = s;
+  a.parts[image * a.channels + c] = float2{float(sa), float(sb)};
 }
 
 // One block per (image, group): dx.
 template <class T>
 __global__ __launch_bounds__(256) void norm_wide_dx_kernel(NormArgs a) {
-  __shared__ float scratch[4];
+  __shared__ double scratch[4];
   const int block = norm_block(a);
   const int64_t image = block / a.groups;
   const int group = block % a.groups, c0 = group * a.width;
   const T* const x = static_cast<const T*>(a.x) + image * a.x_image + c0;
   const T* const g = static_cast<const T*>(a.grad) + image * a.g_image + c0;
   T* const dx = static_cast<T*>(a.y) + image * a.rows * a.channels + c0;
-  const float m = float(a.rows) * float(a.width);
-  float m1 = 0.0f, m2 = 0.0f;
+  const double m = double(a.rows) * a.width;
+  double wa = 0.0, wb = 0.0;
   for (int c = int(threadIdx.x); c < a.width; c += 256) {
     const float w = a.weight ? a.weight[c0 + c] : 1.0f;
     const float2 s = a.parts[image * a.channels + c0 + c];
-    m1 += w * s.x;
-    m2 += w * s.y;
+    wa += w * s.x;
+    wb += w * s.y;
   }
-  m1 = block_sum(m1, scratch) / m;
-  m2 = block_sum(m2, scratch) / m;
+  const float m1 = float(block_sum(wa, scratch) / m), m2 = float(block_sum(wb, scratch) / m);
   const float mean = a.stats[2 * int64_t(block)], rstd = a.stats[2 * int64_t(block) + 1];
   for (int64_t r = 0; r < a.rows; ++r)
     for (int c = int(threadIdx.x); c < a.width; c += 256) {

@@ -252,3 +252,37 @@ def test_long_images_of_many_blocks():
     _close(dx[:1], ref["dx"], ref["dx_err"] + O._stored(ref["dx"], "f32"), "dx")
     _close(dw, images * ref["dweight"], images * ref["dweight_err"], "dweight")
     _close(db, images * ref["dbias"], images * ref["dbias_err"], "dbias")
+
+
+WIDE = [((1, 4096, 1536), 1), ((1, 16384, 2049), 1), ((2, 3000, 771), 3), ((1, 4099, 2056), 8)]
+
+
+@pytest.mark.parametrize("shape,groups", WIDE)
+def test_constant_wide_groups_far_from_zero(shape, groups):
+    """As test_constant_groups_far_from_zero: groups too wide for the kernels that keep a group's channels in a block."""
+    width = shape[2] // groups
+    for value in (1000.1, 10.1, 3.3):
+        x = torch.full(shape, value, device="cuda")
+        bias = torch.randn(shape[2], generator=torch.Generator().manual_seed(1)).cuda()
+        y, stats = rdv.group_norm(x, None, bias, groups, return_stats=True)
+        bound = 317 * value * 2.0 ** -24
+        assert ((y - bias).abs() <= bound).all(), value
+        dx, dw, db = rdv.group_norm_backward(torch.ones_like(x), x, None, bias, groups, stats)
+        assert torch.allclose(db, torch.full_like(db, shape[0] * shape[1]))
+        assert (dw.abs() <= shape[0] * shape[1] * bound).all()
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("shape,groups", WIDE + [((1, 4096, 2304), 1)])
+def test_wide_groups_of_many_rows(shape, groups, dtype):
+    x, grad, w, b = _inputs(shape, dtype, sum(shape))
+    _check(x, grad, w, b, groups, "silu", dtype, f"{shape} {groups} {dtype}")
+
+
+@pytest.mark.parametrize("shape,groups", WIDE)
+def test_wide_groups_of_equal_terms(shape, groups):
+    """Terms whose roundings do not cancel in a sum of them."""
+    x = torch.tensor([0.1, -0.3, 0.7]).repeat(shape[1] // 3 + 1)[:shape[1], None].expand(shape).contiguous().cuda()
+    grad = torch.full(shape, 0.1, device="cuda")
+    w, b = torch.ones(shape[2], device="cuda"), torch.zeros(shape[2], device="cuda")
+    _check(x, grad, w, b, groups, "none", "f32", f"{shape} {groups}")
