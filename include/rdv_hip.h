@@ -573,8 +573,8 @@ typedef struct rdv_group_norm_desc {
 int64_t rdv_group_norm_workspace_bytes(const rdv_group_norm_desc* desc, int32_t backward);
 
 /* y[images, rows, channels] (contiguous, not overlapping x) and, where stats is
- * not NULL, stats[images, groups, 2] = (mean, 1 / sqrt(var + eps)).  weight and
- * bias are fp32 [channels] or NULL (ones, zeros). */
+ * not NULL, stats[images, groups, 2] = (mean, 1 / sqrt(var + eps)), both sums 0
+ * for images without rows.  weight and bias are fp32 [channels] or NULL (ones, zeros). */
 int rdv_group_norm(const rdv_group_norm_desc* desc, const void* x, const float* weight, const float* bias, void* y,
                    float* stats, void* workspace, int64_t workspace_bytes, void* stream);
 

@@ -787,8 +787,8 @@ int rdv_group_norm(const rdv_group_norm_desc* desc, const void* x, const float* 
                    float* stats, void* workspace, int64_t workspace_bytes, void* stream) {
   const int rc = check_group_norm(desc, false);
   if (rc != RDV_OK) return rc;
-  if (desc->images == 0 || desc->rows == 0) return RDV_OK;
-  if (!x || !y) return fail(RDV_ERR_INVALID, "rdv_group_norm: NULL pointer argument");
+  if (desc->images == 0) return RDV_OK;
+  if (desc->rows > 0 && (!x || !y)) return fail(RDV_ERR_INVALID, "rdv_group_norm: NULL pointer argument");
   if (!aligned16(y)) return fail(RDV_ERR_INVALID, "rdv_group_norm: y must be 16-byte aligned");
   const int cu = plan_cu_count();
   if (!aligned16(workspace)) return fail(RDV_ERR_WORKSPACE, "rdv_group_norm: the workspace must be 16-byte aligned");

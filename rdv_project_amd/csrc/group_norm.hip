@@ -919,6 +919,14 @@ __global__ __launch_bounds__(256) void norm_wide_dx_kernel(NormArgs a) {
     }
 }
 
+// The statistics of images without rows: sums of nothing, as of a group of zeros.
+__global__ __launch_bounds__(256) void norm_no_rows_kernel(NormArgs a) {
+  const int64_t i = int64_t(norm_block(a)) * 256 + threadIdx.x;
+  if (i >= int64_t(a.images) * a.groups) return;
+  a.stats[2 * i] = 0.0f;
+  a.stats[2 * i + 1] = 1.0f / sqrtf(a.eps);
+}
+
 // ------------------------------------------------------------------ planning
 
 struct NormPlan {
@@ -1091,6 +1099,13 @@ int64_t group_norm_workspace_bytes(const rdv_group_norm_desc& d, bool backward, 
 
 int launch_group_norm(const rdv_group_norm_desc& d, const void* x, const float* weight, const float* bias, void* y,
                       float* stats, void* ws, int64_t ws_bytes, int cu, hipStream_t stream) {
+  if (d.rows == 0) {
+    NormArgs a = norm_args(d, NormPlan{}, x, weight, bias, nullptr);
+    a.stats = stats;
+    const int64_t blocks = (d.images * d.groups + 255) / 256;
+    if (int rc = check_blocks(blocks)) return rc;
+    return stats ? launch_norm(norm_no_rows_kernel, a, blocks, 256, 0, stream) : int(RDV_OK);
+  }
   const NormPlan p = norm_plan(d, false, cu, alignment({x, y}));
   if (ws_bytes < p.bytes) return fail(RDV_ERR_WORKSPACE, "rdv_group_norm: workspace too small");
   NormArgs a = norm_args(d, p, x, weight, bias, ws);

@@ -286,3 +286,11 @@ def test_wide_groups_of_equal_terms(shape, groups):
     grad = torch.full(shape, 0.1, device="cuda")
     w, b = torch.ones(shape[2], device="cuda"), torch.zeros(shape[2], device="cuda")
     _check(x, grad, w, b, groups, "none", "f32", f"{shape} {groups}")
+
+
+@pytest.mark.parametrize("images,groups", [(1, 1), (3, 2), (300, 4)])
+def test_statistics_of_images_without_rows(images, groups):
+    """Images of no rows have the statistics of sums of nothing, not what their memory held before."""
+    torch.full((images, groups, 2), 7.0, device="cuda")  # freed: the memory that the call's stats are likely to get
+    y, stats = rdv.group_norm(torch.empty(images, 0, 8, device="cuda"), None, None, groups, eps=0.25, return_stats=True)
+    assert y.numel() == 0 and (stats[..., 0] == 0).all() and (stats[..., 1] == 2).all()
