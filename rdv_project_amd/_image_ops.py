@@ -93,7 +93,10 @@ def _grad_tensors(grads, likes, names):
         return tuple(_like_out(None, t) for t in likes)
     if not isinstance(grads, (list, tuple)) or len(grads) != len(likes):
         raise TypeError(f"grads must be ({', '.join(names)})")
-    return tuple(_out_tensor(g, t.shape, t.dtype, t.device, n) for g, t, n in zip(grads, likes, names))
+    grads = tuple(_out_tensor(g, t.shape, t.dtype, t.device, n) for g, t, n in zip(grads, likes, names))
+    for i, g in enumerate(grads):
+        _apart(g, *zip(grads[:i], names))
+    return grads
 
 
 def _apart(out: torch.Tensor, *inputs) -> None:

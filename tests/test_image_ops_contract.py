@@ -153,3 +153,22 @@ def test_library_holds_every_copy_that_the_backward_call_makes(heads):
     copy, stats = 2 * heads * 128 * 4, 2 * heads * 8
     copies = 3 if heads * 128 * 4 >= 1 << 25 else 0
     assert lib.rdv_cross_attention_workspace_bytes(C.byref(d), 1) >= copies * copy + stats
+
+
+@pytest.mark.gpu
+def test_refusals_of_gradients_in_one_buffer():
+    """Gradients whose buffers overlap would overwrite each other."""
+    x, q, k = X.cuda(), Q.cuda(), K.cuda()
+    w, b, st, lse = W.cuda(), B.cuda(), torch.zeros(2, 3, 2).cuda(), LSE.cuda()
+    flat, two = torch.zeros(240).cuda(), torch.zeros(24).cuda()
+    dx, dq, dk = (torch.empty_like(t) for t in (x, q, k))
+    same = flat[:192].reshape(Q.shape), flat[48:240].reshape(K.shape)
+    for call in (
+        lambda: rdv.group_norm_backward(x, x, w, b, 3, st, grads=(dx, two[:12], two[:12])),
+        lambda: rdv.group_norm_backward(x, x, w, b, 3, st, grads=(dx, dx.flatten()[:12], two[:12])),
+        lambda: rdv.cross_attention_backward(q, q, k, k, q, lse, grads=(dq, dk, dk)),
+        lambda: rdv.cross_attention_backward(q, q, k, k, q, lse, grads=(*same, dk)),
+    ):
+        with pytest.raises(AssertionError, match="share memory"):
+            call()
+    rdv.group_norm_backward(x, x, w, b, 3, st, grads=(dx, two[:12], two[12:]))
