@@ -547,9 +547,10 @@ int rdv_broadcast_rows(const float* value, int32_t width, int64_t rows, float* o
 /* ------------------------------------------- image-network operators
  * Build-defined (no counterpart in the reference): what a network over images
  * needs beside its convolutions.  Tensors are fp32, fp16 or bf16 (RDV_DTYPE_*);
- * sums, statistics and softmax terms are fp32 and results are rounded once.
- * Strides are in elements.  Results are the same from call to call (no
- * atomics).  Workspaces are 16-byte aligned device memory that one call uses
+ * sums and statistics are fp32 or fp64 and results are rounded once (16-bit
+ * attention rounds softmax terms and the scores' gradients to its type too, for
+ * the matrix cores).  Strides are in elements.  Results are the same from call
+ * to call (no atomics).  Workspaces are 16-byte aligned device memory that one call uses
  * alone until it has run; their contents need not be kept or cleared.  Results
  * (not rdv_dropout's) are 16-byte aligned, and so is every attention input
  * whose dim and strides are multiples of 16 bytes; others need no alignment. */

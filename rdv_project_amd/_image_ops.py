@@ -365,7 +365,9 @@ def cross_attention_backward(grad, q, k, v, out, lse, key_lengths=None, key_mask
     """(dq, dk, dv) of cross_attention for grad = dL/dout, given the out and lse
     it returned for the same arguments.  dk and dv are summed over the heads
     that share a state head and are 0 at states that do not count; `grads`
-    supplies the three buffers."""
+    supplies the three buffers.  float16 and bfloat16 inputs: the matrix cores
+    take softmax terms and the scores' gradients rounded to that type, and each
+    row's sum of grad * out is of `out` as it was rounded."""
     q, k, v, key_lengths, key_mask, grad, (d, nbytes), device = _attention_inputs(q, k, v, key_lengths, key_mask, scale,
                                                                                   grad)
     out = _like(out, q, "out").contiguous()

@@ -539,7 +539,8 @@ __device__ __forceinline__ void finish_row(const AttnArgs& a, const BlockAt& p, 
 // tiles of KT in LDS (two buffers, one barrier per tile: the next tile's loads are in flight under this tile's products).
 // Bound: a SIMD's vector instructions (the softmax: an fma, an exp2, an addition, half a conversion per score) and matrix
 // instructions add up.  128 dimensions have twice the products of 64 per score:
-//   2 x 16,384 x 4,096, 8 heads of 128, bf16:              530 us, 1.03 PFLOP/s (an 8,192^3 product: 1.18)
+//   2 x 16,384 x 4,096, 8 heads of 128, bf16:              530 us, 1.03 PFLOP/s (an 8,192^3 product: 1.18); twenty such
+//                                                          calls in a row lower the clock: 585 us
 //   4 x 4,096 x 1,024, 8 heads on 4 of 64, fp16:            52 us, 0.66 PFLOP/s
 //   1 x 4,096 x 256, 4 heads of 64, fp32 (a wave per SIMD): 17 us, 63 TFLOP/s (an 8,192^3 product: 153)
 // 16-bit heads of up to 64 dimensions fit 128 registers, four blocks per CU (132: 57 us instead of 52 in the second line).

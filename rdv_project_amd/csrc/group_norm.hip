@@ -262,7 +262,7 @@ __device__ __forceinline__ void group_stats(const NormArgs& a, const NormAt& p, 
   __syncthreads();
   const int items = rows * a.width, step = a.pieces * VE;
   for_groups(p, [&](int g, int l, int lanes, auto join) {
-    const float near = red[g * a.width];  // sums from a mean of the group on: equal values have exactly their mean
+    const float near = red[g * a.width];  // sums from a mean of the group on: equal means have exactly that one
     float s = 0.0f;
 #pragma unroll 1
     for (int k = l; k < items; k += lanes) {
@@ -296,7 +296,7 @@ __device__ __forceinline__ void load_affine(const NormArgs& a, const NormAt& p, 
 }
 
 // act(scale (x - mean) + b) of a piece.  (As one line in x it would be an operation less, but a group of nearly constant
-// values far from zero would become the rounding error of mean scale.)
+// values far from zero would become the rounding error of mean scale.  What is left is the mean's own last place times scale.)
 template <class T, int VE>
 __device__ __forceinline__ void normalise(const NormArgs& a, const Piece<T, VE>& x, const float (&mean)[VE],
                                           const float (&scale)[VE], const float (&b)[VE], T* y) {
