@@ -634,6 +634,120 @@ int rdv_cross_attention_backward(const rdv_attention_desc* desc, const void* gra
 int rdv_dropout(const void* x, const void* residual, void* y, int64_t n, int32_t dtype, double p, uint64_t seed,
                 uint64_t subsequence, void* stream);
 
+/* ------------------------------------------ operators of a prompt's encoder
+ * Build-defined (no counterpart in the reference): what makes the states that
+ * rdv_cross_attention reads, from tokens.  Types, strides, workspaces and
+ * alignment as for the image-network operators; the rows' operators
+ * (rdv_embedding, rdv_rms_norm) need no alignment. */
+
+/* y[i] = scale weight[tokens[i]], a row of zeros where tokens[i] is outside
+ * [0, vocab).  tokens are int32, or int64 with wide_tokens. */
+typedef struct rdv_embedding_desc {
+  int64_t tokens;                          /* 0 .. 2^30                                     */
+  int64_t w_row_stride, g_row_stride;      /* of weight; of grad (backward only)            */
+  int32_t vocab;                           /* 1 .. 2^25                                     */
+  int32_t dim;                             /* 1 .. 2^20                                     */
+  int32_t dtype;                           /* RDV_DTYPE_* of weight, y, grad and dweight    */
+  int32_t wide_tokens;                     /* 0 or 1                                        */
+  float scale;                             /* finite                                        */
+  int32_t reserved;                        /* 0                                             */
+} rdv_embedding_desc;
+
+/* y[tokens, dim], contiguous, apart from weight and tokens. */
+int rdv_embedding(const rdv_embedding_desc* desc, const void* tokens, const void* weight, void* y, void* stream);
+
+/* Bytes of workspace of rdv_embedding_backward; < 0 on error. */
+int64_t rdv_embedding_workspace_bytes(const rdv_embedding_desc* desc);
+
+/* dweight[vocab, dim] (contiguous): row v is scale times the sum of grad's rows
+ * i with tokens[i] = v, in fp32 and in an order that tokens alone gives, rounded
+ * once; zeros for tokens that do not occur. */
+int rdv_embedding_backward(const rdv_embedding_desc* desc, const void* grad, const void* tokens, void* dweight,
+                           void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Root-mean-square normalisation of rows: h = x + residual as it is stored (an
+ * fp32 sum, rounded to dtype; x itself where residual is NULL), and
+ *   y = weight[c] h / sqrt(mean(h^2) + eps). */
+typedef struct rdv_rms_norm_desc {
+  int64_t rows;                            /* 0 .. 2^40 / width                             */
+  int64_t x_row_stride, r_row_stride;      /* of x (backward: of h); of residual            */
+  int64_t g_row_stride, s_row_stride;      /* of grad and grad_sum (backward only)          */
+  int32_t width;                           /* 1 .. 2^20                                     */
+  int32_t dtype;                           /* RDV_DTYPE_* of every tensor but fp32 ones     */
+  float eps;                               /* >= 0                                          */
+  int32_t reserved;                        /* 0                                             */
+} rdv_rms_norm_desc;
+
+/* y[rows, width] and, with residual, sum[rows, width] = h, contiguous; weight is
+ * fp32 [width] or NULL (ones).  sum may be x or residual itself, and y may be x
+ * where there is no residual (contiguous ones).  stats[rows] = 1 / sqrt(mean(h^2)
+ * + eps), where not NULL.  scales not NULL: y is e4m3 bytes and the row's values
+ * are scales[row] times them; scales[row] = max |y| / 448, at least fp32's
+ * smallest normal number (0 for a row of zeros). */
+int rdv_rms_norm(const rdv_rms_norm_desc* desc, const void* x, const void* residual, const float* weight, void* sum,
+                 void* y, float* scales, float* stats, void* stream);
+
+/* Bytes of workspace of rdv_rms_norm_backward; < 0 on error. */
+int64_t rdv_rms_norm_workspace_bytes(const rdv_rms_norm_desc* desc);
+
+/* The gradients of rdv_rms_norm for grad = dL/dy and grad_sum = dL/dh (NULL:
+ * zeros), given h and the stats that it wrote: dx[rows, width] (contiguous), the
+ * gradient of x and of residual alike, and fp32 dweight[width]. */
+int rdv_rms_norm_backward(const rdv_rms_norm_desc* desc, const void* grad, const void* grad_sum, const void* h,
+                          const float* weight, const float* stats, void* dx, float* dweight, void* workspace,
+                          int64_t workspace_bytes, void* stream);
+
+/* Causal attention over packed sequences.  Sequence s is rows token .. token +
+ * tokens - 1 of q[desc.tokens, heads, dim] and rows state .. state + states - 1
+ * of k and v[desc.states, kv_heads, dim]; its i-th token sees its states j <= i +
+ * states - tokens, so that the last one sees all.  Head h reads state head h /
+ * (heads / kv_heads).  Over the states that are seen
+ *   out[i, h] = sum_j softmax_j(scale q . k_j) v_j,
+ *   lse[h, i] = ln sum_j exp(scale q . k_j),
+ * and a token that sees none gets out = 0, lse = -inf.  What k and v hold at
+ * states that a token does not see has no effect on it.  Rows of no sequence are
+ * left as they are, in every result. */
+typedef struct rdv_causal_attention_desc {
+  int64_t tokens, states;                  /* rows of q, out, grad and of k, v; < 2^31 - 1024 */
+  int32_t heads, kv_heads;                 /* kv_heads divides heads                        */
+  int32_t dim;                             /* 1..RDV_ATTENTION_MAX_DIM                      */
+  int32_t dtype;                           /* RDV_DTYPE_* of every tensor but lse           */
+  float scale;
+  int32_t reserved;                        /* 0                                             */
+  int64_t q_stride[2], k_stride[2], v_stride[2];  /* row, head; dim is contiguous           */
+  int64_t g_stride[2];                     /* of grad (backward only)                       */
+} rdv_causal_attention_desc;
+
+/* The list of a call's work, made on the host from the lengths of its sequences
+ * for the current device; every call on sequences of these lengths, with any
+ * strides, scale and buffers of at least this many rows, can use it.  sequences:
+ * [n][4] = (token, tokens, state, states).  No two share a token, and for the
+ * backward call no two share a state.  rdv_causal_attention_plan writes `bytes` =
+ * rdv_causal_attention_plan_bytes(...) bytes (< 0 on error) to host memory; the
+ * calls take them, and a copy of them in device memory (16-byte aligned) that is
+ * complete before they run and stays until they have run. */
+int64_t rdv_causal_attention_plan_bytes(const rdv_causal_attention_desc* desc, const int64_t* sequences, int64_t n,
+                                        int32_t backward);
+int rdv_causal_attention_plan(const rdv_causal_attention_desc* desc, const int64_t* sequences, int64_t n,
+                              int32_t backward, void* plan, int64_t bytes);
+
+/* Bytes of workspace of the forward (backward = 0) or the backward call; < 0 on error. */
+int64_t rdv_causal_attention_workspace_bytes(const rdv_causal_attention_desc* desc, const void* plan, int32_t backward);
+
+/* out[tokens, heads, dim] (contiguous) and, where lse is not NULL, lse[heads, tokens] fp32. */
+int rdv_causal_attention(const rdv_causal_attention_desc* desc, const void* plan, const void* device_plan,
+                         const void* q, const void* k, const void* v, void* out, float* lse, void* workspace,
+                         int64_t workspace_bytes, void* stream);
+
+/* The gradients of rdv_causal_attention for grad = dL/dout, given the out and lse
+ * that it wrote: dq[tokens, heads, dim], dk and dv[states, kv_heads, dim],
+ * contiguous; the gradients of a state head are summed over the heads that read
+ * it, and are 0 at states that no token sees. */
+int rdv_causal_attention_backward(const rdv_causal_attention_desc* desc, const void* plan, const void* device_plan,
+                                  const void* grad, const void* q, const void* k, const void* v, const void* out,
+                                  const float* lse, void* dq, void* dk, void* dv, void* workspace,
+                                  int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

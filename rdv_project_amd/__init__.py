@@ -90,6 +90,15 @@ from ._image_ops import (
     group_norm,
     group_norm_backward,
 )
+from ._prompt_ops import (
+    PackedSequences,
+    causal_attention,
+    causal_attention_backward,
+    embedding,
+    embedding_backward,
+    rms_norm,
+    rms_norm_backward,
+)
 from ._render import composite
 from .grids import (
     Conv2D,

@@ -198,6 +198,54 @@ class AttentionDesc(C.Structure):
     ]
 
 
+class EmbeddingDesc(C.Structure):
+    """Mirror of rdv_embedding_desc."""
+    _fields_ = [
+        ("tokens", C.c_int64),
+        ("w_row_stride", C.c_int64),
+        ("g_row_stride", C.c_int64),
+        ("vocab", C.c_int32),
+        ("dim", C.c_int32),
+        ("dtype", C.c_int32),
+        ("wide_tokens", C.c_int32),
+        ("scale", C.c_float),
+        ("reserved", C.c_int32),
+    ]
+
+
+class RmsNormDesc(C.Structure):
+    """Mirror of rdv_rms_norm_desc."""
+    _fields_ = [
+        ("rows", C.c_int64),
+        ("x_row_stride", C.c_int64),
+        ("r_row_stride", C.c_int64),
+        ("g_row_stride", C.c_int64),
+        ("s_row_stride", C.c_int64),
+        ("width", C.c_int32),
+        ("dtype", C.c_int32),
+        ("eps", C.c_float),
+        ("reserved", C.c_int32),
+    ]
+
+
+class CausalAttentionDesc(C.Structure):
+    """Mirror of rdv_causal_attention_desc."""
+    _fields_ = [
+        ("tokens", C.c_int64),
+        ("states", C.c_int64),
+        ("heads", C.c_int32),
+        ("kv_heads", C.c_int32),
+        ("dim", C.c_int32),
+        ("dtype", C.c_int32),
+        ("scale", C.c_float),
+        ("reserved", C.c_int32),
+        ("q_stride", C.c_int64 * 2),
+        ("k_stride", C.c_int64 * 2),
+        ("v_stride", C.c_int64 * 2),
+        ("g_stride", C.c_int64 * 2),
+    ]
+
+
 class RDVError(RuntimeError):
     """A HIP runtime failure reported by the library."""
 
@@ -276,6 +324,19 @@ _SIGNATURES = {
     "rdv_cross_attention_backward": (C.c_int, [C.POINTER(AttentionDesc), *[C.c_void_p] * 12, C.c_int64, C.c_void_p]),
     "rdv_dropout": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_int32, C.c_double, C.c_uint64,
                               C.c_uint64, C.c_void_p]),
+    "rdv_embedding": (C.c_int, [C.POINTER(EmbeddingDesc), *[C.c_void_p] * 4]),
+    "rdv_embedding_workspace_bytes": (C.c_int64, [C.POINTER(EmbeddingDesc)]),
+    "rdv_embedding_backward": (C.c_int, [C.POINTER(EmbeddingDesc), *[C.c_void_p] * 4, C.c_int64, C.c_void_p]),
+    "rdv_rms_norm": (C.c_int, [C.POINTER(RmsNormDesc), *[C.c_void_p] * 8]),
+    "rdv_rms_norm_workspace_bytes": (C.c_int64, [C.POINTER(RmsNormDesc)]),
+    "rdv_rms_norm_backward": (C.c_int, [C.POINTER(RmsNormDesc), *[C.c_void_p] * 8, C.c_int64, C.c_void_p]),
+    "rdv_causal_attention_plan_bytes": (C.c_int64, [C.POINTER(CausalAttentionDesc), C.c_void_p, C.c_int64, C.c_int32]),
+    "rdv_causal_attention_plan": (C.c_int, [C.POINTER(CausalAttentionDesc), C.c_void_p, C.c_int64, C.c_int32, C.c_void_p,
+                                            C.c_int64]),
+    "rdv_causal_attention_workspace_bytes": (C.c_int64, [C.POINTER(CausalAttentionDesc), C.c_void_p, C.c_int32]),
+    "rdv_causal_attention": (C.c_int, [C.POINTER(CausalAttentionDesc), *[C.c_void_p] * 8, C.c_int64, C.c_void_p]),
+    "rdv_causal_attention_backward": (C.c_int, [C.POINTER(CausalAttentionDesc), *[C.c_void_p] * 12, C.c_int64,
+                                                C.c_void_p]),
 }
 
 _lib = None

@@ -35,6 +35,9 @@ SOURCES = [
     "mlp_generic.hip",
     "train_fused.hip",
     "train.hip",
+    "causal_attention_f32.hip",
+    "causal_attention_f16.hip",
+    "causal_attention_bf16.hip",
     "attention_f32.hip",
     "attention_f16.hip",
     "attention_bf16.hip",
@@ -49,6 +52,9 @@ SOURCES = [
     "group_norm.hip",
     "tensor_data.hip",
     "dropout.hip",
+    "causal_attention.hip",
+    "rms_norm.hip",
+    "embedding.hip",
     "grid_batch.hip",
 ]
 

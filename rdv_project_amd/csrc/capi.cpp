@@ -139,6 +139,29 @@ int launch_attention_backward(const rdv_attention_desc& d, const void* grad, con
                               hipStream_t stream);
 int launch_dropout(const void* x, const void* residual, void* y, int64_t n, int dtype, double p, uint64_t seed,
                    uint64_t subsequence, hipStream_t stream);
+int launch_embedding(const rdv_embedding_desc& d, const void* tokens, const void* weight, void* out, int cu,
+                     hipStream_t stream);
+int64_t embedding_workspace_bytes(const rdv_embedding_desc& d, int cu);
+int launch_embedding_backward(const rdv_embedding_desc& d, const void* grad, const void* tokens, void* dweight,
+                              void* workspace, int cu, hipStream_t stream);
+int64_t rms_norm_workspace_bytes(const rdv_rms_norm_desc& d, int cu);
+int launch_rms_norm(const rdv_rms_norm_desc& d, const void* x, const void* residual, const float* weight, void* sum,
+                    void* y, float* scales, float* stats, int cu, hipStream_t stream);
+int launch_rms_norm_backward(const rdv_rms_norm_desc& d, const void* grad, const void* grad_sum, const void* h,
+                             const float* weight, const float* stats, void* dx, float* dweight, void* workspace,
+                             int cu, hipStream_t stream);
+int64_t causal_attention_plan_bytes(const rdv_causal_attention_desc& d, const int64_t* sequences, int64_t n,
+                                    bool backward, int cu);
+int causal_attention_plan(const rdv_causal_attention_desc& d, const int64_t* sequences, int64_t n, bool backward,
+                          int cu, void* plan, int64_t bytes);
+int64_t causal_attention_workspace_bytes(const rdv_causal_attention_desc& d, const void* plan, bool backward);
+int launch_causal_attention(const rdv_causal_attention_desc& d, const void* plan, const void* device_plan,
+                            const void* q, const void* k, const void* v, void* out, float* lse, void* workspace,
+                            hipStream_t stream);
+int launch_causal_attention_backward(const rdv_causal_attention_desc& d, const void* plan, const void* device_plan,
+                                     const void* grad, const void* q, const void* k, const void* v, const void* out,
+                                     const float* lse, void* dq, void* dk, void* dv, void* workspace,
+                                     hipStream_t stream);
 
 static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
@@ -889,6 +912,183 @@ int rdv_dropout(const void* x, const void* residual, void* y, int64_t n, int32_t
   if (n == 0) return RDV_OK;
   if (!x || !y) return fail(RDV_ERR_INVALID, "rdv_dropout: NULL pointer argument");
   return launch_dropout(x, residual, y, n, dtype, p, seed, subsequence, static_cast<hipStream_t>(stream));
+}
+
+// ------------------------------------------ operators of a prompt's encoder
+static int check_embedding(const rdv_embedding_desc* d, bool backward) {
+  if (!d) return fail(RDV_ERR_INVALID, "embedding: NULL descriptor");
+  if (d->tokens < 0) return fail(RDV_ERR_INVALID, "embedding: tokens must be >= 0");
+  if (d->vocab < 1 || d->dim < 1) return fail(RDV_ERR_INVALID, "embedding: vocab and dim must be >= 1");
+  if (d->tokens > (int64_t(1) << 30) || d->vocab > (1 << 25) || d->dim > (1 << 20))
+    return fail(RDV_ERR_UNSUPPORTED, "embedding: at most 2^30 tokens, 2^25 rows and 2^20 dimensions");
+  if (d->dtype < RDV_DTYPE_F32 || d->dtype > RDV_DTYPE_BF16) return fail(RDV_ERR_INVALID, "embedding: unknown dtype");
+  if (!(d->scale > -3.0e38f && d->scale < 3.0e38f)) return fail(RDV_ERR_INVALID, "embedding: scale must be finite");
+  if (d->wide_tokens != 0 && d->wide_tokens != 1) return fail(RDV_ERR_INVALID, "embedding: wide_tokens must be 0 or 1");
+  if (d->reserved != 0) return fail(RDV_ERR_INVALID, "reserved must be 0");
+  if (!stride_ok(backward ? d->g_row_stride : d->w_row_stride))
+    return fail(RDV_ERR_INVALID, "embedding: strides must be in [0, 2^40)");
+  return RDV_OK;
+}
+
+int rdv_embedding(const rdv_embedding_desc* desc, const void* tokens, const void* weight, void* y, void* stream) {
+  const int rc = check_embedding(desc, false);
+  if (rc != RDV_OK) return rc;
+  if (desc->tokens == 0) return RDV_OK;
+  if (!tokens || !weight || !y) return fail(RDV_ERR_INVALID, "rdv_embedding: NULL pointer argument");
+  return launch_embedding(*desc, tokens, weight, y, plan_cu_count(), static_cast<hipStream_t>(stream));
+}
+
+int64_t rdv_embedding_workspace_bytes(const rdv_embedding_desc* desc) {
+  const int rc = check_embedding(desc, true);
+  return rc != RDV_OK ? rc : embedding_workspace_bytes(*desc, plan_cu_count());
+}
+
+int rdv_embedding_backward(const rdv_embedding_desc* desc, const void* grad, const void* tokens, void* dweight,
+                           void* workspace, int64_t workspace_bytes, void* stream) {
+  const int rc = check_embedding(desc, true);
+  if (rc != RDV_OK) return rc;
+  if (!dweight || (desc->tokens > 0 && (!grad || !tokens)))
+    return fail(RDV_ERR_INVALID, "rdv_embedding_backward: NULL pointer argument");
+  const int cu = plan_cu_count();
+  if (!workspace || workspace_bytes < embedding_workspace_bytes(*desc, cu) || !aligned16(workspace))
+    return fail(RDV_ERR_WORKSPACE, "rdv_embedding_backward: workspace too small or not 16-byte aligned");
+  return launch_embedding_backward(*desc, grad, tokens, dweight, workspace, cu, static_cast<hipStream_t>(stream));
+}
+
+static int check_rms_norm(const rdv_rms_norm_desc* d, bool backward) {
+  if (!d) return fail(RDV_ERR_INVALID, "rms norm: NULL descriptor");
+  if (d->width < 1 || d->width > (1 << 20)) return fail(RDV_ERR_INVALID, "rms norm: width must be in [1, 2^20]");
+  if (d->rows < 0 || d->rows > (int64_t(1) << 40) / d->width) return fail(RDV_ERR_INVALID, "rms norm: too many rows");
+  if (d->dtype < RDV_DTYPE_F32 || d->dtype > RDV_DTYPE_BF16) return fail(RDV_ERR_INVALID, "rms norm: unknown dtype");
+  if (!backward && !(d->eps >= 0.0f)) return fail(RDV_ERR_INVALID, "rms norm: eps must be >= 0");
+  if (d->reserved != 0) return fail(RDV_ERR_INVALID, "reserved must be 0");
+  if (!stride_ok(d->x_row_stride) || !stride_ok(backward ? d->g_row_stride : d->r_row_stride) ||
+      (backward && !stride_ok(d->s_row_stride)))
+    return fail(RDV_ERR_INVALID, "rms norm: strides must be in [0, 2^40)");
+  return RDV_OK;
+}
+
+int rdv_rms_norm(const rdv_rms_norm_desc* desc, const void* x, const void* residual, const float* weight, void* sum,
+                 void* y, float* scales, float* stats, void* stream) {
+  const int rc = check_rms_norm(desc, false);
+  if (rc != RDV_OK) return rc;
+  if (desc->rows == 0) return RDV_OK;
+  if (!x || !y || (residual && !sum)) return fail(RDV_ERR_INVALID, "rdv_rms_norm: NULL pointer argument");
+  return launch_rms_norm(*desc, x, residual, weight, sum, y, scales, stats, plan_cu_count(),
+                         static_cast<hipStream_t>(stream));
+}
+
+int64_t rdv_rms_norm_workspace_bytes(const rdv_rms_norm_desc* desc) {
+  const int rc = check_rms_norm(desc, true);
+  return rc != RDV_OK ? rc : rms_norm_workspace_bytes(*desc, plan_cu_count());
+}
+
+int rdv_rms_norm_backward(const rdv_rms_norm_desc* desc, const void* grad, const void* grad_sum, const void* h,
+                          const float* weight, const float* stats, void* dx, float* dweight, void* workspace,
+                          int64_t workspace_bytes, void* stream) {
+  const int rc = check_rms_norm(desc, true);
+  if (rc != RDV_OK) return rc;
+  if (!dweight || (desc->rows > 0 && (!grad || !h || !stats || !dx)))
+    return fail(RDV_ERR_INVALID, "rdv_rms_norm_backward: NULL pointer argument");
+  const int cu = plan_cu_count();
+  const int64_t need = rms_norm_workspace_bytes(*desc, cu);
+  if (need > 0 && (!workspace || workspace_bytes < need || !aligned16(workspace)))
+    return fail(RDV_ERR_WORKSPACE, "rdv_rms_norm_backward: workspace too small or not 16-byte aligned");
+  return launch_rms_norm_backward(*desc, grad, grad_sum, h, weight, stats, dx, dweight, workspace, cu,
+                                  static_cast<hipStream_t>(stream));
+}
+
+static int check_causal(const rdv_causal_attention_desc* d, bool backward) {
+  if (!d) return fail(RDV_ERR_INVALID, "causal attention: NULL descriptor");
+  const int64_t most = (int64_t(1) << 31) - 1024;
+  if (d->tokens < 0 || d->states < 0 || d->tokens >= most || d->states >= most)
+    return fail(RDV_ERR_INVALID, "causal attention: tokens and states must be in [0, 2^31 - 1024)");
+  if (d->heads < 1 || d->heads > (1 << 16) || d->kv_heads < 1 || d->heads % d->kv_heads != 0)
+    return fail(RDV_ERR_INVALID, "causal attention: heads must be in [1, 65536] and kv_heads must divide it");
+  if (d->dim < 1) return fail(RDV_ERR_INVALID, "causal attention: dim must be >= 1");
+  if (d->dim > RDV_ATTENTION_MAX_DIM)
+    return fail(RDV_ERR_UNSUPPORTED, "causal attention: dim must be at most " + std::to_string(RDV_ATTENTION_MAX_DIM));
+  if (d->dtype < RDV_DTYPE_F32 || d->dtype > RDV_DTYPE_BF16)
+    return fail(RDV_ERR_INVALID, "causal attention: unknown dtype");
+  if (!(d->scale > -3.0e38f && d->scale < 3.0e38f))
+    return fail(RDV_ERR_INVALID, "causal attention: scale must be finite");
+  if (d->reserved != 0) return fail(RDV_ERR_INVALID, "reserved must be 0");
+  for (int i = 0; i < 2; ++i)
+    if (!stride_ok(d->q_stride[i]) || !stride_ok(d->k_stride[i]) || !stride_ok(d->v_stride[i]) ||
+        (backward && !stride_ok(d->g_stride[i])))
+      return fail(RDV_ERR_INVALID, "causal attention: strides must be in [0, 2^40)");
+  return RDV_OK;
+}
+
+int64_t rdv_causal_attention_plan_bytes(const rdv_causal_attention_desc* desc, const int64_t* sequences, int64_t n,
+                                        int32_t backward) {
+  const int rc = check_causal(desc, backward != 0);
+  if (rc != RDV_OK) return rc;
+  try {
+    return causal_attention_plan_bytes(*desc, sequences, n, backward != 0, plan_cu_count());
+  } catch (const std::exception& e) {
+    return fail(RDV_ERR_INVALID, std::string("causal attention: ") + e.what());
+  }
+}
+
+int rdv_causal_attention_plan(const rdv_causal_attention_desc* desc, const int64_t* sequences, int64_t n,
+                              int32_t backward, void* plan, int64_t bytes) {
+  const int rc = check_causal(desc, backward != 0);
+  if (rc != RDV_OK) return rc;
+  if (!plan) return fail(RDV_ERR_INVALID, "rdv_causal_attention_plan: NULL pointer argument");
+  try {
+    return causal_attention_plan(*desc, sequences, n, backward != 0, plan_cu_count(), plan, bytes);
+  } catch (const std::exception& e) {
+    return fail(RDV_ERR_INVALID, std::string("causal attention: ") + e.what());
+  }
+}
+
+int64_t rdv_causal_attention_workspace_bytes(const rdv_causal_attention_desc* desc, const void* plan,
+                                             int32_t backward) {
+  const int rc = check_causal(desc, backward != 0);
+  if (rc != RDV_OK) return rc;
+  if (!plan) return fail(RDV_ERR_INVALID, "rdv_causal_attention_workspace_bytes: NULL pointer argument");
+  return causal_attention_workspace_bytes(*desc, plan, backward != 0);
+}
+
+static int check_causal_call(const rdv_causal_attention_desc* desc, const void* plan, const void* device_plan,
+                             const void* workspace, int64_t workspace_bytes, bool backward) {
+  if (!plan || !device_plan) return fail(RDV_ERR_INVALID, "causal attention: NULL plan");
+  if (!aligned16(device_plan)) return fail(RDV_ERR_INVALID, "causal attention: the plan must be 16-byte aligned");
+  const int64_t need = causal_attention_workspace_bytes(*desc, plan, backward);
+  if (need < 0) return int(need);
+  if (need > 0 && (!workspace || workspace_bytes < need || !aligned16(workspace)))
+    return fail(RDV_ERR_WORKSPACE, "causal attention: workspace too small or not 16-byte aligned");
+  return RDV_OK;
+}
+
+int rdv_causal_attention(const rdv_causal_attention_desc* desc, const void* plan, const void* device_plan,
+                         const void* q, const void* k, const void* v, void* out, float* lse, void* workspace,
+                         int64_t workspace_bytes, void* stream) {
+  int rc = check_causal(desc, false);
+  if (rc == RDV_OK) rc = check_causal_call(desc, plan, device_plan, workspace, workspace_bytes, false);
+  if (rc != RDV_OK) return rc;
+  if (desc->tokens == 0) return RDV_OK;
+  if (!q || !out || (desc->states > 0 && (!k || !v)))
+    return fail(RDV_ERR_INVALID, "rdv_causal_attention: NULL pointer argument");
+  if (!aligned16(out)) return fail(RDV_ERR_INVALID, "rdv_causal_attention: out must be 16-byte aligned");
+  return launch_causal_attention(*desc, plan, device_plan, q, k, v, out, lse, workspace,
+                                 static_cast<hipStream_t>(stream));
+}
+
+int rdv_causal_attention_backward(const rdv_causal_attention_desc* desc, const void* plan, const void* device_plan,
+                                  const void* grad, const void* q, const void* k, const void* v, const void* out,
+                                  const float* lse, void* dq, void* dk, void* dv, void* workspace,
+                                  int64_t workspace_bytes, void* stream) {
+  int rc = check_causal(desc, true);
+  if (rc == RDV_OK) rc = check_causal_call(desc, plan, device_plan, workspace, workspace_bytes, true);
+  if (rc != RDV_OK) return rc;
+  if ((desc->tokens > 0 && (!grad || !q || !out || !lse || !dq)) || (desc->states > 0 && (!k || !v || !dk || !dv)))
+    return fail(RDV_ERR_INVALID, "rdv_causal_attention_backward: NULL pointer argument");
+  if (!aligned16(dq) || !aligned16(dk) || !aligned16(dv))
+    return fail(RDV_ERR_INVALID, "rdv_causal_attention_backward: dq, dk and dv must be 16-byte aligned");
+  return launch_causal_attention_backward(*desc, plan, device_plan, grad, q, k, v, out, lse, dq, dk, dv, workspace,
+                                          static_cast<hipStream_t>(stream));
 }
 
 const char* rdv_mlp_kernel_name(const rdv_mlp_desc* desc) {
