@@ -17,8 +17,8 @@ import math
 import torch
 
 from . import _lib
-from ._image_ops import (_DTYPES, _apart, _check, _data, _gpu_index, _grad_tensors, _image_rows, _like, _on_gpu,
-                         _out_tensor, _ptr, _rows_in_place, _stream, _tensor)
+from ._image_ops import (_DTYPES, _apart, _check, _data, _gpu_index, _grad_tensors, _image_rows, _like, _like_out,
+                         _on_gpu, _out_tensor, _ptr, _rows_in_place, _stream, _tensor)
 from .core import launch_scope
 
 
@@ -58,30 +58,31 @@ def _tokens(tokens) -> torch.Tensor:
 
 @functools.lru_cache(maxsize=4096)
 def _embedding_plan(n, wide, vocab, dim, dtype, scale, w_stride, g_stride, device):
-    """(descriptor, workspace bytes) of a call; g_stride is None for the forward call."""
+    """What a call of this kind needs, by layout alone: (reference to the descriptor, workspace bytes); g_stride is None
+    for the forward call, `device` the GPU it is planned for."""
     if not math.isfinite(scale):
         raise ValueError(f"scale must be finite, got {scale}")
     d = _lib.EmbeddingDesc()
     d.tokens, d.vocab, d.dim, d.dtype, d.wide_tokens, d.scale = n, vocab, dim, _DTYPES[dtype], wide, scale
     d.w_row_stride, d.g_row_stride = w_stride or 0, g_stride or 0
     nbytes = 0 if g_stride is None else _bytes(_lib.load().rdv_embedding_workspace_bytes(C.byref(d)), "embedding")
-    return d, nbytes
+    return C.byref(d), nbytes
 
 
 def _embedding_into(tokens, weight, scale: float, y, device: int) -> None:
     """Launches rdv_embedding into y."""
     tokens = tokens.contiguous()
-    if weight.stride(1) != 1 and weight.shape[1] != 1:
+    vocab, dim = weight.shape
+    if weight.stride(1) != 1 and dim != 1:
         weight = weight.contiguous()
-    d, _ = _embedding_plan(tokens.numel(), tokens.dtype == torch.int64, weight.shape[0], weight.shape[1], weight.dtype,
-                           scale, weight.stride(0), None, device)
-    _check(_lib.load().rdv_embedding(C.byref(d), tokens.data_ptr(), weight.data_ptr(), y.data_ptr(), _stream(device)),
-           "embedding")
+    d, _ = _embedding_plan(tokens.numel(), tokens.dtype == torch.int64, vocab, dim, weight.dtype, scale,
+                           weight.stride(0), None, device)
+    _check(_lib.load().rdv_embedding(d, tokens.data_ptr(), weight.data_ptr(), y.data_ptr(), _stream(device)), "embedding")
 
 
 def _embedding_inputs(tokens, weight):
     tokens, weight = _tokens(tokens), _data(weight, "weight")
-    assert weight.dim() == 2 and weight.shape[0] >= 1 and weight.shape[1] >= 1, "weight must be [vocab, dim]"
+    assert weight.dim() == 2 and min(weight.shape) >= 1, "weight must be [vocab, dim]"
     return tokens, weight
 
 
@@ -92,8 +93,10 @@ def embedding(tokens, weight, scale: float = 1.0, out=None):
     tokens, weight = _embedding_inputs(tokens, weight)
     device = _gpu_index()
     _on_gpu(device, tokens, "tokens", weight, "weight")
-    y = _out_tensor(out, (*tokens.shape, weight.shape[1]), weight.dtype, weight.device, aligned=False)
-    if out is not None:
+    if out is None:
+        y = weight.new_empty((*tokens.shape, weight.shape[1]))
+    else:
+        y = _out_tensor(out, (*tokens.shape, weight.shape[1]), weight.dtype, weight.device, aligned=False)
         _apart(y, (tokens, "tokens"), (weight, "weight"))
     with launch_scope():
         _embedding_into(tokens, weight, float(scale), y, device)
@@ -110,21 +113,23 @@ def embedding_backward(grad, tokens, vocab: int, scale: float = 1.0, out=None):
     assert grad.dim() == tokens.dim() + 1 and grad.shape[:-1] == tokens.shape and grad.shape[-1] >= 1, \
         f"grad must be [{', '.join(map(str, tokens.shape))}, dim], got {list(grad.shape)}"
     vocab, dim = int(vocab), grad.shape[-1]
-    stride = _row_stride(grad.shape, grad.stride())
+    stride = dim if grad.is_contiguous() else _row_stride(grad.shape, grad.stride())
     device = _gpu_index()
     d, nbytes = _embedding_plan(tokens.numel(), tokens.dtype == torch.int64, vocab, dim, grad.dtype, float(scale), None,
                                 dim if stride is None else stride, device)
     _on_gpu(device, grad, "grad", tokens, "tokens")
-    dw = _out_tensor(out, (vocab, dim), grad.dtype, grad.device, aligned=False)
-    if out is not None:
+    if out is None:
+        dw = grad.new_empty((vocab, dim))
+    else:
+        dw = _out_tensor(out, (vocab, dim), grad.dtype, grad.device, aligned=False)
         _apart(dw, (grad, "grad"), (tokens, "tokens"))
     with launch_scope():
         if stride is None:
             grad = grad.contiguous()
         tokens = tokens.contiguous()
         ws = _workspace(nbytes, grad)
-        _check(_lib.load().rdv_embedding_backward(C.byref(d), grad.data_ptr(), tokens.data_ptr(), dw.data_ptr(),
-                                                  _ptr(ws), nbytes, _stream(device)), "embedding_backward")
+        _check(_lib.load().rdv_embedding_backward(d, grad.data_ptr(), tokens.data_ptr(), dw.data_ptr(), _ptr(ws),
+                                                  nbytes, _stream(device)), "embedding_backward")
     return dw
 
 
@@ -133,18 +138,21 @@ def embedding_backward(grad, tokens, vocab: int, scale: float = 1.0, out=None):
 
 @functools.lru_cache(maxsize=4096)
 def _rms_plan(shape, dtype, eps, strides, backward, device):
-    """(descriptor, workspace bytes) of a call on rows [..., width]; strides: of x and residual, or of h, grad and
-    grad_sum."""
+    """What a call on rows [..., width] of these layouts needs, by layout alone: (reference to the descriptor, whether each
+    tensor has to be copied first, workspace bytes).  strides: of x and residual, or of h, grad and grad_sum (None where
+    there is none); `device`: the GPU it is planned for."""
     width = shape[-1]
     assert width >= 1, "x must be [..., width]"
     d = _lib.RmsNormDesc()
     d.rows, d.width, d.dtype, d.eps = math.prod(shape[:-1]), width, _DTYPES[dtype], eps
-    d.x_row_stride = strides[0]
-    if backward:
-        d.g_row_stride, d.s_row_stride = strides[1:]
-        return d, _bytes(_lib.load().rdv_rms_norm_workspace_bytes(C.byref(d)), "rms_norm")
-    d.r_row_stride = strides[1]
-    return d, 0
+    at = [0 if s is None else _row_stride(shape, s) for s in strides]
+    copies = [a is None for a in at]
+    at = [width if a is None else a for a in at]
+    if not backward:
+        d.x_row_stride, d.r_row_stride = at
+        return C.byref(d), copies, 0
+    d.x_row_stride, d.g_row_stride, d.s_row_stride = at
+    return C.byref(d), copies, _bytes(_lib.load().rdv_rms_norm_workspace_bytes(C.byref(d)), "rms_norm")
 
 
 def _rms_param(p, x):
@@ -163,20 +171,16 @@ def _rms_inputs(x, weight):
     return x, _rms_param(weight, x)
 
 
-def _packed_rows(t):
-    """(t, or a contiguous copy where its rows do not lie at one distance; that distance)."""
-    if t is None:
-        return None, 0
-    stride = _row_stride(t.shape, t.stride())
-    return (t.contiguous(), t.shape[-1]) if stride is None else (t, stride)
-
-
 def _rms_norm_into(x, weight, residual, eps: float, y, h, scales, stats, device: int) -> None:
     """Launches rdv_rms_norm into y, and into h, scales and stats (or None)."""
-    (x, sx), (residual, sr) = _packed_rows(x), _packed_rows(residual)
-    d, _ = _rms_plan(x.shape, x.dtype, eps, (sx, sr), False, device)
-    _check(_lib.load().rdv_rms_norm(C.byref(d), x.data_ptr(), _ptr(residual), _ptr(weight), _ptr(h), y.data_ptr(),
-                                    _ptr(scales), _ptr(stats), _stream(device)), "rms_norm")
+    d, copies, _ = _rms_plan(x.shape, x.dtype, eps, (x.stride(), None if residual is None else residual.stride()), False,
+                             device)
+    if copies[0]:
+        x = x.contiguous()
+    if copies[1]:
+        residual = residual.contiguous()
+    _check(_lib.load().rdv_rms_norm(d, x.data_ptr(), _ptr(residual), _ptr(weight), _ptr(h), y.data_ptr(), _ptr(scales),
+                                    _ptr(stats), _stream(device)), "rms_norm")
 
 
 def rms_norm(x, weight, residual=None, eps: float = 1e-6, out=None, sum_out=None, return_stats: bool = False,
@@ -215,14 +219,16 @@ def rms_norm(x, weight, residual=None, eps: float = 1e-6, out=None, sum_out=None
             _apart(y, *inputs, (weight, "weight"))
             _apart(scales, *inputs, (weight, "weight"), (y, "values"))
     else:
-        y = _out_tensor(out, x.shape, x.dtype, dev, aligned=False)
+        y = _like_out(out, x, aligned=False)
         if out is not None:
             (_same_or_apart if residual is None else _apart)(y, inputs[0])
             _apart(y, inputs[1], (weight, "weight"))
     h = None
     if residual is not None:
-        h = _out_tensor(sum_out, x.shape, x.dtype, dev, "sum_out", aligned=False)
-        if sum_out is not None:
+        if sum_out is None:
+            h = _like_out(None, x)
+        else:
+            h = _out_tensor(sum_out, x.shape, x.dtype, dev, "sum_out", aligned=False)
             _same_or_apart(h, *inputs)
             _apart(h, (weight, "weight"), (y, "out"), (scales, "scales"))
     stats = torch.empty(rows, dtype=torch.float32, device=dev) if return_stats else None
@@ -250,7 +256,7 @@ def rms_norm_backward(grad, h, weight, stats, grad_sum=None, grads=None):
     device = _gpu_index()
     _on_gpu(device, h, "h", grad, "grad", weight, "weight", stats, "stats", grad_sum, "grad_sum")
     if grads is None:
-        dx = torch.empty(h.shape, dtype=h.dtype, device=h.device)
+        dx = _like_out(None, h)
         dw = torch.empty(h.shape[-1], dtype=torch.float32, device=h.device)
     else:
         if not isinstance(grads, (list, tuple)) or len(grads) != 2:
@@ -261,10 +267,12 @@ def rms_norm_backward(grad, h, weight, stats, grad_sum=None, grads=None):
             _apart(t, (grad, "grad"), (h, "h"), (weight, "weight"), (stats, "stats"), (grad_sum, "grad_sum"))
         _apart(dw, (dx, "dx"))
     with launch_scope():
-        (h, sh), (grad, sg), (grad_sum, ss) = _packed_rows(h), _packed_rows(grad), _packed_rows(grad_sum)
-        d, nbytes = _rms_plan(h.shape, h.dtype, 0.0, (sh, sg, ss), True, device)
+        d, copies, nbytes = _rms_plan(h.shape, h.dtype, 0.0, (h.stride(), grad.stride(),
+                                                              None if grad_sum is None else grad_sum.stride()), True, device)
+        if any(copies):
+            h, grad, grad_sum = (t.contiguous() if c else t for t, c in zip((h, grad, grad_sum), copies))
         ws = _workspace(nbytes, h)
-        _check(_lib.load().rdv_rms_norm_backward(C.byref(d), grad.data_ptr(), _ptr(grad_sum), h.data_ptr(), _ptr(weight),
+        _check(_lib.load().rdv_rms_norm_backward(d, grad.data_ptr(), _ptr(grad_sum), h.data_ptr(), _ptr(weight),
                                                  stats.data_ptr(), dx.data_ptr(), dw.data_ptr(), _ptr(ws), nbytes,
                                                  _stream(device)), "rms_norm_backward")
     return dx, dw
@@ -309,27 +317,43 @@ class PackedSequences:
         self.dense = sum(b - a for a, b in spans) == self.total_states if self.apart else False
         self._rows = (C.c_int64 * max(1, 4 * len(rows)))(*[x for r in rows for x in r])
         self._plans: dict = {}
+        self._calls: dict = {}
 
     def __len__(self) -> int:
         return len(self.lengths)
 
-    def _plan(self, heads: int, kv_heads: int, dim: int, dtype: int, backward: bool, device: int):
+    def _plan(self, d, backward: bool, device: int):
         """(the list of work in host memory, the same on the GPU) for calls of this kind."""
-        key = heads, kv_heads, dim, dtype, backward, device
+        key = d.heads, d.kv_heads, d.dim, d.dtype, backward, device
         hit = self._plans.get(key)
         if hit is not None:
             return hit
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("the first call of a kind on PackedSequences cannot be captured: make it once before")
-        d = _lib.CausalAttentionDesc()
-        d.tokens, d.states = self.tokens, self.total_states
-        d.heads, d.kv_heads, d.dim, d.dtype, d.scale = heads, kv_heads, dim, dtype, 1.0
         lib, n = _lib.load(), len(self.lengths)
         nbytes = _bytes(lib.rdv_causal_attention_plan_bytes(C.byref(d), self._rows, n, backward), "causal_attention")
         host = torch.empty(nbytes, dtype=torch.uint8)
         _check(lib.rdv_causal_attention_plan(C.byref(d), self._rows, n, backward, host.data_ptr(), nbytes),
                "causal_attention")
         hit = self._plans[key] = host, host.to(f"cuda:{device}")  # a synchronous copy: any stream may read it
+        return hit
+
+    def _call(self, layout, device: int):
+        """What a call on tensors of this layout (_causal_desc's arguments) needs: (descriptor, reference to it, list of
+        work in host memory, on the GPU, workspace bytes)."""
+        hit = self._calls.get((layout, device))
+        if hit is not None:
+            return hit
+        d = _causal_desc(*layout)
+        assert self.tokens <= d.tokens, f"the sequences have {self.tokens} tokens, q {d.tokens} rows"
+        assert self.total_states <= d.states, f"the sequences have {self.total_states} states, k and v {d.states} rows"
+        backward = layout[6] is not None
+        host, lists = self._plan(d, backward, device)
+        nbytes = _bytes(_lib.load().rdv_causal_attention_workspace_bytes(C.byref(d), host.data_ptr(), backward),
+                        "causal_attention")
+        if len(self._calls) >= 256:  # of changing strides or scales: their plans stay
+            self._calls.clear()
+        hit = self._calls[layout, device] = d, C.byref(d), host, lists, nbytes
         return hit
 
 
@@ -344,7 +368,6 @@ def _counts(values, what: str) -> tuple:
     return counts
 
 
-@functools.lru_cache(maxsize=4096)
 def _causal_desc(q_shape, k_shape, v_shape, q_stride, k_stride, v_stride, g_stride, dtype, scale):
     """The descriptor of a call on tensors of this layout; g_stride is None for the forward call."""
     assert len(q_shape) == 3, "q must be [tokens, heads, dim]"
@@ -369,7 +392,7 @@ def _causal_desc(q_shape, k_shape, v_shape, q_stride, k_stride, v_stride, g_stri
 
 
 def _causal_inputs(q, k, v, sequences, scale, grad=None):
-    """The checked inputs as the library reads them, the descriptor, the plan and the workspace's size."""
+    """The checked inputs as the library reads them, and what the call needs (PackedSequences._call)."""
     q, k, v = _data(q, "q"), _data(k, "k"), _data(v, "v")
     if k.dtype != q.dtype or v.dtype != q.dtype:
         raise TypeError(f"q, k and v must have one type, got {q.dtype}, {k.dtype} and {v.dtype}")
@@ -379,26 +402,22 @@ def _causal_inputs(q, k, v, sequences, scale, grad=None):
         q, k, v = _rows_in_place(q), _rows_in_place(k), _rows_in_place(v)
     if grad is not None:
         grad = _rows_in_place(_like(grad, q, "grad"))
-    d = _causal_desc(q.shape, k.shape, v.shape, q.stride(), k.stride(), v.stride(),
-                     None if grad is None else grad.stride(), q.dtype, None if scale is None else float(scale))
-    assert sequences.tokens <= d.tokens, f"the sequences have {sequences.tokens} tokens, q {d.tokens} rows"
-    assert sequences.total_states <= d.states, \
-        f"the sequences have {sequences.total_states} states, k and v {d.states} rows"
+    layout = (q.shape, k.shape, v.shape, q.stride(), k.stride(), v.stride(), None if grad is None else grad.stride(),
+              q.dtype, None if scale is None else float(scale))
     device = _gpu_index()
+    if not q.is_cuda:
+        _causal_desc(*layout)  # what is wrong with the call comes before where it is made
     _on_gpu(device, q, "q", k, "k", v, "v", grad, "grad")
-    host, plan = sequences._plan(d.heads, d.kv_heads, d.dim, d.dtype, grad is not None, device)
-    nbytes = _bytes(_lib.load().rdv_causal_attention_workspace_bytes(C.byref(d), host.data_ptr(), grad is not None),
-                    "causal_attention")
-    return q, k, v, grad, d, (host, plan, nbytes), device
+    return q, k, v, grad, sequences._call(layout, device), device
 
 
-def _causal_attention_into(d, plan, q, k, v, out, lse, device: int) -> None:
+def _causal_attention_into(call, q, k, v, out, lse, device: int) -> None:
     """Launches rdv_causal_attention into out and lse (or None)."""
-    host, lists, nbytes = plan
+    _, d, host, lists, nbytes = call
     ws = _workspace(nbytes, q)
-    _check(_lib.load().rdv_causal_attention(C.byref(d), host.data_ptr(), lists.data_ptr(), q.data_ptr(), k.data_ptr(),
-                                            v.data_ptr(), out.data_ptr(), _ptr(lse), _ptr(ws), nbytes,
-                                            _stream(device)), "causal_attention")
+    _check(_lib.load().rdv_causal_attention(d, host.data_ptr(), lists.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(),
+                                            out.data_ptr(), _ptr(lse), _ptr(ws), nbytes, _stream(device)),
+           "causal_attention")
 
 
 def causal_attention(q, k, v, sequences: PackedSequences, scale: float | None = None, out=None,
@@ -417,8 +436,9 @@ def causal_attention(q, k, v, sequences: PackedSequences, scale: float | None = 
     bfloat16 inputs: the matrix cores take softmax terms rounded to that type;
     float32: float32 throughout."""
     given = q, k, v
-    q, k, v, _, d, plan, device = _causal_inputs(q, k, v, sequences, scale)
-    y = _out_tensor(out, q.shape, q.dtype, q.device)
+    q, k, v, _, call, device = _causal_inputs(q, k, v, sequences, scale)
+    d = call[0]
+    y = _like_out(out, q)
     if out is not None:
         _apart(y, *zip((_tensor(t, n) for t, n in zip(given, "qkv")), "qkv"))
     elif sequences.tokens < d.tokens:
@@ -429,7 +449,7 @@ def causal_attention(q, k, v, sequences: PackedSequences, scale: float | None = 
         if sequences.tokens < d.tokens:
             lse[:, sequences.tokens:].fill_(-math.inf)
     with launch_scope():
-        _causal_attention_into(d, plan, q, k, v, y, lse, device)
+        _causal_attention_into(call, q, k, v, y, lse, device)
     return (y, lse) if return_lse else y
 
 
@@ -444,7 +464,8 @@ def causal_attention_backward(grad, q, k, v, out, lse, sequences: PackedSequence
     type, and each row's sum of grad * out is of `out` as it was rounded."""
     if isinstance(sequences, PackedSequences) and not sequences.apart:
         raise NotImplementedError("gradients of sequences that share states")
-    q, k, v, grad, d, (host, lists, nbytes), device = _causal_inputs(q, k, v, sequences, scale, _tensor(grad, "grad"))
+    q, k, v, grad, call, device = _causal_inputs(q, k, v, sequences, scale, _tensor(grad, "grad"))
+    d, desc, host, lists, nbytes = call
     out = _like(out, q, "out").contiguous()
     lse = _tensor(lse, "lse")
     assert tuple(lse.shape) == (d.heads, d.tokens) and lse.is_contiguous(), \
@@ -467,7 +488,7 @@ def causal_attention_backward(grad, q, k, v, out, lse, sequences: PackedSequence
     with launch_scope():
         out = out if out.data_ptr() % 16 == 0 else out.clone()
         ws = _workspace(nbytes, q)
-        _check(_lib.load().rdv_causal_attention_backward(C.byref(d), host.data_ptr(), lists.data_ptr(), grad.data_ptr(),
+        _check(_lib.load().rdv_causal_attention_backward(desc, host.data_ptr(), lists.data_ptr(), grad.data_ptr(),
                                                          q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
                                                          lse.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
                                                          _ptr(ws), nbytes, _stream(device)),

@@ -141,9 +141,9 @@ int launch_dropout(const void* x, const void* residual, void* y, int64_t n, int 
                    uint64_t subsequence, hipStream_t stream);
 int launch_embedding(const rdv_embedding_desc& d, const void* tokens, const void* weight, void* out, int cu,
                      hipStream_t stream);
-int64_t embedding_workspace_bytes(const rdv_embedding_desc& d, int cu);
+int64_t embedding_workspace_bytes(const rdv_embedding_desc& d);
 int launch_embedding_backward(const rdv_embedding_desc& d, const void* grad, const void* tokens, void* dweight,
-                              void* workspace, int cu, hipStream_t stream);
+                              void* workspace, hipStream_t stream);
 int64_t rms_norm_workspace_bytes(const rdv_rms_norm_desc& d, int cu);
 int launch_rms_norm(const rdv_rms_norm_desc& d, const void* x, const void* residual, const float* weight, void* sum,
                     void* y, float* scales, float* stats, int cu, hipStream_t stream);
@@ -921,6 +921,9 @@ static int check_embedding(const rdv_embedding_desc* d, bool backward) {
   if (d->vocab < 1 || d->dim < 1) return fail(RDV_ERR_INVALID, "embedding: vocab and dim must be >= 1");
   if (d->tokens > (int64_t(1) << 30) || d->vocab > (1 << 25) || d->dim > (1 << 20))
     return fail(RDV_ERR_UNSUPPORTED, "embedding: at most 2^30 tokens, 2^25 rows and 2^20 dimensions");
+  // threads of a launch are counted in 32 bits: one for every 8 bytes of dweight, and of a 64th of grad
+  if (backward && (int64_t(d->vocab) + d->tokens / 64 + 1) * (d->dim + 255) > (int64_t(1) << 33))
+    return fail(RDV_ERR_UNSUPPORTED, "embedding: too large a gradient");
   if (d->dtype < RDV_DTYPE_F32 || d->dtype > RDV_DTYPE_BF16) return fail(RDV_ERR_INVALID, "embedding: unknown dtype");
   if (!(d->scale > -3.0e38f && d->scale < 3.0e38f)) return fail(RDV_ERR_INVALID, "embedding: scale must be finite");
   if (d->wide_tokens != 0 && d->wide_tokens != 1) return fail(RDV_ERR_INVALID, "embedding: wide_tokens must be 0 or 1");
@@ -940,7 +943,7 @@ int rdv_embedding(const rdv_embedding_desc* desc, const void* tokens, const void
 
 int64_t rdv_embedding_workspace_bytes(const rdv_embedding_desc* desc) {
   const int rc = check_embedding(desc, true);
-  return rc != RDV_OK ? rc : embedding_workspace_bytes(*desc, plan_cu_count());
+  return rc != RDV_OK ? rc : embedding_workspace_bytes(*desc);
 }
 
 int rdv_embedding_backward(const rdv_embedding_desc* desc, const void* grad, const void* tokens, void* dweight,
@@ -949,10 +952,9 @@ int rdv_embedding_backward(const rdv_embedding_desc* desc, const void* grad, con
   if (rc != RDV_OK) return rc;
   if (!dweight || (desc->tokens > 0 && (!grad || !tokens)))
     return fail(RDV_ERR_INVALID, "rdv_embedding_backward: NULL pointer argument");
-  const int cu = plan_cu_count();
-  if (!workspace || workspace_bytes < embedding_workspace_bytes(*desc, cu) || !aligned16(workspace))
+  if (!workspace || workspace_bytes < embedding_workspace_bytes(*desc) || !aligned16(workspace))
     return fail(RDV_ERR_WORKSPACE, "rdv_embedding_backward: workspace too small or not 16-byte aligned");
-  return launch_embedding_backward(*desc, grad, tokens, dweight, workspace, cu, static_cast<hipStream_t>(stream));
+  return launch_embedding_backward(*desc, grad, tokens, dweight, workspace, static_cast<hipStream_t>(stream));
 }
 
 static int check_rms_norm(const rdv_rms_norm_desc* d, bool backward) {

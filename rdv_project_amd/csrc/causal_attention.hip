@@ -25,6 +25,7 @@ struct Header {
   int32_t row_slots, key_slots;    // parts
   int32_t pairs, key_pairs;        // pairs of waves share 32 rows, 32 states
   int32_t tile_rows, key_tile;     // rows and states of a block
+  int32_t join_rows, join_parts;   // the most rows, and parts, of a join
   int64_t at_few, at_rows, at_keys, at_row_joins, at_key_joins;  // byte offsets
 };
 constexpr uint64_t kMagic = 0x52445643415553ull;
@@ -86,11 +87,16 @@ Lists make_lists(const rdv_causal_attention_desc& d, const std::vector<Sequence>
   for (const Sequence& s : seqs) blocks += (s.tokens * share + 127) / 128 * d.kv_heads;
   h.pairs = tile == 64 && blocks < cu;
   h.tile_rows = h.pairs ? 64 : 128;
+  // Sequences of at most 32 rows have a kernel of their own, which streams their states.  Where all of those are few they
+  // join the others, whose launch does not last longer for them.
+  int64_t few_states = 0;
+  for (const Sequence& s : seqs)
+    if (s.tokens * share > 32) few_states = 1024;
   std::vector<CausalItem> items;
   int64_t few_total = 0, total = 0;
   for (const Sequence& s : seqs) {
     const int rows = int(s.tokens * share), shift = int(s.states - s.tokens);
-    const bool few = !backward && rows <= 32;
+    const bool few = !backward && rows <= 32 && s.states >= few_states;
     for (int first = 0; first < rows; first += h.tile_rows) {
       const int last = std::min(first + h.tile_rows, rows) - 1, end = std::max(0, last / share + shift + 1);
       CausalItem item{int32_t(s.token), int32_t(s.tokens), int32_t(s.state), int32_t(s.states), first, 0, end, -1};
@@ -106,7 +112,10 @@ Lists make_lists(const rdv_causal_attention_desc& d, const std::vector<Sequence>
     for (const CausalItem& i : whole) put(l.few, l.row_joins, h.row_slots, i, most);
   }
   {
-    const int most = part_size(total, 2 * int64_t(cu), wide ? 64 : 256, 64);
+    // Half as many parts as blocks run at once: more cost more in partial results than they even out (2,048 tokens, 8 heads on
+    // 2 of 128 in bf16, two blocks per CU: 30.1 us, with as many parts 33.7; 8 sequences up to 4,096, 8 heads on 4 of 64 in
+    // fp16, four blocks: 90.7 us, with a quarter 95.5 and with as many 98.1).  At least 256 states, in fp32 64.
+    const int most = part_size(total, int64_t(cu) * (d.dim * element_bytes(d.dtype) > 128 ? 1 : 2), wide ? 64 : 256, 64);
     for (const CausalItem& i : items) put(l.rows, l.row_joins, h.row_slots, i, std::max(most, 64));
   }
   if (items.empty()) h.tile_rows = 32;
@@ -130,9 +139,15 @@ Lists make_lists(const rdv_causal_attention_desc& d, const std::vector<Sequence>
         total += int64_t(n) * share * d.kv_heads;
       }
     }
-    const int most = part_size(total, 2 * int64_t(cu), wide ? 1 : 2, 1);
+    // As many parts as blocks run at once (the 8 sequences above: 263 us both backward kernels, with half as many 310, with
+    // twice 270; 2 x 1,024 tokens, 4 heads on 2 of 64 in fp32: 71.7, with twice as many 81).
+    const int most = part_size(total, int64_t(cu) * (wide || d.dim > 96 ? 1 : 2), wide ? 1 : 2, 1);
     for (const CausalItem& i : items) put(l.keys, l.key_joins, h.key_slots, i, most);
     sort_items(l.keys);
+  }
+  for (const CausalJoin& j : l.row_joins) {
+    h.join_rows = std::max(h.join_rows, std::min(h.tile_rows, j.tokens * share - j.tile));
+    h.join_parts = std::max(h.join_parts, j.count);
   }
   h.few = int32_t(l.few.size());
   h.rows = int32_t(l.rows.size());
@@ -236,7 +251,7 @@ __global__ __launch_bounds__(256) void causal_pack_kernel(const T* x, T* y, int6
 }
 
 // Joins the parts of a tile's rows with weights 2^(top_i - top): 32 lanes hold a row's dimensions, 4 each; `per` such
-// groups of a block (1, 2, 4 or 8) share a row's parts.  Blocks: (tile, state head, 8 / per rows).
+// groups of a block (1, 2, 4 or 8) share a row's parts.  Blocks: (8 / per rows, tile, state head).
 template <class T>
 __global__ __launch_bounds__(256) void causal_join_kernel(CausalArgs a, int per) {
   __shared__ __attribute__((aligned(16))) float sums[8][RDV_ATTENTION_MAX_DIM];
@@ -245,24 +260,25 @@ __global__ __launch_bounds__(256) void causal_join_kernel(CausalArgs a, int per)
   const int hk = int(blockIdx.z), l = int(threadIdx.x) & 31, g = int(threadIdx.x) >> 5, part = g % per;
   const int local = int(blockIdx.x) * (8 / per) + g / per, r = j.tile + local;
   const bool on = local < a.tile_rows && r < j.tokens * a.share;
-  const int64_t step = int64_t(a.kv_heads) * a.tile_rows, first = (int64_t(j.slot) * a.kv_heads + hk) * a.tile_rows + local;
+  const int64_t step = int64_t(a.kv_heads) * a.tile_rows;
+  const int64_t first = on ? (int64_t(j.slot) * a.kv_heads + hk) * a.tile_rows + local : 0;
+  const int count = on ? j.count : 0;
   float top = -INFINITY;
-  if (on)
-    for (int s = l; s < j.count; s += 32) top = fmaxf(top, a.part_ml[first + s * step].x);
+  for (int s = l; s < count; s += 32) top = fmaxf(top, a.part_ml[first + s * step].x);
   for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
   const float ref = top == -INFINITY ? 0.0f : top;
   float total = 0.0f;
   f32x4 o4{};
-  if (on) {
-    for (int s = part; s < j.count; s += per) {
-      const float2 m = a.part_ml[first + s * step];
-      f32x4 v{};
-      if (m.y != 0.0f && 4 * l < a.pdim)  // else no state of this part counts: its row is not written
-        v = *reinterpret_cast<const f32x4*>(a.part + (first + s * step) * a.pdim + 4 * l);
-      const float w = __builtin_amdgcn_exp2f(m.x - ref);
-      total += m.y * w;
-      o4 += v * w;
-    }
+  const float* const row_part = a.part + first * a.pdim + (4 * l < a.pdim ? 4 * l : 0);
+#pragma unroll 4
+  for (int s = part; s < count; s += per) {
+    const float2 m = a.part_ml[first + s * step];
+    const f32x4 v = *reinterpret_cast<const f32x4*>(row_part + s * step * a.pdim);
+    const float w = __builtin_amdgcn_exp2f(m.x - ref);
+    total += m.y * w;
+    const bool counts = m.y != 0.0f;  // else no state of this part does: its row is not written
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o4[i] += counts ? v[i] * w : 0.0f;
   }
   if (per > 1) {
     if (l == 0) totals[g] = total;
@@ -440,10 +456,11 @@ int launch_causal_attention(const rdv_causal_attention_desc& d, const void* plan
   rc = launch_matrix(d.dtype, h.pairs ? kCausalTilePairs : kCausalTile, a, lists, h.at_rows, h.rows, stream);
   if (rc == RDV_OK) rc = launch_matrix(d.dtype, kCausalFew, a, lists, h.at_few, h.few, stream);
   if (rc != RDV_OK) return rc;
-  const int per = h.rows == 0 ? 8 : 1, rows = h.rows == 0 ? 32 : h.tile_rows;
+  int per = 1;
+  while (per < 8 && 4 * per < h.join_parts) per *= 2;
   return launch_joins(a, lists, h.at_row_joins, h.row_joins, [&](unsigned joins) {
     with_dtype(d.dtype, [&](auto t) {
-      causal_join_kernel<decltype(t)><<<dim3(unsigned(rows * per / 8), joins, unsigned(d.kv_heads)), 256, 0, stream>>>(a, per);
+      causal_join_kernel<decltype(t)><<<dim3(unsigned((h.join_rows * per + 7) / 8), joins, unsigned(d.kv_heads)), 256, 0, stream>>>(a, per);
     });
   });
 }

@@ -1,10 +1,12 @@
 // The embedding of tokens, y[i] = scale weight[token_i], and its gradient, dweight[v] = scale (sum of grad's rows whose
 // token is v).  Build-defined (no counterpart in the reference).
 //
-// The gradient groups the tokens by a sort that keeps their order, so that its sums have one order and no atomics:
-//   * embed_sort_kernel: each block takes a range of the vocabulary and goes over all tokens twice: it counts its own, and
-//     those below its range (which tells where its part of the sorted list begins, without a word from other blocks), then
-//     puts its own in place.  The tokens stay in the L2: n tokens of 4 bytes at some 100 GB/s per CU.
+// The gradient groups the tokens by a sort whose order follows from the tokens alone, so that its sums have one order and no
+// floating-point atomics:
+//   * embed_sort_kernel: block b takes the tokens that are b modulo the number of blocks (frequent tokens, which tend to
+//     have neighbouring numbers, so spread over the blocks) and goes over all tokens twice: it counts its own, and those of
+//     the blocks before it (which tells where its part of the sorted list begins, without a word from them), then puts its
+//     own in place.  The tokens stay in the L2.
 //   * embed_rows_kernel: a row of the vocabulary with up to kLong tokens is summed by the lanes that share it and written,
 //     one without tokens is written as zeros.  Longer runs are cut at multiples of kLong of the sorted list: a run's piece
 //     of such a chunk is summed into the workspace.
@@ -17,20 +19,23 @@ namespace rdv {
 namespace {
 
 constexpr int kSortThreads = 1024, kSortWaves = kSortThreads / 64;
-constexpr int kSortRows = 512;  // of the vocabulary, per block at most: 32 KiB of counts
-constexpr int kLong = 64;
+constexpr int kSortList = 224;  // tokens that a wave lists: with the counts below 64 KiB
+constexpr int kSortRows = 512;  // tokens of the vocabulary per block, at most: 32 KiB of counts
+constexpr int kLong = 32;
 
 struct EmbedArgs {
   const void* tokens;      // int32 or int64
   const void *weight, *grad;
   void* out;               // y or dweight
-  int32_t *begin, *place;  // [vocab + 1]: where a token's run begins; [n]: the sorted positions
+  int32_t *begin, *place;  // [blocks * range + 1]: where a token's run begins, at slot(token); [n]: the sorted positions
   int32_t* token;          // [n]: their tokens
-  float* part;             // [chunks][2][dim]: a long run's sum within a chunk, of the run that goes on from the chunk
+  float* part;             // [chunks][2][pdim]: a long run's sum within a chunk, of the run that goes on from the chunk
                            // before, and of the one that begins here
   int64_t n, w_row, g_row;
-  int vocab, dim, range;   // range: rows of the vocabulary per block of embed_sort_kernel
+  int vocab, dim, pdim, range, bits;  // range: tokens of a block of the sort; bits: log2 of its blocks
+  int slices, chunk_blocks;           // waves that share a row's pieces; blocks of embed_rows_kernel that take chunks
   float scale;
+  __device__ __forceinline__ int slot(int token) const { return (token & ((1 << bits) - 1)) * range + (token >> bits); }
 };
 
 template <class I>
@@ -68,29 +73,78 @@ __device__ __forceinline__ int block_count(int v, int* red) {
   return t;
 }
 
-// Waves take contiguous parts of the tokens, so that the order of (wave, step, lane) is theirs.  count[wave][row] becomes
-// where the wave puts its next token of the row.
+// Four tokens of a lane, -1 past the end.
+template <class I>
+struct TokenPiece {
+  typedef I vec __attribute__((ext_vector_type(4)));
+  typedef vec loose __attribute__((aligned(sizeof(I))));
+  int t[4];
+  // tokens of no row of the vocabulary become -1
+  __device__ __forceinline__ void load(const EmbedArgs& a, int64_t i) {
+    vec v;
+    if (i + 4 <= a.n) {
+      v = *reinterpret_cast<const loose*>(static_cast<const I*>(a.tokens) + i);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = i + j < a.n ? static_cast<const I*>(a.tokens)[i + j] : I(-1);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const I x = v[j];
+      t[j] = x >= 0 && x < a.vocab ? int(x) : -1;
+    }
+  }
+};
+
+// Waves take contiguous parts of the tokens, 256 at a step; a run is in the order (wave, step, token of a lane, lane).
+// count[wave][row] becomes where the wave puts its next token of the row.  A wave lists its tokens as it counts them, so that
+// it need not look for them again; with more than kSortList it does.
 template <class I>
 __global__ __launch_bounds__(kSortThreads) void embed_sort_kernel(EmbedArgs a) {
   extern __shared__ int count[];  // [kSortWaves][range]
   __shared__ int red[kSortWaves], wave_sum[kSortWaves];
+  __shared__ int2 lists[kSortWaves][kSortList];  // (token, position)
+  constexpr int kAhead = 4;  // steps whose loads are in flight together
   const int tid = int(threadIdx.x), lane = tid & 63, wave = tid >> 6;
-  const int64_t lo = int64_t(blockIdx.x) * a.range, rows = min(int64_t(a.range), a.vocab - lo);
+  const int block = int(blockIdx.x), low = (1 << a.bits) - 1;
   for (int i = tid; i < kSortWaves * a.range; i += kSortThreads) count[i] = 0;
   __syncthreads();
-  const int64_t per = (a.n + kSortWaves * 64 - 1) / (kSortWaves * 64) * 64, first = wave * per, last = min(first + per, a.n);
+  const int64_t per = (a.n + kSortWaves * 256 - 1) / (kSortWaves * 256) * 256, first = wave * per, last = min(first + per, a.n);
   int* const mine = count + wave * a.range;
-  int below = 0;
-  for (int64_t i = first + lane; i < last; i += 64) {
-    const int64_t t = token_at<I>(a.tokens, i);
-    below += t >= 0 && t < lo;
-    if (t >= lo && t < lo + rows) atomicAdd(&mine[t - lo], 1);
-  }
+  int2* const list = lists[wave];
+  int below = 0, found = 0;
+  // f(tokens of the lanes, their own ones, position of the lane's) for every token of the lanes in turn
+  const auto walk = [&](auto f) {
+    for (int64_t i0 = first; i0 < last; i0 += 256 * kAhead) {
+      TokenPiece<I> p[kAhead];
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) p[k].load(a, i0 + 256 * k < last ? i0 + 256 * k + 4 * lane : a.n);
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int t = p[k].t[j];
+          f(t, t >= 0 && (t & low) == block, int(i0) + 256 * k + 4 * lane + j);
+        }
+    }
+  };
+  walk([&](int t, bool own, int at) {
+    below += t >= 0 && (t & low) < block;
+    const uint64_t all = __ballot(own);
+    if (!all) return;
+    if (own) {
+      atomicAdd(&mine[t >> a.bits], 1);
+      const int q = found + __popcll(all & ((uint64_t(1) << lane) - 1));
+      if (q < kSortList) list[q] = int2{t, at};
+    }
+    found += __popcll(all);
+  });
   const int base = block_count(below, red);  // with a barrier: the counts are whole
   // exclusive sums over (row, wave), a run of rows per thread
   const int each = (a.range + kSortThreads - 1) / kSortThreads;
   int total = 0;
   for (int r = tid * each; r < min((tid + 1) * each, a.range); ++r)
+#pragma unroll
     for (int w = 0; w < kSortWaves; ++w) total += count[w * a.range + r];
   int before = total;
 #pragma unroll
@@ -103,98 +157,124 @@ __global__ __launch_bounds__(kSortThreads) void embed_sort_kernel(EmbedArgs a) {
   int at = base + before - total;
   for (int w = 0; w < wave; ++w) at += wave_sum[w];
   for (int r = tid * each; r < min((tid + 1) * each, a.range); ++r) {
-    if (r < rows) a.begin[lo + r] = at;
+    a.begin[int64_t(block) * a.range + r] = at;
+    int c[kSortWaves];
+#pragma unroll
+    for (int w = 0; w < kSortWaves; ++w) c[w] = count[w * a.range + r];
+#pragma unroll
     for (int w = 0; w < kSortWaves; ++w) {
-      const int c = count[w * a.range + r];
       count[w * a.range + r] = at;
-      at += c;
+      at += c[w];
     }
   }
-  if (lo + rows == a.vocab && tid == kSortThreads - 1) a.begin[a.vocab] = at;
+  if (block == low && tid == kSortThreads - 1) a.begin[(int64_t(block) + 1) * a.range] = at;
   __syncthreads();
-  for (int64_t i0 = first; i0 < last; i0 += 64) {
-    const int64_t i = i0 + lane;
-    const int64_t t = i < last ? token_at<I>(a.tokens, i) : -1;
-    const int r = t >= lo && t < lo + rows ? int(t - lo) : -1;
-    for (uint64_t left = __ballot(r >= 0); left;) {  // each token of this step once
-      const int row = __builtin_amdgcn_readlane(r, __builtin_ctzll(left));
-      const uint64_t same = __ballot(r == row);
-      const int at = mine[row];
-      if (r == row) {
-        const int p = at + __popcll(same & ((uint64_t(1) << lane) - 1));
-        a.place[p] = int(i);
-        a.token[p] = int(t);
+  const auto place = [&](int t, bool own, int position) {
+    for (uint64_t left = __ballot(own); left;) {  // each token of these once
+      const int token = __builtin_amdgcn_readlane(t, __builtin_ctzll(left));
+      const uint64_t same = __ballot(own && t == token);
+      const int to = mine[token >> a.bits];
+      if (own && t == token) {
+        const int q = to + __popcll(same & ((uint64_t(1) << lane) - 1));
+        a.place[q] = position;
+        a.token[q] = t;
       }
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      if (lane == 0) mine[row] = at + __popcll(same);
+      if (lane == 0) mine[token >> a.bits] = to + __popcll(same);
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       left &= ~same;
     }
+  };
+  if (found > kSortList) {
+    walk(place);
+    return;
+  }
+  for (int i = lane; i - lane < found; i += 64) {
+    const int2 v = i < found ? list[i] : int2{-1, 0};
+    place(v.x, i < found, v.y);
   }
 }
 
-// sum += grad's rows at sorted places first .. last - 1, elements d ..
-template <class T>
-__device__ __forceinline__ void add_rows(const EmbedArgs& a, int first, int last, int d, float (&sum)[RowPiece<T>::E]) {
-  typedef RowPiece<T> P;
-  int p = first;
-  for (; p + 4 <= last; p += 4) {
-    P g[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) g[j].load(static_cast<const T*>(a.grad) + int64_t(a.place[p + j]) * a.g_row, d, a.dim);
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-#pragma unroll
-      for (int i = 0; i < P::E; ++i) sum[i] += g[j][i];
-  }
-  for (; p < last; ++p) {
-    P g;
-    g.load(static_cast<const T*>(a.grad) + int64_t(a.place[p]) * a.g_row, d, a.dim);
-#pragma unroll
-    for (int i = 0; i < P::E; ++i) sum[i] += g[i];
-  }
-}
-
-template <class T>
-__device__ __forceinline__ void put_part(float* at, int d, int dim, const float (&sum)[RowPiece<T>::E]) {
-#pragma unroll
-  for (int i = 0; i < RowPiece<T>::E; ++i)
-    if (d + i < dim) at[d + i] = sum[i];
-}
-
-// The first `row_blocks` blocks take the rows of the vocabulary, the others the chunks.
+// sum += grad's rows at sorted places first .. last - 1, elements d .., up to kAdd loads in flight.  The G lanes read G places
+// at once and hand them round.
+constexpr int kAdd = 8;
 template <class T, int G>
-__global__ __launch_bounds__(256) void embed_rows_kernel(EmbedArgs a, int row_blocks) {
+__device__ __forceinline__ void add_rows(const EmbedArgs& a, int first, int last, int d, int lane,
+                                         float (&sum)[RowPiece<T>::E]) {
   typedef RowPiece<T> P;
-  const int lane = int(threadIdx.x) % G, group = int(threadIdx.x) / G;
-  if (int(blockIdx.x) < row_blocks) {
-    const int64_t v = int64_t(blockIdx.x) * (256 / G) + group;
-    if (v >= a.vocab) return;
-    const int first = a.begin[v], last = a.begin[v + 1];
-    if (last - first > kLong) return;
-    T* const out = static_cast<T*>(a.out) + v * a.dim;
-    for (int d = lane * P::E; d < a.dim; d += G * P::E) {
-      float sum[P::E] = {};
-      add_rows<T>(a, first, last, d, sum);
+  constexpr int N = G < kAdd ? G : kAdd;
+  for (int p0 = first; p0 < last; p0 += G) {
+    const int n = min(G, last - p0), mine = a.place[p0 + min(lane, n - 1)];
+    for (int j0 = 0; j0 < n; j0 += N) {
+      P g[N];
+#pragma unroll
+      for (int j = 0; j < N; ++j) {  // past the end the last row again, for nothing
+        const int at = G == 64 ? __builtin_amdgcn_readlane(mine, min(j0 + j, n - 1)) : __shfl(mine, min(j0 + j, n - 1), G);
+        g[j].load(static_cast<const T*>(a.grad) + int64_t(at) * a.g_row, d, a.dim);
+      }
+#pragma unroll
+      for (int j = 0; j < N; ++j)
+#pragma unroll
+        for (int i = 0; i < P::E; ++i) sum[i] += j0 + j < n ? g[j][i] : 0.0f;
+    }
+  }
+}
+
+// G lanes take a slice of G pieces of kRows rows of the vocabulary, neighbours in the sorted list, or of a chunk's sums.  The
+// chunks' blocks come first: they take longest.  Most rows have no token or one: those of all kRows are read at once.
+constexpr int kRows = 4;
+template <class T, int G>
+__global__ __launch_bounds__(256) void embed_rows_kernel(EmbedArgs a) {
+  typedef RowPiece<T> P;
+  const int lane = int(threadIdx.x) % G;
+  const int group = G == 64 ? __builtin_amdgcn_readfirstlane(int(threadIdx.x) >> 6) : int(threadIdx.x) / G;
+  const bool rows = int(blockIdx.x) >= a.chunk_blocks;
+  const uint32_t task = (blockIdx.x - (rows ? a.chunk_blocks : 0)) * (256 / G) + group;
+  const uint32_t item = a.slices == 1 ? task : task / uint32_t(a.slices);
+  const int d = (int(task - item * a.slices) * G + lane) * P::E;  // past dim: lanes that only hand places round, and read for nothing
+  const bool on = d < a.dim;
+  if (rows) {
+    const int64_t slot0 = int64_t(item) * kRows, slots = int64_t(a.range) << a.bits;
+    if (slot0 >= slots) return;
+    int begin[kRows + 1], at[kRows];
+    P g[kRows];
+#pragma unroll
+    for (int r = 0; r <= kRows; ++r) begin[r] = a.begin[min(slot0 + r, slots)];
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) at[r] = begin[r + 1] > begin[r] ? a.place[begin[r]] : -1;
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      g[r] = P{};
+      if (at[r] >= 0 && on) g[r].load(static_cast<const T*>(a.grad) + int64_t(at[r]) * a.g_row, d, a.dim);
+    }
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      const uint32_t slot = uint32_t(min(slot0 + r, slots - 1)), block = slot / uint32_t(a.range);
+      const int64_t v = (int64_t(slot - block * a.range) << a.bits) + block;
+      if (slot0 + r >= slots || v >= a.vocab || begin[r + 1] - begin[r] > kLong) continue;
+      float sum[P::E];
+#pragma unroll
+      for (int i = 0; i < P::E; ++i) sum[i] = g[r][i];
+      add_rows<T, G>(a, begin[r] + 1, begin[r + 1], on ? d : 0, lane, sum);
       P o;
 #pragma unroll
       for (int i = 0; i < P::E; ++i) o.set(i, sum[i] * a.scale);
-      o.store(out, d, a.dim);
+      if (on) o.store(static_cast<T*>(a.out) + v * a.dim, d, a.dim);
     }
     return;
   }
-  const int count = a.begin[a.vocab];
-  const int64_t chunk = (int64_t(blockIdx.x) - row_blocks) * (256 / G) + group;
-  if (chunk * kLong >= count) return;
-  const int first = int(chunk) * kLong, last = min(first + kLong, count);
+  const int count = a.begin[a.range << a.bits];
+  if (int64_t(item) * kLong >= count) return;
+  const int first = int(item) * kLong, last = min(first + kLong, count);
   for (int side = 0; side < 2; ++side) {  // the run of the chunk's first token, and of its last one
-    const int t = a.token[side ? last - 1 : first], b = a.begin[t], e = a.begin[t + 1];
+    const int at = a.slot(a.token[side ? last - 1 : first]), b = a.begin[at], e = a.begin[at + 1];
     if (e - b <= kLong || (b < first) != (side == 0)) continue;
-    for (int d = lane * P::E; d < a.dim; d += G * P::E) {
-      float sum[P::E] = {};
-      add_rows<T>(a, max(b, first), min(e, last), d, sum);
-      put_part<T>(a.part + (chunk * 2 + side) * a.dim, d, a.dim, sum);
-    }
+    float sum[P::E] = {};
+    add_rows<T, G>(a, max(b, first), min(e, last), on ? d : 0, lane, sum);
+    if (!on) continue;
+    float* const part = a.part + (int64_t(item) * 2 + side) * a.pdim + d;
+#pragma unroll
+    for (int i = 0; i < P::E; i += 4) *reinterpret_cast<f32x4*>(part + i) = f32x4{sum[i], sum[i + 1], sum[i + 2], sum[i + 3]};
   }
 }
 
@@ -203,26 +283,31 @@ template <class T, int G>
 __global__ __launch_bounds__(256) void embed_join_kernel(EmbedArgs a) {
   typedef RowPiece<T> P;
   const int lane = int(threadIdx.x) % G, group = int(threadIdx.x) / G;
-  const int count = a.begin[a.vocab];
-  const int64_t chunk = int64_t(blockIdx.x) * (256 / G) + group;
-  if (chunk * kLong >= count) return;
-  const int last = min(int(chunk) * kLong + kLong, count), t = a.token[last - 1], b = a.begin[t], e = a.begin[t + 1];
-  if (e - b <= kLong || b < chunk * kLong) return;
-  const int64_t end = (e - 1) / kLong;  // its last chunk
-  T* const out = static_cast<T*>(a.out) + int64_t(t) * a.dim;
-  for (int d = lane * P::E; d < a.dim; d += G * P::E) {
-    float sum[P::E] = {};
-    for (int64_t c = chunk; c <= end; ++c) {
-      const float* const part = a.part + (c * 2 + (c == chunk)) * a.dim;
+  const uint32_t task = blockIdx.x * (256 / G) + group, chunk = a.slices == 1 ? task : task / uint32_t(a.slices);
+  const int d = (int(task - chunk * a.slices) * G + lane) * P::E, count = a.begin[a.range << a.bits];
+  if (d >= a.dim || int64_t(chunk) * kLong >= count) return;
+  const int last = min(int(chunk) * kLong + kLong, count), t = a.token[last - 1], at = a.slot(t);
+  const int b = a.begin[at], e = a.begin[at + 1];
+  if (e - b <= kLong || b < int(chunk) * kLong) return;
+  const int more = (e - 1) / kLong - int(chunk);  // chunks after this one
+  const float* part = a.part + (int64_t(chunk) * 2 + 1) * a.pdim + d;
+  float sum[P::E];
 #pragma unroll
-      for (int i = 0; i < P::E; ++i)
-        if (d + i < a.dim) sum[i] += part[d + i];
+  for (int i = 0; i < P::E; ++i) sum[i] = part[i];
+  part += a.pdim;  // the next chunks' first places
+#pragma unroll 8
+  for (int c = 0; c < more; ++c) {
+#pragma unroll
+    for (int i = 0; i < P::E; i += 4) {
+      const f32x4 v = *reinterpret_cast<const f32x4*>(part + int64_t(c) * 2 * a.pdim + i);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) sum[i + j] += v[j];
     }
-    P o;
-#pragma unroll
-    for (int i = 0; i < P::E; ++i) o.set(i, sum[i] * a.scale);
-    o.store(out, d, a.dim);
   }
+  P o;
+#pragma unroll
+  for (int i = 0; i < P::E; ++i) o.set(i, sum[i] * a.scale);
+  o.store(static_cast<T*>(a.out) + int64_t(t) * a.dim, d, a.dim);
 }
 
 template <class F>
@@ -234,20 +319,23 @@ auto with_lanes(int dim, int dtype, F&& f) {
 }
 
 struct Plan {
-  int range, blocks;  // of the sort
-  int64_t chunks, begin, place, token, part, bytes;
+  int range, bits, pdim;  // tokens per block of the sort, log2 of its blocks; dim rounded up to 16 bytes
+  int64_t chunks, place, token, part, bytes;
 };
 int64_t align256(int64_t bytes) { return (bytes + 255) / 256 * 256; }
-Plan make_plan(const rdv_embedding_desc& d, int cu) {
+Plan make_plan(const rdv_embedding_desc& d) {
   Plan p{};
-  // as many blocks as CUs, as long as a block has 16 rows
-  p.range = int(std::min<int64_t>(kSortRows, std::max<int64_t>(16, (int64_t(d.vocab) + cu - 1) / cu)));
-  p.blocks = int((int64_t(d.vocab) + p.range - 1) / p.range);
+  // a block per CU and up to kSortRows tokens each, fewer blocks where they would have less than 16
+  p.bits = 0;
+  while ((int64_t(d.vocab) >> p.bits) > kSortRows || (p.bits < 8 && (d.vocab >> p.bits) > 16)) ++p.bits;
+  p.range = int(((int64_t(d.vocab) - 1) >> p.bits) + 1);
+  const int e = d.dtype == RDV_DTYPE_F32 ? 4 : 8;
+  p.pdim = (d.dim + e - 1) / e * e;
   p.chunks = (d.tokens + kLong - 1) / kLong;
-  p.place = align256((int64_t(d.vocab) + 1) * 4);
+  p.place = align256((int64_t(p.range) * (int64_t(1) << p.bits) + 1) * 4);
   p.token = p.place + align256(d.tokens * 4);
   p.part = p.token + align256(d.tokens * 4);
-  p.bytes = p.part + p.chunks * 2 * d.dim * 4;
+  p.bytes = p.part + (d.tokens > kLong ? p.chunks * 2 * p.pdim * 4 : 0);
   return p;
 }
 
@@ -265,7 +353,7 @@ EmbedArgs make_args(const rdv_embedding_desc& d, const void* tokens) {
 
 }  // namespace
 
-int64_t embedding_workspace_bytes(const rdv_embedding_desc& d, int cu) { return make_plan(d, cu).bytes; }
+int64_t embedding_workspace_bytes(const rdv_embedding_desc& d) { return make_plan(d).bytes; }
 
 int launch_embedding(const rdv_embedding_desc& d, const void* tokens, const void* weight, void* out, int cu,
                      hipStream_t stream) {
@@ -286,29 +374,35 @@ int launch_embedding(const rdv_embedding_desc& d, const void* tokens, const void
 }
 
 int launch_embedding_backward(const rdv_embedding_desc& d, const void* grad, const void* tokens, void* dweight,
-                              void* workspace, int cu, hipStream_t stream) {
-  const Plan p = make_plan(d, cu);
+                              void* workspace, hipStream_t stream) {
+  const Plan p = make_plan(d);
   uint8_t* const ws = static_cast<uint8_t*>(workspace);
   EmbedArgs a = make_args(d, tokens);
   a.grad = grad;
   a.out = dweight;
   a.range = p.range;
+  a.bits = p.bits;
+  a.pdim = p.pdim;
   a.begin = reinterpret_cast<int32_t*>(ws);
   a.place = reinterpret_cast<int32_t*>(ws + p.place);
   a.token = reinterpret_cast<int32_t*>(ws + p.token);
   a.part = reinterpret_cast<float*>(ws + p.part);
   const int lds = kSortWaves * p.range * 4;
-  if (d.wide_tokens) embed_sort_kernel<int64_t><<<unsigned(p.blocks), kSortThreads, lds, stream>>>(a);
-  else embed_sort_kernel<int32_t><<<unsigned(p.blocks), kSortThreads, lds, stream>>>(a);
+  if (d.wide_tokens) embed_sort_kernel<int64_t><<<1u << p.bits, kSortThreads, lds, stream>>>(a);
+  else embed_sort_kernel<int32_t><<<1u << p.bits, kSortThreads, lds, stream>>>(a);
   RDV_HIP_TRY(hipGetLastError());
   return with_dtype(d.dtype, [&](auto t) {
     using T = decltype(t);
     return with_lanes(d.dim, d.dtype, [&](auto g) {
-      constexpr int G = decltype(g)::value;
-      const int64_t rows = (int64_t(d.vocab) + 256 / G - 1) / (256 / G), chunks = (p.chunks + 256 / G - 1) / (256 / G);
-      embed_rows_kernel<T, G><<<unsigned(rows + chunks), 256, 0, stream>>>(a, int(rows));
+      constexpr int G = decltype(g)::value, E = RowPiece<T>::E;
+      a.slices = (p.pdim / E + G - 1) / G;
+      const auto blocks = [&](int64_t items) { return (items * a.slices + 256 / G - 1) / (256 / G); };
+      const int64_t chunks = d.tokens > kLong ? blocks(p.chunks) : 0;
+      a.chunk_blocks = int(chunks);
+      const int64_t rows = ((int64_t(p.range) << p.bits) + kRows - 1) / kRows;
+      embed_rows_kernel<T, G><<<unsigned(chunks + blocks(rows)), 256, 0, stream>>>(a);
       RDV_HIP_TRY(hipGetLastError());
-      if (d.tokens > kLong) {
+      if (chunks > 0) {
         embed_join_kernel<T, G><<<unsigned(chunks), 256, 0, stream>>>(a);
         RDV_HIP_TRY(hipGetLastError());
       }
