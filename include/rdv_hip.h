@@ -734,18 +734,21 @@ int rdv_causal_attention_plan(const rdv_causal_attention_desc* desc, const int64
 /* Bytes of workspace of the forward (backward = 0) or the backward call; < 0 on error. */
 int64_t rdv_causal_attention_workspace_bytes(const rdv_causal_attention_desc* desc, const void* plan, int32_t backward);
 
-/* out[tokens, heads, dim] (contiguous) and, where lse is not NULL, lse[heads, tokens] fp32. */
+/* out[tokens, heads, dim] (contiguous) and, where not NULL, lse[heads, tokens]
+ * fp32 and rest, like out: what rounding out to a 16-bit type left, in that type
+ * (not written for fp32). */
 int rdv_causal_attention(const rdv_causal_attention_desc* desc, const void* plan, const void* device_plan,
-                         const void* q, const void* k, const void* v, void* out, float* lse, void* workspace,
-                         int64_t workspace_bytes, void* stream);
+                         const void* q, const void* k, const void* v, void* out, float* lse, void* rest,
+                         void* workspace, int64_t workspace_bytes, void* stream);
 
-/* The gradients of rdv_causal_attention for grad = dL/dout, given the out and lse
- * that it wrote: dq[tokens, heads, dim], dk and dv[states, kv_heads, dim],
+/* The gradients of rdv_causal_attention for grad = dL/dout, given the out, lse and
+ * rest that it wrote (rest may be NULL: each row's sum of grad * out is then of
+ * out as it was rounded): dq[tokens, heads, dim], dk and dv[states, kv_heads, dim],
  * contiguous; the gradients of a state head are summed over the heads that read
  * it, and are 0 at states that no token sees. */
 int rdv_causal_attention_backward(const rdv_causal_attention_desc* desc, const void* plan, const void* device_plan,
                                   const void* grad, const void* q, const void* k, const void* v, const void* out,
-                                  const float* lse, void* dq, void* dk, void* dv, void* workspace,
+                                  const float* lse, const void* rest, void* dq, void* dk, void* dv, void* workspace,
                                   int64_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus

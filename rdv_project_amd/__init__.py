@@ -91,6 +91,7 @@ from ._image_ops import (
     group_norm_backward,
 )
 from ._prompt_ops import (
+    AttentionStats,
     PackedSequences,
     causal_attention,
     causal_attention_backward,
@@ -130,6 +131,7 @@ from .rendering import (
     VoxelMajorantField,
 )
 from .nn import (
+    CausalAttentionTensorOp,
     ConcatTensorOp,
     Conv2DTensorOp,
     Conv2DTensorOpFast,
@@ -140,7 +142,9 @@ from .nn import (
     CrossAttentionTensorOp,
     Downsample2xTensorOp,
     DropoutTensorOp,
+    EmbeddingTensorOp,
     GroupNormTensorOp,
+    RMSNormTensorOp,
     Upsample2xTensorOp,
     DensityRGB,
     LinearTensorOp,

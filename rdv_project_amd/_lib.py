@@ -334,8 +334,8 @@ _SIGNATURES = {
     "rdv_causal_attention_plan": (C.c_int, [C.POINTER(CausalAttentionDesc), C.c_void_p, C.c_int64, C.c_int32, C.c_void_p,
                                             C.c_int64]),
     "rdv_causal_attention_workspace_bytes": (C.c_int64, [C.POINTER(CausalAttentionDesc), C.c_void_p, C.c_int32]),
-    "rdv_causal_attention": (C.c_int, [C.POINTER(CausalAttentionDesc), *[C.c_void_p] * 8, C.c_int64, C.c_void_p]),
-    "rdv_causal_attention_backward": (C.c_int, [C.POINTER(CausalAttentionDesc), *[C.c_void_p] * 12, C.c_int64,
+    "rdv_causal_attention": (C.c_int, [C.POINTER(CausalAttentionDesc), *[C.c_void_p] * 9, C.c_int64, C.c_void_p]),
+    "rdv_causal_attention_backward": (C.c_int, [C.POINTER(CausalAttentionDesc), *[C.c_void_p] * 13, C.c_int64,
                                                 C.c_void_p]),
 }
 

@@ -13,6 +13,7 @@ from __future__ import annotations
 import ctypes as C
 import functools
 import math
+from typing import NamedTuple, Optional
 
 import torch
 
@@ -357,6 +358,14 @@ class PackedSequences:
         return hit
 
 
+class AttentionStats(NamedTuple):
+    """What causal_attention_backward takes from the forward call beside its result."""
+    #: [heads, tokens] float32, the logarithm of each softmax's denominator (-inf where nothing is seen)
+    lse: torch.Tensor
+    #: like out, what rounding it to a 16-bit type left; None for float32
+    rest: Optional[torch.Tensor]
+
+
 def _counts(values, what: str) -> tuple:
     values = values.tolist() if isinstance(values, torch.Tensor) else values
     try:
@@ -411,12 +420,12 @@ def _causal_inputs(q, k, v, sequences, scale, grad=None):
     return q, k, v, grad, sequences._call(layout, device), device
 
 
-def _causal_attention_into(call, q, k, v, out, lse, device: int) -> None:
-    """Launches rdv_causal_attention into out and lse (or None)."""
+def _causal_attention_into(call, q, k, v, out, lse, rest, device: int) -> None:
+    """Launches rdv_causal_attention into out, and into lse and rest (or None)."""
     _, d, host, lists, nbytes = call
     ws = _workspace(nbytes, q)
     _check(_lib.load().rdv_causal_attention(d, host.data_ptr(), lists.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(),
-                                            out.data_ptr(), _ptr(lse), _ptr(ws), nbytes, _stream(device)),
+                                            out.data_ptr(), _ptr(lse), _ptr(rest), _ptr(ws), nbytes, _stream(device)),
            "causal_attention")
 
 
@@ -429,12 +438,13 @@ def causal_attention(q, k, v, sequences: PackedSequences, scale: float | None = 
     1 / sqrt(dim).  What k and v hold at states that a token does not see has no
     effect on it, and a token that sees none gets 0.
 
-    Returns out [tokens, heads, dim] and with return_lse also lse [heads, tokens]
-    float32, the logarithm of each softmax's denominator (-inf where nothing is
-    seen), which causal_attention_backward takes.  Rows behind the last sequence
-    are left as they are in `out`, and are 0 (-inf) in fresh results.  float16 and
-    bfloat16 inputs: the matrix cores take softmax terms rounded to that type;
-    float32: float32 throughout."""
+    Returns out [tokens, heads, dim] and with return_lse also AttentionStats (lse,
+    rest), which causal_attention_backward takes: lse [heads, tokens] float32, the
+    logarithm of each softmax's denominator (-inf where nothing is seen), and rest,
+    like out, what rounding out to a 16-bit type left (None for float32).  Rows
+    behind the last sequence are left as they are in `out`, and are 0 (-inf) in
+    fresh results.  float16 and bfloat16 inputs: the matrix cores take softmax terms
+    rounded to that type; float32: float32 throughout."""
     given = q, k, v
     q, k, v, _, call, device = _causal_inputs(q, k, v, sequences, scale)
     d = call[0]
@@ -443,41 +453,48 @@ def causal_attention(q, k, v, sequences: PackedSequences, scale: float | None = 
         _apart(y, *zip((_tensor(t, n) for t, n in zip(given, "qkv")), "qkv"))
     elif sequences.tokens < d.tokens:
         y[sequences.tokens:].zero_()
-    lse = None
+    lse = rest = None
     if return_lse:
         lse = torch.empty((d.heads, d.tokens), dtype=torch.float32, device=q.device)
+        rest = None if q.dtype == torch.float32 else _like_out(None, y)
         if sequences.tokens < d.tokens:
             lse[:, sequences.tokens:].fill_(-math.inf)
+            if rest is not None:
+                rest[sequences.tokens:].zero_()
     with launch_scope():
-        _causal_attention_into(call, q, k, v, y, lse, device)
-    return (y, lse) if return_lse else y
+        _causal_attention_into(call, q, k, v, y, lse, rest, device)
+    return (y, AttentionStats(lse, rest)) if return_lse else y
 
 
-def causal_attention_backward(grad, q, k, v, out, lse, sequences: PackedSequences, scale: float | None = None,
+def causal_attention_backward(grad, q, k, v, out, stats, sequences: PackedSequences, scale: float | None = None,
                               grads=None):
-    """(dq, dk, dv) of causal_attention for grad = dL/dout, given the out and lse it
-    returned for the same arguments.  dk and dv are summed over the heads that
+    """(dq, dk, dv) of causal_attention for grad = dL/dout, given the out and stats
+    that it returned for the same arguments with return_lse (stats may be lse alone:
+    each row's sum of grad * out is then of `out` as it was rounded).  dk and dv are summed over the heads that
     share a state head and are 0 at states that no token sees; no two sequences may
     share states.  `grads` supplies the three buffers, whose rows that belong to no
     sequence are left as they are (0 in fresh ones).  float16 and bfloat16 inputs:
     the matrix cores take softmax terms and the scores' gradients rounded to that
-    type, and each row's sum of grad * out is of `out` as it was rounded."""
+    type."""
     if isinstance(sequences, PackedSequences) and not sequences.apart:
         raise NotImplementedError("gradients of sequences that share states")
     q, k, v, grad, call, device = _causal_inputs(q, k, v, sequences, scale, _tensor(grad, "grad"))
     d, desc, host, lists, nbytes = call
     out = _like(out, q, "out").contiguous()
+    lse, rest = stats if isinstance(stats, (list, tuple)) and len(stats) == 2 else (stats, None)
     lse = _tensor(lse, "lse")
+    if rest is not None:
+        rest = _like(rest, q, "rest").contiguous()
     assert tuple(lse.shape) == (d.heads, d.tokens) and lse.is_contiguous(), \
         f"lse must be a contiguous [{d.heads}, {d.tokens}] tensor, as causal_attention returns it"
     if lse.dtype != torch.float32:
         raise TypeError(f"lse must be float32, got {lse.dtype}")
-    _on_gpu(device, out, "out", lse, "lse")
+    _on_gpu(device, out, "out", lse, "lse", rest, "rest")
     given = grads is not None
     dq, dk, dv = _grad_tensors(grads, (q, k, v), ("dq", "dk", "dv"))
     if given:
         for t in (dq, dk, dv):
-            _apart(t, (grad, "grad"), (q, "q"), (k, "k"), (v, "v"), (out, "out"), (lse, "lse"))
+            _apart(t, (grad, "grad"), (q, "q"), (k, "k"), (v, "v"), (out, "out"), (lse, "lse"), (rest, "rest"))
     else:
         if sequences.tokens < d.tokens:
             dq[sequences.tokens:].zero_()
@@ -487,10 +504,11 @@ def causal_attention_backward(grad, q, k, v, out, lse, sequences: PackedSequence
             dv[at:].zero_()
     with launch_scope():
         out = out if out.data_ptr() % 16 == 0 else out.clone()
+        rest = rest if rest is None or rest.data_ptr() % 16 == 0 else rest.clone()
         ws = _workspace(nbytes, q)
         _check(_lib.load().rdv_causal_attention_backward(desc, host.data_ptr(), lists.data_ptr(), grad.data_ptr(),
                                                          q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
-                                                         lse.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
-                                                         _ptr(ws), nbytes, _stream(device)),
+                                                         lse.data_ptr(), _ptr(rest), dq.data_ptr(), dk.data_ptr(),
+                                                         dv.data_ptr(), _ptr(ws), nbytes, _stream(device)),
                "causal_attention_backward")
     return dq, dk, dv

@@ -156,12 +156,12 @@ int causal_attention_plan(const rdv_causal_attention_desc& d, const int64_t* seq
                           int cu, void* plan, int64_t bytes);
 int64_t causal_attention_workspace_bytes(const rdv_causal_attention_desc& d, const void* plan, bool backward);
 int launch_causal_attention(const rdv_causal_attention_desc& d, const void* plan, const void* device_plan,
-                            const void* q, const void* k, const void* v, void* out, float* lse, void* workspace,
-                            hipStream_t stream);
+                            const void* q, const void* k, const void* v, void* out, float* lse, void* rest,
+                            void* workspace, hipStream_t stream);
 int launch_causal_attention_backward(const rdv_causal_attention_desc& d, const void* plan, const void* device_plan,
                                      const void* grad, const void* q, const void* k, const void* v, const void* out,
-                                     const float* lse, void* dq, void* dk, void* dv, void* workspace,
-                                     hipStream_t stream);
+                                     const float* lse, const void* rest, void* dq, void* dk, void* dv,
+                                     void* workspace, hipStream_t stream);
 
 static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
@@ -1005,8 +1005,8 @@ static int check_causal(const rdv_causal_attention_desc* d, bool backward) {
   const int64_t most = (int64_t(1) << 31) - 1024;
   if (d->tokens < 0 || d->states < 0 || d->tokens >= most || d->states >= most)
     return fail(RDV_ERR_INVALID, "causal attention: tokens and states must be in [0, 2^31 - 1024)");
-  if (d->heads < 1 || d->heads > (1 << 16) || d->kv_heads < 1 || d->heads % d->kv_heads != 0)
-    return fail(RDV_ERR_INVALID, "causal attention: heads must be in [1, 65536] and kv_heads must divide it");
+  if (d->heads < 1 || d->heads >= (1 << 16) || d->kv_heads < 1 || d->heads % d->kv_heads != 0)
+    return fail(RDV_ERR_INVALID, "causal attention: heads must be in [1, 65535] and kv_heads must divide it");
   if (d->dim < 1) return fail(RDV_ERR_INVALID, "causal attention: dim must be >= 1");
   if (d->dim > RDV_ATTENTION_MAX_DIM)
     return fail(RDV_ERR_UNSUPPORTED, "causal attention: dim must be at most " + std::to_string(RDV_ATTENTION_MAX_DIM));
@@ -1065,22 +1065,23 @@ static int check_causal_call(const rdv_causal_attention_desc* desc, const void* 
 }
 
 int rdv_causal_attention(const rdv_causal_attention_desc* desc, const void* plan, const void* device_plan,
-                         const void* q, const void* k, const void* v, void* out, float* lse, void* workspace,
-                         int64_t workspace_bytes, void* stream) {
+                         const void* q, const void* k, const void* v, void* out, float* lse, void* rest,
+                         void* workspace, int64_t workspace_bytes, void* stream) {
   int rc = check_causal(desc, false);
   if (rc == RDV_OK) rc = check_causal_call(desc, plan, device_plan, workspace, workspace_bytes, false);
   if (rc != RDV_OK) return rc;
   if (desc->tokens == 0) return RDV_OK;
   if (!q || !out || (desc->states > 0 && (!k || !v)))
     return fail(RDV_ERR_INVALID, "rdv_causal_attention: NULL pointer argument");
-  if (!aligned16(out)) return fail(RDV_ERR_INVALID, "rdv_causal_attention: out must be 16-byte aligned");
-  return launch_causal_attention(*desc, plan, device_plan, q, k, v, out, lse, workspace,
+  if (!aligned16(out) || !aligned16(rest))
+    return fail(RDV_ERR_INVALID, "rdv_causal_attention: out and rest must be 16-byte aligned");
+  return launch_causal_attention(*desc, plan, device_plan, q, k, v, out, lse, rest, workspace,
                                  static_cast<hipStream_t>(stream));
 }
 
 int rdv_causal_attention_backward(const rdv_causal_attention_desc* desc, const void* plan, const void* device_plan,
                                   const void* grad, const void* q, const void* k, const void* v, const void* out,
-                                  const float* lse, void* dq, void* dk, void* dv, void* workspace,
+                                  const float* lse, const void* rest, void* dq, void* dk, void* dv, void* workspace,
                                   int64_t workspace_bytes, void* stream) {
   int rc = check_causal(desc, true);
   if (rc == RDV_OK) rc = check_causal_call(desc, plan, device_plan, workspace, workspace_bytes, true);
@@ -1089,8 +1090,8 @@ int rdv_causal_attention_backward(const rdv_causal_attention_desc* desc, const v
     return fail(RDV_ERR_INVALID, "rdv_causal_attention_backward: NULL pointer argument");
   if (!aligned16(dq) || !aligned16(dk) || !aligned16(dv))
     return fail(RDV_ERR_INVALID, "rdv_causal_attention_backward: dq, dk and dv must be 16-byte aligned");
-  return launch_causal_attention_backward(*desc, plan, device_plan, grad, q, k, v, out, lse, dq, dk, dv, workspace,
-                                          static_cast<hipStream_t>(stream));
+  return launch_causal_attention_backward(*desc, plan, device_plan, grad, q, k, v, out, lse, rest, dq, dk, dv,
+                                          workspace, static_cast<hipStream_t>(stream));
 }
 
 const char* rdv_mlp_kernel_name(const rdv_mlp_desc* desc) {

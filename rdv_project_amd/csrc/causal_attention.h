@@ -43,10 +43,10 @@ struct CausalJoin {        // a tile whose results are in parts
 };
 
 struct CausalArgs {
-  const void *q, *k, *v, *g, *o;
+  const void *q, *k, *v, *g, *o, *r;   // r: rest, like o, or NULL
   const CausalItem* items;
   const CausalJoin* joins;
-  void *out, *dq, *dk, *dv;
+  void *out, *rest, *dq, *dk, *dv;     // rest (16-bit types, or NULL): what out's rounding left
   float* lse;              // [heads][tokens]
   float2* stats;           // backward: (lse log2 e, delta), [heads][tokens], by causal_dq_kernel
   float *part, *part2;     // [slot][state head][row of the tile][pdim]
@@ -162,6 +162,25 @@ __device__ __forceinline__ void causal_walk(const CausalArgs& a, const CausalAt&
 
 // ------------------------------------------------------------------ forward
 
+// Four values of an output row at `to`, and what their rounding leaves.  (A backward call that took a row's sum of dO O from O
+// as it was rounded had errors of up to 6e-3 in bf16 dQ and dK of rows that see two states, and of 2.7e-3 of long ones, where
+// rounding the results themselves makes 1.7e-3; with the rest it is 2.2e-3 to 2.5e-3.)
+template <class T>
+__device__ __forceinline__ void store_result(const CausalArgs& a, int64_t to, int d, f32x4 x) {
+  store_quad(static_cast<T*>(a.out) + to, d, a.odim, x[0], x[1], x[2], x[3]);
+  if (sizeof(T) == 2 && a.rest) {
+    f32x4 y;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      // what fp32's own rounding of the scores can make is left out: where a row sees one state, the rest is then nothing,
+      // and so are the gradients of q and k
+      y[i] = x[i] - to_f32(T(x[i]));
+      y[i] = fabsf(y[i]) > 0x1p-16f * fabsf(x[i]) ? y[i] : 0.0f;
+    }
+    store_quad(static_cast<T*>(a.rest) + to, d, a.odim, y[0], y[1], y[2], y[3]);
+  }
+}
+
 // A column's results: out and lse, or the part's sums.
 template <class T, int ND>
 __device__ __forceinline__ void causal_finish(const CausalArgs& a, const CausalAt& at, int local, int r,
@@ -185,13 +204,13 @@ __device__ __forceinline__ void causal_finish(const CausalArgs& a, const CausalA
   }
   const float inv = total > 0.0f ? 1.0f / total : (total == 0.0f ? 0.0f : total);
   const CausalRow row(a, at.hk, r);
-  T* const out = static_cast<T*>(a.out) + ((int64_t(p.token) + row.query) * a.heads + row.head) * a.odim;
+  const int64_t to = ((int64_t(p.token) + row.query) * a.heads + row.head) * a.odim;
 #pragma unroll
   for (int d = 0; d < ND; ++d)
 #pragma unroll
     for (int j = 0; j < 4; ++j)
-      store_quad(out, 32 * d + 8 * j + 4 * h, a.odim, sm.o[d][4 * j] * inv, sm.o[d][4 * j + 1] * inv,
-                 sm.o[d][4 * j + 2] * inv, sm.o[d][4 * j + 3] * inv);
+      store_result<T>(a, to, 32 * d + 8 * j + 4 * h,
+                      f32x4{sm.o[d][4 * j], sm.o[d][4 * j + 1], sm.o[d][4 * j + 2], sm.o[d][4 * j + 3]} * inv);
   if (a.lse && h == 0)
     a.lse[int64_t(row.head) * a.tokens + p.token + row.query] =
         total == 0.0f ? -INFINITY : (sm.top + __builtin_amdgcn_logf(total)) * kLn2;
@@ -425,6 +444,11 @@ __global__ __launch_bounds__(256, NC * sizeof(T) > 16 ? 1 : NC * sizeof(T) > 8 ?
     f32x16 product{};
 #pragma unroll
     for (int e = 0; e < NC; ++e) product = mma(of[e], gf[e], product);
+    if (sizeof(T) == 2 && a.r) {
+      load_frags<T, NC>(causal_ptr<T>(a.r, a.os, at.p, row), a.dim, h, of);
+#pragma unroll
+      for (int e = 0; e < NC; ++e) product = mma(of[e], gf[e], product);
+    }
 #pragma unroll
     for (int i = 0; i < 16; ++i) delta = n32 == 8 * (i >> 2) + 4 * h + (i & 3) ? product[i] : delta;
     delta = sum_halves(delta);

@@ -40,11 +40,19 @@ struct Lists {
   std::vector<CausalJoin> row_joins, key_joins;
 };
 
-// An item's work, in states or tiles of rows, for the order of the list.
-int work_of(const CausalItem& i) { return i.end - i.begin; }
+// Blocks of the kernels that run on a CU at once (their launch bounds).
+int blocks_at_once(CausalKernel which, int dtype, int dim) {
+  const int nc = dim <= 32 ? 2 : dim <= 48 ? 3 : dim <= 64 ? 4 : dim <= 80 ? 5 : dim <= 96 ? 6 : 8;
+  const int bytes = nc * element_bytes(dtype);
+  if (which == kCausalTile) return bytes > 24 ? 1 : bytes > 8 ? 2 : 4;
+  if (which == kCausalDq) return bytes > 16 ? 1 : bytes > 8 ? 2 : 3;
+  return nc > (dtype == RDV_DTYPE_F32 ? 2 : 6) ? 1 : 2;
+}
 
-// Puts an item, in parts of at most `most` (a multiple of `step`) where it is longer.
-void put(std::vector<CausalItem>& items, std::vector<CausalJoin>& joins, int32_t& slots, CausalItem item, int most) {
+// Puts an item, in parts of at most `most` (a multiple of `step`) where it is longer.  even: parts of one length, else all but
+// the last of `most`.
+void put(std::vector<CausalItem>& items, std::vector<CausalJoin>& joins, int32_t& slots, CausalItem item, int most, int step,
+         bool even) {
   const int length = item.end - item.begin;
   if (length <= most) {
     item.slot = -1;
@@ -52,24 +60,34 @@ void put(std::vector<CausalItem>& items, std::vector<CausalJoin>& joins, int32_t
     return;
   }
   const int count = (length + most - 1) / most;
-  joins.push_back(CausalJoin{item.token, item.tokens, item.state, item.states, item.tile, slots, count, 0});
-  for (int i = 0; i < count; ++i) {
+  if (even) most = ((length + count - 1) / count + step - 1) / step * step;
+  joins.push_back(CausalJoin{item.token, item.tokens, item.state, item.states, item.tile, slots, 0, 0});
+  for (int64_t first = item.begin; first < item.end; first += most) {
     CausalItem part = item;
-    part.begin = item.begin + i * most;
-    part.end = std::min(item.end, part.begin + most);
+    part.begin = int32_t(first);
+    part.end = int32_t(std::min<int64_t>(item.end, first + most));
     part.slot = slots++;
     items.push_back(part);
+    ++joins.back().count;
   }
 }
 
 // The largest part of an axis: the average share of `want` blocks, at least `least`, in steps.
 int part_size(int64_t total, int64_t want, int least, int step) {
-  const int64_t share = (total + want - 1) / want;
+  const int64_t share = std::min<int64_t>((total + want - 1) / want, 1 << 30);
   return int((std::max<int64_t>(share, least) + step - 1) / step * step);
 }
 
-void sort_items(std::vector<CausalItem>& items) {
-  std::stable_sort(items.begin(), items.end(), [](const CausalItem& a, const CausalItem& b) { return work_of(a) > work_of(b); });
+// Items in falling order of work, so that the long ones do not come last.  The first `rounds` times `per` of them begin
+// together, one of each round to a CU: every other round is turned round, so that the CUs begin with about equal sums.
+// (8,192 tokens, 8 heads on 4 of 64 in fp16: 109 -> 104.7 us, backward 318 -> 304; with neighbours paired from both ends
+// instead, as if a CU's first blocks followed one another: 135 and 396.)
+void sort_items(std::vector<CausalItem>& items, int per, int rounds) {
+  std::stable_sort(items.begin(), items.end(),
+                   [](const CausalItem& a, const CausalItem& b) { return a.end - a.begin > b.end - b.begin; });
+  const int64_t count = int64_t(items.size());
+  for (int64_t r = 1; r < rounds && r * per < count; r += 2)
+    std::reverse(items.begin() + r * per, items.begin() + std::min<int64_t>(count, (r + 1) * per));
 }
 
 Lists make_lists(const rdv_causal_attention_desc& d, const std::vector<Sequence>& seqs, bool backward, int cu) {
@@ -109,18 +127,24 @@ Lists make_lists(const rdv_causal_attention_desc& d, const std::vector<Sequence>
     const int most = part_size(few_total, 8 * int64_t(cu), 256, 128);
     std::vector<CausalItem> whole;
     whole.swap(l.few);
-    for (const CausalItem& i : whole) put(l.few, l.row_joins, h.row_slots, i, most);
+    for (const CausalItem& i : whole) put(l.few, l.row_joins, h.row_slots, i, most, 128, false);
+    sort_items(l.few, 1, 0);
   }
+  const int per = std::max(1, cu / d.kv_heads);  // items of a round: one to a CU
   {
-    // Half as many parts as blocks run at once: more cost more in partial results than they even out (2,048 tokens, 8 heads on
-    // 2 of 128 in bf16, two blocks per CU: 30.1 us, with as many parts 33.7; 8 sequences up to 4,096, 8 heads on 4 of 64 in
-    // fp16, four blocks: 90.7 us, with a quarter 95.5 and with as many 98.1).  At least 256 states, in fp32 64.
-    const int most = part_size(total, int64_t(cu) * (d.dim * element_bytes(d.dtype) > 128 ? 1 : 2), wide ? 64 : 256, 64);
-    for (const CausalItem& i : items) put(l.rows, l.row_joins, h.row_slots, i, std::max(most, 64));
+    // Parts are for tiles that would outlast the others.  Half as many as blocks run at once: more cost more in partial
+    // results than they even out (2,048 tokens, 8 heads on 2 of 128 in bf16, two blocks per CU: 30.1 us, with as many parts
+    // 33.7; 8 sequences up to 4,096, 8 heads on 4 of 64 in fp16, four blocks: 83 us, with as many parts 89).  Two blocks per
+    // CU with much to do: as many (8,192 tokens, 8 heads on 2 of 128 in bf16: 164 us, with half as many 190).  At least 256
+    // states, in fp32 64.
+    const CausalKernel which = backward ? kCausalDq : kCausalTile;
+    const int once = blocks_at_once(which, d.dtype, d.dim);
+    const int parts = once == 2 && total >= 4096 * int64_t(cu) ? 2 : std::max(1, once / 2);
+    const int most = part_size(total, int64_t(cu) * parts, wide ? 64 : 256, 64);
+    for (const CausalItem& i : items) put(l.rows, l.row_joins, h.row_slots, i, most, 64, !backward);
+    sort_items(l.rows, per, once);
   }
   if (items.empty()) h.tile_rows = 32;
-  sort_items(l.few);
-  sort_items(l.rows);
   if (backward) {
     const int rt = tile;
     blocks = 0;
@@ -140,10 +164,12 @@ Lists make_lists(const rdv_causal_attention_desc& d, const std::vector<Sequence>
       }
     }
     // As many parts as blocks run at once (the 8 sequences above: 263 us both backward kernels, with half as many 310, with
-    // twice 270; 2 x 1,024 tokens, 4 heads on 2 of 64 in fp32: 71.7, with twice as many 81).
-    const int most = part_size(total, int64_t(cu) * (wide || d.dim > 96 ? 1 : 2), wide ? 1 : 2, 1);
-    for (const CausalItem& i : items) put(l.keys, l.key_joins, h.key_slots, i, most);
-    sort_items(l.keys);
+    // twice 270; 2 x 1,024 tokens, 4 heads on 2 of 64 in fp32: 71.7, with twice as many 81).  Parts of one length lost: the
+    // short rests fill the gaps (the 8 sequences: 254 -> 269).
+    const int once = blocks_at_once(kCausalDkv, d.dtype, d.dim);
+    const int most = part_size(total, int64_t(cu) * once, wide ? 1 : 2, 1);
+    for (const CausalItem& i : items) put(l.keys, l.key_joins, h.key_slots, i, most, 1, false);
+    sort_items(l.keys, per, once);
   }
   for (const CausalJoin& j : l.row_joins) {
     h.join_rows = std::max(h.join_rows, std::min(h.tile_rows, j.tokens * share - j.tile));
@@ -200,8 +226,8 @@ bool in_place(const rdv_causal_attention_desc& d, const int64_t (&s)[2], int64_t
 
 struct Layout {
   int dim, pdim;          // dimensions rounded up to 16 bytes, to 4
-  bool packed[5];         // q, k, v, grad, out: whether the kernels read a copy
-  int64_t packs[5], stats, part, part2, ml, bytes;
+  bool packed[6];         // q, k, v, grad, out, rest: whether the kernels read a copy
+  int64_t packs[6], stats, part, part2, ml, bytes;
 };
 
 Layout make_layout(const rdv_causal_attention_desc& d, const Header& h) {
@@ -215,8 +241,9 @@ Layout make_layout(const rdv_causal_attention_desc& d, const Header& h) {
   p.packed[2] = !in_place(d, d.v_stride, d.states, d.kv_heads);
   p.packed[3] = h.backward && !in_place(d, d.g_stride, d.tokens, d.heads);
   p.packed[4] = h.backward && !in_place(d, out, d.tokens, d.heads);
+  p.packed[5] = p.packed[4] && d.dtype != RDV_DTYPE_F32;
   int64_t at = 0;
-  for (int i = 0; i < 5; ++i) {
+  for (int i = 0; i < 6; ++i) {
     p.packs[i] = at;
     const bool k = i == 1 || i == 2;
     if (p.packed[i]) at += align256((k ? d.states * d.kv_heads : d.tokens * d.heads) * p.dim * element_bytes(d.dtype));
@@ -293,8 +320,7 @@ __global__ __launch_bounds__(256) void causal_join_kernel(CausalArgs a, int per)
   if (!on) return;
   const float inv = total > 0.0f ? 1.0f / total : (total == 0.0f ? 0.0f : total);
   const CausalRow row(a, hk, r);
-  T* const out = static_cast<T*>(a.out) + ((int64_t(j.token) + row.query) * a.heads + row.head) * a.odim;
-  store_quad(out, 4 * l, a.odim, o4[0] * inv, o4[1] * inv, o4[2] * inv, o4[3] * inv);
+  store_result<T>(a, ((int64_t(j.token) + row.query) * a.heads + row.head) * a.odim, 4 * l, o4 * inv);
   if (a.lse && l == 0)
     a.lse[int64_t(row.head) * a.tokens + j.token + row.query] =
         total == 0.0f ? -INFINITY : (top + __builtin_amdgcn_logf(total)) * kLn2;
@@ -435,7 +461,8 @@ int64_t causal_attention_workspace_bytes(const rdv_causal_attention_desc& d, con
 }
 
 int launch_causal_attention(const rdv_causal_attention_desc& d, const void* plan, const void* device_plan, const void* q,
-                            const void* k, const void* v, void* out, float* lse, void* workspace, hipStream_t stream) {
+                            const void* k, const void* v, void* out, float* lse, void* rest, void* workspace,
+                            hipStream_t stream) {
   Header h;
   int rc = read_header(d, plan, false, h);
   if (rc != RDV_OK) return rc;
@@ -449,6 +476,7 @@ int launch_causal_attention(const rdv_causal_attention_desc& d, const void* plan
   if (rc == RDV_OK) rc = input(d, p, 2, v, d.v_stride, d.states, d.kv_heads, ws, &a.v, a.vs, stream);
   if (rc != RDV_OK) return rc;
   a.out = out;
+  a.rest = rest;
   a.lse = lse;
   a.tile_rows = h.tile_rows;
   a.part = reinterpret_cast<float*>(ws + p.part);
@@ -467,7 +495,8 @@ int launch_causal_attention(const rdv_causal_attention_desc& d, const void* plan
 
 int launch_causal_attention_backward(const rdv_causal_attention_desc& d, const void* plan, const void* device_plan,
                                      const void* grad, const void* q, const void* k, const void* v, const void* out,
-                                     const float* lse, void* dq, void* dk, void* dv, void* workspace, hipStream_t stream) {
+                                     const float* lse, const void* rest, void* dq, void* dk, void* dv, void* workspace,
+                                     hipStream_t stream) {
   Header h;
   int rc = read_header(d, plan, true, h);
   if (rc != RDV_OK) return rc;
@@ -481,6 +510,7 @@ int launch_causal_attention_backward(const rdv_causal_attention_desc& d, const v
   if (rc == RDV_OK) rc = input(d, p, 2, v, d.v_stride, d.states, d.kv_heads, ws, &a.v, a.vs, stream);
   if (rc == RDV_OK) rc = input(d, p, 3, grad, d.g_stride, d.tokens, d.heads, ws, &a.g, a.gs, stream);
   if (rc == RDV_OK) rc = input(d, p, 4, out, os, d.tokens, d.heads, ws, &a.o, a.os, stream);
+  if (rc == RDV_OK && rest && d.dtype != RDV_DTYPE_F32) rc = input(d, p, 5, rest, os, d.tokens, d.heads, ws, &a.r, a.os, stream);
   if (rc != RDV_OK) return rc;
   a.lse = const_cast<float*>(lse);
   a.stats = reinterpret_cast<float2*>(ws + p.stats);

@@ -73,26 +73,28 @@ __device__ __forceinline__ int block_count(int v, int* red) {
   return t;
 }
 
-// Four tokens of a lane, -1 past the end.
+// Four tokens of a lane, -1 for those of no row of the vocabulary and past the end.  Without a branch, so that several steps'
+// loads are in flight together: the last lanes read the last four tokens, of which those at `from` and later are theirs.
 template <class I>
 struct TokenPiece {
   typedef I vec __attribute__((ext_vector_type(4)));
   typedef vec loose __attribute__((aligned(sizeof(I))));
-  int t[4];
-  // tokens of no row of the vocabulary become -1
-  __device__ __forceinline__ void load(const EmbedArgs& a, int64_t i) {
-    vec v;
-    if (i + 4 <= a.n) {
-      v = *reinterpret_cast<const loose*>(static_cast<const I*>(a.tokens) + i);
+  vec v;
+  int64_t at;  // of the first
+  __device__ __forceinline__ void load(const EmbedArgs& a, int64_t from) {
+    const I* const tokens = static_cast<const I*>(a.tokens);
+    if (a.n >= 4) {
+      at = min(from, a.n - 4);
+      v = *reinterpret_cast<const loose*>(tokens + at);
     } else {
+      at = 0;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) v[j] = i + j < a.n ? static_cast<const I*>(a.tokens)[i + j] : I(-1);
+      for (int j = 0; j < 4; ++j) v[j] = j < a.n ? tokens[j] : I(-1);
     }
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const I x = v[j];
-      t[j] = x >= 0 && x < a.vocab ? int(x) : -1;
-    }
+  }
+  __device__ __forceinline__ int token(const EmbedArgs& a, int64_t from, int j) const {
+    const I x = v[j];
+    return x >= 0 && x < a.vocab && at + j >= from ? int(x) : -1;
   }
 };
 
@@ -123,8 +125,8 @@ __global__ __launch_bounds__(kSortThreads) void embed_sort_kernel(EmbedArgs a) {
       for (int k = 0; k < kAhead; ++k)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const int t = p[k].t[j];
-          f(t, t >= 0 && (t & low) == block, int(i0) + 256 * k + 4 * lane + j);
+          const int t = p[k].token(a, i0 + 256 * k < last ? i0 + 256 * k + 4 * lane : a.n, j);
+          f(t, t >= 0 && (t & low) == block, int(p[k].at) + j);
         }
     }
   };
@@ -278,35 +280,43 @@ __global__ __launch_bounds__(256) void embed_rows_kernel(EmbedArgs a) {
   }
 }
 
-// Chunk by chunk: the long run that begins in it.
+// Chunk by chunk and slice by slice: the long run that begins in it, its parts shared by the block's groups.
 template <class T, int G>
 __global__ __launch_bounds__(256) void embed_join_kernel(EmbedArgs a) {
   typedef RowPiece<T> P;
+  constexpr int kGroups = 256 / G;
+  __shared__ __attribute__((aligned(16))) float sums[kGroups][G * P::E];
   const int lane = int(threadIdx.x) % G, group = int(threadIdx.x) / G;
-  const uint32_t task = blockIdx.x * (256 / G) + group, chunk = a.slices == 1 ? task : task / uint32_t(a.slices);
-  const int d = (int(task - chunk * a.slices) * G + lane) * P::E, count = a.begin[a.range << a.bits];
-  if (d >= a.dim || int64_t(chunk) * kLong >= count) return;
+  const uint32_t chunk = a.slices == 1 ? blockIdx.x : blockIdx.x / uint32_t(a.slices);
+  const int d = (int(blockIdx.x - chunk * a.slices) * G + lane) * P::E, count = a.begin[a.range << a.bits];
+  if (int64_t(chunk) * kLong >= count) return;
   const int last = min(int(chunk) * kLong + kLong, count), t = a.token[last - 1], at = a.slot(t);
   const int b = a.begin[at], e = a.begin[at + 1];
   if (e - b <= kLong || b < int(chunk) * kLong) return;
   const int more = (e - 1) / kLong - int(chunk);  // chunks after this one
-  const float* part = a.part + (int64_t(chunk) * 2 + 1) * a.pdim + d;
-  float sum[P::E];
-#pragma unroll
-  for (int i = 0; i < P::E; ++i) sum[i] = part[i];
-  part += a.pdim;  // the next chunks' first places
-#pragma unroll 8
-  for (int c = 0; c < more; ++c) {
+  // its own part is the chunk's second one, the others are their chunks' first ones
+  const float* const part = a.part + (int64_t(chunk) * 2 + 1) * a.pdim + (d < a.dim ? d : 0);
+  float sum[P::E] = {};
+#pragma unroll 4
+  for (int c = group; c <= more; c += kGroups) {
 #pragma unroll
     for (int i = 0; i < P::E; i += 4) {
-      const f32x4 v = *reinterpret_cast<const f32x4*>(part + int64_t(c) * 2 * a.pdim + i);
+      const f32x4 v = *reinterpret_cast<const f32x4*>(part + (int64_t(c) * 2 - (c > 0)) * a.pdim + i);
 #pragma unroll
       for (int j = 0; j < 4; ++j) sum[i + j] += v[j];
     }
   }
+#pragma unroll
+  for (int i = 0; i < P::E; ++i) sums[group][lane * P::E + i] = sum[i];
+  __syncthreads();
+  if (group != 0 || d >= a.dim) return;
   P o;
 #pragma unroll
-  for (int i = 0; i < P::E; ++i) o.set(i, sum[i] * a.scale);
+  for (int i = 0; i < P::E; ++i) {
+    float v = sum[i];
+    for (int g = 1; g < kGroups; ++g) v += sums[g][lane * P::E + i];
+    o.set(i, v * a.scale);
+  }
   o.store(static_cast<T*>(a.out) + int64_t(t) * a.dim, d, a.dim);
 }
 
@@ -403,7 +413,7 @@ int launch_embedding_backward(const rdv_embedding_desc& d, const void* grad, con
       embed_rows_kernel<T, G><<<unsigned(chunks + blocks(rows)), 256, 0, stream>>>(a);
       RDV_HIP_TRY(hipGetLastError());
       if (chunks > 0) {
-        embed_join_kernel<T, G><<<unsigned(chunks), 256, 0, stream>>>(a);
+        embed_join_kernel<T, G><<<unsigned(p.chunks * a.slices), 256, 0, stream>>>(a);
         RDV_HIP_TRY(hipGetLastError());
       }
       return int(RDV_OK);

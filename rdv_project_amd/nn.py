@@ -21,13 +21,14 @@ TensorOperation nodes dispatch eagerly, one kernel per op:
   ConcatTensorOp                 nn.py:1128-1150
 Build-defined additions (no reference counterpart): FrequencyEncoding, Softplus,
 Sigmoid, DensityRGB, and the image networks' GroupNormTensorOp,
-CrossAttentionTensorOp and DropoutTensorOp.
+CrossAttentionTensorOp and DropoutTensorOp, and the prompt's encoder's
+EmbeddingTensorOp, RMSNormTensorOp and CausalAttentionTensorOp.
 """
 from __future__ import annotations
 
 import torch
 
-from . import _conv, _image_ops, _lib, _tensor_ops
+from . import _conv, _image_ops, _lib, _prompt_ops, _tensor_ops
 from .core import RDVObject, wrap
 from .maths import Map, TensorOperation, _as_op_input
 
@@ -674,3 +675,91 @@ class DropoutTensorOp(TensorOperation):
         x, p, seed, subsequence = _image_ops._dropout_inputs(self.x_buf, self.p, self.seed, self.subsequence)
         residual = None if self.residual_buf is None else self.residual_buf.as_tensor("torch")
         _image_ops._dropout_into(x, p, seed, subsequence, residual, self._result_t, _image_ops._gpu_index())
+
+
+# ------------------------------------------------- a prompt's encoder (build-defined)
+
+class EmbeddingTensorOp(TensorOperation):
+    """scale * weight[token] for tokens [rows] (int32 or int64; a row of zeros
+    outside [0, vocab)) from weight [vocab, C].  result [rows, C] fp32.
+    evaluate() reads the tokens again.  embedding is the form for other types and
+    training."""
+
+    _TILE_ROWS = 1
+    _TILE_COLS = 1
+
+    def __init__(self, tokens, weight, scale: float = 1.0) -> None:
+        self.tokens_buf, self.weight = wrap(_prompt_ops._tokens(tokens)), wrap(weight)
+        self.scale = float(scale)
+        tokens, weight = self._inputs()
+        assert tokens.dim() == 1, "EmbeddingTensorOp requires tokens [rows]"
+        self._upstream = None
+        super().__init__([tokens.shape[0], weight.shape[1]])
+
+    def _inputs(self):
+        tokens, weight = _prompt_ops._embedding_inputs(self.tokens_buf, self.weight)
+        if weight.dtype != torch.float32:
+            raise TypeError(f"weight must be float32, got {weight.dtype}")
+        return tokens, weight
+
+    def _forward(self) -> None:
+        _prompt_ops._embedding_into(*self._inputs(), self.scale, self._result_t, _image_ops._gpu_index())
+
+
+class RMSNormTensorOp(TensorOperation):
+    """weight * x / sqrt(mean(x^2) + eps) over the rows of x [rows, C] (a buffer or
+    an upstream TensorOperation), weight [C] or None.  result [rows, C] fp32.
+    rms_norm is the form with a residual, for other types and training."""
+
+    _TILE_ROWS = 1
+    _TILE_COLS = 1
+
+    def __init__(self, x, weight, eps: float = 1e-6) -> None:
+        data, shape, upstream = _as_op_input(x)
+        assert len(shape) == 2, "RMSNormTensorOp requires a 2D (rows, C) input"
+        self.x_buf, self.eps = _op_float32(data, "x"), float(eps)
+        self.weight = None if weight is None else weight if isinstance(weight, RDVObject) else wrap(_float32(weight))
+        _prompt_ops._rms_inputs(self.x_buf, self.weight)  # checked before anything is allocated
+        self._upstream = upstream
+        super().__init__(shape)
+
+    def _forward(self) -> None:
+        x, weight = _prompt_ops._rms_inputs(self.x_buf, self.weight)
+        _prompt_ops._rms_norm_into(x, weight, None, self.eps, self._result_t, None, None, None, _image_ops._gpu_index())
+
+
+class CausalAttentionTensorOp(TensorOperation):
+    """softmax(q k^T / sqrt(D)) v per head within packed sequences, each token
+    seeing itself and what is before it, from q [rows, heads * D], k and v [states,
+    kv_heads * D] (kv_heads defaults to heads and divides it; D at most 128); each
+    input a buffer or an upstream TensorOperation; sequences: PackedSequences (one
+    of all rows by default).  result [rows, heads * D] fp32; rows behind the last
+    sequence are 0.  causal_attention is the form for other types and training."""
+
+    _TILE_ROWS = 1
+    _TILE_COLS = 1
+
+    def __init__(self, q, k, v, heads: int, kv_heads: int | None = None, sequences=None) -> None:
+        (qd, qs, qu), (kd, ks, ku), (vd, vs, vu) = _as_op_input(q), _as_op_input(k), _as_op_input(v)
+        kv_heads = heads if kv_heads is None else kv_heads
+        assert len(qs) == 2 and len(ks) == 2 and ks == vs, \
+            "CausalAttentionTensorOp requires 2D (rows, heads * D) inputs, k and v of one shape"
+        assert heads >= 1 and kv_heads >= 1 and heads % kv_heads == 0, \
+            f"kv_heads ({kv_heads}) must divide heads ({heads})"
+        assert qs[1] % heads == 0, f"q's channels ({qs[1]}) must be a multiple of heads ({heads})"
+        dim = qs[1] // heads
+        assert ks[1] == kv_heads * dim, f"k and v must have kv_heads * {dim} = {kv_heads * dim} channels, got {ks[1]}"
+        self.q_buf, self.k_buf, self.v_buf = _op_float32(qd, "q"), _op_float32(kd, "k"), _op_float32(vd, "v")
+        self.heads, self.kv_heads, self.D = int(heads), int(kv_heads), int(dim)
+        self.sequences = _prompt_ops.PackedSequences([qs[0]], [ks[0]]) if sequences is None else sequences
+        ups = [u for u in (qu, ku, vu) if u is not None]
+        self._upstream = ups[0] if ups else None
+        self._extra_upstreams = tuple(ups[1:])
+        super().__init__(qs)
+
+    def _forward(self) -> None:
+        q, k, v = (t.as_tensor("torch").unflatten(1, (h, self.D)) for t, h in
+                   ((self.q_buf, self.heads), (self.k_buf, self.kv_heads), (self.v_buf, self.kv_heads)))
+        q, k, v, _, call, device = _prompt_ops._causal_inputs(q, k, v, self.sequences, None)
+        self._result_t[self.sequences.tokens:].zero_()
+        _prompt_ops._causal_attention_into(call, q, k, v, self._result_t, None, None, device)
