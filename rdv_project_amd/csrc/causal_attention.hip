@@ -132,14 +132,14 @@ Lists make_lists(const rdv_causal_attention_desc& d, const std::vector<Sequence>
   }
   const int per = std::max(1, cu / d.kv_heads);  // items of a round: one to a CU
   {
-    // Parts are for tiles that would outlast the others.  Half as many as blocks run at once: more cost more in partial
+    // Parts are for tiles that would outlast the others.  Half as many as blocks run at once (rounded up): more cost more in partial
     // results than they even out (2,048 tokens, 8 heads on 2 of 128 in bf16, two blocks per CU: 30.1 us, with as many parts
     // 33.7; 8 sequences up to 4,096, 8 heads on 4 of 64 in fp16, four blocks: 83 us, with as many parts 89).  Two blocks per
     // CU with much to do: as many (8,192 tokens, 8 heads on 2 of 128 in bf16: 164 us, with half as many 190).  At least 256
     // states, in fp32 64.
     const CausalKernel which = backward ? kCausalDq : kCausalTile;
     const int once = blocks_at_once(which, d.dtype, d.dim);
-    const int parts = once == 2 && total >= 4096 * int64_t(cu) ? 2 : std::max(1, once / 2);
+    const int parts = once == 2 && total >= 4096 * int64_t(cu) ? 2 : (once + 1) / 2;
     const int most = part_size(total, int64_t(cu) * parts, wide ? 64 : 256, 64);
     for (const CausalItem& i : items) put(l.rows, l.row_joins, h.row_slots, i, most, 64, !backward);
     sort_items(l.rows, per, once);

@@ -12,6 +12,8 @@
 //     of such a chunk is summed into the workspace.
 //   * embed_join_kernel: adds up the pieces of the long runs.
 // Bound: HBM, the rows of grad that are read and the whole vocabulary's that are written.
+#include <type_traits>
+
 #include "rows.h"
 
 namespace rdv {
@@ -73,32 +75,14 @@ __device__ __forceinline__ int block_count(int v, int* red) {
   return t;
 }
 
-// Four tokens of a lane, -1 for those of no row of the vocabulary and past the end.  Without a branch, so that several steps'
-// loads are in flight together: the last lanes read the last four tokens, of which those at `from` and later are theirs.
+// A token as a row of the vocabulary, -1 outside it.
 template <class I>
-struct TokenPiece {
-  typedef I vec __attribute__((ext_vector_type(4)));
-  typedef vec loose __attribute__((aligned(sizeof(I))));
-  vec v;
-  int64_t at;  // of the first
-  __device__ __forceinline__ void load(const EmbedArgs& a, int64_t from) {
-    const I* const tokens = static_cast<const I*>(a.tokens);
-    if (a.n >= 4) {
-      at = min(from, a.n - 4);
-      v = *reinterpret_cast<const loose*>(tokens + at);
-    } else {
-      at = 0;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) v[j] = j < a.n ? tokens[j] : I(-1);
-    }
-  }
-  __device__ __forceinline__ int token(const EmbedArgs& a, int64_t from, int j) const {
-    const I x = v[j];
-    return x >= 0 && x < a.vocab && at + j >= from ? int(x) : -1;
-  }
-};
+__device__ __forceinline__ int known(I x, int vocab) {
+  typedef typename std::make_unsigned<I>::type U;
+  return U(x) < U(vocab) ? int(x) : -1;
+}
 
-// Waves take contiguous parts of the tokens, 256 at a step; a run is in the order (wave, step, token of a lane, lane).
+// Waves take contiguous parts of the tokens; a run is in the order in which its wave comes to them.
 // count[wave][row] becomes where the wave puts its next token of the row.  A wave lists its tokens as it counts them, so that
 // it need not look for them again; with more than kSortList it does.
 template <class I>
@@ -115,33 +99,37 @@ __global__ __launch_bounds__(kSortThreads) void embed_sort_kernel(EmbedArgs a) {
   int* const mine = count + wave * a.range;
   int2* const list = lists[wave];
   int below = 0, found = 0;
-  // f(tokens of the lanes, their own ones, position of the lane's) for every token of the lanes in turn
+  // f(token, position) for every token of the lanes in turn, four of a lane at a step; the last ones one by one
   const auto walk = [&](auto f) {
-    for (int64_t i0 = first; i0 < last; i0 += 256 * kAhead) {
-      TokenPiece<I> p[kAhead];
+    typedef I vec __attribute__((ext_vector_type(4)));
+    typedef vec loose __attribute__((aligned(sizeof(I))));
+    const I* const tokens = static_cast<const I*>(a.tokens);
+    int64_t i0 = first;
+    for (; i0 + 256 * kAhead <= last; i0 += 256 * kAhead) {
+      vec v[kAhead];
 #pragma unroll
-      for (int k = 0; k < kAhead; ++k) p[k].load(a, i0 + 256 * k < last ? i0 + 256 * k + 4 * lane : a.n);
+      for (int k = 0; k < kAhead; ++k) v[k] = *reinterpret_cast<const loose*>(tokens + i0 + 256 * k + 4 * lane);
 #pragma unroll
       for (int k = 0; k < kAhead; ++k)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int t = p[k].token(a, i0 + 256 * k < last ? i0 + 256 * k + 4 * lane : a.n, j);
-          f(t, t >= 0 && (t & low) == block, int(p[k].at) + j);
-        }
+        for (int j = 0; j < 4; ++j) f(known<I>(v[k][j], a.vocab), int(i0) + 256 * k + 4 * lane + j);
     }
+    for (; i0 < last; i0 += 64) f(i0 + lane < last ? known<I>(tokens[i0 + lane], a.vocab) : -1, int(i0) + lane);
   };
-  walk([&](int t, bool own, int at) {
-    below += t >= 0 && (t & low) < block;
-    const uint64_t all = __ballot(own);
+  walk([&](int t, int at) {
+    const int to = t & low;
+    const uint64_t valid = __ballot(t >= 0);
+    below += __popcll(__ballot(to < block) & valid);
+    const uint64_t all = __ballot(to == block) & valid;
     if (!all) return;
-    if (own) {
+    if ((all >> lane) & 1) {
       atomicAdd(&mine[t >> a.bits], 1);
       const int q = found + __popcll(all & ((uint64_t(1) << lane) - 1));
       if (q < kSortList) list[q] = int2{t, at};
     }
     found += __popcll(all);
   });
-  const int base = block_count(below, red);  // with a barrier: the counts are whole
+  const int base = block_count(lane == 0 ? below : 0, red);  // with a barrier: the counts are whole
   // exclusive sums over (row, wave), a run of rows per thread
   const int each = (a.range + kSortThreads - 1) / kSortThreads;
   int total = 0;
@@ -188,7 +176,7 @@ __global__ __launch_bounds__(kSortThreads) void embed_sort_kernel(EmbedArgs a) {
     }
   };
   if (found > kSortList) {
-    walk(place);
+    walk([&](int t, int at) { place(t, t >= 0 && (t & low) == block, at); });
     return;
   }
   for (int i = lane; i - lane < found; i += 64) {

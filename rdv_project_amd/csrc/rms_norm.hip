@@ -79,18 +79,26 @@ __global__ __launch_bounds__(block_threads<G>()) void rms_norm_kernel(RmsArgs a)
       w[k][i] = d < a.width ? (a.weight ? a.weight[d] : 1.0f) : 0.0f;
     }
   int slot = 0;
-  for (int64_t row = int64_t(blockIdx.x) * kGroups + int(threadIdx.x) / G; row < a.rows;
-       row += int64_t(gridDim.x) * kGroups) {
-    P h[K];
-    const T* const x = static_cast<const T*>(a.x) + row * a.x_row;
+  // a row's loads are in flight under the work on the one before it
+  P x[K], r[K];
+  const auto load = [&](int64_t row) {
+    if (row >= a.rows) return;
 #pragma unroll
-    for (int k = 0; k < K; ++k) h[k].load(x, (k * G + lane) * E, a.width);
+    for (int k = 0; k < K; ++k) x[k].load(static_cast<const T*>(a.x) + row * a.x_row, (k * G + lane) * E, a.width);
     if (a.residual) {
-      P r[K];
-      const T* const res = static_cast<const T*>(a.residual) + row * a.r_row;
-      T* const sum = static_cast<T*>(a.sum) + row * a.width;
 #pragma unroll
-      for (int k = 0; k < K; ++k) r[k].load(res, (k * G + lane) * E, a.width);
+      for (int k = 0; k < K; ++k) r[k].load(static_cast<const T*>(a.residual) + row * a.r_row, (k * G + lane) * E, a.width);
+    }
+  };
+  const int64_t step = int64_t(gridDim.x) * kGroups;
+  int64_t row = int64_t(blockIdx.x) * kGroups + int(threadIdx.x) / G;
+  load(row);
+  for (; row < a.rows; row += step) {
+    P h[K];
+#pragma unroll
+    for (int k = 0; k < K; ++k) h[k] = x[k];
+    if (a.residual) {
+      T* const sum = static_cast<T*>(a.sum) + row * a.width;
 #pragma unroll
       for (int k = 0; k < K; ++k) {
 #pragma unroll
@@ -98,6 +106,7 @@ __global__ __launch_bounds__(block_threads<G>()) void rms_norm_kernel(RmsArgs a)
         h[k].store(sum, (k * G + lane) * E, a.width);
       }
     }
+    load(row + step);
     float sq = 0.0f, top = 0.0f;
 #pragma unroll
     for (int k = 0; k < K; ++k)
@@ -168,21 +177,35 @@ __global__ __launch_bounds__(block_threads<G>()) void rms_norm_back_kernel(RmsAr
       dw[k][i] = 0.0f;
     }
   int slot = 0;
-  for (int64_t row = int64_t(blockIdx.x) * kGroups + group; row < a.rows; row += int64_t(gridDim.x) * kGroups) {
-    P h[K], g[K], s[K];
-    const T* const hr = static_cast<const T*>(a.x) + row * a.x_row;
-    const T* const gr = static_cast<const T*>(a.grad) + row * a.g_row;
-    const float rstd = a.stats[row];
+  // a row's loads are in flight under the work on the one before it
+  P nh[K], ng[K], ns[K];
+  float next = 0.0f;
+  const auto load = [&](int64_t row) {
+    if (row >= a.rows) return;
+    next = a.stats[row];
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      h[k].load(hr, (k * G + lane) * E, a.width);
-      g[k].load(gr, (k * G + lane) * E, a.width);
+      nh[k].load(static_cast<const T*>(a.x) + row * a.x_row, (k * G + lane) * E, a.width);
+      ng[k].load(static_cast<const T*>(a.grad) + row * a.g_row, (k * G + lane) * E, a.width);
     }
     if (a.grad_sum) {
-      const T* const sr = static_cast<const T*>(a.grad_sum) + row * a.s_row;
 #pragma unroll
-      for (int k = 0; k < K; ++k) s[k].load(sr, (k * G + lane) * E, a.width);
+      for (int k = 0; k < K; ++k) ns[k].load(static_cast<const T*>(a.grad_sum) + row * a.s_row, (k * G + lane) * E, a.width);
     }
+  };
+  const int64_t step = int64_t(gridDim.x) * kGroups;
+  int64_t row = int64_t(blockIdx.x) * kGroups + group;
+  load(row);
+  for (; row < a.rows; row += step) {
+    P h[K], g[K], s[K];
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      h[k] = nh[k];
+      g[k] = ng[k];
+      s[k] = ns[k];
+    }
+    const float rstd = next;
+    load(row + step);
     float dot = 0.0f;
 #pragma unroll
     for (int k = 0; k < K; ++k)
@@ -334,7 +357,7 @@ __global__ __launch_bounds__(256) void rms_norm_zero_kernel(float* p, int n) {
   if (i < n) p[i] = 0.0f;
 }
 
-struct Shape {
+struct Shape {  // threads that share a row (0: a block that reads it twice), pieces of each
   int group, each;
   bool wide() const { return group == 0; }
   int row_groups() const { return group == 0 || group > 256 ? 1 : 256 / group; }  // of a block
@@ -342,14 +365,16 @@ struct Shape {
 
 // Threads that share a row and pieces of each: as few threads as hold the row in four pieces each, so that a wave has a row
 // to itself without barriers, and as many as there are pieces while the rows alone do not fill the chip.
-Shape shape_of(int64_t rows, int width, int dtype, int cu) {
+Shape shape_of(int64_t rows, int width, int dtype, bool backward, int cu) {
   const int e = dtype == RDV_DTYPE_F32 ? 4 : 8, pieces = (width + e - 1) / e;
   for (int g = 8; g <= 64; g *= 2)
     if (pieces <= g) return Shape{g, 1};
-  if (pieces <= 256 && rows > 4 * int64_t(cu)) return Shape{64, pieces <= 128 ? 2 : 4};
+  const int most = backward && e == 8 ? 2 : 4;  // pieces of a thread: backward it has a weight and a sum for every channel
+  if (pieces <= 64 * most && rows > 4 * int64_t(cu)) return Shape{64, pieces <= 128 ? 2 : 4};
   if (pieces <= 256) return Shape{256, 1};
   if (pieces <= 512) return Shape{256, 2};
-  if (pieces <= 1024) return Shape{256, 4};
+  if (pieces <= 256 * most) return Shape{256, 4};
+  if (pieces <= 1024) return Shape{1024, 1};
   if (pieces <= 2048) return Shape{1024, 2};
   if (pieces <= 4096) return Shape{1024, 4};
   return Shape{0, 0};
@@ -360,7 +385,7 @@ int blocks_of(int64_t rows, const Shape& s, int per_cu, int cu) {
   return int(std::min<int64_t>(want, int64_t(cu) * (s.row_groups() == 1 && s.group != 256 ? std::max(1, per_cu / 4) : per_cu)));
 }
 
-constexpr int kForwardBlocks = 8, kBackwardBlocks = 4;  // per CU, of 256 threads
+constexpr int kForwardBlocks = 6, kBackwardBlocks = 3;  // per CU, of 256 threads
 
 template <class F>
 auto with_shape(const Shape& s, F&& f) {
@@ -375,6 +400,7 @@ auto with_shape(const Shape& s, F&& f) {
   RDV_SHAPE(256, 1)
   RDV_SHAPE(256, 2)
   RDV_SHAPE(256, 4)
+  RDV_SHAPE(1024, 1)
   RDV_SHAPE(1024, 2)
 #undef RDV_SHAPE
   return f(std::integral_constant<int, 1024>{}, std::integral_constant<int, 4>{});
@@ -384,7 +410,7 @@ auto with_shape(const Shape& s, F&& f) {
 
 int64_t rms_norm_workspace_bytes(const rdv_rms_norm_desc& d, int cu) {
   if (d.rows == 0) return 0;
-  return int64_t(blocks_of(d.rows, shape_of(d.rows, d.width, d.dtype, cu), kBackwardBlocks, cu)) * d.width * 4;
+  return int64_t(blocks_of(d.rows, shape_of(d.rows, d.width, d.dtype, true, cu), kBackwardBlocks, cu)) * d.width * 4;
 }
 
 int launch_rms_norm(const rdv_rms_norm_desc& d, const void* x, const void* residual, const float* weight, void* sum, void* y,
@@ -402,7 +428,7 @@ int launch_rms_norm(const rdv_rms_norm_desc& d, const void* x, const void* resid
   a.r_row = d.r_row_stride;
   a.width = d.width;
   a.eps = d.eps;
-  const Shape s = shape_of(d.rows, d.width, d.dtype, cu);
+  const Shape s = shape_of(d.rows, d.width, d.dtype, false, cu);
   const unsigned blocks = unsigned(blocks_of(d.rows, s, kForwardBlocks, cu));
   with_dtype(d.dtype, [&](auto t) {
     using T = decltype(t);
@@ -413,7 +439,8 @@ int launch_rms_norm(const rdv_rms_norm_desc& d, const void* x, const void* resid
     }
     with_shape(s, [&](auto g, auto k) {
       constexpr int G = decltype(g)::value, K = decltype(k)::value;
-      if (scales) rms_norm_kernel<T, G, K, true><<<blocks, block_threads<G>(), 0, stream>>>(a);
+      if constexpr (G == 1024 && K == 1) return;  // backward only
+      else if (scales) rms_norm_kernel<T, G, K, true><<<blocks, block_threads<G>(), 0, stream>>>(a);
       else rms_norm_kernel<T, G, K, false><<<blocks, block_threads<G>(), 0, stream>>>(a);
     });
   });
@@ -442,7 +469,7 @@ int launch_rms_norm_backward(const rdv_rms_norm_desc& d, const void* grad, const
   a.g_row = d.g_row_stride;
   a.s_row = d.s_row_stride;
   a.width = d.width;
-  const Shape s = shape_of(d.rows, d.width, d.dtype, cu);
+  const Shape s = shape_of(d.rows, d.width, d.dtype, true, cu);
   const int blocks = blocks_of(d.rows, s, kBackwardBlocks, cu);
   with_dtype(d.dtype, [&](auto t) {
     using T = decltype(t);
@@ -452,7 +479,8 @@ int launch_rms_norm_backward(const rdv_rms_norm_desc& d, const void* grad, const
     }
     with_shape(s, [&](auto g, auto k) {
       constexpr int G = decltype(g)::value, K = decltype(k)::value;
-      rms_norm_back_kernel<T, G, K><<<unsigned(blocks), block_threads<G>(), 0, stream>>>(a);
+      if constexpr (sizeof(T) == 4 || G == 1024 || K < 4)  // see shape_of
+        rms_norm_back_kernel<T, G, K><<<unsigned(blocks), block_threads<G>(), 0, stream>>>(a);
     });
   });
   RDV_HIP_TRY(hipGetLastError());
