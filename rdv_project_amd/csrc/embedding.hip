@@ -21,7 +21,7 @@ namespace rdv {
 namespace {
 
 constexpr int kSortThreads = 1024, kSortWaves = kSortThreads / 64;
-constexpr int kSortList = 224;  // tokens that a wave lists: with the counts below 64 KiB
+constexpr int kSortList = 448;  // tokens that a wave lists: with the counts below 64 KiB
 constexpr int kSortRows = 512;  // tokens of the vocabulary per block, at most: 32 KiB of counts
 constexpr int kLong = 32;
 
@@ -82,54 +82,74 @@ __device__ __forceinline__ int known(I x, int vocab) {
   return U(x) < U(vocab) ? int(x) : -1;
 }
 
-// Waves take contiguous parts of the tokens; a run is in the order in which its wave comes to them.
+// A run is in the order (wave, step), and in that in which a wave comes to the tokens of a step.
 // count[wave][row] becomes where the wave puts its next token of the row.  A wave lists its tokens as it counts them, so that
 // it need not look for them again; with more than kSortList it does.
 template <class I>
 __global__ __launch_bounds__(kSortThreads) void embed_sort_kernel(EmbedArgs a) {
   extern __shared__ int count[];  // [kSortWaves][range]
   __shared__ int red[kSortWaves], wave_sum[kSortWaves];
-  __shared__ int2 lists[kSortWaves][kSortList];  // (token, position)
+  __shared__ int lists[kSortWaves][kSortList];  // positions
   constexpr int kAhead = 4;  // steps whose loads are in flight together
   const int tid = int(threadIdx.x), lane = tid & 63, wave = tid >> 6;
   const int block = int(blockIdx.x), low = (1 << a.bits) - 1;
   for (int i = tid; i < kSortWaves * a.range; i += kSortThreads) count[i] = 0;
   __syncthreads();
-  const int64_t per = (a.n + kSortWaves * 256 - 1) / (kSortWaves * 256) * 256, first = wave * per, last = min(first + per, a.n);
+  constexpr int kStep = kSortWaves * 256;  // tokens of the block's step, 256 of a wave
+  const int steps = int(a.n / kStep);
+  const auto at_step = [&](int i) { return int64_t(i) * kStep + wave * 256 + 4 * lane; };
   int* const mine = count + wave * a.range;
-  int2* const list = lists[wave];
+  int* const list = lists[wave];
   int below = 0, found = 0;
-  // f(token, position) for every token of the lanes in turn, four of a lane at a step; the last ones one by one
+  typedef I vec __attribute__((ext_vector_type(4)));
+  typedef vec loose __attribute__((aligned(sizeof(I))));
+  const I* const tokens = static_cast<const I*>(a.tokens);
+  // f(four tokens of the lane, the first one's position) over the wave's part: -1 outside the vocabulary
   const auto walk = [&](auto f) {
-    typedef I vec __attribute__((ext_vector_type(4)));
-    typedef vec loose __attribute__((aligned(sizeof(I))));
-    const I* const tokens = static_cast<const I*>(a.tokens);
-    int64_t i0 = first;
-    for (; i0 + 256 * kAhead <= last; i0 += 256 * kAhead) {
+    const auto step = [&](const vec& v, int at) {
+      int t[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) t[j] = known<I>(v[j], a.vocab);
+      f(t, at);
+    };
+    int i = 0;
+    for (; i + kAhead <= steps; i += kAhead) {
       vec v[kAhead];
 #pragma unroll
-      for (int k = 0; k < kAhead; ++k) v[k] = *reinterpret_cast<const loose*>(tokens + i0 + 256 * k + 4 * lane);
+      for (int k = 0; k < kAhead; ++k) v[k] = *reinterpret_cast<const loose*>(tokens + at_step(i + k));
 #pragma unroll
-      for (int k = 0; k < kAhead; ++k)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) f(known<I>(v[k][j], a.vocab), int(i0) + 256 * k + 4 * lane + j);
+      for (int k = 0; k < kAhead; ++k) step(v[k], int(at_step(i + k)));
     }
-    for (; i0 < last; i0 += 64) f(i0 + lane < last ? known<I>(tokens[i0 + lane], a.vocab) : -1, int(i0) + lane);
+    for (; i < steps; ++i) step(*reinterpret_cast<const loose*>(tokens + at_step(i)), int(at_step(i)));
+    const int64_t rest = at_step(steps);
+    vec v;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = rest + j < a.n ? tokens[rest + j] : I(-1);
+    step(v, int(rest));
   };
-  walk([&](int t, int at) {
-    const int to = t & low;
-    const uint64_t valid = __ballot(t >= 0);
-    below += __popcll(__ballot(to < block) & valid);
-    const uint64_t all = __ballot(to == block) & valid;
-    if (!all) return;
-    if ((all >> lane) & 1) {
-      atomicAdd(&mine[t >> a.bits], 1);
-      const int q = found + __popcll(all & ((uint64_t(1) << lane) - 1));
-      if (q < kSortList) list[q] = int2{t, at};
+  // A token's block, from its low bits; the sign stays, so that a -1 is of none and before none.
+  const uint32_t bits = uint32_t(low) | 0x80000000u;
+  walk([&](const int (&t)[4], int at) {
+    uint32_t other[4];  // 0: the block's own
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t of = uint32_t(t[j]) & bits;
+      below += of < uint32_t(block);
+      other[j] = of ^ uint32_t(block);
     }
-    found += __popcll(all);
+    if (!__any(min(min(other[0], other[1]), min(other[2], other[3])) == 0)) return;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint64_t all = __ballot(other[j] == 0);
+      if (other[j] == 0) {
+        atomicAdd(&mine[t[j] >> a.bits], 1);
+        const int q = found + __popcll(all & ((uint64_t(1) << lane) - 1));
+        if (q < kSortList) list[q] = at + j;
+      }
+      found += __popcll(all);
+    }
   });
-  const int base = block_count(lane == 0 ? below : 0, red);  // with a barrier: the counts are whole
+  const int base = block_count(below, red);  // with a barrier: the counts are whole
   // exclusive sums over (row, wave), a run of rows per thread
   const int each = (a.range + kSortThreads - 1) / kSortThreads;
   int total = 0;
@@ -176,12 +196,15 @@ __global__ __launch_bounds__(kSortThreads) void embed_sort_kernel(EmbedArgs a) {
     }
   };
   if (found > kSortList) {
-    walk([&](int t, int at) { place(t, t >= 0 && (t & low) == block, at); });
+    walk([&](const int (&t)[4], int at) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) place(t[j], t[j] >= 0 && (t[j] & low) == block, at + j);
+    });
     return;
   }
   for (int i = lane; i - lane < found; i += 64) {
-    const int2 v = i < found ? list[i] : int2{-1, 0};
-    place(v.x, i < found, v.y);
+    const int at = i < found ? list[i] : 0;
+    place(i < found ? int(tokens[at]) : -1, i < found, at);
   }
 }
 
