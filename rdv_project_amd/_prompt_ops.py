@@ -282,6 +282,9 @@ def rms_norm_backward(grad, h, weight, stats, grad_sum=None, grads=None):
 # ------------------------------------------------------------ causal attention
 
 
+_CAPTURED: list = []  # lists of work that graphs read
+
+
 class PackedSequences:
     """Sequences packed one after the other, for causal_attention: sequence s is
     lengths[s] rows of q, after those of the sequences before it, and states[s] rows
@@ -294,7 +297,8 @@ class PackedSequences:
     It holds the lists of work that the kernels take, made on the host at the first
     call of each kind (heads, dimensions, type, direction) on each GPU and copied
     there: keep it for all layers and steps on sequences of these lengths.  That
-    first call waits for the copy, and cannot be captured into a graph."""
+    first call waits for the copy, and cannot be captured into a graph.  Lists that a
+    graph has captured are kept until the process ends."""
 
     def __init__(self, lengths, states=None, starts=None) -> None:
         self.lengths = _counts(lengths, "lengths")
@@ -324,7 +328,8 @@ class PackedSequences:
         return len(self.lengths)
 
     def _plan(self, d, backward: bool, device: int):
-        """(the list of work in host memory, the same on the GPU) for calls of this kind."""
+        """(the list of work in host memory, the same on the GPU, the stream that it was allocated on) for calls of this
+        kind."""
         key = d.heads, d.kv_heads, d.dim, d.dtype, backward, device
         hit = self._plans.get(key)
         if hit is not None:
@@ -336,25 +341,33 @@ class PackedSequences:
         host = torch.empty(nbytes, dtype=torch.uint8)
         _check(lib.rdv_causal_attention_plan(C.byref(d), self._rows, n, backward, host.data_ptr(), nbytes),
                "causal_attention")
-        hit = self._plans[key] = host, host.to(f"cuda:{device}")  # a synchronous copy: any stream may read it
-        return hit
+        lists = host.to(f"cuda:{device}")  # a synchronous copy: any stream may read it
+        return self._plans.setdefault(key, (host, lists, _stream(device)))  # another thread may have been first
 
     def _call(self, layout, device: int):
         """What a call on tensors of this layout (_causal_desc's arguments) needs: (descriptor, reference to it, list of
         work in host memory, on the GPU, workspace bytes)."""
         hit = self._calls.get((layout, device))
-        if hit is not None:
-            return hit
+        if hit is None:
+            hit = self._plan_call(layout, device)
+        # The list's memory outlives what reads it: the launches of streams other than its own, and a graph's replays.
+        if hit[5] != _stream(device):
+            hit[3].record_stream(torch.cuda.current_stream())
+        if torch.cuda.is_current_stream_capturing() and not any(hit[3] is t for t in _CAPTURED):
+            _CAPTURED.append(hit[3])
+        return hit[:5]
+
+    def _plan_call(self, layout, device: int):
         d = _causal_desc(*layout)
         assert self.tokens <= d.tokens, f"the sequences have {self.tokens} tokens, q {d.tokens} rows"
         assert self.total_states <= d.states, f"the sequences have {self.total_states} states, k and v {d.states} rows"
         backward = layout[6] is not None
-        host, lists = self._plan(d, backward, device)
+        host, lists, stream = self._plan(d, backward, device)
         nbytes = _bytes(_lib.load().rdv_causal_attention_workspace_bytes(C.byref(d), host.data_ptr(), backward),
                         "causal_attention")
         if len(self._calls) >= 256:  # of changing strides or scales: their plans stay
             self._calls.clear()
-        hit = self._calls[layout, device] = d, C.byref(d), host, lists, nbytes
+        hit = self._calls[layout, device] = d, C.byref(d), host, lists, nbytes, stream
         return hit
 
 

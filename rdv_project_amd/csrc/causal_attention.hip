@@ -136,7 +136,7 @@ Lists make_lists(const rdv_causal_attention_desc& d, const std::vector<Sequence>
     // results than they even out (2,048 tokens, 8 heads on 2 of 128 in bf16, two blocks per CU: 30.1 us, with as many parts
     // 33.7; 8 sequences up to 4,096, 8 heads on 4 of 64 in fp16, four blocks: 83 us, with as many parts 89).  Two blocks per
     // CU with much to do: as many (8,192 tokens, 8 heads on 2 of 128 in bf16: 164 us, with half as many 190).  At least 256
-    // states, in fp32 64.
+    // states, in fp32 64 (32, a tile of more than 64 dimensions: 2,000 tokens, 4 heads of 128 87 us instead of 66).
     const CausalKernel which = backward ? kCausalDq : kCausalTile;
     const int once = blocks_at_once(which, d.dtype, d.dim);
     const int parts = once == 2 && total >= 4096 * int64_t(cu) ? 2 : (once + 1) / 2;

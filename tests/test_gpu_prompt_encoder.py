@@ -160,3 +160,43 @@ def test_streams():
             assert all(map(torch.equal, g, want))
     finally:
         rdv.set_synchronous(prev)
+
+
+def test_plans_outlive_their_sequences():
+    """A graph's replays, and another stream's launches, read the list of work of PackedSequences that are gone."""
+    q = torch.randn(300, 4, 32).cuda()
+    want = rdv.causal_attention(q, q, q, rdv.PackedSequences((100, 200)))
+    prev = rdv.set_synchronous(False)
+    try:
+        def spoil():  # what the allocator hands out next
+            for n in (512, 1024, 2048, 4096):
+                torch.full((8, n), 0x7f, dtype=torch.uint8, device="cuda")
+
+        seqs = rdv.PackedSequences((100, 200))
+        rdv.causal_attention(q, q, q, seqs)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = rdv.causal_attention(q, q, q, seqs)
+        kept = {t.data_ptr() for t in rdv._prompt_ops._CAPTURED}
+        assert all(lists.data_ptr() in kept for _, lists, _ in seqs._plans.values())
+        del seqs
+        for _ in range(3):
+            spoil()
+            out.zero_()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, want)
+        side = torch.cuda.Stream()
+        for _ in range(20):
+            seqs = rdv.PackedSequences((100, 200))
+            rdv.causal_attention(q, q, q, seqs)
+            side.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(side):
+                out = rdv.causal_attention(q, q, q, seqs)
+            del seqs
+            spoil()
+            torch.cuda.synchronize()
+            assert torch.equal(out, want)
+    finally:
+        rdv.set_synchronous(prev)
