@@ -248,3 +248,31 @@ def test_rounding_of_out_stays_out_of_the_gradients(dtype, length):
     for got, want in ((dq, ds @ b), (dk, ds.transpose(2, 3).contiguous() @ a)):
         want = want.transpose(1, 2).reshape(got.shape)
         assert (got.double() - want).norm() <= 1.01 * u * 2 ** 0.5 * want.norm()
+
+
+def test_rows_far_apart():
+    """Rows 2^25 bytes apart, which are copied before they are read."""
+    base = torch.randn(5, 1 << 23, generator=torch.Generator().manual_seed(3)).cuda()
+    q, k, v, g = (base[:, at:at + 128].unflatten(1, (2, 64)) for at in (0, 128, 256, 384))
+    _check(rdv.PackedSequences((3, 2)), q, k, v, g, "f32", what="far")
+    stats = rdv.causal_attention(q, k, v, rdv.PackedSequences((3, 2)), return_lse=True)
+    near = rdv.causal_attention(*(t.contiguous() for t in (q, k, v)), rdv.PackedSequences((3, 2)), return_lse=True)
+    assert torch.equal(stats[0], near[0]) and torch.equal(stats[1].lse, near[1].lse)
+
+
+def test_offsets_past_32_bits():
+    """A cache of more than 2^31 elements; sequences at its end."""
+    n = 1 << 21
+    cache = torch.empty(n + 300, 8, 128, dtype=torch.bfloat16, device="cuda")
+    tail = cache[n:]
+    tail.copy_(torch.randn(300, 8, 128, generator=torch.Generator().manual_seed(4)))
+    q = torch.randn(102, 16, 128, generator=torch.Generator().manual_seed(5)).to(torch.bfloat16).cuda()
+    far = rdv.PackedSequences((1, 100, 1), (200, 100, 0), (n, n + 200, 0))
+    near = rdv.PackedSequences((1, 100, 1), (200, 100, 0), (0, 200, 0))
+    out, stats = rdv.causal_attention(q, cache, cache, far, return_lse=True)
+    want, wstats = rdv.causal_attention(q, tail, tail, near, return_lse=True)
+    assert torch.equal(out, want) and torch.equal(stats.lse, wstats.lse)
+    grads = [torch.empty_like(q), torch.empty_like(cache), torch.empty_like(cache)]
+    got = rdv.causal_attention_backward(q, q, cache, cache, out, stats, far, grads=grads)
+    ref = rdv.causal_attention_backward(q, q, tail, tail, want, wstats, near)
+    assert torch.equal(got[0], ref[0]) and torch.equal(got[1][n:], ref[1]) and torch.equal(got[2][n:], ref[2])

@@ -129,3 +129,18 @@ def test_infinities_stay_with_their_tokens():
     weight = torch.ones(4, 8).cuda()
     weight[0] = float("nan")
     assert not rdv.embedding(t, weight)[4].any()  # an unknown token reads no row
+
+
+def test_offsets_past_32_bits():
+    """A table of more than 2^31 elements."""
+    vocab = (1 << 21) + 10
+    table = torch.empty(vocab, 1024, dtype=torch.bfloat16, device="cuda")
+    table[-20:] = torch.randn(20, 1024)
+    tokens = (torch.arange(40, device="cuda") % 25 + vocab - 20).to(torch.int32)
+    y = rdv.embedding(tokens, table)
+    known = tokens < vocab
+    assert torch.equal(y[known], table[tokens[known].long()]) and not y[~known].any()
+    grad = torch.randn(40, 1024).to(torch.bfloat16).cuda()
+    small = rdv.embedding_backward(grad, tokens - (vocab - 20), 20)
+    dw = rdv.embedding_backward(grad, tokens, vocab, out=table)
+    assert torch.equal(dw[-20:], small) and not dw[:-20].any()

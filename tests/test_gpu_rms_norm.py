@@ -176,3 +176,17 @@ def test_gradients_by_differences():
             moved[at] += sign * step
             ends.append(loss(moved, w) if t is x else loss(x, moved))
         assert abs((ends[0] - ends[1]) / (2 * step) - grad[at]) < 1e-5 * (1 + abs(grad[at]))
+
+
+def test_offsets_past_32_bits():
+    """The last rows of more than 2^31 elements, the others zeros, which add nothing to dweight."""
+    rows = (1 << 21) + 5
+    x = torch.zeros(rows, 1024, dtype=torch.bfloat16, device="cuda")
+    x[-5:] = torch.randn(5, 1024)
+    w = torch.rand(1024).cuda()
+    y, stats = rdv.rms_norm(x, w, return_stats=True)
+    dx, dw = rdv.rms_norm_backward(y, x, w, stats)
+    assert not y[:-5].any() and not dx[:-5].any()
+    ref = O.rms_norm(_np(x[-5:]), _np(w), 1e-6, "bf16", _np(y[-5:]))
+    for got, name in ((y[-5:], "y"), (stats[-5:], "stats"), (dx[-5:], "dx"), (dw, "dweight")):
+        _close(got, ref[name], ref[name + "_err"], name)
