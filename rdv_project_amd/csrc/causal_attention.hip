@@ -49,18 +49,14 @@ int blocks_at_once(CausalKernel which, int dtype, int dim) {
   return nc > (dtype == RDV_DTYPE_F32 ? 2 : 6) ? 1 : 2;
 }
 
-// Puts an item, in parts of at most `most` (a multiple of `step`) where it is longer.  even: parts of one length, else all but
-// the last of `most`.
-void put(std::vector<CausalItem>& items, std::vector<CausalJoin>& joins, int32_t& slots, CausalItem item, int most, int step,
-         bool even) {
-  const int length = item.end - item.begin;
-  if (length <= most) {
+// Puts an item, in parts of `most` where it is longer.  (The short rest fills a gap: with parts of one length, 8,192 tokens, 8
+// heads on 2 of 128 in bf16, took 184 us instead of 162, and the backward call on the 8 sequences below 281 instead of 269.)
+void put(std::vector<CausalItem>& items, std::vector<CausalJoin>& joins, int32_t& slots, CausalItem item, int most) {
+  if (item.end - item.begin <= most) {
     item.slot = -1;
     items.push_back(item);
     return;
   }
-  const int count = (length + most - 1) / most;
-  if (even) most = ((length + count - 1) / count + step - 1) / step * step;
   joins.push_back(CausalJoin{item.token, item.tokens, item.state, item.states, item.tile, slots, 0, 0});
   for (int64_t first = item.begin; first < item.end; first += most) {
     CausalItem part = item;
@@ -127,22 +123,27 @@ Lists make_lists(const rdv_causal_attention_desc& d, const std::vector<Sequence>
     const int most = part_size(few_total, 8 * int64_t(cu), 256, 128);
     std::vector<CausalItem> whole;
     whole.swap(l.few);
-    for (const CausalItem& i : whole) put(l.few, l.row_joins, h.row_slots, i, most, 128, false);
+    for (const CausalItem& i : whole) put(l.few, l.row_joins, h.row_slots, i, most);
     sort_items(l.few, 1, 0);
   }
   const int per = std::max(1, cu / d.kv_heads);  // items of a round: one to a CU
   {
-    // Parts are for tiles that would outlast the others.  Half as many as blocks run at once (rounded up): more cost more in partial
-    // results than they even out (2,048 tokens, 8 heads on 2 of 128 in bf16, two blocks per CU: 30.1 us, with as many parts
-    // 33.7; 8 sequences up to 4,096, 8 heads on 4 of 64 in fp16, four blocks: 83 us, with as many parts 89).  Two blocks per
-    // CU with much to do: as many (8,192 tokens, 8 heads on 2 of 128 in bf16: 164 us, with half as many 190).  At least 256
-    // states, in fp32 64 (32, a tile of more than 64 dimensions: 2,000 tokens, 4 heads of 128 87 us instead of 66).
+    // Parts are for tiles that would outlast the others; more of them cost more in partial results than they even out.  So
+    // there are about as many as half of the blocks that run at once (us):
+    //                                                              a CU's  0.8   1.3   1.7   2.5 times that
+    //   8 sequences up to 4,096, 8 heads on 4 of 64, fp16, 4 at once:   86    93    86    91    96
+    //   1 x 4,096, 8 heads on 4 of 64, fp16, 4 at once:                 43    45    49    50    58
+    //   1 x 4,096, 8 heads on 2 of 128, bf16, 2 at once:                68    74    59    60    74
+    //   1 x 2,000, 4 heads of 128, fp32, one at a time:                 67    75    82    84    90
+    // and a quarter more where two run at once; with much to do there as many as run (1 x 8,192, 8 heads on 2 of 128, bf16: 162
+    // us, with half as many 183, with 1.3 times as many 180).  At least 256 states, in fp32 64 (32, a tile of more than 64
+    // dimensions: 2,000 tokens, 4 heads of 128 87 us instead of 66).
     const CausalKernel which = backward ? kCausalDq : kCausalTile;
-    const int once = blocks_at_once(which, d.dtype, d.dim);
-    const int parts = once == 2 && total >= 4096 * int64_t(cu) ? 2 : (once + 1) / 2;
-    const int most = part_size(total, int64_t(cu) * parts, wide ? 64 : 256, 64);
-    for (const CausalItem& i : items) put(l.rows, l.row_joins, h.row_slots, i, most, 64, !backward);
-    sort_items(l.rows, per, once);
+    const int64_t once = blocks_at_once(which, d.dtype, d.dim);
+    const int64_t want = once != 2 ? cu * ((once + 1) / 2) : total >= 4096 * int64_t(cu) ? 2 * cu : cu * 5 / 4;
+    const int most = part_size(total, want, wide ? 64 : 256, 64);
+    for (const CausalItem& i : items) put(l.rows, l.row_joins, h.row_slots, i, most);
+    sort_items(l.rows, per, int(once));
   }
   if (items.empty()) h.tile_rows = 32;
   if (backward) {
@@ -163,12 +164,11 @@ Lists make_lists(const rdv_causal_attention_desc& d, const std::vector<Sequence>
         total += int64_t(n) * share * d.kv_heads;
       }
     }
-    // As many parts as blocks run at once (the 8 sequences above: 263 us both backward kernels, with half as many 310, with
-    // twice 270; 2 x 1,024 tokens, 4 heads on 2 of 64 in fp32: 71.7, with twice as many 81).  Parts of one length lost: the
-    // short rests fill the gaps (the 8 sequences: 254 -> 269).
+    // As many parts as blocks run at once (the 8 sequences: 269 us both backward kernels, with 0.6, 1.3 and 2.5 times as many
+    // 293, 281 and 284; 1 x 8,192 of 64: 322, 362, 370, 345; 1 x 2,000 in fp32: 187, 227, 240, 223).
     const int once = blocks_at_once(kCausalDkv, d.dtype, d.dim);
     const int most = part_size(total, int64_t(cu) * once, wide ? 1 : 2, 1);
-    for (const CausalItem& i : items) put(l.keys, l.key_joins, h.key_slots, i, most, 1, false);
+    for (const CausalItem& i : items) put(l.keys, l.key_joins, h.key_slots, i, most);
     sort_items(l.keys, per, once);
   }
   for (const CausalJoin& j : l.row_joins) {
