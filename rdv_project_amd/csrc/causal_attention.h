@@ -216,7 +216,10 @@ __device__ __forceinline__ void causal_finish(const CausalArgs& a, const CausalA
         total == 0.0f ? -INFINITY : (sm.top + __builtin_amdgcn_logf(total)) * kLn2;
 }
 
-// Many rows: a block of 4 waves, 32 rows each (or 64 rows shared by pairs of waves), as attn_tile_kernel.
+// Many rows: a block of 4 waves, 32 rows each (or 64 rows shared by pairs of waves), as attn_tile_kernel.  Bound: a SIMD's
+// vector and matrix instructions add up (of 64 dimensions in fp16 56 and 30% of the cycles, of 128 in bf16 50 and 54%).
+//   16,384 tokens, 16 heads on 4 of 128, bf16: 1.00 to 1.07 ms, 1.03 to 1.10 PFLOP/s (an 8,192^3 product: 1.13 to 1.18)
+//   8 sequences up to 4,096 tokens, 8 heads on 4 of 64, fp16: 80 us, 0.67 PFLOP/s (such a product: 1.06 to 1.13)
 template <class T, int NC, int WK>
 __global__ __launch_bounds__(256, NC * sizeof(T) > 24 ? 1 : NC * sizeof(T) > 8 ? 2 : 4) void causal_tile_kernel(CausalArgs a) {
   using G = AttnTile<T, NC>;
@@ -310,6 +313,7 @@ __global__ __launch_bounds__(256, NC * sizeof(T) > 24 ? 1 : NC * sizeof(T) > 8 ?
 }
 
 // At most 32 rows of a sequence: a single token's heads, or few tokens.  The waves split the states, as attn_few_kernel.
+// Bound: HBM.  16 tokens against 2,000 to 32,000 states, 16 heads on 4 of 128, bf16: 125 us for 569 MB, 4.5 TB/s.
 template <class T, int NC>
 __global__ __launch_bounds__(256, NC * sizeof(T) > 16 ? 1 : 2) void causal_few_kernel(CausalArgs a) {
   using G = AttnTile<T, NC>;
@@ -414,7 +418,8 @@ __global__ __launch_bounds__(256, NC * sizeof(T) > 16 ? 1 : 2) void causal_few_k
 
 // ------------------------------------------------------------------ backward
 
-// dQ, and each row's (lse, delta) for causal_dkv_kernel; as attn_dq_kernel.
+// dQ, and each row's (lse, delta) for causal_dkv_kernel; as attn_dq_kernel.  The 8 sequences above: 105 us, 0.76 PFLOP/s of its
+// three products; vector and matrix instructions take 50 and 36% of the cycles.
 template <class T, int NC, int WK>
 __global__ __launch_bounds__(256, NC * sizeof(T) > 16 ? 1 : NC * sizeof(T) > 8 ? 2 : 3) void causal_dq_kernel(CausalArgs a) {
   using G = AttnTile<T, NC>;
@@ -540,7 +545,9 @@ __global__ __launch_bounds__(256, NC * sizeof(T) > 16 ? 1 : NC * sizeof(T) > 8 ?
 
 // dK and dV: a block of 4 waves, 32 states each (WR = 2: pairs of waves share 32 states and take a half of each tile), goes
 // over the tokens that see any of them, head by head of those that share the state head, in tiles of RT tokens of one head:
-// tile t is the t % n-th of the t / n-th head, n tiles from token `from` on.  As attn_dkv_kernel.
+// tile t is the t % n-th of the t / n-th head, n tiles from token `from` on.  As attn_dkv_kernel.  The 8 sequences above: 145
+// us, 0.74 PFLOP/s of its four products (37 and 32% of the cycles: two waves per SIMD do not cover its LDS reads).  Three
+// waves, whose registers spill, took 203 us; both halves of a tile's scores before the first one's terms made no difference.
 template <class T, int NC, int WR>
 __global__ __launch_bounds__(256, NC > (sizeof(T) == 4 ? 2 : 6) ? 1 : 2) void causal_dkv_kernel(CausalArgs a) {
   using G = AttnTile<T, NC>;

@@ -11,7 +11,15 @@
 //     one without tokens is written as zeros.  Longer runs are cut at multiples of kLong of the sorted list: a run's piece
 //     of such a chunk is summed into the workspace.
 //   * embed_join_kernel: adds up the pieces of the long runs.
-// Bound: HBM, the rows of grad that are read and the whole vocabulary's that are written.
+// Bound: HBM, the rows of grad that are read and the whole vocabulary's that are written.  64 x 1,024 tokens, five in eight of
+// them known and the most frequent one 6% of those, of 50,000 x 1,024 in bf16 (a 2 GiB copy: 4.8 to 5.1 TB/s):
+//   embed_kernel       39 us for 183 MB, 4.7 TB/s
+//   embed_sort_kernel  18 us (4,096 tokens 6.5, 262,144 47: 26 bytes a cycle and CU), by the instructions per token of each
+//                      block: tokens begin at other places in each block made no difference.  With ranges of neighbouring
+//                      tokens per block, as frequent ones are, it took 190 us
+//   embed_rows_kernel  51 us for 194 MB, 3.8 TB/s: three loads that wait for one another, four rows of a wave at once (one
+//                      row at a time 69 us)
+//   embed_join_kernel  5.5 us
 #include <type_traits>
 
 #include "rows.h"
