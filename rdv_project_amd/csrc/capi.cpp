@@ -921,7 +921,7 @@ static int check_embedding(const rdv_embedding_desc* d, bool backward) {
   if (d->vocab < 1 || d->dim < 1) return fail(RDV_ERR_INVALID, "embedding: vocab and dim must be >= 1");
   if (d->tokens > (int64_t(1) << 30) || d->vocab > (1 << 25) || d->dim > (1 << 20))
     return fail(RDV_ERR_UNSUPPORTED, "embedding: at most 2^30 tokens, 2^25 rows and 2^20 dimensions");
-  // threads of a launch are counted in 32 bits: one for every 8 bytes of dweight, and of a 64th of grad
+  // blocks are counted in 32 bits
   if (backward && (int64_t(d->vocab) + d->tokens / 64 + 1) * (d->dim + 255) > (int64_t(1) << 33))
     return fail(RDV_ERR_UNSUPPORTED, "embedding: too large a gradient");
   if (d->dtype < RDV_DTYPE_F32 || d->dtype > RDV_DTYPE_BF16) return fail(RDV_ERR_INVALID, "embedding: unknown dtype");

@@ -44,6 +44,7 @@ struct EmbedArgs {
   int64_t n, w_row, g_row;
   int vocab, dim, pdim, range, bits;  // range: tokens of a block of the sort; bits: log2 of its blocks
   int slices, chunk_blocks;           // waves that share a row's pieces; blocks of embed_rows_kernel that take chunks
+  uint32_t block0;                    // of this launch
   float scale;
   __device__ __forceinline__ int slot(int token) const { return (token & ((1 << bits) - 1)) * range + (token >> bits); }
 };
@@ -249,8 +250,9 @@ __global__ __launch_bounds__(256) void embed_rows_kernel(EmbedArgs a) {
   typedef RowPiece<T> P;
   const int lane = int(threadIdx.x) % G;
   const int group = G == 64 ? __builtin_amdgcn_readfirstlane(int(threadIdx.x) >> 6) : int(threadIdx.x) / G;
-  const bool rows = int(blockIdx.x) >= a.chunk_blocks;
-  const uint32_t task = (blockIdx.x - (rows ? a.chunk_blocks : 0)) * (256 / G) + group;
+  const uint32_t at_block = a.block0 + blockIdx.x;
+  const bool rows = at_block >= uint32_t(a.chunk_blocks);
+  const uint32_t task = (at_block - (rows ? a.chunk_blocks : 0)) * (256 / G) + group;
   const uint32_t item = a.slices == 1 ? task : task / uint32_t(a.slices);
   const int d = (int(task - item * a.slices) * G + lane) * P::E;  // past dim: lanes that only hand places round, and read for nothing
   const bool on = d < a.dim;
@@ -306,8 +308,8 @@ __global__ __launch_bounds__(256) void embed_join_kernel(EmbedArgs a) {
   constexpr int kGroups = 256 / G;
   __shared__ __attribute__((aligned(16))) float sums[kGroups][G * P::E];
   const int lane = int(threadIdx.x) % G, group = int(threadIdx.x) / G;
-  const uint32_t chunk = a.slices == 1 ? blockIdx.x : blockIdx.x / uint32_t(a.slices);
-  const int d = (int(blockIdx.x - chunk * a.slices) * G + lane) * P::E, count = a.begin[a.range << a.bits];
+  const uint32_t task = a.block0 + blockIdx.x, chunk = a.slices == 1 ? task : task / uint32_t(a.slices);
+  const int d = (int(task - chunk * a.slices) * G + lane) * P::E, count = a.begin[a.range << a.bits];
   if (int64_t(chunk) * kLong >= count) return;
   const int last = min(int(chunk) * kLong + kLong, count), t = a.token[last - 1], at = a.slot(t);
   const int b = a.begin[at], e = a.begin[at + 1];
@@ -429,13 +431,15 @@ int launch_embedding_backward(const rdv_embedding_desc& d, const void* grad, con
       const int64_t chunks = d.tokens > kLong ? blocks(p.chunks) : 0;
       a.chunk_blocks = int(chunks);
       const int64_t rows = ((int64_t(p.range) << p.bits) + kRows - 1) / kRows;
-      embed_rows_kernel<T, G><<<unsigned(chunks + blocks(rows)), 256, 0, stream>>>(a);
-      RDV_HIP_TRY(hipGetLastError());
-      if (chunks > 0) {
-        embed_join_kernel<T, G><<<unsigned(p.chunks * a.slices), 256, 0, stream>>>(a);
-        RDV_HIP_TRY(hipGetLastError());
-      }
-      return int(RDV_OK);
+      const int rc = launch_blocks(chunks + blocks(rows), 256, [&](int64_t first, unsigned count) {
+        a.block0 = uint32_t(first);
+        embed_rows_kernel<T, G><<<count, 256, 0, stream>>>(a);
+      });
+      if (rc != RDV_OK || chunks == 0) return rc;
+      return launch_blocks(p.chunks * a.slices, 256, [&](int64_t first, unsigned count) {
+        a.block0 = uint32_t(first);
+        embed_join_kernel<T, G><<<count, 256, 0, stream>>>(a);
+      });
     });
   });
 }

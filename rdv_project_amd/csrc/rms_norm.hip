@@ -260,8 +260,8 @@ __global__ __launch_bounds__(block_threads<G>()) void rms_norm_back_kernel(RmsAr
   }
 }
 
-// Rows wider than a block's registers: a block per row, which reads it twice, element by element.  Sums are fp64: a thread takes many values
-// one after the other.
+// Rows wider than a block's registers: a block per row, which reads it twice, element by element.  Sums are fp64: a thread
+// takes many values one after the other.
 __device__ __forceinline__ double block_sum(double v, double* red) {
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);

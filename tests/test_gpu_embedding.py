@@ -144,3 +144,15 @@ def test_offsets_past_32_bits():
     small = rdv.embedding_backward(grad, tokens - (vocab - 20), 20)
     dw = rdv.embedding_backward(grad, tokens, vocab, out=table)
     assert torch.equal(dw[-20:], small) and not dw[:-20].any()
+
+
+def test_the_most_tokens():
+    """2^30 of them: more threads than one launch takes."""
+    n, vocab = 1 << 30, 1000
+    tokens = torch.arange(n, dtype=torch.int32, device="cuda").remainder_(vocab)
+    grad = torch.ones(n, 1, dtype=torch.float16, device="cuda")
+    dw = rdv.embedding_backward(grad, tokens, vocab, scale=2.0 ** -8)
+    # runs of 2^30 // vocab or one more ones, whose sums are exact in float32 (below 2^24)
+    runs = torch.full((vocab, 1), n // vocab, device="cuda")
+    runs[:n % vocab] += 1
+    assert torch.equal(dw, (runs.float() * 2.0 ** -8).half())

@@ -190,3 +190,20 @@ def test_offsets_past_32_bits():
     ref = O.rms_norm(_np(x[-5:]), _np(w), 1e-6, "bf16", _np(y[-5:]))
     for got, name in ((y[-5:], "y"), (stats[-5:], "stats"), (dx[-5:], "dx"), (dw, "dweight")):
         _close(got, ref[name], ref[name + "_err"], name)
+
+
+@pytest.mark.parametrize("width", [64, 777, 4096, 33000])
+def test_eight_bits_with_statistics(width):
+    """What a call returns beside 8 bits is what it returns beside y, and its values are y's."""
+    x, r = torch.randn(5, width).half().cuda(), torch.randn(5, width).half().cuda()
+    w = (1 + 0.1 * torch.randn(width)).cuda()
+    y, h, stats = rdv.rms_norm(x, w, residual=r, return_stats=True)
+    buffers = torch.empty(5, width, dtype=torch.float8_e4m3fn, device="cuda"), torch.empty(5, device="cuda")
+    (values, scales), h8, stats8 = rdv.rms_norm(x, w, residual=r, return_stats=True, eight_bits=True, out=buffers)
+    assert values is buffers[0] and scales is buffers[1]
+    assert torch.equal(h8, h) and torch.equal(stats8, stats)
+    # y is rounded by 2^-11 and the value by 2^-4, or by half of e4m3's smallest step (2^-10) times the scale
+    back, y = values.double() * scales.double()[:, None], y.double()
+    assert ((back - y).abs() <= y.abs() * (2.0 ** -4 + 2.0 ** -10) + scales.double()[:, None] * 2.0 ** -10 + 2.0 ** -25).all()
+    (values, scales), stats8 = rdv.rms_norm(x, w, return_stats=True, eight_bits=True)
+    assert torch.equal(stats8, rdv.rms_norm(x, w, return_stats=True)[1])
