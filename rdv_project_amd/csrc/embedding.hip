@@ -7,19 +7,20 @@
 //     have neighbouring numbers, so spread over the blocks) and goes over all tokens twice: it counts its own, and those of
 //     the blocks before it (which tells where its part of the sorted list begins, without a word from them), then puts its
 //     own in place.  The tokens stay in the L2.
-//   * embed_rows_kernel: a row of the vocabulary with up to kLong tokens is summed by the lanes that share it and written,
-//     one without tokens is written as zeros.  Longer runs are cut at multiples of kLong of the sorted list: a run's piece
+//   * embed_rows_kernel: a row of the vocabulary with up to a.run tokens is summed by the lanes that share it and written,
+//     one without tokens is written as zeros.  Longer runs are cut at multiples of that of the sorted list: a run's piece
 //     of such a chunk is summed into the workspace.
 //   * embed_join_kernel: adds up the pieces of the long runs.
 // Bound: HBM, the rows of grad that are read and the whole vocabulary's that are written.  64 x 1,024 tokens, five in eight of
 // them known and the most frequent one 6% of those, of 50,000 x 1,024 in bf16 (a 2 GiB copy: 4.8 to 5.1 TB/s):
 //   embed_kernel       39 us for 183 MB, 4.7 TB/s
-//   embed_sort_kernel  18 us (4,096 tokens 6.5, 262,144 47: 26 bytes a cycle and CU), by the instructions per token of each
-//                      block: tokens begin at other places in each block made no difference.  With ranges of neighbouring
-//                      tokens per block, as frequent ones are, it took 190 us
+//   embed_sort_kernel  17 us, of which the first walk takes 12, by its instructions per token (13 us where all tokens are
+//                      equally frequent, then 4,096 6.0 and 262,144 33).  Loads further ahead and another first token
+//                      for each block made no difference.  With ranges of neighbouring tokens per block, as frequent ones
+//                      are, it took 190 us
 //   embed_rows_kernel  51 us for 194 MB, 3.8 TB/s: three loads that wait for one another, four rows of a wave at once (one
 //                      row at a time 69 us)
-//   embed_join_kernel  5.5 us
+//   embed_join_kernel  5 us
 #include <type_traits>
 
 #include "rows.h"
@@ -30,8 +31,7 @@ namespace {
 
 constexpr int kSortThreads = 1024, kSortWaves = kSortThreads / 64;
 constexpr int kSortList = 448;  // tokens that a wave lists: with the counts below 64 KiB
-constexpr int kSortRows = 512;  // tokens of the vocabulary per block, at most: 32 KiB of counts
-constexpr int kLong = 32;
+constexpr int kSortRows = 512;  // tokens of the vocabulary per block, at most (or one more): 32 KiB of counts
 
 struct EmbedArgs {
   const void* tokens;      // int32 or int64
@@ -44,6 +44,7 @@ struct EmbedArgs {
   int64_t n, w_row, g_row;
   int vocab, dim, pdim, range, bits;  // range: tokens of a block of the sort; bits: log2 of its blocks
   int slices, chunk_blocks;           // waves that share a row's pieces; blocks of embed_rows_kernel that take chunks
+  int run, chunk_bits;                // the most tokens of a run that is summed at once, a chunk's tokens; its log2
   uint32_t block0;                    // of this launch
   float scale;
   __device__ __forceinline__ int slot(int token) const { return (token & ((1 << bits) - 1)) * range + (token >> bits); }
@@ -109,6 +110,7 @@ __global__ __launch_bounds__(kSortThreads) void embed_sort_kernel(EmbedArgs a) {
   const auto at_step = [&](int i) { return int64_t(i) * kStep + wave * 256 + 4 * lane; };
   int* const mine = count + wave * a.range;
   int* const list = lists[wave];
+  const uint64_t lower = (uint64_t(1) << lane) - 1;
   int below = 0, found = 0;
   typedef I vec __attribute__((ext_vector_type(4)));
   typedef vec loose __attribute__((aligned(sizeof(I))));
@@ -129,7 +131,10 @@ __global__ __launch_bounds__(kSortThreads) void embed_sort_kernel(EmbedArgs a) {
 #pragma unroll
       for (int k = 0; k < kAhead; ++k) step(v[k], int(at_step(i + k)));
     }
-    for (; i < steps; ++i) step(*reinterpret_cast<const loose*>(tokens + at_step(i)), int(at_step(i)));
+    for (; i < steps; ++i) {
+      const vec v = *reinterpret_cast<const loose*>(tokens + at_step(i));
+      step(v, int(at_step(i)));
+    }
     const int64_t rest = at_step(steps);
     vec v;
 #pragma unroll
@@ -152,7 +157,7 @@ __global__ __launch_bounds__(kSortThreads) void embed_sort_kernel(EmbedArgs a) {
       const uint64_t all = __ballot(other[j] == 0);
       if (other[j] == 0) {
         atomicAdd(&mine[t[j] >> a.bits], 1);
-        const int q = found + __popcll(all & ((uint64_t(1) << lane) - 1));
+        const int q = found + __popcll(all & lower);
         if (q < kSortList) list[q] = at + j;
       }
       found += __popcll(all);
@@ -188,21 +193,41 @@ __global__ __launch_bounds__(kSortThreads) void embed_sort_kernel(EmbedArgs a) {
   }
   if (block == low && tid == kSortThreads - 1) a.begin[(int64_t(block) + 1) * a.range] = at;
   __syncthreads();
+  // Puts the lanes' own tokens.  Lanes of the same row are found row by row for the first kEach rows, then bit by bit of what
+  // is left: a frequent token takes most lanes of a step, rare ones are all different (row by row alone 65,536 tokens of
+  // 50,000 take 17.2 us where all are equally frequent; bit by bit alone 13.1, and 17.9 where one is 6% of them).
+  const int row_bits = 32 - __builtin_clz(a.range);
+  constexpr int kEach = 3;
   const auto place = [&](int t, bool own, int position) {
-    for (uint64_t left = __ballot(own); left;) {  // each token of these once
-      const int token = __builtin_amdgcn_readlane(t, __builtin_ctzll(left));
-      const uint64_t same = __ballot(own && t == token);
-      const int to = mine[token >> a.bits];
-      if (own && t == token) {
-        const int q = to + __popcll(same & ((uint64_t(1) << lane) - 1));
-        a.place[q] = position;
-        a.token[q] = t;
-      }
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      if (lane == 0) mine[token >> a.bits] = to + __popcll(same);
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      left &= ~same;
+    const int row = t >> a.bits;
+    uint64_t left = __ballot(own), same = 0;
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) {
+      if (left == 0) break;
+      const int next = __builtin_amdgcn_readlane(row, __builtin_ctzll(left));
+      const uint64_t these = __ballot(own && row == next);
+      if (row == next) same = these;
+      left &= ~these;
     }
+    if (left != 0) {
+      uint64_t alike = left;
+      for (int b = 0; b < row_bits; ++b) {
+        const bool set = (row >> b) & 1;
+        const uint64_t with = __ballot(set);
+        alike &= set ? with : ~with;
+      }
+      if ((left >> lane) & 1) same = alike;
+    }
+    const int before = __popcll(same & lower);
+    int to = 0;
+    if (own) {
+      to = mine[row];
+      a.place[to + before] = position;
+      a.token[to + before] = t;
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    if (own && before == 0) mine[row] = to + __popcll(same);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   };
   if (found > kSortList) {
     walk([&](const int (&t)[4], int at) {
@@ -211,9 +236,13 @@ __global__ __launch_bounds__(kSortThreads) void embed_sort_kernel(EmbedArgs a) {
     });
     return;
   }
-  for (int i = lane; i - lane < found; i += 64) {
-    const int at = i < found ? list[i] : 0;
-    place(i < found ? int(tokens[at]) : -1, i < found, at);
+  const auto listed = [&](int i) { return i < found ? list[i] : -1; };
+  int position = listed(lane), token = position >= 0 ? int(tokens[position]) : -1;
+  for (int i = 64; i - 64 < found; i += 64) {  // the next ones' loads under the work on these
+    const int next = listed(i + lane), next_token = next >= 0 ? int(tokens[next]) : -1;
+    place(token, position >= 0, position);
+    position = next;
+    token = next_token;
   }
 }
 
@@ -274,7 +303,7 @@ __global__ __launch_bounds__(256) void embed_rows_kernel(EmbedArgs a) {
     for (int r = 0; r < kRows; ++r) {
       const uint32_t slot = uint32_t(min(slot0 + r, slots - 1)), block = slot / uint32_t(a.range);
       const int64_t v = (int64_t(slot - block * a.range) << a.bits) + block;
-      if (slot0 + r >= slots || v >= a.vocab || begin[r + 1] - begin[r] > kLong) continue;
+      if (slot0 + r >= slots || v >= a.vocab || begin[r + 1] - begin[r] > a.run) continue;
       float sum[P::E];
 #pragma unroll
       for (int i = 0; i < P::E; ++i) sum[i] = g[r][i];
@@ -287,11 +316,11 @@ __global__ __launch_bounds__(256) void embed_rows_kernel(EmbedArgs a) {
     return;
   }
   const int count = a.begin[a.range << a.bits];
-  if (int64_t(item) * kLong >= count) return;
-  const int first = int(item) * kLong, last = min(first + kLong, count);
+  const int first = int(item << a.chunk_bits), last = min(first + a.run, count);
+  if (first >= count) return;
   for (int side = 0; side < 2; ++side) {  // the run of the chunk's first token, and of its last one
     const int at = a.slot(a.token[side ? last - 1 : first]), b = a.begin[at], e = a.begin[at + 1];
-    if (e - b <= kLong || (b < first) != (side == 0)) continue;
+    if (e - b <= a.run || (b < first) != (side == 0)) continue;
     float sum[P::E] = {};
     add_rows<T, G>(a, max(b, first), min(e, last), on ? d : 0, lane, sum);
     if (!on) continue;
@@ -310,11 +339,12 @@ __global__ __launch_bounds__(256) void embed_join_kernel(EmbedArgs a) {
   const int lane = int(threadIdx.x) % G, group = int(threadIdx.x) / G;
   const uint32_t task = a.block0 + blockIdx.x, chunk = a.slices == 1 ? task : task / uint32_t(a.slices);
   const int d = (int(task - chunk * a.slices) * G + lane) * P::E, count = a.begin[a.range << a.bits];
-  if (int64_t(chunk) * kLong >= count) return;
-  const int last = min(int(chunk) * kLong + kLong, count), t = a.token[last - 1], at = a.slot(t);
+  const int first = int(chunk << a.chunk_bits);
+  if (first >= count) return;
+  const int last = min(first + a.run, count), t = a.token[last - 1], at = a.slot(t);
   const int b = a.begin[at], e = a.begin[at + 1];
-  if (e - b <= kLong || b < int(chunk) * kLong) return;
-  const int more = (e - 1) / kLong - int(chunk);  // chunks after this one
+  if (e - b <= a.run || b < first) return;
+  const int more = ((e - 1) >> a.chunk_bits) - int(chunk);  // chunks after this one
   // its own part is the chunk's second one, the others are their chunks' first ones
   const float* const part = a.part + (int64_t(chunk) * 2 + 1) * a.pdim + (d < a.dim ? d : 0);
   float sum[P::E] = {};
@@ -351,6 +381,7 @@ auto with_lanes(int dim, int dtype, F&& f) {
 
 struct Plan {
   int range, bits, pdim;  // tokens per block of the sort, log2 of its blocks; dim rounded up to 16 bytes
+  int chunk_bits;         // log2 of the tokens that one group sums
   int64_t chunks, place, token, part, bytes;
 };
 int64_t align256(int64_t bytes) { return (bytes + 255) / 256 * 256; }
@@ -362,11 +393,15 @@ Plan make_plan(const rdv_embedding_desc& d) {
   p.range = int(((int64_t(d.vocab) - 1) >> p.bits) + 1);
   const int e = d.dtype == RDV_DTYPE_F32 ? 4 : 8;
   p.pdim = (d.dim + e - 1) / e * e;
-  p.chunks = (d.tokens + kLong - 1) / kLong;
+  // With few tokens the longest run decides, with many the parts' traffic (us of the gradient, with chunks of 16, 32 and 64:
+  // 2,013 tokens of 10,007 x 321 in fp32 17.9, 20.2 and 26.3; 16,384 of 1,000 x 512 in fp16 23.6, 24.5 and 30.9; 65,536 of
+  // 50,000 x 1,024 in bf16 73.9, 64.5 and 63.1; 262,144 of 50,000 x 512 219, 198 and 194).
+  p.chunk_bits = d.tokens <= 16384 ? 4 : 5;
+  p.chunks = (d.tokens + (1 << p.chunk_bits) - 1) >> p.chunk_bits;
   p.place = align256((int64_t(p.range) * (int64_t(1) << p.bits) + 1) * 4);
   p.token = p.place + align256(d.tokens * 4);
   p.part = p.token + align256(d.tokens * 4);
-  p.bytes = p.part + (d.tokens > kLong ? p.chunks * 2 * p.pdim * 4 : 0);
+  p.bytes = p.part + (p.chunks > 1 ? p.chunks * 2 * p.pdim * 4 : 0);
   return p;
 }
 
@@ -414,6 +449,8 @@ int launch_embedding_backward(const rdv_embedding_desc& d, const void* grad, con
   a.range = p.range;
   a.bits = p.bits;
   a.pdim = p.pdim;
+  a.run = 1 << p.chunk_bits;
+  a.chunk_bits = p.chunk_bits;
   a.begin = reinterpret_cast<int32_t*>(ws);
   a.place = reinterpret_cast<int32_t*>(ws + p.place);
   a.token = reinterpret_cast<int32_t*>(ws + p.token);
@@ -428,7 +465,7 @@ int launch_embedding_backward(const rdv_embedding_desc& d, const void* grad, con
       constexpr int G = decltype(g)::value, E = RowPiece<T>::E;
       a.slices = (p.pdim / E + G - 1) / G;
       const auto blocks = [&](int64_t items) { return (items * a.slices + 256 / G - 1) / (256 / G); };
-      const int64_t chunks = d.tokens > kLong ? blocks(p.chunks) : 0;
+      const int64_t chunks = p.chunks > 1 ? blocks(p.chunks) : 0;
       a.chunk_blocks = int(chunks);
       const int64_t rows = ((int64_t(p.range) << p.bits) + kRows - 1) / kRows;
       const int rc = launch_blocks(chunks + blocks(rows), 256, [&](int64_t first, unsigned count) {
