@@ -101,12 +101,13 @@ def _grad_tensors(grads, likes, names):
 
 def _apart(out: torch.Tensor, *inputs) -> None:
     """The kernels read inputs after they have begun to write: no sharing of memory."""
+    a, size = out.data_ptr(), out.numel() * out.element_size()
     for t, what in inputs:
-        if t is not None and t.numel() and out.numel():
-            span = sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1
-            a, b = out.data_ptr(), t.data_ptr()
-            assert a >= b + span * t.element_size() or b >= a + out.numel() * out.element_size(), \
-                f"out must not share memory with {what}"
+        if t is not None and size and t.numel():
+            b = t.data_ptr()
+            if b < a + size:
+                span = t.numel() if t.is_contiguous() else sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1
+                assert a >= b + span * t.element_size(), f"out must not share memory with {what}"
 
 
 def _check(rc: int, what: str) -> None:
