@@ -276,3 +276,22 @@ def test_offsets_past_32_bits():
     got = rdv.causal_attention_backward(q, q, cache, cache, out, stats, far, grads=grads)
     ref = rdv.causal_attention_backward(q, q, tail, tail, want, wstats, near)
     assert torch.equal(got[0], ref[0]) and torch.equal(got[1][n:], ref[1]) and torch.equal(got[2][n:], ref[2])
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("lengths,states,hq,hkv,d", [
+    ((3, 40), (3, 70), 200, 1, 16), ((1, 2), (500, 2), 33, 1, 64), ((2, 5), (90, 3), 130, 2, 40), ((9,), (9,), 48, 48, 8),
+])
+def test_many_heads(dtype, lengths, states, hq, hkv, d):
+    """Tokens whose heads on one state head fill more than a wave's, or a block's, rows."""
+    seqs = rdv.PackedSequences(lengths, states)
+    _check(seqs, *_inputs(sum(lengths), sum(states), hq, hkv, d, dtype), dtype, what=f"{hq} on {hkv} {dtype}")
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_many_short_sequences(dtype):
+    g = np.random.default_rng(3)
+    lengths = g.integers(0, 4, 400)
+    states = np.where(g.uniform(size=400) < 0.5, lengths, g.integers(0, 30, 400))
+    seqs = rdv.PackedSequences(lengths, states)
+    _check(seqs, *_inputs(int(lengths.sum()), int(states.sum()), 2, 1, 24, dtype), dtype, what=dtype)
