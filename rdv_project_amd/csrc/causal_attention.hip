@@ -45,6 +45,7 @@ int blocks_at_once(CausalKernel which, int dtype, int dim) {
   const int nc = dim <= 32 ? 2 : dim <= 48 ? 3 : dim <= 64 ? 4 : dim <= 80 ? 5 : dim <= 96 ? 6 : 8;
   const int bytes = nc * element_bytes(dtype);
   if (which == kCausalTile) return bytes > 24 ? 1 : bytes > 8 ? 2 : 4;
+  if (which == kCausalFew) return bytes > 16 ? 1 : 2;
   if (which == kCausalDq) return bytes > 16 ? 1 : bytes > 8 ? 2 : 3;
   return nc > (dtype == RDV_DTYPE_F32 ? 2 : 6) ? 1 : 2;
 }
@@ -118,9 +119,14 @@ Lists make_lists(const rdv_causal_attention_desc& d, const std::vector<Sequence>
       (few ? few_total : total) += int64_t(end) * d.kv_heads;
     }
   }
-  // Few rows stream the states: up to eight blocks per CU, so that unequal lengths fill the chip to the end.
+  // Few rows stream the states, in as many parts as blocks run at once: more of them cost more at their beginnings and in the
+  // join than they even out (us):                              that many  1.5x   2x    4x   0.5x
+  //   16 tokens, 2,000 to 32,000 states, 16 heads on 4 of 128, bf16:   129   128   130   135   147
+  //   32 x 8,192 states, 16 heads on 2 of 128, bf16:                    51    53    52    61    50
+  //   40 of 100 to 9,000 states, 8 heads on 2 of 128, bf16:             38    38    39    41    40
+  //   16 x 3,000 states, 8 heads on 4 of 128, fp32, one at a time:      50    59    68    68    -
   {
-    const int most = part_size(few_total, 8 * int64_t(cu), 256, 128);
+    const int most = part_size(few_total, cu * blocks_at_once(kCausalFew, d.dtype, d.dim), 256, 128);
     std::vector<CausalItem> whole;
     whole.swap(l.few);
     for (const CausalItem& i : whole) put(l.few, l.row_joins, h.row_slots, i, most);
