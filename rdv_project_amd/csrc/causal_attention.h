@@ -543,15 +543,23 @@ __global__ __launch_bounds__(256, NC * sizeof(T) > 16 ? 1 : NC * sizeof(T) > 8 ?
     }
 }
 
+// Waves of causal_dkv_kernel on a SIMD.
+template <class T, int NC>
+constexpr int dkv_waves() { return NC > (sizeof(T) == 4 ? 2 : 6) ? 1 : 2; }
+
 // dK and dV: a block of 4 waves, 32 states each (WR = 2: pairs of waves share 32 states and take a half of each tile), goes
 // over the tokens that see any of them, head by head of those that share the state head, in tiles of RT tokens of one head:
 // tile t is the t % n-th of the t / n-th head, n tiles from token `from` on.  As attn_dkv_kernel.  The 8 sequences above: 145
 // us, 0.74 PFLOP/s of its four products (37 and 32% of the cycles: two waves per SIMD do not cover its LDS reads).  Three
 // waves, whose registers spill, took 203 us; both halves of a tile's scores before the first one's terms made no difference.
 template <class T, int NC, int WR>
-__global__ __launch_bounds__(256, NC > (sizeof(T) == 4 ? 2 : 6) ? 1 : 2) void causal_dkv_kernel(CausalArgs a) {
+__global__ __launch_bounds__(256, (dkv_waves<T, NC>())) void causal_dkv_kernel(CausalArgs a) {
   using G = AttnTile<T, NC>;
   constexpr int RT = attn_tile_keys<T, NC>(), SUB = RT / 32, ND = G::ND;
+  // Priority for the wave at the matrix cores (8,192 tokens, 8 heads on 4 of 64 in fp16, both backward kernels: 315 us, without
+  // it 324); alone on its SIMD it has the compiler's own mix of instructions instead (4,096 tokens, 8 heads on 2 of 128 in
+  // fp16: 250 us, with priorities 270).
+  constexpr bool kPriority = dkv_waves<T, NC>() > 1;
   static_assert(SUB >= WR, "a tile has 32 rows for every wave of a state group");
   __shared__ __attribute__((aligned(16))) struct {
     uint8_t tiles[2][2][RT * G::kRow];
@@ -632,13 +640,13 @@ __global__ __launch_bounds__(256, NC > (sizeof(T) == 4 ? 2 : 6) ? 1 : 2) void ca
             const uint8_t* const tq = tiles[t & 1][0] + 32 * u * G::kRow;
             const uint8_t* const tg = tiles[t & 1][1] + 32 * u * G::kRow;
             f32x16 s{}, dp{};
-            __builtin_amdgcn_s_setprio(1);
+            if (kPriority) __builtin_amdgcn_s_setprio(1);
 #pragma unroll
             for (int e = 0; e < NC; ++e) {
               s = mma(row_frag<T, NC>(tq, n32, e, h), kf[e], s);
               dp = mma(row_frag<T, NC>(tg, n32, e, h), vf[e], dp);
             }
-            __builtin_amdgcn_s_setprio(0);
+            if (kPriority) __builtin_amdgcn_s_setprio(0);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
               const f32x4 l = *reinterpret_cast<const f32x4*>(&row_lse[t & 1][32 * u + 8 * j + 4 * h]);
@@ -669,7 +677,7 @@ __global__ __launch_bounds__(256, NC > (sizeof(T) == 4 ? 2 : 6) ? 1 : 2) void ca
               masked_product<T, NC>(tq, dp, bits, dk, h);
               continue;
             }
-            __builtin_amdgcn_s_setprio(1);
+            if (kPriority) __builtin_amdgcn_s_setprio(1);
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
               const auto pf = result_frag<T>(s, half);
@@ -680,7 +688,7 @@ __global__ __launch_bounds__(256, NC > (sizeof(T) == 4 ? 2 : 6) ? 1 : 2) void ca
                 dk[d] = mma(col_frag<T, NC>(tq, half, d, lane), sf, dk[d]);
               }
             }
-            __builtin_amdgcn_s_setprio(0);
+            if (kPriority) __builtin_amdgcn_s_setprio(0);
           }
         }
         hand_over((t + 1) & 1);
