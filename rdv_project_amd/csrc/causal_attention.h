@@ -313,7 +313,7 @@ __global__ __launch_bounds__(256, NC * sizeof(T) > 24 ? 1 : NC * sizeof(T) > 8 ?
 }
 
 // At most 32 rows of a sequence: a single token's heads, or few tokens.  The waves split the states, as attn_few_kernel.
-// Bound: HBM.  16 tokens against 2,000 to 32,000 states, 16 heads on 4 of 128, bf16: 125 us for 569 MB, 4.5 TB/s.
+// Bound: HBM.  16 tokens against 2,000 to 32,000 states, 16 heads on 4 of 128, bf16: 124 us for 569 MB, 4.6 TB/s.
 template <class T, int NC>
 __global__ __launch_bounds__(256, NC * sizeof(T) > 16 ? 1 : 2) void causal_few_kernel(CausalArgs a) {
   using G = AttnTile<T, NC>;
