@@ -719,8 +719,8 @@ typedef struct rdv_causal_attention_desc {
 } rdv_causal_attention_desc;
 
 /* The list of a call's work, made on the host from the lengths of its sequences
- * for the current device; every call on sequences of these lengths, with any
- * strides, scale and buffers of at least this many rows, can use it.  sequences:
+ * for the current device; every call on these sequences, with any strides, scale
+ * and rows of q, k and v that hold them (also fewer than desc has), can use it.  sequences:
  * [n][4] = (token, tokens, state, states).  No two share a token, and for the
  * backward call no two share a state.  rdv_causal_attention_plan writes `bytes` =
  * rdv_causal_attention_plan_bytes(...) bytes (< 0 on error) to host memory; the

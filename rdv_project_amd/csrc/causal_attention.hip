@@ -18,7 +18,7 @@ int element_bytes(int dtype) { return dtype == RDV_DTYPE_F32 ? 4 : 2; }
 struct Header {
   uint64_t magic;
   int64_t bytes;
-  rdv_causal_attention_desc desc;  // what it was made for: heads, kv_heads, dim, dtype, tokens, states
+  rdv_causal_attention_desc desc;  // what it was made for: heads, kv_heads, dim, dtype; tokens and states that the sequences need
   int32_t backward, cu;
   int32_t few, rows, keys;         // items: few rows, tiles of rows, tiles of states (dK and dV)
   int32_t row_joins, key_joins;
@@ -91,7 +91,14 @@ Lists make_lists(const rdv_causal_attention_desc& d, const std::vector<Sequence>
   Lists l;
   Header& h = l.h;
   h.magic = kMagic;
-  h.desc = d;
+  h.desc.heads = d.heads;
+  h.desc.kv_heads = d.kv_heads;
+  h.desc.dim = d.dim;
+  h.desc.dtype = d.dtype;
+  for (const Sequence& s : seqs) {  // the rows that calls have to have, whatever the tensors at hand have
+    if (s.tokens > 0) h.desc.tokens = std::max(h.desc.tokens, s.token + s.tokens);
+    if (s.states > 0) h.desc.states = std::max(h.desc.states, s.state + s.states);
+  }
   h.backward = backward;
   h.cu = cu;
   const int share = d.heads / d.kv_heads;

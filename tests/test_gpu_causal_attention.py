@@ -295,3 +295,19 @@ def test_many_short_sequences(dtype):
     states = np.where(g.uniform(size=400) < 0.5, lengths, g.integers(0, 30, 400))
     seqs = rdv.PackedSequences(lengths, states)
     _check(seqs, *_inputs(int(lengths.sum()), int(states.sum()), 2, 1, 24, dtype), dtype, what=dtype)
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_one_plan_on_tensors_of_falling_lengths(dtype):
+    """One PackedSequences on longer and on shorter buffers, longest first: the same bits as with one of its own."""
+    lengths, states, starts = (1, 40), (90, 33), (0, 100)
+    q, k, v, g = _inputs(120, 200, 4, 2, 64, dtype)
+    seqs = rdv.PackedSequences(lengths, states, starts)
+    for rows, cols in ((120, 200), (50, 140), (41, 133)):
+        a = q[:rows], k[:cols], v[:cols]
+        out, stats = rdv.causal_attention(*a, seqs, return_lse=True)
+        own = rdv.PackedSequences(lengths, states, starts)
+        want, wstats = rdv.causal_attention(*a, own, return_lse=True)
+        assert torch.equal(out, want) and torch.equal(stats.lse, wstats.lse)
+        got = rdv.causal_attention_backward(g[:rows], *a, out, stats, seqs)
+        assert all(map(torch.equal, got, rdv.causal_attention_backward(g[:rows], *a, out, stats, own)))

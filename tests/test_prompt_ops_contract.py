@@ -312,3 +312,15 @@ def test_refusals_of_buffers():
     ):
         with pytest.raises(error, match=text):
             call()
+
+
+@pytest.mark.parametrize("backward", [0, 1])
+def test_plans_need_the_rows_of_their_sequences(backward):
+    """A plan serves every call whose tensors hold its sequences, whatever rows those that it was made with had."""
+    lib, rows = _lib.load(), [(2, 5, 3, 6), (0, 2, 11, 9), (90, 0, 190, 0)]  # 7 tokens, 20 states
+    plan = _plan(_desc(tokens=100, states=200), rows, backward)
+    ok = lambda **kw: lib.rdv_causal_attention_workspace_bytes(C.byref(_desc(**kw)), plan.ctypes.data, backward)
+    assert ok(tokens=100, states=200) >= 0 and ok(tokens=7, states=20) >= 0 and ok(tokens=1000, states=20) >= 0
+    for kw in (dict(tokens=6, states=200), dict(tokens=100, states=19)):
+        assert ok(**kw) == _lib.RDV_ERR_INVALID and "made for other" in _lib.last_error()
+    assert np.array_equal(plan, _plan(_desc(tokens=500, states=200), rows, backward))
