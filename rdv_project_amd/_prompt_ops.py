@@ -380,14 +380,13 @@ class AttentionStats(NamedTuple):
 
 
 def _counts(values, what: str) -> tuple:
-    values = values.tolist() if isinstance(values, torch.Tensor) else values
     try:
-        counts = tuple(int(v) for v in values)
+        values = tuple(values.tolist() if isinstance(values, torch.Tensor) else values)
+        if any(not 0 <= v < 1 << 31 or int(v) != v for v in values):  # NaN and infinities too
+            raise ValueError(f"{what} must be whole numbers in [0, 2^31)")
+        return tuple(int(v) for v in values)
     except TypeError:
         raise TypeError(f"{what} must be whole numbers, one per sequence") from None
-    if any(c != v for c, v in zip(counts, values)) or any(c < 0 or c >= 1 << 31 for c in counts):
-        raise ValueError(f"{what} must be whole numbers in [0, 2^31)")
-    return counts
 
 
 def _causal_desc(q_shape, k_shape, v_shape, q_stride, k_stride, v_stride, g_stride, dtype, scale):

@@ -324,3 +324,15 @@ def test_plans_need_the_rows_of_their_sequences(backward):
     for kw in (dict(tokens=6, states=200), dict(tokens=100, states=19)):
         assert ok(**kw) == _lib.RDV_ERR_INVALID and "made for other" in _lib.last_error()
     assert np.array_equal(plan, _plan(_desc(tokens=500, states=200), rows, backward))
+
+
+def test_lengths_may_be_any_iterable():
+    """Numbers that can be read once are checked as a list's are."""
+    s = rdv.PackedSequences(map(int, "302"), (x for x in (5, 1, 0)), iter((7, 0, 2)))
+    assert (s.lengths, s.states, s.starts) == ((3, 0, 2), (5, 1, 0), (7, 0, 2))
+    for values in ((1.5,), (1, 1e10), (float("nan"),), (float("inf"),), (1 << 40,)):
+        for make in (list, iter, lambda v: (x for x in v)):
+            with pytest.raises(ValueError, match="lengths"):
+                rdv.PackedSequences(make(values))
+            with pytest.raises(ValueError, match="states"):
+                rdv.PackedSequences((1,) * len(values), make(values))
