@@ -592,6 +592,9 @@ __global__ __launch_bounds__(256, (dkv_waves<T, NC>())) void causal_dkv_kernel(C
   Dma<T, NC, RT> dq, dg;
   dq.init(a.qs[0], a.dim, wave, lane);
   dg.init(a.gs[0], a.dim, wave, lane);
+  // The 32 rows from `query` on see all of the wave's states where query is one of the `clears` from `clear` on.  Rows past
+  // the last token have scores and terms too, of q = 0 and lse = inf, and those are NaN against an infinite state.
+  const int clear = key0 + 31 - at.shift, clears = max(at.p.tokens - 31 - clear, 0);
   float2 st{INFINITY, 0.0f};
   auto load = [&](int t, int buf) {
     const int x = t / n, query = from + (t - x * n) * RT, head = at.hk * a.share + x, left = at.p.tokens - query;
@@ -658,8 +661,8 @@ __global__ __launch_bounds__(256, (dkv_waves<T, NC>())) void causal_dkv_kernel(C
                 dp[4 * j + i] = (dp[4 * j + i] + y[i]) * s[4 * j + i];
               }
             }
-            const uint32_t bits = suffix_bits(key - at.shift - query);
-            const bool masked = query + at.shift < key0 + 31;
+            const uint32_t bits = suffix_bits(key - at.shift - query) & prefix_bits(at.p.tokens - 1 - query);
+            const bool masked = uint32_t(query - clear) >= uint32_t(clears);
             if (masked) {
               mask_result(s, bits, h, 0.0f);
               mask_result(dp, bits, h, 0.0f);

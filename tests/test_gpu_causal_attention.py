@@ -311,3 +311,26 @@ def test_one_plan_on_tensors_of_falling_lengths(dtype):
         assert torch.equal(out, want) and torch.equal(stats.lse, wstats.lse)
         got = rdv.causal_attention_backward(g[:rows], *a, out, stats, seqs)
         assert all(map(torch.equal, got, rdv.causal_attention_backward(g[:rows], *a, out, stats, own)))
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("lengths,states,hq,d", [((40,), (40,), 2, 64), ((9, 70), (30, 70), 4, 32), ((33, 5), (33, 5), 2, 128),
+                                                 ((2100,), (2100,), 2, 64), ((100,), (170,), 2, 96)])
+def test_infinite_state_without_weight(dtype, lengths, states, hq, d):
+    """A state whose scores are all -inf has no weight: dk and dv are what they are with scores so low that their terms are
+    0, bit for bit, and 0 at that state, also where a sequence's rows end inside a tile."""
+    q, k, v, g = _inputs(sum(lengths), sum(states), hq, 2, d, dtype)
+    seqs = rdv.PackedSequences(lengths, states)
+    q[..., 0] = -1.0
+    at = [sum(states[:i]) + 1 for i in range(len(states))] + [sum(states[:i + 1]) - 2 for i in range(len(states))]
+    got = []
+    for value in (3e4, math.inf):
+        k[at, :, 0] = value
+        out, stats = rdv.causal_attention(q, k, v, seqs, return_lse=True)
+        _, dk, dv = rdv.causal_attention_backward(g, q, k, v, out, stats, seqs)
+        got.append((out, stats.lse, dk, dv))
+    low, inf = got
+    assert all(torch.isfinite(t).all() for t in inf)
+    assert not inf[2][at].any() and not inf[3][at].any()
+    for a, b, what in zip(low, inf, ("out", "lse", "dk", "dv")):
+        assert torch.equal(a, b), what
