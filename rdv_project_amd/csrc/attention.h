@@ -1087,6 +1087,13 @@ __global__ __launch_bounds__(256, NC > (sizeof(T) == 4 ? 2 : 6) ? 1 : 2) void at
               dp[4 * j + i] = (dp[4 * j + i] + w[i]) * s[4 * j + i];
             }
           }
+          // rows past the last one have scores and terms too, of q = 0 and lse = inf: NaN against an infinite state
+          const int left = a.rows - begin - t * RT - 32 * u;
+          if (left < 32) {
+            const uint32_t bits = left > 0 ? (1u << left) - 1u : 0u;
+            mask_result(s, bits, h, 0.0f);
+            mask_result(dp, bits, h, 0.0f);
+          }
           if (shrink != 1.0f) dp *= shrink;
           const float fit = fit_terms<T>(dp, counts);
           if (fit != 1.0f) {

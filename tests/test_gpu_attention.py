@@ -408,3 +408,25 @@ def test_backward_of_many_wide_rows():
     for part in dq.split(1 << 23, 1):
         assert not part.any()
     assert not dk.any() and (dv == 2.0 ** 7).all()
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("queries,keys,hq,d", [(40, 50, 2, 64), (70, 33, 4, 32), (5, 200, 2, 128), (1100, 60, 2, 64), (100, 170, 2, 96)])
+def test_infinite_state_without_weight(dtype, queries, keys, hq, d):
+    """A state whose scores are all -inf has no weight: dk and dv are what they are with scores so low that their terms are
+    0, bit for bit, and 0 at that state, also where the rows end inside a tile."""
+    r = torch.Generator().manual_seed(queries + keys)
+    make = lambda *s: torch.randn(s, generator=r).to(TYPES[dtype]).cuda()
+    q, k, v, g = make(2, queries, hq, d), make(2, keys, 2, d), make(2, keys, 2, d), make(2, queries, hq, d)
+    q[..., 0] = -1.0
+    got = []
+    for value in (3e4, float("inf")):
+        k[:, [1, keys - 2], :, 0] = value
+        out, lse = rdv.cross_attention(q, k, v, return_lse=True)
+        _, dk, dv = rdv.cross_attention_backward(g, q, k, v, out, lse)
+        got.append((out, lse, dk, dv))
+    low, inf = got
+    assert all(torch.isfinite(t).all() for t in inf)
+    assert not inf[2][:, [1, keys - 2]].any() and not inf[3][:, [1, keys - 2]].any()
+    for a, b, what in zip(low, inf, ("out", "lse", "dk", "dv")):
+        assert torch.equal(a, b), what
