@@ -120,14 +120,15 @@ __global__ __launch_bounds__(block_threads<G>()) void rms_norm_kernel(RmsArgs a)
       for (int i = 0; i < E; ++i) {
         const float v = h[k][i];
         sq = fmaf(v, v, sq);
-        if (EIGHT) top = fmaxf(top, fabsf(v * w[k][i]));
+        if (EIGHT) top = LaneMax::join(top, fabsf(v * w[k][i]));
       }
     const float2 t = joint.template operator()<LaneSum, LaneMax>(sq, top, slot);
     slot ^= 1;
     const float rstd = 1.0f / sqrtf(t.x / float(a.width) + a.eps);
     if (a.stats && lane == 0) a.stats[row] = rstd;
     if constexpr (EIGHT) {
-      // the largest |y| times the scale's inverse is 448; a scale below fp32's normal range is raised to it
+      // the largest |y| times the scale's inverse is 448; a scale below fp32's normal range is raised to it (a NaN stays: of a
+      // row with a NaN in y, weight's too, nothing is a number)
       float scale = t.y * rstd / kMostE4m3;
       if (scale < 1.17549435e-38f && t.y != 0.0f) scale = 1.17549435e-38f;
       const float f = scale == 0.0f ? 0.0f : 1.0f / scale;
@@ -289,14 +290,14 @@ __global__ __launch_bounds__(1024) void rms_norm_wide_kernel(RmsArgs a) {
       if (res) sum[d] = v = T(to_f32(v) + to_f32(res[d]));
       const float f = to_f32(v);
       sq += double(f) * double(f);
-      if (EIGHT) top = fmaxf(top, fabsf(f * (a.weight ? a.weight[d] : 1.0f)));
+      if (EIGHT) top = LaneMax::join(top, fabsf(f * (a.weight ? a.weight[d] : 1.0f)));
     }
     sq = block_sum(sq, red);
     if (EIGHT) {
       top = join_lanes<LaneMax, 64>(top);
       if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = top;
       __syncthreads();
-      for (int w = 0; w < 16; ++w) top = fmaxf(top, tops[w]);
+      for (int w = 0; w < 16; ++w) top = LaneMax::join(top, tops[w]);
     }
     const float rstd = 1.0f / sqrtf(float(sq / double(a.width)) + a.eps);
     if (a.stats && threadIdx.x == 0) a.stats[row] = rstd;

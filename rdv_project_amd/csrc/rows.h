@@ -44,8 +44,8 @@ struct RowPiece {
 struct LaneSum {
   __device__ __forceinline__ static float join(float a, float b) { return a + b; }
 };
-struct LaneMax {
-  __device__ __forceinline__ static float join(float a, float b) { return fmaxf(a, b); }
+struct LaneMax {  // NaN where one of them is (v_maximum3_f32; fmaxf drops a NaN)
+  __device__ __forceinline__ static float join(float a, float b) { return __builtin_elementwise_maximum(a, b); }
 };
 template <class Op, int G>
 __device__ __forceinline__ float join_lanes(float v) {

@@ -207,3 +207,23 @@ def test_eight_bits_with_statistics(width):
     assert ((back - y).abs() <= y.abs() * (2.0 ** -4 + 2.0 ** -10) + scales.double()[:, None] * 2.0 ** -10 + 2.0 ** -25).all()
     (values, scales), stats8 = rdv.rms_norm(x, w, return_stats=True, eight_bits=True)
     assert torch.equal(stats8, rdv.rms_norm(x, w, return_stats=True)[1])
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("width", [40, 1100, 9000, 40000])
+def test_eight_bits_of_a_weight_that_is_nan(dtype, width):
+    """max |y| of a row with a NaN in y is NaN, and so are its scale and what it stands for; an infinite y gives an infinite
+    scale, NaN there and zeros elsewhere."""
+    x = torch.randn(4, width).to(TYPES[dtype]).cuda()
+    x[3] = 0
+    w = (torch.rand(width) + 0.5).cuda()
+    for at in (0, width // 2, width - 1):
+        bad = w.clone()
+        bad[at] = float("nan")
+        values, scales = rdv.rms_norm(x, bad, eight_bits=True)
+        assert torch.isnan(scales).all() and torch.isnan(values.float()).all()
+        bad[at] = float("inf")
+        values, scales = rdv.rms_norm(x[:3], bad, eight_bits=True)
+        assert torch.isinf(scales).all()
+        nan = torch.isnan(values.float())
+        assert nan[:, at].all() and nan.sum() == 3 and not values.float().nan_to_num().any()
