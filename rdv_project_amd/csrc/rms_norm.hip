@@ -14,6 +14,8 @@
 //   65,536 x 1,024 with a residual                 537 MB    93 us, 5.8 TB/s
 //   its gradients with grad_sum                    537 MB   116 us, 4.6 TB/s, and 4.8 us for the sum of dweight's parts
 //   8 x 1,024 with a residual, fp16                          3.8 us; 1,003 x 777 in fp32 4.2, backward 6.8 and 3.9
+#include <cmath>
+
 #include "rows.h"
 
 namespace rdv {
@@ -28,6 +30,7 @@ struct RmsArgs {
   float* part;              // backward: dweight's sums of each block
   int64_t rows, x_row, r_row, g_row, s_row;
   int width;
+  int run;                  // backward: rows that are added to dweight's sums one after the other
   float eps;
 };
 
@@ -183,6 +186,29 @@ __global__ __launch_bounds__(block_threads<G>()) void rms_norm_back_kernel(RmsAr
       w[k][i] = d < a.width ? (a.weight ? a.weight[d] : 1.0f) : 0.0f;
       dw[k][i] = 0.0f;
     }
+  // The sums of a run of rows: groups of a wave or less add them up in registers; a group that is a block, whose registers are
+  // full, writes each run's to a place of its own in the workspace (to add them up there costs 16 registers: 168 -> 186 of two
+  // pieces in fp16, a wave per SIMD less).
+  float runs[kGroups > 1 ? K : 1][kGroups > 1 ? E : 1] = {};
+  const int64_t part_step = int64_t(gridDim.x) * a.width;
+  float* part = a.part + int64_t(blockIdx.x) * a.width;
+  int left = a.run;
+  const auto end_run = [&] {
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+      for (int i = 0; i < E; ++i) {
+        if constexpr (kGroups > 1) {
+          runs[k][i] += dw[k][i];
+        } else {
+          const int d = (k * G + lane) * E + i;
+          if (d < a.width) part[d] = dw[k][i];
+        }
+        dw[k][i] = 0.0f;
+      }
+    if (kGroups == 1) part += part_step;
+    left = a.run;
+  };
   int slot = 0;
   // a row's loads are in flight under the work on the one before it
   P nh[K], ng[K], ns[K];
@@ -236,14 +262,15 @@ __global__ __launch_bounds__(block_threads<G>()) void rms_norm_back_kernel(RmsAr
       }
       o.store(dx, (k * G + lane) * E, a.width);
     }
+    if (--left == 0) end_run();
   }
-  // the block's groups join their sums, a run of pieces at a time
-  float* const part = a.part + int64_t(blockIdx.x) * a.width;
+  end_run();
+  // the block's groups join their sums, a piece of each lane at a time
+  if constexpr (kGroups > 1) {
 #pragma unroll
-  for (int k = 0; k < K; ++k) {
-    if constexpr (kGroups > 1) {
+    for (int k = 0; k < K; ++k) {
 #pragma unroll
-      for (int i = 0; i < E; ++i) sums[group][lane * E + i] = dw[k][i];
+      for (int i = 0; i < E; ++i) sums[group][lane * E + i] = runs[k][i];
       __syncthreads();
       for (int j = int(threadIdx.x); j < G * E; j += kThreads) {
         float t = sums[0][j];
@@ -251,12 +278,6 @@ __global__ __launch_bounds__(block_threads<G>()) void rms_norm_back_kernel(RmsAr
         if (k * G * E + j < a.width) part[k * G * E + j] = t;
       }
       __syncthreads();
-    } else {
-#pragma unroll
-      for (int i = 0; i < E; ++i) {
-        const int d = (k * G + lane) * E + i;
-        if (d < a.width) part[d] = dw[k][i];
-      }
     }
   }
 }
@@ -340,14 +361,14 @@ __global__ __launch_bounds__(1024) void rms_norm_wide_back_kernel(RmsArgs a) {
   }
 }
 
-// dweight: the sum of the blocks' sums, 64 threads per channel, in one order.
+// dweight: the sum of the blocks' sums, 64 threads per channel, in one order and in 64 bits, however many they are.
 __global__ __launch_bounds__(1024) void rms_norm_weight_kernel(const float* part, int blocks, int width, float* dweight) {
-  __shared__ float sums[64][17];
+  __shared__ double sums[64][17];
   const int col = int(threadIdx.x) & 15, share = int(threadIdx.x) >> 4, d = int(blockIdx.x) * 16 + col;
-  float t = 0.0f;
+  double t = 0.0;
   if (d < width) {
 #pragma unroll 4
-    for (int b = share; b < blocks; b += 64) t += part[int64_t(b) * width + d];
+    for (int b = share; b < blocks; b += 64) t += double(part[int64_t(b) * width + d]);
   }
   sums[share][col] = t;
   __syncthreads();
@@ -356,7 +377,7 @@ __global__ __launch_bounds__(1024) void rms_norm_weight_kernel(const float* part
     if (share < n) sums[share][col] += sums[share + n][col];
     __syncthreads();
   }
-  if (share == 0 && d < width) dweight[d] = sums[0][col];
+  if (share == 0 && d < width) dweight[d] = float(sums[0][col]);
 }
 
 __global__ __launch_bounds__(256) void rms_norm_zero_kernel(float* p, int n) {
@@ -394,6 +415,26 @@ int blocks_of(int64_t rows, const Shape& s, int per_cu, int cu) {
 
 constexpr int kForwardBlocks = 6, kBackwardBlocks = 3;  // per CU, of 256 threads
 
+// A group of the backward call adds at most 128 rows one after the other to dweight's sums, whose roundings can all have one
+// sign (2^26 equal rows of 8 in fp32, 2,731 in a group: off by 576 2^-24; 2^18 of 8,200 in fp16, 1,024: by 253).  Groups of a
+// wave or less then add up those sums (beyond 128 of them runs are longer, both the square root); blocks that are a group
+// leave them to rms_norm_weight_kernel.  Rows past the registers have rounds of blocks instead of runs (65,536 x 40,000 in
+// bf16: 22.4 ms with 256 rows of a block, 15.2 with 128; in registers rounds cost, 2^17 x 8,192 1.55 -> 1.71).
+struct Runs {
+  int blocks, run, parts;
+};
+Runs runs_of(int64_t rows, const Shape& s, int cu) {
+  const int blocks = blocks_of(rows, s, kBackwardBlocks, cu);
+  const int64_t groups = int64_t(blocks) * s.row_groups(), each = (rows + groups - 1) / groups;
+  if (s.wide()) return Runs{int(blocks * ((each + 127) / 128)), 0, 1};
+  if (s.row_groups() == 1) {
+    int run = 128;
+    while (each % run == 0) --run;  // then blocks of a row less have as many runs
+    return Runs{blocks, run, int(each / run) + 1};
+  }
+  return Runs{blocks, int(std::max<int64_t>(128, int64_t(std::sqrt(double(each))))), 1};
+}
+
 template <class F>
 auto with_shape(const Shape& s, F&& f) {
 #define RDV_SHAPE(G, K) \
@@ -417,7 +458,8 @@ auto with_shape(const Shape& s, F&& f) {
 
 int64_t rms_norm_workspace_bytes(const rdv_rms_norm_desc& d, int cu) {
   if (d.rows == 0) return 0;
-  return int64_t(blocks_of(d.rows, shape_of(d.rows, d.width, d.dtype, true, cu), kBackwardBlocks, cu)) * d.width * 4;
+  const Runs r = runs_of(d.rows, shape_of(d.rows, d.width, d.dtype, true, cu), cu);
+  return int64_t(r.blocks) * r.parts * d.width * 4;
 }
 
 int launch_rms_norm(const rdv_rms_norm_desc& d, const void* x, const void* residual, const float* weight, void* sum, void* y,
@@ -477,7 +519,8 @@ int launch_rms_norm_backward(const rdv_rms_norm_desc& d, const void* grad, const
   a.s_row = d.s_row_stride;
   a.width = d.width;
   const Shape s = shape_of(d.rows, d.width, d.dtype, true, cu);
-  const int blocks = blocks_of(d.rows, s, kBackwardBlocks, cu);
+  const auto [blocks, run, parts] = runs_of(d.rows, s, cu);
+  a.run = run;
   with_dtype(d.dtype, [&](auto t) {
     using T = decltype(t);
     if (s.wide()) {
@@ -491,7 +534,7 @@ int launch_rms_norm_backward(const rdv_rms_norm_desc& d, const void* grad, const
     });
   });
   RDV_HIP_TRY(hipGetLastError());
-  rms_norm_weight_kernel<<<unsigned((d.width + 15) / 16), 1024, 0, stream>>>(a.part, blocks, d.width, dweight);
+  rms_norm_weight_kernel<<<unsigned((d.width + 15) / 16), 1024, 0, stream>>>(a.part, blocks * parts, d.width, dweight);
   RDV_HIP_TRY(hipGetLastError());
   return RDV_OK;
 }

@@ -227,3 +227,20 @@ def test_eight_bits_of_a_weight_that_is_nan(dtype, width):
         assert torch.isinf(scales).all()
         nan = torch.isnan(values.float())
         assert nan[:, at].all() and nan.sum() == 3 and not values.float().nan_to_num().any()
+
+
+@pytest.mark.parametrize("dtype,rows,width", [("f32", 1 << 26, 8), ("f32", 1 << 22, 136), ("f32", 1 << 20, 1100),
+                                              ("f16", 1 << 18, 8200), ("f16", 1 << 18, 33000), ("f16", 32767, 4100),
+                                              ("f16", 32768, 4100), ("f16", 32769, 4100), ("f32", 65537, 5000),
+                                              ("f32", 98304, 1100), ("f32", 98305, 1100), ("f16", 32769, 33000)])
+def test_dweight_of_very_many_rows(dtype, rows, width):
+    """Equal rows, whose terms' roundings do not cancel.  A thread adds at most 128 terms one after the other, 127 U32 of
+    their sum, then at most 22 of those sums (the 2,731 rows of a group of 2^26 rows in 24,576 of them), 21 U32; the groups
+    of a block add up to 32, 31 U32; then it is 64 bits, rounded once.  A term is two products, 2 U32."""
+    r = torch.Generator().manual_seed(width)
+    x = torch.tensor([1.0, 2.0]).repeat(width // 2).to(TYPES[dtype]).cuda()
+    grad = (1 + torch.rand(width, generator=r)).to(TYPES[dtype]).cuda()
+    stats = torch.full((rows,), 0.4 ** 0.5).cuda()
+    _, dw = rdv.rms_norm_backward(grad.expand(rows, -1), x.expand(rows, -1), None, stats)
+    want = rows * grad.double() * x.double() * stats[0].double()
+    assert ((dw.double() - want).abs() <= (127 + 21 + 31 + 1 + 2) * 2.0 ** -24 * want).all()
