@@ -330,12 +330,16 @@ __global__ __launch_bounds__(256) void embed_rows_kernel(EmbedArgs a) {
   }
 }
 
-// Chunk by chunk and slice by slice: the long run that begins in it, its parts shared by the block's groups.
+// Chunk by chunk and slice by slice: the long run that begins in it, its parts shared by the block's groups.  A frequent
+// token's are thousands, whose roundings can all have one sign (2^18 equal gradients of 68 of one token in fp32: off by 479
+// 2^-24), so at most 128 are added one after the other, and those sums in 64 bits.  (All in 64 bits half of 262,144 tokens of
+// 50,000 x 512 in bf16 took 376 us, 32 at a time 374, 128 at a time 368, in fp32 362.)
+constexpr int kJoin = 128;
 template <class T, int G>
 __global__ __launch_bounds__(256) void embed_join_kernel(EmbedArgs a) {
   typedef RowPiece<T> P;
   constexpr int kGroups = 256 / G;
-  __shared__ __attribute__((aligned(16))) float sums[kGroups][G * P::E];
+  __shared__ double sums[kGroups][P::E][G];
   const int lane = int(threadIdx.x) % G, group = int(threadIdx.x) / G;
   const uint32_t task = a.block0 + blockIdx.x, chunk = a.slices == 1 ? task : task / uint32_t(a.slices);
   const int d = (int(task - chunk * a.slices) * G + lane) * P::E, count = a.begin[a.range << a.bits];
@@ -347,26 +351,32 @@ __global__ __launch_bounds__(256) void embed_join_kernel(EmbedArgs a) {
   const int more = ((e - 1) >> a.chunk_bits) - int(chunk);  // chunks after this one
   // its own part is the chunk's second one, the others are their chunks' first ones
   const float* const part = a.part + (int64_t(chunk) * 2 + 1) * a.pdim + (d < a.dim ? d : 0);
-  float sum[P::E] = {};
+  double sum[P::E] = {};
+  for (int c = group; c <= more;) {
+    float run[P::E] = {};
+    const int end = min(more + 1, c + kJoin * kGroups);
 #pragma unroll 4
-  for (int c = group; c <= more; c += kGroups) {
+    for (; c < end; c += kGroups) {
 #pragma unroll
-    for (int i = 0; i < P::E; i += 4) {
-      const f32x4 v = *reinterpret_cast<const f32x4*>(part + (int64_t(c) * 2 - (c > 0)) * a.pdim + i);
+      for (int i = 0; i < P::E; i += 4) {
+        const f32x4 v = *reinterpret_cast<const f32x4*>(part + (int64_t(c) * 2 - (c > 0)) * a.pdim + i);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) sum[i + j] += v[j];
+        for (int j = 0; j < 4; ++j) run[i + j] += v[j];
+      }
     }
+#pragma unroll
+    for (int i = 0; i < P::E; ++i) sum[i] += double(run[i]);
   }
 #pragma unroll
-  for (int i = 0; i < P::E; ++i) sums[group][lane * P::E + i] = sum[i];
+  for (int i = 0; i < P::E; ++i) sums[group][i][lane] = sum[i];
   __syncthreads();
   if (group != 0 || d >= a.dim) return;
   P o;
 #pragma unroll
   for (int i = 0; i < P::E; ++i) {
-    float v = sum[i];
-    for (int g = 1; g < kGroups; ++g) v += sums[g][lane * P::E + i];
-    o.set(i, v * a.scale);
+    double v = sum[i];
+    for (int g = 1; g < kGroups; ++g) v += sums[g][i][lane];
+    o.set(i, float(v) * a.scale);
   }
   o.store(static_cast<T*>(a.out) + int64_t(t) * a.dim, d, a.dim);
 }

@@ -156,3 +156,19 @@ def test_the_most_tokens():
     runs = torch.full((vocab, 1), n // vocab, device="cuda")
     runs[:n % vocab] += 1
     assert torch.equal(dw, (runs.float() * 2.0 ** -8).half())
+
+
+@pytest.mark.parametrize("n,dim,frequent", [(1 << 18, 68, 1.0), (1 << 18, 68, 0.5), (1 << 20, 8, 1.0), (1 << 19, 321, 0.5)])
+def test_very_long_runs(n, dim, frequent):
+    """Equal gradients, whose roundings do not cancel, of a token that is all or half of very many.  At most 32 are added
+    one after the other, 31 U32 of their sum; of those sums at most 128, 127 U32; the rest in 64 bits; one more rounding, and
+    one of the scale's product."""
+    r = torch.Generator().manual_seed(dim)
+    grad = (1 + torch.rand(dim, generator=r)).cuda()
+    tokens = torch.full((n,), 3, dtype=torch.int32)
+    tokens[int(n * frequent):] = torch.arange(n - int(n * frequent), dtype=torch.int32) % 500 + 4
+    tokens = tokens[torch.randperm(n, generator=r)].cuda()
+    dw = rdv.embedding_backward(grad.expand(n, -1), tokens, 600, scale=1.7)
+    count = torch.bincount(tokens, minlength=600).double()[:, None]
+    want = count * grad.double() * float(torch.tensor(1.7))
+    assert ((dw.double() - want).abs() <= (31 + 127 + 1 + 1) * 2.0 ** -24 * want).all()
