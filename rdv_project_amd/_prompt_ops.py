@@ -13,6 +13,7 @@ from __future__ import annotations
 import ctypes as C
 import functools
 import math
+import threading
 from typing import NamedTuple, Optional
 
 import torch
@@ -283,6 +284,7 @@ def rms_norm_backward(grad, h, weight, stats, grad_sum=None, grads=None):
 
 
 _CAPTURED: list = []  # lists of work that graphs read
+_CAPTURED_LOCK = threading.Lock()
 
 
 class PackedSequences:
@@ -298,7 +300,8 @@ class PackedSequences:
     call of each kind (heads, dimensions, type, direction) on each GPU and copied
     there: keep it for all layers and steps on sequences of these lengths.  That
     first call waits for the copy, and cannot be captured into a graph.  Lists that a
-    graph has captured are kept until the process ends."""
+    graph has captured are kept, also when the PackedSequences is gone, until
+    release() or the end of the process: nothing tells when a graph is."""
 
     def __init__(self, lengths, states=None, starts=None) -> None:
         self.lengths = _counts(lengths, "lengths")
@@ -353,9 +356,18 @@ class PackedSequences:
         # The list's memory outlives what reads it: the launches of streams other than its own, and a graph's replays.
         if hit[5] != _stream(device):
             hit[3].record_stream(torch.cuda.current_stream())
-        if torch.cuda.is_current_stream_capturing() and not any(hit[3] is t for t in _CAPTURED):
-            _CAPTURED.append(hit[3])
+        if torch.cuda.is_current_stream_capturing():
+            with _CAPTURED_LOCK:
+                if not any(hit[3] is t for t in _CAPTURED):
+                    _CAPTURED.append(hit[3])
         return hit[:5]
+
+    def release(self) -> None:
+        """Lets go of the lists that graphs have captured: to be called when every replay of those graphs has run and
+        none follows.  Eager calls and new graphs can go on using the sequences."""
+        mine = [lists for _, lists, _ in list(self._plans.values())]
+        with _CAPTURED_LOCK:
+            _CAPTURED[:] = [t for t in _CAPTURED if not any(t is m for m in mine)]
 
     def _plan_call(self, layout, device: int):
         d = _causal_desc(*layout)

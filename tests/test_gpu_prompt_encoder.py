@@ -200,3 +200,34 @@ def test_plans_outlive_their_sequences():
             assert torch.equal(out, want)
     finally:
         rdv.set_synchronous(prev)
+
+
+def test_lists_of_captured_graphs_are_released():
+    """release() lets go of the lists that graphs have read, and the sequences go on being usable."""
+    q = torch.randn(300, 4, 32).cuda()
+    prev = rdv.set_synchronous(False)
+    try:
+        before = len(rdv._prompt_ops._CAPTURED)
+        for i in range(3):
+            seqs = rdv.PackedSequences((100, 200 - i))
+            other = rdv.PackedSequences((150, 150))
+            rdv.causal_attention(q, q, q, seqs)
+            rdv.causal_attention(q, q, q, other)
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                out, stats = rdv.causal_attention(q, q, q, seqs, return_lse=True)
+                apart = rdv.causal_attention(q, q, q, other)
+            graph.replay()
+            torch.cuda.synchronize()
+            assert len(rdv._prompt_ops._CAPTURED) == before + 2
+            assert torch.equal(out, rdv.causal_attention(q, q, q, seqs))
+            seqs.release()
+            assert len(rdv._prompt_ops._CAPTURED) == before + 1
+            seqs.release()
+            other.release()
+            assert len(rdv._prompt_ops._CAPTURED) == before
+            assert torch.equal(out, rdv.causal_attention(q, q, q, seqs))
+            assert torch.equal(apart, rdv.causal_attention(q, q, q, other))
+            del graph
+    finally:
+        rdv.set_synchronous(prev)
