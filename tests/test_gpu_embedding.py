@@ -172,3 +172,36 @@ def test_very_long_runs(n, dim, frequent):
     count = torch.bincount(tokens, minlength=600).double()[:, None]
     want = count * grad.double() * float(torch.tensor(1.7))
     assert ((dw.double() - want).abs() <= (31 + 127 + 1 + 1) * 2.0 ** -24 * want).all()
+
+
+def _check_many(tokens, vocab, dim, dtype, what):
+    """The gradient alone, as _check does it, with numpy's sums."""
+    grad = torch.randn(len(tokens), dim, generator=torch.Generator().manual_seed(dim + vocab)).to(TYPES[dtype]).cuda()
+    dw = rdv.embedding_backward(grad, torch.tensor(tokens, dtype=torch.int32).cuda(), vocab, scale=0.7)
+    known, g = (tokens >= 0) & (tokens < vocab), _np(grad)
+    ref, size = np.zeros((vocab, dim)), np.zeros((vocab, dim))
+    np.add.at(ref, tokens[known], g[known])
+    np.add.at(size, tokens[known], np.abs(g[known]))
+    count = np.bincount(tokens[known], minlength=vocab)[:, None]
+    _close(dw, ref * 0.7, (count + 3) * O.U32 * size * 0.7 + O._stored(ref * 0.7, dtype), what)
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("n,vocab,dim", [(16384, 1000, 16), (16385, 1000, 16), (40000, 1000, 16), (40000, 50000, 8),
+                                         (40000, 16, 24), (100000, 700, 8), (60000, 5, 72), (33000, 200000, 4)])
+@pytest.mark.parametrize("even", [False, True])
+def test_many_tokens(dtype, n, vocab, dim, even):
+    """Runs of 32, from 16,385 tokens on, in several blocks of the sort; waves with more tokens than they list (16 or 5 rows:
+    one block; 700: the most frequent ones' blocks)."""
+    _check_many(_tokens(n, vocab, even=even), vocab, dim, dtype, f"{n} of {vocab} x {dim} {dtype}")
+
+
+@pytest.mark.parametrize("more", [0, 20000])
+@pytest.mark.parametrize("length", [15, 16, 17, 31, 32, 33, 47, 48, 49, 63, 65])
+@pytest.mark.parametrize("first", [0, 1, 15, 16, 17, 31, 32, 33])
+def test_runs_at_the_chunks_ends(length, first, more):
+    """Runs that begin and end at or beside multiples of 16 and of 32, what is summed at once, of the sorted list: 16 of up
+    to 16,384 tokens, 32 of more."""
+    tokens = np.concatenate([np.zeros(first, np.int64), np.full(length, 1), np.full(33, 2), np.full(16, 3), np.full(more, 5)])
+    np.random.default_rng(length + first).shuffle(tokens)
+    _check_many(tokens, 6, 12, "f32", f"{first} then {length}, {more} more")
