@@ -244,3 +244,10 @@ def test_dweight_of_very_many_rows(dtype, rows, width):
     _, dw = rdv.rms_norm_backward(grad.expand(rows, -1), x.expand(rows, -1), None, stats)
     want = rows * grad.double() * x.double() * stats[0].double()
     assert ((dw.double() - want).abs() <= (127 + 21 + 31 + 1 + 2) * 2.0 ** -24 * want).all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,width", [(600, 9000), (600, 40000), (2000, 4096), (600, 16385)])
+def test_many_wide_rows(dtype, rows, width):
+    """More rows than blocks of those that share a row among 256 or 1,024 threads, in registers and past them."""
+    _check(rows, width, dtype, what=f"{rows} x {width} {dtype}")
