@@ -336,3 +336,26 @@ def test_lengths_may_be_any_iterable():
                 rdv.PackedSequences(make(values))
             with pytest.raises(ValueError, match="states"):
                 rdv.PackedSequences((1,) * len(values), make(values))
+
+
+@pytest.mark.parametrize("lengths,kv_heads,pairs", [((64,), 1, True), ((700, 0, 1, 33), 2, True), ((20000,), 8, False),
+                                                    ((2000,) * 20, 4, False)])
+@pytest.mark.parametrize("backward", [0, 1])
+def test_tiles_are_as_the_plan_says(lengths, kv_heads, pairs, backward):
+    """A block's rows and states: 64 where pairs of waves share them, because blocks of 128 would leave CUs idle."""
+    rows, t = [], 0
+    for a in lengths:
+        rows.append((t, a, t, a))
+        t += a
+    plan = _plan(_desc(tokens=t, states=t, heads=2 * kv_heads, kv_heads=kv_heads), rows, backward)
+    words = plan[:256].view(np.int32)[(16 + C.sizeof(_lib.CausalAttentionDesc)) // 4:]
+    (row_pairs, key_pairs, tile_rows, key_tile), (few, tiles, keys, _, _) = words[9:13].tolist(), _items(plan)
+    assert (bool(row_pairs), tile_rows) == (pairs, 64 if pairs else 128)
+    assert {i[4] % tile_rows for i in tiles} == {0}
+    for token, a, _, _ in rows:
+        firsts = {i[4] for i in few + tiles if i[:2] == [token, a]}
+        assert firsts == set(range(0, 2 * a, tile_rows))
+        if backward:
+            assert {i[4] for i in keys if i[:2] == [token, a]} == set(range(0, a, key_tile))
+    if backward:
+        assert (bool(key_pairs), key_tile) == (pairs, 64 if pairs else 128)
