@@ -921,8 +921,9 @@ static int check_embedding(const rdv_embedding_desc* d, bool backward) {
   if (d->vocab < 1 || d->dim < 1) return fail(RDV_ERR_INVALID, "embedding: vocab and dim must be >= 1");
   if (d->tokens > (int64_t(1) << 30) || d->vocab > (1 << 25) || d->dim > (1 << 20))
     return fail(RDV_ERR_UNSUPPORTED, "embedding: at most 2^30 tokens, 2^25 rows and 2^20 dimensions");
-  // blocks are counted in 32 bits
-  if (backward && (int64_t(d->vocab) + d->tokens / 64 + 1) * (d->dim + 255) > (int64_t(1) << 33))
+  // slices of at least 256 elements of what the launches share out are counted in 32 bits: four rows of the vocabulary (which
+  // its blocks round up to twice as many at most), or a chunk of at least 16 tokens
+  if (backward && (int64_t(d->vocab) / 2 + d->tokens / 16 + 256) * ((d->dim + 255) / 256) >= (int64_t(1) << 32))
     return fail(RDV_ERR_UNSUPPORTED, "embedding: too large a gradient");
   if (d->dtype < RDV_DTYPE_F32 || d->dtype > RDV_DTYPE_BF16) return fail(RDV_ERR_INVALID, "embedding: unknown dtype");
   if (!(d->scale > -3.0e38f && d->scale < 3.0e38f)) return fail(RDV_ERR_INVALID, "embedding: scale must be finite");

@@ -205,3 +205,19 @@ def test_runs_at_the_chunks_ends(length, first, more):
     tokens = np.concatenate([np.zeros(first, np.int64), np.full(length, 1), np.full(33, 2), np.full(16, 3), np.full(more, 5)])
     np.random.default_rng(length + first).shuffle(tokens)
     _check_many(tokens, 6, 12, "f32", f"{first} then {length}, {more} more")
+
+
+@pytest.mark.parametrize("vocab,dim", [(1 << 25, 64), ((1 << 20) + 3, 9000)])
+def test_the_largest_gradients(vocab, dim):
+    """The most rows, and rows whose elements are more than 2^33, as a small table's."""
+    g = torch.Generator().manual_seed(dim)
+    at = torch.cat([torch.tensor([0, vocab - 1]), torch.randint(0, vocab, (500,), generator=g)]).unique()
+    pick = torch.randint(0, len(at), (3000,), generator=g)
+    grad = torch.randn(3000, dim, generator=g).to(torch.bfloat16).cuda()
+    small = rdv.embedding_backward(grad, pick.to(torch.int32).cuda(), len(at), scale=0.5)
+    dw = rdv.embedding_backward(grad, at[pick].to(torch.int32).cuda(), vocab, scale=0.5)
+    at = at.cuda()
+    used = torch.bincount(pick, minlength=len(at)).cuda() > 0
+    assert used.sum() > 400 and torch.allclose(dw[at].float(), small.float(), rtol=2.0 ** -7, atol=1e-6)
+    dw[at] = 0
+    assert not any(part.any() for part in dw.split(1 << 18))

@@ -359,3 +359,16 @@ def test_tiles_are_as_the_plan_says(lengths, kv_heads, pairs, backward):
             assert {i[4] for i in keys if i[:2] == [token, a]} == set(range(0, a, key_tile))
     if backward:
         assert (bool(key_pairs), key_tile) == (pairs, 64 if pairs else 128)
+
+
+@pytest.mark.parametrize("tokens,vocab,dim,fits", [
+    (1000, 1 << 25, 1, True), (1000, 1 << 25, 4096, True), (1 << 20, 1 << 25, 64, True), (1 << 30, 1000, 1024, True),
+    (0, 1 << 20, 1 << 20, True), (1 << 20, 256000, 16384, True), (1, 1 << 25, 1 << 20, False), (1 << 30, 5, 1 << 20, False),
+])
+def test_embedding_gradients_that_fit(tokens, vocab, dim, fits):
+    """Every vocabulary that the forward call takes has a gradient, up to what launches can count."""
+    lib = _lib.load()
+    for dtype in (_lib.DTYPE_F32, _lib.DTYPE_BF16):
+        d = _lib.EmbeddingDesc(tokens=tokens, vocab=vocab, dim=dim, dtype=dtype, scale=1.0, g_row_stride=dim)
+        got = lib.rdv_embedding_workspace_bytes(C.byref(d))
+        assert got >= vocab * 4 if fits else got == _lib.RDV_ERR_UNSUPPORTED and "too large" in _lib.last_error()
