@@ -660,8 +660,10 @@ int rdv_embedding(const rdv_embedding_desc* desc, const void* tokens, const void
 int64_t rdv_embedding_workspace_bytes(const rdv_embedding_desc* desc);
 
 /* dweight[vocab, dim] (contiguous): row v is scale times the sum of grad's rows
- * i with tokens[i] = v, in fp32 and in an order that tokens alone gives, rounded
- * once; zeros for tokens that do not occur. */
+ * i with tokens[i] = v, in fp32 (partial sums of very frequent tokens in fp64)
+ * and in an order that tokens alone gives, rounded once; zeros for tokens that
+ * do not occur.  (vocab / 2 + tokens / 16 + 256) ceil(dim / 256) < 2^32; the sort
+ * reads all tokens once for every 512 rows of vocab, or CU. */
 int rdv_embedding_backward(const rdv_embedding_desc* desc, const void* grad, const void* tokens, void* dweight,
                            void* workspace, int64_t workspace_bytes, void* stream);
 
@@ -683,7 +685,8 @@ typedef struct rdv_rms_norm_desc {
  * where there is no residual (contiguous ones).  stats[rows] = 1 / sqrt(mean(h^2)
  * + eps), where not NULL.  scales not NULL: y is e4m3 bytes and the row's values
  * are scales[row] times them; scales[row] = max |y| / 448, at least fp32's
- * smallest normal number (0 for a row of zeros). */
+ * smallest normal number (0 for a row of zeros), NaN where a y is.  Squares are
+ * fp32: rows of elements past 1.8e19 become 0. */
 int rdv_rms_norm(const rdv_rms_norm_desc* desc, const void* x, const void* residual, const float* weight, void* sum,
                  void* y, float* scales, float* stats, void* stream);
 
@@ -692,7 +695,8 @@ int64_t rdv_rms_norm_workspace_bytes(const rdv_rms_norm_desc* desc);
 
 /* The gradients of rdv_rms_norm for grad = dL/dy and grad_sum = dL/dh (NULL:
  * zeros), given h and the stats that it wrote: dx[rows, width] (contiguous), the
- * gradient of x and of residual alike, and fp32 dweight[width]. */
+ * gradient of x and of residual alike, and fp32 dweight[width] (no thread adds
+ * more than 128 rows, or the square root of its rows, one after the other). */
 int rdv_rms_norm_backward(const rdv_rms_norm_desc* desc, const void* grad, const void* grad_sum, const void* h,
                           const float* weight, const float* stats, void* dx, float* dweight, void* workspace,
                           int64_t workspace_bytes, void* stream);

@@ -108,9 +108,10 @@ def embedding(tokens, weight, scale: float = 1.0, out=None):
 def embedding_backward(grad, tokens, vocab: int, scale: float = 1.0, out=None):
     """The gradient of weight of embedding(tokens, weight, scale) for grad =
     dL/dy [*tokens.shape, dim]: [vocab, dim] in grad's type, row v scale times the
-    sum of the rows of grad whose token is v, in float32 and rounded once; zeros
-    for tokens that do not occur.  The order of a sum follows from the tokens
-    alone, so the same call gives the same bits."""
+    sum of the rows of grad whose token is v, in float32 (partial sums of very
+    frequent tokens in float64) and rounded once; zeros for tokens that do not
+    occur.  The order of a sum follows from the tokens alone, so the same call
+    gives the same bits."""
     grad, tokens = _data(grad, "grad"), _tokens(tokens)
     assert grad.dim() == tokens.dim() + 1 and grad.shape[:-1] == tokens.shape and grad.shape[-1] >= 1, \
         f"grad must be [{', '.join(map(str, tokens.shape))}, dim], got {list(grad.shape)}"
@@ -196,8 +197,8 @@ def rms_norm(x, weight, residual=None, eps: float = 1e-6, out=None, sum_out=None
     `sum_out` is h's buffer, which may be x or residual itself; `out` is y's, which
     may be x itself where there is no residual.  eight_bits: in y's place stands
     (values, scales), float8_e4m3fn [..., width] and float32 [...], for products in
-    8 bits: y is scales times values, scales = max |y| / 448 of the row (`out`: the
-    two buffers)."""
+    8 bits: y is scales times values, scales = max |y| / 448 of the row, NaN where a
+    y is (`out`: the two buffers)."""
     x, weight = _rms_inputs(x, weight)
     eps = float(eps)
     if not 0.0 <= eps < math.inf:

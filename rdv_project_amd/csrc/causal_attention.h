@@ -217,7 +217,8 @@ __device__ __forceinline__ void causal_finish(const CausalArgs& a, const CausalA
 }
 
 // Many rows: a block of 4 waves, 32 rows each (or 64 rows shared by pairs of waves), as attn_tile_kernel.  Bound: a SIMD's
-// vector and matrix instructions add up (of 64 dimensions in fp16 56 and 30% of the cycles, of 128 in bf16 50 and 54%).
+// vector and matrix instructions, which overlap in part (of 64 dimensions in fp16 56 and 30% of the cycles, of 128 in bf16 50
+// and 55%).
 //   16,384 tokens, 16 heads on 4 of 128, bf16: 1.00 to 1.07 ms, 1.03 to 1.10 PFLOP/s (an 8,192^3 product: 1.13 to 1.18)
 //   8 sequences up to 4,096 tokens, 8 heads on 4 of 64, fp16: 80 us, 0.67 PFLOP/s (such a product: 1.06 to 1.13)
 template <class T, int NC, int WK>

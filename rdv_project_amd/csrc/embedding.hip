@@ -4,20 +4,21 @@
 // The gradient groups the tokens by a sort whose order follows from the tokens alone, so that its sums have one order and no
 // floating-point atomics:
 //   * embed_sort_kernel: block b takes the tokens that are b modulo the number of blocks (frequent tokens, which tend to
-//     have neighbouring numbers, so spread over the blocks) and goes over all tokens twice: it counts its own, and those of
-//     the blocks before it (which tells where its part of the sorted list begins, without a word from them), then puts its
-//     own in place.  The tokens stay in the L2.
+//     have neighbouring numbers, so spread over the blocks) and goes over all tokens: it counts and lists its own, and counts
+//     those of the blocks before it (which tells where its part of the sorted list begins, without a word from them), then
+//     puts its own in place.  The tokens stay in the L2.  So the cost is tokens times blocks: one per CU up to 131,000 rows of
+//     the vocabulary, one per 512 rows beyond.
 //   * embed_rows_kernel: a row of the vocabulary with up to a.run tokens is summed by the lanes that share it and written,
 //     one without tokens is written as zeros.  Longer runs are cut at multiples of that of the sorted list: a run's piece
 //     of such a chunk is summed into the workspace.
-//   * embed_join_kernel: adds up the pieces of the long runs.
+//   * embed_join_kernel: adds up the pieces of the long runs, a run's in one block per slice of its row.
 // Bound: HBM, the rows of grad that are read and the whole vocabulary's that are written.  64 x 1,024 tokens, five in eight of
 // them known and the most frequent one 6% of those, of 50,000 x 1,024 in bf16 (a 2 GiB copy: 4.8 to 5.1 TB/s):
 //   embed_kernel       39 us for 183 MB, 4.7 TB/s
 //   embed_sort_kernel  17 us, of which the first walk takes 12, by its instructions per token (13 us where all tokens are
-//                      equally frequent, then 4,096 6.0 and 262,144 33).  Loads further ahead and another first token
-//                      for each block made no difference.  With ranges of neighbouring tokens per block, as frequent ones
-//                      are, it took 190 us
+//                      equally frequent, then 4,096 6.0 and 262,144 32; of a vocabulary of 256,000 19 and 44, of 2^20 50
+//                      and 130, of 2^25 1,200 and 3,400).  Loads further ahead and another first token for each block made
+//                      no difference.  With ranges of neighbouring tokens per block, as frequent ones are, it took 190 us
 //   embed_rows_kernel  51 us for 194 MB, 3.8 TB/s: three loads that wait for one another, four rows of a wave at once (one
 //                      row at a time 69 us)
 //   embed_join_kernel  5 us
@@ -397,7 +398,8 @@ struct Plan {
 int64_t align256(int64_t bytes) { return (bytes + 255) / 256 * 256; }
 Plan make_plan(const rdv_embedding_desc& d) {
   Plan p{};
-  // a block per CU and up to kSortRows tokens each, fewer blocks where they would have less than 16
+  // a block per CU, fewer where they would have less than 16 rows of the vocabulary, more where a block would have more than
+  // kSortRows of them (past 131,000 rows: all of those go over all tokens)
   p.bits = 0;
   while ((int64_t(d.vocab) >> p.bits) > kSortRows || (p.bits < 8 && (d.vocab >> p.bits) > 16)) ++p.bits;
   p.range = int(((int64_t(d.vocab) - 1) >> p.bits) + 1);
